@@ -226,6 +226,152 @@ def sample(logits: torch.Tensor, temperature=None, top_k=None, top_p=None, seeds
     return out
 
 
+# ---- the 8-bit KV cache: the four steps above over a cache of half the bytes
+# One layer is uint8 [pages][kv heads][128 d + 32]: per page and head the key codes, the value codes and eight fp32 scales, one for each block of 16 tokens of
+# keys and of values (csrc/kv8.cuh has the order of the codes; kv8_codes / kv8_records below).  A code c stands for (c - 128) * scale.
+KV8_BLOCK = 16
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise N.NativeError(what)
+
+
+def _kv8_layer(layer: torch.Tensor, d: int, what: str):
+    """(pages, kv heads) of a layer; all tensors of a call have to be on its device."""
+    _need(layer.is_cuda and layer.dtype == torch.uint8 and layer.dim() == 3 and layer.is_contiguous(), what + ": the cache is contiguous CUDA uint8 [pages, nkv, record]")
+    _need(layer.shape[2] == 128 * d + 32, what + ": the cache's records are not those of this head_dim")
+    return layer.shape[0], layer.shape[1]
+
+
+def _kv8_ints(t, dev, what: str) -> torch.Tensor:
+    """int32 on the device; a list goes up in a copy that the host waits for."""
+    if not isinstance(t, torch.Tensor):
+        t = torch.tensor(t, dtype=torch.int32, device=dev).reshape(-1)
+    _need(t.dtype == torch.int32 and t.device == dev and t.is_contiguous(), what + ": contiguous int32 on the cache's device")
+    return t
+
+
+def _kv8_table(t: torch.Tensor, dev, what: str) -> torch.Tensor:
+    _need(t.dtype == torch.int32 and t.device == dev and t.dim() == 2 and t.is_contiguous(), what + ": page_table is contiguous int32 [sequences, pages] on the cache's device")
+    return t
+
+
+def _kv8_call(dev, name: str, *args) -> None:
+    """A library call on the device's current stream, whichever device is the current one."""
+    fn = getattr(N.load(), name)
+    if dev.index == torch.cuda.current_device():
+        N.check(fn(*args, N.cur_stream()), name)
+    else:
+        with torch.cuda.device(dev):
+            N.check(fn(*args, N.cur_stream()), name)
+
+
+def kv8_cache_alloc(num_pages: int, nkv: int, d: int, device) -> torch.Tensor:
+    """One layer of 8-bit KV cache, all zeros."""
+    _need(d in (64, 128), "kv8_cache_alloc: head_dim 64 or 128")
+    return torch.zeros(num_pages, nkv, 128 * d + 32, device=device, dtype=torch.uint8)
+
+
+def rope_kv8_append(qkv_partials: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor, seq_rows: torch.Tensor,
+                    page_table: torch.Tensor, kv8_layer: torch.Tensor, nq: int, nkv: int, d: int) -> torch.Tensor:
+    """rope_kv_append into the 8-bit cache -> q fp16 [T, nq, d].  Tokens of one sequence stand side by side in `positions` / `seq_rows`, without gaps.  A block
+    whose scale is too small for a new token is rescaled, the tokens before it in the block with it; a block that is entered at its first token starts anew.
+    Tokens without a place (a position outside the tables, a page outside the cache) are not written."""
+    what = "rope_kv8_append"
+    dev = kv8_layer.device
+    pages, heads = _kv8_layer(kv8_layer, d, what)
+    _need(heads == nkv, what + ": the cache has another number of heads")
+    _need(qkv_partials.dim() == 3 and qkv_partials.dtype == torch.float32 and qkv_partials.device == dev, what + ": qkv_partials is fp32 [S, T, (nq + 2 nkv) d] on the cache's device")
+    S, T, width = qkv_partials.shape
+    _need(width == (nq + 2 * nkv) * d and qkv_partials.stride(2) == 1 and (T < 2 or qkv_partials.stride(1) == width), what + ": qkv_partials has rows of (nq + 2 nkv) d")
+    _need(cos.dtype == torch.float32 and sin.dtype == torch.float32 and cos.device == dev and sin.device == dev and cos.is_contiguous() and sin.is_contiguous()
+          and cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] * 2 == d, what + ": cos and sin are contiguous fp32 [positions, d / 2] on the cache's device")
+    positions, seq_rows = _kv8_ints(positions, dev, what), _kv8_ints(seq_rows, dev, what)
+    _need(positions.numel() == T and seq_rows.numel() == T, what + ": a position and a sequence for every token")
+    page_table = _kv8_table(page_table, dev, what)
+    q = torch.empty(T, nq, d, device=dev, dtype=torch.float16)
+    _kv8_call(dev, "ft_rope_kv8_append", qkv_partials.data_ptr(), S, qkv_partials.stride(0), cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(),
+              seq_rows.data_ptr(), page_table.data_ptr(), page_table.shape[0], page_table.shape[1], q.data_ptr(), kv8_layer.data_ptr(), pages, T, nq, nkv, d)
+    return q
+
+
+def kv8_read(kv8_layer: torch.Tensor, page_table: torch.Tensor, req_start, req_slot, req_pos0, rows: int, d: int):
+    """Keys and values back as fp16 [rows, nkv, d] each: request r gets rows req_start[r] .. req_start[r + 1] - 1, from position req_pos0[r] of page-table row
+    req_slot[r] on.  Rows that no request owns, and rows without a page, are zeros.  The lists are int32 tensors on the device, or anything a tensor is made of."""
+    what = "kv8_read"
+    dev = kv8_layer.device
+    pages, nkv = _kv8_layer(kv8_layer, d, what)
+    page_table = _kv8_table(page_table, dev, what)
+    req_start, req_slot, req_pos0 = _kv8_ints(req_start, dev, what), _kv8_ints(req_slot, dev, what), _kv8_ints(req_pos0, dev, what)
+    n = req_slot.numel()
+    _need(req_start.numel() == n + 1 and req_pos0.numel() == n, what + ": a start and a position for every request, and the end")
+    _need(rows >= 0, what + ": a number of rows")
+    k = torch.empty(rows, nkv, d, device=dev, dtype=torch.float16)
+    v = torch.empty(rows, nkv, d, device=dev, dtype=torch.float16)
+    _kv8_call(dev, "ft_kv8_read", kv8_layer.data_ptr(), pages, page_table.data_ptr(), page_table.shape[0], page_table.shape[1], req_start.data_ptr(),
+              req_slot.data_ptr(), req_pos0.data_ptr(), n, rows, k.data_ptr(), v.data_ptr(), nkv, d)
+    return k, v
+
+
+def _kv8_query(q: torch.Tensor, kv8_layer: torch.Tensor, page_table: torch.Tensor, planes: int, what: str):
+    dev = kv8_layer.device
+    _need(q.dim() == 3 and q.dtype == torch.float16 and q.device == dev and q.is_contiguous(), what + ": q is contiguous fp16 [rows, nq, d] on the cache's device")
+    pages, nkv = _kv8_layer(kv8_layer, q.shape[2], what)
+    _need(planes in (1, 2), what + ": one plane or two")
+    out = torch.empty(q.shape[0], q.shape[1] * q.shape[2], device=dev, dtype=torch.bfloat16)
+    return dev, pages, nkv, _kv8_table(page_table, dev, what), out, torch.empty_like(out) if planes == 2 else None
+
+
+def attn_decode_kv8(q: torch.Tensor, kv8_layer: torch.Tensor, page_table: torch.Tensor, ctx_lens: torch.Tensor, planes: int = 2):
+    """attn_decode over the 8-bit cache: q fp16 [B, nq, d], up to eight query heads a key head -> bf16 (hi, lo) planes [B, nq * d], lo None with planes = 1.  A
+    sequence without keys gives zeros; keys on pages outside the cache are hidden."""
+    what = "attn_decode_kv8"
+    dev, pages, nkv, page_table, out, lo = _kv8_query(q, kv8_layer, page_table, planes, what)
+    ctx_lens = _kv8_ints(ctx_lens, dev, what)
+    B, nq, d = q.shape
+    _need(ctx_lens.numel() == B and page_table.shape[0] >= B, what + ": a context length and a page-table row for every query")
+    _kv8_call(dev, "ft_attn_decode_kv8", q.data_ptr(), kv8_layer.data_ptr(), pages, page_table.data_ptr(), page_table.shape[1], ctx_lens.data_ptr(), out.data_ptr(),
+              N.ptr(lo), B, nq, nkv, d)
+    return out, lo
+
+
+def attn_prefill_kv8(q: torch.Tensor, kv8_layer: torch.Tensor, page_table: torch.Tensor, req_q_start, req_slot, req_pos0, planes: int = 2):
+    """attn_prefill over the 8-bit cache, up to eight query heads a key head.  The lists are int32 tensors on the device (then nothing goes up, and the call can be
+    captured) or anything a tensor is made of.  Rows that no request owns are zeros; keys on pages outside the cache are hidden.  -> (hi, lo), lo None with planes = 1."""
+    what = "attn_prefill_kv8"
+    dev, pages, nkv, page_table, out, lo = _kv8_query(q, kv8_layer, page_table, planes, what)
+    req_q_start, req_slot, req_pos0 = _kv8_ints(req_q_start, dev, what), _kv8_ints(req_slot, dev, what), _kv8_ints(req_pos0, dev, what)
+    n = req_slot.numel()
+    _need(req_q_start.numel() == n + 1 and req_pos0.numel() == n, what + ": a start and a position for every request, and the end")
+    T, nq, d = q.shape
+    _kv8_call(dev, "ft_attn_prefill_kv8", q.data_ptr(), kv8_layer.data_ptr(), pages, page_table.data_ptr(), page_table.shape[0], page_table.shape[1],
+              req_q_start.data_ptr(), req_slot.data_ptr(), req_pos0.data_ptr(), n, T, out.data_ptr(), N.ptr(lo), nq, nkv, d)
+    return out, lo
+
+
+def _kv8_offsets(d: int, device) -> torch.Tensor:
+    """Where the code of (keys 0 | values 1, token, dim) lies in a record."""
+    t, i = torch.arange(KV_TILE, device=device)[:, None], torch.arange(d, device=device)[None, :]
+    piece = (i >> 6) * (KV_TILE * 64)
+    return torch.stack([piece + t * 64 + (i & 63), KV_TILE * d + piece + (t ^ (t >> 1 & 1)) * 64 + ((i & 63) ^ (t & 4) * 8)])
+
+
+def kv8_codes(records: torch.Tensor, d: int):
+    """records [..., 128 d + 32] as stored -> codes uint8 [..., 2, 64, d], scales fp32 [..., 2, 4]."""
+    at = _kv8_offsets(d, records.device)
+    scales = records[..., 2 * KV_TILE * d:].contiguous().view(torch.float32)
+    return records[..., at.reshape(-1)].reshape(records.shape[:-1] + at.shape), scales.reshape(records.shape[:-1] + (2, KV_TILE // KV8_BLOCK))
+
+
+def kv8_records(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """inverse of kv8_codes."""
+    d, lead = codes.shape[-1], codes.shape[:-3]
+    body = torch.empty(lead + (2 * KV_TILE * d,), device=codes.device, dtype=torch.uint8)
+    body[..., _kv8_offsets(d, codes.device).reshape(-1)] = codes.reshape(body.shape)
+    return torch.cat([body, scales.to(torch.float32).contiguous().reshape(lead + (-1,)).view(torch.uint8)], -1)
+
+
 # ---- KV cache (un)swizzle helpers for tests: logical [tokens, d] <-> stored slab
 # A stored slab is d / 64 sub-slabs of [64 tokens][64 dims]; inside a sub-slab the eight 16-byte chunks of a row are
 # XOR-swizzled with the row index (csrc/common.cuh: kv_swizzled_chunk).  The XOR is an involution.

@@ -124,6 +124,11 @@ SIGNATURES = {
     "ft_attn_prefill_order_tiles": (_I, [_VP, _VP, _VP, _VP, _I, _I, _I, _I, _I]),
     "ft_attn_prefill_ordered": (_I, [_VP, _VP, _VP, _I, _VP, _VP, _VP, _VP, _VP, _I, _VP, _VP, _I, _I, _I, _I, _I, _VP]),
     "ft_attn_prefill": (_I, [_VP, _VP, _VP, _I, _VP, _VP, _VP, _VP, _VP, _I, _VP, _VP, _I, _I, _I, _I, _VP]),
+    "ft_kv8_record_bytes": (_LL, [_I]),
+    "ft_rope_kv8_append": (_I, [_VP, _I, _LL, _VP, _VP, _I, _VP, _VP, _VP, _I, _I, _VP, _VP, _I, _I, _I, _I, _I, _VP]),
+    "ft_kv8_read": (_I, [_VP, _I, _VP, _I, _I, _VP, _VP, _VP, _I, _I, _VP, _VP, _I, _I, _VP]),
+    "ft_attn_decode_kv8": (_I, [_VP, _VP, _I, _VP, _I, _VP, _VP, _VP, _I, _I, _I, _I, _VP]),
+    "ft_attn_prefill_kv8": (_I, [_VP, _VP, _I, _VP, _I, _I, _VP, _VP, _VP, _I, _I, _VP, _VP, _I, _I, _I, _VP]),
     "ft_sample": (_I, [_VP, _I, _I, _VP, _VP, _VP, _VP, _VP, _VP]),
 }
 

@@ -662,6 +662,35 @@ int ft_attn_prefill(const void* q, const void* kv_layer, const int* page_table, 
                     const int* tile_q0, int n_tiles, void* out, void* out_lo, int nq, int nkv, int d,
                     int q_rows, void* stream);
 
+/* The KV cache in 8 bits: K4, K5 and K6 over a cache of half the bytes, and reading it back.  One layer is [page][kv_head][record], a page = 64 tokens, a record
+ * (ft_kv8_record_bytes: 128 d + 32) = key codes [d/64][64][64] | value codes [d/64][64][64] | 8 fp32 scales, keys' then values', one for each block of 16 tokens.
+ * A code c (one byte) stands for (c - 128) * scale of its block.  Key of token t, dim i: piece i / 64, row t, byte i % 64; value: row t ^ (t >> 1 & 1), byte
+ * (i % 64) ^ 8 (t & 4).  A cache of zero bytes is a cache of zeros.  head_dim 64 or 128; q, qkv, out and the cache on 16 bytes.
+ * Page numbers outside [0, num_pages), page-table rows outside [0, table_rows) and positions beyond max_pages * 64 name no token: nothing is written there, zeros
+ * are read, and attention does not see such keys.  A query that sees no key at all gives zeros.  The calls read and write what they are given only; all but
+ * append may run at the same time on any streams, append beside nothing that touches the same pages.
+ *
+ * ft_rope_kv8_append: ft_rope_kv_append into this cache (n_angles = rows of cos_t / sin_t; a token beyond them is not written, its q is 0).  Per block and head, with a = max |x| over the block's new
+ * tokens (NaN counts as 0, what lies beyond fp16's range as its end) and s_old the block's scale where it holds tokens below the first new one, else 0:
+ * s = max(s_old, a / 127); tokens below the first new one c <- rint(c s_old / s); new ones c = rint(x / s).  Tokens of a sequence stand side by side in the lists
+ * and without gaps; a block that two separate stretches of the list share is written by both at once. */
+long long ft_kv8_record_bytes(int d);
+int ft_rope_kv8_append(const float* qkv, int n_splits, long long split_stride, const float* cos_t, const float* sin_t, int n_angles,
+                       const int* positions, const int* seq_rows, const int* page_table, int table_rows, int max_pages, void* q_out,
+                       void* kv8_layer, int num_pages, int T, int nq, int nkv, int d, void* stream);
+/* rows of keys and values as fp16 [rows][nkv][d] (cut to fp16's range): request r owns rows req_start[r] .. req_start[r + 1] - 1 (req_start grows) and starts at position
+ * req_pos0[r] of page-table row req_slot[r].  All `rows` rows are written; those that no request owns with zeros. */
+int ft_kv8_read(const void* kv8_layer, int num_pages, const int* page_table, int table_rows, int max_pages, const int* req_start,
+                const int* req_slot, const int* req_pos0, int n_req, int rows, void* k_out, void* v_out, int nkv, int d, void* stream);
+/* One query token per sequence: q FP16 [B][nq][d], nq / nkv up to 8, out bf16 [B][nq*d] (+ residual plane out_lo, may be NULL). */
+int ft_attn_decode_kv8(const void* q, const void* kv8_layer, int num_pages, const int* page_table, int max_pages, const int* ctx_lens, void* out,
+                       void* out_lo, int B, int nq, int nkv, int d, void* stream);
+/* Causal attention of prompt portions: q FP16 [T][nq][d], nq / nkv up to 8, request r owns rows req_q_start[r] .. req_q_start[r + 1] - 1 (req_q_start grows), page-table row req_slot[r],
+ * and its first query sits at position req_pos0[r].  The lists are DEVICE arrays.  All T rows of out (and out_lo, may be NULL) are written; those that no request owns with zeros. */
+int ft_attn_prefill_kv8(const void* q, const void* kv8_layer, int num_pages, const int* page_table, int table_rows, int max_pages,
+                        const int* req_q_start, const int* req_slot, const int* req_pos0, int n_req, int T, void* out, void* out_lo, int nq, int nkv,
+                        int d, void* stream);
+
 /* K7: per-row temperature / top-k / top-p sampling (argmax when temperature <= 0; a null temperature says so for all rows).
  * A row without any logit above minus infinity gives index 0. */
 int ft_sample(const float* logits, int B, int V, const float* temperature, const int* top_k,
