@@ -101,22 +101,24 @@ struct Kv8Query {
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
         const float m_new = fmaxf(m, most);                          // finite: a page has a token
         const float v_new = fmaxf(vref, fmaxf(fmaxf(vs.x, vs.y), fmaxf(vs.z, vs.w)));
-        const float v_inv = v_new > 0.f ? 1.f / v_new : 0.f;
-        const float alpha = exp2f(m - m_new);
-        const float keep = alpha * (vref * v_inv);
-        l *= alpha;
-        m = m_new;
-        vref = v_new;
-        const float k0 = __shfl_sync(0xffffffffu, keep, 8 * tq), k1 = __shfl_sync(0xffffffffu, keep, 8 * tq + 4);
+        const float v_inv = v_new > 0.f ? __fdividef(1.f, v_new) : 0.f;
+        if (__any_sync(0xffffffffu, m_new > m || v_new > vref)) {    // after the first few pages rarely
+            const float alpha = ex2_fast(m - m_new);
+            const float keep = alpha * (vref * v_inv);
+            l *= alpha;
+            m = m_new;
+            vref = v_new;
+            const float k0 = __shfl_sync(0xffffffffu, keep, 8 * tq), k1 = __shfl_sync(0xffffffffu, keep, 8 * tq + 4);
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) o[i][0] *= k0, o[i][1] *= k1, o[i][2] *= k0, o[i][3] *= k1;
+            for (int i = 0; i < D / 16; ++i) o[i][0] *= k0, o[i][1] *= k1, o[i][2] *= k0, o[i][3] *= k1;
+        }
         const float vscale[4] = {vs.x * v_inv, vs.y * v_inv, vs.z * v_inv, vs.w * v_inv};
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {                             // a block of 16 tokens
             uint32_t b[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float p0 = exp2f(p[2 * kk + h][0] - m), p1 = exp2f(p[2 * kk + h][1] - m);
+                const float p0 = ex2_fast(p[2 * kk + h][0] - m), p1 = ex2_fast(p[2 * kk + h][1] - m);
                 l += p0 + p1;
                 const __half2 t = __floats2half2_rn(p0 * vscale[kk], p1 * vscale[kk]);
                 b[h] = *reinterpret_cast<const uint32_t*>(&t);

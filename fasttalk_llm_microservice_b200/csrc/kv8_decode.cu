@@ -1,70 +1,368 @@
 // Attention of one query token per sequence over the 8-bit KV cache (kv8.cuh): out[b][h] = sum_j softmax_j(q . k_j / sqrt(D)) v_j, j < ctx_lens[b].
 //
-// One CTA per (sequence, key head); its warps take the pages in turn and their results are put together at the end.
+// What bounds it is the cache's bytes, so the list of all (sequence, key head, page) is cut into equal shares, one for each of two CTAs per SM, however ragged
+// the batch is.  In a CTA one warp copies records (a page of a head: codes and scales in one piece) into a ring of shared memory, and the others take whole
+// records in turn (Kv8Query in kv8.cuh).  A (sequence, head) that several CTAs have parts of is put together by the last of them to arrive, in the order of the
+// parts.  Where there is a CTA for every (sequence, head) and none of them is long, each CTA takes a whole one instead: no parts, nothing to put together.
+//
+// Nothing is planned ahead of the kernel: every CTA adds up the sequences' pages itself (one read of ctx_lens).  What the arrival counters need, zeros, is
+// written by a kernel of its own whose end this one waits for only when it has its first part ready.
 #include "common.cuh"
 #include "ft_internal.h"
 #include "kv8.cuh"
 
 namespace ft {
 
-constexpr int K8D_WARPS = 8, K8D_GROUP = 8;      // warps a CTA; query heads a key head at most
+constexpr int K8D_GROUP = 8;                     // query heads a key head at most
+constexpr int K8D_WHOLE_PAGES = 16;              // with page tables no wider than this, and a CTA for each (sequence, head), there are never parts
 constexpr float K8D_LOG2E = 1.4426950408889634f;
 
+__device__ int g_kv8_waits;                      // waits that ran out on this device so far (ft_kv8_waits)
+
 template <int D>
-__global__ void __launch_bounds__(K8D_WARPS * 32)
+struct K8Decode {
+    static constexpr int WARPS = D == 64 ? 7 : 4;                            // that compute; one more copies (two CTAs of eight warps: 128 registers a thread, of nine 96)
+    static constexpr int STAGES = D == 64 ? 11 : 5;                          // 90 / 82 KB on their way
+    static constexpr int THREADS = (WARPS + 1) * 32;
+    static constexpr int REC = D + 2;                                        // O[D], m, l
+    static constexpr int BARS = STAGES * Kv8<D>::REC;                        // byte offsets in shared memory
+    static constexpr int TOKENS = BARS + 2 * STAGES * 8;
+    static constexpr int MERGE = (TOKENS + STAGES * 4 + 15) / 16 * 16;
+    static constexpr int SMEM = MERGE + WARPS * K8D_GROUP * REC * 4;
+    static constexpr size_t PART = (size_t)K8D_GROUP * REC;                  // floats of a part
+};
+
+__global__ void kv8_decode_zero_kernel(int* counters, int n) {
+    pdl_launch_dependents();
+    for (int i = threadIdx.x; i < n; i += blockDim.x) counters[i] = 0;
+}
+
+template <int D>
+__global__ void __launch_bounds__(K8Decode<D>::THREADS, 2)
 kv8_decode_kernel(const __half* __restrict__ q, const uint8_t* __restrict__ cache, int num_pages, const int* __restrict__ page_table, int max_pages,
-                  const int* __restrict__ ctx_lens, __nv_bfloat16* __restrict__ out, __nv_bfloat16* __restrict__ out_lo, int nq, int nkv, float scale_log2) {
-    __shared__ float rec_s[K8D_WARPS][K8D_GROUP][D + 2];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
-    const int b = blockIdx.x / nkv, kvh = blockIdx.x % nkv, G = nq / nkv;
-    const int ctx = min(ctx_lens[b], max_pages * kKvTile);
-    const int tiles = (max(ctx, 0) + kKvTile - 1) / kKvTile;
-    Kv8Query<D> a;
-    a.clear();
-    a.load_query(g < G ? q + ((size_t)b * nq + (size_t)kvh * G + g) * D : nullptr, tq);
-    for (int t = warp; t < tiles; t += K8D_WARPS) {
-        const int page = page_table[(size_t)b * max_pages + t];
-        if (page < 0 || page >= num_pages) continue;
-        a.page(cache + ((size_t)page * nkv + kvh) * Kv8<D>::REC, min(ctx - t * kKvTile, kKvTile), scale_log2, g, tq);
+                  const int* __restrict__ ctx_lens, __nv_bfloat16* __restrict__ out, __nv_bfloat16* __restrict__ out_lo, int* counters, float* parts,
+                  int* err, int B, int nq, int nkv, float scale_log2) {
+    using C = K8Decode<D>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BARS);
+    uint64_t* empty = full + C::STAGES;
+    int* tokens = reinterpret_cast<int*>(smem + C::TOKENS);                  // of the page in each stage; 0: a page that is not there
+    float* merge = reinterpret_cast<float*>(smem + C::MERGE);
+    __shared__ long long s_sum[C::WARPS + 1];
+    __shared__ int s_most[C::WARPS + 1], s_b, s_last;
+    __shared__ long long s_base;
+    __shared__ volatile int dead;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tq = lane & 3;
+    const int G = nq / nkv;
+    if (tid == 0) {
+        for (int s = 0; s < C::STAGES; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
+        fence_mbar_init();
+        dead = 0;
     }
-    a.store(&rec_s[warp][0][0], g, tq);
+    auto ctx_of = [&](int b) { return max(0, min(ctx_lens[b], max_pages * kKvTile)); };
+    auto pages_of = [&](int b) { return (ctx_of(b) + kKvTile - 1) / kKvTile; };
+
+    // ---------------- the plan: this CTA's share of the flat list [sequence][head][page]
+    const int chunk = (B + C::THREADS - 1) / C::THREADS;
+    const int b0 = min(B, tid * chunk), b1 = min(B, b0 + chunk);
+    long long mine = 0;
+    int most = 0;
+    for (int b = b0; b < b1; ++b) {
+        const int n = pages_of(b);
+        mine += n;
+        most = max(most, n);
+    }
+    long long before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += up;
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 31) s_sum[warp] = before, s_most[warp] = most;
     __syncthreads();
-    for (int e = threadIdx.x; e < G * D; e += K8D_WARPS * 32) {
-        const int h = e / D, dim = e % D;
-        float M = -INFINITY, L = 0.f, O = 0.f;
-        for (int w = 0; w < K8D_WARPS; ++w) M = fmaxf(M, rec_s[w][h][D]);
-        for (int w = 0; w < K8D_WARPS; ++w) {
-            const float f = M == -INFINITY ? 0.f : exp2f(rec_s[w][h][D] - M);
-            L += rec_s[w][h][D + 1] * f;
-            O += rec_s[w][h][dim] * f;
-        }
-        const float r = L > 0.f ? O / L : 0.f;                       // a sequence without a visible key: zeros
-        const size_t at = ((size_t)b * nq + (size_t)kvh * G) * D + e;
-        const __nv_bfloat16 hb = __float2bfloat16(r);
-        out[at] = hb;
-        if (out_lo) out_lo[at] = __float2bfloat16(r - __bfloat162float(hb));
+    long long total = 0;
+    before -= mine;
+#pragma unroll
+    for (int w = 0; w <= C::WARPS; ++w) {
+        if (w < warp) before += s_sum[w];
+        total += s_sum[w];
+        most = max(most, s_most[w]);
     }
+    total *= nkv;
+    const long long per = (total + gridDim.x - 1) / gridDim.x;
+    const bool each = (long long)B * nkv <= gridDim.x;
+    const bool whole = each && (parts == nullptr || (most + C::WARPS - 1) / C::WARPS <= (per + C::WARPS - 1) / C::WARPS + 1);
+    long long f = per * blockIdx.x, f_end = min(f + per, total);
+    int b, h, t;
+    if (whole) {
+        b = blockIdx.x / nkv;
+        if (b >= B) {
+            pdl_wait();
+            return;
+        }
+        h = blockIdx.x % nkv;
+        t = 0;
+        f = 0;
+        f_end = pages_of(b);
+    } else {
+        if (before * nkv <= f && f < (before + mine) * nkv) {
+            int x = b0;
+            for (int n; before * nkv + (long long)(n = pages_of(x)) * nkv <= f; ++x) before += n;
+            s_b = x;
+            s_base = before;
+        }
+        __syncthreads();
+        if (f >= f_end) f_end = f;
+        b = s_b;
+        const long long rest = f - s_base * nkv;
+        const int n = f < f_end ? pages_of(b) : 1;
+        h = (int)(rest / n);
+        t = (int)(rest % n);
+    }
+    // a sequence without keys has no page and so no share: zeros
+    auto zeros = [&](int b_, int h0, int h1) {
+        for (int e = tid; e < (h1 - h0) * G * D; e += C::THREADS) {
+            const size_t at = ((size_t)b_ * nq + (size_t)h0 * G) * D + e;
+            out[at] = __float2bfloat16(0.f);
+            if (out_lo) out_lo[at] = __float2bfloat16(0.f);
+        }
+    };
+    if (whole) {
+        if (f_end == 0) zeros(b, h, h + 1);
+    } else {
+        for (int i = blockIdx.x; i < B; i += gridDim.x)
+            if (pages_of(i) == 0) zeros(i, 0, nkv);
+    }
+    if (f >= f_end) {
+        pdl_wait();
+        return;
+    }
+
+    int n_pages = pages_of(b);
+    // the next stretch of this share that lies in one (sequence, head): pages t0 .. t1 - 1
+    int seg_b, seg_h, t0, t1;
+    auto next = [&]() {
+        if (f >= f_end) return false;
+        while (t >= n_pages) {
+            t = 0;
+            if (++h == nkv) {
+                h = 0;
+                do n_pages = pages_of(++b);
+                while (n_pages == 0);
+            }
+        }
+        const int take = (int)min(f_end - f, (long long)(n_pages - t));
+        seg_b = b; seg_h = h; t0 = t; t1 = t + take;
+        t = t1;
+        f += take;
+        return true;
+    };
+
+    if (warp == C::WARPS) {
+        // ---------------- copies: one record a page
+        const uint64_t pol = policy_evict_first();                           // every byte is read once
+        int it = 0, asked = 0;
+        bool ok = true;
+        while (next()) {
+            const int ctx = ctx_of(seg_b);
+            const int* pt = page_table + (size_t)seg_b * max_pages;
+            for (int p0 = t0; p0 < t1; p0 += 32) {
+                const int my_page = p0 + lane < t1 ? pt[p0 + lane] : -1;
+                const int n = min(32, t1 - p0);
+                for (int i = 0; i < n; ++i, ++it) {
+                    const int page = __shfl_sync(0xffffffffu, my_page, i);
+                    if (lane == 0 && ok) {
+                        const int s = it % C::STAGES;
+                        ok = mbar_wait_limited(&empty[s], (it / C::STAGES & 1) ^ 1, &dead);
+                        if (!ok) continue;
+                        asked = it + 1;
+                        const bool there = page >= 0 && page < num_pages;
+                        tokens[s] = there ? min(kKvTile, ctx - (p0 + i) * kKvTile) : 0;
+                        if (there) {
+                            mbar_expect_tx(&full[s], Kv8<D>::REC);
+                            tma_bulk_g2s(smem + s * Kv8<D>::REC, cache + ((size_t)page * nkv + seg_h) * Kv8<D>::REC, Kv8<D>::REC, &full[s], pol);
+                        } else {
+                            mbar_arrive(&full[s]);
+                        }
+                    }
+                }
+            }
+        }
+        if (lane == 0 && (!ok || dead)) {                                    // gave up: what is under way still lands in this CTA's memory
+            *err = 1;
+            for (int i = max(0, asked - C::STAGES); i < asked; ++i)
+                for (int k = 0; k < kWaitLimit && !mbar_try_wait(&full[i % C::STAGES], i / C::STAGES & 1); ++k) {}
+        }
+        pdl_wait();
+        return;
+    }
+
+    // ---------------- the others: page it of the share is warp it % WARPS's
+    int it = 0;
+    while (next()) {
+        Kv8Query<D> a;
+        a.clear();
+        a.load_query(g < G ? q + ((size_t)seg_b * nq + (size_t)seg_h * G + g) * D : nullptr, tq);
+        bool ok = true;
+        for (int i = it + (warp - it % C::WARPS + C::WARPS) % C::WARPS; i < it + t1 - t0; i += C::WARPS) {
+            const int s = i % C::STAGES;
+            if (!mbar_wait_limited(&full[s], i / C::STAGES & 1, &dead)) {
+                ok = false;
+                break;
+            }
+            const int n = tokens[s];
+            if (n) a.page(smem + s * Kv8<D>::REC, n, scale_log2, g, tq);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[s]);
+        }
+        it += t1 - t0;
+        if (!ok) {                                                           // NaN for all that this (sequence, head) says
+            *err = 1;
+            a.m = 0.f;
+            a.l = NAN;
+        }
+        a.store(merge + (size_t)warp * C::PART, g, tq);
+        asm volatile("bar.sync 1, %0;" ::"n"(C::WARPS * 32) : "memory");
+        const bool all = t0 == 0 && t1 == n_pages;
+        const long long first = f - t1;                                      // of the (sequence, head) in the flat list (a whole one has no parts)
+        const int c0 = all ? 0 : (int)(first / per), c1 = all ? 0 : (int)((first + n_pages - 1) / per);
+        float* part = parts + (2 * (size_t)blockIdx.x + (t0 == 0)) * C::PART;
+        const size_t row = ((size_t)seg_b * nq + (size_t)seg_h * G) * D;
+        auto put = [&](int e, float x, float y, float l) {                   // two dims; a query without a visible key: zeros
+            const float r = l == 0.f ? 0.f : 1.f / l;
+            x *= r, y *= r;
+            const uint32_t hi = pack_bf16(x, y);
+            *reinterpret_cast<uint32_t*>(out + row + e) = hi;
+            if (out_lo) *reinterpret_cast<uint32_t*>(out_lo + row + e) = pack_bf16(x - bf16_lo(hi), y - bf16_hi(hi));
+        };
+        for (int e = 2 * tid; e < G * D; e += 2 * C::WARPS * 32) {
+            const int hg = e / D, dim = e % D;
+            const float* rec = merge + (size_t)hg * C::REC;
+            float m[C::WARPS], M = -INFINITY, L = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+            for (int w = 0; w < C::WARPS; ++w) m[w] = rec[w * C::PART + D], M = fmaxf(M, m[w]);
+#pragma unroll
+            for (int w = 0; w < C::WARPS; ++w) {
+                const float z = m[w] == -INFINITY ? 0.f : exp2f(m[w] - M);
+                const float2 o = *reinterpret_cast<const float2*>(rec + w * C::PART + dim);
+                L = fmaf(rec[w * C::PART + D + 1], z, L);
+                x = fmaf(o.x, z, x);
+                y = fmaf(o.y, z, y);
+            }
+            if (all) {
+                put(e, x, y, L);
+            } else {
+                *reinterpret_cast<float2*>(part + (size_t)hg * C::REC + dim) = make_float2(x, y);
+                if (dim == 0) *reinterpret_cast<float2*>(part + (size_t)hg * C::REC + D) = make_float2(M, L);
+            }
+        }
+        if (!all) {
+            // the last CTA to deliver a part puts all of them together, in their order
+            pdl_wait();                                                      // the counters are zeros now
+            asm volatile("bar.sync 1, %0;" ::"n"(C::WARPS * 32) : "memory");
+            if (tid == 0) {
+                __threadfence();
+                s_last = atomicAdd(&counters[c0], 1) == c1 - c0;
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(C::WARPS * 32) : "memory");
+            if (s_last) {
+                __threadfence();
+                for (int e = 2 * tid; e < G * D; e += 2 * C::WARPS * 32) {
+                    const int hg = e / D, dim = e % D;
+                    float M = -INFINITY, L = 0.f, x = 0.f, y = 0.f;
+                    for (int c = c0; c <= c1; c += 4) {                      // four parts asked for at once
+                        float2 ml[4], o[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const float* rec = parts + (2 * (size_t)min(c + k, c1) + (c + k == c0)) * C::PART + (size_t)hg * C::REC;
+                            ml[k] = __ldcg(reinterpret_cast<const float2*>(rec + D));
+                            o[k] = __ldcg(reinterpret_cast<const float2*>(rec + dim));
+                            if (c + k > c1) ml[k] = make_float2(-INFINITY, 0.f);
+                        }
+                        float Mn = M;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) Mn = fmaxf(Mn, ml[k].x);
+                        const float keep = M == -INFINITY ? 0.f : exp2f(M - Mn);
+                        L *= keep, x *= keep, y *= keep;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const float z = ml[k].x == -INFINITY ? 0.f : exp2f(ml[k].x - Mn);
+                            L = fmaf(ml[k].y, z, L);
+                            x = fmaf(o[k].x, z, x);
+                            y = fmaf(o[k].y, z, y);
+                        }
+                        M = Mn;
+                    }
+                    put(e, x, y, L);
+                }
+            }
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(C::WARPS * 32) : "memory");
+    }
+    pdl_wait();                                                              // this kernel ends behind the one before it
+}
+
+// counters (one for each CTA that a split (sequence, head) can begin in), then two parts a CTA: of the (sequence, head) it begins in the middle of, and of the one it ends in
+static int kv8_decode_ctas() { return 2 * device_sms(); }
+static size_t kv8_decode_counters(int ctas) { return (size_t)(ctas + 63) / 64 * 64; }
+
+template <int D>
+static int launch_kv8_decode(const void* q, const void* cache, int num_pages, const int* page_table, int max_pages, const int* ctx_lens, void* out, void* out_lo,
+                             void* scratch, int B, int nq, int nkv, cudaStream_t st) {
+    using C = K8Decode<D>;
+    static PerDeviceFlag attr_set;
+    if (!attr_set.done()) {
+        FT_CHECK_CUDA(cudaFuncSetAttribute(kv8_decode_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        attr_set.mark();
+    }
+    int* err = nullptr;
+    FT_CHECK_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&err), g_kv8_waits));
+    const int ctas = kv8_decode_ctas();
+    const bool whole = (long long)B * nkv <= ctas && max_pages <= K8D_WHOLE_PAGES;
+    FT_REQUIRE(whole || scratch, "ft_attn_decode_kv8: needs ft_attn_decode_kv8_scratch_bytes of work memory");
+    int* counters = whole ? nullptr : (int*)scratch;
+    float* parts = whole ? nullptr : (float*)scratch + kv8_decode_counters(ctas);
+    const float scale_log2 = K8D_LOG2E / sqrtf((float)D);
+    if (whole) {
+        kv8_decode_kernel<D><<<B * nkv, C::THREADS, C::SMEM, st>>>((const __half*)q, (const uint8_t*)cache, num_pages, page_table, max_pages, ctx_lens,
+                                                                   (__nv_bfloat16*)out, (__nv_bfloat16*)out_lo, counters, parts, err, B, nq, nkv, scale_log2);
+        FT_CHECK_CUDA(cudaGetLastError());
+        return 0;
+    }
+    kv8_decode_zero_kernel<<<1, 128, 0, st>>>(counters, ctas);
+    FT_CHECK_CUDA(cudaGetLastError());
+    // starts beside the zeroes; what was in the stream before them is done by then
+    FT_CHECK_CUDA(launch_after(kv8_decode_kernel<D>, dim3(ctas), dim3(C::THREADS), C::SMEM, st, (const __half*)q, (const uint8_t*)cache, num_pages, page_table,
+                               max_pages, ctx_lens, (__nv_bfloat16*)out, (__nv_bfloat16*)out_lo, counters, parts, err, B, nq, nkv, scale_log2));
+    return 0;
 }
 
 }  // namespace ft
 
+extern "C" long long ft_attn_decode_kv8_scratch_bytes(int d) {
+    FT_REQUIRE(d == 64 || d == 128, "ft_attn_decode_kv8_scratch_bytes: head_dim %d not supported (64 or 128)", d);
+    const int ctas = ft::kv8_decode_ctas();
+    return (long long)(ft::kv8_decode_counters(ctas) + 2 * (size_t)ctas * ft::K8D_GROUP * (d + 2)) * 4;
+}
+
+extern "C" int ft_kv8_waits(void) {
+    int n = 0;
+    FT_CHECK_CUDA(cudaMemcpyFromSymbol(&n, ft::g_kv8_waits, sizeof(n)));
+    return n;
+}
+
 extern "C" int ft_attn_decode_kv8(const void* q, const void* kv8_layer, int num_pages, const int* page_table, int max_pages, const int* ctx_lens, void* out,
-                                  void* out_lo, int B, int nq, int nkv, int d, void* stream) {
+                                  void* out_lo, void* scratch, int B, int nq, int nkv, int d, void* stream) {
     using namespace ft;
     FT_REQUIRE(d == 64 || d == 128, "ft_attn_decode_kv8: head_dim %d not supported (64 or 128)", d);
     FT_REQUIRE(nq >= 1 && nkv >= 1 && nq % nkv == 0 && nq / nkv <= K8D_GROUP, "ft_attn_decode_kv8: GQA group %d/%d not supported", nq, nkv);
-    FT_REQUIRE(B >= 0 && max_pages >= 0 && num_pages >= 0 && max_pages <= INT32_MAX / kKvTile && (long long)B * nkv <= INT32_MAX,
-               "ft_attn_decode_kv8: bad sizes B=%d nkv=%d max_pages=%d num_pages=%d", B, nkv, max_pages, num_pages);
+    FT_REQUIRE(B >= 0 && max_pages >= 0 && num_pages >= 0 && max_pages <= INT32_MAX / kKvTile, "ft_attn_decode_kv8: bad sizes B=%d max_pages=%d num_pages=%d", B,
+               max_pages, num_pages);
     if (B == 0) return 0;
     FT_REQUIRE(q && kv8_layer && page_table && ctx_lens && out, "ft_attn_decode_kv8: null argument");
-    FT_REQUIRE(((uintptr_t)q | (uintptr_t)kv8_layer) % 16 == 0, "ft_attn_decode_kv8: tensors on 16 bytes");
-    const float scale_log2 = K8D_LOG2E / sqrtf((float)d);
-    auto go = [&](auto kernel) {
-        kernel<<<B * nkv, K8D_WARPS * 32, 0, (cudaStream_t)stream>>>((const __half*)q, (const uint8_t*)kv8_layer, num_pages, page_table, max_pages, ctx_lens,
-                                                                     (__nv_bfloat16*)out, (__nv_bfloat16*)out_lo, nq, nkv, scale_log2);
-    };
-    if (d == 64) go(kv8_decode_kernel<64>);
-    else go(kv8_decode_kernel<128>);
-    FT_CHECK_CUDA(cudaGetLastError());
-    return 0;
+    FT_REQUIRE(((uintptr_t)q | (uintptr_t)kv8_layer | (uintptr_t)out | (uintptr_t)out_lo | (uintptr_t)scratch) % 16 == 0, "ft_attn_decode_kv8: tensors on 16 bytes");
+    return d == 64 ? launch_kv8_decode<64>(q, kv8_layer, num_pages, page_table, max_pages, ctx_lens, out, out_lo, scratch, B, nq, nkv, (cudaStream_t)stream)
+                   : launch_kv8_decode<128>(q, kv8_layer, num_pages, page_table, max_pages, ctx_lens, out, out_lo, scratch, B, nq, nkv, (cudaStream_t)stream);
 }

@@ -232,44 +232,71 @@ def sample(logits: torch.Tensor, temperature=None, top_k=None, top_p=None, seeds
 KV8_BLOCK = 16
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise N.NativeError(what)
+def _refuse(what: str, why: str) -> None:
+    raise N.NativeError(f"{what}: {why}")
 
 
 def _kv8_layer(layer: torch.Tensor, d: int, what: str):
     """(pages, kv heads) of a layer; all tensors of a call have to be on its device."""
-    _need(layer.is_cuda and layer.dtype == torch.uint8 and layer.dim() == 3 and layer.is_contiguous(), what + ": the cache is contiguous CUDA uint8 [pages, nkv, record]")
-    _need(layer.shape[2] == 128 * d + 32, what + ": the cache's records are not those of this head_dim")
-    return layer.shape[0], layer.shape[1]
+    if not (layer.is_cuda and layer.dtype == torch.uint8 and layer.dim() == 3 and layer.is_contiguous()):
+        _refuse(what, "the cache is contiguous CUDA uint8 [pages, nkv, record]")
+    pages, nkv, record = layer.shape
+    if record != 128 * d + 32:
+        _refuse(what, "the cache's records are not those of this head_dim")
+    return pages, nkv
 
 
-def _kv8_ints(t, dev, what: str) -> torch.Tensor:
-    """int32 on the device; a list goes up in a copy that the host waits for."""
+def _kv8_ints(t, dev, what: str, n: int = -1, name: str = "") -> torch.Tensor:
+    """int32 on the device, n of them; a list goes up in a copy that the host waits for."""
     if not isinstance(t, torch.Tensor):
         t = torch.tensor(t, dtype=torch.int32, device=dev).reshape(-1)
-    _need(t.dtype == torch.int32 and t.device == dev and t.is_contiguous(), what + ": contiguous int32 on the cache's device")
+    if not (t.dtype == torch.int32 and t.device == dev and t.is_contiguous()):
+        _refuse(what, f"{name} is contiguous int32 on the cache's device")
+    if n >= 0 and t.numel() != n:
+        _refuse(what, f"{name} has {n} numbers here, not {t.numel()}")
     return t
 
 
-def _kv8_table(t: torch.Tensor, dev, what: str) -> torch.Tensor:
-    _need(t.dtype == torch.int32 and t.device == dev and t.dim() == 2 and t.is_contiguous(), what + ": page_table is contiguous int32 [sequences, pages] on the cache's device")
-    return t
+def _kv8_table(t: torch.Tensor, dev, what: str):
+    if not (t.dtype == torch.int32 and t.device == dev and t.dim() == 2 and t.is_contiguous()):
+        _refuse(what, "page_table is contiguous int32 [sequences, pages] on the cache's device")
+    return t.shape
+
+
+def _kv8_requests(req_start, req_slot, req_pos0, dev, what: str):
+    req_slot = _kv8_ints(req_slot, dev, what, name="req_slot")
+    n = req_slot.numel()
+    return _kv8_ints(req_start, dev, what, n + 1, "req_start"), req_slot, _kv8_ints(req_pos0, dev, what, n, "req_pos0"), n
 
 
 def _kv8_call(dev, name: str, *args) -> None:
     """A library call on the device's current stream, whichever device is the current one."""
     fn = getattr(N.load(), name)
     if dev.index == torch.cuda.current_device():
-        N.check(fn(*args, N.cur_stream()), name)
+        rc = fn(*args, N.device_stream(dev.index))
     else:
         with torch.cuda.device(dev):
-            N.check(fn(*args, N.cur_stream()), name)
+            rc = fn(*args, N.device_stream(dev.index))
+    if rc < 0:
+        N.check(rc, name)
+
+
+_kv8_sizes = {}
+
+
+def _kv8_scratch_bytes(dev, name: str, d: int) -> int:
+    key = (dev.index, name, d)
+    n = _kv8_sizes.get(key)
+    if n is None:
+        with torch.cuda.device(dev):
+            n = _kv8_sizes[key] = N.check(getattr(N.load(), name)(d), name)
+    return n
 
 
 def kv8_cache_alloc(num_pages: int, nkv: int, d: int, device) -> torch.Tensor:
     """One layer of 8-bit KV cache, all zeros."""
-    _need(d in (64, 128), "kv8_cache_alloc: head_dim 64 or 128")
+    if d not in (64, 128):
+        _refuse("kv8_cache_alloc", "head_dim 64 or 128")
     return torch.zeros(num_pages, nkv, 128 * d + 32, device=device, dtype=torch.uint8)
 
 
@@ -281,18 +308,23 @@ def rope_kv8_append(qkv_partials: torch.Tensor, cos: torch.Tensor, sin: torch.Te
     what = "rope_kv8_append"
     dev = kv8_layer.device
     pages, heads = _kv8_layer(kv8_layer, d, what)
-    _need(heads == nkv, what + ": the cache has another number of heads")
-    _need(qkv_partials.dim() == 3 and qkv_partials.dtype == torch.float32 and qkv_partials.device == dev, what + ": qkv_partials is fp32 [S, T, (nq + 2 nkv) d] on the cache's device")
-    S, T, width = qkv_partials.shape
-    _need(width == (nq + 2 * nkv) * d and qkv_partials.stride(2) == 1 and (T < 2 or qkv_partials.stride(1) == width), what + ": qkv_partials has rows of (nq + 2 nkv) d")
-    _need(cos.dtype == torch.float32 and sin.dtype == torch.float32 and cos.device == dev and sin.device == dev and cos.is_contiguous() and sin.is_contiguous()
-          and cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] * 2 == d, what + ": cos and sin are contiguous fp32 [positions, d / 2] on the cache's device")
-    positions, seq_rows = _kv8_ints(positions, dev, what), _kv8_ints(seq_rows, dev, what)
-    _need(positions.numel() == T and seq_rows.numel() == T, what + ": a position and a sequence for every token")
-    page_table = _kv8_table(page_table, dev, what)
+    width = (nq + 2 * nkv) * d
+    if heads != nkv:
+        _refuse(what, "the cache has another number of heads")
+    if not (qkv_partials.dim() == 3 and qkv_partials.dtype == torch.float32 and qkv_partials.device == dev and qkv_partials.shape[2] == width):
+        _refuse(what, "qkv_partials is fp32 [S, T, (nq + 2 nkv) d] on the cache's device")
+    S, T, _ = qkv_partials.shape
+    part, row, one = qkv_partials.stride()
+    if one != 1 or (row != width and T > 1):
+        _refuse(what, "the rows of qkv_partials lie one behind the other")
+    if not (cos.dtype == sin.dtype == torch.float32 and cos.device == sin.device == dev and cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] * 2 == d
+            and cos.is_contiguous() and sin.is_contiguous()):
+        _refuse(what, "cos and sin are contiguous fp32 [positions, d / 2] on the cache's device")
+    positions, seq_rows = _kv8_ints(positions, dev, what, T, "positions"), _kv8_ints(seq_rows, dev, what, T, "seq_rows")
+    rows, most = _kv8_table(page_table, dev, what)
     q = torch.empty(T, nq, d, device=dev, dtype=torch.float16)
-    _kv8_call(dev, "ft_rope_kv8_append", qkv_partials.data_ptr(), S, qkv_partials.stride(0), cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(),
-              seq_rows.data_ptr(), page_table.data_ptr(), page_table.shape[0], page_table.shape[1], q.data_ptr(), kv8_layer.data_ptr(), pages, T, nq, nkv, d)
+    _kv8_call(dev, "ft_rope_kv8_append", qkv_partials.data_ptr(), S, part, cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(),
+              seq_rows.data_ptr(), page_table.data_ptr(), rows, most, q.data_ptr(), kv8_layer.data_ptr(), pages, T, nq, nkv, d)
     return q
 
 
@@ -302,37 +334,42 @@ def kv8_read(kv8_layer: torch.Tensor, page_table: torch.Tensor, req_start, req_s
     what = "kv8_read"
     dev = kv8_layer.device
     pages, nkv = _kv8_layer(kv8_layer, d, what)
-    page_table = _kv8_table(page_table, dev, what)
-    req_start, req_slot, req_pos0 = _kv8_ints(req_start, dev, what), _kv8_ints(req_slot, dev, what), _kv8_ints(req_pos0, dev, what)
-    n = req_slot.numel()
-    _need(req_start.numel() == n + 1 and req_pos0.numel() == n, what + ": a start and a position for every request, and the end")
-    _need(rows >= 0, what + ": a number of rows")
+    table_rows, most = _kv8_table(page_table, dev, what)
+    req_start, req_slot, req_pos0, n = _kv8_requests(req_start, req_slot, req_pos0, dev, what)
+    if rows < 0:
+        _refuse(what, "a number of rows")
     k = torch.empty(rows, nkv, d, device=dev, dtype=torch.float16)
     v = torch.empty(rows, nkv, d, device=dev, dtype=torch.float16)
-    _kv8_call(dev, "ft_kv8_read", kv8_layer.data_ptr(), pages, page_table.data_ptr(), page_table.shape[0], page_table.shape[1], req_start.data_ptr(),
+    _kv8_call(dev, "ft_kv8_read", kv8_layer.data_ptr(), pages, page_table.data_ptr(), table_rows, most, req_start.data_ptr(),
               req_slot.data_ptr(), req_pos0.data_ptr(), n, rows, k.data_ptr(), v.data_ptr(), nkv, d)
     return k, v
 
 
-def _kv8_query(q: torch.Tensor, kv8_layer: torch.Tensor, page_table: torch.Tensor, planes: int, what: str):
+def _kv8_query(q: torch.Tensor, kv8_layer: torch.Tensor, planes: int, what: str):
     dev = kv8_layer.device
-    _need(q.dim() == 3 and q.dtype == torch.float16 and q.device == dev and q.is_contiguous(), what + ": q is contiguous fp16 [rows, nq, d] on the cache's device")
-    pages, nkv = _kv8_layer(kv8_layer, q.shape[2], what)
-    _need(planes in (1, 2), what + ": one plane or two")
-    out = torch.empty(q.shape[0], q.shape[1] * q.shape[2], device=dev, dtype=torch.bfloat16)
-    return dev, pages, nkv, _kv8_table(page_table, dev, what), out, torch.empty_like(out) if planes == 2 else None
+    if not (q.dim() == 3 and q.dtype == torch.float16 and q.device == dev and q.is_contiguous()):
+        _refuse(what, "q is contiguous fp16 [rows, nq, d] on the cache's device")
+    rows, nq, d = q.shape
+    pages, nkv = _kv8_layer(kv8_layer, d, what)
+    if planes != 1 and planes != 2:
+        _refuse(what, "one plane or two")
+    out = torch.empty(rows, nq * d, device=dev, dtype=torch.bfloat16)
+    return dev, pages, nkv, rows, nq, d, out, torch.empty_like(out) if planes == 2 else None
 
 
 def attn_decode_kv8(q: torch.Tensor, kv8_layer: torch.Tensor, page_table: torch.Tensor, ctx_lens: torch.Tensor, planes: int = 2):
     """attn_decode over the 8-bit cache: q fp16 [B, nq, d], up to eight query heads a key head -> bf16 (hi, lo) planes [B, nq * d], lo None with planes = 1.  A
     sequence without keys gives zeros; keys on pages outside the cache are hidden."""
     what = "attn_decode_kv8"
-    dev, pages, nkv, page_table, out, lo = _kv8_query(q, kv8_layer, page_table, planes, what)
-    ctx_lens = _kv8_ints(ctx_lens, dev, what)
-    B, nq, d = q.shape
-    _need(ctx_lens.numel() == B and page_table.shape[0] >= B, what + ": a context length and a page-table row for every query")
-    _kv8_call(dev, "ft_attn_decode_kv8", q.data_ptr(), kv8_layer.data_ptr(), pages, page_table.data_ptr(), page_table.shape[1], ctx_lens.data_ptr(), out.data_ptr(),
-              N.ptr(lo), B, nq, nkv, d)
+    dev, pages, nkv, B, nq, d, out, lo = _kv8_query(q, kv8_layer, planes, what)
+    ctx_lens = _kv8_ints(ctx_lens, dev, what, B, "ctx_lens")
+    rows, most = _kv8_table(page_table, dev, what)
+    if rows < B:
+        _refuse(what, "a page-table row for every query")
+    n = _kv8_scratch_bytes(dev, "ft_attn_decode_kv8_scratch_bytes", d)
+    scratch = torch.empty(n, device=dev, dtype=torch.uint8) if most > 16 or B * nkv > 256 else None
+    _kv8_call(dev, "ft_attn_decode_kv8", q.data_ptr(), kv8_layer.data_ptr(), pages, page_table.data_ptr(), most, ctx_lens.data_ptr(), out.data_ptr(),
+              N.ptr(lo), N.ptr(scratch), B, nq, nkv, d)
     return out, lo
 
 
@@ -340,13 +377,11 @@ def attn_prefill_kv8(q: torch.Tensor, kv8_layer: torch.Tensor, page_table: torch
     """attn_prefill over the 8-bit cache, up to eight query heads a key head.  The lists are int32 tensors on the device (then nothing goes up, and the call can be
     captured) or anything a tensor is made of.  Rows that no request owns are zeros; keys on pages outside the cache are hidden.  -> (hi, lo), lo None with planes = 1."""
     what = "attn_prefill_kv8"
-    dev, pages, nkv, page_table, out, lo = _kv8_query(q, kv8_layer, page_table, planes, what)
-    req_q_start, req_slot, req_pos0 = _kv8_ints(req_q_start, dev, what), _kv8_ints(req_slot, dev, what), _kv8_ints(req_pos0, dev, what)
-    n = req_slot.numel()
-    _need(req_q_start.numel() == n + 1 and req_pos0.numel() == n, what + ": a start and a position for every request, and the end")
-    T, nq, d = q.shape
-    _kv8_call(dev, "ft_attn_prefill_kv8", q.data_ptr(), kv8_layer.data_ptr(), pages, page_table.data_ptr(), page_table.shape[0], page_table.shape[1],
-              req_q_start.data_ptr(), req_slot.data_ptr(), req_pos0.data_ptr(), n, T, out.data_ptr(), N.ptr(lo), nq, nkv, d)
+    dev, pages, nkv, T, nq, d, out, lo = _kv8_query(q, kv8_layer, planes, what)
+    rows, most = _kv8_table(page_table, dev, what)
+    req_q_start, req_slot, req_pos0, n = _kv8_requests(req_q_start, req_slot, req_pos0, dev, what)
+    _kv8_call(dev, "ft_attn_prefill_kv8", q.data_ptr(), kv8_layer.data_ptr(), pages, page_table.data_ptr(), rows, most, req_q_start.data_ptr(),
+              req_slot.data_ptr(), req_pos0.data_ptr(), n, T, out.data_ptr(), N.ptr(lo), nq, nkv, d)
     return out, lo
 
 

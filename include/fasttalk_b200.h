@@ -682,9 +682,15 @@ int ft_rope_kv8_append(const float* qkv, int n_splits, long long split_stride, c
  * req_pos0[r] of page-table row req_slot[r].  All `rows` rows are written; those that no request owns with zeros. */
 int ft_kv8_read(const void* kv8_layer, int num_pages, const int* page_table, int table_rows, int max_pages, const int* req_start,
                 const int* req_slot, const int* req_pos0, int n_req, int rows, void* k_out, void* v_out, int nkv, int d, void* stream);
-/* One query token per sequence: q FP16 [B][nq][d], nq / nkv up to 8, out bf16 [B][nq*d] (+ residual plane out_lo, may be NULL). */
+/* One query token per sequence: q FP16 [B][nq][d], nq / nkv up to 8, out bf16 [B][nq*d] (+ residual plane out_lo, may be NULL).  scratch: work memory of
+ * ft_attn_decode_kv8_scratch_bytes(d) bytes (of the current device), in any state, not shared by calls that may overlap; NULL will do where max_pages <= 16 and B * nkv is no larger than twice
+ * the number of SMs. */
+long long ft_attn_decode_kv8_scratch_bytes(int d);
 int ft_attn_decode_kv8(const void* q, const void* kv8_layer, int num_pages, const int* page_table, int max_pages, const int* ctx_lens, void* out,
-                       void* out_lo, int B, int nq, int nkv, int d, void* stream);
+                       void* out_lo, void* scratch, int B, int nq, int nkv, int d, void* stream);
+/* Every wait inside the kernels of this cache has a limit; one that runs out leaves NaN in the rows it was for.  -> 1 if that has happened on the current device since the library
+ * was loaded, else 0 (waits for the device). */
+int ft_kv8_waits(void);
 /* Causal attention of prompt portions: q FP16 [T][nq][d], nq / nkv up to 8, request r owns rows req_q_start[r] .. req_q_start[r + 1] - 1 (req_q_start grows), page-table row req_slot[r],
  * and its first query sits at position req_pos0[r].  The lists are DEVICE arrays.  All T rows of out (and out_lo, may be NULL) are written; those that no request owns with zeros. */
 int ft_attn_prefill_kv8(const void* q, const void* kv8_layer, int num_pages, const int* page_table, int table_rows, int max_pages,
