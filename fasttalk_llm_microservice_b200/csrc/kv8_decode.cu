@@ -17,12 +17,14 @@ constexpr int K8D_GROUP = 8;                     // query heads a key head at mo
 constexpr int K8D_WHOLE_PAGES = 16;              // with page tables no wider than this, and a CTA for each (sequence, head), there are never parts
 constexpr float K8D_LOG2E = 1.4426950408889634f;
 
-__device__ int g_kv8_waits;                      // waits that ran out on this device so far (ft_kv8_waits)
+__device__ int g_kv8_waits;                      // 1: a wait ran out on this device (ft_kv8_waits)
 
 template <int D>
 struct K8Decode {
-    static constexpr int WARPS = D == 64 ? 7 : 4;                            // that compute; one more copies (two CTAs of eight warps: 128 registers a thread, of nine 96)
-    static constexpr int STAGES = D == 64 ? 11 : 5;                          // 90 / 82 KB on their way
+    static constexpr int WARPS = D == 64 ? 6 : 5;                            // that compute; one more copies
+    static constexpr int STAGES = D == 64 ? 12 : 5;                          // 99 / 82 KB on their way
+    // A stage is always the same warp's: a warp that another one's page passes in the same stage would take the phase before its own for its own
+    static_assert(STAGES % WARPS == 0, "a stage belongs to one warp");
     static constexpr int THREADS = (WARPS + 1) * 32;
     static constexpr int REC = D + 2;                                        // O[D], m, l
     static constexpr int BARS = STAGES * Kv8<D>::REC;                        // byte offsets in shared memory
@@ -208,10 +210,8 @@ kv8_decode_kernel(const __half* __restrict__ q, const uint8_t* __restrict__ cach
         bool ok = true;
         for (int i = it + (warp - it % C::WARPS + C::WARPS) % C::WARPS; i < it + t1 - t0; i += C::WARPS) {
             const int s = i % C::STAGES;
-            if (!mbar_wait_limited(&full[s], i / C::STAGES & 1, &dead)) {
-                ok = false;
-                break;
-            }
+            ok = __all_sync(0xffffffffu, mbar_wait_limited(&full[s], i / C::STAGES & 1, &dead));
+            if (!ok) break;
             const int n = tokens[s];
             if (n) a.page(smem + s * Kv8<D>::REC, n, scale_log2, g, tq);
             __syncwarp();
@@ -304,6 +304,19 @@ kv8_decode_kernel(const __half* __restrict__ q, const uint8_t* __restrict__ cach
     pdl_wait();                                                              // this kernel ends behind the one before it
 }
 
+// where this device's count of waits that ran out lies (looked up once for each device)
+int kv8_waits_address(int** at) {
+    static int* known[kMaxDevices];
+    const int dev = current_device_slot();
+    if (!known[dev]) {
+        int* p = nullptr;
+        FT_CHECK_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_kv8_waits));
+        known[dev] = p;
+    }
+    *at = known[dev];
+    return 0;
+}
+
 // counters (one for each CTA that a split (sequence, head) can begin in), then two parts a CTA: of the (sequence, head) it begins in the middle of, and of the one it ends in
 static int kv8_decode_ctas() { return 2 * device_sms(); }
 static size_t kv8_decode_counters(int ctas) { return (size_t)(ctas + 63) / 64 * 64; }
@@ -318,7 +331,7 @@ static int launch_kv8_decode(const void* q, const void* cache, int num_pages, co
         attr_set.mark();
     }
     int* err = nullptr;
-    FT_CHECK_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&err), g_kv8_waits));
+    if (int r = kv8_waits_address(&err)) return r;
     const int ctas = kv8_decode_ctas();
     const bool whole = (long long)B * nkv <= ctas && max_pages <= K8D_WHOLE_PAGES;
     FT_REQUIRE(whole || scratch, "ft_attn_decode_kv8: needs ft_attn_decode_kv8_scratch_bytes of work memory");
