@@ -1,0 +1,119 @@
+// The walk over the units of work of the prompt attention (kv8_prefill.cu): plain arithmetic, the same on the host
+#pragma once
+#include "common.cuh"
+
+namespace ft {
+
+struct Kv8Prompt {
+    const __half* q;
+    const uint8_t* cache;
+    const int *page_table, *req_q_start, *req_slot, *req_pos0;
+    __nv_bfloat16 *out, *out_lo;
+    int* counters;
+    float* parts;
+    int* err;
+    int num_pages, table_rows, max_pages, n_req, T, nq, nkv;
+    int G, th;                                                       // query heads a key head, tokens of a half
+    unsigned inv_g;                                                  // row / G = row * inv_g >> 16
+    float scale_log2;
+};
+
+// sum over i < n of floor((a i + b) / 64): the lattice points below a line, by Euclid's steps
+__host__ __device__ inline long long floor_sum64(long long n, long long a, long long b) {
+    long long m = 64, sum = 0;
+    while (n > 0) {
+        sum += n * (n - 1) / 2 * (a / m) + n * (b / m);
+        a %= m;
+        b %= m;
+        const long long top = a * n + b;
+        n = top / m;
+        b = top % m;
+        const long long t = a;
+        a = m;
+        m = t;
+        if (m == 0) break;
+    }
+    return sum;
+}
+
+// one request: its rows of q, tiles of 2 th tokens, steps of its tiles
+struct Kv8Request {
+    int row0, len, pos0, slot, tiles;
+    __host__ __device__ __forceinline__ void load(const Kv8Prompt& p, int r) {
+        row0 = max(0, min(p.req_q_start[r], p.T));
+        len = max(0, min(p.req_q_start[r + 1], p.T) - row0);
+        pos0 = max(0, min(p.req_pos0[r], p.max_pages * kKvTile));
+        slot = p.req_slot[r];
+        tiles = (len + 2 * p.th - 1) / (2 * p.th);
+    }
+    __host__ __device__ __forceinline__ int tokens(const Kv8Prompt& p, int i) const { return min(2 * p.th, len - i * 2 * p.th); }
+    __host__ __device__ __forceinline__ int pages(const Kv8Prompt& p, int i) const { return (pos0 + i * 2 * p.th + tokens(p, i) - 1) / kKvTile + 1; }
+    __host__ __device__ __forceinline__ int steps(const Kv8Prompt& p, int i) const {
+        const int n = pages(p, i);
+        return tokens(p, i) <= p.th ? (n + 1) / 2 : n;
+    }
+    __host__ __device__ __forceinline__ long long before(const Kv8Prompt& p, int i) const { return floor_sum64(i, 2 * p.th, (long long)pos0 + 2 * p.th - 1) + i; }   // steps of the full tiles 0 .. i - 1
+    __host__ __device__ __forceinline__ long long all(const Kv8Prompt& p) const { return tiles ? before(p, tiles - 1) + steps(p, tiles - 1) : 0; }
+};
+
+// A CTA's share, walked stretch by stretch; a stretch = steps t0 .. t1 - 1 of one unit
+struct Kv8Walk {
+    Kv8Request q;
+    long long f, f_end;                                              // where it is in the flat list of steps
+    int r, h, i, t, t0, t1, n_steps, n_pages, n_tok;
+    bool few;
+    __host__ __device__ __forceinline__ void unit(const Kv8Prompt& p) {
+        n_tok = q.tokens(p, i);
+        n_pages = q.pages(p, i);
+        few = n_tok <= p.th;
+        n_steps = few ? (n_pages + 1) / 2 : n_pages;
+    }
+    __host__ __device__ __forceinline__ bool next(const Kv8Prompt& p) {
+        if (f >= f_end) return false;
+        if (t >= n_steps) {
+            t = 0;
+            if (++i == q.tiles) {
+                i = 0;
+                if (++h == p.nkv) {
+                    h = 0;
+                    do q.load(p, ++r);
+                    while (q.len == 0);
+                }
+            }
+            unit(p);
+        }
+        t0 = t;
+        t1 = t + (int)min(f_end - f, (long long)(n_steps - t));
+        t = t1;
+        f += t1 - t0;
+        return true;
+    }
+    // where step (or, where each CTA takes whole units, unit) `at` of the flat list lies; `before` of them belong to requests ahead of r0, and it is r0's or a later one's
+    __host__ __device__ inline void seek(const Kv8Prompt& p, bool whole, int r0, long long before, long long at) {
+        for (r = r0;; ++r) {
+            q.load(p, r);
+            const long long n = whole ? q.tiles : q.all(p);
+            if (at < (before + n) * p.nkv) {
+                long long rest = at - before * p.nkv;
+                h = (int)(rest / n);
+                rest -= h * n;
+                int lo = 0, hi = q.tiles - 1;                        // the last tile that begins at or before rest
+                while (!whole && lo < hi) {
+                    const int mid = (lo + hi + 1) >> 1;
+                    if (q.before(p, mid) <= rest) lo = mid; else hi = mid - 1;
+                }
+                i = whole ? (int)rest : lo;
+                t = whole ? 0 : (int)(rest - q.before(p, lo));
+                return;
+            }
+            before += n;
+        }
+    }
+    // pages of the stretch, in the order in which they are asked for
+    __host__ __device__ __forceinline__ int page0() const { return few ? 2 * t0 : t0; }
+    __host__ __device__ __forceinline__ int page1() const { return few ? min(2 * t1, n_pages) : t1; }
+    __host__ __device__ __forceinline__ int row0(const Kv8Prompt& p) const { return q.row0 + i * 2 * p.th; }
+    __host__ __device__ __forceinline__ int position0(const Kv8Prompt& p) const { return q.pos0 + i * 2 * p.th; }
+};
+
+}  // namespace ft

@@ -692,10 +692,12 @@ int ft_attn_decode_kv8(const void* q, const void* kv8_layer, int num_pages, cons
  * was loaded, else 0 (waits for the device). */
 int ft_kv8_waits(void);
 /* Causal attention of prompt portions: q FP16 [T][nq][d], nq / nkv up to 8, request r owns rows req_q_start[r] .. req_q_start[r + 1] - 1 (req_q_start grows), page-table row req_slot[r],
- * and its first query sits at position req_pos0[r].  The lists are DEVICE arrays.  All T rows of out (and out_lo, may be NULL) are written; those that no request owns with zeros. */
+ * and its first query sits at position req_pos0[r].  The lists are DEVICE arrays.  All T rows of out (and out_lo, may be NULL) are written; those that no request owns with zeros.
+ * scratch: work memory of ft_attn_prefill_kv8_scratch_bytes(d) bytes (of the current device), in any state, not shared by calls that may overlap. */
+long long ft_attn_prefill_kv8_scratch_bytes(int d);
 int ft_attn_prefill_kv8(const void* q, const void* kv8_layer, int num_pages, const int* page_table, int table_rows, int max_pages,
-                        const int* req_q_start, const int* req_slot, const int* req_pos0, int n_req, int T, void* out, void* out_lo, int nq, int nkv,
-                        int d, void* stream);
+                        const int* req_q_start, const int* req_slot, const int* req_pos0, int n_req, int T, void* out, void* out_lo, void* scratch,
+                        int nq, int nkv, int d, void* stream);
 
 /* K7: per-row temperature / top-k / top-p sampling (argmax when temperature <= 0; a null temperature says so for all rows).
  * A row without any logit above minus infinity gives index 0. */
