@@ -11,7 +11,7 @@
 // to the largest of the stretch of pages at hand, which the same warps look up ahead (vref; the output takes it back).  Both roundings are fp16's 2^-11 of a value.
 //
 // The flat list of all (request, key head, tile, page) is cut into equal shares, one for each SM: a causal list's units differ in length by any factor, and shares do
-// not.  A unit that lies in several shares is put together by the last CTA to arrive, in the parts' order.  Where there is an SM for every unit and none is much longer than
+// not.  A unit that lies in several shares is put together by a second kernel, in the parts' order.  Where there is an SM for every unit and none is much longer than
 // a share, each CTA takes a whole one.  Everything is found by each CTA from the lists on the device; nothing is planned ahead.
 #include "common.cuh"
 #include "ft_internal.h"
@@ -33,7 +33,7 @@ template <int D>
 struct K8Prefill {
     static constexpr int KH = D / 64;
     static constexpr int TILE = 2 * KH * K8P_PIECE;                  // K | V of a page in fp16
-    static constexpr int S16 = D == 64 ? 6 : 3, S8 = D == 64 ? 6 : 4;
+    static constexpr int S16 = D == 64 ? 6 : 3, S8 = D == 64 ? 6 : 3;
     static constexpr int QBLK = K8P_ROWS * 128;                      // [128 rows][64 dims]
     static constexpr int Q_BYTES = 2 * KH * QBLK;
     static constexpr int KV = Q_BYTES, REC = KV + S16 * TILE, BARS = REC + S8 * Kv8<D>::REC;
@@ -43,10 +43,8 @@ struct K8Prefill {
     static constexpr size_t PART = (size_t)2 * K8P_ROWS * (D + 2);   // floats of a part: O [256][D], then (m, l) [256]
 };
 
-__global__ void kv8_prefill_zero_kernel(int* counters, int n) {
-    pdl_launch_dependents();
-    for (int i = threadIdx.x; i < n; i += blockDim.x) counters[i] = 0;
-}
+// floats that the descriptions of split units take at the head of the work memory
+static size_t kv8_prefill_splits(int ctas) { return (size_t)(ctas + 15) / 16 * 16 * (sizeof(Kv8Split) / 4); }
 
 template <int D>
 __global__ void __launch_bounds__(K8P_THREADS, 1)
@@ -69,7 +67,8 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
     int* there_s = reinterpret_cast<int*>(kscale_s + 4 * C::S16);            // [S8]
     __shared__ uint32_t tmem_slot;
     __shared__ long long s_sum[K8P_THREADS / 32], s_units[K8P_THREADS / 32];
-    __shared__ int s_most[K8P_THREADS / 32], s_r, s_h, s_i, s_t, s_last;
+    __shared__ int s_most[K8P_THREADS / 32], s_r, s_h, s_i, s_t;
+    __shared__ float2 s_ml[K8P_SOFT];
     __shared__ float s_vref[4], s_vmax[K8P_CONV / 32];
     __shared__ volatile int dead;
 
@@ -125,7 +124,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
     total *= p.nkv;
     n_units *= p.nkv;
     const long long per = (total + gridDim.x - 1) / gridDim.x;
-    const bool whole = n_units <= gridDim.x && most <= per + K8P_WHOLE;
+    const bool whole = p.split == nullptr || (n_units <= gridDim.x && most <= per + K8P_WHOLE);      // no room for parts: the host knows that there are none
     // the flat list is one of units or of steps
     const long long len = whole ? n_units : total, each = whole ? 1 : per;
     w.f = min(len, each * blockIdx.x);
@@ -264,14 +263,17 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
             }
             if (seg) ok = ok && mbar_wait_limited(q_empty, (seg - 1) & 1, &dead);
             ok = __all_sync(0xffffffffu, ok);
-            const int halves = !ok ? 0 : w.few ? 1 : 2, row0 = w.row0(p), chunks = D / 8;
-            for (int k = ct; k < halves * K8P_ROWS * chunks; k += K8P_CONV) {
-                const int c = k % chunks, rr = k / chunks, h = rr >> 7, row = rr & 127;
+            const int halves = !ok ? 0 : w.few ? 1 : 2, row0 = w.row0(p);
+            constexpr int CH = D / 8;
+#pragma unroll 8
+            for (int k = ct; k < halves * K8P_ROWS * CH; k += K8P_CONV) {    // 16 bytes each, all on their way at once; zeros for rows without a token
+                const int c = k % CH, rr = k / CH, h = rr >> 7, row = rr & 127;
                 const int tok = row * p.inv_g >> 16, head = row - tok * p.G;
                 const bool on = tok < p.th && h * p.th + tok < w.n_tok;
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (on) v = *reinterpret_cast<const uint4*>(p.q + ((size_t)(row0 + h * p.th + tok) * p.nq + (size_t)w.h * p.G + head) * D + c * 8);
-                *reinterpret_cast<uint4*>(smem + (h * KH + (c >> 3)) * C::QBLK + row * 128 + ((c & 7) ^ (row & 7)) * 16) = v;
+                const __half* from = p.q + ((size_t)(row0 + (on ? h * p.th + tok : 0)) * p.nq + (size_t)w.h * p.G + (on ? head : 0)) * D + c * 8;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem + (h * KH + (c >> 3)) * C::QBLK + row * 128 + ((c & 7) ^ (row & 7)) * 16)),
+                             "l"(from), "r"(on ? 16 : 0)
+                             : "memory");
             }
             vmax = warp_max(vmax);
             if (lane == 0) s_vmax[cw] = vmax;
@@ -280,6 +282,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
             asm volatile("bar.sync 2, %0;" ::"n"(K8P_CONV) : "memory");
             if (ct == 0) s_vref[seg & 3] = vmax;                             // the softmax warps may still be at the end of the stretch before the last
             const float vinv = vmax > 0.f ? 1.f / vmax : 0.f;
+            asm volatile("cp.async.wait_all;" ::: "memory");
             fence_proxy_async();
             __syncwarp();
             if (lane == 0 && ok) mbar_arrive(q_full);
@@ -331,6 +334,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
         const int tok = row * p.inv_g >> 16, head = row - tok * p.G;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
         const uint32_t s_at = lanes + C::COL_S + 2 * h * 64, o_at = lanes + C::COL_O + h * D;
+        if (st == 0 && p.split) p.split[blockIdx.x].parts = 0;
         // rows that no request owns
         {
             const int a = p.n_req ? max(0, min(p.req_q_start[0], p.T)) : p.T, b = p.n_req ? max(a, min(p.req_q_start[p.n_req], p.T)) : p.T;
@@ -434,9 +438,26 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                 l_run = NAN;
                 m_ref = 0.f;
             }
-            const float vref = ok ? s_vref[seg & 3] : 0.f;
+            float vref = ok && mine_n ? s_vref[seg & 3] : 0.f;
             const bool all = w.t0 == 0 && w.t1 == w.n_steps;
             const size_t off = ((size_t)(w.row0(p) + my_tok) * p.nq + (size_t)w.h * p.G + head) * D;
+            auto put = [&](int c, const uint32_t* o) {                       // 16 dims of the row
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float x = __uint_as_float(o[2 * k]), y = __uint_as_float(o[2 * k + 1]);
+                    hi[k] = pack_bf16(x, y);
+                    lo[k] = pack_bf16(x - bf16_lo(hi[k]), y - bf16_hi(hi[k]));
+                }
+                uint4* to = reinterpret_cast<uint4*>(p.out + off + 16 * c);
+                to[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                to[1] = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+                if (p.out_lo) {
+                    to = reinterpret_cast<uint4*>(p.out_lo + off + 16 * c);
+                    to[0] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    to[1] = make_uint4(lo[4], lo[5], lo[6], lo[7]);
+                }
+            };
             if (all && !w.few) {
                 const float inv = l_run == 0.f ? 0.f : vref / l_run;         // a query without a visible key: zeros
 #pragma unroll 1
@@ -444,98 +465,60 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                     uint32_t o[16];
                     tmem_ld16_nowait(o_at + 16 * c, o);
                     tmem_ld_wait();
-                    if (!valid) continue;
-                    uint32_t hi[8], lo[8];
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const float x = __uint_as_float(o[2 * k]) * inv, y = __uint_as_float(o[2 * k + 1]) * inv;
-                        hi[k] = pack_bf16(x, y);
-                        lo[k] = pack_bf16(x - bf16_lo(hi[k]), y - bf16_hi(hi[k]));
-                    }
-                    uint4* to = reinterpret_cast<uint4*>(p.out + off + 16 * c);
-                    to[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    to[1] = make_uint4(hi[4], hi[5], hi[6], hi[7]);
-                    if (p.out_lo) {
-                        to = reinterpret_cast<uint4*>(p.out_lo + off + 16 * c);
-                        to[0] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                        to[1] = make_uint4(lo[4], lo[5], lo[6], lo[7]);
-                    }
+                    for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * inv);
+                    if (valid) put(c, o);
                 }
+            } else if (all) {
+                // two halves of the pages: each half of the warps puts half of the dims together
+                s_ml[st] = make_float2(m_ref, l_run);
+                tc_fence_before();
+                asm volatile("bar.sync 1, %0;" ::"n"(K8P_SOFT) : "memory");
+                tc_fence_after();
+                if (ok) vref = s_vref[seg & 3];                              // a half without a page has waited for nothing before
+                const float2 other = s_ml[st ^ K8P_ROWS];
+                const float m = fmaxf(m_ref, other.x);
+                const float z = m_ref == -INFINITY ? 0.f : exp2f(m_ref - m), zo = other.x == -INFINITY ? 0.f : exp2f(other.x - m);
+                const float L = h == 0 ? l_run * z + other.y * zo : other.y * zo + l_run * z;
+                const float inv = L == 0.f ? 0.f : vref / L;
+#pragma unroll 1
+                for (int c = h * (D / 32); c < (h + 1) * (D / 32); ++c) {
+                    uint32_t o[16], x[16];
+                    tmem_ld16_nowait(o_at + 16 * c, o);
+                    tmem_ld16_nowait(lanes + C::COL_O + (1 - h) * D + 16 * c, x);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {                           // a half without a page has nothing in tensor memory
+                        const float u = z == 0.f ? 0.f : __uint_as_float(o[k]) * z, v = zo == 0.f ? 0.f : __uint_as_float(x[k]) * zo;
+                        o[k] = __float_as_uint((h == 0 ? u + v : v + u) * inv);
+                    }
+                    if (valid) put(c, o);
+                }
+                asm volatile("bar.sync 1, %0;" ::"n"(K8P_SOFT) : "memory");
             } else {
                 // a part: O in its own size, maximum and sum of each row; the halves of a unit of few tokens are two parts
                 float* part = p.parts + (2 * (size_t)blockIdx.x + (w.t0 == 0)) * C::PART;
-                const int rr = h * K8P_ROWS + row;
+                const int rr = h * K8P_ROWS + row;                           // (not st: a warp's rows are those lanes of tensor memory that it may read)
 #pragma unroll 1
                 for (int c = 0; c < D / 16; ++c) {
                     uint32_t o[16];
                     tmem_ld16_nowait(o_at + 16 * c, o);
                     tmem_ld_wait();
-                    if (!valid) continue;
                     float4* to = reinterpret_cast<float4*>(part + (size_t)rr * D + 16 * c);
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        to[k] = mine_n ? make_float4(__uint_as_float(o[4 * k]) * vref, __uint_as_float(o[4 * k + 1]) * vref, __uint_as_float(o[4 * k + 2]) * vref,
+                        if (valid) to[k] = mine_n ? make_float4(__uint_as_float(o[4 * k]) * vref, __uint_as_float(o[4 * k + 1]) * vref, __uint_as_float(o[4 * k + 2]) * vref,
                                                      __uint_as_float(o[4 * k + 3]) * vref)
                                        : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
                 if (valid) *reinterpret_cast<float2*>(part + (size_t)2 * K8P_ROWS * D + 2 * rr) = make_float2(m_ref, l_run);
-                const long long first = w.f - w.t1;                          // of the unit in the flat list
-                const int c0 = all ? (int)blockIdx.x : (int)(first / per), c1 = all ? (int)blockIdx.x : (int)((first + w.n_steps - 1) / per);
-                __threadfence();
-                if (!all) pdl_wait();                                        // the counters are zeros now
-                asm volatile("bar.sync 1, %0;" ::"n"(K8P_SOFT) : "memory");
-                if (st == 0) {
-                    s_last = all || atomicAdd(&p.counters[c0], 1) == c1 - c0;
-                    __threadfence();
-                }
-                asm volatile("bar.sync 1, %0;" ::"n"(K8P_SOFT) : "memory");
-                if (s_last) {
-                    constexpr int LR = D / 4;                                // lanes a row
-                    const int d4 = st % LR * 4, subs = w.few ? 2 : 1;
-                    for (int r2 = st / LR; r2 < (w.few ? 1 : 2) * K8P_ROWS; r2 += K8P_SOFT / LR) {
-                        const int rw = r2 & 127, tk = rw * p.inv_g >> 16, t2 = (r2 >> 7) * p.th + tk;
-                        if (tk >= p.th || t2 >= w.n_tok) continue;
-                        float M = -INFINITY, L = 0.f;
-                        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                        const int np = (c1 - c0 + 1) * subs;
-                        for (int c = 0; c < np; c += 4) {
-                            float2 ml[4];
-                            float4 o[4];
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {                    // four parts asked for at once
-                                const int x = min(c + k, np - 1), cta = c0 + x / subs, rec_row = r2 + (x % subs) * K8P_ROWS;
-                                const float* rec = p.parts + (2 * (size_t)cta + (cta == c0)) * C::PART;
-                                ml[k] = __ldcg(reinterpret_cast<const float2*>(rec + (size_t)2 * K8P_ROWS * D + 2 * rec_row));
-                                o[k] = __ldcg(reinterpret_cast<const float4*>(rec + (size_t)rec_row * D + d4));
-                                if (c + k >= np) ml[k] = make_float2(-INFINITY, 0.f);
-                            }
-                            const float Mn = fmaxf(M, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)));
-                            const float keep = M == -INFINITY ? 0.f : exp2f(M - Mn);
-                            L *= keep; acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const float z = ml[k].x == -INFINITY ? 0.f : exp2f(ml[k].x - Mn);
-                                L = fmaf(ml[k].y, z, L);
-                                acc = fma_f4(o[k], make_float4(z, z, z, z), acc);
-                            }
-                            M = Mn;
-                        }
-                        const float inv = L == 0.f ? 0.f : 1.f / L;
-                        const float x0 = acc.x * inv, x1 = acc.y * inv, x2 = acc.z * inv, x3 = acc.w * inv;
-                        const uint32_t h0 = pack_bf16(x0, x1), h1 = pack_bf16(x2, x3);
-                        const size_t to = ((size_t)(w.row0(p) + t2) * p.nq + (size_t)w.h * p.G + (rw - tk * p.G)) * D + d4;
-                        *reinterpret_cast<uint2*>(p.out + to) = make_uint2(h0, h1);
-                        if (p.out_lo)
-                            *reinterpret_cast<uint2*>(p.out_lo + to) = make_uint2(pack_bf16(x0 - bf16_lo(h0), x1 - bf16_hi(h0)), pack_bf16(x2 - bf16_lo(h1), x3 - bf16_hi(h1)));
-                    }
-                }
-                asm volatile("bar.sync 1, %0;" ::"n"(K8P_SOFT) : "memory");  // s_last, and the parts, are free again
+                if (st == 0 && w.t0 == 0)                                    // the unit begins here: what the next kernel has to know of it
+                    p.split[blockIdx.x] = Kv8Split{(int)((w.f - w.t1 + w.n_steps - 1) / per) - (int)blockIdx.x + 1, w.row0(p), w.h, w.few ? -w.n_tok : w.n_tok};
             }
             base += n;
             ++seg;
         }
     }
-    pdl_wait();                                                              // this kernel ends behind the one before it
     tc_fence_before();
     __syncthreads();
     if (warp == 1) {
@@ -544,25 +527,101 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
     }
 }
 
-static size_t kv8_prefill_counters(int ctas) { return (size_t)(ctas + 63) / 64 * 64; }
+// Units that lie in several shares, out of their parts.  CTA (c, y) takes rows of the unit that begins in share c and goes on in the next ones.  Few parts: a group of D / 4
+// lanes takes a row; many (few tokens over a long history): all groups take one row, every eighth (sixteenth) part each.
+constexpr int K8P_MERGE = 256, K8P_SLICES = 16, K8P_FEW_PARTS = 6;
+template <int D>
+__global__ void __launch_bounds__(K8P_MERGE)
+kv8_prefill_merge_kernel(const __grid_constant__ Kv8Prompt p) {
+    using C = K8Prefill<D>;
+    constexpr int LR = D / 4, GROUPS = K8P_MERGE / LR;
+    __shared__ float4 s_acc[GROUPS][LR];
+    __shared__ float2 s_ml[GROUPS];
+    pdl_wait();
+    const Kv8Split u = p.split[blockIdx.x];
+    if (u.parts == 0) return;
+    const bool few = u.tokens < 0;
+    const int n_tok = few ? -u.tokens : u.tokens, subs = few ? 2 : 1, np = u.parts * subs;
+    const int group = threadIdx.x / LR, d4 = threadIdx.x % LR * 4;
+    const bool alone = np <= K8P_FEW_PARTS;                          // a group has a row to itself
+    const int step = alone ? K8P_SLICES * GROUPS : K8P_SLICES;
+    for (int r = alone ? blockIdx.y * GROUPS + group : blockIdx.y; r < (few ? 1 : 2) * K8P_ROWS; r += step) {
+        const int row = r & 127, tok = row * p.inv_g >> 16, t = (r >> 7) * p.th + tok;
+        if (tok >= p.th || t >= n_tok) continue;                     // the same for all that take the row
+        float M = -INFINITY, L = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int first = alone ? 0 : group, stride = alone ? 1 : GROUPS;
+        for (int x0 = first; x0 < np; x0 += 4 * stride) {
+            float2 ml[4];
+            float4 o[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {                            // four parts asked for at once
+                const int x = min(x0 + k * stride, np - 1), cta = blockIdx.x + x / subs, rec_row = r + (x % subs) * K8P_ROWS;
+                const float* rec = p.parts + (2 * (size_t)cta + (x < subs)) * C::PART;
+                ml[k] = *reinterpret_cast<const float2*>(rec + (size_t)2 * K8P_ROWS * D + 2 * rec_row);
+                o[k] = *reinterpret_cast<const float4*>(rec + (size_t)rec_row * D + d4);
+                if (x0 + k * stride >= np) ml[k] = make_float2(-INFINITY, 0.f);
+            }
+            const float Mn = fmaxf(M, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)));
+            const float keep = M == -INFINITY ? 0.f : exp2f(M - Mn);
+            L *= keep; acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float z = ml[k].x == -INFINITY ? 0.f : exp2f(ml[k].x - Mn);
+                L = fmaf(ml[k].y, z, L);
+                acc = fma_f4(o[k], make_float4(z, z, z, z), acc);
+            }
+            M = Mn;
+        }
+        if (!alone) {
+            s_acc[group][threadIdx.x % LR] = acc;
+            if (d4 == 0) s_ml[group] = make_float2(M, L);
+            __syncthreads();
+            if (group == 0) {
+                float Mn = M;
+                for (int k = 1; k < GROUPS; ++k) Mn = fmaxf(Mn, s_ml[k].x);
+                float Ls = 0.f;
+                float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int k = 0; k < GROUPS; ++k) {
+                    const float z = s_ml[k].x == -INFINITY ? 0.f : exp2f(s_ml[k].x - Mn);
+                    Ls = fmaf(s_ml[k].y, z, Ls);
+                    a = fma_f4(s_acc[k][threadIdx.x], make_float4(z, z, z, z), a);
+                }
+                L = Ls;
+                acc = a;
+            }
+            __syncthreads();
+            if (group) continue;
+        }
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        const float y0 = acc.x * inv, y1 = acc.y * inv, y2 = acc.z * inv, y3 = acc.w * inv;
+        const uint32_t h0 = pack_bf16(y0, y1), h1 = pack_bf16(y2, y3);
+        const size_t to = ((size_t)(u.row0 + t) * p.nq + (size_t)u.head * p.G + (row - tok * p.G)) * D + d4;
+        *reinterpret_cast<uint2*>(p.out + to) = make_uint2(h0, h1);
+        if (p.out_lo)
+            *reinterpret_cast<uint2*>(p.out_lo + to) = make_uint2(pack_bf16(y0 - bf16_lo(h0), y1 - bf16_hi(h0)), pack_bf16(y2 - bf16_lo(h1), y3 - bf16_hi(h1)));
+    }
+}
 
 template <int D>
 static int launch_kv8_prefill(Kv8Prompt& p, void* scratch, cudaStream_t st) {
     using C = K8Prefill<D>;
-    static_assert(C::SMEM <= 232448 - 512 && (C::BARS + C::N_BARS * 8) % 16 == 0 && C::REC % 1024 == 0, "shared memory");
+    static_assert(C::SMEM <= 232448 - 3072 && (C::BARS + C::N_BARS * 8) % 16 == 0 && C::REC % 16 == 0, "shared memory");
     static PerDeviceFlag attr_set;
     if (!attr_set.done()) {
         FT_CHECK_CUDA(cudaFuncSetAttribute(kv8_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
         attr_set.mark();
     }
     const int ctas = device_sms();
-    p.counters = (int*)scratch;
-    p.parts = (float*)scratch + kv8_prefill_counters(ctas);
+    // parts only where a unit can be longer than a share by more than K8P_WHOLE, or there are more units than SMs
+    const bool parts = ((long long)p.T / (2 * p.th) + p.n_req) * p.nkv > ctas || p.max_pages > K8P_WHOLE;
+    FT_REQUIRE(!parts || scratch, "ft_attn_prefill_kv8: needs ft_attn_prefill_kv8_scratch_bytes of work memory");
+    p.split = parts ? (Kv8Split*)scratch : nullptr;
+    p.parts = (float*)scratch + kv8_prefill_splits(ctas);
     if (int r = kv8_waits_address(&p.err)) return r;
-    kv8_prefill_zero_kernel<<<1, 128, 0, st>>>(p.counters, ctas);
+    kv8_prefill_kernel<D><<<ctas, K8P_THREADS, C::SMEM, st>>>(p);
     FT_CHECK_CUDA(cudaGetLastError());
-    // starts beside the zeroes; what was in the stream before them is done by then
-    FT_CHECK_CUDA(launch_after(kv8_prefill_kernel<D>, dim3(ctas), dim3(K8P_THREADS), C::SMEM, st, (const Kv8Prompt&)p));
+    if (parts) FT_CHECK_CUDA(launch_after(kv8_prefill_merge_kernel<D>, dim3(ctas, K8P_SLICES), dim3(K8P_MERGE), 0, st, (const Kv8Prompt&)p));
     return 0;
 }
 
@@ -571,7 +630,7 @@ static int launch_kv8_prefill(Kv8Prompt& p, void* scratch, cudaStream_t st) {
 extern "C" long long ft_attn_prefill_kv8_scratch_bytes(int d) {
     FT_REQUIRE(d == 64 || d == 128, "ft_attn_prefill_kv8_scratch_bytes: head_dim %d not supported (64 or 128)", d);
     const int ctas = ft::device_sms();
-    return (long long)(ft::kv8_prefill_counters(ctas) + 2 * (size_t)ctas * (d == 64 ? ft::K8Prefill<64>::PART : ft::K8Prefill<128>::PART)) * 4;
+    return (long long)(ft::kv8_prefill_splits(ctas) + 2 * (size_t)ctas * (d == 64 ? ft::K8Prefill<64>::PART : ft::K8Prefill<128>::PART)) * 4;
 }
 
 extern "C" int ft_attn_prefill_kv8(const void* q, const void* kv8_layer, int num_pages, const int* page_table, int table_rows, int max_pages,
@@ -583,7 +642,7 @@ extern "C" int ft_attn_prefill_kv8(const void* q, const void* kv8_layer, int num
     FT_REQUIRE(T >= 0 && n_req >= 0 && table_rows >= 0 && max_pages >= 0 && num_pages >= 0 && (long long)max_pages * kKvTile + T <= INT32_MAX - 64,
                "ft_attn_prefill_kv8: bad sizes T=%d n_req=%d nkv=%d table %d x %d, %d pages", T, n_req, nkv, table_rows, max_pages, num_pages);
     if (T == 0) return 0;
-    FT_REQUIRE(q && kv8_layer && out && scratch && (n_req == 0 || (page_table && req_q_start && req_slot && req_pos0)), "ft_attn_prefill_kv8: null argument");
+    FT_REQUIRE(q && kv8_layer && out && (n_req == 0 || (page_table && req_q_start && req_slot && req_pos0)), "ft_attn_prefill_kv8: null argument");
     FT_REQUIRE(((uintptr_t)q | (uintptr_t)kv8_layer | (uintptr_t)out | (uintptr_t)out_lo | (uintptr_t)scratch) % 16 == 0, "ft_attn_prefill_kv8: tensors on 16 bytes");
     const int G = nq / nkv;
     Kv8Prompt p{(const __half*)q, (const uint8_t*)kv8_layer, page_table, req_q_start, req_slot, req_pos0, (__nv_bfloat16*)out, (__nv_bfloat16*)out_lo, nullptr, nullptr,

@@ -4,12 +4,15 @@
 
 namespace ft {
 
+// a unit that begins in a share and goes on in the next ones: how many, its first row of q, its key head, its tokens (below zero: few, whose halves are parts)
+struct Kv8Split { int parts, row0, head, tokens; };
+
 struct Kv8Prompt {
     const __half* q;
     const uint8_t* cache;
     const int *page_table, *req_q_start, *req_slot, *req_pos0;
     __nv_bfloat16 *out, *out_lo;
-    int* counters;
+    Kv8Split* split;
     float* parts;
     int* err;
     int num_pages, table_rows, max_pages, n_req, T, nq, nkv;

@@ -380,7 +380,8 @@ def attn_prefill_kv8(q: torch.Tensor, kv8_layer: torch.Tensor, page_table: torch
     dev, pages, nkv, T, nq, d, out, lo = _kv8_query(q, kv8_layer, planes, what)
     rows, most = _kv8_table(page_table, dev, what)
     req_q_start, req_slot, req_pos0, n = _kv8_requests(req_q_start, req_slot, req_pos0, dev, what)
-    scratch = torch.empty(_kv8_scratch_bytes(dev, "ft_attn_prefill_kv8_scratch_bytes", d), device=dev, dtype=torch.uint8)
+    size = _kv8_scratch_bytes(dev, "ft_attn_prefill_kv8_scratch_bytes", d)
+    scratch = torch.empty(size, device=dev, dtype=torch.uint8)
     _kv8_call(dev, "ft_attn_prefill_kv8", q.data_ptr(), kv8_layer.data_ptr(), pages, page_table.data_ptr(), rows, most, req_q_start.data_ptr(),
               req_slot.data_ptr(), req_pos0.data_ptr(), n, T, out.data_ptr(), N.ptr(lo), scratch.data_ptr(), nq, nkv, d)
     return out, lo
