@@ -3,16 +3,19 @@
 //
 // A unit of work is a tile of query tokens of one request and one key head: two halves of up to 128 rows (row = token * G + head of the group), so that every
 // record that reaches an SM serves both.  Per page and half, as in attention_tc.cu:  S = Q K^T (M128 N64 K=D, both operands in shared memory), one thread a row
-// for the softmax, P to tensor memory over the scores it came from, O += P V (A from tensor memory, M128 N=D K64).  A unit whose tokens fill one half only gives
-// both halves the same queries and every other page each.
+// for the softmax, P to tensor memory, O += P V (A from tensor memory, M128 N=D K64).  A unit whose tokens fill one half only gives both halves the same queries and
+// every other page each.
 //
-// The tensor cores want fp16, so four warps turn each record into the two operands, swizzled as the instructions read them: key codes as they are (the blocks' scales
+// The tensor cores want fp16, so eight warps turn each record into the two operands, swizzled as the instructions read them: key codes as they are (the blocks' scales
 // go to the scores, one multiplication per 16 of them for the maximum and the multiply-add's factor for the exponents), value codes times their block's scale relative
-// to the largest of the stretch of pages at hand, which the same warps look up ahead (vref; the output takes it back).  Both roundings are fp16's 2^-11 of a value.
+// to the largest of the stretch of pages at hand, which the same warps look up ahead (the output takes it back).  Both roundings are fp16's 2^-11 of a value.
 //
 // The flat list of all (request, key head, tile, page) is cut into equal shares, one for each SM: a causal list's units differ in length by any factor, and shares do
 // not.  A unit that lies in several shares is put together by a second kernel, in the parts' order.  Where there is an SM for every unit and none is much longer than
-// a share, each CTA takes a whole one.  Everything is found by each CTA from the lists on the device; nothing is planned ahead.
+// a share, each CTA takes a whole one.  One warp of each CTA finds its share from the lists on the device and tells the others stretch by stretch; nothing is planned
+// ahead of the kernel.
+//
+// What bounds it: a page's chain of hand-overs in each half (scores - exponentials - probabilities - products), TIMES_HERE.
 #include "common.cuh"
 #include "ft_internal.h"
 #include "kv8.cuh"
@@ -20,8 +23,13 @@
 
 namespace ft {
 
-constexpr int K8P_THREADS = 448;                 // warp 0 copies records, 1 issues products, 2 .. 9 softmax (half = (warp - 2) / 4), 10 .. 13 convert
-constexpr int K8P_SOFT = 256, K8P_CONV = 128;
+// Groups of four warps: warp 0 copies records, 1 and 2 issue the halves' products, 3 finds the work, 4 .. 11 softmax (half = (warp - 4) / 4), 12 .. 19 convert.  The
+// softmax threads hold a page's scores and take registers that the others give up: 64 + 2 x 144 + 2 x 64 = 5 x 96 a lane of the SM's quarter.
+constexpr int K8P_THREADS = 640;
+constexpr int K8P_REGS = 96, K8P_REGS_ISSUE = 64, K8P_REGS_SOFT = 144, K8P_REGS_CONV = 64;
+static_assert(K8P_REGS_ISSUE + 2 * K8P_REGS_SOFT + 2 * K8P_REGS_CONV <= 5 * K8P_REGS, "what the block is launched with");
+constexpr int K8P_SOFT = 256, K8P_CONV = 256;
+constexpr int K8P_LISTENERS = 19;                // warps that hear of a stretch: all but the one that tells
 constexpr int K8P_ROWS = 128;                    // rows of a half
 constexpr int K8P_GROUP = 8;                     // query heads a key head at most
 constexpr int K8P_PIECE = kKvTile * 128;         // [64 tokens][64 dims] in fp16; 64 rows of a Q block
@@ -34,14 +42,42 @@ struct K8Prefill {
     static constexpr int KH = D / 64;
     static constexpr int TILE = 2 * KH * K8P_PIECE;                  // K | V of a page in fp16
     static constexpr int S16 = D == 64 ? 6 : 3, S8 = D == 64 ? 6 : 3;
+    static constexpr int NS = D == 64 ? 2 : 1;                       // score buffers of a half
     static constexpr int QBLK = K8P_ROWS * 128;                      // [128 rows][64 dims]
     static constexpr int Q_BYTES = 2 * KH * QBLK;
-    static constexpr int KV = Q_BYTES, REC = KV + S16 * TILE, BARS = REC + S8 * Kv8<D>::REC;
-    static constexpr int N_BARS = 2 * S16 + 2 * S8 + 2 + 12 + 2;              // an even number: 16-byte words behind them
-    static constexpr int SMEM = 1024 + BARS + N_BARS * 8 + S16 * 16 + S8 * 4;
-    static constexpr int COL_S = 0, COL_O = 256, COLS = 512;
-    static constexpr size_t PART = (size_t)2 * K8P_ROWS * (D + 2);   // floats of a part: O [256][D], then (m, l) [256]
+    static constexpr int KV = Q_BYTES, REC = KV + S16 * TILE, SMEM = 1024 + REC + S8 * Kv8<D>::REC;
+    // tensor memory: scores [half][NS][64 columns], probabilities [half][2][32] (pairs of fp16), O [half][D]
+    static constexpr int COL_S = 0, COL_P = 2 * NS * 64, COL_O = COL_P + 128, COLS = 512;
+    static_assert(COL_O + 2 * D <= COLS, "tensor memory");
+    static constexpr size_t PART = (size_t)2 * K8P_ROWS * (D + 2);   // floats of a part: O [D / 4][256 rows][4], then (m, l) [256]
 };
+
+// two fp32 sums in one instruction, and the largest of three
+__device__ __forceinline__ f32x2 sum2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float max3(uint32_t a, uint32_t b, uint32_t c) { return max3(__uint_as_float(a), __uint_as_float(b), __uint_as_float(c)); }
+__device__ __forceinline__ float max3(float a, uint32_t b, uint32_t c) { return max3(a, __uint_as_float(b), __uint_as_float(c)); }
+
+// Registers that tcgen05.ld fills are there after the wait only, which the compiler cannot see from its operands: nothing that reads them moves ahead of this
+template <int N>
+__device__ __forceinline__ void tmem_arrived(uint32_t* r) {
+    tmem_ld_wait();
+#pragma unroll
+    for (int c = 0; c < N; c += 8)
+        asm volatile("" : "+r"(r[c]), "+r"(r[c + 1]), "+r"(r[c + 2]), "+r"(r[c + 3]), "+r"(r[c + 4]), "+r"(r[c + 5]), "+r"(r[c + 6]), "+r"(r[c + 7]));
+}
+// A warp's wait (all lanes ask, so that the warp stays together)
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
+    return __all_sync(0xffffffffu, mbar_wait_limited(bar, parity, dead));
+}
 
 // floats that the descriptions of split units take at the head of the work memory
 static size_t kv8_prefill_splits(int ctas) { return (size_t)(ctas + 15) / 16 * 16 * (sizeof(Kv8Split) / 4); }
@@ -53,33 +89,39 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
     constexpr int KH = C::KH;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem + C::BARS);         // [S16] a page's operands are there
-    uint64_t* kv_empty = kv_full + C::S16;
-    uint64_t* rec_full = kv_empty + C::S16;                                  // [S8] a record is there
-    uint64_t* rec_empty = rec_full + C::S8;
-    uint64_t* q_full = rec_empty + C::S8;
-    uint64_t* q_empty = q_full + 1;
-    uint64_t* s_full = q_empty + 1;                                          // [2][2] half, buffer: scores are in tensor memory
-    uint64_t* p_full = s_full + 4;                                           // [2][2] probabilities are
-    uint64_t* pv_done = p_full + 4;                                          // [2][2] O += P V retired
-    uint64_t* drained = pv_done + 4;                                         // all products retired (after a wait that ran out)
-    float* kscale_s = reinterpret_cast<float*>(kv_full + C::N_BARS);                 // [S16][4], times scale_log2; the first below 0: the page is not there
-    int* there_s = reinterpret_cast<int*>(kscale_s + 4 * C::S16);            // [S8]
+    __shared__ uint64_t rec_full[C::S8], rec_empty[C::S8];                   // a record is there
+    __shared__ uint64_t kv_full[C::S16], kv_empty[C::S16];                   // a page's operands are
+    __shared__ uint64_t q_full, q_empty;                                     // the queries of a stretch
+    __shared__ uint64_t s_full[2][C::NS], s_free[2];                         // half, buffer: scores are in tensor memory; (NS = 1) and in registers
+    __shared__ uint64_t p_full[2][2], pv_done[2][2];                         // probabilities are in tensor memory; O += P V retired
+    __shared__ uint64_t seg_full[4], seg_empty[4];                           // a stretch has been told; all have done with it
+    __shared__ uint64_t vmax_full;                                           // the largest scale of a stretch's values is known
+    __shared__ uint64_t halves_met;                                          // all softmax warps are here
+    __shared__ uint64_t drained[2];                                          // all products of a half retired (after a wait that ran out)
+    __shared__ Kv8Stretch told[4];
+    __shared__ unsigned vmax_s[4];                                           // bits of a number that is not negative: they order as it does
+    __shared__ __align__(16) float kscale_s[C::S16][4];                      // times scale_log2; the first below 0: the page is not there
+    __shared__ int there_s[C::S8];
+    __shared__ float2 ml_s[K8P_SOFT];
     __shared__ uint32_t tmem_slot;
-    __shared__ long long s_sum[K8P_THREADS / 32], s_units[K8P_THREADS / 32];
-    __shared__ int s_most[K8P_THREADS / 32], s_r, s_h, s_i, s_t;
-    __shared__ float2 s_ml[K8P_SOFT];
-    __shared__ float s_vref[4], s_vmax[K8P_CONV / 32];
     __shared__ volatile int dead;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    int* const err = p.err;
     if (tid == 0) {
-        for (int s = 0; s < C::S16; ++s) mbar_init(&kv_full[s], K8P_CONV / 32), mbar_init(&kv_empty[s], 1);
+        for (int s = 0; s < C::S16; ++s) mbar_init(&kv_full[s], K8P_CONV / 32), mbar_init(&kv_empty[s], 2);
         for (int s = 0; s < C::S8; ++s) mbar_init(&rec_full[s], 1), mbar_init(&rec_empty[s], K8P_CONV / 32);
-        mbar_init(q_full, K8P_CONV / 32);
-        mbar_init(q_empty, 1);
-        for (int k = 0; k < 4; ++k) mbar_init(&s_full[k], 1), mbar_init(&p_full[k], K8P_ROWS / 32), mbar_init(&pv_done[k], 1);
-        mbar_init(drained, 1);
+        for (int s = 0; s < 4; ++s) mbar_init(&seg_full[s], 1), mbar_init(&seg_empty[s], K8P_LISTENERS);
+        mbar_init(&q_full, K8P_CONV / 32);
+        mbar_init(&q_empty, 2);
+        mbar_init(&vmax_full, K8P_CONV / 32);
+        mbar_init(&halves_met, K8P_SOFT / 32);
+        for (int h = 0; h < 2; ++h) {
+            for (int s = 0; s < C::NS; ++s) mbar_init(&s_full[h][s], 1);
+            mbar_init(&s_free[h], K8P_ROWS / 32);
+            for (int s = 0; s < 2; ++s) mbar_init(&p_full[h][s], K8P_ROWS / 32), mbar_init(&pv_done[h][s], 1);
+            mbar_init(&drained[h], 1);
+        }
         fence_mbar_init();
         dead = 0;
     }
@@ -87,218 +129,242 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
         tmem_alloc(&tmem_slot, C::COLS);
         tmem_relinquish();
     }
-
-    // ---------------- the plan: this CTA's share
-    const int chunk = (p.n_req + K8P_THREADS - 1) / K8P_THREADS;
-    const int r0 = min(p.n_req, tid * chunk), r1 = min(p.n_req, r0 + chunk);
-    Kv8Walk w;
-    long long mine = 0, units = 0;
-    int most = 0;
-    for (int r = r0; r < r1; ++r) {
-        w.q.load(p, r);
-        mine += w.q.all(p);
-        units += w.q.tiles;
-        if (w.q.tiles) most = max(most, max(w.q.steps(p, w.q.tiles - 1), w.q.tiles > 1 ? w.q.steps(p, w.q.tiles - 2) : 0));
-    }
-    long long b_steps = mine, b_units = units;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, b_steps, o), y = __shfl_up_sync(0xffffffffu, b_units, o);
-        if (lane >= o) b_steps += x, b_units += y;
-    }
-    most = __reduce_max_sync(0xffffffffu, most);
-    if (lane == 31) s_sum[warp] = b_steps, s_units[warp] = b_units, s_most[warp] = most;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
-    b_steps -= mine;
-    b_units -= units;
-    long long total = 0, n_units = 0;
-    for (int k = 0; k < K8P_THREADS / 32; ++k) {
-        if (k < warp) b_steps += s_sum[k], b_units += s_units[k];
-        total += s_sum[k];
-        n_units += s_units[k];
-        most = max(most, s_most[k]);
-    }
-    total *= p.nkv;
-    n_units *= p.nkv;
-    const long long per = (total + gridDim.x - 1) / gridDim.x;
-    const bool whole = p.split == nullptr || (n_units <= gridDim.x && most <= per + K8P_WHOLE);      // no room for parts: the host knows that there are none
-    // the flat list is one of units or of steps
-    const long long len = whole ? n_units : total, each = whole ? 1 : per;
-    w.f = min(len, each * blockIdx.x);
-    w.f_end = min(len, w.f + each);
-    const bool work = w.f < w.f_end;
-    const long long at0 = whole ? b_units : b_steps;
-    if (work && at0 * p.nkv <= w.f && w.f < (at0 + (whole ? units : mine)) * p.nkv) {
-        w.seek(p, whole, r0, at0, w.f);
-        s_r = w.r; s_h = w.h; s_i = w.i; s_t = w.t;
-    }
-    __syncthreads();
-    if (work) {
-        w.r = s_r; w.h = s_h; w.i = s_i; w.t = s_t;
-        w.q.load(p, w.r);
-        w.unit(p);
-        if (whole) w.f = 0, w.f_end = w.n_steps;
-    }
     bool ok = true;                                                          // false: a wait ran out
-    int* const err = p.err;
+    // the n-th stretch of the share, or one without pages behind the last; and this warp's word that it has done with it
+    auto hear = [&](int n) {
+        ok = ok && warp_wait(&seg_full[n & 3], n >> 2 & 1, &dead);
+        Kv8Stretch w = told[n & 3];
+        if (!ok) w.pages = 0;
+        return w;
+    };
+    auto done = [&](int n) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&seg_empty[n & 3]);
+    };
 
-    if (warp == 0) {
+    // (the register counts change inside the branches, where the compiler sees what they are for)
+    if (warp < 4) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(K8P_REGS_ISSUE));
+      if (warp == 3) {
+        // ---------------- the plan: this CTA's share, stretch by stretch.  A lane adds up a run of requests
+        const int chunk = (p.n_req + 31) / 32;
+        const int r0 = min(p.n_req, lane * chunk), r1 = min(p.n_req, r0 + chunk);
+        Kv8Walk w;
+        long long mine = 0, units = 0;
+        int most = 0;
+        for (int r = r0; r < r1; ++r) {
+            w.q.load(p, r);
+            mine += w.q.all(p);
+            units += w.q.tiles;
+            if (w.q.tiles) most = max(most, max(w.q.steps(p, w.q.tiles - 1), w.q.tiles > 1 ? w.q.steps(p, w.q.tiles - 2) : 0));
+        }
+        long long b_steps = mine, b_units = units;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, b_steps, o), y = __shfl_up_sync(0xffffffffu, b_units, o);
+            if (lane >= o) b_steps += x, b_units += y;
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
+        const long long total = __shfl_sync(0xffffffffu, b_steps, 31) * p.nkv, n_units = __shfl_sync(0xffffffffu, b_units, 31) * p.nkv;
+        b_steps -= mine;
+        b_units -= units;
+        const long long per = (total + gridDim.x - 1) / gridDim.x;
+        const bool whole = p.split == nullptr || (n_units <= gridDim.x && most <= per + K8P_WHOLE);      // (no room for parts: the host knows that there are none)
+        // the flat list is one of units or of steps
+        const long long len = whole ? n_units : total, each = whole ? 1 : per, at0 = whole ? b_units : b_steps;
+        w.f = min(len, each * blockIdx.x);
+        w.f_end = min(len, w.f + each);
+        const bool work = w.f < w.f_end;
+        if (work ? at0 * p.nkv <= w.f && w.f < (at0 + (whole ? units : mine)) * p.nkv : lane == 0) {      // one lane
+            if (work) {
+                w.seek(p, whole, r0, at0, w.f);
+                w.unit(p);
+                if (whole) w.f = 0, w.f_end = w.n_steps;
+            }
+            for (int n = 0, more = 1; more; ++n) {
+                more = w.next(p);
+                if (!mbar_wait_limited(&seg_empty[n & 3], (n >> 2 & 1) ^ 1, &dead)) {
+                    *err = 1;
+                    break;
+                }
+                if (more) told[n & 3] = w.stretch(p, per, blockIdx.x);
+                else told[n & 3].pages = 0;
+                vmax_s[n & 3] = 0;
+                mbar_arrive(&seg_full[n & 3]);
+            }
+        }
+        __syncwarp();
+      } else if (warp == 0) {
         // ---------------- copies: one record a page
         const uint64_t pol = policy_evict_last();                            // read again by other tiles
         int it = 0, asked = 0;
-        while (w.next(p)) {
-            const int* pt = p.page_table + (size_t)w.q.slot * p.max_pages;
-            const int most_here = w.q.slot >= 0 && w.q.slot < p.table_rows ? p.max_pages : 0;
-            const int p1 = w.page1();
-            for (int p0 = w.page0(); p0 < p1; p0 += 32) {
-                const int mine_ = p0 + lane;
-                const int my_page = mine_ < p1 && mine_ < most_here ? pt[mine_] : -1;
+        bool go = true;
+        for (int seg = 0;; ++seg) {
+            const Kv8Stretch w = hear(seg);
+            if (w.pages == 0) break;
+            const int* pt = p.page_table + (size_t)w.slot * p.max_pages;
+            const int most_here = w.slot >= 0 && w.slot < p.table_rows ? p.max_pages : 0;
+            const int p1 = w.page0 + w.pages;
+            for (int p0 = w.page0; p0 < p1; p0 += 32) {
+                const int mine = p0 + lane;
+                const int my_page = mine < p1 && mine < most_here ? pt[mine] : -1;
                 const int n = min(32, p1 - p0);
                 for (int k = 0; k < n; ++k, ++it) {
                     const int page = __shfl_sync(0xffffffffu, my_page, k);
-                    if (lane == 0 && ok) {
+                    if (lane == 0 && go) {
                         const int s = it % C::S8;
-                        ok = mbar_wait_limited(&rec_empty[s], (it / C::S8 & 1) ^ 1, &dead);
-                        if (!ok) continue;
+                        go = mbar_wait_limited(&rec_empty[s], (it / C::S8 & 1) ^ 1, &dead);
+                        if (!go) continue;
                         asked = it + 1;
                         const bool there = page >= 0 && page < p.num_pages;
                         there_s[s] = there;
                         if (there) {
                             mbar_expect_tx(&rec_full[s], Kv8<D>::REC);
-                            tma_bulk_g2s(smem + C::REC + s * Kv8<D>::REC, p.cache + ((size_t)page * p.nkv + w.h) * Kv8<D>::REC, Kv8<D>::REC, &rec_full[s], pol);
+                            tma_bulk_g2s(smem + C::REC + s * Kv8<D>::REC, p.cache + ((size_t)page * p.nkv + w.head) * Kv8<D>::REC, Kv8<D>::REC, &rec_full[s], pol);
                         } else {
                             mbar_arrive(&rec_full[s]);
                         }
                     }
                 }
             }
+            done(seg);
         }
-        if (lane == 0 && (!ok || dead)) {                                    // what is under way still lands in this CTA's memory
+        if (lane == 0 && (!go || !ok || dead)) {                             // what is under way still lands in this CTA's memory
             *err = 1;
             for (int i = max(0, asked - C::S8); i < asked; ++i)
                 for (int k = 0; k < kWaitLimit && !mbar_try_wait(&rec_full[i % C::S8], i / C::S8 & 1); ++k) {}
         }
-    } else if (warp == 1) {
-        // ---------------- products
-        if (elect_one()) {
-            constexpr uint32_t idesc_qk = umma_idesc_f16(K8P_ROWS, kKvTile, false), idesc_pv = umma_idesc_f16(K8P_ROWS, D, true);
-            const uint32_t q_addr = smem_u32(smem), kv_addr = smem_u32(smem + C::KV);
-            int base = 0, seg = 0;                                           // pages so far; stretches so far
-            int n_qk[2] = {0, 0}, n_pv[2] = {0, 0};                          // products of each half so far
-            auto issue_qk = [&](int h, int page, int qh) {                   // page: counted over the whole share
-                const int s = page % C::S16;
-                ok = ok && mbar_wait_limited(&kv_full[s], page / C::S16 & 1, &dead);
-                if (!ok) return;
+      } else {
+        // ---------------- products, one warp a half
+        constexpr uint32_t idesc_qk = umma_idesc_f16(K8P_ROWS, kKvTile, false), idesc_pv = umma_idesc_f16(K8P_ROWS, D, true);
+        const int h = warp - 1;
+        const bool lead = elect_one();
+        // operands' descriptors differ in their addresses alone, in units of 16 bytes
+        const uint64_t q_desc = umma_desc_k128(smem_u32(smem)), k_desc = umma_desc_k128(smem_u32(smem + C::KV)), v_desc = umma_desc_mn128(smem_u32(smem + C::KV) + KH * K8P_PIECE);
+        const uint32_t s_at = tmem + C::COL_S + h * C::NS * 64, p_at = tmem + C::COL_P + h * 64, o_at = tmem + C::COL_O + h * D;
+        int base = 0, n_qk = 0, n_pv = 0;                                    // pages of the share, products of this half so far
+        auto issue_qk = [&](int page, int qh) {                              // page: counted over the whole share
+            const int s = page % C::S16, buf = n_qk % C::NS;
+            if (C::NS == 1) ok = mbar_wait_limited(&s_free[h], (n_qk & 1) ^ 1, &dead);
+            ok = ok && mbar_wait_limited(&kv_full[s], page / C::S16 & 1, &dead);
+            if (!ok) return;
+            ++n_qk;
+            tc_fence_after();
+            const uint64_t a = q_desc + (uint64_t)(qh * KH * (C::QBLK >> 4)), b = k_desc + (uint64_t)(s * (C::TILE >> 4));
+#pragma unroll
+            for (int kh = 0; kh < KH; ++kh)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) umma_bf16(s_at + buf * 64, a + kh * (C::QBLK >> 4) + 2 * k, b + kh * (K8P_PIECE >> 4) + 2 * k, idesc_qk, (kh | k) != 0);
+            umma_commit(&s_full[h][buf]);
+        };
+        auto issue_pv = [&](int page, bool first, bool alone) {
+            const int s = page % C::S16, buf = n_pv & 1;
+            ok = mbar_wait_limited(&p_full[h][buf], n_pv >> 1 & 1, &dead);
+            if (!ok) return;
+            ++n_pv;
+            tc_fence_after();
+            const uint64_t b = v_desc + (uint64_t)(s * (C::TILE >> 4));
+#pragma unroll
+            for (int k = 0; k < kKvTile / 16; ++k) umma_f16_ts(o_at, p_at + buf * 32 + 8 * k, b + k * (2048 >> 4), idesc_pv, k != 0 || !first);
+            umma_commit(&pv_done[h][buf]);
+            umma_commit(&kv_empty[s]);
+            if (alone) umma_commit(&kv_empty[s]);                            // the other half has no use for this page
+        };
+        for (int seg = 0;; ++seg) {
+            const Kv8Stretch w = hear(seg);
+            if (w.pages == 0) break;
+            const int mine_n = w.few ? (w.pages - h + 1) / 2 : w.pages;      // page i of this half is page j of the stretch
+            auto page_of = [&](int i) { return base + (w.few ? h + 2 * i : i); };
+            if (lead) {
+                ok = mbar_wait_limited(&q_full, seg & 1, &dead);
                 tc_fence_after();
-                const int buf = n_qk[h]++ & 1;
-#pragma unroll
-                for (int kh = 0; kh < KH; ++kh) {
-                    const uint64_t a = umma_desc_k128(q_addr + (qh * KH + kh) * C::QBLK), b = umma_desc_k128(kv_addr + s * C::TILE + kh * K8P_PIECE);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) umma_bf16(tmem + C::COL_S + (2 * h + buf) * 64, a + 2 * k, b + 2 * k, idesc_qk, (kh | k) != 0);
+                if (ok && mine_n == 0) umma_commit(&q_empty);
+                // Scores run NS pages ahead.  With two buffers page i + 2's follow the product that reads page i's probabilities, which says that page i's scores
+                // have been read; with one, page i + 1's follow the softmax's word that it has them in registers, ahead of that product.  Either way scores that are
+                // there mean that the product before the last is done, and the probabilities' buffer with it.
+                for (int i = -C::NS; ok && i < mine_n; ++i) {
+                    if (C::NS == 2 && i >= 0) issue_pv(page_of(i), i == 0, w.few);
+                    if (ok && i + C::NS < mine_n) issue_qk(page_of(i + C::NS), w.few ? 0 : h);
+                    if (i + C::NS == mine_n - 1) umma_commit(&q_empty);
+                    if (C::NS == 1 && ok && i >= 0) issue_pv(page_of(i), i == 0, w.few);
                 }
-                umma_commit(&s_full[2 * h + buf]);
-            };
-            auto issue_pv = [&](int h, int page, bool first, bool last) {
-                const int s = page % C::S16, buf = n_pv[h] & 1;
-                ok = ok && mbar_wait_limited(&p_full[2 * h + buf], n_pv[h] >> 1 & 1, &dead);
-                if (!ok) return;
-                ++n_pv[h];
-                tc_fence_after();
-#pragma unroll
-                for (int k = 0; k < kKvTile / 16; ++k)
-                    umma_f16_ts(tmem + C::COL_O + h * D, tmem + C::COL_S + (2 * h + buf) * 64 + 8 * k,
-                                umma_desc_mn128(kv_addr + s * C::TILE + KH * K8P_PIECE + k * 2048), idesc_pv, k != 0 || !first);
-                umma_commit(&pv_done[2 * h + buf]);
-                if (last) umma_commit(&kv_empty[s]);
-            };
-            while (ok && w.next(p)) {
-                ok = mbar_wait_limited(q_full, seg & 1, &dead);
-                if (!ok) break;
-                tc_fence_after();
-                const int n = w.page1() - w.page0();
-                if (w.few) {
-                    // page j is half (j & 1)'s; scores run two pages ahead
-                    for (int j = -2; ok && j < n; ++j) {
-                        if (j >= 0) issue_pv(j & 1, base + j, j < 2, true);
-                        if (j + 2 < n) issue_qk(j & 1, base + j + 2, 0);
-                        if (j + 2 == n - 1) umma_commit(q_empty);
-                    }
-                } else {
-                    for (int j = -2; ok && j < n; ++j)
-                        for (int h = 0; h < 2; ++h) {
-                            if (j >= 0) issue_pv(h, base + j, j == 0, h == 1);
-                            if (j + 2 < n) issue_qk(h, base + j + 2, h);
-                            if (j + 2 == n - 1 && h == 1) umma_commit(q_empty);
-                        }
-                }
-                base += n;
-                ++seg;
             }
-            if (!ok) {                                                       // nothing may still run in tensor memory when it is given back
-                *err = 1;
-                umma_commit(drained);
-                for (int k = 0; k < kWaitLimit && !mbar_try_wait(drained, 0); ++k) {}
-            }
+            base += w.pages;
+            ok = __all_sync(0xffffffffu, ok);
+            done(seg);
+        }
+        if (!ok && lead) {                                                   // nothing may still run in tensor memory when it is given back
+            *err = 1;
+            umma_commit(&drained[h]);
+            for (int k = 0; k < kWaitLimit && !mbar_try_wait(&drained[h], 0); ++k) {}
         }
         __syncwarp();
-    } else if (warp >= 2 + K8P_SOFT / 32) {
+      }
+    } else if (warp >= 12) {
         // ---------------- conversion: Q of each stretch, then its pages
-        const int ct = tid - 64 - K8P_SOFT, cw = ct >> 5;
-        int it = 0, seg = 0;
-        while (w.next(p)) {                                                  // after a wait that ran out: only the barriers that the four warps share
-            const int g0 = w.page0(), g1 = w.page1();
-            // the largest scale of the stretch's values: its pages are asked for first, the answers are used after Q
-            const int* pt = p.page_table + (size_t)w.q.slot * p.max_pages;
-            const int most_here = w.q.slot >= 0 && w.q.slot < p.table_rows ? min(g1, p.max_pages) : 0;
-            float vmax = 0.f;
-            for (int k = g0 + ct; k < most_here; k += K8P_CONV) {
-                const int page = pt[k];
-                if (page < 0 || page >= p.num_pages) continue;
-                const float4 v = *reinterpret_cast<const float4*>(p.cache + ((size_t)page * p.nkv + w.h) * Kv8<D>::REC + Kv8<D>::SCALES + 16);
-                vmax = fmaxf(vmax, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(K8P_REGS_CONV));
+        const int ct = tid - 128 - K8P_SOFT;
+        int it = 0;
+        for (int seg = 0;; ++seg) {
+            const Kv8Stretch w = hear(seg);
+            if (w.pages == 0) break;
+            for (int step = 0; step < 2; ++step) {
+                if ((step == 0) == (seg == 0)) {
+                    // the queries, 16 bytes at a time and all on their way at once; zeros for rows without a token
+                    if (seg) ok = warp_wait(&q_empty, (seg - 1) & 1, &dead);
+                    if (!ok) break;
+                    constexpr int CH = D / 8;
+#pragma unroll 4
+                    for (int k = ct; k < (w.few ? 1 : 2) * K8P_ROWS * CH; k += K8P_CONV) {
+                        const int c = k % CH, rr = k / CH, h = rr >> 7, row = rr & 127;
+                        const int tok = row * p.inv_g >> 16, head = row - tok * p.G;
+                        const bool on = tok < p.th && h * p.th + tok < w.tokens;
+                        const __half* from = p.q + ((size_t)(w.row0 + (on ? h * p.th + tok : 0)) * p.nq + (size_t)w.head * p.G + (on ? head : 0)) * D + c * 8;
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem + (h * KH + (c >> 3)) * C::QBLK + row * 128 + ((c & 7) ^ (row & 7)) * 16)),
+                                     "l"(from), "r"(on ? 16 : 0)
+                                     : "memory");
+                    }
+                } else {
+                    // the largest scale of the stretch's values
+                    const int* pt = p.page_table + (size_t)w.slot * p.max_pages;
+                    const int end = w.slot >= 0 && w.slot < p.table_rows ? min(w.page0 + w.pages, p.max_pages) : 0;
+                    float vmax = 0.f;
+                    for (int k = w.page0 + ct; k < end; k += K8P_CONV) {
+                        const int page = pt[k];
+                        if (page < 0 || page >= p.num_pages) continue;
+                        const float4 v = *reinterpret_cast<const float4*>(p.cache + ((size_t)page * p.nkv + w.head) * Kv8<D>::REC + Kv8<D>::SCALES + 16);
+                        vmax = fmaxf(vmax, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+                    }
+                    vmax = warp_max(vmax);
+                    if (lane == 0) {
+                        atomicMax(&vmax_s[seg & 3], __float_as_uint(vmax));
+                        mbar_arrive(&vmax_full);
+                    }
+                }
             }
-            if (seg) ok = ok && mbar_wait_limited(q_empty, (seg - 1) & 1, &dead);
-            ok = __all_sync(0xffffffffu, ok);
-            const int halves = !ok ? 0 : w.few ? 1 : 2, row0 = w.row0(p);
-            constexpr int CH = D / 8;
-#pragma unroll 8
-            for (int k = ct; k < halves * K8P_ROWS * CH; k += K8P_CONV) {    // 16 bytes each, all on their way at once; zeros for rows without a token
-                const int c = k % CH, rr = k / CH, h = rr >> 7, row = rr & 127;
-                const int tok = row * p.inv_g >> 16, head = row - tok * p.G;
-                const bool on = tok < p.th && h * p.th + tok < w.n_tok;
-                const __half* from = p.q + ((size_t)(row0 + (on ? h * p.th + tok : 0)) * p.nq + (size_t)w.h * p.G + (on ? head : 0)) * D + c * 8;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem + (h * KH + (c >> 3)) * C::QBLK + row * 128 + ((c & 7) ^ (row & 7)) * 16)),
-                             "l"(from), "r"(on ? 16 : 0)
-                             : "memory");
+            if (ok) {
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full);
+                ok = warp_wait(&vmax_full, seg & 1, &dead);
             }
-            vmax = warp_max(vmax);
-            if (lane == 0) s_vmax[cw] = vmax;
-            asm volatile("bar.sync 2, %0;" ::"n"(K8P_CONV) : "memory");
-            vmax = fmaxf(fmaxf(s_vmax[0], s_vmax[1]), fmaxf(s_vmax[2], s_vmax[3]));
-            asm volatile("bar.sync 2, %0;" ::"n"(K8P_CONV) : "memory");
-            if (ct == 0) s_vref[seg & 3] = vmax;                             // the softmax warps may still be at the end of the stretch before the last
-            const float vinv = vmax > 0.f ? 1.f / vmax : 0.f;
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0 && ok) mbar_arrive(q_full);
-            ++seg;
-            for (int k = g0; ok && k < g1; ++k, ++it) {
+            const float vmax = __uint_as_float(vmax_s[seg & 3]), vinv = vmax > 0.f ? 1.f / vmax : 0.f;
+            for (int k = 0; ok && k < w.pages; ++k, ++it) {
                 const int s8 = it % C::S8, s16 = it % C::S16;
-                ok = mbar_wait_limited(&rec_full[s8], it / C::S8 & 1, &dead) && mbar_wait_limited(&kv_empty[s16], (it / C::S16 & 1) ^ 1, &dead);
-                ok = __all_sync(0xffffffffu, ok);
+                ok = warp_wait(&rec_full[s8], it / C::S8 & 1, &dead) && warp_wait(&kv_empty[s16], (it / C::S16 & 1) ^ 1, &dead);
                 if (!ok) break;
                 const uint8_t* rec = smem + C::REC + s8 * Kv8<D>::REC;
                 uint8_t* dst = smem + C::KV + s16 * C::TILE;
                 const bool there = there_s[s8];
                 const float* scales = reinterpret_cast<const float*>(rec + Kv8<D>::SCALES);
                 // a block of zeros keeps a factor above 0, so that hidden scores stay minus infinity
-                if (ct < 4) kscale_s[4 * s16 + ct] = there ? fmaxf(scales[ct] * p.scale_log2, 1e-37f) : -1.f;
-#pragma unroll 4
+                if (ct < 4) kscale_s[s16][ct] = there ? fmaxf(scales[ct] * p.scale_log2, 1e-37f) : -1.f;
+#pragma unroll
                 for (int u = ct; u < kKvTile * D / 16; u += K8P_CONV) {      // keys: 16 codes, two chunks of the swizzled row
                     const int piece = u >> 8, t = u >> 2 & 63, c = u & 3;
                     uint4 x = *reinterpret_cast<const uint4*>(rec + u * 16);
@@ -308,7 +374,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                     *reinterpret_cast<uint4*>(at + ((2 * c + 1) ^ (t & 7)) * 16) = make_uint4(kv8_lo(x.z), kv8_hi(x.z), kv8_lo(x.w), kv8_hi(x.w));
                 }
                 dst += KH * K8P_PIECE;
-#pragma unroll 4
+#pragma unroll
                 for (int u = ct; u < kKvTile * D / 16; u += K8P_CONV) {      // values, by where they lie
                     const int piece = u >> 8, slot = u >> 2 & 63, t = slot ^ (slot >> 1 & 1), c = (u & 3) ^ (t >> 1 & 2);
                     uint4 x = *reinterpret_cast<const uint4*>(rec + Kv8<D>::SLAB + u * 16);
@@ -326,14 +392,17 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&kv_full[s16]), mbar_arrive(&rec_empty[s8]);
             }
+            done(seg);
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
         // ---------------- softmax: one thread a row
-        const int st = tid - 64, h = (warp - 2) >> 2, quarter = warp & 3;
-        const int row = quarter * 32 + lane;                                 // lane of tensor memory
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(K8P_REGS_SOFT));
+        const int st = tid - 128, h = (warp - 4) >> 2;
+        const int row = st & 127;                                            // lane of tensor memory: warp % 4 is the quarter that a warp may read
         const int tok = row * p.inv_g >> 16, head = row - tok * p.G;
-        const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-        const uint32_t s_at = lanes + C::COL_S + 2 * h * 64, o_at = lanes + C::COL_O + h * D;
+        const uint32_t lanes = tmem + ((uint32_t)(row & 96) << 16);
+        const uint32_t s_at = lanes + C::COL_S + h * C::NS * 64, p_at = lanes + C::COL_P + h * 64, o_at = lanes + C::COL_O + h * D;
         if (st == 0 && p.split) p.split[blockIdx.x].parts = 0;
         // rows that no request owns
         {
@@ -347,48 +416,85 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                 }
             }
         }
-        int base = 0, seg = 0, cnt = 0;                                      // pages and stretches of the share, pages of this half so far
-        while (w.next(p)) {
-            const int g0 = w.page0(), n = w.page1() - g0;
-            const int mine_n = w.few ? (n - h + 1) / 2 : n;                  // pages of this half
+        // the largest of a page's scores, in log2 units
+        auto largest = [](const uint32_t* sr, const float* ks) {
+            float most = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const uint32_t* x = sr + 16 * b;
+                float t0 = max3(x[0], x[1], x[2]), t1 = max3(x[3], x[4], x[5]);
+                t0 = max3(t0, x[6], x[7]), t1 = max3(t1, x[8], x[9]);
+                t0 = max3(t0, x[10], x[11]), t1 = max3(t1, x[12], x[13]);
+                t0 = max3(t0, x[14], x[15]);
+                most = fmaxf(most, fmaxf(t0, t1) * ks[b]);
+            }
+            return most;
+        };
+        int base = 0, cnt = 0, met = 0;                                      // pages of the share, pages of this half so far; meetings of the halves
+        for (int seg = 0;; ++seg) {
+            const Kv8Stretch w = hear(seg);
+            if (w.pages == 0) break;
+            const int mine_n = w.few ? (w.pages - h + 1) / 2 : w.pages;      // pages of this half
             const int my_tok = w.few ? tok : h * p.th + tok;
-            const bool valid = tok < p.th && my_tok < w.n_tok;
-            const int pos = w.position0(p) + my_tok;
+            const bool valid = tok < p.th && my_tok < w.tokens;
             float m_ref = -INFINITY, l_run = 0.f;                            // in log2 units
+            int it = base + (w.few ? h : 0), ahead = w.pos0 + my_tok - (w.page0 + (w.few ? h : 0)) * kKvTile;     // page of the share; the row's position from the page's first key on
             for (int i = 0; i < mine_n; ++i, ++cnt) {
-                const int j = w.few ? h + 2 * i : i;                         // page of the stretch
-                const int buf = cnt & 1, ph = cnt >> 1 & 1, it = base + j, s16 = it % C::S16;
-                ok = ok && mbar_wait_limited(&s_full[2 * h + buf], ph, &dead) && mbar_wait_limited(&kv_full[s16], it / C::S16 & 1, &dead);
-                ok = __all_sync(0xffffffffu, ok);
+                const int sb = cnt % C::NS, pb = cnt & 1;
+                ok = ok && warp_wait(&s_full[h][sb], cnt / C::NS & 1, &dead);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t at = s_at + buf * 64;
                 uint32_t sr[64];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld16_nowait(at + 16 * c, sr + 16 * c);
-                const float4 ks4 = *reinterpret_cast<const float4*>(kscale_s + 4 * s16);
-                const float ks[4] = {ks4.x, ks4.y, ks4.z, ks4.w};
-                tmem_ld_wait();
-                const int seen = ks4.x < 0.f ? -1 : pos - (g0 + j) * kKvTile;         // the last key of the page that the row sees
+                for (int c = 0; c < 4; ++c) tmem_ld16_nowait(s_at + sb * 64 + 16 * c, sr + 16 * c);
+                // (the page's scales are visible: they were written ahead of the operands that the product behind this barrier read)
+                const float4 k4 = *reinterpret_cast<const float4*>(kscale_s[it % C::S16]);
+                const float ks[4] = {fabsf(k4.x), fabsf(k4.y), fabsf(k4.z), fabsf(k4.w)};
+                tmem_arrived<64>(sr);
+                if constexpr (C::NS == 1) {                                  // the scores are in registers: the next ones may be formed
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&s_free[h]);
+                }
+                const int seen = k4.x < 0.f ? -1 : ahead;                    // the last key of the page that the row sees
+                it += w.few ? 2 : 1;
+                ahead -= w.few ? 2 * kKvTile : kKvTile;
                 if (seen < kKvTile - 1) {
 #pragma unroll
                     for (int c = 0; c < 64; ++c) sr[c] = c <= seen ? sr[c] : 0xff800000u;
                 }
-                float tmax = -INFINITY;
+                const uint32_t at = p_at + pb * 32;
+                // The exponentials are taken with the maximum of the pages before while this page's is found; where it has grown by too much they are taken again.
+                // (The stretch's first page has nothing before it.)
+                bool known = i == 0;
+                if (known) m_ref = largest(sr, ks);
+                f32x2 sum[2];
+                for (;;) {
+                    const float mu = m_ref == -INFINITY ? 0.f : m_ref;
+                    const f32x2 minus = pack2(-mu, -mu);
+                    sum[0] = sum[1] = 0;                                     // pairs of fp32 zeros
 #pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    float t2[2] = {-INFINITY, -INFINITY};
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t pk[16];
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) t2[c & 1] = fmaxf(t2[c & 1], __uint_as_float(sr[16 * b + c]));
-                    tmax = fmaxf(tmax, fmaxf(t2[0], t2[1]) * fabsf(ks[b]));
-                }
-                const float m_new = fmaxf(m_ref, tmax);
-                const bool grow = valid && m_new > m_ref + K8P_GROW;
-                if (i == 0) {
-                    m_ref = m_new;
-                } else if (__any_sync(0xffffffffu, grow)) {
-                    ok = mbar_wait_limited(&pv_done[2 * h + ((cnt - 1) & 1)], (cnt - 1) >> 1 & 1, &dead);
-                    ok = __all_sync(0xffffffffu, ok);
+                        for (int e = 0; e < 16; ++e) {
+                            const int c = half * 32 + 2 * e;
+                            const float f = ks[c >> 4];
+                            float p0, p1;
+                            unpack2(fma2(pack2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), pack2(f, f), minus), p0, p1);
+                            p0 = ex2_fast(p0), p1 = ex2_fast(p1);
+                            sum[e & 1] = sum2(sum[e & 1], pack2(p0, p1));
+                            const __half2 t = __floats2half2_rn(p0, p1);
+                            pk[e] = *reinterpret_cast<const uint32_t*>(&t);
+                        }
+                        tmem_st16(at + 16 * half, pk);
+                    }
+                    if (known) break;
+                    const float m_new = fmaxf(m_ref, largest(sr, ks));
+                    // rows without a token say nothing: a row's rounding depends on its own request alone
+                    if (!__any_sync(0xffffffffu, valid && m_new > m_ref + K8P_GROW)) break;
+                    known = true;
+                    ok = warp_wait(&pv_done[h][pb ^ 1], (cnt - 1) >> 1 & 1, &dead);
                     if (!ok) break;
                     tc_fence_after();
                     const float alpha = m_new == -INFINITY ? 1.f : exp2f(m_ref - m_new);
@@ -398,39 +504,28 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                     for (int c = 0; c < D / 16; ++c) {
                         uint32_t o[16];
                         tmem_ld16_nowait(o_at + 16 * c, o);
-                        tmem_ld_wait();
+                        tmem_arrived<16>(o);
 #pragma unroll
                         for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
                         tmem_st16(o_at + 16 * c, o);
                     }
-                    tmem_st_wait();
                 }
-                const float mu = m_ref == -INFINITY ? 0.f : m_ref;
-                float ps[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c16 = 0; c16 < 2; ++c16) {
-                    uint32_t pk[16];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float f = fabsf(ks[2 * c16 + (e >> 3)]);
-                        const float p0 = ex2_fast(fmaf(__uint_as_float(sr[c16 * 32 + 2 * e]), f, -mu));
-                        const float p1 = ex2_fast(fmaf(__uint_as_float(sr[c16 * 32 + 2 * e + 1]), f, -mu));
-                        ps[(2 * e) & 3] += p0;
-                        ps[(2 * e + 1) & 3] += p1;
-                        const __half2 t = __floats2half2_rn(p0, p1);
-                        pk[e] = *reinterpret_cast<const uint32_t*>(&t);
-                    }
-                    tmem_st16(at + 16 * c16, pk);
-                }
+                if (!ok) break;
                 tmem_st_wait();
-                l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+                float a0, a1;
+                unpack2(sum2(sum[0], sum[1]), a0, a1);
+                l_run += a0 + a1;
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[2 * h + buf]);
+                if (lane == 0) mbar_arrive(&p_full[h][pb]);
             }
-            if (ok && mine_n) {
-                ok = mbar_wait_limited(&pv_done[2 * h + ((cnt - 1) & 1)], (cnt - 1) >> 1 & 1, &dead);
-                ok = __all_sync(0xffffffffu, ok);
+            if (ok && mine_n) ok = warp_wait(&pv_done[h][(cnt - 1) & 1], (cnt - 1) >> 1 & 1, &dead);
+            if (w.few && w.parts == 0) {                                     // the halves' maxima and sums; and a half without a page has waited for nothing yet
+                ml_s[st] = make_float2(m_ref, l_run);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&halves_met);
+                ok = ok && warp_wait(&halves_met, met++ & 1, &dead);
             }
             tc_fence_after();
             if (!ok) {                                                       // NaN for all that this unit says
@@ -438,85 +533,78 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                 l_run = NAN;
                 m_ref = 0.f;
             }
-            float vref = ok && mine_n ? s_vref[seg & 3] : 0.f;
-            const bool all = w.t0 == 0 && w.t1 == w.n_steps;
-            const size_t off = ((size_t)(w.row0(p) + my_tok) * p.nq + (size_t)w.h * p.G + head) * D;
-            auto put = [&](int c, const uint32_t* o) {                       // 16 dims of the row
-                uint32_t hi[8], lo[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const float x = __uint_as_float(o[2 * k]), y = __uint_as_float(o[2 * k + 1]);
-                    hi[k] = pack_bf16(x, y);
-                    lo[k] = pack_bf16(x - bf16_lo(hi[k]), y - bf16_hi(hi[k]));
+            const float vref = ok ? __uint_as_float(*(volatile unsigned*)&vmax_s[seg & 3]) : 0.f;
+            if (w.parts == 0) {
+                float inv = l_run == 0.f ? 0.f : vref / l_run, z = 1.f, zo = 0.f;        // a query without a visible key: zeros
+                if (w.few && ok) {
+                    const float2 other = ml_s[st ^ K8P_ROWS];
+                    const float m = fmaxf(m_ref, other.x);
+                    z = m_ref == -INFINITY ? 0.f : exp2f(m_ref - m), zo = other.x == -INFINITY ? 0.f : exp2f(other.x - m);
+                    const float L = h == 0 ? l_run * z + other.y * zo : other.y * zo + l_run * z;
+                    inv = L == 0.f ? 0.f : vref / L;
                 }
-                uint4* to = reinterpret_cast<uint4*>(p.out + off + 16 * c);
-                to[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                to[1] = make_uint4(hi[4], hi[5], hi[6], hi[7]);
-                if (p.out_lo) {
-                    to = reinterpret_cast<uint4*>(p.out_lo + off + 16 * c);
-                    to[0] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                    to[1] = make_uint4(lo[4], lo[5], lo[6], lo[7]);
-                }
-            };
-            if (all && !w.few) {
-                const float inv = l_run == 0.f ? 0.f : vref / l_run;         // a query without a visible key: zeros
+                const size_t off = ((size_t)(w.row0 + my_tok) * p.nq + (size_t)w.head * p.G + head) * D;
+                const int c0 = w.few ? h * (D / 32) : 0, c1 = w.few ? c0 + D / 32 : D / 16;      // few: each half of the warps puts half of the dims together
 #pragma unroll 1
-                for (int c = 0; c < D / 16; ++c) {
-                    uint32_t o[16];
+                for (int c = c0; c < c1; ++c) {
+                    uint32_t o[16], hi[8], lo[8];
                     tmem_ld16_nowait(o_at + 16 * c, o);
-                    tmem_ld_wait();
+                    tmem_arrived<16>(o);
+                    if (w.few) {                                             // a half without a page has nothing in tensor memory
+                        uint32_t x[16];
+                        tmem_ld16_nowait(lanes + C::COL_O + (1 - h) * D + 16 * c, x);
+                        tmem_arrived<16>(x);
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * inv);
-                    if (valid) put(c, o);
-                }
-            } else if (all) {
-                // two halves of the pages: each half of the warps puts half of the dims together
-                s_ml[st] = make_float2(m_ref, l_run);
-                tc_fence_before();
-                asm volatile("bar.sync 1, %0;" ::"n"(K8P_SOFT) : "memory");
-                tc_fence_after();
-                if (ok) vref = s_vref[seg & 3];                              // a half without a page has waited for nothing before
-                const float2 other = s_ml[st ^ K8P_ROWS];
-                const float m = fmaxf(m_ref, other.x);
-                const float z = m_ref == -INFINITY ? 0.f : exp2f(m_ref - m), zo = other.x == -INFINITY ? 0.f : exp2f(other.x - m);
-                const float L = h == 0 ? l_run * z + other.y * zo : other.y * zo + l_run * z;
-                const float inv = L == 0.f ? 0.f : vref / L;
-#pragma unroll 1
-                for (int c = h * (D / 32); c < (h + 1) * (D / 32); ++c) {
-                    uint32_t o[16], x[16];
-                    tmem_ld16_nowait(o_at + 16 * c, o);
-                    tmem_ld16_nowait(lanes + C::COL_O + (1 - h) * D + 16 * c, x);
-                    tmem_ld_wait();
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) {                           // a half without a page has nothing in tensor memory
-                        const float u = z == 0.f ? 0.f : __uint_as_float(o[k]) * z, v = zo == 0.f ? 0.f : __uint_as_float(x[k]) * zo;
-                        o[k] = __float_as_uint((h == 0 ? u + v : v + u) * inv);
+                        for (int k = 0; k < 16; ++k) {
+                            const float u = z == 0.f ? 0.f : __uint_as_float(o[k]) * z, v = zo == 0.f ? 0.f : __uint_as_float(x[k]) * zo;
+                            o[k] = __float_as_uint(h == 0 ? u + v : v + u);
+                        }
                     }
-                    if (valid) put(c, o);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const float x = __uint_as_float(o[2 * k]) * inv, y = __uint_as_float(o[2 * k + 1]) * inv;
+                        hi[k] = pack_bf16(x, y);
+                        lo[k] = pack_bf16(x - bf16_lo(hi[k]), y - bf16_hi(hi[k]));
+                    }
+                    if (valid) {
+                        uint4* to = reinterpret_cast<uint4*>(p.out + off + 16 * c);
+                        to[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        to[1] = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+                        if (p.out_lo) {
+                            to = reinterpret_cast<uint4*>(p.out_lo + off + 16 * c);
+                            to[0] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                            to[1] = make_uint4(lo[4], lo[5], lo[6], lo[7]);
+                        }
+                    }
                 }
-                asm volatile("bar.sync 1, %0;" ::"n"(K8P_SOFT) : "memory");
+                if (w.few) {                                                 // the other half has read what the next products write over
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&halves_met);
+                    ok = ok && warp_wait(&halves_met, met++ & 1, &dead);
+                }
             } else {
-                // a part: O in its own size, maximum and sum of each row; the halves of a unit of few tokens are two parts
-                float* part = p.parts + (2 * (size_t)blockIdx.x + (w.t0 == 0)) * C::PART;
-                const int rr = h * K8P_ROWS + row;                           // (not st: a warp's rows are those lanes of tensor memory that it may read)
+                // a part: O in its own size, 16 bytes a row side by side, maximum and sum of each row; the halves of a unit of few tokens are two parts
+                float4* part = reinterpret_cast<float4*>(p.parts + (2 * (size_t)blockIdx.x + w.begins) * C::PART);
+                const float f = mine_n ? vref : 0.f;
 #pragma unroll 1
                 for (int c = 0; c < D / 16; ++c) {
                     uint32_t o[16];
                     tmem_ld16_nowait(o_at + 16 * c, o);
-                    tmem_ld_wait();
-                    float4* to = reinterpret_cast<float4*>(part + (size_t)rr * D + 16 * c);
+                    tmem_arrived<16>(o);
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        if (valid) to[k] = mine_n ? make_float4(__uint_as_float(o[4 * k]) * vref, __uint_as_float(o[4 * k + 1]) * vref, __uint_as_float(o[4 * k + 2]) * vref,
-                                                     __uint_as_float(o[4 * k + 3]) * vref)
+                        if (valid)
+                            part[(size_t)(4 * c + k) * (2 * K8P_ROWS) + st] =
+                                mine_n ? make_float4(__uint_as_float(o[4 * k]) * f, __uint_as_float(o[4 * k + 1]) * f, __uint_as_float(o[4 * k + 2]) * f, __uint_as_float(o[4 * k + 3]) * f)
                                        : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
-                if (valid) *reinterpret_cast<float2*>(part + (size_t)2 * K8P_ROWS * D + 2 * rr) = make_float2(m_ref, l_run);
-                if (st == 0 && w.t0 == 0)                                    // the unit begins here: what the next kernel has to know of it
-                    p.split[blockIdx.x] = Kv8Split{(int)((w.f - w.t1 + w.n_steps - 1) / per) - (int)blockIdx.x + 1, w.row0(p), w.h, w.few ? -w.n_tok : w.n_tok};
+                if (valid) reinterpret_cast<float2*>(part + (size_t)(D / 4) * (2 * K8P_ROWS))[st] = make_float2(m_ref, l_run);
+                if (st == 0 && w.begins)                                     // what the next kernel has to know of the unit
+                    p.split[blockIdx.x] = Kv8Split{w.parts, w.row0, w.head, w.few ? -w.tokens : w.tokens};
             }
-            base += n;
-            ++seg;
+            base += w.pages;
+            done(seg);
         }
     }
     tc_fence_before();
@@ -527,86 +615,109 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
     }
 }
 
-// Units that lie in several shares, out of their parts.  CTA (c, y) takes rows of the unit that begins in share c and goes on in the next ones.  Few parts: a group of D / 4
-// lanes takes a row; many (few tokens over a long history): all groups take one row, every eighth (sixteenth) part each.
-constexpr int K8P_MERGE = 256, K8P_SLICES = 16, K8P_FEW_PARTS = 6;
+// Units that lie in several shares, out of their parts.  CTA (c, y) puts together dims 16 y .. 16 y + 15 of the unit that begins in share c and goes on in the next
+// ones; a lane has a row, a warp 32 of them side by side.  Few parts: each warp has rows of its own; many (few tokens over a long history): all warps have the same rows
+// and every eighth part each.
+constexpr int K8P_MERGE_WARPS = 2 * K8P_ROWS / 32, K8P_FEW_PARTS = 8;
 template <int D>
-__global__ void __launch_bounds__(K8P_MERGE)
+__global__ void __launch_bounds__(K8P_MERGE_WARPS * 32)
 kv8_prefill_merge_kernel(const __grid_constant__ Kv8Prompt p) {
     using C = K8Prefill<D>;
-    constexpr int LR = D / 4, GROUPS = K8P_MERGE / LR;
-    __shared__ float4 s_acc[GROUPS][LR];
-    __shared__ float2 s_ml[GROUPS];
+    __shared__ float acc_s[K8P_MERGE_WARPS][18][32];
     pdl_wait();
     const Kv8Split u = p.split[blockIdx.x];
     if (u.parts == 0) return;
     const bool few = u.tokens < 0;
     const int n_tok = few ? -u.tokens : u.tokens, subs = few ? 2 : 1, np = u.parts * subs;
-    const int group = threadIdx.x / LR, d4 = threadIdx.x % LR * 4;
-    const bool alone = np <= K8P_FEW_PARTS;                          // a group has a row to itself
-    const int step = alone ? K8P_SLICES * GROUPS : K8P_SLICES;
-    for (int r = alone ? blockIdx.y * GROUPS + group : blockIdx.y; r < (few ? 1 : 2) * K8P_ROWS; r += step) {
-        const int row = r & 127, tok = row * p.inv_g >> 16, t = (r >> 7) * p.th + tok;
-        if (tok >= p.th || t >= n_tok) continue;                     // the same for all that take the row
-        float M = -INFINITY, L = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        const int first = alone ? 0 : group, stride = alone ? 1 : GROUPS;
-        for (int x0 = first; x0 < np; x0 += 4 * stride) {
-            float2 ml[4];
-            float4 o[4];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = blockIdx.y;
+    const bool alone = np <= K8P_FEW_PARTS;
+    for (int g = alone ? warp : 0; g < (few ? 1 : 2) * K8P_ROWS / 32; g += alone ? K8P_MERGE_WARPS : 1) {
+        const int r = 32 * g + lane, row = r & 127, tok = row * p.inv_g >> 16, t = (r >> 7) * p.th + tok;
+        const bool valid = tok < p.th && t < n_tok;
+        if (!__any_sync(0xffffffffu, valid)) continue;               // the same for all warps of the CTA that are at g
+        float M = -INFINITY, L = 0.f, acc[16];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {                            // four parts asked for at once
-                const int x = min(x0 + k * stride, np - 1), cta = blockIdx.x + x / subs, rec_row = r + (x % subs) * K8P_ROWS;
-                const float* rec = p.parts + (2 * (size_t)cta + (x < subs)) * C::PART;
-                ml[k] = *reinterpret_cast<const float2*>(rec + (size_t)2 * K8P_ROWS * D + 2 * rec_row);
-                o[k] = *reinterpret_cast<const float4*>(rec + (size_t)rec_row * D + d4);
-                if (x0 + k * stride >= np) ml[k] = make_float2(-INFINITY, 0.f);
+        for (int k = 0; k < 16; ++k) acc[k] = 0.f;
+        const int first = alone ? 0 : warp, stride = alone ? 1 : K8P_MERGE_WARPS;
+        for (int x0 = first; x0 < np; x0 += 2 * stride) {
+            float2 ml[2];
+            float4 o[2][4];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {                            // two parts asked for at once
+                const int x = min(x0 + k * stride, np - 1);
+                const float4* part = reinterpret_cast<const float4*>(p.parts + (2 * (size_t)(blockIdx.x + x / subs) + (x < subs)) * C::PART);
+                const int rr = r + (x % subs) * K8P_ROWS;
+                ml[k] = make_float2(-INFINITY, 0.f);
+                if (valid && x0 + k * stride < np) ml[k] = reinterpret_cast<const float2*>(part + (size_t)(D / 4) * (2 * K8P_ROWS))[rr];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[k][e] = valid ? part[(size_t)(4 * c + e) * (2 * K8P_ROWS) + rr] : make_float4(0.f, 0.f, 0.f, 0.f);
             }
-            const float Mn = fmaxf(M, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)));
+            const float Mn = fmaxf(M, fmaxf(ml[0].x, ml[1].x));
             const float keep = M == -INFINITY ? 0.f : exp2f(M - Mn);
-            L *= keep; acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+            L *= keep;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < 16; ++k) acc[k] *= keep;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
                 const float z = ml[k].x == -INFINITY ? 0.f : exp2f(ml[k].x - Mn);
                 L = fmaf(ml[k].y, z, L);
-                acc = fma_f4(o[k], make_float4(z, z, z, z), acc);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    acc[4 * e] = fmaf(o[k][e].x, z, acc[4 * e]);
+                    acc[4 * e + 1] = fmaf(o[k][e].y, z, acc[4 * e + 1]);
+                    acc[4 * e + 2] = fmaf(o[k][e].z, z, acc[4 * e + 2]);
+                    acc[4 * e + 3] = fmaf(o[k][e].w, z, acc[4 * e + 3]);
+                }
             }
             M = Mn;
         }
         if (!alone) {
-            s_acc[group][threadIdx.x % LR] = acc;
-            if (d4 == 0) s_ml[group] = make_float2(M, L);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) acc_s[warp][k][lane] = acc[k];
+            acc_s[warp][16][lane] = M;
+            acc_s[warp][17][lane] = L;
             __syncthreads();
-            if (group == 0) {
-                float Mn = M;
-                for (int k = 1; k < GROUPS; ++k) Mn = fmaxf(Mn, s_ml[k].x);
-                float Ls = 0.f;
-                float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (int k = 0; k < GROUPS; ++k) {
-                    const float z = s_ml[k].x == -INFINITY ? 0.f : exp2f(s_ml[k].x - Mn);
-                    Ls = fmaf(s_ml[k].y, z, Ls);
-                    a = fma_f4(s_acc[k][threadIdx.x], make_float4(z, z, z, z), a);
+            if (warp == 0) {
+                float Mn = M, Ls = 0.f;
+                for (int x = 1; x < K8P_MERGE_WARPS; ++x) Mn = fmaxf(Mn, acc_s[x][16][lane]);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) acc[k] = 0.f;
+                for (int x = 0; x < K8P_MERGE_WARPS; ++x) {
+                    const float z = acc_s[x][16][lane] == -INFINITY ? 0.f : exp2f(acc_s[x][16][lane] - Mn);
+                    Ls = fmaf(acc_s[x][17][lane], z, Ls);
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) acc[k] = fmaf(acc_s[x][k][lane], z, acc[k]);
                 }
                 L = Ls;
-                acc = a;
             }
             __syncthreads();
-            if (group) continue;
+            if (warp) continue;
         }
+        if (!valid) continue;
         const float inv = L == 0.f ? 0.f : 1.f / L;
-        const float y0 = acc.x * inv, y1 = acc.y * inv, y2 = acc.z * inv, y3 = acc.w * inv;
-        const uint32_t h0 = pack_bf16(y0, y1), h1 = pack_bf16(y2, y3);
-        const size_t to = ((size_t)(u.row0 + t) * p.nq + (size_t)u.head * p.G + (row - tok * p.G)) * D + d4;
-        *reinterpret_cast<uint2*>(p.out + to) = make_uint2(h0, h1);
-        if (p.out_lo)
-            *reinterpret_cast<uint2*>(p.out_lo + to) = make_uint2(pack_bf16(y0 - bf16_lo(h0), y1 - bf16_hi(h0)), pack_bf16(y2 - bf16_lo(h1), y3 - bf16_hi(h1)));
+        uint32_t hi[8], lo[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float x = acc[2 * k] * inv, y = acc[2 * k + 1] * inv;
+            hi[k] = pack_bf16(x, y);
+            lo[k] = pack_bf16(x - bf16_lo(hi[k]), y - bf16_hi(hi[k]));
+        }
+        const size_t off = ((size_t)(u.row0 + t) * p.nq + (size_t)u.head * p.G + (row - tok * p.G)) * D + 16 * c;
+        uint4* to = reinterpret_cast<uint4*>(p.out + off);
+        to[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        to[1] = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+        if (p.out_lo) {
+            to = reinterpret_cast<uint4*>(p.out_lo + off);
+            to[0] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            to[1] = make_uint4(lo[4], lo[5], lo[6], lo[7]);
+        }
     }
 }
 
 template <int D>
 static int launch_kv8_prefill(Kv8Prompt& p, void* scratch, cudaStream_t st) {
     using C = K8Prefill<D>;
-    static_assert(C::SMEM <= 232448 - 3072 && (C::BARS + C::N_BARS * 8) % 16 == 0 && C::REC % 16 == 0, "shared memory");
+    static_assert(C::SMEM <= 232448 - 4096 && C::REC % 16 == 0, "shared memory");
     static PerDeviceFlag attr_set;
     if (!attr_set.done()) {
         FT_CHECK_CUDA(cudaFuncSetAttribute(kv8_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
@@ -621,7 +732,7 @@ static int launch_kv8_prefill(Kv8Prompt& p, void* scratch, cudaStream_t st) {
     if (int r = kv8_waits_address(&p.err)) return r;
     kv8_prefill_kernel<D><<<ctas, K8P_THREADS, C::SMEM, st>>>(p);
     FT_CHECK_CUDA(cudaGetLastError());
-    if (parts) FT_CHECK_CUDA(launch_after(kv8_prefill_merge_kernel<D>, dim3(ctas, K8P_SLICES), dim3(K8P_MERGE), 0, st, (const Kv8Prompt&)p));
+    if (parts) FT_CHECK_CUDA(launch_after(kv8_prefill_merge_kernel<D>, dim3(ctas, D / 16), dim3(K8P_MERGE_WARPS * 32), 0, st, (const Kv8Prompt&)p));
     return 0;
 }
 

@@ -21,22 +21,22 @@ struct Kv8Prompt {
     float scale_log2;
 };
 
-// sum over i < n of floor((a i + b) / 64): the lattice points below a line, by Euclid's steps
-__host__ __device__ inline long long floor_sum64(long long n, long long a, long long b) {
-    long long m = 64, sum = 0;
+// sum over i < n of floor((a i + b) / 64): the lattice points below a line, by Euclid's steps.  Only the first has a large constant; all divisions are of 32 bits (a <= 256, n <= 2^22)
+__host__ __device__ inline long long floor_sum64(unsigned n, unsigned a, unsigned b) {
+    unsigned m = 64;
+    unsigned long long sum = 0;
     while (n > 0) {
-        sum += n * (n - 1) / 2 * (a / m) + n * (b / m);
+        sum += (unsigned long long)n * (n - 1) / 2 * (a / m) + (unsigned long long)n * (b / m);
         a %= m;
         b %= m;
-        const long long top = a * n + b;
+        const unsigned top = a * n + b;
         n = top / m;
         b = top % m;
-        const long long t = a;
+        const unsigned t = a;
         a = m;
         m = t;
-        if (m == 0) break;
     }
-    return sum;
+    return (long long)sum;
 }
 
 // one request: its rows of q, tiles of 2 th tokens, steps of its tiles
@@ -55,9 +55,12 @@ struct Kv8Request {
         const int n = pages(p, i);
         return tokens(p, i) <= p.th ? (n + 1) / 2 : n;
     }
-    __host__ __device__ __forceinline__ long long before(const Kv8Prompt& p, int i) const { return floor_sum64(i, 2 * p.th, (long long)pos0 + 2 * p.th - 1) + i; }   // steps of the full tiles 0 .. i - 1
+    __host__ __device__ __forceinline__ long long before(const Kv8Prompt& p, int i) const { return floor_sum64(i, 2 * p.th, pos0 + 2 * p.th - 1) + i; }   // steps of the full tiles 0 .. i - 1
     __host__ __device__ __forceinline__ long long all(const Kv8Prompt& p) const { return tiles ? before(p, tiles - 1) + steps(p, tiles - 1) : 0; }
 };
+
+// A stretch of pages of one unit.  parts: 0 = it is the whole unit; else, where the unit begins, how many shares it lies in
+struct Kv8Stretch { int page0, pages, few, row0, tokens, pos0, head, slot, begins, parts; };
 
 // A CTA's share, walked stretch by stretch; a stretch = steps t0 .. t1 - 1 of one unit
 struct Kv8Walk {
@@ -111,6 +114,21 @@ struct Kv8Walk {
             }
             before += n;
         }
+    }
+    // the stretch as the other warps get it; per: steps of a share
+    __host__ __device__ inline Kv8Stretch stretch(const Kv8Prompt& p, long long per, int share) const {
+        Kv8Stretch s;
+        s.page0 = page0();
+        s.pages = page1() - s.page0;
+        s.few = few;
+        s.row0 = row0(p);
+        s.tokens = n_tok;
+        s.pos0 = position0(p);
+        s.head = h;
+        s.slot = q.slot;
+        s.begins = t0 == 0;
+        s.parts = t0 == 0 && t1 == n_steps ? 0 : t0 == 0 ? (int)((f - t1 + n_steps - 1) / per) - share + 1 : 1;
+        return s;
     }
     // pages of the stretch, in the order in which they are asked for
     __host__ __device__ __forceinline__ int page0() const { return few ? 2 * t0 : t0; }
