@@ -12,7 +12,8 @@
 //
 // The flat list of all (request, key head, tile, page) is cut into equal shares, one for each SM: a causal list's units differ in length by any factor, and shares do
 // not.  A unit that lies in several shares is put together by a second kernel, in the parts' order.  Where there is an SM for every unit and none is much longer than
-// a share, each CTA takes a whole one.  One warp of each CTA finds its share from the lists on the device and tells the others stretch by stretch; nothing is planned
+// a share, each CTA takes a whole one.  (A unit's list is longer than its pages by what its start and end cost.  With one buffer of scores a half, at D = 128, the halves of a
+// unit of few tokens gain nothing over one: a page counts as one there.)  One warp of each CTA finds its share from the lists on the device and tells the others stretch by stretch; nothing is planned
 // ahead of the kernel.
 //
 // What bounds it: a page's chain of hand-overs in each half (scores - exponentials - probabilities - products), TIMES_HERE.
@@ -172,8 +173,8 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
         const long long total = __shfl_sync(0xffffffffu, b_steps, 31) * p.nkv, n_units = __shfl_sync(0xffffffffu, b_units, 31) * p.nkv;
         b_steps -= mine;
         b_units -= units;
-        const long long per = (total + gridDim.x - 1) / gridDim.x;
-        const bool whole = p.split == nullptr || (n_units <= gridDim.x && most <= per + K8P_WHOLE);      // (no room for parts: the host knows that there are none)
+        const long long per = kv8_div(total + gridDim.x - 1, gridDim.x);
+        const bool whole = p.split == nullptr || (n_units <= gridDim.x && most + kKv8Start <= per + K8P_WHOLE);      // (no room for parts: the host knows that there are none)
         // the flat list is one of units or of steps
         const long long len = whole ? n_units : total, each = whole ? 1 : per, at0 = whole ? b_units : b_steps;
         w.f = min(len, each * blockIdx.x);
@@ -757,6 +758,6 @@ extern "C" int ft_attn_prefill_kv8(const void* q, const void* kv8_layer, int num
     FT_REQUIRE(((uintptr_t)q | (uintptr_t)kv8_layer | (uintptr_t)out | (uintptr_t)out_lo | (uintptr_t)scratch) % 16 == 0, "ft_attn_prefill_kv8: tensors on 16 bytes");
     const int G = nq / nkv;
     Kv8Prompt p{(const __half*)q, (const uint8_t*)kv8_layer, page_table, req_q_start, req_slot, req_pos0, (__nv_bfloat16*)out, (__nv_bfloat16*)out_lo, nullptr, nullptr,
-                nullptr, num_pages, table_rows, max_pages, n_req, T, nq, nkv, G, K8P_ROWS / G, (65536u + G - 1) / G, K8P_LOG2E / sqrtf((float)d)};
+                nullptr, num_pages, table_rows, max_pages, n_req, T, nq, nkv, G, K8P_ROWS / G, d == 64 ? 2 : 1, (65536u + G - 1) / G, K8P_LOG2E / sqrtf((float)d)};
     return d == 64 ? launch_kv8_prefill<64>(p, scratch, (cudaStream_t)stream) : launch_kv8_prefill<128>(p, scratch, (cudaStream_t)stream);
 }

@@ -17,6 +17,7 @@ struct Kv8Prompt {
     int* err;
     int num_pages, table_rows, max_pages, n_req, T, nq, nkv;
     int G, th;                                                       // query heads a key head, tokens of a half
+    int few_pages;                                                   // pages of a step of a unit of few tokens
     unsigned inv_g;                                                  // row / G = row * inv_g >> 16
     float scale_log2;
 };
@@ -39,6 +40,14 @@ __host__ __device__ inline long long floor_sum64(unsigned n, unsigned a, unsigne
     return (long long)sum;
 }
 
+// What a unit costs beyond its pages, in pages: it takes that much more of the flat list, behind its last step
+constexpr int kKv8Start = 3;
+
+// a / b, most often of numbers below 2^32
+__host__ __device__ inline long long kv8_div(long long a, long long b) {
+    return ((unsigned long long)a | (unsigned long long)b) >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b);
+}
+
 // one request: its rows of q, tiles of 2 th tokens, steps of its tiles
 struct Kv8Request {
     int row0, len, pos0, slot, tiles;
@@ -53,10 +62,10 @@ struct Kv8Request {
     __host__ __device__ __forceinline__ int pages(const Kv8Prompt& p, int i) const { return (pos0 + i * 2 * p.th + tokens(p, i) - 1) / kKvTile + 1; }
     __host__ __device__ __forceinline__ int steps(const Kv8Prompt& p, int i) const {
         const int n = pages(p, i);
-        return tokens(p, i) <= p.th ? (n + 1) / 2 : n;
+        return tokens(p, i) <= p.th ? (n + p.few_pages - 1) / p.few_pages : n;
     }
-    __host__ __device__ __forceinline__ long long before(const Kv8Prompt& p, int i) const { return floor_sum64(i, 2 * p.th, pos0 + 2 * p.th - 1) + i; }   // steps of the full tiles 0 .. i - 1
-    __host__ __device__ __forceinline__ long long all(const Kv8Prompt& p) const { return tiles ? before(p, tiles - 1) + steps(p, tiles - 1) : 0; }
+    __host__ __device__ __forceinline__ long long before(const Kv8Prompt& p, int i) const { return floor_sum64(i, 2 * p.th, pos0 + 2 * p.th - 1) + i * (1LL + kKv8Start); }   // lengths of the full tiles 0 .. i - 1
+    __host__ __device__ __forceinline__ long long all(const Kv8Prompt& p) const { return tiles ? before(p, tiles - 1) + steps(p, tiles - 1) + kKv8Start : 0; }
 };
 
 // A stretch of pages of one unit.  parts: 0 = it is the whole unit; else, where the unit begins, how many shares it lies in
@@ -65,34 +74,38 @@ struct Kv8Stretch { int page0, pages, few, row0, tokens, pos0, head, slot, begin
 // A CTA's share, walked stretch by stretch; a stretch = steps t0 .. t1 - 1 of one unit
 struct Kv8Walk {
     Kv8Request q;
-    long long f, f_end;                                              // where it is in the flat list of steps
+    long long f, f_end, first;                                       // where it is in the flat list; where the unit begins
     int r, h, i, t, t0, t1, n_steps, n_pages, n_tok;
     bool few;
     __host__ __device__ __forceinline__ void unit(const Kv8Prompt& p) {
         n_tok = q.tokens(p, i);
         n_pages = q.pages(p, i);
         few = n_tok <= p.th;
-        n_steps = few ? (n_pages + 1) / 2 : n_pages;
+        n_steps = few ? (n_pages + p.few_pages - 1) / p.few_pages : n_pages;
     }
     __host__ __device__ __forceinline__ bool next(const Kv8Prompt& p) {
-        if (f >= f_end) return false;
-        if (t >= n_steps) {
-            t = 0;
-            if (++i == q.tiles) {
-                i = 0;
-                if (++h == p.nkv) {
-                    h = 0;
-                    do q.load(p, ++r);
-                    while (q.len == 0);
+        for (;;) {
+            if (f >= f_end) return false;
+            if (t >= n_steps + kKv8Start) {
+                t = 0;
+                if (++i == q.tiles) {
+                    i = 0;
+                    if (++h == p.nkv) {
+                        h = 0;
+                        do q.load(p, ++r);
+                        while (q.len == 0);
+                    }
                 }
+                unit(p);
             }
-            unit(p);
+            const int take = (int)min(f_end - f, (long long)(n_steps + kKv8Start - t));
+            first = f - t;
+            t0 = min(t, n_steps);
+            t1 = min(t + take, n_steps);
+            t += take;
+            f += take;
+            if (t1 > t0) return true;                                // else all of it was behind the unit's last step
         }
-        t0 = t;
-        t1 = t + (int)min(f_end - f, (long long)(n_steps - t));
-        t = t1;
-        f += t1 - t0;
-        return true;
     }
     // where step (or, where each CTA takes whole units, unit) `at` of the flat list lies; `before` of them belong to requests ahead of r0, and it is r0's or a later one's
     __host__ __device__ inline void seek(const Kv8Prompt& p, bool whole, int r0, long long before, long long at) {
@@ -101,7 +114,7 @@ struct Kv8Walk {
             const long long n = whole ? q.tiles : q.all(p);
             if (at < (before + n) * p.nkv) {
                 long long rest = at - before * p.nkv;
-                h = (int)(rest / n);
+                h = (int)kv8_div(rest, n);
                 rest -= h * n;
                 int lo = 0, hi = q.tiles - 1;                        // the last tile that begins at or before rest
                 while (!whole && lo < hi) {
@@ -118,8 +131,8 @@ struct Kv8Walk {
     // the stretch as the other warps get it; per: steps of a share
     __host__ __device__ inline Kv8Stretch stretch(const Kv8Prompt& p, long long per, int share) const {
         Kv8Stretch s;
-        s.page0 = page0();
-        s.pages = page1() - s.page0;
+        s.page0 = page0(p.few_pages);
+        s.pages = page1(p.few_pages) - s.page0;
         s.few = few;
         s.row0 = row0(p);
         s.tokens = n_tok;
@@ -127,12 +140,12 @@ struct Kv8Walk {
         s.head = h;
         s.slot = q.slot;
         s.begins = t0 == 0;
-        s.parts = t0 == 0 && t1 == n_steps ? 0 : t0 == 0 ? (int)((f - t1 + n_steps - 1) / per) - share + 1 : 1;
+        s.parts = t0 == 0 && t1 == n_steps ? 0 : t0 == 0 ? (int)kv8_div(first + n_steps - 1, per) - share + 1 : 1;
         return s;
     }
     // pages of the stretch, in the order in which they are asked for
-    __host__ __device__ __forceinline__ int page0() const { return few ? 2 * t0 : t0; }
-    __host__ __device__ __forceinline__ int page1() const { return few ? min(2 * t1, n_pages) : t1; }
+    __host__ __device__ __forceinline__ int page0(int p_few) const { return few ? p_few * t0 : t0; }
+    __host__ __device__ __forceinline__ int page1(int p_few) const { return few ? min(p_few * t1, n_pages) : t1; }
     __host__ __device__ __forceinline__ int row0(const Kv8Prompt& p) const { return q.row0 + i * 2 * p.th; }
     __host__ __device__ __forceinline__ int position0(const Kv8Prompt& p) const { return q.pos0 + i * 2 * p.th; }
 };
