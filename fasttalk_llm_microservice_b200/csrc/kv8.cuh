@@ -45,22 +45,23 @@ __device__ __forceinline__ uint32_t byte_perm(uint32_t a, uint32_t b, uint32_t s
 }
 
 // ------------------------------------------------------------------ one query token a sequence, up to eight query heads a key head (mma.sync m16n8k16)
-// A warp takes whole pages.  S[query][token] = Q K^T with the query heads in the M rows (rows 8 .. 15 are zeros), so that a lane holds one query's scores of two
-// neighbouring tokens: exactly what the second product wants as its B operand, O^T[dim][query] = V^T P^T, where all 16 rows are dims.  The order of the dims in the
-// first product is the lanes' (16 bytes of a token a lane), that of the dims in the second theirs too (8 neighbouring dims of each 64 a lane).
-// Codes are multiplied as they are; the keys' scale goes to the scores, the values' to the probabilities, relative to the largest values' scale that the warp has
+// A warp takes whole pages.  S[token][query] = K Q^T with 16 tokens in the M rows: K is the A operand, 16 bytes of two tokens a lane, in whatever order of the dims the
+// lanes have them (Q is loaded in the same).  The probabilities, transposed 8 x 8 at a time, are the B operand of O^T[dim][query] = V^T P^T, where all 16 rows are dims:
+// 8 neighbouring ones of each 64 a lane.  (With the queries in the rows of the first product nothing is transposed, but half the rows are zeros: 32 products a page
+// instead of 16 at D = 64, and their operands put together by 200 moves.)
+// Codes are multiplied as they are; the keys' scale goes to the exponents, the values' to the probabilities, relative to the largest values' scale that the warp has
 // seen (vref), or small values would leave fp16's range.
 template <int D>
 struct Kv8Query {
-    uint32_t q[D / 16][2];      // A operand, rows 0 .. 7
+    uint32_t q[D / 16][2];      // B operand
     float o[D / 16][4];         // O^T / vref: dims 64 sub + 8 g + 2 i (+ 1), queries 2 tq (+ 1), at [4 sub + i][2 * (dim & 1) + (query & 1)]
-    float m, l, vref;           // of query g: maximum in log2 units, sum
+    float m[2], l[2], vref;     // of queries 2 tq (+ 1): maximum in log2 units, this lane's tokens' sum
 
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-        m = -INFINITY;
-        l = vref = 0.f;
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = vref = 0.f;
     }
     // row: query head g of the group, or null
     __device__ __forceinline__ void load_query(const __half* row, int tq) {
@@ -78,79 +79,94 @@ struct Kv8Query {
     }
     // the first n (1 .. 64) tokens of the page at rec
     __device__ __forceinline__ void page(const uint8_t* rec, int n, float scale_log2, int g, int tq) {
-        const float4 ks = *reinterpret_cast<const float4*>(rec + Kv8<D>::SCALES), vs = *reinterpret_cast<const float4*>(rec + Kv8<D>::SCALES + 16);
-        const float kscale[4] = {ks.x * scale_log2, ks.y * scale_log2, ks.z * scale_log2, ks.w * scale_log2};
-        float p[8][2], most = -INFINITY;
+        const float4 k4 = *reinterpret_cast<const float4*>(rec + Kv8<D>::SCALES), vs = *reinterpret_cast<const float4*>(rec + Kv8<D>::SCALES + 16);
+        const float ks[4] = {k4.x * scale_log2, k4.y * scale_log2, k4.z * scale_log2, k4.w * scale_log2};
+        float s[4][4], most[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float s[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int b = 0; b < 4; ++b) {                                // a block of 16 tokens
+            s[b][0] = s[b][1] = s[b][2] = s[b][3] = 0.f;
 #pragma unroll
             for (int sub = 0; sub < D / 64; ++sub) {
-                const uint4 w = *reinterpret_cast<const uint4*>(rec + kv8_key_chunk(8 * j + g, sub * 4 + tq));
-                const uint32_t c[4] = {w.x, w.y, w.z, w.w};
+                const uint4 w0 = *reinterpret_cast<const uint4*>(rec + kv8_key_chunk(16 * b + g, sub * 4 + tq));
+                const uint4 w1 = *reinterpret_cast<const uint4*>(rec + kv8_key_chunk(16 * b + 8 + g, sub * 4 + tq));
+                const uint32_t c0[4] = {w0.x, w0.y, w0.z, w0.w}, c1[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) mma_f16_16816(s, q[sub * 4 + k][0], 0u, q[sub * 4 + k][1], 0u, kv8_lo(c[k]), kv8_hi(c[k]));
-            }
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                p[j][e] = 8 * j + 2 * tq + e < n ? s[e] * kscale[j >> 1] : -INFINITY;
-                most = fmaxf(most, p[j][e]);
+                for (int k = 0; k < 4; ++k) mma_f16_16816(s[b], kv8_lo(c0[k]), kv8_lo(c1[k]), kv8_hi(c0[k]), kv8_hi(c1[k]), q[sub * 4 + k][0], q[sub * 4 + k][1]);
             }
         }
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        const float m_new = fmaxf(m, most);                          // finite: a page has a token
+        if (n < kKvTile) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[b][e] = 16 * b + 8 * (e >> 1) + g < n ? s[b][e] : -INFINITY;
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const float f = fmaxf(ks[b], 1e-37f);                    // a block of zeros: hidden scores stay minus infinity
+            most[0] = fmaxf(most[0], fmaxf(s[b][0], s[b][2]) * f);
+            most[1] = fmaxf(most[1], fmaxf(s[b][1], s[b][3]) * f);
+        }
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) {
+            most[0] = fmaxf(most[0], __shfl_xor_sync(0xffffffffu, most[0], x));
+            most[1] = fmaxf(most[1], __shfl_xor_sync(0xffffffffu, most[1], x));
+        }
         const float v_new = fmaxf(vref, fmaxf(fmaxf(vs.x, vs.y), fmaxf(vs.z, vs.w)));
         const float v_inv = v_new > 0.f ? __fdividef(1.f, v_new) : 0.f;
-        if (__any_sync(0xffffffffu, m_new > m || v_new > vref)) {    // after the first few pages rarely
-            const float alpha = ex2_fast(m - m_new);
-            const float keep = alpha * (vref * v_inv);
-            l *= alpha;
-            m = m_new;
-            vref = v_new;
-            const float k0 = __shfl_sync(0xffffffffu, keep, 8 * tq), k1 = __shfl_sync(0xffffffffu, keep, 8 * tq + 4);
+        if (__any_sync(0xffffffffu, most[0] > m[0] || most[1] > m[1] || v_new > vref)) {     // after the first few pages rarely
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) o[i][0] *= k0, o[i][1] *= k1, o[i][2] *= k0, o[i][3] *= k1;
+            for (int e = 0; e < 2; ++e) {
+                const float m_new = fmaxf(m[e], most[e]);            // finite: a page has a token
+                const float alpha = ex2_fast(m[e] - m_new), keep = alpha * (vref * v_inv);
+                l[e] *= alpha;
+                m[e] = m_new;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) o[i][e] *= keep, o[i][2 + e] *= keep;
+            }
+            vref = v_new;
         }
         const float vscale[4] = {vs.x * v_inv, vs.y * v_inv, vs.z * v_inv, vs.w * v_inv};
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {                             // a block of 16 tokens
-            uint32_t b[2];
+        for (int b = 0; b < 4; ++b) {
+            const float f = fmaxf(ks[b], 1e-37f);
+            const float p0 = ex2_fast(fmaf(s[b][0], f, -m[0])), p1 = ex2_fast(fmaf(s[b][1], f, -m[1]));
+            const float p2 = ex2_fast(fmaf(s[b][2], f, -m[0])), p3 = ex2_fast(fmaf(s[b][3], f, -m[1]));
+            l[0] += p0 + p2;
+            l[1] += p1 + p3;
+            uint32_t pb[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float p0 = ex2_fast(p[2 * kk + h][0] - m), p1 = ex2_fast(p[2 * kk + h][1] - m);
-                l += p0 + p1;
-                const __half2 t = __floats2half2_rn(p0 * vscale[kk], p1 * vscale[kk]);
-                b[h] = *reinterpret_cast<const uint32_t*>(&t);
+                const __half2 t = h ? __floats2half2_rn(p2 * vscale[b], p3 * vscale[b]) : __floats2half2_rn(p0 * vscale[b], p1 * vscale[b]);
+                asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pb[h]) : "r"(*reinterpret_cast<const uint32_t*>(&t)));
             }
 #pragma unroll
             for (int sub = 0; sub < D / 64; ++sub) {
                 uint2 t[4];                                          // tokens 2 tq, + 1, + 8, + 9
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    t[e] = *reinterpret_cast<const uint2*>(rec + kv8_value_chunk<D>(16 * kk + 2 * tq + (e & 1) + (e >> 1) * 8, sub * 4 + (g >> 1)) + (g & 1) * 8);
+                    t[e] = *reinterpret_cast<const uint2*>(rec + kv8_value_chunk<D>(16 * b + 2 * tq + (e & 1) + (e >> 1) * 8, sub * 4 + (g >> 1)) + (g & 1) * 8);
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
                     const uint32_t t0 = w ? t[0].y : t[0].x, t1 = w ? t[1].y : t[1].x, t2 = w ? t[2].y : t[2].x, t3 = w ? t[3].y : t[3].x;
                     const uint32_t x = byte_perm(t0, t1, 0x5140), y = byte_perm(t0, t1, 0x7362), u = byte_perm(t2, t3, 0x5140), v = byte_perm(t2, t3, 0x7362);
-                    mma_f16_16816(o[sub * 4 + 2 * w], kv8_lo(x), kv8_hi(x), kv8_lo(u), kv8_hi(u), b[0], b[1]);
-                    mma_f16_16816(o[sub * 4 + 2 * w + 1], kv8_lo(y), kv8_hi(y), kv8_lo(v), kv8_hi(v), b[0], b[1]);
+                    mma_f16_16816(o[sub * 4 + 2 * w], kv8_lo(x), kv8_hi(x), kv8_lo(u), kv8_hi(u), pb[0], pb[1]);
+                    mma_f16_16816(o[sub * 4 + 2 * w + 1], kv8_lo(y), kv8_hi(y), kv8_lo(v), kv8_hi(v), pb[0], pb[1]);
                 }
             }
         }
     }
     // the warp's state as a record of eight query heads, O in its own size: [query][D | m | l]
     __device__ __forceinline__ void store(float* rec, int g, int tq) {
-        float sum = l + __shfl_xor_sync(0xffffffffu, l, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i)
+        for (int e = 0; e < 2; ++e) {
+            float sum = l[e];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                float* at = rec + (size_t)(2 * tq + e) * (D + 2) + (i >> 2) * 64 + 8 * g + 2 * (i & 3);
-                *reinterpret_cast<float2*>(at) = make_float2(o[i][e] * vref, o[i][2 + e] * vref);
-            }
-        if (tq == 0) *reinterpret_cast<float2*>(rec + (size_t)g * (D + 2) + D) = make_float2(m, sum);
+            for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            float* at = rec + (size_t)(2 * tq + e) * (D + 2);
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) *reinterpret_cast<float2*>(at + (i >> 2) * 64 + 8 * g + 2 * (i & 3)) = make_float2(o[i][e] * vref, o[i][2 + e] * vref);
+            if (g == 0) *reinterpret_cast<float2*>(at + D) = make_float2(m[e], sum);
+        }
     }
 };
 

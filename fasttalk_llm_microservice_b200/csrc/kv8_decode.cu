@@ -50,9 +50,9 @@ kv8_decode_kernel(const __half* __restrict__ q, const uint8_t* __restrict__ cach
     uint64_t* empty = full + C::STAGES;
     int* tokens = reinterpret_cast<int*>(smem + C::TOKENS);                  // of the page in each stage; 0: a page that is not there
     float* merge = reinterpret_cast<float*>(smem + C::MERGE);
-    __shared__ long long s_sum[C::WARPS + 1];
+    __shared__ int s_sum[C::WARPS + 1];
     __shared__ int s_most[C::WARPS + 1], s_b, s_last;
-    __shared__ long long s_base;
+    __shared__ int s_base;
     __shared__ volatile int dead;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tq = lane & 3;
@@ -68,23 +68,23 @@ kv8_decode_kernel(const __half* __restrict__ q, const uint8_t* __restrict__ cach
     // ---------------- the plan: this CTA's share of the flat list [sequence][head][page]
     const int chunk = (B + C::THREADS - 1) / C::THREADS;
     const int b0 = min(B, tid * chunk), b1 = min(B, b0 + chunk);
-    long long mine = 0;
+    int mine = 0;                                                            // (the host has seen that 32 bits hold the whole list)
     int most = 0;
     for (int b = b0; b < b1; ++b) {
         const int n = pages_of(b);
         mine += n;
         most = max(most, n);
     }
-    long long before = mine;
+    int before = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, before, o);
+        const int up = __shfl_up_sync(0xffffffffu, before, o);
         if (lane >= o) before += up;
     }
     most = __reduce_max_sync(0xffffffffu, most);
     if (lane == 31) s_sum[warp] = before, s_most[warp] = most;
     __syncthreads();
-    long long total = 0;
+    int total = 0;
     before -= mine;
 #pragma unroll
     for (int w = 0; w <= C::WARPS; ++w) {
@@ -93,10 +93,10 @@ kv8_decode_kernel(const __half* __restrict__ q, const uint8_t* __restrict__ cach
         most = max(most, s_most[w]);
     }
     total *= nkv;
-    const long long per = (total + gridDim.x - 1) / gridDim.x;
-    const bool each = (long long)B * nkv <= gridDim.x;
+    const int per = (int)((unsigned)(total + gridDim.x - 1) / gridDim.x);
+    const bool each = B * nkv <= (int)gridDim.x;
     const bool whole = each && (parts == nullptr || (most + C::WARPS - 1) / C::WARPS <= (per + C::WARPS - 1) / C::WARPS + 1);
-    long long f = per * blockIdx.x, f_end = min(f + per, total);
+    int f = min(per * (int)blockIdx.x, total), f_end = min(f + per, total);
     int b, h, t;
     if (whole) {
         b = blockIdx.x / nkv;
@@ -111,17 +111,17 @@ kv8_decode_kernel(const __half* __restrict__ q, const uint8_t* __restrict__ cach
     } else {
         if (before * nkv <= f && f < (before + mine) * nkv) {
             int x = b0;
-            for (int n; before * nkv + (long long)(n = pages_of(x)) * nkv <= f; ++x) before += n;
+            for (int n; (before + (n = pages_of(x))) * nkv <= f; ++x) before += n;
             s_b = x;
             s_base = before;
         }
         __syncthreads();
         if (f >= f_end) f_end = f;
         b = s_b;
-        const long long rest = f - s_base * nkv;
+        const unsigned rest = f - s_base * nkv;
         const int n = f < f_end ? pages_of(b) : 1;
-        h = (int)(rest / n);
-        t = (int)(rest % n);
+        h = (int)(rest / (unsigned)n);
+        t = (int)(rest - (unsigned)h * n);
     }
     // a sequence without keys has no page and so no share: zeros
     auto zeros = [&](int b_, int h0, int h1) {
@@ -155,7 +155,7 @@ kv8_decode_kernel(const __half* __restrict__ q, const uint8_t* __restrict__ cach
                 while (n_pages == 0);
             }
         }
-        const int take = (int)min(f_end - f, (long long)(n_pages - t));
+        const int take = min(f_end - f, n_pages - t);
         seg_b = b; seg_h = h; t0 = t; t1 = t + take;
         t = t1;
         f += take;
@@ -220,14 +220,14 @@ kv8_decode_kernel(const __half* __restrict__ q, const uint8_t* __restrict__ cach
         it += t1 - t0;
         if (!ok) {                                                           // NaN for all that this (sequence, head) says
             *err = 1;
-            a.m = 0.f;
-            a.l = NAN;
+            a.m[0] = a.m[1] = 0.f;
+            a.l[0] = a.l[1] = NAN;
         }
         a.store(merge + (size_t)warp * C::PART, g, tq);
         asm volatile("bar.sync 1, %0;" ::"n"(C::WARPS * 32) : "memory");
         const bool all = t0 == 0 && t1 == n_pages;
-        const long long first = f - t1;                                      // of the (sequence, head) in the flat list (a whole one has no parts)
-        const int c0 = all ? 0 : (int)(first / per), c1 = all ? 0 : (int)((first + n_pages - 1) / per);
+        const int first = f - t1;                                            // of the (sequence, head) in the flat list (a whole one has no parts)
+        const int c0 = all ? 0 : (int)((unsigned)first / (unsigned)per), c1 = all ? 0 : (int)((unsigned)(first + n_pages - 1) / (unsigned)per);
         float* part = parts + (2 * (size_t)blockIdx.x + (t0 == 0)) * C::PART;
         const size_t row = ((size_t)seg_b * nq + (size_t)seg_h * G) * D;
         auto put = [&](int e, float x, float y, float l) {                   // two dims; a query without a visible key: zeros
@@ -371,8 +371,8 @@ extern "C" int ft_attn_decode_kv8(const void* q, const void* kv8_layer, int num_
     using namespace ft;
     FT_REQUIRE(d == 64 || d == 128, "ft_attn_decode_kv8: head_dim %d not supported (64 or 128)", d);
     FT_REQUIRE(nq >= 1 && nkv >= 1 && nq % nkv == 0 && nq / nkv <= K8D_GROUP, "ft_attn_decode_kv8: GQA group %d/%d not supported", nq, nkv);
-    FT_REQUIRE(B >= 0 && max_pages >= 0 && num_pages >= 0 && max_pages <= INT32_MAX / kKvTile, "ft_attn_decode_kv8: bad sizes B=%d max_pages=%d num_pages=%d", B,
-               max_pages, num_pages);
+    FT_REQUIRE(B >= 0 && max_pages >= 0 && num_pages >= 0 && max_pages <= INT32_MAX / kKvTile && ((double)B + 1) * nkv * (max_pages + 1) + 4096 <= INT32_MAX,
+               "ft_attn_decode_kv8: bad sizes B=%d nkv=%d max_pages=%d num_pages=%d", B, nkv, max_pages, num_pages);
     if (B == 0) return 0;
     FT_REQUIRE(q && kv8_layer && page_table && ctx_lens && out, "ft_attn_decode_kv8: null argument");
     FT_REQUIRE(((uintptr_t)q | (uintptr_t)kv8_layer | (uintptr_t)out | (uintptr_t)out_lo | (uintptr_t)scratch) % 16 == 0, "ft_attn_decode_kv8: tensors on 16 bytes");
