@@ -46,8 +46,8 @@ int launch_gemm(const CUtensorMap& mw, const CUtensorMap& mx, const CUtensorMap*
                 int T, int K, int splits, const ft_gemm_epilogue& epi, bool pdl, cudaStream_t stream,
                 const CUtensorMap* mx_half = nullptr, const CUtensorMap* mx_lo_half = nullptr);
 
-// ---- kv8_decode.cu: device address of the word that kernels of the 8-bit cache set when a wait runs out
-int kv8_waits_address(int** at);
+// ---- kv8_prefill.cu: 1 once a wait has run out in a kernel of that file
+int kv8_prefill_waits(int* out);
 
 // ---- gemm_plain.cu: out[t][n] = sum_k (hi + lo)[t][k] W[n][k], fp32 results without a fused layer step
 int launch_gemm_plain(const void* w, const void* hi, const void* lo, float* out, int n_out, int T, int K, cudaStream_t stream);

@@ -80,6 +80,8 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
     return __all_sync(0xffffffffu, mbar_wait_limited(bar, parity, dead));
 }
 
+__device__ int g_kv8_prefill_waits;              // 1: a wait ran out on this device (ft_kv8_waits)
+
 // floats that the descriptions of split units take at the head of the work memory
 static size_t kv8_prefill_splits(int ctas) { return (size_t)(ctas + 15) / 16 * 16 * (sizeof(Kv8Split) / 4); }
 
@@ -108,7 +110,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
     __shared__ volatile int dead;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    int* const err = p.err;
+    int* const err = &g_kv8_prefill_waits;
     if (tid == 0) {
         for (int s = 0; s < C::S16; ++s) mbar_init(&kv_full[s], K8P_CONV / 32), mbar_init(&kv_empty[s], 2);
         for (int s = 0; s < C::S8; ++s) mbar_init(&rec_full[s], 1), mbar_init(&rec_empty[s], K8P_CONV / 32);
@@ -730,10 +732,14 @@ static int launch_kv8_prefill(Kv8Prompt& p, void* scratch, cudaStream_t st) {
     FT_REQUIRE(!parts || scratch, "ft_attn_prefill_kv8: needs ft_attn_prefill_kv8_scratch_bytes of work memory");
     p.split = parts ? (Kv8Split*)scratch : nullptr;
     p.parts = (float*)scratch + kv8_prefill_splits(ctas);
-    if (int r = kv8_waits_address(&p.err)) return r;
     kv8_prefill_kernel<D><<<ctas, K8P_THREADS, C::SMEM, st>>>(p);
     FT_CHECK_CUDA(cudaGetLastError());
     if (parts) FT_CHECK_CUDA(launch_after(kv8_prefill_merge_kernel<D>, dim3(ctas, D / 16), dim3(K8P_MERGE_WARPS * 32), 0, st, (const Kv8Prompt&)p));
+    return 0;
+}
+
+int kv8_prefill_waits(int* out) {
+    FT_CHECK_CUDA(cudaMemcpyFromSymbol(out, g_kv8_prefill_waits, sizeof(*out)));
     return 0;
 }
 
@@ -758,6 +764,6 @@ extern "C" int ft_attn_prefill_kv8(const void* q, const void* kv8_layer, int num
     FT_REQUIRE(((uintptr_t)q | (uintptr_t)kv8_layer | (uintptr_t)out | (uintptr_t)out_lo | (uintptr_t)scratch) % 16 == 0, "ft_attn_prefill_kv8: tensors on 16 bytes");
     const int G = nq / nkv;
     Kv8Prompt p{(const __half*)q, (const uint8_t*)kv8_layer, page_table, req_q_start, req_slot, req_pos0, (__nv_bfloat16*)out, (__nv_bfloat16*)out_lo, nullptr, nullptr,
-                nullptr, num_pages, table_rows, max_pages, n_req, T, nq, nkv, G, K8P_ROWS / G, d == 64 ? 2 : 1, (65536u + G - 1) / G, K8P_LOG2E / sqrtf((float)d)};
+                num_pages, table_rows, max_pages, n_req, T, nq, nkv, G, K8P_ROWS / G, d == 64 ? 2 : 1, (65536u + G - 1) / G, K8P_LOG2E / sqrtf((float)d)};
     return d == 64 ? launch_kv8_prefill<64>(p, scratch, (cudaStream_t)stream) : launch_kv8_prefill<128>(p, scratch, (cudaStream_t)stream);
 }

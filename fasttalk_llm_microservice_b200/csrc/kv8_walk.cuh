@@ -14,7 +14,6 @@ struct Kv8Prompt {
     __nv_bfloat16 *out, *out_lo;
     Kv8Split* split;
     float* parts;
-    int* err;
     int num_pages, table_rows, max_pages, n_req, T, nq, nkv;
     int G, th;                                                       // query heads a key head, tokens of a half
     int few_pages;                                                   // pages of a step of a unit of few tokens

@@ -236,47 +236,49 @@ def _refuse(what: str, why: str) -> None:
     raise N.NativeError(f"{what}: {why}")
 
 
+# The checks below run ahead of every call: a step of single tokens takes a few microseconds on the GPU, so they ask tensors for numbers, not for objects.
 def _kv8_layer(layer: torch.Tensor, d: int, what: str):
-    """(pages, kv heads) of a layer; all tensors of a call have to be on its device."""
-    if not (layer.is_cuda and layer.dtype == torch.uint8 and layer.dim() == 3 and layer.is_contiguous()):
+    """(device, pages, kv heads) of a layer; all tensors of a call have to be on its device."""
+    index = layer.get_device()
+    if index < 0 or layer.dtype is not torch.uint8 or layer.dim() != 3 or not layer.is_contiguous():
         _refuse(what, "the cache is contiguous CUDA uint8 [pages, nkv, record]")
     pages, nkv, record = layer.shape
     if record != 128 * d + 32:
         _refuse(what, "the cache's records are not those of this head_dim")
-    return pages, nkv
+    return index, pages, nkv
 
 
-def _kv8_ints(t, dev, what: str, n: int = -1, name: str = "") -> torch.Tensor:
-    """int32 on the device, n of them; a list goes up in a copy that the host waits for."""
+def _kv8_ints(t, index: int, what: str, n: int, name: str) -> torch.Tensor:
+    """int32 on the device, n of them (n < 0: any number); a list goes up in a copy that the host waits for."""
     if not isinstance(t, torch.Tensor):
-        t = torch.tensor(t, dtype=torch.int32, device=dev).reshape(-1)
-    if not (t.dtype == torch.int32 and t.device == dev and t.is_contiguous()):
+        t = torch.tensor(t, dtype=torch.int32, device=f"cuda:{index}").reshape(-1)
+    if t.dtype is not torch.int32 or t.get_device() != index or not t.is_contiguous():
         _refuse(what, f"{name} is contiguous int32 on the cache's device")
     if n >= 0 and t.numel() != n:
         _refuse(what, f"{name} has {n} numbers here, not {t.numel()}")
     return t
 
 
-def _kv8_table(t: torch.Tensor, dev, what: str):
-    if not (t.dtype == torch.int32 and t.device == dev and t.dim() == 2 and t.is_contiguous()):
+def _kv8_table(t: torch.Tensor, index: int, what: str):
+    if t.dtype is not torch.int32 or t.get_device() != index or t.dim() != 2 or not t.is_contiguous():
         _refuse(what, "page_table is contiguous int32 [sequences, pages] on the cache's device")
     return t.shape
 
 
-def _kv8_requests(req_start, req_slot, req_pos0, dev, what: str):
-    req_slot = _kv8_ints(req_slot, dev, what, name="req_slot")
+def _kv8_requests(req_start, req_slot, req_pos0, index: int, what: str):
+    req_slot = _kv8_ints(req_slot, index, what, -1, "req_slot")
     n = req_slot.numel()
-    return _kv8_ints(req_start, dev, what, n + 1, "req_start"), req_slot, _kv8_ints(req_pos0, dev, what, n, "req_pos0"), n
+    return _kv8_ints(req_start, index, what, n + 1, "req_start"), req_slot, _kv8_ints(req_pos0, index, what, n, "req_pos0"), n
 
 
-def _kv8_call(dev, name: str, *args) -> None:
+def _kv8_call(index: int, name: str, *args) -> None:
     """A library call on the device's current stream, whichever device is the current one."""
-    fn = getattr(N.load(), name)
-    if dev.index == torch.cuda.current_device():
-        rc = fn(*args, N.device_stream(dev.index))
+    fn, stream = getattr(N.load(), name), torch._C._cuda_getCurrentRawStream(index)
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, stream)
     else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, N.device_stream(dev.index))
+        with torch.cuda.device(index):
+            rc = fn(*args, stream)
     if rc < 0:
         N.check(rc, name)
 
@@ -284,13 +286,12 @@ def _kv8_call(dev, name: str, *args) -> None:
 _kv8_sizes = {}
 
 
-def _kv8_scratch_bytes(dev, name: str, d: int) -> int:
-    key = (dev.index, name, d)
-    n = _kv8_sizes.get(key)
+def _kv8_scratch(index: int, name: str, d: int) -> torch.Tensor:
+    n = _kv8_sizes.get((index, name, d))
     if n is None:
-        with torch.cuda.device(dev):
-            n = _kv8_sizes[key] = N.check(getattr(N.load(), name)(d), name)
-    return n
+        with torch.cuda.device(index):
+            n = _kv8_sizes[index, name, d] = N.check(getattr(N.load(), name)(d), name)
+    return torch.empty(n, device=index, dtype=torch.uint8)
 
 
 def kv8_cache_alloc(num_pages: int, nkv: int, d: int, device) -> torch.Tensor:
@@ -306,24 +307,23 @@ def rope_kv8_append(qkv_partials: torch.Tensor, cos: torch.Tensor, sin: torch.Te
     whose scale is too small for a new token is rescaled, the tokens before it in the block with it; a block that is entered at its first token starts anew.
     Tokens without a place (a position outside the tables, a page outside the cache) are not written."""
     what = "rope_kv8_append"
-    dev = kv8_layer.device
-    pages, heads = _kv8_layer(kv8_layer, d, what)
+    index, pages, heads = _kv8_layer(kv8_layer, d, what)
     width = (nq + 2 * nkv) * d
     if heads != nkv:
         _refuse(what, "the cache has another number of heads")
-    if not (qkv_partials.dim() == 3 and qkv_partials.dtype == torch.float32 and qkv_partials.device == dev and qkv_partials.shape[2] == width):
+    if qkv_partials.dim() != 3 or qkv_partials.dtype is not torch.float32 or qkv_partials.get_device() != index or qkv_partials.shape[2] != width:
         _refuse(what, "qkv_partials is fp32 [S, T, (nq + 2 nkv) d] on the cache's device")
     S, T, _ = qkv_partials.shape
     part, row, one = qkv_partials.stride()
     if one != 1 or (row != width and T > 1):
         _refuse(what, "the rows of qkv_partials lie one behind the other")
-    if not (cos.dtype == sin.dtype == torch.float32 and cos.device == sin.device == dev and cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] * 2 == d
-            and cos.is_contiguous() and sin.is_contiguous()):
+    if (cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or cos.get_device() != index or sin.get_device() != index or cos.dim() != 2
+            or cos.shape != sin.shape or cos.shape[1] * 2 != d or not cos.is_contiguous() or not sin.is_contiguous()):
         _refuse(what, "cos and sin are contiguous fp32 [positions, d / 2] on the cache's device")
-    positions, seq_rows = _kv8_ints(positions, dev, what, T, "positions"), _kv8_ints(seq_rows, dev, what, T, "seq_rows")
-    rows, most = _kv8_table(page_table, dev, what)
-    q = torch.empty(T, nq, d, device=dev, dtype=torch.float16)
-    _kv8_call(dev, "ft_rope_kv8_append", qkv_partials.data_ptr(), S, part, cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(),
+    positions, seq_rows = _kv8_ints(positions, index, what, T, "positions"), _kv8_ints(seq_rows, index, what, T, "seq_rows")
+    rows, most = _kv8_table(page_table, index, what)
+    q = torch.empty(T, nq, d, device=index, dtype=torch.float16)
+    _kv8_call(index, "ft_rope_kv8_append", qkv_partials.data_ptr(), S, part, cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(),
               seq_rows.data_ptr(), page_table.data_ptr(), rows, most, q.data_ptr(), kv8_layer.data_ptr(), pages, T, nq, nkv, d)
     return q
 
@@ -332,44 +332,44 @@ def kv8_read(kv8_layer: torch.Tensor, page_table: torch.Tensor, req_start, req_s
     """Keys and values back as fp16 [rows, nkv, d] each: request r gets rows req_start[r] .. req_start[r + 1] - 1, from position req_pos0[r] of page-table row
     req_slot[r] on.  Rows that no request owns, and rows without a page, are zeros.  The lists are int32 tensors on the device, or anything a tensor is made of."""
     what = "kv8_read"
-    dev = kv8_layer.device
-    pages, nkv = _kv8_layer(kv8_layer, d, what)
-    table_rows, most = _kv8_table(page_table, dev, what)
-    req_start, req_slot, req_pos0, n = _kv8_requests(req_start, req_slot, req_pos0, dev, what)
+    index, pages, nkv = _kv8_layer(kv8_layer, d, what)
+    table_rows, most = _kv8_table(page_table, index, what)
+    req_start, req_slot, req_pos0, n = _kv8_requests(req_start, req_slot, req_pos0, index, what)
     if rows < 0:
         _refuse(what, "a number of rows")
-    k = torch.empty(rows, nkv, d, device=dev, dtype=torch.float16)
-    v = torch.empty(rows, nkv, d, device=dev, dtype=torch.float16)
-    _kv8_call(dev, "ft_kv8_read", kv8_layer.data_ptr(), pages, page_table.data_ptr(), table_rows, most, req_start.data_ptr(),
-              req_slot.data_ptr(), req_pos0.data_ptr(), n, rows, k.data_ptr(), v.data_ptr(), nkv, d)
+    k = torch.empty(rows, nkv, d, device=index, dtype=torch.float16)
+    v = torch.empty_like(k)
+    _kv8_call(index, "ft_kv8_read", kv8_layer.data_ptr(), pages, page_table.data_ptr(), table_rows, most, req_start.data_ptr(), req_slot.data_ptr(),
+              req_pos0.data_ptr(), n, rows, k.data_ptr(), v.data_ptr(), nkv, d)
     return k, v
 
 
 def _kv8_query(q: torch.Tensor, kv8_layer: torch.Tensor, planes: int, what: str):
-    dev = kv8_layer.device
-    if not (q.dim() == 3 and q.dtype == torch.float16 and q.device == dev and q.is_contiguous()):
-        _refuse(what, "q is contiguous fp16 [rows, nq, d] on the cache's device")
+    if q.dim() != 3 or q.dtype is not torch.float16 or not q.is_contiguous():
+        _refuse(what, "q is contiguous fp16 [rows, nq, d]")
     rows, nq, d = q.shape
-    pages, nkv = _kv8_layer(kv8_layer, d, what)
+    index, pages, nkv = _kv8_layer(kv8_layer, d, what)
+    if q.get_device() != index:
+        _refuse(what, "q is on another device than the cache")
     if planes != 1 and planes != 2:
         _refuse(what, "one plane or two")
-    out = torch.empty(rows, nq * d, device=dev, dtype=torch.bfloat16)
-    return dev, pages, nkv, rows, nq, d, out, torch.empty_like(out) if planes == 2 else None
+    out = torch.empty(rows, nq * d, device=index, dtype=torch.bfloat16)
+    return index, pages, nkv, rows, nq, d, out, torch.empty_like(out) if planes == 2 else None
 
 
 def attn_decode_kv8(q: torch.Tensor, kv8_layer: torch.Tensor, page_table: torch.Tensor, ctx_lens: torch.Tensor, planes: int = 2):
     """attn_decode over the 8-bit cache: q fp16 [B, nq, d], up to eight query heads a key head -> bf16 (hi, lo) planes [B, nq * d], lo None with planes = 1.  A
     sequence without keys gives zeros; keys on pages outside the cache are hidden."""
     what = "attn_decode_kv8"
-    dev, pages, nkv, B, nq, d, out, lo = _kv8_query(q, kv8_layer, planes, what)
-    ctx_lens = _kv8_ints(ctx_lens, dev, what, B, "ctx_lens")
-    rows, most = _kv8_table(page_table, dev, what)
+    index, pages, nkv, B, nq, d, out, lo = _kv8_query(q, kv8_layer, planes, what)
+    ctx_lens = _kv8_ints(ctx_lens, index, what, B, "ctx_lens")
+    rows, most = _kv8_table(page_table, index, what)
     if rows < B:
         _refuse(what, "a page-table row for every query")
-    n = _kv8_scratch_bytes(dev, "ft_attn_decode_kv8_scratch_bytes", d)
-    scratch = torch.empty(n, device=dev, dtype=torch.uint8) if most > 16 or B * nkv > 256 else None
-    _kv8_call(dev, "ft_attn_decode_kv8", q.data_ptr(), kv8_layer.data_ptr(), pages, page_table.data_ptr(), most, ctx_lens.data_ptr(), out.data_ptr(),
-              N.ptr(lo), N.ptr(scratch), B, nq, nkv, d)
+    # the library needs none for a few sequences whose page tables are short
+    scratch = _kv8_scratch(index, "ft_attn_decode_kv8_scratch_bytes", d) if most > 16 or B * nkv > 256 else None
+    _kv8_call(index, "ft_attn_decode_kv8", q.data_ptr(), kv8_layer.data_ptr(), pages, page_table.data_ptr(), most, ctx_lens.data_ptr(), out.data_ptr(),
+              0 if lo is None else lo.data_ptr(), 0 if scratch is None else scratch.data_ptr(), B, nq, nkv, d)
     return out, lo
 
 
@@ -377,13 +377,12 @@ def attn_prefill_kv8(q: torch.Tensor, kv8_layer: torch.Tensor, page_table: torch
     """attn_prefill over the 8-bit cache, up to eight query heads a key head.  The lists are int32 tensors on the device (then nothing goes up, and the call can be
     captured) or anything a tensor is made of.  Rows that no request owns are zeros; keys on pages outside the cache are hidden.  -> (hi, lo), lo None with planes = 1."""
     what = "attn_prefill_kv8"
-    dev, pages, nkv, T, nq, d, out, lo = _kv8_query(q, kv8_layer, planes, what)
-    rows, most = _kv8_table(page_table, dev, what)
-    req_q_start, req_slot, req_pos0, n = _kv8_requests(req_q_start, req_slot, req_pos0, dev, what)
-    size = _kv8_scratch_bytes(dev, "ft_attn_prefill_kv8_scratch_bytes", d)
-    scratch = torch.empty(size, device=dev, dtype=torch.uint8)
-    _kv8_call(dev, "ft_attn_prefill_kv8", q.data_ptr(), kv8_layer.data_ptr(), pages, page_table.data_ptr(), rows, most, req_q_start.data_ptr(),
-              req_slot.data_ptr(), req_pos0.data_ptr(), n, T, out.data_ptr(), N.ptr(lo), scratch.data_ptr(), nq, nkv, d)
+    index, pages, nkv, T, nq, d, out, lo = _kv8_query(q, kv8_layer, planes, what)
+    rows, most = _kv8_table(page_table, index, what)
+    req_q_start, req_slot, req_pos0, n = _kv8_requests(req_q_start, req_slot, req_pos0, index, what)
+    scratch = _kv8_scratch(index, "ft_attn_prefill_kv8_scratch_bytes", d)
+    _kv8_call(index, "ft_attn_prefill_kv8", q.data_ptr(), kv8_layer.data_ptr(), pages, page_table.data_ptr(), rows, most, req_q_start.data_ptr(),
+              req_slot.data_ptr(), req_pos0.data_ptr(), n, T, out.data_ptr(), 0 if lo is None else lo.data_ptr(), scratch.data_ptr(), nq, nkv, d)
     return out, lo
 
 

@@ -171,12 +171,6 @@ def ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-def device_stream(index: int) -> int:
-    """The current stream of a device (cur_stream() without the Python object: 0.1 us instead of 3)."""
-    import torch
-    return torch._C._cuda_getCurrentRawStream(index)
-
-
 def cur_stream() -> int:
     import torch
     return torch.cuda.current_stream().cuda_stream
