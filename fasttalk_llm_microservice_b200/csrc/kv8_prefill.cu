@@ -157,29 +157,28 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
         const int chunk = (p.n_req + 31) / 32;
         const int r0 = min(p.n_req, lane * chunk), r1 = min(p.n_req, r0 + chunk);
         Kv8Walk w;
-        long long mine = 0, units = 0;
-        int most = 0;
+        int mine = 0, units = 0, most = 0;
         for (int r = r0; r < r1; ++r) {
             w.q.load(p, r);
             mine += w.q.all(p);
             units += w.q.tiles;
             if (w.q.tiles) most = max(most, max(w.q.steps(p, w.q.tiles - 1), w.q.tiles > 1 ? w.q.steps(p, w.q.tiles - 2) : 0));
         }
-        long long b_steps = mine, b_units = units;
+        int b_steps = mine, b_units = units;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long x = __shfl_up_sync(0xffffffffu, b_steps, o), y = __shfl_up_sync(0xffffffffu, b_units, o);
+            const int x = __shfl_up_sync(0xffffffffu, b_steps, o), y = __shfl_up_sync(0xffffffffu, b_units, o);
             if (lane >= o) b_steps += x, b_units += y;
         }
         most = __reduce_max_sync(0xffffffffu, most);
-        const long long total = __shfl_sync(0xffffffffu, b_steps, 31) * p.nkv, n_units = __shfl_sync(0xffffffffu, b_units, 31) * p.nkv;
+        const int total = __shfl_sync(0xffffffffu, b_steps, 31) * p.nkv, n_units = __shfl_sync(0xffffffffu, b_units, 31) * p.nkv, ctas = gridDim.x;
         b_steps -= mine;
         b_units -= units;
-        const long long per = kv8_div(total + gridDim.x - 1, gridDim.x);
-        const bool whole = p.split == nullptr || (n_units <= gridDim.x && most + kKv8Start <= per + K8P_WHOLE);      // (no room for parts: the host knows that there are none)
+        const int per = (unsigned)(total + ctas - 1) / (unsigned)ctas;
+        const bool whole = p.split == nullptr || (n_units <= ctas && most + kKv8Start <= per + K8P_WHOLE);      // (no room for parts: the host knows that there are none)
         // the flat list is one of units or of steps
-        const long long len = whole ? n_units : total, each = whole ? 1 : per, at0 = whole ? b_units : b_steps;
-        w.f = min(len, each * blockIdx.x);
+        const int len = whole ? n_units : total, each = whole ? 1 : per, at0 = whole ? b_units : b_steps;
+        w.f = min(len, each * (int)blockIdx.x);
         w.f_end = min(len, w.f + each);
         const bool work = w.f < w.f_end;
         if (work ? at0 * p.nkv <= w.f && w.f < (at0 + (whole ? units : mine)) * p.nkv : lane == 0) {      // one lane
@@ -642,26 +641,27 @@ kv8_prefill_merge_kernel(const __grid_constant__ Kv8Prompt p) {
 #pragma unroll
         for (int k = 0; k < 16; ++k) acc[k] = 0.f;
         const int first = alone ? 0 : warp, stride = alone ? 1 : K8P_MERGE_WARPS;
-        for (int x0 = first; x0 < np; x0 += 2 * stride) {
-            float2 ml[2];
-            float4 o[2][4];
+        for (int x0 = first; x0 < np; x0 += 4 * stride) {
+            float2 ml[4];
+            float4 o[4][4];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {                            // two parts asked for at once
+            for (int k = 0; k < 4; ++k) {                            // four parts asked for at once
                 const int x = min(x0 + k * stride, np - 1);
                 const float4* part = reinterpret_cast<const float4*>(p.parts + (2 * (size_t)(blockIdx.x + x / subs) + (x < subs)) * C::PART);
                 const int rr = r + (x % subs) * K8P_ROWS;
+                const bool on = valid && x0 + k * stride < np;
                 ml[k] = make_float2(-INFINITY, 0.f);
-                if (valid && x0 + k * stride < np) ml[k] = reinterpret_cast<const float2*>(part + (size_t)(D / 4) * (2 * K8P_ROWS))[rr];
+                if (on) ml[k] = reinterpret_cast<const float2*>(part + (size_t)(D / 4) * (2 * K8P_ROWS))[rr];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[k][e] = valid ? part[(size_t)(4 * c + e) * (2 * K8P_ROWS) + rr] : make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int e = 0; e < 4; ++e) o[k][e] = on ? part[(size_t)(4 * c + e) * (2 * K8P_ROWS) + rr] : make_float4(0.f, 0.f, 0.f, 0.f);
             }
-            const float Mn = fmaxf(M, fmaxf(ml[0].x, ml[1].x));
+            const float Mn = fmaxf(M, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)));
             const float keep = M == -INFINITY ? 0.f : exp2f(M - Mn);
             L *= keep;
 #pragma unroll
             for (int k = 0; k < 16; ++k) acc[k] *= keep;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
+            for (int k = 0; k < 4; ++k) {
                 const float z = ml[k].x == -INFINITY ? 0.f : exp2f(ml[k].x - Mn);
                 L = fmaf(ml[k].y, z, L);
 #pragma unroll
@@ -759,6 +759,9 @@ extern "C" int ft_attn_prefill_kv8(const void* q, const void* kv8_layer, int num
     FT_REQUIRE(nq >= 1 && nkv >= 1 && nq % nkv == 0 && nq / nkv <= K8P_GROUP, "ft_attn_prefill_kv8: GQA group %d/%d not supported", nq, nkv);
     FT_REQUIRE(T >= 0 && n_req >= 0 && table_rows >= 0 && max_pages >= 0 && num_pages >= 0 && (long long)max_pages * kKvTile + T <= INT32_MAX - 64,
                "ft_attn_prefill_kv8: bad sizes T=%d n_req=%d nkv=%d table %d x %d, %d pages", T, n_req, nkv, table_rows, max_pages, num_pages);
+    // the work's list: at most so many tiles of at most so many pages, and what the shares are rounded up by
+    FT_REQUIRE(((double)T / (2 * (K8P_ROWS / (nq / nkv))) + n_req) * ((double)max_pages + T / kKvTile + 2 + kKv8Start) * nkv + 4096 <= INT32_MAX,
+               "ft_attn_prefill_kv8: %d tokens of %d requests over %d pages are more than one call takes", T, n_req, max_pages);
     if (T == 0) return 0;
     FT_REQUIRE(q && kv8_layer && out && (n_req == 0 || (page_table && req_q_start && req_slot && req_pos0)), "ft_attn_prefill_kv8: null argument");
     FT_REQUIRE(((uintptr_t)q | (uintptr_t)kv8_layer | (uintptr_t)out | (uintptr_t)out_lo | (uintptr_t)scratch) % 16 == 0, "ft_attn_prefill_kv8: tensors on 16 bytes");

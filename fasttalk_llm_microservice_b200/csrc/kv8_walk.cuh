@@ -21,12 +21,12 @@ struct Kv8Prompt {
     float scale_log2;
 };
 
-// sum over i < n of floor((a i + b) / 64): the lattice points below a line, by Euclid's steps.  Only the first has a large constant; all divisions are of 32 bits (a <= 256, n <= 2^22)
-__host__ __device__ inline long long floor_sum64(unsigned n, unsigned a, unsigned b) {
-    unsigned m = 64;
-    unsigned long long sum = 0;
+// The flat list's length fits 31 bits (the host has seen to it), so do all sums and differences along it.
+// sum over i < n of floor((a i + b) / 64): the lattice points below a line, by Euclid's steps.  Each term is a part of the result (or wraps and is multiplied by 0)
+__host__ __device__ inline int floor_sum64(unsigned n, unsigned a, unsigned b) {
+    unsigned m = 64, sum = 0;
     while (n > 0) {
-        sum += (unsigned long long)n * (n - 1) / 2 * (a / m) + (unsigned long long)n * (b / m);
+        sum += (n & 1 ? (n - 1) / 2 * n : n / 2 * (n - 1)) * (a / m) + n * (b / m);
         a %= m;
         b %= m;
         const unsigned top = a * n + b;
@@ -36,16 +36,11 @@ __host__ __device__ inline long long floor_sum64(unsigned n, unsigned a, unsigne
         a = m;
         m = t;
     }
-    return (long long)sum;
+    return (int)sum;
 }
 
 // What a unit costs beyond its pages, in pages: it takes that much more of the flat list, behind its last step
 constexpr int kKv8Start = 3;
-
-// a / b, most often of numbers below 2^32
-__host__ __device__ inline long long kv8_div(long long a, long long b) {
-    return ((unsigned long long)a | (unsigned long long)b) >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b);
-}
 
 // one request: its rows of q, tiles of 2 th tokens, steps of its tiles
 struct Kv8Request {
@@ -63,8 +58,8 @@ struct Kv8Request {
         const int n = pages(p, i);
         return tokens(p, i) <= p.th ? (n + p.few_pages - 1) / p.few_pages : n;
     }
-    __host__ __device__ __forceinline__ long long before(const Kv8Prompt& p, int i) const { return floor_sum64(i, 2 * p.th, pos0 + 2 * p.th - 1) + i * (1LL + kKv8Start); }   // lengths of the full tiles 0 .. i - 1
-    __host__ __device__ __forceinline__ long long all(const Kv8Prompt& p) const { return tiles ? before(p, tiles - 1) + steps(p, tiles - 1) + kKv8Start : 0; }
+    __host__ __device__ __forceinline__ int before(const Kv8Prompt& p, int i) const { return floor_sum64(i, 2 * p.th, pos0 + 2 * p.th - 1) + i * (1 + kKv8Start); }   // lengths of the full tiles 0 .. i - 1
+    __host__ __device__ __forceinline__ int all(const Kv8Prompt& p) const { return tiles ? before(p, tiles - 1) + steps(p, tiles - 1) + kKv8Start : 0; }
 };
 
 // A stretch of pages of one unit.  parts: 0 = it is the whole unit; else, where the unit begins, how many shares it lies in
@@ -73,7 +68,7 @@ struct Kv8Stretch { int page0, pages, few, row0, tokens, pos0, head, slot, begin
 // A CTA's share, walked stretch by stretch; a stretch = steps t0 .. t1 - 1 of one unit
 struct Kv8Walk {
     Kv8Request q;
-    long long f, f_end, first;                                       // where it is in the flat list; where the unit begins
+    int f, f_end, first;                                       // where it is in the flat list; where the unit begins
     int r, h, i, t, t0, t1, n_steps, n_pages, n_tok;
     bool few;
     __host__ __device__ __forceinline__ void unit(const Kv8Prompt& p) {
@@ -97,7 +92,7 @@ struct Kv8Walk {
                 }
                 unit(p);
             }
-            const int take = (int)min(f_end - f, (long long)(n_steps + kKv8Start - t));
+            const int take = min(f_end - f, n_steps + kKv8Start - t);
             first = f - t;
             t0 = min(t, n_steps);
             t1 = min(t + take, n_steps);
@@ -107,28 +102,28 @@ struct Kv8Walk {
         }
     }
     // where step (or, where each CTA takes whole units, unit) `at` of the flat list lies; `before` of them belong to requests ahead of r0, and it is r0's or a later one's
-    __host__ __device__ inline void seek(const Kv8Prompt& p, bool whole, int r0, long long before, long long at) {
+    __host__ __device__ inline void seek(const Kv8Prompt& p, bool whole, int r0, int before, int at) {
         for (r = r0;; ++r) {
             q.load(p, r);
-            const long long n = whole ? q.tiles : q.all(p);
+            const int n = whole ? q.tiles : q.all(p);
             if (at < (before + n) * p.nkv) {
-                long long rest = at - before * p.nkv;
-                h = (int)kv8_div(rest, n);
+                int rest = at - before * p.nkv;
+                h = (int)((unsigned)rest / (unsigned)n);
                 rest -= h * n;
                 int lo = 0, hi = q.tiles - 1;                        // the last tile that begins at or before rest
                 while (!whole && lo < hi) {
                     const int mid = (lo + hi + 1) >> 1;
                     if (q.before(p, mid) <= rest) lo = mid; else hi = mid - 1;
                 }
-                i = whole ? (int)rest : lo;
-                t = whole ? 0 : (int)(rest - q.before(p, lo));
+                i = whole ? rest : lo;
+                t = whole ? 0 : rest - q.before(p, lo);
                 return;
             }
             before += n;
         }
     }
     // the stretch as the other warps get it; per: steps of a share
-    __host__ __device__ inline Kv8Stretch stretch(const Kv8Prompt& p, long long per, int share) const {
+    __host__ __device__ inline Kv8Stretch stretch(const Kv8Prompt& p, int per, int share) const {
         Kv8Stretch s;
         s.page0 = page0(p.few_pages);
         s.pages = page1(p.few_pages) - s.page0;
@@ -139,7 +134,7 @@ struct Kv8Walk {
         s.head = h;
         s.slot = q.slot;
         s.begins = t0 == 0;
-        s.parts = t0 == 0 && t1 == n_steps ? 0 : t0 == 0 ? (int)kv8_div(first + n_steps - 1, per) - share + 1 : 1;
+        s.parts = t0 == 0 && t1 == n_steps ? 0 : t0 == 0 ? (int)((unsigned)(first + n_steps - 1) / (unsigned)per) - share + 1 : 1;
         return s;
     }
     // pages of the stretch, in the order in which they are asked for
