@@ -366,29 +366,30 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                 const float* scales = reinterpret_cast<const float*>(rec + Kv8<D>::SCALES);
                 // a block of zeros keeps a factor above 0, so that hidden scores stay minus infinity
                 if (ct < 4) kscale_s[s16][ct] = there ? fmaxf(scales[ct] * p.scale_log2, 1e-37f) : -1.f;
+                if (there) {
 #pragma unroll
-                for (int u = ct; u < kKvTile * D / 16; u += K8P_CONV) {      // keys: 16 codes, two chunks of the swizzled row
-                    const int piece = u >> 8, t = u >> 2 & 63, c = u & 3;
-                    uint4 x = *reinterpret_cast<const uint4*>(rec + u * 16);
-                    if (!there) x = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-                    uint8_t* at = dst + piece * K8P_PIECE + t * 128;
-                    *reinterpret_cast<uint4*>(at + ((2 * c) ^ (t & 7)) * 16) = make_uint4(kv8_lo(x.x), kv8_hi(x.x), kv8_lo(x.y), kv8_hi(x.y));
-                    *reinterpret_cast<uint4*>(at + ((2 * c + 1) ^ (t & 7)) * 16) = make_uint4(kv8_lo(x.z), kv8_hi(x.z), kv8_lo(x.w), kv8_hi(x.w));
-                }
-                dst += KH * K8P_PIECE;
+                    for (int u = ct; u < kKvTile * D / 16; u += K8P_CONV) {  // keys: 16 codes, two chunks of the swizzled row
+                        const int piece = u >> 8, t = u >> 2 & 63, c = u & 3;
+                        const uint4 x = *reinterpret_cast<const uint4*>(rec + u * 16);
+                        uint8_t* at = dst + piece * K8P_PIECE + t * 128;
+                        *reinterpret_cast<uint4*>(at + ((2 * c) ^ (t & 7)) * 16) = make_uint4(kv8_lo(x.x), kv8_hi(x.x), kv8_lo(x.y), kv8_hi(x.y));
+                        *reinterpret_cast<uint4*>(at + ((2 * c + 1) ^ (t & 7)) * 16) = make_uint4(kv8_lo(x.z), kv8_hi(x.z), kv8_lo(x.w), kv8_hi(x.w));
+                    }
 #pragma unroll
-                for (int u = ct; u < kKvTile * D / 16; u += K8P_CONV) {      // values, by where they lie
-                    const int piece = u >> 8, slot = u >> 2 & 63, t = slot ^ (slot >> 1 & 1), c = (u & 3) ^ (t >> 1 & 2);
-                    uint4 x = *reinterpret_cast<const uint4*>(rec + Kv8<D>::SLAB + u * 16);
-                    if (!there) x = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-                    const __half2 f = __float2half2_rn(there ? scales[4 + (t >> 4)] * vinv : 0.f);
-                    auto mul = [&](uint32_t y) {
-                        const __half2 z = __hmul2(*reinterpret_cast<const __half2*>(&y), f);
-                        return *reinterpret_cast<const uint32_t*>(&z);
-                    };
-                    uint8_t* at = dst + piece * K8P_PIECE + t * 128;
-                    *reinterpret_cast<uint4*>(at + ((2 * c) ^ (t & 7)) * 16) = make_uint4(mul(kv8_lo(x.x)), mul(kv8_hi(x.x)), mul(kv8_lo(x.y)), mul(kv8_hi(x.y)));
-                    *reinterpret_cast<uint4*>(at + ((2 * c + 1) ^ (t & 7)) * 16) = make_uint4(mul(kv8_lo(x.z)), mul(kv8_hi(x.z)), mul(kv8_lo(x.w)), mul(kv8_hi(x.w)));
+                    for (int u = ct; u < kKvTile * D / 16; u += K8P_CONV) {  // values, by where they lie
+                        const int piece = u >> 8, slot = u >> 2 & 63, t = slot ^ (slot >> 1 & 1), c = (u & 3) ^ (t >> 1 & 2);
+                        const uint4 x = *reinterpret_cast<const uint4*>(rec + Kv8<D>::SLAB + u * 16);
+                        const __half2 f = __float2half2_rn(scales[4 + (t >> 4)] * vinv);
+                        auto mul = [&](uint32_t y) {
+                            const __half2 z = __hmul2(*reinterpret_cast<const __half2*>(&y), f);
+                            return *reinterpret_cast<const uint32_t*>(&z);
+                        };
+                        uint8_t* at = dst + (KH + piece) * K8P_PIECE + t * 128;
+                        *reinterpret_cast<uint4*>(at + ((2 * c) ^ (t & 7)) * 16) = make_uint4(mul(kv8_lo(x.x)), mul(kv8_hi(x.x)), mul(kv8_lo(x.y)), mul(kv8_hi(x.y)));
+                        *reinterpret_cast<uint4*>(at + ((2 * c + 1) ^ (t & 7)) * 16) = make_uint4(mul(kv8_lo(x.z)), mul(kv8_hi(x.z)), mul(kv8_lo(x.w)), mul(kv8_hi(x.w)));
+                    }
+                } else {                                                     // hidden probabilities are zeros, and so must be what they are multiplied by
+                    for (int u = ct; u < C::TILE / 16; u += K8P_CONV) *reinterpret_cast<uint4*>(dst + u * 16) = make_uint4(0u, 0u, 0u, 0u);
                 }
                 fence_proxy_async();
                 __syncwarp();
