@@ -71,6 +71,7 @@ kv8_append_kernel(const Kv8Append p, int kv_rows, int kv_ctas) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int sub = lane % LR, rsub = lane / LR;
     const int angles = min(p.n_angles, p.max_pages * kKvTile);
+    pdl_wait();
     const size_t width = (size_t)(p.nq + 2 * p.nkv) * D;
 
     if ((int)blockIdx.x >= kv_ctas) {
@@ -209,6 +210,7 @@ kv8_read_kernel(const uint8_t* __restrict__ cache, const int* __restrict__ page_
                 const int* __restrict__ req_start, const int* __restrict__ req_slot, const int* __restrict__ req_pos0, int n_req, int rows, int nkv,
                 uint8_t* __restrict__ k_out, uint8_t* __restrict__ v_out) {
     __shared__ int s_page[K8_READ_ROWS], s_tok[K8_READ_ROWS];
+    pdl_wait();
     const int row0 = blockIdx.x * K8_READ_ROWS;
     if (threadIdx.x < 32) {
         // lane i: row i; its request is the last that starts at or before it
@@ -301,9 +303,7 @@ extern "C" int ft_rope_kv8_append(const float* qkv, int n_splits, long long spli
     const long long q_tasks = (long long)T * ((nq + K8_QHEADS - 1) / K8_QHEADS), q_ctas = (q_tasks + K8_WARPS - 1) / K8_WARPS;
     FT_REQUIRE(q_tasks <= INT32_MAX && kv_ctas + q_ctas <= INT32_MAX, "ft_rope_kv8_append: %d tokens of %d + %d heads", T, nq, nkv);
     const int grid = (int)(kv_ctas + q_ctas);
-    if (d == 64) kv8_append_kernel<64><<<grid, K8_WARPS * 32, 0, (cudaStream_t)stream>>>(p, (int)kv_rows, (int)kv_ctas);
-    else kv8_append_kernel<128><<<grid, K8_WARPS * 32, 0, (cudaStream_t)stream>>>(p, (int)kv_rows, (int)kv_ctas);
-    FT_CHECK_CUDA(cudaGetLastError());
+    FT_CHECK_CUDA(launch_after(d == 64 ? kv8_append_kernel<64> : kv8_append_kernel<128>, dim3(grid), dim3(K8_WARPS * 32), 0, (cudaStream_t)stream, p, (int)kv_rows, (int)kv_ctas));
     return 0;
 }
 
@@ -319,12 +319,7 @@ extern "C" int ft_kv8_read(const void* kv8_layer, int num_pages, const int* page
     const long long tasks = (long long)nkv * 2 * K8_READ_ROWS * (d / 16), per = K8_READ_TASKS * K8_READ_THREADS;
     FT_REQUIRE((tasks + per - 1) / per <= 65535, "ft_kv8_read: %d heads", nkv);
     const dim3 grid((rows + K8_READ_ROWS - 1) / K8_READ_ROWS, (unsigned)((tasks + per - 1) / per));
-    auto go = [&](auto kernel) {
-        kernel<<<grid, K8_READ_THREADS, 0, (cudaStream_t)stream>>>((const uint8_t*)kv8_layer, page_table, table_rows, max_pages, num_pages, req_start, req_slot, req_pos0,
-                                                                   n_req, rows, nkv, (uint8_t*)k_out, (uint8_t*)v_out);
-    };
-    if (d == 64) go(kv8_read_kernel<64>);
-    else go(kv8_read_kernel<128>);
-    FT_CHECK_CUDA(cudaGetLastError());
+    FT_CHECK_CUDA(launch_after(d == 64 ? kv8_read_kernel<64> : kv8_read_kernel<128>, grid, dim3(K8_READ_THREADS), 0, (cudaStream_t)stream, (const uint8_t*)kv8_layer,
+                               page_table, table_rows, max_pages, num_pages, req_start, req_slot, req_pos0, n_req, rows, nkv, (uint8_t*)k_out, (uint8_t*)v_out));
     return 0;
 }

@@ -36,6 +36,7 @@ struct K8Decode {
 };
 
 __global__ void kv8_decode_zero_kernel(int* counters, int n) {
+    pdl_wait();                                      // what was in the stream before is done: the kernel behind this one need not wait for it again
     pdl_launch_dependents();
     for (int i = threadIdx.x; i < n; i += blockDim.x) counters[i] = 0;
 }
@@ -64,6 +65,7 @@ kv8_decode_kernel(const __half* __restrict__ q, const uint8_t* __restrict__ cach
         fence_mbar_init();
         dead = 0;
     }
+    if (parts == nullptr) pdl_wait();                                        // nothing of this call's ran before
     auto ctx_of = [&](int b) { return max(0, min(ctx_lens[b], max_pages * kKvTile)); };
     auto pages_of = [&](int b) { return (ctx_of(b) + kKvTile - 1) / kKvTile; };
 
@@ -333,14 +335,12 @@ static int launch_kv8_decode(const void* q, const void* cache, int num_pages, co
     float* parts = whole ? nullptr : (float*)scratch + kv8_decode_counters(ctas);
     const float scale_log2 = K8D_LOG2E / sqrtf((float)D);
     if (whole) {
-        kv8_decode_kernel<D><<<B * nkv, C::THREADS, C::SMEM, st>>>((const __half*)q, (const uint8_t*)cache, num_pages, page_table, max_pages, ctx_lens,
-                                                                   (__nv_bfloat16*)out, (__nv_bfloat16*)out_lo, counters, parts, B, nq, nkv, scale_log2);
-        FT_CHECK_CUDA(cudaGetLastError());
+        FT_CHECK_CUDA(launch_after(kv8_decode_kernel<D>, dim3(B * nkv), dim3(C::THREADS), C::SMEM, st, (const __half*)q, (const uint8_t*)cache, num_pages, page_table,
+                                   max_pages, ctx_lens, (__nv_bfloat16*)out, (__nv_bfloat16*)out_lo, counters, parts, B, nq, nkv, scale_log2));
         return 0;
     }
-    kv8_decode_zero_kernel<<<1, 128, 0, st>>>(counters, ctas);
-    FT_CHECK_CUDA(cudaGetLastError());
-    // starts beside the zeroes; what was in the stream before them is done by then
+    FT_CHECK_CUDA(launch_after(kv8_decode_zero_kernel, dim3(1), dim3(128), 0, st, counters, ctas));
+    // starts beside the zeroes, for which it waits when it has its first part ready
     FT_CHECK_CUDA(launch_after(kv8_decode_kernel<D>, dim3(ctas), dim3(C::THREADS), C::SMEM, st, (const __half*)q, (const uint8_t*)cache, num_pages, page_table,
                                max_pages, ctx_lens, (__nv_bfloat16*)out, (__nv_bfloat16*)out_lo, counters, parts, B, nq, nkv, scale_log2));
     return 0;

@@ -136,6 +136,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
+    pdl_wait();
     bool ok = true;                                                          // false: a wait ran out
     // the n-th stretch of the share, or one without pages behind the last; and this warp's word that it has done with it
     auto hear = [&](int n) {
@@ -733,8 +734,7 @@ static int launch_kv8_prefill(Kv8Prompt& p, void* scratch, cudaStream_t st) {
     FT_REQUIRE(!parts || scratch, "ft_attn_prefill_kv8: needs ft_attn_prefill_kv8_scratch_bytes of work memory");
     p.split = parts ? (Kv8Split*)scratch : nullptr;
     p.parts = (float*)scratch + kv8_prefill_splits(ctas);
-    kv8_prefill_kernel<D><<<ctas, K8P_THREADS, C::SMEM, st>>>(p);
-    FT_CHECK_CUDA(cudaGetLastError());
+    FT_CHECK_CUDA(launch_after(kv8_prefill_kernel<D>, dim3(ctas), dim3(K8P_THREADS), C::SMEM, st, (const Kv8Prompt&)p));
     if (parts) FT_CHECK_CUDA(launch_after(kv8_prefill_merge_kernel<D>, dim3(ctas, D / 16), dim3(K8P_MERGE_WARPS * 32), 0, st, (const Kv8Prompt&)p));
     return 0;
 }
