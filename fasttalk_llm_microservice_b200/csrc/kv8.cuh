@@ -79,7 +79,8 @@ struct Kv8Query {
     }
     // the first n (1 .. 64) tokens of the page at rec
     __device__ __forceinline__ void page(const uint8_t* rec, int n, float scale_log2, int g, int tq) {
-        const float4 k4 = *reinterpret_cast<const float4*>(rec + Kv8<D>::SCALES), vs = *reinterpret_cast<const float4*>(rec + Kv8<D>::SCALES + 16);
+        const float4 k4 = *reinterpret_cast<const float4*>(rec + Kv8<D>::SCALES);
+        float4 vs = *reinterpret_cast<const float4*>(rec + Kv8<D>::SCALES + 16);
         const float ks[4] = {k4.x * scale_log2, k4.y * scale_log2, k4.z * scale_log2, k4.w * scale_log2};
         float s[4][4], most[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -99,6 +100,10 @@ struct Kv8Query {
             for (int b = 0; b < 4; ++b)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[b][e] = 16 * b + 8 * (e >> 1) + g < n ? s[b][e] : -INFINITY;
+            // blocks behind the last token: whatever their scales are, nothing comes of it (the keys' meets minus infinity alone)
+            if (n <= 16) vs.y = 0.f;
+            if (n <= 32) vs.z = 0.f;
+            if (n <= 48) vs.w = 0.f;
         }
 #pragma unroll
         for (int b = 0; b < 4; ++b) {

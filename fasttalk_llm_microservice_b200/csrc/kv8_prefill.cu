@@ -29,7 +29,7 @@ namespace ft {
 constexpr int K8P_THREADS = 640;
 constexpr int K8P_REGS = 96, K8P_REGS_ISSUE = 64, K8P_REGS_SOFT = 144, K8P_REGS_CONV = 64;
 static_assert(K8P_REGS_ISSUE + 2 * K8P_REGS_SOFT + 2 * K8P_REGS_CONV <= 5 * K8P_REGS, "what the block is launched with");
-constexpr int K8P_SOFT = 256, K8P_CONV = 256;
+constexpr int K8P_SOFT = 256, K8P_CONV = 256;    // (256: four threads a row of a piece)
 constexpr int K8P_LISTENERS = 19;                // warps that hear of a stretch: all but the one that tells
 constexpr int K8P_ROWS = 128;                    // rows of a half
 constexpr int K8P_GROUP = 8;                     // query heads a key head at most
@@ -75,9 +75,21 @@ __device__ __forceinline__ void tmem_arrived(uint32_t* r) {
     for (int c = 0; c < N; c += 8)
         asm volatile("" : "+r"(r[c]), "+r"(r[c + 1]), "+r"(r[c + 2]), "+r"(r[c + 3]), "+r"(r[c + 4]), "+r"(r[c + 5]), "+r"(r[c + 6]), "+r"(r[c + 7]));
 }
+// Waits that end, as those of common.cuh do, but a few instructions each: this kernel has some twenty of them among five kinds of warps, and its time hangs on what the
+// instruction caches hold (unrolled, they and the rest were 104 KB, and 16 KB more or less of waits outside the loops over pages was 8 % of its time)
+__device__ __forceinline__ bool small_mbar_wait_limited(uint64_t* bar, uint32_t parity, volatile int* dead, int limit = kWaitLimit) {
+#pragma unroll 1
+    for (int i = 0; i < limit; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*dead) return false;
+    }
+    *dead = 1;
+    return false;
+}
+constexpr int kStretchLimit = 64 * kWaitLimit;   // a stretch may be a million keys
 // A warp's wait (all lanes ask, so that the warp stays together)
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
-    return __all_sync(0xffffffffu, mbar_wait_limited(bar, parity, dead));
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* dead, int limit = kWaitLimit) {
+    return __all_sync(0xffffffffu, small_mbar_wait_limited(bar, parity, dead, limit));
 }
 
 __device__ int g_kv8_prefill_waits;              // 1: a wait ran out on this device (ft_kv8_waits)
@@ -104,7 +116,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
     __shared__ Kv8Stretch told[4];
     __shared__ unsigned vmax_s[4];                                           // bits of a number that is not negative: they order as it does
     __shared__ __align__(16) float kscale_s[C::S16][4];                      // times scale_log2; the first below 0: the page is not there
-    __shared__ int there_s[C::S8];
+    __shared__ int blocks_s[C::S8];                                          // of 16 tokens, that some query of the unit sees; 0: the page is not there
     __shared__ float2 ml_s[K8P_SOFT];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int dead;
@@ -140,7 +152,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
     bool ok = true;                                                          // false: a wait ran out
     // the n-th stretch of the share, or one without pages behind the last; and this warp's word that it has done with it
     auto hear = [&](int n) {
-        ok = ok && warp_wait(&seg_full[n & 3], n >> 2 & 1, &dead);
+        ok = ok && warp_wait(&seg_full[n & 3], n >> 2 & 1, &dead, kStretchLimit);
         Kv8Stretch w = told[n & 3];
         if (!ok) w.pages = 0;
         return w;
@@ -159,8 +171,11 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
         const int r0 = min(p.n_req, lane * chunk), r1 = min(p.n_req, r0 + chunk);
         Kv8Walk w;
         int mine = 0, units = 0, most = 0;
+        bool grows = true;                                                   // a list that does not is not walked: its sums could be any
+#pragma unroll 1
         for (int r = r0; r < r1; ++r) {
             w.q.load(p, r);
+            grows = grows && p.req_q_start[r] <= p.req_q_start[r + 1];
             mine += w.q.all(p);
             units += w.q.tiles;
             if (w.q.tiles) most = max(most, max(w.q.steps(p, w.q.tiles - 1), w.q.tiles > 1 ? w.q.steps(p, w.q.tiles - 2) : 0));
@@ -181,16 +196,17 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
         const int len = whole ? n_units : total, each = whole ? 1 : per, at0 = whole ? b_units : b_steps;
         w.f = min(len, each * (int)blockIdx.x);
         w.f_end = min(len, w.f + each);
-        const bool work = w.f < w.f_end;
+        const bool work = __all_sync(0xffffffffu, grows) && w.f < w.f_end;
         if (work ? at0 * p.nkv <= w.f && w.f < (at0 + (whole ? units : mine)) * p.nkv : lane == 0) {      // one lane
             if (work) {
                 w.seek(p, whole, r0, at0, w.f);
                 w.unit(p);
                 if (whole) w.f = 0, w.f_end = w.n_steps;
             }
+#pragma unroll 1
             for (int n = 0, more = 1; more; ++n) {
                 more = w.next(p);
-                if (!mbar_wait_limited(&seg_empty[n & 3], (n >> 2 & 1) ^ 1, &dead)) {
+                if (!small_mbar_wait_limited(&seg_empty[n & 3], (n >> 2 & 1) ^ 1, &dead, kStretchLimit)) {
                     *err = 1;
                     break;
                 }
@@ -206,25 +222,28 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
         const uint64_t pol = policy_evict_last();                            // read again by other tiles
         int it = 0, asked = 0;
         bool go = true;
+#pragma unroll 1
         for (int seg = 0;; ++seg) {
             const Kv8Stretch w = hear(seg);
             if (w.pages == 0) break;
             const int* pt = p.page_table + (size_t)w.slot * p.max_pages;
             const int most_here = w.slot >= 0 && w.slot < p.table_rows ? p.max_pages : 0;
             const int p1 = w.page0 + w.pages;
+#pragma unroll 1
             for (int p0 = w.page0; p0 < p1; p0 += 32) {
                 const int mine = p0 + lane;
                 const int my_page = mine < p1 && mine < most_here ? pt[mine] : -1;
                 const int n = min(32, p1 - p0);
+#pragma unroll 1
                 for (int k = 0; k < n; ++k, ++it) {
                     const int page = __shfl_sync(0xffffffffu, my_page, k);
                     if (lane == 0 && go) {
                         const int s = it % C::S8;
-                        go = mbar_wait_limited(&rec_empty[s], (it / C::S8 & 1) ^ 1, &dead);
+                        go = small_mbar_wait_limited(&rec_empty[s], (it / C::S8 & 1) ^ 1, &dead);
                         if (!go) continue;
                         asked = it + 1;
                         const bool there = page >= 0 && page < p.num_pages;
-                        there_s[s] = there;
+                        blocks_s[s] = there ? min(4, (w.pos0 + w.tokens - 1 - (p0 + k) * kKvTile) / kKv8Block + 1) : 0;
                         if (there) {
                             mbar_expect_tx(&rec_full[s], Kv8<D>::REC);
                             tma_bulk_g2s(smem + C::REC + s * Kv8<D>::REC, p.cache + ((size_t)page * p.nkv + w.head) * Kv8<D>::REC, Kv8<D>::REC, &rec_full[s], pol);
@@ -238,7 +257,9 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
         }
         if (lane == 0 && (!go || !ok || dead)) {                             // what is under way still lands in this CTA's memory
             *err = 1;
+#pragma unroll 1
             for (int i = max(0, asked - C::S8); i < asked; ++i)
+#pragma unroll 1
                 for (int k = 0; k < kWaitLimit && !mbar_try_wait(&rec_full[i % C::S8], i / C::S8 & 1); ++k) {}
         }
       } else {
@@ -252,8 +273,8 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
         int base = 0, n_qk = 0, n_pv = 0;                                    // pages of the share, products of this half so far
         auto issue_qk = [&](int page, int qh) {                              // page: counted over the whole share
             const int s = page % C::S16, buf = n_qk % C::NS;
-            if (C::NS == 1) ok = mbar_wait_limited(&s_free[h], (n_qk & 1) ^ 1, &dead);
-            ok = ok && mbar_wait_limited(&kv_full[s], page / C::S16 & 1, &dead);
+            if (C::NS == 1) ok = small_mbar_wait_limited(&s_free[h], (n_qk & 1) ^ 1, &dead);
+            ok = ok && small_mbar_wait_limited(&kv_full[s], page / C::S16 & 1, &dead);
             if (!ok) return;
             ++n_qk;
             tc_fence_after();
@@ -266,7 +287,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
         };
         auto issue_pv = [&](int page, bool first, bool alone) {
             const int s = page % C::S16, buf = n_pv & 1;
-            ok = mbar_wait_limited(&p_full[h][buf], n_pv >> 1 & 1, &dead);
+            ok = small_mbar_wait_limited(&p_full[h][buf], n_pv >> 1 & 1, &dead);
             if (!ok) return;
             ++n_pv;
             tc_fence_after();
@@ -277,18 +298,20 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
             umma_commit(&kv_empty[s]);
             if (alone) umma_commit(&kv_empty[s]);                            // the other half has no use for this page
         };
+#pragma unroll 1
         for (int seg = 0;; ++seg) {
             const Kv8Stretch w = hear(seg);
             if (w.pages == 0) break;
             const int mine_n = w.few ? (w.pages - h + 1) / 2 : w.pages;      // page i of this half is page j of the stretch
             auto page_of = [&](int i) { return base + (w.few ? h + 2 * i : i); };
             if (lead) {
-                ok = mbar_wait_limited(&q_full, seg & 1, &dead);
+                ok = small_mbar_wait_limited(&q_full, seg & 1, &dead);
                 tc_fence_after();
                 if (ok && mine_n == 0) umma_commit(&q_empty);
                 // Scores run NS pages ahead.  With two buffers page i + 2's follow the product that reads page i's probabilities, which says that page i's scores
                 // have been read; with one, page i + 1's follow the softmax's word that it has them in registers, ahead of that product.  Either way scores that are
                 // there mean that the product before the last is done, and the probabilities' buffer with it.
+#pragma unroll 1
                 for (int i = -C::NS; ok && i < mine_n; ++i) {
                     if (C::NS == 2 && i >= 0) issue_pv(page_of(i), i == 0, w.few);
                     if (ok && i + C::NS < mine_n) issue_qk(page_of(i + C::NS), w.few ? 0 : h);
@@ -303,6 +326,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
         if (!ok && lead) {                                                   // nothing may still run in tensor memory when it is given back
             *err = 1;
             umma_commit(&drained[h]);
+#pragma unroll 1
             for (int k = 0; k < kWaitLimit && !mbar_try_wait(&drained[h], 0); ++k) {}
         }
         __syncwarp();
@@ -312,9 +336,11 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(K8P_REGS_CONV));
         const int ct = tid - 128 - K8P_SOFT;
         int it = 0;
+#pragma unroll 1
         for (int seg = 0;; ++seg) {
             const Kv8Stretch w = hear(seg);
             if (w.pages == 0) break;
+#pragma unroll 1
             for (int step = 0; step < 2; ++step) {
                 if ((step == 0) == (seg == 0)) {
                     // the queries, 16 bytes at a time and all on their way at once; zeros for rows without a token
@@ -336,11 +362,13 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                     const int* pt = p.page_table + (size_t)w.slot * p.max_pages;
                     const int end = w.slot >= 0 && w.slot < p.table_rows ? min(w.page0 + w.pages, p.max_pages) : 0;
                     float vmax = 0.f;
+#pragma unroll 1
                     for (int k = w.page0 + ct; k < end; k += K8P_CONV) {
                         const int page = pt[k];
                         if (page < 0 || page >= p.num_pages) continue;
                         const float4 v = *reinterpret_cast<const float4*>(p.cache + ((size_t)page * p.nkv + w.head) * Kv8<D>::REC + Kv8<D>::SCALES + 16);
-                        vmax = fmaxf(vmax, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+                        const int seen = w.pos0 + w.tokens - 1 - k * kKvTile;        // blocks behind the last token do not count
+                        vmax = fmaxf(fmaxf(vmax, v.x), fmaxf(seen >= 16 ? v.y : 0.f, fmaxf(seen >= 32 ? v.z : 0.f, seen >= 48 ? v.w : 0.f)));
                     }
                     vmax = warp_max(vmax);
                     if (lane == 0) {
@@ -357,17 +385,20 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                 ok = warp_wait(&vmax_full, seg & 1, &dead);
             }
             const float vmax = __uint_as_float(vmax_s[seg & 3]), vinv = vmax > 0.f ? 1.f / vmax : 0.f;
+#pragma unroll 1
             for (int k = 0; ok && k < w.pages; ++k, ++it) {
                 const int s8 = it % C::S8, s16 = it % C::S16;
                 ok = warp_wait(&rec_full[s8], it / C::S8 & 1, &dead) && warp_wait(&kv_empty[s16], (it / C::S16 & 1) ^ 1, &dead);
                 if (!ok) break;
                 const uint8_t* rec = smem + C::REC + s8 * Kv8<D>::REC;
                 uint8_t* dst = smem + C::KV + s16 * C::TILE;
-                const bool there = there_s[s8];
+                const int blocks = blocks_s[s8];
                 const float* scales = reinterpret_cast<const float*>(rec + Kv8<D>::SCALES);
                 // a block of zeros keeps a factor above 0, so that hidden scores stay minus infinity
-                if (ct < 4) kscale_s[s16][ct] = there ? fmaxf(scales[ct] * p.scale_log2, 1e-37f) : -1.f;
-                if (there) {
+                if (ct < 4) kscale_s[s16][ct] = blocks ? fmaxf(scales[ct] * p.scale_log2, 1e-37f) : -1.f;
+                if (blocks) {
+                    // a thread's tokens are of one block; of one behind the last token, whatever its scale is, nothing comes
+                    const __half2 f = __float2half2_rn(ct >> 6 < blocks ? scales[4 + (ct >> 6)] * vinv : 0.f);
 #pragma unroll
                     for (int u = ct; u < kKvTile * D / 16; u += K8P_CONV) {  // keys: 16 codes, two chunks of the swizzled row
                         const int piece = u >> 8, t = u >> 2 & 63, c = u & 3;
@@ -380,7 +411,6 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                     for (int u = ct; u < kKvTile * D / 16; u += K8P_CONV) {  // values, by where they lie
                         const int piece = u >> 8, slot = u >> 2 & 63, t = slot ^ (slot >> 1 & 1), c = (u & 3) ^ (t >> 1 & 2);
                         const uint4 x = *reinterpret_cast<const uint4*>(rec + Kv8<D>::SLAB + u * 16);
-                        const __half2 f = __float2half2_rn(scales[4 + (t >> 4)] * vinv);
                         auto mul = [&](uint32_t y) {
                             const __half2 z = __hmul2(*reinterpret_cast<const __half2*>(&y), f);
                             return *reinterpret_cast<const uint32_t*>(&z);
@@ -390,6 +420,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                         *reinterpret_cast<uint4*>(at + ((2 * c + 1) ^ (t & 7)) * 16) = make_uint4(mul(kv8_lo(x.z)), mul(kv8_hi(x.z)), mul(kv8_lo(x.w)), mul(kv8_hi(x.w)));
                     }
                 } else {                                                     // hidden probabilities are zeros, and so must be what they are multiplied by
+#pragma unroll 1
                     for (int u = ct; u < C::TILE / 16; u += K8P_CONV) *reinterpret_cast<uint4*>(dst + u * 16) = make_uint4(0u, 0u, 0u, 0u);
                 }
                 fence_proxy_async();
@@ -412,8 +443,10 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
         {
             const int a = p.n_req ? max(0, min(p.req_q_start[0], p.T)) : p.T, b = p.n_req ? max(a, min(p.req_q_start[p.n_req], p.T)) : p.T;
             const int n = a + p.T - b;
+#pragma unroll 1
             for (int i = blockIdx.x; i < n; i += gridDim.x) {
                 const size_t at = (size_t)(i < a ? i : b + i - a) * p.nq * D;
+#pragma unroll 1
                 for (int e = 8 * st; e < p.nq * D; e += 8 * K8P_SOFT) {
                     *reinterpret_cast<uint4*>(p.out + at + e) = make_uint4(0u, 0u, 0u, 0u);
                     if (p.out_lo) *reinterpret_cast<uint4*>(p.out_lo + at + e) = make_uint4(0u, 0u, 0u, 0u);
@@ -435,6 +468,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
             return most;
         };
         int base = 0, cnt = 0, met = 0;                                      // pages of the share, pages of this half so far; meetings of the halves
+#pragma unroll 1
         for (int seg = 0;; ++seg) {
             const Kv8Stretch w = hear(seg);
             if (w.pages == 0) break;
@@ -443,6 +477,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
             const bool valid = tok < p.th && my_tok < w.tokens;
             float m_ref = -INFINITY, l_run = 0.f;                            // in log2 units
             int it = base + (w.few ? h : 0), ahead = w.pos0 + my_tok - (w.page0 + (w.few ? h : 0)) * kKvTile;     // page of the share; the row's position from the page's first key on
+#pragma unroll 1
             for (int i = 0; i < mine_n; ++i, ++cnt) {
                 const int sb = cnt % C::NS, pb = cnt & 1;
                 ok = ok && warp_wait(&s_full[h][sb], cnt / C::NS & 1, &dead);
@@ -473,6 +508,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                 bool known = i == 0;
                 if (known) m_ref = largest(sr, ks);
                 f32x2 sum[2];
+#pragma unroll 1
                 for (;;) {
                     const float mu = m_ref == -INFINITY ? 0.f : m_ref;
                     const f32x2 minus = pack2(-mu, -mu);

@@ -25,6 +25,7 @@ struct Kv8Prompt {
 // sum over i < n of floor((a i + b) / 64): the lattice points below a line, by Euclid's steps.  Each term is a part of the result (or wraps and is multiplied by 0)
 __host__ __device__ inline int floor_sum64(unsigned n, unsigned a, unsigned b) {
     unsigned m = 64, sum = 0;
+#pragma unroll 1
     while (n > 0) {
         sum += (n & 1 ? (n - 1) / 2 * n : n / 2 * (n - 1)) * (a / m) + n * (b / m);
         a %= m;
@@ -78,6 +79,7 @@ struct Kv8Walk {
         n_steps = few ? (n_pages + p.few_pages - 1) / p.few_pages : n_pages;
     }
     __host__ __device__ __forceinline__ bool next(const Kv8Prompt& p) {
+#pragma unroll 1
         for (;;) {
             if (f >= f_end) return false;
             if (t >= n_steps + kKv8Start) {
@@ -86,6 +88,7 @@ struct Kv8Walk {
                     i = 0;
                     if (++h == p.nkv) {
                         h = 0;
+#pragma unroll 1
                         do q.load(p, ++r);
                         while (q.len == 0);
                     }
@@ -103,6 +106,7 @@ struct Kv8Walk {
     }
     // where step (or, where each CTA takes whole units, unit) `at` of the flat list lies; `before` of them belong to requests ahead of r0, and it is r0's or a later one's
     __host__ __device__ inline void seek(const Kv8Prompt& p, bool whole, int r0, int before, int at) {
+#pragma unroll 1
         for (r = r0;; ++r) {
             q.load(p, r);
             const int n = whole ? q.tiles : q.all(p);
@@ -111,6 +115,7 @@ struct Kv8Walk {
                 h = (int)((unsigned)rest / (unsigned)n);
                 rest -= h * n;
                 int lo = 0, hi = q.tiles - 1;                        // the last tile that begins at or before rest
+#pragma unroll 1
                 while (!whole && lo < hi) {
                     const int mid = (lo + hi + 1) >> 1;
                     if (q.before(p, mid) <= rest) lo = mid; else hi = mid - 1;

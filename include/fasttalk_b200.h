@@ -667,7 +667,7 @@ int ft_attn_prefill(const void* q, const void* kv_layer, const int* page_table, 
  * A code c (one byte) stands for (c - 128) * scale of its block.  Key of token t, dim i: piece i / 64, row t, byte i % 64; value: row t ^ (t >> 1 & 1), byte
  * (i % 64) ^ 8 (t & 4).  A cache of zero bytes is a cache of zeros.  head_dim 64 or 128; q, qkv, out and the cache on 16 bytes.
  * Page numbers outside [0, num_pages), page-table rows outside [0, table_rows) and positions beyond max_pages * 64 name no token: nothing is written there, zeros
- * are read, and attention does not see such keys.  A query that sees no key at all gives zeros.  The calls read and write what they are given only; all but
+ * are read, and attention does not see such keys.  What lies behind a sequence's last token, in its blocks' scales too, may be anything.  A query that sees no key at all gives zeros.  The calls read and write what they are given only; all but
  * append may run at the same time on any streams, append beside nothing that touches the same pages.
  *
  * ft_rope_kv8_append: ft_rope_kv_append into this cache (n_angles = rows of cos_t / sin_t; a token beyond them is not written, its q is 0).  Per block and head, with a = max |x| over the block's new
@@ -688,11 +688,12 @@ int ft_kv8_read(const void* kv8_layer, int num_pages, const int* page_table, int
 long long ft_attn_decode_kv8_scratch_bytes(int d);
 int ft_attn_decode_kv8(const void* q, const void* kv8_layer, int num_pages, const int* page_table, int max_pages, const int* ctx_lens, void* out,
                        void* out_lo, void* scratch, int B, int nq, int nkv, int d, void* stream);
-/* Every wait inside the kernels of this cache has a limit; one that runs out leaves NaN in the rows it was for.  -> 1 if that has happened on the current device since the library
- * was loaded, else 0 (waits for the device). */
+/* Every wait inside the kernels of this cache has a limit; one that runs out ends its CTA, whose rows are NaN or not written.  -> 1 if that has happened on the current device since
+ * the library was loaded, else 0 (waits for the device). */
 int ft_kv8_waits(void);
 /* Causal attention of prompt portions: q FP16 [T][nq][d], nq / nkv up to 8, request r owns rows req_q_start[r] .. req_q_start[r + 1] - 1 (req_q_start grows), page-table row req_slot[r],
- * and its first query sits at position req_pos0[r].  The lists are DEVICE arrays.  All T rows of out (and out_lo, may be NULL) are written; those that no request owns with zeros.
+ * and its first query sits at position req_pos0[r].  The lists are DEVICE arrays.  All T rows of out (and out_lo, may be NULL) are written; those that no request owns with zeros
+ * (where req_q_start does not grow, none of them means anything).
  * scratch: work memory of ft_attn_prefill_kv8_scratch_bytes(d) bytes (of the current device), in any state, not shared by calls that may overlap. */
 long long ft_attn_prefill_kv8_scratch_bytes(int d);
 int ft_attn_prefill_kv8(const void* q, const void* kv8_layer, int num_pages, const int* page_table, int table_rows, int max_pages,

@@ -496,6 +496,64 @@ def test_prefill_single_tokens_are_decode(K):
     assert off <= 127 * 0.012 * 8 * 2.0 ** -9
 
 
+# ------------------------------------------------------------------------------------------------ what lies behind the last token
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf, 3e38])
+@pytest.mark.parametrize("nq,nkv,d", [(8, 2, 64), (6, 2, 128)])
+def test_scales_behind_the_last_token_may_be_anything(K, nq, nkv, d, bad):
+    """A cache in memory that was never cleared: blocks that no token of the sequence has reached hold any scale, keys' and values'."""
+    lengths = [16, 17, 33, 48, 49, 63, 64, 1, 200, 3 * 64 + 47]
+    q, cache, table = decode_case(K, lengths, nq, nkv, d, seed=13)
+    codes, scales = K.kv8_codes(cache, d)
+    dirty, clean = scales.clone(), scales.clone()
+    for b, n in enumerate(lengths):
+        last, behind = int(table[b, (n - 1) // 64]), (n - 1) % 64 // 16 + 1
+        dirty[last, :, :, behind:] = bad
+        clean[last, :, :, behind:] = 0
+    runs = [(i32(list(range(11))), i32(list(range(10))), i32([n - 1 for n in lengths])), (i32([0, 10]), i32([9]), i32([lengths[9] - 10]))]
+    a, b = K.kv8_records(codes, dirty), K.kv8_records(codes, clean)
+    for x, y in zip(K.attn_decode_kv8(q, a, table, i32(lengths)), K.attn_decode_kv8(q, b, table, i32(lengths))):
+        assert torch.equal(x, y) and torch.isfinite(x).all()
+    for lists in runs:
+        for x, y in zip(K.attn_prefill_kv8(q, a, table, *lists), K.attn_prefill_kv8(q, b, table, *lists)):
+            assert torch.equal(x, y) and torch.isfinite(x).all()
+    check_decode(K, q, b, table, lengths, planes=2)
+
+
+def test_append_enters_a_block_of_any_scale(K):
+    """A block's first token replaces whatever scale the block had; a token further on keeps it."""
+    nq, nkv, d = 2, 1, 64
+    for bad in (math.nan, math.inf, 1e30):
+        codes = torch.randint(0, 256, (2, nkv, 2, 64, d), device=DEV).to(torch.uint8)
+        cache = K.kv8_records(codes, torch.full((2, nkv, 2, 4), bad, device=DEV))
+        x = torch.randn(1, 20, 4 * d, device=DEV)
+        ones, zeros = torch.ones(64, d // 2, device=DEV), torch.zeros(64, d // 2, device=DEV)
+        K.rope_kv8_append(x, ones, zeros, i32(list(range(16, 36))), i32([0] * 20), i32([[1]]), cache, nq, nkv, d)
+        _, s = K.kv8_codes(cache, d)
+        assert (s[1, :, :, 1:3] < 0.1).all() and not (s[1, :, :, 0] < 0.1).any() and not (s[1, :, :, 3] < 0.1).any()
+        k, v = K.kv8_read(cache, i32([[1]]), i32([0, 20]), i32([0]), i32([16]), 20, d)
+        want = x[0].reshape(20, -1, d)
+        assert (k[:, 0].float() - want[:, 2]).abs().max() < 0.05 and (v[:, 0].float() - want[:, 3]).abs().max() < 0.05
+
+
+def test_lists_that_do_not_grow_are_not_walked(K):
+    """Nothing is promised about the rows; the call ends, and the next one is whole."""
+    case = prompt_case(K, [(100, 40), (0, 30), (7, 5)], 8, 2, 64, seed=3)
+    q, cache, table, starts, slots, pos0 = case
+    for bad in ([0, 75, 0, 75], [75, 0, 75, 0], [0, -5, 70, 75], [40, 30, 20, 10], [1 << 30, 0, 1 << 30, 5]):
+        K.attn_prefill_kv8(q, cache, table, bad, slots, pos0)
+        K.kv8_read(cache, table, bad, slots, pos0, 75, 64)
+    check_prompt(K, case, planes=2)
+    # growing ones may reach beyond q, or begin before it: what there is of them is done
+    for wide in ([-9, 40, 70, 1 << 30], [0, 40, 70, 76]):
+        hi, lo = K.attn_prefill_kv8(q, cache, table, wide, slots, pos0)
+        assert torch.isfinite(hi.float()).all()
+
+
+def test_no_wait_has_run_out(K):
+    from fasttalk_llm_microservice_b200 import native
+    assert native.load().ft_kv8_waits() == 0
+
+
 # ------------------------------------------------------------------------------------------------ together, as they are used
 def conversation(K, nq, nkv, d, seed, stream=None, steps=5):
     """A prompt in two portions beside a second session, then single tokens: append and attention as a step runs them.  -> outputs, and what they should be."""
