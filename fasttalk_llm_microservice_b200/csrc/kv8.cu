@@ -8,7 +8,8 @@
 //
 // A warp takes the runs that begin among one (or four, where there are many tokens) of the list, for one head's keys or values; a run = neighbouring tokens that go
 // to one block of one sequence.  Its rows stay in registers between the maximum and the rounding, so the projection is read once, all of it asked for before the
-// first number is used: what bounds a prompt's portion is that reading.
+// first number is used: what bounds a prompt's portion is that reading.  1954 tokens of four sequences behind 1003 each, in two
+// parts, 32 + 16 heads of 128: 125 MB in 29.5 us, 4.25 TB/s (a row at a time 64 us); 64 single tokens, 32 + 16 heads of 64: 8.1 us, list, page and scale read one after the other.
 #include "common.cuh"
 #include "ft_internal.h"
 #include "kv8.cuh"
@@ -17,7 +18,7 @@ namespace ft {
 
 constexpr int K8_WARPS = 8;
 constexpr int K8_QHEADS = 8;                 // query heads a warp takes
-constexpr int K8_MANY = 256;                 // tokens from which a warp looks at four of them (most of a prompt's tokens begin no run; single tokens all do)
+constexpr int K8_MANY = 512;                 // tokens from which a warp looks at four of them: most of a prompt's begin no run (1800 tokens 14.3 against 18.9 us, 700 9.8 / 11.9, 400 11.6 / 10.4), single ones all do (64 15.1 / 7.9)
 
 struct Kv8Append {
     const float* qkv;
@@ -201,7 +202,8 @@ kv8_append_kernel(const Kv8Append p, int kv_rows, int kv_ctas) {
 // ------------------------------------------------------------------ reading back
 // Row i of k and v: (c - 128) * s of the request that owns it, in fp16 (cut to its range); rows that no request owns, and rows whose page lies outside the
 // cache, are zeros.  A CTA takes 16 rows of eight (sixteen) heads' keys or values: 16 bytes of codes a load, 32 bytes of fp16 a store, four loads on their way a
-// thread.  Bound by memory (one byte in, two out).
+// thread.  Bound by memory (one byte in, two out): 16 sequences of 2048 .. 1987 tokens, 8 heads of 64 (99 MB): 18.9 us, 5.3 TB/s; 5003 tokens of 8 heads of
+// 128 (31 MB): 8.6 us, 3.6 TB/s, too short for more.  With one load at a time 23.7 and 9.9 us.
 constexpr int K8_READ_ROWS = 16, K8_READ_THREADS = 256, K8_READ_TASKS = 4;
 
 template <int D>

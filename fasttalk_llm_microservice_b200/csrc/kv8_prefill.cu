@@ -16,7 +16,13 @@
 // unit of few tokens gain nothing over one: a page counts as one there.)  One warp of each CTA finds its share from the lists on the device and tells the others stretch by stretch; nothing is planned
 // ahead of the kernel.
 //
-// What bounds it: a page's chain of hand-overs in each half (scores - exponentials - probabilities - products), TIMES_HERE.
+// What bounds it: each half's chain of a page, scores out of tensor memory - exponentials - probabilities into it - products - next scores, and the instructions of
+// eight softmax and eight converting warps around it: about 2200 clocks (1.15 us) a page of both halves at either head size, where the exponentials alone take 1024 (the SFU's
+// 16 a clock and SM).  Four prompts of 2048 .. 1578 tokens, 32 heads over 8 of 64: 152 us, 372 TFLOP/s; six portions of 211 .. 153 tokens behind about 5000, heads of 128:
+// 124 us, 674 TFLOP/s; five tokens behind 16001 on one rank's heads: 25 us, of which 6 pass until the first scores and 3 to 7 in the second kernel.
+// Measured on the way, us for the first two: shares of pages alone, without a unit's start and end, 175 / 176 (with them 153 / 126); the next page's scores read ahead of this
+// page's exponentials 251 / 349 (with two buffers they are formed only behind the products that wait for this page's probabilities); copies and conversions that nap between
+// their tries 223 / 339; longer waits written out in every role, 173 / 138 against 153 / 127 (instruction fetch).
 #include "common.cuh"
 #include "ft_internal.h"
 #include "kv8.cuh"
@@ -36,7 +42,9 @@ constexpr int K8P_GROUP = 8;                     // query heads a key head at mo
 constexpr int K8P_PIECE = kKvTile * 128;         // [64 tokens][64 dims] in fp16; 64 rows of a Q block
 constexpr float K8P_LOG2E = 1.4426950408889634f;
 constexpr float K8P_GROW = 8.f;                  // O is rescaled when a row's maximum has grown by more than 2^8
-constexpr int K8P_WHOLE = 5;                     // pages that a share may be shorter than a whole unit for parts not to pay
+constexpr int K8P_WHOLE = 10;
+// (pages that a share may be shorter than a whole unit for parts not to pay: 5 / 10 / 15 for four portions of 100 tokens behind 300, heads of 128, 24.8 / 19.6 / 19.6 us; six of
+// 100 behind 1000 36.5 / 34.4 / 34.4, heads of 64 27.5 / 30.2 / 30.5; three of 150 behind 900 24.3 / 24.2 / 29.9; two of 300, heads of 128, 17 us whole and 22 in parts)
 
 template <int D>
 struct K8Prefill {
