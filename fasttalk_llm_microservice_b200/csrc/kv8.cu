@@ -9,7 +9,7 @@
 // A warp takes the runs that begin among one (or four, where there are many tokens) of the list, for one head's keys or values; a run = neighbouring tokens that go
 // to one block of one sequence.  Its rows stay in registers between the maximum and the rounding, so the projection is read once, all of it asked for before the
 // first number is used: what bounds a prompt's portion is that reading.  1954 tokens of four sequences behind 1003 each, in two
-// parts, 32 + 16 heads of 128: 125 MB in 29.5 us, 4.25 TB/s (a row at a time 64 us); 64 single tokens, 32 + 16 heads of 64: 8.1 us, list, page and scale read one after the other.
+// parts, 32 + 16 heads of 128 (116 MB): 24.6 us, 4.7 TB/s (with the rows read back 29, a row at a time 64); 64 single tokens, 32 + 16 heads of 64: 4.2 us, list, page and scale read one after the other.
 #include "common.cuh"
 #include "ft_internal.h"
 #include "kv8.cuh"
@@ -18,7 +18,8 @@ namespace ft {
 
 constexpr int K8_WARPS = 8;
 constexpr int K8_QHEADS = 8;                 // query heads a warp takes
-constexpr int K8_MANY = 512;                 // tokens from which a warp looks at four of them: most of a prompt's begin no run (1800 tokens 14.3 against 18.9 us, 700 9.8 / 11.9, 400 11.6 / 10.4), single ones all do (64 15.1 / 7.9)
+constexpr int K8_MANY = 512;                 // tokens from which a warp looks at four of them: most of a prompt's begin no run, single ones all do.
+                                             // Four against one, us, their rows read back in 4 to 5 of them: 1800 in portions of 300 14.3 / 18.9, 700 in one 9.8 / 11.9, 400 in portions of 100 11.6 / 10.4, 64 single 15.1 / 7.9
 
 struct Kv8Append {
     const float* qkv;
