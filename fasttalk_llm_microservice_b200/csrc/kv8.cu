@@ -10,6 +10,8 @@
 // to one block of one sequence.  Its rows stay in registers between the maximum and the rounding, so the projection is read once, all of it asked for before the
 // first number is used: what bounds a prompt's portion is that reading.  1954 tokens of four sequences behind 1003 each, in two
 // parts, 32 + 16 heads of 128 (116 MB): 24.6 us, 4.7 TB/s (with the rows read back 29, a row at a time 64); 64 single tokens, 32 + 16 heads of 64: 4.2 us, list, page and scale read one after the other.
+#include <type_traits>
+
 #include "common.cuh"
 #include "ft_internal.h"
 #include "kv8.cuh"
@@ -69,11 +71,11 @@ __device__ __forceinline__ float4 kv8_rotate(float4 x, float4 c, float4 s, int s
 template <int D>
 __global__ void __launch_bounds__(K8_WARPS * 32, 2)
 kv8_append_kernel(const Kv8Append p, int kv_rows, int kv_ctas) {
+    pdl_wait();
     constexpr int LR = D / 4, RP = 32 / LR, N = kKv8Block / RP, HL = D / 8;      // lanes a row, rows a pass, passes; lanes of half a row
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int sub = lane % LR, rsub = lane / LR;
     const int angles = min(p.n_angles, p.max_pages * kKvTile);
-    pdl_wait();
     const size_t width = (size_t)(p.nq + 2 * p.nkv) * D;
 
     if ((int)blockIdx.x >= kv_ctas) {
@@ -212,8 +214,8 @@ __global__ void __launch_bounds__(K8_READ_THREADS)
 kv8_read_kernel(const uint8_t* __restrict__ cache, const int* __restrict__ page_table, int table_rows, int max_pages, int num_pages,
                 const int* __restrict__ req_start, const int* __restrict__ req_slot, const int* __restrict__ req_pos0, int n_req, int rows, int nkv,
                 uint8_t* __restrict__ k_out, uint8_t* __restrict__ v_out) {
-    __shared__ int s_page[K8_READ_ROWS], s_tok[K8_READ_ROWS];
     pdl_wait();
+    __shared__ int s_page[K8_READ_ROWS], s_tok[K8_READ_ROWS];
     const int row0 = blockIdx.x * K8_READ_ROWS;
     if (threadIdx.x < 32) {
         // lane i: row i; its request is the last that starts at or before it
@@ -306,7 +308,10 @@ extern "C" int ft_rope_kv8_append(const float* qkv, int n_splits, long long spli
     const long long q_tasks = (long long)T * ((nq + K8_QHEADS - 1) / K8_QHEADS), q_ctas = (q_tasks + K8_WARPS - 1) / K8_WARPS;
     FT_REQUIRE(q_tasks <= INT32_MAX && kv_ctas + q_ctas <= INT32_MAX, "ft_rope_kv8_append: %d tokens of %d + %d heads", T, nq, nkv);
     const int grid = (int)(kv_ctas + q_ctas);
-    FT_CHECK_CUDA(launch_after(d == 64 ? kv8_append_kernel<64> : kv8_append_kernel<128>, dim3(grid), dim3(K8_WARPS * 32), 0, (cudaStream_t)stream, p, (int)kv_rows, (int)kv_ctas));
+    auto send = [&](auto head) {
+        return launch_after(kv8_append_kernel<decltype(head)::value>, dim3(grid), dim3(K8_WARPS * 32), 0, (cudaStream_t)stream, p, (int)kv_rows, (int)kv_ctas);
+    };
+    FT_CHECK_CUDA(d == 64 ? send(std::integral_constant<int, 64>{}) : send(std::integral_constant<int, 128>{}));
     return 0;
 }
 
@@ -322,7 +327,10 @@ extern "C" int ft_kv8_read(const void* kv8_layer, int num_pages, const int* page
     const long long tasks = (long long)nkv * 2 * K8_READ_ROWS * (d / 16), per = K8_READ_TASKS * K8_READ_THREADS;
     FT_REQUIRE((tasks + per - 1) / per <= 65535, "ft_kv8_read: %d heads", nkv);
     const dim3 grid((rows + K8_READ_ROWS - 1) / K8_READ_ROWS, (unsigned)((tasks + per - 1) / per));
-    FT_CHECK_CUDA(launch_after(d == 64 ? kv8_read_kernel<64> : kv8_read_kernel<128>, grid, dim3(K8_READ_THREADS), 0, (cudaStream_t)stream, (const uint8_t*)kv8_layer,
-                               page_table, table_rows, max_pages, num_pages, req_start, req_slot, req_pos0, n_req, rows, nkv, (uint8_t*)k_out, (uint8_t*)v_out));
+    auto send = [&](auto head) {
+        return launch_after(kv8_read_kernel<decltype(head)::value>, grid, dim3(K8_READ_THREADS), 0, (cudaStream_t)stream, (const uint8_t*)kv8_layer, page_table, table_rows,
+                            max_pages, num_pages, req_start, req_slot, req_pos0, n_req, rows, nkv, (uint8_t*)k_out, (uint8_t*)v_out);
+    };
+    FT_CHECK_CUDA(d == 64 ? send(std::integral_constant<int, 64>{}) : send(std::integral_constant<int, 128>{}));
     return 0;
 }

@@ -6,10 +6,10 @@
 // parts.  Where there is a CTA for every (sequence, head) and none of them is long, each CTA takes a whole one instead: no parts, nothing to put together.
 //
 // Nothing is planned ahead of the kernel: every CTA adds up the sequences' pages itself (one read of ctx_lens).  What the arrival counters need, zeros, is
-// written by a kernel of its own whose end this one waits for only when it has its first part ready.
+// written by a kernel of its own ahead of this one.
 //
-// 64 sequences of about 2000 keys, 32 heads over 8 of 64 (133 MB): 32.6 us, 4.1 TB/s.  The first record lands about 4 us after the start (lengths, page number and record are
-// read one after the other), then the shares stream at about 5.7 TB/s, and the parts are put together in the last 5.  Three of 30011 .. 9377 keys, heads of 128: 29.9 us.  On the
+// 64 sequences of about 2000 keys, 32 heads over 8 of 64 (133 MB): 33.0 us, 4.0 TB/s.  The first record lands about 4 us after the start (lengths, page number and record are
+// read one after the other), then the shares stream at about 5.7 TB/s, and the parts are put together in the last 5.  Three of 30011 .. 9377 keys, heads of 128: 30.0 us.  On the
 // way, for the two: shares with the queries in the rows of the first product 36 / 38, the tokens in them 32 / 34, and then all warps putting parts together 32 / 30.
 #include "common.cuh"
 #include "ft_internal.h"
@@ -41,8 +41,7 @@ struct K8Decode {
 };
 
 __global__ void kv8_decode_zero_kernel(int* counters, int n) {
-    pdl_wait();                                      // what was in the stream before is done: the kernel behind this one need not wait for it again
-    pdl_launch_dependents();
+    pdl_wait();
     for (int i = threadIdx.x; i < n; i += blockDim.x) counters[i] = 0;
 }
 
@@ -51,6 +50,7 @@ __global__ void __launch_bounds__(K8Decode<D>::THREADS, 2)
 kv8_decode_kernel(const __half* __restrict__ q, const uint8_t* __restrict__ cache, int num_pages, const int* __restrict__ page_table, int max_pages,
                   const int* __restrict__ ctx_lens, __nv_bfloat16* __restrict__ out, __nv_bfloat16* __restrict__ out_lo, int* counters, float* parts,
                   int B, int nq, int nkv, float scale_log2) {
+    pdl_wait();
     using C = K8Decode<D>;
     extern __shared__ __align__(128) uint8_t smem[];
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BARS);
@@ -70,7 +70,6 @@ kv8_decode_kernel(const __half* __restrict__ q, const uint8_t* __restrict__ cach
         fence_mbar_init();
         dead = 0;
     }
-    if (parts == nullptr) pdl_wait();                                        // nothing of this call's ran before
     auto ctx_of = [&](int b) { return max(0, min(ctx_lens[b], max_pages * kKvTile)); };
     auto pages_of = [&](int b) { return (ctx_of(b) + kKvTile - 1) / kKvTile; };
 
@@ -109,10 +108,7 @@ kv8_decode_kernel(const __half* __restrict__ q, const uint8_t* __restrict__ cach
     int b, h, t;
     if (whole) {
         b = blockIdx.x / nkv;
-        if (b >= B) {
-            pdl_wait();
-            return;
-        }
+        if (b >= B) return;
         h = blockIdx.x % nkv;
         t = 0;
         f = 0;
@@ -147,7 +143,6 @@ kv8_decode_kernel(const __half* __restrict__ q, const uint8_t* __restrict__ cach
             if (pages_of(i) == 0) zeros(i, 0, nkv);
     }
     if (f >= f_end) {
-        pdl_wait();
         return;
     }
 
@@ -206,7 +201,6 @@ kv8_decode_kernel(const __half* __restrict__ q, const uint8_t* __restrict__ cach
             for (int i = max(0, asked - C::STAGES); i < asked; ++i)
                 for (int k = 0; k < kWaitLimit && !mbar_try_wait(&full[i % C::STAGES], i / C::STAGES & 1); ++k) {}
         }
-        pdl_wait();
         return;
     }
 
@@ -269,7 +263,6 @@ kv8_decode_kernel(const __half* __restrict__ q, const uint8_t* __restrict__ cach
             if (final) break;
             // The last CTA to deliver a part puts all of them together: each warp takes every WARPS-th part, in their order, and then they are records of the
             // warps once more.  (All threads walking all parts one after the other: 12 us at the end of three sequences of 20000 keys, 19 parts each.)
-            pdl_wait();                                                      // the counters are zeros now
             asm volatile("bar.sync 1, %0;" ::"n"(C::WARPS * 32) : "memory");
             if (tid == 0) {
                 __threadfence();
@@ -317,7 +310,6 @@ kv8_decode_kernel(const __half* __restrict__ q, const uint8_t* __restrict__ cach
         }
         asm volatile("bar.sync 1, %0;" ::"n"(C::WARPS * 32) : "memory");
     }
-    pdl_wait();                                                              // this kernel ends behind the one before it
 }
 
 // counters (one for each CTA that a split (sequence, head) can begin in), then two parts a CTA: of the (sequence, head) it begins in the middle of, and of the one it ends in

@@ -670,9 +670,9 @@ constexpr int K8P_MERGE_WARPS = 2 * K8P_ROWS / 32, K8P_FEW_PARTS = 8;
 template <int D>
 __global__ void __launch_bounds__(K8P_MERGE_WARPS * 32)
 kv8_prefill_merge_kernel(const __grid_constant__ Kv8Prompt p) {
+    pdl_wait();
     using C = K8Prefill<D>;
     __shared__ float acc_s[K8P_MERGE_WARPS][18][32];
-    pdl_wait();
     const Kv8Split u = p.split[blockIdx.x];
     if (u.parts == 0) return;
     const bool few = u.tokens < 0;
