@@ -337,7 +337,6 @@ static int launch_kv8_decode(const void* q, const void* cache, int num_pages, co
         return 0;
     }
     FT_CHECK_CUDA(launch_after(kv8_decode_zero_kernel, dim3(1), dim3(128), 0, st, counters, ctas));
-    // starts beside the zeroes, for which it waits when it has its first part ready
     FT_CHECK_CUDA(launch_after(kv8_decode_kernel<D>, dim3(ctas), dim3(C::THREADS), C::SMEM, st, (const __half*)q, (const uint8_t*)cache, num_pages, page_table,
                                max_pages, ctx_lens, (__nv_bfloat16*)out, (__nv_bfloat16*)out_lo, counters, parts, B, nq, nkv, scale_log2));
     return 0;

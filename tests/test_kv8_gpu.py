@@ -133,7 +133,7 @@ def check_append(K, before, after, table, reqs, k, v, d):
     left_c, left_s = c0.clone(), s0.clone()
     at = 0
     for i, (cached, new) in enumerate(reqs):
-        for b0 in range(cached // 16 * 16, cached + new, 16):
+        for b0 in range(cached // 16 * 16, cached + new, 16) if new else ():
             lo, hi = max(b0, cached), min(b0 + 16, cached + new)
             page, row, blk = int(table[i, b0 // 64]), b0 % 64, b0 % 64 // 16
             for what, x in ((0, k), (1, v)):
@@ -261,6 +261,44 @@ def test_append_prompt_and_single_tokens_side_by_side(K):
     K.rope_kv8_append(wide[:, 1], cos, sin, pos, seq, table, cache, nq, nkv, d)
     _, rk, rv = rotated(qkv, cos, sin, pos, nq, nkv, d)
     check_append(K, before, cache, table, reqs, rk, rv, d)
+
+
+@pytest.mark.parametrize("nq,nkv,d", [(8, 2, 64), (3, 1, 128)])
+@pytest.mark.parametrize("reqs", [
+    [(37 * i % 300, 1 + (i % 3 == 0)) for i in range(383)],                            # 511 tokens, the last list of which a warp looks at one
+    [(37 * i % 300, 1 + (i % 3 == 0)) for i in range(384)] + [(9, 0)],                 # 512, single tokens and pairs: runs begin at every place of a warp's four
+    [(0, 700)], [(3, 257), (15, 2), (16, 1), (47, 255), (0, 30)],                      # runs that begin in one warp's four and end in another's
+    [(5, 509), (63, 3), (64, 1)], [(13, 1021)],                                        # lists that end inside a warp's four
+])
+def test_append_of_many_tokens(K, nq, nkv, d, reqs):
+    args = append_inputs(K, reqs, nq, nkv, d, 1, seed=d + len(reqs), amplitude=2.0)
+    qkv, cos, sin, pos, seq, table, cache = args
+    before = cache.clone()
+    K.rope_kv8_append(*args, nq, nkv, d)
+    _, rk, rv = rotated(qkv, cos, sin, pos, nq, nkv, d)
+    check_append(K, before, cache, table, reqs, rk, rv, d)
+
+
+def test_append_of_many_tokens_without_a_place(K):
+    """Lists long enough for four tokens a warp, some of whose tokens lie outside the table or the cache: those are not written, their neighbours are."""
+    nq, nkv, d, T = 1, 1, 64, 601
+    cache = K.kv8_cache_alloc(T, nkv, d, DEV)
+    table = torch.arange(T, device=DEV, dtype=torch.int32)[:, None].contiguous()
+    table[5::11] = -1
+    table[7::11] = T
+    seq, pos = torch.arange(T, device=DEV, dtype=torch.int32), torch.zeros(T, device=DEV, dtype=torch.int32)
+    seq[3::13] = T
+    pos[4::13] = 64
+    pos[6::13] = -1
+    x = torch.randn(1, T, 3 * d, generator=gen(4), device=DEV)
+    ones, zeros = torch.ones(64, d // 2, device=DEV), torch.zeros(64, d // 2, device=DEV)
+    K.rope_kv8_append(x, ones, zeros, pos, seq, table, cache, nq, nkv, d)
+    placed = (seq < T) & (pos == 0)
+    placed &= (table[:, 0] >= 0) & (table[:, 0] < T)
+    _, scales = K.kv8_codes(cache, d)
+    most = x[0].reshape(T, 3, d)[:, 1:].abs().amax(-1)                                 # keys, values
+    assert (scales[~placed] == 0).all()
+    assert ((scales[placed, 0, :, 0] - most[placed] / 127).abs() <= most[placed] / 127 * 2.0 ** -22).all()
 
 
 def test_append_queries_are_those_of_the_fp16_cache(K):
@@ -436,6 +474,14 @@ def test_prefill(K, nq, nkv, d, reqs):
 @pytest.mark.parametrize("reqs", [[(0, 700)], [(3000, 5)], [(2990, 33), (0, 300), (100, 64), (1500, 1)], [(30 * i, 1 + 7 * i) for i in range(20)], [(9000, 2), (50, 2)]])
 def test_prefill_long_and_many(K, nq, nkv, d, reqs):
     check_prompt(K, prompt_case(K, reqs, nq, nkv, d, seed=len(reqs)), planes=2)
+
+
+@pytest.mark.parametrize("nq,nkv,d", [(32, 8, 64), (32, 8, 128), (16, 16, 128)])
+@pytest.mark.parametrize("reqs", [[(300, 100)] * 4, [(64 * 9 - 5, 5)] * 4, [(64 * 10 - 5, 5)] * 4, [(64 * 10, 7)] * 4, [(900, 150)] * 3, [(64 * 14, 40)] * 2,
+                                  [(i * 13 % 500, 20) for i in range(40)], [(900, 60)] * 19])
+def test_prefill_whole_units_and_parts(K, nq, nkv, d, reqs):
+    """Units around ten pages longer than a share, page tables around ten pages wide, and more units than SMs: whole, or in parts that are put together."""
+    check_prompt(K, prompt_case(K, reqs, nq, nkv, d, seed=len(reqs) + reqs[0][0]), planes=2)
 
 
 @pytest.mark.parametrize("before,after", [(0, 0), (3, 0), (0, 5), (70, 200)])
