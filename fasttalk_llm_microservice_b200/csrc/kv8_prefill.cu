@@ -178,34 +178,25 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
         const int chunk = (p.n_req + 31) / 32;
         const int r0 = min(p.n_req, lane * chunk), r1 = min(p.n_req, r0 + chunk);
         Kv8Walk w;
-        int mine = 0, units = 0, most = 0;
-        bool grows = true;                                                   // a list that does not is not walked: its sums could be any
+        Kv8Sums mine;
 #pragma unroll 1
-        for (int r = r0; r < r1; ++r) {
-            w.q.load(p, r);
-            grows = grows && p.req_q_start[r] <= p.req_q_start[r + 1];
-            mine += w.q.all(p);
-            units += w.q.tiles;
-            if (w.q.tiles) most = max(most, max(w.q.steps(p, w.q.tiles - 1), w.q.tiles > 1 ? w.q.steps(p, w.q.tiles - 2) : 0));
-        }
-        int b_steps = mine, b_units = units;
+        for (int r = r0; r < r1; ++r) mine.add(p, r);
+        int b_steps = mine.steps, b_units = mine.units;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int x = __shfl_up_sync(0xffffffffu, b_steps, o), y = __shfl_up_sync(0xffffffffu, b_units, o);
             if (lane >= o) b_steps += x, b_units += y;
         }
-        most = __reduce_max_sync(0xffffffffu, most);
+        const int most = __reduce_max_sync(0xffffffffu, mine.most);
         const int total = __shfl_sync(0xffffffffu, b_steps, 31) * p.nkv, n_units = __shfl_sync(0xffffffffu, b_units, 31) * p.nkv, ctas = gridDim.x;
-        b_steps -= mine;
-        b_units -= units;
+        b_steps -= mine.steps;
+        b_units -= mine.units;
         const int per = (unsigned)(total + ctas - 1) / (unsigned)ctas;
         const bool whole = p.split == nullptr || (n_units <= ctas && most + kKv8Start <= per + K8P_WHOLE);      // (no room for parts: the host knows that there are none)
         // the flat list is one of units or of steps
         const int len = whole ? n_units : total, each = whole ? 1 : per, at0 = whole ? b_units : b_steps;
-        w.f = min(len, each * (int)blockIdx.x);
-        w.f_end = min(len, w.f + each);
-        const bool work = __all_sync(0xffffffffu, grows) && w.f < w.f_end;
-        if (work ? at0 * p.nkv <= w.f && w.f < (at0 + (whole ? units : mine)) * p.nkv : lane == 0) {      // one lane
+        const bool work = w.share(__all_sync(0xffffffffu, mine.grows), len, each, blockIdx.x);
+        if (work ? at0 * p.nkv <= w.f && w.f < (at0 + (whole ? mine.units : mine.steps)) * p.nkv : lane == 0) {      // one lane
             if (work) {
                 w.seek(p, whole, r0, at0, w.f);
                 w.unit(p);

@@ -63,6 +63,20 @@ struct Kv8Request {
     __host__ __device__ __forceinline__ int all(const Kv8Prompt& p) const { return tiles ? before(p, tiles - 1) + steps(p, tiles - 1) + kKv8Start : 0; }
 };
 
+// What a run of requests adds up to: steps and units of one key head, the longest unit's steps, and whether the list grows
+struct Kv8Sums {
+    int steps = 0, units = 0, most = 0;
+    bool grows = true;
+    __host__ __device__ __forceinline__ void add(const Kv8Prompt& p, int r) {
+        Kv8Request q;
+        q.load(p, r);
+        grows = grows && p.req_q_start[r] <= p.req_q_start[r + 1];
+        steps += q.all(p);
+        units += q.tiles;
+        if (q.tiles) most = max(most, max(q.steps(p, q.tiles - 1), q.tiles > 1 ? q.steps(p, q.tiles - 2) : 0));
+    }
+};
+
 // A stretch of pages of one unit.  parts: 0 = it is the whole unit; else, where the unit begins, how many shares it lies in
 struct Kv8Stretch { int page0, pages, few, row0, tokens, pos0, head, slot, begins, parts; };
 
@@ -103,6 +117,13 @@ struct Kv8Walk {
             f += take;
             if (t1 > t0) return true;                                // else all of it was behind the unit's last step
         }
+    }
+    // the share of CTA `cta` in a list of `len`, `each` of them a CTA.  true: there is something in it.  Where the requests' list does not grow there is not: its sums
+    // could be any, and next() must find nothing to walk, since nothing else of the walk is set then
+    __host__ __device__ __forceinline__ bool share(bool grows, int len, int each, int cta) {
+        f = grows ? min(len, each * cta) : 0;
+        f_end = grows ? min(len, f + each) : 0;
+        return f < f_end;
     }
     // where step (or, where each CTA takes whole units, unit) `at` of the flat list lies; `before` of them belong to requests ahead of r0, and it is r0's or a later one's
     __host__ __device__ inline void seek(const Kv8Prompt& p, bool whole, int r0, int before, int at) {
