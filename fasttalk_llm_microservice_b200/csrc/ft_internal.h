@@ -48,6 +48,8 @@ int launch_gemm(const CUtensorMap& mw, const CUtensorMap& mx, const CUtensorMap*
 
 // ---- kv8_prefill.cu: 1 once a wait has run out in a kernel of that file
 int kv8_prefill_waits(int* out);
+// ---- kv8_decode.cu: tries of a wait in the kernels of the 8-bit cache (ft_kv8_set_wait_limit)
+int kv8_wait_limit();
 
 // ---- gemm_plain.cu: out[t][n] = sum_k (hi + lo)[t][k] W[n][k], fp32 results without a fused layer step
 int launch_gemm_plain(const void* w, const void* hi, const void* lo, float* out, int n_out, int T, int K, cudaStream_t stream);

@@ -44,6 +44,26 @@ __device__ __forceinline__ uint32_t byte_perm(uint32_t a, uint32_t b, uint32_t s
     return r;
 }
 
+// Waits that end, as those of common.cuh do, with the number of tries as an argument (ft_kv8_set_wait_limit) and a few instructions each: the prompt kernel has some
+// twenty of them among five kinds of warps, and its time hangs on what the instruction caches hold (unrolled, they and the rest were 104 KB, and 16 KB more or less of
+// waits outside the loops over pages was 8 % of its time).  Who gives up touches none of the barriers again: what it skipped would make it take one phase for another.
+__device__ __forceinline__ bool kv8_mbar_wait_limited(uint64_t* bar, uint32_t parity, volatile int* dead, int limit) {
+#pragma unroll 1
+    for (int i = 0; i < limit; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*dead) return false;
+    }
+    *dead = 1;
+    return false;
+}
+// What must have ended before the memory that it writes is given back, however the CTA ends: the copies of a ring's last phases
+__device__ __forceinline__ void kv8_copies_landed(uint64_t* full, int stages, int asked) {
+#pragma unroll 1
+    for (int i = max(0, asked - stages); i < asked; ++i)
+#pragma unroll 1
+        for (int k = 0; k < kWaitLimit && !mbar_try_wait(&full[i % stages], i / stages & 1); ++k) {}
+}
+
 // ------------------------------------------------------------------ one query token a sequence, up to eight query heads a key head (mma.sync m16n8k16)
 // A warp takes whole pages.  S[token][query] = K Q^T with 16 tokens in the M rows: K is the A operand, 16 bytes of two tokens a lane, in whatever order of the dims the
 // lanes have them (Q is loaded in the same).  The probabilities, transposed 8 x 8 at a time, are the B operand of O^T[dim][query] = V^T P^T, where all 16 rows are dims:

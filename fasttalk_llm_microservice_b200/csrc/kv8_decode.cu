@@ -11,6 +11,8 @@
 // 64 sequences of about 2000 keys, 32 heads over 8 of 64 (133 MB): 33.0 us, 4.0 TB/s.  The first record lands about 4 us after the start (lengths, page number and record are
 // read one after the other), then the shares stream at about 5.7 TB/s, and the parts are put together in the last 5.  Three of 30011 .. 9377 keys, heads of 128: 30.0 us.  On the
 // way, for the two: shares with the queries in the rows of the first product 36 / 38, the tokens in them 32 / 34, and then all warps putting parts together 32 / 30.
+#include <atomic>
+
 #include "common.cuh"
 #include "ft_internal.h"
 #include "kv8.cuh"
@@ -49,7 +51,7 @@ template <int D>
 __global__ void __launch_bounds__(K8Decode<D>::THREADS, 2)
 kv8_decode_kernel(const __half* __restrict__ q, const uint8_t* __restrict__ cache, int num_pages, const int* __restrict__ page_table, int max_pages,
                   const int* __restrict__ ctx_lens, __nv_bfloat16* __restrict__ out, __nv_bfloat16* __restrict__ out_lo, int* counters, float* parts,
-                  int B, int nq, int nkv, float scale_log2) {
+                  int B, int nq, int nkv, float scale_log2, int wait_limit) {
     pdl_wait();
     using C = K8Decode<D>;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -181,7 +183,7 @@ kv8_decode_kernel(const __half* __restrict__ q, const uint8_t* __restrict__ cach
                     const int page = __shfl_sync(0xffffffffu, my_page, i);
                     if (lane == 0 && ok) {
                         const int s = it % C::STAGES;
-                        ok = mbar_wait_limited(&empty[s], (it / C::STAGES & 1) ^ 1, &dead);
+                        ok = kv8_mbar_wait_limited(&empty[s], (it / C::STAGES & 1) ^ 1, &dead, wait_limit);
                         if (!ok) continue;
                         asked = it + 1;
                         const bool there = page >= 0 && page < num_pages;
@@ -196,24 +198,23 @@ kv8_decode_kernel(const __half* __restrict__ q, const uint8_t* __restrict__ cach
                 }
             }
         }
-        if (lane == 0 && (!ok || dead)) {                                    // gave up: what is under way still lands in this CTA's memory
-            *err = 1;
-            for (int i = max(0, asked - C::STAGES); i < asked; ++i)
-                for (int k = 0; k < kWaitLimit && !mbar_try_wait(&full[i % C::STAGES], i / C::STAGES & 1); ++k) {}
+        if (lane == 0) {
+            if (!ok) *err = 1;
+            kv8_copies_landed(full, C::STAGES, asked);                       // (those who read them may give up at any time)
         }
         return;
     }
 
     // ---------------- the others: page it of the share is warp it % WARPS's
     int it = 0;
+    bool ok = true;                                                          // false from the first wait on that ran out
     while (next()) {
         Kv8Query<D> a;
         a.clear();
         a.load_query(g < G ? q + ((size_t)seg_b * nq + (size_t)seg_h * G + g) * D : nullptr, tq);
-        bool ok = true;
-        for (int i = it + (warp - it % C::WARPS + C::WARPS) % C::WARPS; i < it + t1 - t0; i += C::WARPS) {
+        for (int i = it + (warp - it % C::WARPS + C::WARPS) % C::WARPS; ok && i < it + t1 - t0; i += C::WARPS) {
             const int s = i % C::STAGES;
-            ok = __all_sync(0xffffffffu, mbar_wait_limited(&full[s], i / C::STAGES & 1, &dead));
+            ok = __all_sync(0xffffffffu, kv8_mbar_wait_limited(&full[s], i / C::STAGES & 1, &dead, wait_limit));
             if (!ok) break;
             const int n = tokens[s];
             if (n) a.page(smem + s * Kv8<D>::REC, n, scale_log2, g, tq);
@@ -312,6 +313,9 @@ kv8_decode_kernel(const __half* __restrict__ q, const uint8_t* __restrict__ cach
     }
 }
 
+static std::atomic<int> g_kv8_wait_limit{kWaitLimit};
+int kv8_wait_limit() { return g_kv8_wait_limit.load(std::memory_order_relaxed); }
+
 // counters (one for each CTA that a split (sequence, head) can begin in), then two parts a CTA: of the (sequence, head) it begins in the middle of, and of the one it ends in
 static int kv8_decode_ctas() { return 2 * device_sms(); }
 static size_t kv8_decode_counters(int ctas) { return (size_t)(ctas + 63) / 64 * 64; }
@@ -333,12 +337,12 @@ static int launch_kv8_decode(const void* q, const void* cache, int num_pages, co
     const float scale_log2 = K8D_LOG2E / sqrtf((float)D);
     if (whole) {
         FT_CHECK_CUDA(launch_after(kv8_decode_kernel<D>, dim3(B * nkv), dim3(C::THREADS), C::SMEM, st, (const __half*)q, (const uint8_t*)cache, num_pages, page_table,
-                                   max_pages, ctx_lens, (__nv_bfloat16*)out, (__nv_bfloat16*)out_lo, counters, parts, B, nq, nkv, scale_log2));
+                                   max_pages, ctx_lens, (__nv_bfloat16*)out, (__nv_bfloat16*)out_lo, counters, parts, B, nq, nkv, scale_log2, kv8_wait_limit()));
         return 0;
     }
     FT_CHECK_CUDA(launch_after(kv8_decode_zero_kernel, dim3(1), dim3(128), 0, st, counters, ctas));
     FT_CHECK_CUDA(launch_after(kv8_decode_kernel<D>, dim3(ctas), dim3(C::THREADS), C::SMEM, st, (const __half*)q, (const uint8_t*)cache, num_pages, page_table,
-                               max_pages, ctx_lens, (__nv_bfloat16*)out, (__nv_bfloat16*)out_lo, counters, parts, B, nq, nkv, scale_log2));
+                               max_pages, ctx_lens, (__nv_bfloat16*)out, (__nv_bfloat16*)out_lo, counters, parts, B, nq, nkv, scale_log2, kv8_wait_limit()));
     return 0;
 }
 
@@ -349,6 +353,8 @@ extern "C" long long ft_attn_decode_kv8_scratch_bytes(int d) {
     const int ctas = ft::kv8_decode_ctas();
     return (long long)(ft::kv8_decode_counters(ctas) + 2 * (size_t)ctas * ft::K8D_GROUP * (d + 2)) * 4;
 }
+
+extern "C" void ft_kv8_set_wait_limit(int tries) { ft::g_kv8_wait_limit = tries < 0 || tries > ft::kWaitLimit ? ft::kWaitLimit : tries; }
 
 extern "C" int ft_kv8_waits(void) {
     int n = 0, m = 0;

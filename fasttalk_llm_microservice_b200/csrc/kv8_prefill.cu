@@ -83,21 +83,10 @@ __device__ __forceinline__ void tmem_arrived(uint32_t* r) {
     for (int c = 0; c < N; c += 8)
         asm volatile("" : "+r"(r[c]), "+r"(r[c + 1]), "+r"(r[c + 2]), "+r"(r[c + 3]), "+r"(r[c + 4]), "+r"(r[c + 5]), "+r"(r[c + 6]), "+r"(r[c + 7]));
 }
-// Waits that end, as those of common.cuh do, but a few instructions each: this kernel has some twenty of them among five kinds of warps, and its time hangs on what the
-// instruction caches hold (unrolled, they and the rest were 104 KB, and 16 KB more or less of waits outside the loops over pages was 8 % of its time)
-__device__ __forceinline__ bool small_mbar_wait_limited(uint64_t* bar, uint32_t parity, volatile int* dead, int limit = kWaitLimit) {
-#pragma unroll 1
-    for (int i = 0; i < limit; ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if (*dead) return false;
-    }
-    *dead = 1;
-    return false;
-}
-constexpr int kStretchLimit = 64 * kWaitLimit;   // a stretch may be a million keys
+constexpr int kStretchWaits = 64;                // times the limit, for what takes a whole stretch: it may be a million keys
 // A warp's wait (all lanes ask, so that the warp stays together)
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* dead, int limit = kWaitLimit) {
-    return __all_sync(0xffffffffu, small_mbar_wait_limited(bar, parity, dead, limit));
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* dead, int limit) {
+    return __all_sync(0xffffffffu, kv8_mbar_wait_limited(bar, parity, dead, limit));
 }
 
 __device__ int g_kv8_prefill_waits;              // 1: a wait ran out on this device (ft_kv8_waits)
@@ -120,7 +109,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
     __shared__ uint64_t seg_full[4], seg_empty[4];                           // a stretch has been told; all have done with it
     __shared__ uint64_t vmax_full;                                           // the largest scale of a stretch's values is known
     __shared__ uint64_t halves_met;                                          // all softmax warps are here
-    __shared__ uint64_t drained[2];                                          // all products of a half retired (after a wait that ran out)
+    __shared__ uint64_t drained[2];                                          // all products of a half retired
     __shared__ Kv8Stretch told[4];
     __shared__ unsigned vmax_s[4];                                           // bits of a number that is not negative: they order as it does
     __shared__ __align__(16) float kscale_s[C::S16][4];                      // times scale_log2; the first below 0: the page is not there
@@ -160,7 +149,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
     bool ok = true;                                                          // false: a wait ran out
     // the n-th stretch of the share, or one without pages behind the last; and this warp's word that it has done with it
     auto hear = [&](int n) {
-        ok = ok && warp_wait(&seg_full[n & 3], n >> 2 & 1, &dead, kStretchLimit);
+        ok = ok && warp_wait(&seg_full[n & 3], n >> 2 & 1, &dead, kStretchWaits * p.wait_limit);
         Kv8Stretch w = told[n & 3];
         if (!ok) w.pages = 0;
         return w;
@@ -205,10 +194,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
 #pragma unroll 1
             for (int n = 0, more = 1; more; ++n) {
                 more = w.next(p);
-                if (!small_mbar_wait_limited(&seg_empty[n & 3], (n >> 2 & 1) ^ 1, &dead, kStretchLimit)) {
-                    *err = 1;
-                    break;
-                }
+                if (!kv8_mbar_wait_limited(&seg_empty[n & 3], (n >> 2 & 1) ^ 1, &dead, kStretchWaits * p.wait_limit)) break;
                 if (more) told[n & 3] = w.stretch(p, per, blockIdx.x);
                 else told[n & 3].pages = 0;
                 vmax_s[n & 3] = 0;
@@ -238,7 +224,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                     const int page = __shfl_sync(0xffffffffu, my_page, k);
                     if (lane == 0 && go) {
                         const int s = it % C::S8;
-                        go = small_mbar_wait_limited(&rec_empty[s], (it / C::S8 & 1) ^ 1, &dead);
+                        go = kv8_mbar_wait_limited(&rec_empty[s], (it / C::S8 & 1) ^ 1, &dead, p.wait_limit);
                         if (!go) continue;
                         asked = it + 1;
                         const bool there = page >= 0 && page < p.num_pages;
@@ -254,13 +240,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
             }
             done(seg);
         }
-        if (lane == 0 && (!go || !ok || dead)) {                             // what is under way still lands in this CTA's memory
-            *err = 1;
-#pragma unroll 1
-            for (int i = max(0, asked - C::S8); i < asked; ++i)
-#pragma unroll 1
-                for (int k = 0; k < kWaitLimit && !mbar_try_wait(&rec_full[i % C::S8], i / C::S8 & 1); ++k) {}
-        }
+        if (lane == 0) kv8_copies_landed(rec_full, C::S8, asked);            // (those who read them may give up at any time)
       } else {
         // ---------------- products, one warp a half
         constexpr uint32_t idesc_qk = umma_idesc_f16(K8P_ROWS, kKvTile, false), idesc_pv = umma_idesc_f16(K8P_ROWS, D, true);
@@ -272,8 +252,8 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
         int base = 0, n_qk = 0, n_pv = 0;                                    // pages of the share, products of this half so far
         auto issue_qk = [&](int page, int qh) {                              // page: counted over the whole share
             const int s = page % C::S16, buf = n_qk % C::NS;
-            if (C::NS == 1) ok = small_mbar_wait_limited(&s_free[h], (n_qk & 1) ^ 1, &dead);
-            ok = ok && small_mbar_wait_limited(&kv_full[s], page / C::S16 & 1, &dead);
+            if (C::NS == 1) ok = kv8_mbar_wait_limited(&s_free[h], (n_qk & 1) ^ 1, &dead, p.wait_limit);
+            ok = ok && kv8_mbar_wait_limited(&kv_full[s], page / C::S16 & 1, &dead, p.wait_limit);
             if (!ok) return;
             ++n_qk;
             tc_fence_after();
@@ -286,7 +266,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
         };
         auto issue_pv = [&](int page, bool first, bool alone) {
             const int s = page % C::S16, buf = n_pv & 1;
-            ok = small_mbar_wait_limited(&p_full[h][buf], n_pv >> 1 & 1, &dead);
+            ok = kv8_mbar_wait_limited(&p_full[h][buf], n_pv >> 1 & 1, &dead, p.wait_limit);
             if (!ok) return;
             ++n_pv;
             tc_fence_after();
@@ -304,7 +284,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
             const int mine_n = w.few ? (w.pages - h + 1) / 2 : w.pages;      // page i of this half is page j of the stretch
             auto page_of = [&](int i) { return base + (w.few ? h + 2 * i : i); };
             if (lead) {
-                ok = small_mbar_wait_limited(&q_full, seg & 1, &dead);
+                ok = kv8_mbar_wait_limited(&q_full, seg & 1, &dead, p.wait_limit);
                 tc_fence_after();
                 if (ok && mine_n == 0) umma_commit(&q_empty);
                 // Scores run NS pages ahead.  With two buffers page i + 2's follow the product that reads page i's probabilities, which says that page i's scores
@@ -322,8 +302,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
             ok = __all_sync(0xffffffffu, ok);
             done(seg);
         }
-        if (!ok && lead) {                                                   // nothing may still run in tensor memory when it is given back
-            *err = 1;
+        if (lead) {                                                          // nothing may still run in tensor memory when it is given back, whoever gave up
             umma_commit(&drained[h]);
 #pragma unroll 1
             for (int k = 0; k < kWaitLimit && !mbar_try_wait(&drained[h], 0); ++k) {}
@@ -343,7 +322,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
             for (int step = 0; step < 2; ++step) {
                 if ((step == 0) == (seg == 0)) {
                     // the queries, 16 bytes at a time and all on their way at once; zeros for rows without a token
-                    if (seg) ok = warp_wait(&q_empty, (seg - 1) & 1, &dead);
+                    if (seg) ok = warp_wait(&q_empty, (seg - 1) & 1, &dead, p.wait_limit);
                     if (!ok) break;
                     constexpr int CH = D / 8;
 #pragma unroll 4
@@ -381,13 +360,13 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_full);
-                ok = warp_wait(&vmax_full, seg & 1, &dead);
+                ok = warp_wait(&vmax_full, seg & 1, &dead, p.wait_limit);
             }
             const float vmax = __uint_as_float(vmax_s[seg & 3]), vinv = vmax > 0.f ? 1.f / vmax : 0.f;
 #pragma unroll 1
             for (int k = 0; ok && k < w.pages; ++k, ++it) {
                 const int s8 = it % C::S8, s16 = it % C::S16;
-                ok = warp_wait(&rec_full[s8], it / C::S8 & 1, &dead) && warp_wait(&kv_empty[s16], (it / C::S16 & 1) ^ 1, &dead);
+                ok = warp_wait(&rec_full[s8], it / C::S8 & 1, &dead, p.wait_limit) && warp_wait(&kv_empty[s16], (it / C::S16 & 1) ^ 1, &dead, p.wait_limit);
                 if (!ok) break;
                 const uint8_t* rec = smem + C::REC + s8 * Kv8<D>::REC;
                 uint8_t* dst = smem + C::KV + s16 * C::TILE;
@@ -479,7 +458,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
 #pragma unroll 1
             for (int i = 0; i < mine_n; ++i, ++cnt) {
                 const int sb = cnt % C::NS, pb = cnt & 1;
-                ok = ok && warp_wait(&s_full[h][sb], cnt / C::NS & 1, &dead);
+                ok = ok && warp_wait(&s_full[h][sb], cnt / C::NS & 1, &dead, p.wait_limit);
                 if (!ok) break;
                 tc_fence_after();
                 uint32_t sr[64];
@@ -533,7 +512,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                     // rows without a token say nothing: a row's rounding depends on its own request alone
                     if (!__any_sync(0xffffffffu, valid && m_new > m_ref + K8P_GROW)) break;
                     known = true;
-                    ok = warp_wait(&pv_done[h][pb ^ 1], (cnt - 1) >> 1 & 1, &dead);
+                    ok = warp_wait(&pv_done[h][pb ^ 1], (cnt - 1) >> 1 & 1, &dead, p.wait_limit);
                     if (!ok) break;
                     tc_fence_after();
                     const float alpha = m_new == -INFINITY ? 1.f : exp2f(m_ref - m_new);
@@ -558,17 +537,16 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[h][pb]);
             }
-            if (ok && mine_n) ok = warp_wait(&pv_done[h][(cnt - 1) & 1], (cnt - 1) >> 1 & 1, &dead);
+            if (ok && mine_n) ok = warp_wait(&pv_done[h][(cnt - 1) & 1], (cnt - 1) >> 1 & 1, &dead, p.wait_limit);
             if (w.few && w.parts == 0) {                                     // the halves' maxima and sums; and a half without a page has waited for nothing yet
                 ml_s[st] = make_float2(m_ref, l_run);
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&halves_met);
-                ok = ok && warp_wait(&halves_met, met++ & 1, &dead);
+                ok = ok && warp_wait(&halves_met, met++ & 1, &dead, p.wait_limit);
             }
             tc_fence_after();
             if (!ok) {                                                       // NaN for all that this unit says
-                *err = 1;
                 l_run = NAN;
                 m_ref = 0.f;
             }
@@ -620,7 +598,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&halves_met);
-                    ok = ok && warp_wait(&halves_met, met++ & 1, &dead);
+                    ok = ok && warp_wait(&halves_met, met++ & 1, &dead, p.wait_limit);
                 }
             } else {
                 // a part: O in its own size, 16 bytes a row side by side, maximum and sum of each row; the halves of a unit of few tokens are two parts
@@ -645,9 +623,11 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
             base += w.pages;
             done(seg);
         }
+        tmem_st_wait();
     }
     tc_fence_before();
     __syncthreads();
+    if (tid == 0 && dead) *err = 1;
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, C::COLS);
@@ -803,6 +783,6 @@ extern "C" int ft_attn_prefill_kv8(const void* q, const void* kv8_layer, int num
     FT_REQUIRE(((uintptr_t)q | (uintptr_t)kv8_layer | (uintptr_t)out | (uintptr_t)out_lo | (uintptr_t)scratch) % 16 == 0, "ft_attn_prefill_kv8: tensors on 16 bytes");
     const int G = nq / nkv;
     Kv8Prompt p{(const __half*)q, (const uint8_t*)kv8_layer, page_table, req_q_start, req_slot, req_pos0, (__nv_bfloat16*)out, (__nv_bfloat16*)out_lo, nullptr, nullptr,
-                num_pages, table_rows, max_pages, n_req, T, nq, nkv, G, K8P_ROWS / G, d == 64 ? 2 : 1, (65536u + G - 1) / G, K8P_LOG2E / sqrtf((float)d)};
+                num_pages, table_rows, max_pages, n_req, T, nq, nkv, G, K8P_ROWS / G, d == 64 ? 2 : 1, ft::kv8_wait_limit(), (65536u + G - 1) / G, K8P_LOG2E / sqrtf((float)d)};
     return d == 64 ? launch_kv8_prefill<64>(p, scratch, (cudaStream_t)stream) : launch_kv8_prefill<128>(p, scratch, (cudaStream_t)stream);
 }

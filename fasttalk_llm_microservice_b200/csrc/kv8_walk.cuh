@@ -17,6 +17,7 @@ struct Kv8Prompt {
     int num_pages, table_rows, max_pages, n_req, T, nq, nkv;
     int G, th;                                                       // query heads a key head, tokens of a half
     int few_pages;                                                   // pages of a step of a unit of few tokens
+    int wait_limit;                                                  // tries of a wait
     unsigned inv_g;                                                  // row / G = row * inv_g >> 16
     float scale_log2;
 };

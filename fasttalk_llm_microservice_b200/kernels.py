@@ -386,6 +386,14 @@ def attn_prefill_kv8(q: torch.Tensor, kv8_layer: torch.Tensor, page_table: torch
     return out, lo
 
 
+def kv8_check(device=None) -> None:
+    """Waits for the device (the current one by default) and raises if a kernel of this cache has ever given up on a wait there: rows of some call since the library
+    was loaded mean nothing.  No call asks by itself, since that would make the host wait."""
+    with torch.cuda.device(device):
+        if N.check(N.load().ft_kv8_waits(), "ft_kv8_waits"):
+            raise N.NativeError("8-bit KV cache: a wait inside a kernel ran out; outputs of this process are not to be trusted")
+
+
 def _kv8_offsets(d: int, device) -> torch.Tensor:
     """Where the code of (keys 0 | values 1, token, dim) lies in a record."""
     t, i = torch.arange(KV_TILE, device=device)[:, None], torch.arange(d, device=device)[None, :]

@@ -129,6 +129,7 @@ SIGNATURES = {
     "ft_kv8_read": (_I, [_VP, _I, _VP, _I, _I, _VP, _VP, _VP, _I, _I, _VP, _VP, _I, _I, _VP]),
     "ft_attn_decode_kv8_scratch_bytes": (_LL, [_I]),
     "ft_kv8_waits": (_I, []),
+    "ft_kv8_set_wait_limit": (None, [_I]),
     "ft_attn_decode_kv8": (_I, [_VP, _VP, _I, _VP, _I, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _VP]),
     "ft_attn_prefill_kv8_scratch_bytes": (_LL, [_I]),
     "ft_attn_prefill_kv8": (_I, [_VP, _VP, _I, _VP, _I, _I, _VP, _VP, _VP, _I, _I, _VP, _VP, _VP, _I, _I, _I, _VP]),
