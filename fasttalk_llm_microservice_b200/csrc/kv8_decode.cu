@@ -358,6 +358,7 @@ extern "C" void ft_kv8_set_wait_limit(int tries) { ft::g_kv8_wait_limit = tries 
 
 extern "C" int ft_kv8_waits(void) {
     int n = 0, m = 0;
+    FT_CHECK_CUDA(cudaDeviceSynchronize());                                  // the copies below wait for the default stream only
     FT_CHECK_CUDA(cudaMemcpyFromSymbol(&n, ft::g_kv8_decode_waits, sizeof(n)));
     if (int r = ft::kv8_prefill_waits(&m)) return r;
     return n | m;

@@ -689,7 +689,7 @@ long long ft_attn_decode_kv8_scratch_bytes(int d);
 int ft_attn_decode_kv8(const void* q, const void* kv8_layer, int num_pages, const int* page_table, int max_pages, const int* ctx_lens, void* out,
                        void* out_lo, void* scratch, int B, int nq, int nkv, int d, void* stream);
 /* Every wait inside the kernels of this cache has a limit; one that runs out ends its CTA, and the rows that this CTA had a part in mean nothing (NaN, not written, or put together
- * without it).  -> 1 if that has happened on the current device since the library was loaded, else 0 (waits for the device).
+ * without it).  -> 1 if that has happened on the current device since the library was loaded, else 0.  Waits for all that the device has been given, on every stream.
  * ft_kv8_set_wait_limit: tries of a wait in the calls that follow (below 0: the library's own limit, a million).  With 0 every wait runs out at once, so that a host can see what it does then. */
 int ft_kv8_waits(void);
 void ft_kv8_set_wait_limit(int tries);

@@ -103,6 +103,17 @@ def test_waits_that_run_out(K):
     assert r.returncode == 0 and "gave up and went on" in r.stdout, r.stdout + r.stderr
 
 
+def test_the_flag_is_read_behind_every_stream(K):
+    """Streams that do not wait for the default one among them: what they still run could set the flag."""
+    from fasttalk_llm_microservice_b200 import native
+    st = torch.cuda.Stream()
+    assert native.load().ft_kv8_waits() == 0                   # (a first call may wait for other reasons)
+    with torch.cuda.stream(st):
+        torch.cuda._sleep(100_000_000)                         # some 50 ms
+    assert native.load().ft_kv8_waits() == 0
+    assert st.query()
+
+
 @pytest.fixture(scope="module", autouse=True)
 def no_wait_has_run_out(K):
     """After all of this file's calls, on whatever stream."""
