@@ -15,6 +15,11 @@ namespace ft {
 constexpr int kKv8Block = 16;                 // tokens that share a scale
 constexpr float kKv8Least = 7.888609052210118e-31f;      // 2^-100: a block with nothing larger is a block of zeros (its scale's reciprocal has to be a number)
 
+// What the prompt attention keeps of a query, in log2 units: m = a maximum of its scores, for the sum of probabilities in fp32; h = one of score + log2(value scale), for the
+// weights p * scale in fp16.  These are formed 2^7 / 2^h of their size: below 2^15 until h has grown by 2^8, and fp16's normal numbers reach down to 2^-21 of the largest.
+// m may lag by 2^30.  h is kept at or above m - 100, or a query whose weight lies on zeros would divide by nothing: values below 2^-100 of 1 count as zeros there.
+constexpr float kKv8Top = 7.f, kKv8GrowH = 8.f, kKv8GrowM = 30.f, kKv8Low = 100.f;
+
 template <int D>
 struct Kv8 {
     static constexpr int SLAB = kKvTile * D;              // codes of the keys (or values) of one page and head

@@ -41,7 +41,6 @@ constexpr int K8P_ROWS = 128;                    // rows of a half
 constexpr int K8P_GROUP = 8;                     // query heads a key head at most
 constexpr int K8P_PIECE = kKvTile * 128;         // [64 tokens][64 dims] in fp16; 64 rows of a Q block
 constexpr float K8P_LOG2E = 1.4426950408889634f;
-constexpr float K8P_GROW = 8.f;                  // O is rescaled when a row's maximum has grown by more than 2^8
 constexpr int K8P_WHOLE = 10;
 // (pages that a share may be shorter than a whole unit for parts not to pay: 5 / 10 / 15 for four portions of 100 tokens behind 300, heads of 128, 24.8 / 19.6 / 19.6 us; six of
 // 100 behind 1000 36.5 / 34.4 / 34.4, heads of 64 27.5 / 30.2 / 30.5; three of 150 behind 900 24.3 / 24.2 / 29.9; two of 300, heads of 128, 17 us whole and 22 in parts)
@@ -107,14 +106,14 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
     __shared__ uint64_t s_full[2][C::NS], s_free[2];                         // half, buffer: scores are in tensor memory; (NS = 1) and in registers
     __shared__ uint64_t p_full[2][2], pv_done[2][2];                         // probabilities are in tensor memory; O += P V retired
     __shared__ uint64_t seg_full[4], seg_empty[4];                           // a stretch has been told; all have done with it
-    __shared__ uint64_t vmax_full;                                           // the largest scale of a stretch's values is known
     __shared__ uint64_t halves_met;                                          // all softmax warps are here
     __shared__ uint64_t drained[2];                                          // all products of a half retired
     __shared__ Kv8Stretch told[4];
-    __shared__ unsigned vmax_s[4];                                           // bits of a number that is not negative: they order as it does
     __shared__ __align__(16) float kscale_s[C::S16][4];                      // times scale_log2; the first below 0: the page is not there
+    __shared__ __align__(16) float vscale_s[C::S16][4], vlog_s[C::S16][4];   // of the values; 0 for blocks behind the unit's last token.  And their log2
     __shared__ int blocks_s[C::S8];                                          // of 16 tokens, that some query of the unit sees; 0: the page is not there
     __shared__ float2 ml_s[K8P_SOFT];
+    __shared__ float size_s[K8P_SOFT];                                       // what a row's O is multiplied by to be in its own size
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int dead;
 
@@ -126,7 +125,6 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
         for (int s = 0; s < 4; ++s) mbar_init(&seg_full[s], 1), mbar_init(&seg_empty[s], K8P_LISTENERS);
         mbar_init(&q_full, K8P_CONV / 32);
         mbar_init(&q_empty, 2);
-        mbar_init(&vmax_full, K8P_CONV / 32);
         mbar_init(&halves_met, K8P_SOFT / 32);
         for (int h = 0; h < 2; ++h) {
             for (int s = 0; s < C::NS; ++s) mbar_init(&s_full[h][s], 1);
@@ -197,7 +195,6 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                 if (!kv8_mbar_wait_limited(&seg_empty[n & 3], (n >> 2 & 1) ^ 1, &dead, kStretchWaits * p.wait_limit)) break;
                 if (more) told[n & 3] = w.stretch(p, per, blockIdx.x);
                 else told[n & 3].pages = 0;
-                vmax_s[n & 3] = 0;
                 mbar_arrive(&seg_full[n & 3]);
             }
         }
@@ -318,51 +315,25 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
         for (int seg = 0;; ++seg) {
             const Kv8Stretch w = hear(seg);
             if (w.pages == 0) break;
-#pragma unroll 1
-            for (int step = 0; step < 2; ++step) {
-                if ((step == 0) == (seg == 0)) {
-                    // the queries, 16 bytes at a time and all on their way at once; zeros for rows without a token
-                    if (seg) ok = warp_wait(&q_empty, (seg - 1) & 1, &dead, p.wait_limit);
-                    if (!ok) break;
-                    constexpr int CH = D / 8;
-#pragma unroll 4
-                    for (int k = ct; k < (w.few ? 1 : 2) * K8P_ROWS * CH; k += K8P_CONV) {
-                        const int c = k % CH, rr = k / CH, h = rr >> 7, row = rr & 127;
-                        const int tok = row * p.inv_g >> 16, head = row - tok * p.G;
-                        const bool on = tok < p.th && h * p.th + tok < w.tokens;
-                        const __half* from = p.q + ((size_t)(w.row0 + (on ? h * p.th + tok : 0)) * p.nq + (size_t)w.head * p.G + (on ? head : 0)) * D + c * 8;
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem + (h * KH + (c >> 3)) * C::QBLK + row * 128 + ((c & 7) ^ (row & 7)) * 16)),
-                                     "l"(from), "r"(on ? 16 : 0)
-                                     : "memory");
-                    }
-                } else {
-                    // the largest scale of the stretch's values
-                    const int* pt = p.page_table + (size_t)w.slot * p.max_pages;
-                    const int end = w.slot >= 0 && w.slot < p.table_rows ? min(w.page0 + w.pages, p.max_pages) : 0;
-                    float vmax = 0.f;
-#pragma unroll 1
-                    for (int k = w.page0 + ct; k < end; k += K8P_CONV) {
-                        const int page = pt[k];
-                        if (page < 0 || page >= p.num_pages) continue;
-                        const float4 v = *reinterpret_cast<const float4*>(p.cache + ((size_t)page * p.nkv + w.head) * Kv8<D>::REC + Kv8<D>::SCALES + 16);
-                        const int seen = w.pos0 + w.tokens - 1 - k * kKvTile;        // blocks behind the last token do not count
-                        vmax = fmaxf(fmaxf(vmax, v.x), fmaxf(seen >= 16 ? v.y : 0.f, fmaxf(seen >= 32 ? v.z : 0.f, seen >= 48 ? v.w : 0.f)));
-                    }
-                    vmax = warp_max(vmax);
-                    if (lane == 0) {
-                        atomicMax(&vmax_s[seg & 3], __float_as_uint(vmax));
-                        mbar_arrive(&vmax_full);
-                    }
-                }
-            }
+            // the queries, 16 bytes at a time and all on their way at once; zeros for rows without a token
+            if (seg) ok = warp_wait(&q_empty, (seg - 1) & 1, &dead, p.wait_limit);
             if (ok) {
+                constexpr int CH = D / 8;
+#pragma unroll 4
+                for (int k = ct; k < (w.few ? 1 : 2) * K8P_ROWS * CH; k += K8P_CONV) {
+                    const int c = k % CH, rr = k / CH, h = rr >> 7, row = rr & 127;
+                    const int tok = row * p.inv_g >> 16, head = row - tok * p.G;
+                    const bool on = tok < p.th && h * p.th + tok < w.tokens;
+                    const __half* from = p.q + ((size_t)(w.row0 + (on ? h * p.th + tok : 0)) * p.nq + (size_t)w.head * p.G + (on ? head : 0)) * D + c * 8;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem + (h * KH + (c >> 3)) * C::QBLK + row * 128 + ((c & 7) ^ (row & 7)) * 16)),
+                                 "l"(from), "r"(on ? 16 : 0)
+                                 : "memory");
+                }
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_full);
-                ok = warp_wait(&vmax_full, seg & 1, &dead, p.wait_limit);
             }
-            const float vmax = __uint_as_float(vmax_s[seg & 3]), vinv = vmax > 0.f ? 1.f / vmax : 0.f;
 #pragma unroll 1
             for (int k = 0; ok && k < w.pages; ++k, ++it) {
                 const int s8 = it % C::S8, s16 = it % C::S16;
@@ -373,10 +344,13 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                 const int blocks = blocks_s[s8];
                 const float* scales = reinterpret_cast<const float*>(rec + Kv8<D>::SCALES);
                 // a block of zeros keeps a factor above 0, so that hidden scores stay minus infinity
-                if (ct < 4) kscale_s[s16][ct] = blocks ? fmaxf(scales[ct] * p.scale_log2, 1e-37f) : -1.f;
+                if (ct < 4) {
+                    const float v = ct < blocks ? scales[4 + ct] : 0.f;      // of a block behind the last token, whatever its scale is, nothing comes
+                    kscale_s[s16][ct] = blocks ? fmaxf(scales[ct] * p.scale_log2, 1e-37f) : -1.f;
+                    vscale_s[s16][ct] = v;
+                    vlog_s[s16][ct] = __log2f(fabsf(v));
+                }
                 if (blocks) {
-                    // a thread's tokens are of one block; of one behind the last token, whatever its scale is, nothing comes
-                    const __half2 f = __float2half2_rn(ct >> 6 < blocks ? scales[4 + (ct >> 6)] * vinv : 0.f);
 #pragma unroll
                     for (int u = ct; u < kKvTile * D / 16; u += K8P_CONV) {  // keys: 16 codes, two chunks of the swizzled row
                         const int piece = u >> 8, t = u >> 2 & 63, c = u & 3;
@@ -389,13 +363,9 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                     for (int u = ct; u < kKvTile * D / 16; u += K8P_CONV) {  // values, by where they lie
                         const int piece = u >> 8, slot = u >> 2 & 63, t = slot ^ (slot >> 1 & 1), c = (u & 3) ^ (t >> 1 & 2);
                         const uint4 x = *reinterpret_cast<const uint4*>(rec + Kv8<D>::SLAB + u * 16);
-                        auto mul = [&](uint32_t y) {
-                            const __half2 z = __hmul2(*reinterpret_cast<const __half2*>(&y), f);
-                            return *reinterpret_cast<const uint32_t*>(&z);
-                        };
                         uint8_t* at = dst + (KH + piece) * K8P_PIECE + t * 128;
-                        *reinterpret_cast<uint4*>(at + ((2 * c) ^ (t & 7)) * 16) = make_uint4(mul(kv8_lo(x.x)), mul(kv8_hi(x.x)), mul(kv8_lo(x.y)), mul(kv8_hi(x.y)));
-                        *reinterpret_cast<uint4*>(at + ((2 * c + 1) ^ (t & 7)) * 16) = make_uint4(mul(kv8_lo(x.z)), mul(kv8_hi(x.z)), mul(kv8_lo(x.w)), mul(kv8_hi(x.w)));
+                        *reinterpret_cast<uint4*>(at + ((2 * c) ^ (t & 7)) * 16) = make_uint4(kv8_lo(x.x), kv8_hi(x.x), kv8_lo(x.y), kv8_hi(x.y));
+                        *reinterpret_cast<uint4*>(at + ((2 * c + 1) ^ (t & 7)) * 16) = make_uint4(kv8_lo(x.z), kv8_hi(x.z), kv8_lo(x.w), kv8_hi(x.w));
                     }
                 } else {                                                     // hidden probabilities are zeros, and so must be what they are multiplied by
 #pragma unroll 1
@@ -431,9 +401,10 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                 }
             }
         }
-        // the largest of a page's scores, in log2 units
-        auto largest = [](const uint32_t* sr, const float* ks) {
+        // the largest of a page's scores, and of score + log2(value scale), in log2 units
+        auto largest = [](const uint32_t* sr, const float* ks, const float* vl, float& heavy) {
             float most = -INFINITY;
+            heavy = -INFINITY;
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
                 const uint32_t* x = sr + 16 * b;
@@ -441,7 +412,9 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                 t0 = max3(t0, x[6], x[7]), t1 = max3(t1, x[8], x[9]);
                 t0 = max3(t0, x[10], x[11]), t1 = max3(t1, x[12], x[13]);
                 t0 = max3(t0, x[14], x[15]);
-                most = fmaxf(most, fmaxf(t0, t1) * ks[b]);
+                const float t = fmaxf(t0, t1) * ks[b];
+                most = fmaxf(most, t);
+                heavy = fmaxf(heavy, t + vl[b]);
             }
             return most;
         };
@@ -453,7 +426,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
             const int mine_n = w.few ? (w.pages - h + 1) / 2 : w.pages;      // pages of this half
             const int my_tok = w.few ? tok : h * p.th + tok;
             const bool valid = tok < p.th && my_tok < w.tokens;
-            float m_ref = -INFINITY, l_run = 0.f;                            // in log2 units
+            float m_ref = -INFINITY, h_ref = -INFINITY, r = 1.f, l_run = 0.f;        // r = 2^(m - h + 7): a weight is p * scale * r
             int it = base + (w.few ? h : 0), ahead = w.pos0 + my_tok - (w.page0 + (w.few ? h : 0)) * kKvTile;     // page of the share; the row's position from the page's first key on
 #pragma unroll 1
             for (int i = 0; i < mine_n; ++i, ++cnt) {
@@ -467,6 +440,9 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                 // (the page's scales are visible: they were written ahead of the operands that the product behind this barrier read)
                 const float4 k4 = *reinterpret_cast<const float4*>(kscale_s[it % C::S16]);
                 const float ks[4] = {fabsf(k4.x), fabsf(k4.y), fabsf(k4.z), fabsf(k4.w)};
+                const float4 l4 = *reinterpret_cast<const float4*>(vlog_s[it % C::S16]);
+                const float vl[4] = {l4.x, l4.y, l4.z, l4.w};
+                const float* vs = vscale_s[it % C::S16];
                 tmem_arrived<64>(sr);
                 if constexpr (C::NS == 1) {                                  // the scores are in registers: the next ones may be formed
                     tc_fence_before();
@@ -481,10 +457,14 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                     for (int c = 0; c < 64; ++c) sr[c] = c <= seen ? sr[c] : 0xff800000u;
                 }
                 const uint32_t at = p_at + pb * 32;
-                // The exponentials are taken with the maximum of the pages before while this page's is found; where it has grown by too much they are taken again.
+                // The exponentials are taken with the references of the pages before while this page's are found; where one has grown by too much they are taken again.
                 // (The stretch's first page has nothing before it.)
                 bool known = i == 0;
-                if (known) m_ref = largest(sr, ks);
+                if (known) {
+                    m_ref = largest(sr, ks, vl, h_ref);
+                    h_ref = fmaxf(h_ref, m_ref - kKv8Low);
+                    r = m_ref == -INFINITY ? 1.f : exp2f(m_ref - h_ref + kKv8Top);
+                }
                 f32x2 sum[2];
 #pragma unroll 1
                 for (;;) {
@@ -497,27 +477,32 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
                             const int c = half * 32 + 2 * e;
-                            const float f = ks[c >> 4];
+                            const float f = ks[c >> 4], g = vs[c >> 4] * r;
                             float p0, p1;
                             unpack2(fma2(pack2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), pack2(f, f), minus), p0, p1);
                             p0 = ex2_fast(p0), p1 = ex2_fast(p1);
-                            sum[e & 1] = sum2(sum[e & 1], pack2(p0, p1));
+                            const f32x2 both = pack2(p0, p1);
+                            sum[e & 1] = sum2(sum[e & 1], both);
+                            unpack2(mul2(both, pack2(g, g)), p0, p1);
                             const __half2 t = __floats2half2_rn(p0, p1);
                             pk[e] = *reinterpret_cast<const uint32_t*>(&t);
                         }
                         tmem_st16(at + 16 * half, pk);
                     }
                     if (known) break;
-                    const float m_new = fmaxf(m_ref, largest(sr, ks));
+                    float h_new;
+                    const float m_new = fmaxf(m_ref, largest(sr, ks, vl, h_new));
+                    h_new = fmaxf(fmaxf(h_ref, h_new), m_new - kKv8Low);
                     // rows without a token say nothing: a row's rounding depends on its own request alone
-                    if (!__any_sync(0xffffffffu, valid && m_new > m_ref + K8P_GROW)) break;
+                    if (!__any_sync(0xffffffffu, valid && (m_new > m_ref + kKv8GrowM || h_new > h_ref + kKv8GrowH))) break;
                     known = true;
                     ok = warp_wait(&pv_done[h][pb ^ 1], (cnt - 1) >> 1 & 1, &dead, p.wait_limit);
                     if (!ok) break;
                     tc_fence_after();
-                    const float alpha = m_new == -INFINITY ? 1.f : exp2f(m_ref - m_new);
-                    l_run *= alpha;
+                    const float alpha = m_new == -INFINITY ? 1.f : exp2f(h_ref - h_new);
+                    if (m_new != -INFINITY) l_run *= exp2f(m_ref - m_new), r = exp2f(m_new - h_new + kKv8Top);
                     m_ref = m_new;
+                    h_ref = h_new;
 #pragma unroll 1
                     for (int c = 0; c < D / 16; ++c) {
                         uint32_t o[16];
@@ -540,6 +525,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
             if (ok && mine_n) ok = warp_wait(&pv_done[h][(cnt - 1) & 1], (cnt - 1) >> 1 & 1, &dead, p.wait_limit);
             if (w.few && w.parts == 0) {                                     // the halves' maxima and sums; and a half without a page has waited for nothing yet
                 ml_s[st] = make_float2(m_ref, l_run);
+                size_s[st] = 1.f / r;
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&halves_met);
@@ -550,15 +536,16 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                 l_run = NAN;
                 m_ref = 0.f;
             }
-            const float vref = ok ? __uint_as_float(*(volatile unsigned*)&vmax_s[seg & 3]) : 0.f;
+            const float size = 1.f / r;                                      // O times this is in its own size
             if (w.parts == 0) {
-                float inv = l_run == 0.f ? 0.f : vref / l_run, z = 1.f, zo = 0.f;        // a query without a visible key: zeros
+                float inv = l_run == 0.f ? 0.f : size / l_run, z = 1.f, zo = 0.f;        // a query without a visible key: zeros
                 if (w.few && ok) {
                     const float2 other = ml_s[st ^ K8P_ROWS];
                     const float m = fmaxf(m_ref, other.x);
                     z = m_ref == -INFINITY ? 0.f : exp2f(m_ref - m), zo = other.x == -INFINITY ? 0.f : exp2f(other.x - m);
                     const float L = h == 0 ? l_run * z + other.y * zo : other.y * zo + l_run * z;
-                    inv = L == 0.f ? 0.f : vref / L;
+                    inv = L == 0.f ? 0.f : 1.f / L;
+                    z *= size, zo *= size_s[st ^ K8P_ROWS];
                 }
                 const size_t off = ((size_t)(w.row0 + my_tok) * p.nq + (size_t)w.head * p.G + head) * D;
                 const int c0 = w.few ? h * (D / 32) : 0, c1 = w.few ? c0 + D / 32 : D / 16;      // few: each half of the warps puts half of the dims together
@@ -603,7 +590,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
             } else {
                 // a part: O in its own size, 16 bytes a row side by side, maximum and sum of each row; the halves of a unit of few tokens are two parts
                 float4* part = reinterpret_cast<float4*>(p.parts + (2 * (size_t)blockIdx.x + w.begins) * C::PART);
-                const float f = mine_n ? vref : 0.f;
+                const float f = mine_n ? size : 0.f;
 #pragma unroll 1
                 for (int c = 0; c < D / 16; ++c) {
                     uint32_t o[16];

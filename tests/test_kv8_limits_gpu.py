@@ -1,4 +1,10 @@
-"""The 8-bit KV cache's kernels at the edges of what they promise: lists of any kind, memory around the outputs, waits that run out."""
+"""The 8-bit KV cache's kernels at the edges of what they promise: lists of any kind, memory around the outputs, waits that run out, scales far apart, every key counted once.
+
+Tolerance of attention, for an element of the output, w the exact probabilities, v the values, s their blocks' scales: a weight times its scale is rounded to fp16 (2^-11 of it;
+below fp16's normal numbers 2^-25 with the largest at 2^7 or more, times a code of at most 128: n * 2^-25 * max(w s) for n keys); a score of d products summed in fp32 is off by
+delta = (d + 8) * 2^-23 * sum |q k| / sqrt(d) at worst, once in the numerator and once in the sum; an instruction adds 16 keys to an fp32 sum, off by 2^-22 of it: n * 2^-26;
+exponentials and references 2^-18 together.  So ((2^-11 + 2^-18 + 2 delta + n * 2^-26) * sum w |v| + n * 2^-25 * max(w s)), over the keys that the row sees and no others."""
+import math
 import os
 import subprocess
 import sys
@@ -7,7 +13,7 @@ import pytest
 import torch
 
 from test_kernels_gpu import Guarded
-from test_kv8_gpu import DEV, check_prompt, i32, prompt_case
+from test_kv8_gpu import DEV, F64, check_prompt, gen, i32, prompt_case, tables, values
 
 pytestmark = pytest.mark.gpu
 
@@ -131,3 +137,144 @@ def test_long_lists_that_do_not_grow_are_not_walked(K, nq, nkv, d):
         guarded_prefill(K, (q, cache, table, bad, slots, pos0))
     small = prompt_case(K, [(100, 40), (0, 30), (7, 5)], nq, nkv, d, seed=3)
     check_prompt(K, small, planes=2)
+
+
+def tight(K, q, cache, row, pos0):
+    """Rows of q [T][nq][d] at positions pos0 .. of a page-table row -> (out, tolerance) [T][nq][d] in 64 bits."""
+    T, nq, d = q.shape
+    G = nq // cache.shape[1]
+    n = max(0, min(pos0 + T, row.numel() * 64))
+    x, there = values(K, cache, row, n, d)
+    if n == 0:
+        return torch.zeros(T, nq, d, device=DEV, dtype=F64), torch.zeros(T, nq, d, device=DEV, dtype=F64)
+    pages = row[: -(-n // 64)].long()
+    _, sc = K.kv8_codes(cache[torch.where((pages >= 0) & (pages < cache.shape[0]), pages, 0)], d)
+    s = sc[:, :, 1].to(F64).repeat_interleave(16, -1).transpose(1, 2).reshape(-1, cache.shape[1])[:n].repeat_interleave(G, 1)          # [n][nq]
+    k, v = x[0].repeat_interleave(G, 1), x[1].repeat_interleave(G, 1)
+    qd = q.to(F64)
+    hidden = ((torch.arange(n, device=DEV)[None, :] > pos0 + torch.arange(T, device=DEV)[:, None]) | ~there[None, :])[None]
+    scores = (torch.einsum("thd,nhd->htn", qd, k) / math.sqrt(d)).masked_fill(hidden, -math.inf)
+    size = (torch.einsum("thd,nhd->htn", qd.abs(), k.abs()) / math.sqrt(d)).masked_fill(hidden, 0.0).amax(-1)                           # [h][t]
+    m = scores.amax(-1, keepdim=True)
+    w = torch.exp(scores - torch.where(m > -math.inf, m, 0.0))
+    w = w / torch.where(m > -math.inf, w.sum(-1, keepdim=True), 1.0)
+    out = torch.einsum("htn,nhd->thd", w, v)
+    rel = 2.0 ** -11 + 2.0 ** -18 + 2 * (d + 8) * 2.0 ** -23 * size.T + n * 2.0 ** -26
+    tol = rel[..., None] * torch.einsum("htn,nhd->thd", w, v.abs()) + n * 2.0 ** -25 * (w * s.T[:, None]).amax(-1).T[..., None]
+    return out, tol
+
+
+def near(got, want, tol):
+    """Two planes: the sum is within the tolerance and half a step of the second plane."""
+    off = ((got[0].to(F64) + got[1].to(F64)).reshape(want.shape) - want).abs()
+    over = off - tol - want.abs() * 2.0 ** -15 - 1e-36
+    assert over.numel() == 0 or over.max().item() <= 0, (off.max().item(), (off / (tol + 1e-36)).max().item())
+
+
+def both_kinds(K, q, cache, table, reqs):
+    """Prompt attention of all portions against 64 bits."""
+    starts = [0]
+    for _, n in reqs:
+        starts.append(starts[-1] + n)
+    want = [tight(K, q[a:b], cache, table[i], p) for i, ((p, _), a, b) in enumerate(zip(reqs, starts, starts[1:]))]
+    near(K.attn_prefill_kv8(q, cache, table, i32(starts), i32(list(range(len(reqs)))), i32([p for p, _ in reqs])), torch.cat([o for o, _ in want]), torch.cat([t for _, t in want]))
+
+
+# ------------------------------------------------------------------------------------------------ values of very different size
+@pytest.mark.parametrize("nq,nkv,d", [(8, 2, 64), (6, 2, 128), (4, 4, 128), (8, 1, 64)])
+@pytest.mark.parametrize("reqs", [[(0, 100)], [(40, 70), (0, 1), (130, 200)], [(700, 5), (0, 16), (64, 3)]])
+@pytest.mark.parametrize("step", [30.0, 1.0 / 30.0])
+def test_values_of_later_tokens_do_not_touch_earlier_rows(K, nq, nkv, d, reqs, step):
+    """Every block's values are thirty times larger (or smaller) than those of the block before it: what a row does not see takes none of its bits."""
+    q, cache, table, *_ = prompt_case(K, reqs, nq, nkv, d, seed=nq + d)
+    codes, scales = K.kv8_codes(cache, d)
+    for i, (p, n) in enumerate(reqs):
+        for b in range(-(-(p + n) // 16)):
+            scales[int(table[i, b // 4]), :, 1, b % 4] = 0.01 * step ** (b - (p + n) / 32)
+    both_kinds(K, q, K.kv8_records(codes, scales.clamp(max=500.0)), table, reqs)
+
+
+@pytest.mark.parametrize("nq,nkv,d", [(8, 2, 64), (6, 2, 128)])
+@pytest.mark.parametrize("large", [40.0, 500.0])
+def test_large_values_that_nobody_attends_to(K, nq, nkv, d, large):
+    """A block of values up to 65504 whose keys lie far on the other side of the queries, and values of 0.1 everywhere else."""
+    reqs = [(1990, 10), (60, 200), (0, 64)]
+    q, cache, table, *_ = prompt_case(K, reqs, nq, nkv, d, seed=d)
+    q = q.abs() * 0.2
+    codes, scales = K.kv8_codes(cache, d)
+    scales[:, :, 1] = 0.001
+    for i, page in ((0, 3), (0, 20), (1, 1), (2, 0)):
+        page = int(table[i, page])
+        scales[page, :, 0, 1], scales[page, :, 1, 1] = 1.0, large
+        codes[page, :, 0, 16:32] = 1
+    both_kinds(K, q, K.kv8_records(codes, scales), table, reqs)
+
+
+@pytest.mark.parametrize("nq,nkv,d", [(8, 2, 64), (6, 2, 128)])
+def test_blocks_of_zeros_that_all_attend_to(K, nq, nkv, d):
+    """Nearly all weight on keys whose values are zeros (their codes may be anything): the rest of the values keeps its bits."""
+    reqs = [(300, 40), (0, 130), (500, 1)]
+    q, cache, table, *_ = prompt_case(K, reqs, nq, nkv, d, seed=2 * d)
+    q = q.abs() * 0.5
+    codes, scales = K.kv8_codes(cache, d)
+    for i in range(3):
+        page = int(table[i, 0])
+        scales[page, :, 0, 0], scales[page, :, 1, 0] = 0.01, 0.0
+        codes[page, :, 0, :16] = 200
+    both_kinds(K, q, K.kv8_records(codes, scales), table, reqs)
+
+
+# ------------------------------------------------------------------------------------------------ every key counted, and once
+def means(K, nq, nkv, d, lengths, seed):
+    g = gen(seed)
+    pages = sum(-(-n // 64) for n in lengths) + 2
+    table = tables(lengths, pages, g)
+    codes = torch.randint(1, 256, (pages, nkv, 2, 64, d), generator=g, device=DEV).to(torch.uint8)
+    codes[:, :, 1] = 128
+    number = 1 + torch.arange(64, device=DEV) * 37 % 127                               # of a token
+    for i, n in enumerate(lengths):
+        for p in range(-(-n // 64)):
+            codes[int(table[i, p]), :, 1, :, p % d] = (128 + number).to(torch.uint8)[None]
+    cache = K.kv8_records(codes, torch.full((pages, nkv, 2, 4), 0.0078125, device=DEV))
+    most = max(1, max(lengths))
+    weight = torch.zeros(-(-most // 64) * 64, d, device=DEV, dtype=F64)
+    at = torch.arange(weight.shape[0], device=DEV)
+    weight[at, at // 64 % d] = number[at % 64].to(F64) / 128
+    sums = weight.cumsum(0)
+
+    def want(last, real):
+        """Means up to and with position `last`, zeros where there is no key."""
+        m = sums[last] / (last + 1)[:, None].to(F64) * real[:, None]
+        return m[:, None].expand(len(last), nq, d)
+    return cache, table, want
+
+
+@pytest.mark.parametrize("nq,nkv,d", [(32, 8, 64), (32, 8, 128), (16, 4, 128), (5, 1, 64), (16, 16, 128)])
+@pytest.mark.parametrize("lengths", [[20000], [9000, 1, 0, 500], [64 * 40] * 9, [300] * 70 + [5000], [(i * 97) % 900 for i in range(200)], [77], [64, 65]])
+def test_decode_counts_every_key_once(K, nq, nkv, d, lengths):
+    """Queries of zeros: the result is the mean of the values, and each page has a dim (of d) and each token a number of its own."""
+    cache, table, want = means(K, nq, nkv, d, lengths, seed=len(lengths))
+    q = torch.zeros(len(lengths), nq, d, device=DEV, dtype=torch.float16)
+    ends = torch.tensor([max(0, n - 1) for n in lengths], device=DEV)
+    near(K.attn_decode_kv8(q, cache, table, i32(lengths)), want(ends, i32(lengths) > 0), torch.zeros((), device=DEV, dtype=F64))
+
+
+@pytest.mark.parametrize("nq,nkv,d", [(32, 8, 64), (32, 8, 128), (3, 1, 128), (16, 16, 128), (16, 2, 64), (5, 1, 64)])
+@pytest.mark.parametrize("reqs", [[(0, 700)], [(16001, 5)], [(2990, 33), (0, 300), (100, 64), (1500, 1)], [(30 * i, 1 + 7 * i) for i in range(20)], [(300, 100)] * 4, [(900, 60)] * 19, [(63, 2)]])
+def test_prefill_counts_every_key_once(K, nq, nkv, d, reqs):
+    lengths = [p + n for p, n in reqs]
+    cache, table, want = means(K, nq, nkv, d, lengths, seed=len(reqs))
+    starts = [0]
+    for _, n in reqs:
+        starts.append(starts[-1] + n)
+    q = torch.zeros(starts[-1], nq, d, device=DEV, dtype=torch.float16)
+    last = torch.tensor([p + j for p, n in reqs for j in range(n)], device=DEV)
+    got = K.attn_prefill_kv8(q, cache, table, i32(starts), i32(list(range(len(reqs)))), i32([p for p, _ in reqs]))
+    near(got, want(last, torch.ones_like(last)), torch.zeros((), device=DEV, dtype=F64))
+
+
+@pytest.mark.parametrize("nq,nkv,d", [(32, 8, 64), (24, 8, 128), (7, 1, 64)])
+@pytest.mark.parametrize("reqs", [[(9000, 3), (50, 2)], [(64 * i, 1) for i in range(30)], [(0, 400), (333, 100)]])
+def test_attention_element_by_element(K, nq, nkv, d, reqs):
+    q, cache, table, *_ = prompt_case(K, reqs, nq, nkv, d, seed=nq)
+    both_kinds(K, q, cache, table, reqs)
