@@ -15,7 +15,7 @@ namespace ft {
 constexpr int kKv8Block = 16;                 // tokens that share a scale
 constexpr float kKv8Least = 7.888609052210118e-31f;      // 2^-100: a block with nothing larger is a block of zeros (its scale's reciprocal has to be a number)
 
-// What the prompt attention keeps of a query, in log2 units: m = a maximum of its scores, for the sum of probabilities in fp32; h = one of score + log2(value scale), for the
+// What both attention kernels keep of a query, in log2 units: m = a maximum of its scores, for the sum of probabilities in fp32; h = one of score + log2(value scale), for the
 // weights p * scale in fp16.  These are formed 2^7 / 2^h of their size: below 2^15 until h has grown by 2^8, and fp16's normal numbers reach down to 2^-21 of the largest.
 // m may lag by 2^30.  h is kept at or above m - 100, or a query whose weight lies on zeros would divide by nothing: values below 2^-100 of 1 count as zeros there.
 constexpr float kKv8Top = 7.f, kKv8GrowH = 8.f, kKv8GrowM = 30.f, kKv8Low = 100.f;
@@ -74,19 +74,20 @@ __device__ __forceinline__ void kv8_copies_landed(uint64_t* full, int stages, in
 // lanes have them (Q is loaded in the same).  The probabilities, transposed 8 x 8 at a time, are the B operand of O^T[dim][query] = V^T P^T, where all 16 rows are dims:
 // 8 neighbouring ones of each 64 a lane.  (With the queries in the rows of the first product nothing is transposed, but half the rows are zeros: 32 products a page
 // instead of 16 at D = 64, and their operands put together by 200 moves.)
-// Codes are multiplied as they are; the keys' scale goes to the exponents, the values' to the probabilities, relative to the largest values' scale that the warp has
-// seen (vref), or small values would leave fp16's range.
+// Codes are multiplied as they are; the keys' scale goes to the exponents, the values' to the probabilities.  Such a weight p * scale is rounded to fp16 relative to the
+// largest of its query so far (kKv8Top above): neither a large value without weight nor a key without a value takes another's bits.
 template <int D>
 struct Kv8Query {
     uint32_t q[D / 16][2];      // B operand
-    float o[D / 16][4];         // O^T / vref: dims 64 sub + 8 g + 2 i (+ 1), queries 2 tq (+ 1), at [4 sub + i][2 * (dim & 1) + (query & 1)]
-    float m[2], l[2], vref;     // of queries 2 tq (+ 1): maximum in log2 units, this lane's tokens' sum
+    float o[D / 16][4];         // O^T times r: dims 64 sub + 8 g + 2 i (+ 1), queries 2 tq (+ 1), at [4 sub + i][2 * (dim & 1) + (query & 1)]
+    float m[2], h[2], r[2], l[2];       // of queries 2 tq (+ 1): the references, 2^(m - h + 7), this lane's tokens' sum
 
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-        m[0] = m[1] = -INFINITY;
-        l[0] = l[1] = vref = 0.f;
+        m[0] = m[1] = h[0] = h[1] = -INFINITY;
+        r[0] = r[1] = 1.f;
+        l[0] = l[1] = 0.f;
     }
     // row: query head g of the group, or null
     __device__ __forceinline__ void load_query(const __half* row, int tq) {
@@ -107,7 +108,7 @@ struct Kv8Query {
         const float4 k4 = *reinterpret_cast<const float4*>(rec + Kv8<D>::SCALES);
         float4 vs = *reinterpret_cast<const float4*>(rec + Kv8<D>::SCALES + 16);
         const float ks[4] = {k4.x * scale_log2, k4.y * scale_log2, k4.z * scale_log2, k4.w * scale_log2};
-        float s[4][4], most[2] = {-INFINITY, -INFINITY};
+        float s[4][4], most[2] = {-INFINITY, -INFINITY}, heavy[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int b = 0; b < 4; ++b) {                                // a block of 16 tokens
             s[b][0] = s[b][1] = s[b][2] = s[b][3] = 0.f;
@@ -130,43 +131,51 @@ struct Kv8Query {
             if (n <= 32) vs.z = 0.f;
             if (n <= 48) vs.w = 0.f;
         }
+        const float vscale[4] = {vs.x, vs.y, vs.z, vs.w}, vl[4] = {__log2f(fabsf(vs.x)), __log2f(fabsf(vs.y)), __log2f(fabsf(vs.z)), __log2f(fabsf(vs.w))};
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
             const float f = fmaxf(ks[b], 1e-37f);                    // a block of zeros: hidden scores stay minus infinity
-            most[0] = fmaxf(most[0], fmaxf(s[b][0], s[b][2]) * f);
-            most[1] = fmaxf(most[1], fmaxf(s[b][1], s[b][3]) * f);
+            const float t0 = fmaxf(s[b][0], s[b][2]) * f, t1 = fmaxf(s[b][1], s[b][3]) * f;
+            most[0] = fmaxf(most[0], t0);
+            most[1] = fmaxf(most[1], t1);
+            heavy[0] = fmaxf(heavy[0], t0 + vl[b]);
+            heavy[1] = fmaxf(heavy[1], t1 + vl[b]);
         }
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) {
-            most[0] = fmaxf(most[0], __shfl_xor_sync(0xffffffffu, most[0], x));
-            most[1] = fmaxf(most[1], __shfl_xor_sync(0xffffffffu, most[1], x));
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                most[e] = fmaxf(most[e], __shfl_xor_sync(0xffffffffu, most[e], x));
+                heavy[e] = fmaxf(heavy[e], __shfl_xor_sync(0xffffffffu, heavy[e], x));
+            }
         }
-        const float v_new = fmaxf(vref, fmaxf(fmaxf(vs.x, vs.y), fmaxf(vs.z, vs.w)));
-        const float v_inv = v_new > 0.f ? __fdividef(1.f, v_new) : 0.f;
-        if (__any_sync(0xffffffffu, most[0] > m[0] || most[1] > m[1] || v_new > vref)) {     // after the first few pages rarely
+        const bool grown = most[0] > m[0] + kKv8GrowM || most[1] > m[1] + kKv8GrowM || heavy[0] > h[0] + kKv8GrowH || heavy[1] > h[1] + kKv8GrowH;
+        if (__any_sync(0xffffffffu, grown)) {                        // after the first few pages rarely
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const float m_new = fmaxf(m[e], most[e]);            // finite: a page has a token
-                const float alpha = ex2_fast(m[e] - m_new), keep = alpha * (vref * v_inv);
-                l[e] *= alpha;
+                const float h_new = fmaxf(fmaxf(h[e], heavy[e]), m_new - kKv8Low);
+                const float keep = ex2_fast(h[e] - h_new);
+                l[e] *= ex2_fast(m[e] - m_new);
                 m[e] = m_new;
+                h[e] = h_new;
+                r[e] = ex2_fast(m_new - h_new + kKv8Top);
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) o[i][e] *= keep, o[i][2 + e] *= keep;
             }
-            vref = v_new;
         }
-        const float vscale[4] = {vs.x * v_inv, vs.y * v_inv, vs.z * v_inv, vs.w * v_inv};
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
             const float f = fmaxf(ks[b], 1e-37f);
             const float p0 = ex2_fast(fmaf(s[b][0], f, -m[0])), p1 = ex2_fast(fmaf(s[b][1], f, -m[1]));
             const float p2 = ex2_fast(fmaf(s[b][2], f, -m[0])), p3 = ex2_fast(fmaf(s[b][3], f, -m[1]));
+            const float g0 = vscale[b] * r[0], g1 = vscale[b] * r[1];
             l[0] += p0 + p2;
             l[1] += p1 + p3;
             uint32_t pb[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const __half2 t = h ? __floats2half2_rn(p2 * vscale[b], p3 * vscale[b]) : __floats2half2_rn(p0 * vscale[b], p1 * vscale[b]);
+                const __half2 t = h ? __floats2half2_rn(p2 * g0, p3 * g1) : __floats2half2_rn(p0 * g0, p1 * g1);
                 asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pb[h]) : "r"(*reinterpret_cast<const uint32_t*>(&t)));
             }
 #pragma unroll
@@ -192,9 +201,10 @@ struct Kv8Query {
             float sum = l[e];
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            const float size = 1.f / r[e];
             float* at = rec + (size_t)(2 * tq + e) * (D + 2);
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) *reinterpret_cast<float2*>(at + (i >> 2) * 64 + 8 * g + 2 * (i & 3)) = make_float2(o[i][e] * vref, o[i][2 + e] * vref);
+            for (int i = 0; i < D / 16; ++i) *reinterpret_cast<float2*>(at + (i >> 2) * 64 + 8 * g + 2 * (i & 3)) = make_float2(o[i][e] * size, o[i][2 + e] * size);
             if (g == 0) *reinterpret_cast<float2*>(at + D) = make_float2(m[e], sum);
         }
     }

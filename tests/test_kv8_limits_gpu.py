@@ -172,12 +172,16 @@ def near(got, want, tol):
 
 
 def both_kinds(K, q, cache, table, reqs):
-    """Prompt attention of all portions against 64 bits."""
+    """Prompt attention of all portions; decode of each portion's last token; both against 64 bits."""
     starts = [0]
     for _, n in reqs:
         starts.append(starts[-1] + n)
     want = [tight(K, q[a:b], cache, table[i], p) for i, ((p, _), a, b) in enumerate(zip(reqs, starts, starts[1:]))]
     near(K.attn_prefill_kv8(q, cache, table, i32(starts), i32(list(range(len(reqs)))), i32([p for p, _ in reqs])), torch.cat([o for o, _ in want]), torch.cat([t for _, t in want]))
+    last = [i for i, (_, n) in enumerate(reqs) if n]
+    rows = [starts[i + 1] - 1 for i in last]
+    near(K.attn_decode_kv8(q[rows].contiguous(), cache, table[last].contiguous(), i32([sum(reqs[i]) for i in last])),
+         torch.stack([want[i][0][-1] for i in last]), torch.stack([want[i][1][-1] for i in last]))
 
 
 # ------------------------------------------------------------------------------------------------ values of very different size
