@@ -75,7 +75,6 @@ kv8_append_kernel(const Kv8Append p, int kv_rows, int kv_ctas) {
     constexpr int LR = D / 4, RP = 32 / LR, N = kKv8Block / RP, HL = D / 8;      // lanes a row, rows a pass, passes; lanes of half a row
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int sub = lane % LR, rsub = lane / LR;
-    const int angles = min(p.n_angles, p.max_pages * kKvTile);
     const size_t width = (size_t)(p.nq + 2 * p.nkv) * D;
 
     if ((int)blockIdx.x >= kv_ctas) {
@@ -85,7 +84,7 @@ kv8_append_kernel(const Kv8Append p, int kv_rows, int kv_ctas) {
         const int t = (int)(task / groups), h0 = (int)(task % groups) * K8_QHEADS;
         if (t >= p.T) return;
         const int pos = p.positions[t];
-        const bool on = pos >= 0 && pos < angles;
+        const bool on = pos >= 0 && pos < p.n_angles;
         const float4 c = load_f4(p.cos_t + (size_t)(on ? pos : 0) * (D / 2) + (sub % HL) * 4), s = load_f4(p.sin_t + (size_t)(on ? pos : 0) * (D / 2) + (sub % HL) * 4);
         const float* row = p.qkv + (size_t)t * width + sub * 4;
         float4 x[K8_QHEADS / RP];
@@ -144,7 +143,7 @@ kv8_append_kernel(const Kv8Append p, int kv_rows, int kv_ctas) {
             for (int i = 0; i < N; ++i) {
                 const int r = i * RP + rsub;
                 const int ps = __shfl_sync(0xffffffffu, run_pos, base + r);
-                const bool on = r < n && ps < angles;
+                const bool on = r < n && ps < p.n_angles;
                 if (!is_v) {
                     const size_t at = (size_t)(on ? ps : 0) * (D / 2) + (sub % HL) * 4;
                     x[i] = kv8_rotate<D>(x[i], load_f4(p.cos_t + at), load_f4(p.sin_t + at), sub);
@@ -183,7 +182,7 @@ kv8_append_kernel(const Kv8Append p, int kv_rows, int kv_ctas) {
                 for (int i = 0; i < N; ++i) {
                     const int r = i * RP + rsub;
                     const int ps = __shfl_sync(0xffffffffu, run_pos, base + r);
-                    if (r < n && ps < angles) *code_at(ps & 15) = code(x[i].x) | code(x[i].y) << 8 | code(x[i].z) << 16 | code(x[i].w) << 24;
+                    if (r < n && ps < p.n_angles) *code_at(ps & 15) = code(x[i].x) | code(x[i].y) << 8 | code(x[i].z) << 16 | code(x[i].w) << 24;
                 }
                 __syncwarp();
                 if (lane == 0) *scale = s;

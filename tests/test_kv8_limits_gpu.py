@@ -13,7 +13,7 @@ import pytest
 import torch
 
 from test_kernels_gpu import Guarded
-from test_kv8_gpu import DEV, F64, check_prompt, gen, i32, prompt_case, tables, values
+from test_kv8_gpu import DEV, F64, check_prompt, gen, i32, prompt_case, rotated, tables, values
 
 pytestmark = pytest.mark.gpu
 
@@ -282,3 +282,18 @@ def test_prefill_counts_every_key_once(K, nq, nkv, d, reqs):
 def test_attention_element_by_element(K, nq, nkv, d, reqs):
     q, cache, table, *_ = prompt_case(K, reqs, nq, nkv, d, seed=nq)
     both_kinds(K, q, cache, table, reqs)
+
+
+# ------------------------------------------------------------------------------------------------ writing
+def test_queries_beyond_the_page_table_are_rotated(K):
+    """q is 0 where there is no angle; a position that only the page table lacks has one (prompt attention lets such queries see what there is)."""
+    nq, nkv, d = 3, 1, 64
+    cache, table = K.kv8_cache_alloc(1, nkv, d, DEV), i32([[0]])
+    x = torch.randn(1, 5, (nq + 2 * nkv) * d, generator=gen(1), device=DEV)
+    ang = torch.rand(100, d // 2, generator=gen(2), device=DEV, dtype=F64)
+    cos, sin, pos = ang.cos().float(), ang.sin().float(), i32([63, 64, 99, 100, 1 << 30])
+    q = K.rope_kv8_append(x, cos, sin, pos, i32([0] * 5), table, cache, nq, nkv, d)
+    want, k, v = rotated(x, cos, sin, pos.clamp(max=99), nq, nkv, d)
+    assert ((q[:3].to(F64) - want[:3]).abs() <= want[:3].abs() * 2.0 ** -11 + 2.0 ** -19).all() and (q[3:] == 0).all()
+    _, s = K.kv8_codes(cache, d)
+    assert (s[0, 0, :, :3] == 0).all() and (s[0, 0, :, 3] > 0).all()
