@@ -159,6 +159,11 @@ kv8_append_kernel(const Kv8Append p, int kv_rows, int kv_ctas) {
             rows = __reduce_or_sync(0xffffffffu, rows);
             low = __reduce_min_sync(0xffffffffu, low);
             if (first == t0 + i0) held = (1u << low) - 1;
+            if (__popc(rows) < n) {
+                // a token whose row a later one of these 16 takes is not written: of two stores at once either could stand
+                const unsigned like = __match_any_sync(0xffffffffu, lane >= base && lane < base + n ? run_pos : -1 - lane);
+                if (like >> lane >> 1) run_pos = INT32_MAX;
+            }
             if (rows) {
                 const float s_old = held ? s_was : 0.f;
                 const float s_new = a > kKv8Least ? a / 127.f : 0.f;

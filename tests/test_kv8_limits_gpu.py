@@ -297,3 +297,20 @@ def test_queries_beyond_the_page_table_are_rotated(K):
     assert ((q[:3].to(F64) - want[:3]).abs() <= want[:3].abs() * 2.0 ** -11 + 2.0 ** -19).all() and (q[3:] == 0).all()
     _, s = K.kv8_codes(cache, d)
     assert (s[0, 0, :, :3] == 0).all() and (s[0, 0, :, 3] > 0).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("pos", [[3, 3], [0, 1, 2, 2, 2, 3, 1, 1, 0], [5] * 16, [5] * 17 + [4, 4], list(range(16)) + [3, 15, 7] + [2] * 20, [9, 8, 9, 8, 9, 8, 9]])
+def test_the_later_of_two_tokens_for_one_row_stands(K, d, pos):
+    nq, nkv = 1, 2
+    x = torch.randn(1, len(pos), (nq + 2 * nkv) * d, generator=gen(d), device=DEV)
+    ones, zeros = torch.ones(16, d // 2, device=DEV), torch.zeros(16, d // 2, device=DEV)
+    for _ in range(20):
+        cache = K.kv8_cache_alloc(1, nkv, d, DEV)
+        K.rope_kv8_append(x, ones, zeros, i32(pos), i32([0] * len(pos)), i32([[0]]), cache, nq, nkv, d)
+        k, v = K.kv8_read(cache, i32([[0]]), i32([0, 16]), i32([0]), i32([0]), 16, d)
+        _, scales = K.kv8_codes(cache, d)
+        rows = x[0].reshape(len(pos), -1, d)
+        for p, i in {p: i for i, p in enumerate(pos)}.items():
+            for what, got in ((0, k), (1, v)):
+                assert ((got[p].float() - rows[i, nq + what * nkv:nq + (what + 1) * nkv]).abs() <= scales[0, :, what, 0][:, None] * 2.01).all()      # up to four passes over the block
