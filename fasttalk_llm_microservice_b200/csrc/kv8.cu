@@ -181,13 +181,22 @@ kv8_append_kernel(const Kv8Append p, int kv_rows, int kv_ctas) {
                         *at = y;
                     }
                 }
-                const float inv = s > 0.f ? 1.f / s : 0.f;
-                auto code = [&](float v) { return (uint32_t)(max(-127, min(127, __float2int_rn(v * inv))) + 128); };
+                // rint(v / s) + 128 in the low byte: the product with the reciprocal, rounded to a whole number c by adding 1.5 * 2^23 (+ 128), is the quotient's own
+                // unless that lies next to a border; then the remainder v - c s, which fp32 holds there, says on which side: |v - c s| > s / 2, or half
+                // of it and c odd (numbers that are not negative order as their bits do).  A block of zeros may hold numbers below 2^-100: codes of 0.  A division for each
+                // number was 1 us slower at 1954 tokens.
+                const float inv = s > 0.f ? 1.f / s : 0.f, half = s > 0.f ? 0.5f * s : INFINITY;
+                auto code = [&](float v) {
+                    constexpr float shift = 12583040.f;
+                    const float t = fmaf(v, inv, shift), rest = fmaf(shift - t, s, v);
+                    return __float_as_uint(__float_as_uint(fabsf(rest)) + (__float_as_uint(t) & 1) > __float_as_uint(half) ? t + copysignf(1.f, rest) : t);
+                };
+                auto codes = [&](float4 v) { return byte_perm(byte_perm(code(v.x), code(v.y), 0x0040), byte_perm(code(v.z), code(v.w), 0x0040), 0x5410); };
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const int r = i * RP + rsub;
                     const int ps = __shfl_sync(0xffffffffu, run_pos, base + r);
-                    if (r < n && ps < p.n_angles) *code_at(ps & 15) = code(x[i].x) | code(x[i].y) << 8 | code(x[i].z) << 16 | code(x[i].w) << 24;
+                    if (r < n && ps < p.n_angles) *code_at(ps & 15) = codes(x[i]);
                 }
                 __syncwarp();
                 if (lane == 0) *scale = s;

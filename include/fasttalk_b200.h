@@ -672,7 +672,7 @@ int ft_attn_prefill(const void* q, const void* kv_layer, const int* page_table, 
  *
  * ft_rope_kv8_append: ft_rope_kv_append into this cache (n_angles = rows of cos_t / sin_t; a token that has none is not written and its q is 0; one that only the page table lacks is rotated all the same).  Per block and head, with a = max |x| over the block's new
  * tokens (NaN counts as 0, what lies beyond fp16's range as its end) and s_old the block's scale where it holds tokens below the first new one, else 0:
- * s = max(s_old, a / 127); tokens below the first new one c <- rint(c s_old / s); new ones c = rint(x / s).  Tokens of a sequence stand side by side in the lists
+ * s = max(s_old, a / 127); tokens below the first new one c <- rint(c f), f = s_old / s in fp32; new ones c = rint(x / s), ties to even.  Tokens of a sequence stand side by side in the lists
  * and without gaps; a block that two separate stretches of the list share is written by both at once. */
 long long ft_kv8_record_bytes(int d);
 int ft_rope_kv8_append(const float* qkv, int n_splits, long long split_stride, const float* cos_t, const float* sin_t, int n_angles,

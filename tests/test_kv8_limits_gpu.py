@@ -314,3 +314,29 @@ def test_the_later_of_two_tokens_for_one_row_stands(K, d, pos):
         for p, i in {p: i for i, p in enumerate(pos)}.items():
             for what, got in ((0, k), (1, v)):
                 assert ((got[p].float() - rows[i, nq + what * nkv:nq + (what + 1) * nkv]).abs() <= scales[0, :, what, 0][:, None] * 2.01).all()      # up to four passes over the block
+
+
+@pytest.mark.parametrize("d,T", [(64, 40), (128, 40), (64, 600)])
+def test_codes_are_the_quotients(K, d, T):
+    """c = rint(x / s), not x times a reciprocal: with numbers that reach the rounding as they are, code by code."""
+    nq, nkv = 1, 2
+    cache = K.kv8_cache_alloc(-(-T // 64), nkv, d, DEV)
+    x = torch.randn(1, T, (nq + 2 * nkv) * d, generator=gen(T), device=DEV)
+    ones, zeros = torch.ones(T, d // 2, device=DEV), torch.zeros(T, d // 2, device=DEV)
+    table = torch.arange(-(-T // 64), device=DEV, dtype=torch.int32)[None]
+    # numbers next to a border between two codes
+    rows = x[0].reshape(T, -1, d)
+    for b in range(0, T, 16):
+        most = rows[b:b + 16, nq:].abs().amax((0, 2))                                  # [2 nkv]
+        step = most / 127
+        rows[b:b + 16, nq:, 8:40] = ((torch.randint(-126, 126, (rows[b:b + 16].shape[0], 2 * nkv, 32), generator=gen(b), device=DEV) + 0.5) * step[None, :, None])
+        rows[b, nq:, 0] = most
+    K.rope_kv8_append(x, ones, zeros, torch.arange(T, device=DEV, dtype=torch.int32), i32([0] * T), table, cache, nq, nkv, d)
+    codes, scales = K.kv8_codes(cache, d)
+    kv = rows[:, nq:].reshape(T, 2, nkv, d).cpu()
+    for t in range(T):
+        for what in (0, 1):
+            most = kv[t // 16 * 16:t // 16 * 16 + 16, what].abs().amax((0, 2))
+            s = scales[t // 64, :, what, t % 64 // 16].cpu()
+            assert torch.equal(s, most / 127)
+            assert torch.equal(codes[t // 64, :, what, t % 64].cpu().to(F64) - 128, torch.round(kv[t, what].to(F64) / s[:, None].to(F64)))
