@@ -310,7 +310,7 @@ extern "C" int ft_rope_kv8_append(const float* qkv, int n_splits, long long spli
                max_pages, num_pages);
     FT_REQUIRE(max_pages <= INT32_MAX / kKvTile - 1, "ft_rope_kv8_append: %d pages a sequence", max_pages);
     if (T == 0) return 0;
-    FT_REQUIRE(qkv && cos_t && sin_t && positions && seq_rows && page_table && q_out && kv8_layer, "ft_rope_kv8_append: null argument");
+    FT_REQUIRE(qkv && cos_t && sin_t && positions && seq_rows && q_out && kv8_there(page_table, table_rows, max_pages, kv8_layer, num_pages), "ft_rope_kv8_append: null argument");
     FT_REQUIRE(n_angles >= 1, "ft_rope_kv8_append: no angles");
     FT_REQUIRE(((uintptr_t)qkv | (uintptr_t)cos_t | (uintptr_t)sin_t | (uintptr_t)q_out | (uintptr_t)kv8_layer) % 16 == 0 && split_stride % 4 == 0,
                "ft_rope_kv8_append: tensors on 16 bytes");
@@ -335,7 +335,7 @@ extern "C" int ft_kv8_read(const void* kv8_layer, int num_pages, const int* page
     FT_REQUIRE(rows >= 0 && n_req >= 0 && nkv >= 1 && table_rows >= 0 && max_pages >= 0 && num_pages >= 0,
                "ft_kv8_read: bad sizes rows=%d n_req=%d nkv=%d table %d x %d, %d pages", rows, n_req, nkv, table_rows, max_pages, num_pages);
     if (rows == 0) return 0;
-    FT_REQUIRE(k_out && v_out && kv8_layer && (n_req == 0 || (req_start && req_slot && req_pos0 && page_table)), "ft_kv8_read: null argument");
+    FT_REQUIRE(k_out && v_out && (n_req == 0 || (req_start && req_slot && req_pos0 && kv8_there(page_table, table_rows, max_pages, kv8_layer, num_pages))), "ft_kv8_read: null argument");
     FT_REQUIRE(((uintptr_t)kv8_layer | (uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0, "ft_kv8_read: tensors on 16 bytes");
     const long long tasks = (long long)nkv * 2 * K8_READ_ROWS * (d / 16), per = K8_READ_TASKS * K8_READ_THREADS;
     FT_REQUIRE((tasks + per - 1) / per <= 65535, "ft_kv8_read: %d heads", nkv);

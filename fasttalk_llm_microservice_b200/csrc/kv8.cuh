@@ -27,6 +27,11 @@ struct Kv8 {
     static constexpr int REC = 2 * SLAB + 32;
 };
 
+// A page table without rows or pages, and a cache without pages, may be null: nothing is read there
+inline bool kv8_there(const void* page_table, int table_rows, int max_pages, const void* layer, int num_pages) {
+    return (page_table || table_rows == 0 || max_pages == 0) && (layer || num_pages == 0);
+}
+
 // Byte of a record at which 16-byte chunk c of token t begins
 __device__ __forceinline__ int kv8_key_chunk(int t, int c) { return (c >> 2) * (kKvTile * 64) + t * 64 + (c & 3) * 16; }
 template <int D>

@@ -372,7 +372,7 @@ extern "C" int ft_attn_decode_kv8(const void* q, const void* kv8_layer, int num_
     FT_REQUIRE(B >= 0 && max_pages >= 0 && num_pages >= 0 && max_pages <= INT32_MAX / kKvTile && ((double)B + 1) * nkv * (max_pages + 1) + 4096 <= INT32_MAX,
                "ft_attn_decode_kv8: bad sizes B=%d nkv=%d max_pages=%d num_pages=%d", B, nkv, max_pages, num_pages);
     if (B == 0) return 0;
-    FT_REQUIRE(q && kv8_layer && page_table && ctx_lens && out, "ft_attn_decode_kv8: null argument");
+    FT_REQUIRE(q && ctx_lens && out && kv8_there(page_table, B, max_pages, kv8_layer, num_pages), "ft_attn_decode_kv8: null argument");
     FT_REQUIRE(((uintptr_t)q | (uintptr_t)kv8_layer | (uintptr_t)out | (uintptr_t)out_lo | (uintptr_t)scratch) % 16 == 0, "ft_attn_decode_kv8: tensors on 16 bytes");
     return d == 64 ? launch_kv8_decode<64>(q, kv8_layer, num_pages, page_table, max_pages, ctx_lens, out, out_lo, scratch, B, nq, nkv, (cudaStream_t)stream)
                    : launch_kv8_decode<128>(q, kv8_layer, num_pages, page_table, max_pages, ctx_lens, out, out_lo, scratch, B, nq, nkv, (cudaStream_t)stream);

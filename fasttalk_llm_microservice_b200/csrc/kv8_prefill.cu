@@ -766,7 +766,7 @@ extern "C" int ft_attn_prefill_kv8(const void* q, const void* kv8_layer, int num
     FT_REQUIRE(((double)T / (2 * (K8P_ROWS / (nq / nkv))) + n_req) * ((double)max_pages + T / kKvTile + 2 + kKv8Start) * nkv + 4096 <= INT32_MAX,
                "ft_attn_prefill_kv8: %d tokens of %d requests over %d pages are more than one call takes", T, n_req, max_pages);
     if (T == 0) return 0;
-    FT_REQUIRE(q && kv8_layer && out && (n_req == 0 || (page_table && req_q_start && req_slot && req_pos0)), "ft_attn_prefill_kv8: null argument");
+    FT_REQUIRE(q && out && (n_req == 0 || (req_q_start && req_slot && req_pos0 && kv8_there(page_table, table_rows, max_pages, kv8_layer, num_pages))), "ft_attn_prefill_kv8: null argument");
     FT_REQUIRE(((uintptr_t)q | (uintptr_t)kv8_layer | (uintptr_t)out | (uintptr_t)out_lo | (uintptr_t)scratch) % 16 == 0, "ft_attn_prefill_kv8: tensors on 16 bytes");
     const int G = nq / nkv;
     Kv8Prompt p{(const __half*)q, (const uint8_t*)kv8_layer, page_table, req_q_start, req_slot, req_pos0, (__nv_bfloat16*)out, (__nv_bfloat16*)out_lo, nullptr, nullptr,

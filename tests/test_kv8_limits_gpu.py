@@ -340,3 +340,26 @@ def test_codes_are_the_quotients(K, d, T):
             s = scales[t // 64, :, what, t % 64 // 16].cpu()
             assert torch.equal(s, most / 127)
             assert torch.equal(codes[t // 64, :, what, t % 64].cpu().to(F64) - 128, torch.round(kv[t, what].to(F64) / s[:, None].to(F64)))
+
+
+# ------------------------------------------------------------------------------------------------ what is empty
+def test_empty_tables_and_caches(K):
+    """Page tables without pages or without rows, caches without pages: nothing is written, and zeros come back."""
+    nq, nkv, d = 4, 1, 64
+    q = torch.randn(2, nq, d, device=DEV).half()
+    cache, none = K.kv8_cache_alloc(2, nkv, d, DEV), K.kv8_cache_alloc(0, nkv, d, DEV)
+    wide, narrow, nothing = i32([[0, 1], [1, 0]]), torch.empty(2, 0, device=DEV, dtype=torch.int32), torch.empty(0, 2, device=DEV, dtype=torch.int32)
+    tab = torch.ones(8, d // 2, device=DEV)
+    x = torch.randn(1, 2, (nq + 2 * nkv) * d, device=DEV)
+    for layer, table in ((cache, narrow), (none, wide), (none, narrow), (cache, nothing), (none, nothing)):
+        for planes in (1, 2):
+            for out in K.attn_prefill_kv8(q, layer, table, [0, 1, 2], [0, 1], [3, 100], planes=planes):
+                assert out is None or (out == 0).all()
+            if table.shape[0] == 2:
+                for out in K.attn_decode_kv8(q, layer, table, i32([3, 70]), planes=planes):
+                    assert out is None or (out == 0).all()
+        k, v = K.kv8_read(layer, table, [0, 1, 2], [0, 1], [3, 100], 2, d)
+        assert (k == 0).all() and (v == 0).all()
+        turned = K.rope_kv8_append(x, tab, tab * 0, i32([3, 5]), i32([0, 1]), table, layer, nq, nkv, d)
+        assert torch.equal(turned, x[0].reshape(2, -1, d)[:, :nq].half())
+    assert (cache == 0).all()
