@@ -111,7 +111,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
     __shared__ Kv8Stretch told[4];
     __shared__ __align__(16) float kscale_s[C::S16][4];                      // times scale_log2; the first below 0: the page is not there
     __shared__ __align__(16) float vscale_s[C::S16][4], vlog_s[C::S16][4];   // of the values; 0 for blocks behind the unit's last token.  And their log2
-    __shared__ int blocks_s[C::S8];                                          // of 16 tokens, that some query of the unit sees; 0: the page is not there
+    __shared__ int blocks_s[C::S8];                                          // of 16 tokens, that some query of the unit sees; 0: none, or the page is not there
     __shared__ float2 ml_s[K8P_SOFT];
     __shared__ float size_s[K8P_SOFT];                                       // what a row's O is multiplied by to be in its own size
     __shared__ uint32_t tmem_slot;
@@ -225,7 +225,7 @@ kv8_prefill_kernel(const __grid_constant__ Kv8Prompt p) {
                         if (!go) continue;
                         asked = it + 1;
                         const bool there = page >= 0 && page < p.num_pages;
-                        blocks_s[s] = there ? min(4, (w.pos0 + w.tokens - 1 - (p0 + k) * kKvTile) / kKv8Block + 1) : 0;
+                        blocks_s[s] = there ? max(0, min(4, ((w.pos0 + w.tokens - 1 - (p0 + k) * kKvTile) >> 4) + 1)) : 0;
                         if (there) {
                             mbar_expect_tx(&rec_full[s], Kv8<D>::REC);
                             tma_bulk_g2s(smem + C::REC + s * Kv8<D>::REC, p.cache + ((size_t)page * p.nkv + w.head) * Kv8<D>::REC, Kv8<D>::REC, &rec_full[s], pol);

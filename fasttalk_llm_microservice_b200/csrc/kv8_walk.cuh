@@ -44,13 +44,15 @@ __host__ __device__ inline int floor_sum64(unsigned n, unsigned a, unsigned b) {
 // What a unit costs beyond its pages, in pages: it takes that much more of the flat list, behind its last step
 constexpr int kKv8Start = 3;
 
-// one request: its rows of q, tiles of 2 th tokens, steps of its tiles
+// one request: its rows of q, tiles of 2 th tokens, steps of its tiles.  at = the position of row0, which may lie ahead of the sequence: the list is made as if it were 0 then
 struct Kv8Request {
-    int row0, len, pos0, slot, tiles;
+    int row0, len, at, pos0, slot, tiles;
     __host__ __device__ __forceinline__ void load(const Kv8Prompt& p, int r) {
         row0 = max(0, min(p.req_q_start[r], p.T));
         len = max(0, min(p.req_q_start[r + 1], p.T) - row0);
-        pos0 = max(0, min(p.req_pos0[r], p.max_pages * kKvTile));
+        const long long first = (long long)p.req_pos0[r] + ((long long)row0 - p.req_q_start[r]), low = -p.T, high = p.max_pages * kKvTile;
+        at = (int)(first < low ? low : first > high ? high : first);
+        pos0 = max(0, at);
         slot = p.req_slot[r];
         tiles = (len + 2 * p.th - 1) / (2 * p.th);
     }
@@ -168,7 +170,7 @@ struct Kv8Walk {
     __host__ __device__ __forceinline__ int page0(int p_few) const { return few ? p_few * t0 : t0; }
     __host__ __device__ __forceinline__ int page1(int p_few) const { return few ? min(p_few * t1, n_pages) : t1; }
     __host__ __device__ __forceinline__ int row0(const Kv8Prompt& p) const { return q.row0 + i * 2 * p.th; }
-    __host__ __device__ __forceinline__ int position0(const Kv8Prompt& p) const { return q.pos0 + i * 2 * p.th; }
+    __host__ __device__ __forceinline__ int position0(const Kv8Prompt& p) const { return q.at + i * 2 * p.th; }
 };
 
 }  // namespace ft

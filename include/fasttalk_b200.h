@@ -694,7 +694,7 @@ int ft_attn_decode_kv8(const void* q, const void* kv8_layer, int num_pages, cons
 int ft_kv8_waits(void);
 void ft_kv8_set_wait_limit(int tries);
 /* Causal attention of prompt portions: q FP16 [T][nq][d], nq / nkv up to 8, request r owns rows req_q_start[r] .. req_q_start[r + 1] - 1 (req_q_start grows), page-table row req_slot[r],
- * and its first query sits at position req_pos0[r].  The lists are DEVICE arrays.  All T rows of out (and out_lo, may be NULL) are written; those that no request owns with zeros
+ * and its first query sits at position req_pos0[r]; rows outside q are left out, rows ahead of position 0 see nothing.  The lists are DEVICE arrays.  All T rows of out (and out_lo, may be NULL) are written; those that no request owns with zeros
  * (where req_q_start does not grow, none of them means anything).
  * scratch: work memory of ft_attn_prefill_kv8_scratch_bytes(d) bytes (of the current device), in any state, not shared by calls that may overlap. */
 long long ft_attn_prefill_kv8_scratch_bytes(int d);

@@ -13,7 +13,7 @@ import pytest
 import torch
 
 from test_kernels_gpu import Guarded
-from test_kv8_gpu import DEV, F64, check_prompt, gen, i32, prompt_case, rotated, tables, values
+from test_kv8_gpu import DEV, F64, check_prompt, gen, i32, prompt_case, random_cache, rotated, tables, values
 
 pytestmark = pytest.mark.gpu
 
@@ -363,3 +363,23 @@ def test_empty_tables_and_caches(K):
         turned = K.rope_kv8_append(x, tab, tab * 0, i32([3, 5]), i32([0, 1]), table, layer, nq, nkv, d)
         assert torch.equal(turned, x[0].reshape(2, -1, d)[:, :nq].half())
     assert (cache == 0).all()
+
+
+@pytest.mark.parametrize("nq,nkv,d", [(8, 2, 64), (3, 1, 128)])
+def test_portions_that_begin_ahead_of_q_or_of_the_sequence(K, nq, nkv, d):
+    """A request's first rows may lie ahead of q's first, its first positions ahead of the sequence's: the others keep theirs, and rows ahead of position 0 see nothing."""
+    lengths = [400, 300, 64]
+    g = gen(d)
+    cache = random_cache(K, 16, nkv, d, g)
+    table = tables(lengths, 16, g)
+    for starts, pos0 in (([-100, 150, 151, 200], [20, -3, 10]), ([0, 90, 150, 160], [-70, -7, -200]), ([-5, 3, 70, 71], [-10, -64, 63]), ([-(1 << 31), 40, 41, 50], [5, 5, -(1 << 31)])):
+        T = starts[-1]
+        q = (1.5 * torch.randn(T, nq, d, generator=g, device=DEV)).half()
+        want, tol = torch.zeros(T, nq, d, device=DEV, dtype=F64), torch.zeros(T, nq, d, device=DEV, dtype=F64)
+        for i in range(3):
+            for t in range(max(0, starts[i]), starts[i + 1]):
+                at = pos0[i] + t - starts[i]
+                if at >= 0:
+                    o, e = tight(K, q[t:t + 1], cache, table[i], at)
+                    want[t], tol[t] = o[0], e[0]
+        near(K.attn_prefill_kv8(q, cache, table, i32(starts), i32([0, 1, 2]), i32(pos0)), want, tol)

@@ -134,3 +134,19 @@ def test_sums_of_floors(lib):
         want = int(((a * i + b) // 64).sum())
         assert want < 2 ** 31
         assert lib.kv8_floor_sum64(n, a, b) == want
+
+
+def test_positions_of_portions_that_begin_ahead(lib):
+    """Rows ahead of q's first, positions ahead of the sequence's first: a tile's rows keep the positions that the lists give them (only what lies behind the table is drawn in)."""
+    rng = random.Random(8)
+    for i in range(200):
+        R = rng.randint(1, 8)
+        starts = [-rng.choice([0, 5, 100, 1000, 1 << 31])]
+        for _ in range(R):
+            starts.append(max(starts[-1], -1000) + rng.choice([0, 1, 50, 300, 900]))
+        starts[-1] = max(starts[-1], 1)
+        pos0 = [rng.choice([0, -3, -64, -700, -(1 << 31), rng.randint(0, 3000)]) for _ in range(R)]
+        rows = check(lib, starts, pos0, G=rng.randint(1, 8), nkv=rng.randint(1, 3))
+        for cta, row0, tokens, head, page0, pages, few, at, *_, slot in rows.tolist():
+            first = max(starts[slot], 0)                               # the request's first row of q
+            assert at == max(-starts[-1], min(pos0[slot] + first - starts[slot], 6400)) + row0 - first
