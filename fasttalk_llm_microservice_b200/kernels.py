@@ -286,6 +286,13 @@ def _kv8_call(index: int, name: str, *args) -> None:
 _kv8_sizes = {}
 
 
+def _kv8_sms(index: int) -> int:
+    n = _kv8_sizes.get(index)
+    if n is None:
+        n = _kv8_sizes[index] = torch.cuda.get_device_properties(index).multi_processor_count
+    return n
+
+
 def _kv8_scratch(index: int, name: str, d: int) -> torch.Tensor:
     n = _kv8_sizes.get((index, name, d))
     if n is None:
@@ -367,7 +374,7 @@ def attn_decode_kv8(q: torch.Tensor, kv8_layer: torch.Tensor, page_table: torch.
     if rows < B:
         _refuse(what, "a page-table row for every query")
     # the library needs none for a few sequences whose page tables are short
-    scratch = _kv8_scratch(index, "ft_attn_decode_kv8_scratch_bytes", d) if most > 16 or B * nkv > 256 else None
+    scratch = _kv8_scratch(index, "ft_attn_decode_kv8_scratch_bytes", d) if most > 16 or B * nkv > 2 * _kv8_sms(index) else None
     _kv8_call(index, "ft_attn_decode_kv8", q.data_ptr(), kv8_layer.data_ptr(), pages, page_table.data_ptr(), most, ctx_lens.data_ptr(), out.data_ptr(),
               0 if lo is None else lo.data_ptr(), 0 if scratch is None else scratch.data_ptr(), B, nq, nkv, d)
     return out, lo

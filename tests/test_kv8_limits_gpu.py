@@ -383,3 +383,17 @@ def test_portions_that_begin_ahead_of_q_or_of_the_sequence(K, nq, nkv, d):
                     o, e = tight(K, q[t:t + 1], cache, table[i], at)
                     want[t], tol[t] = o[0], e[0]
         near(K.attn_prefill_kv8(q, cache, table, i32(starts), i32([0, 1, 2]), i32(pos0)), want, tol)
+
+
+def test_work_memory_goes_by_the_devices_sms(K, monkeypatch):
+    """The library does without for up to two (sequence, head) an SM: the call leaves it out by the same count, on a device of any size."""
+    import types
+    asked = []
+    monkeypatch.setattr(K, "_kv8_call", lambda index, name, *args: asked.append(args[8]))
+    q, cache = torch.zeros(74, 8, 64, device=DEV, dtype=torch.float16), K.kv8_cache_alloc(1, 4, 64, DEV)
+    table = torch.zeros(74, 16, device=DEV, dtype=torch.int32)
+    for sms, rows in ((148, 74), (148, 73), (100, 50), (100, 51), (64, 74)):
+        monkeypatch.setattr(K, "_kv8_sizes", {})
+        monkeypatch.setattr(torch.cuda, "get_device_properties", lambda *_: types.SimpleNamespace(multi_processor_count=sms))
+        K.attn_decode_kv8(q[:rows], cache, table, torch.zeros(rows, device=DEV, dtype=torch.int32))
+        assert (asked.pop() == 0) == (rows * 4 <= 2 * sms), (sms, rows)
