@@ -41,9 +41,10 @@ constexpr int K8P_ROWS = 128;                    // rows of a half
 constexpr int K8P_GROUP = 8;                     // query heads a key head at most
 constexpr int K8P_PIECE = kKvTile * 128;         // [64 tokens][64 dims] in fp16; 64 rows of a Q block
 constexpr float K8P_LOG2E = 1.4426950408889634f;
-constexpr int K8P_WHOLE = 10;
-// (pages that a share may be shorter than a whole unit for parts not to pay: 5 / 10 / 15 for four portions of 100 tokens behind 300, heads of 128, 24.8 / 19.6 / 19.6 us; six of
-// 100 behind 1000 36.5 / 34.4 / 34.4, heads of 64 27.5 / 30.2 / 30.5; three of 150 behind 900 24.3 / 24.2 / 29.9; two of 300, heads of 128, 17 us whole and 22 in parts)
+constexpr int K8P_WHOLE = 7;
+// (pages that a share may be shorter than a whole unit for parts not to pay, us with 5 / 7 / 10.  Heads of 128: four portions of 100 tokens behind 300 22.0 / 20.4 / 20.4, three of
+// 150 behind 900 34.1 / 33.8 / 36.9, six of 100 behind 1000 38.8 / 37.0 / 37.0.  Heads of 64: four of 100 behind 300 18.1 / 17.0 / 17.1, 700 and 619 behind 333 with a key head
+// each 28.0 / 28.1 / 31.8, six of 100 behind 1000 31.8 / 32.5 / 32.5)
 
 template <int D>
 struct K8Prefill {

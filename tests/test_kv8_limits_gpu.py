@@ -264,7 +264,8 @@ def test_decode_counts_every_key_once(K, nq, nkv, d, lengths):
 
 
 @pytest.mark.parametrize("nq,nkv,d", [(32, 8, 64), (32, 8, 128), (3, 1, 128), (16, 16, 128), (16, 2, 64), (5, 1, 64)])
-@pytest.mark.parametrize("reqs", [[(0, 700)], [(16001, 5)], [(2990, 33), (0, 300), (100, 64), (1500, 1)], [(30 * i, 1 + 7 * i) for i in range(20)], [(300, 100)] * 4, [(900, 60)] * 19, [(63, 2)]])
+@pytest.mark.parametrize("reqs", [[(0, 700)], [(16001, 5)], [(2990, 33), (0, 300), (100, 64), (1500, 1)], [(30 * i, 1 + 7 * i) for i in range(20)], [(300, 100)] * 4, [(900, 60)] * 19, [(63, 2)],
+                                  [(64 * 6 - 5, 5)] * 4, [(64 * 7 - 5, 5)] * 4, [(64 * 7, 7)] * 4, [(64 * 11, 40)] * 2, [(333, 700), (333, 619)]])
 def test_prefill_counts_every_key_once(K, nq, nkv, d, reqs):
     lengths = [p + n for p, n in reqs]
     cache, table, want = means(K, nq, nkv, d, lengths, seed=len(reqs))
