@@ -13,7 +13,7 @@ import pytest
 import torch
 
 from test_kernels_gpu import Guarded
-from test_kv8_gpu import DEV, F64, check_prompt, gen, i32, prompt_case, random_cache, rotated, tables, values
+from test_kv8_gpu import DEV, F64, append_inputs, check_prompt, decode_case, gen, i32, prompt_case, random_cache, rotated, tables, values
 
 pytestmark = pytest.mark.gpu
 
@@ -64,11 +64,51 @@ def guarded_prefill(K, case, planes=2):
     return out.t.reshape(T, nq * d), lo.t.reshape(T, nq * d)
 
 
+# ------------------------------------------------------------------------------------------------ memory around the outputs
+@pytest.mark.parametrize("nq,nkv,d", [(32, 8, 64), (24, 8, 128), (5, 1, 64), (16, 16, 128)])
+def test_nothing_is_written_outside(K, nq, nkv, d):
+    """Whole units and parts, one token and many, one plane and two; pages outside the cache, lists that reach beyond q, lengths beyond the table."""
+    for reqs in ([(0, 700)], [(5000, 5)], [(100, 300), (0, 2), (64, 64)], [(900, 60)] * 19, [(0, 1)], [(30 * i, 1 + 7 * i) for i in range(20)]):
+        q, cache, table, starts, slots, pos0 = prompt_case(K, reqs, nq, nkv, d, seed=2, before=1, after=3)
+        table[0, 0] = cache.shape[0]
+        guarded_prefill(K, (q, cache, table, starts, slots, pos0), planes=1)
+        guarded_prefill(K, (q, cache, table, [*starts[:-1], 1 << 30], slots, [*pos0[:-1], 1 << 30]), planes=2)
+        guarded_prefill(K, (q, cache, table, [-9, *starts[1:]], [1 << 30, *slots[1:]], [-(1 << 31), *pos0[1:]]), planes=2)
+    for lengths, width in (([700, 0, 64, 5000], None), ([77, 0, 64], 2), ([300] * 70, 5), ([20000], None)):
+        q, cache, table = decode_case(K, lengths, nq, nkv, d, seed=1, width=width)
+        table[0, 0] = -1
+        guarded_decode(K, (q, cache, table, lengths), planes=1)
+        guarded_decode(K, (q, cache, table, [1 << 30, *lengths[1:]]), planes=2)
+
+
+@pytest.mark.parametrize("nq,nkv,d", [(32, 8, 64), (24, 8, 128), (5, 1, 64)])
+@pytest.mark.parametrize("reqs", [[(0, 1)], [(70, 1), (0, 1), (15, 1)], [(7, 100), (0, 16), (130, 3)], [(13, 1021)]])
+def test_append_and_read_stay_inside(K, nq, nkv, d, reqs):
+    from fasttalk_llm_microservice_b200 import native
+    qkv, cos, sin, pos, seq, table, cache = append_inputs(K, reqs, nq, nkv, d, 2, seed=d)
+    lib, st = native.load(), torch.cuda.current_stream().cuda_stream
+    T, layer, q = qkv.shape[1], Guarded(cache.numel(), torch.uint8), Guarded(qkv.shape[1] * nq * d, torch.float16)
+    layer.t.copy_(cache.reshape(-1))
+    native.check(lib.ft_rope_kv8_append(qkv.data_ptr(), 2, qkv.stride(0), cos.data_ptr(), sin.data_ptr(), cos.shape[0], pos.data_ptr(), seq.data_ptr(), table.data_ptr(), *table.shape,
+                                        q.t.data_ptr(), layer.t.data_ptr(), cache.shape[0], T, nq, nkv, d, st), "append")
+    want = K.rope_kv8_append(qkv, cos, sin, pos, seq, table, cache, nq, nkv, d)
+    assert torch.equal(q.t.reshape(want.shape), want) and torch.equal(layer.t.reshape(cache.shape), cache)
+    lists = [i32(v) for v in ([3, *[4 + sum(n for _, n in reqs[:i + 1]) for i in range(len(reqs))]], list(range(len(reqs))), [p for p, _ in reqs])]
+    rows = T + 9
+    k, v = Guarded(rows * nkv * d, torch.float16), Guarded(rows * nkv * d, torch.float16)
+    native.check(lib.ft_kv8_read(layer.t.data_ptr(), cache.shape[0], table.data_ptr(), *table.shape, *(t.data_ptr() for t in lists), len(reqs), rows, k.t.data_ptr(), v.t.data_ptr(),
+                                 nkv, d, st), "read")
+    torch.cuda.synchronize()
+    for a, b in zip((k, v), K.kv8_read(cache, table, *lists, rows, d)):
+        assert torch.equal(a.t.reshape(b.shape), b)
+    assert all(g.intact() for g in (layer, q, k, v))
+
+
 # ------------------------------------------------------------------------------------------------ waits
 GIVE_UP = """
 import torch
 from fasttalk_llm_microservice_b200 import kernels as K, native
-from test_kv8_gpu import DEV, decode_case, i32, prompt_case
+from test_kv8_gpu import decode_case, prompt_case
 from test_kv8_limits_gpu import guarded_decode, guarded_prefill
 
 lib = native.load()
