@@ -438,3 +438,61 @@ def test_work_memory_goes_by_the_devices_sms(K, monkeypatch):
         monkeypatch.setattr(torch.cuda, "get_device_properties", lambda *_: types.SimpleNamespace(multi_processor_count=sms))
         K.attn_decode_kv8(q[:rows], cache, table, torch.zeros(rows, device=DEV, dtype=torch.int32))
         assert (asked.pop() == 0) == (rows * 4 <= 2 * sms), (sms, rows)
+
+
+# ------------------------------------------------------------------------------------------------ large and many
+@pytest.mark.parametrize("nq,nkv,d", [(32, 8, 64), (32, 8, 128)])
+def test_pages_beyond_four_gigabytes(K, nq, nkv, d):
+    """The last pages of a cache of 5 GB: written, read back, attended to."""
+    pages = 5 * 2 ** 30 // (nkv * (128 * d + 32))
+    cache = torch.empty(pages, nkv, 128 * d + 32, device=DEV, dtype=torch.uint8)
+    reqs = [(0, 200), (0, 70)]
+    table = torch.full((2, 4), -1, device=DEV, dtype=torch.int32)
+    table[0], table[1, :2] = i32([pages - 1, pages - 3, pages - 9, pages - 2]), i32([pages - 4, pages - 7])
+    qkv, cos, sin, pos, seq, _, _ = append_inputs(K, reqs, nq, nkv, d, 1, seed=d)
+    q = K.rope_kv8_append(qkv, cos, sin, pos, seq, table, cache, nq, nkv, d)
+    small = K.kv8_cache_alloc(16, nkv, d, DEV)
+    low = torch.where(table < 0, table, table - (pages - 16))
+    assert torch.equal(q, K.rope_kv8_append(qkv, cos, sin, pos, seq, low, small, nq, nkv, d))
+    lists = i32([0, 200, 270]), i32([0, 1]), i32([0, 0])
+    for a, b in zip(K.kv8_read(cache, table, *lists, 270, d), K.kv8_read(small, low, *lists, 270, d)):
+        assert torch.equal(a, b)
+    for a, b in zip(K.attn_prefill_kv8(q, cache, table, *lists), K.attn_prefill_kv8(q, small, low, *lists)):
+        assert torch.equal(a, b)
+    for a, b in zip(K.attn_decode_kv8(q[[199, 269]].contiguous(), cache, table, i32([200, 70])), K.attn_decode_kv8(q[[199, 269]].contiguous(), small, low, i32([200, 70]))):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("nq,nkv,d", [(4, 1, 64), (6, 2, 128)])
+def test_thousands_of_requests(K, nq, nkv, d):
+    """1500 portions of none to three tokens, several of one sequence among them; as many sequences of one token each; as many stretches read back."""
+    g = gen(d)
+    lengths = [(i * 37) % 150 + 4 for i in range(300)]
+    cache = random_cache(K, sum(-(-n // 64) for n in lengths), nkv, d, g)
+    table = tables(lengths, cache.shape[0], g)
+    slots = [(i * 7) % 300 for i in range(1500)]
+    news = [(i * 5) % 4 for i in range(1500)]
+    pos0 = [(i * 11) % (lengths[s] - 3) for i, s in enumerate(slots)]
+    starts = [0]
+    for n in news:
+        starts.append(starts[-1] + n)
+    rows = torch.tensor([i for i, n in enumerate(news) for _ in range(n)], device=DEV)
+    at = torch.tensor([pos0[i] + j for i, n in enumerate(news) for j in range(n)], device=DEV)
+    q = (1.5 * torch.randn(starts[-1], nq, d, generator=g, device=DEV)).half()
+    got = K.attn_prefill_kv8(q, cache, table, i32(starts), i32(slots), i32(pos0))
+    one = K.attn_decode_kv8(q, cache, table[i32(slots)[rows].long()].contiguous(), (at + 1).int())
+    back = K.kv8_read(cache, table, i32(starts), i32(slots), i32(pos0), starts[-1], d)
+    for s in range(300):
+        mine = (i32(slots)[rows] == s).nonzero()[:, 0]
+        x, _ = values(K, cache, table[s], lengths[s], d)
+        for t in mine.tolist():
+            p = int(at[t])
+            for what in (0, 1):
+                assert ((back[what][t].to(F64) - x[what, p]).abs() <= x[what, p].abs() * (2.0 ** -11 + 2.0 ** -24) + 2.0 ** -25).all()
+        if s % 10 == 0 and len(mine):
+            want = [tight(K, q[t:t + 1], cache, table[s], int(at[t])) for t in mine.tolist()]
+            for out in (got, one):
+                near([o[mine] for o in out], torch.cat([o for o, _ in want]).reshape(len(mine), -1), torch.cat([e for _, e in want]).reshape(len(mine), -1))
+    # every row, with and without the parts' kernel, by two kernels
+    off = (got[0].float() + got[1].float() - one[0].float() - one[1].float()).abs().max()
+    assert off <= 127 * 0.012 * 8 * 2.0 ** -9
