@@ -2,14 +2,14 @@
 //
 // Append.  x = the sum of the projection's split-K parts, keys rotated; per block of 16 tokens, head and keys | values, with a = max |x| over the block's new
 // rows and s_old the block's scale where it holds rows below the first new one (else 0):
-//   s = max(s_old, a / 127);   rows below the first new one: c <- rint(c * s_old / s);   new rows: c = rint(x / s)
+//   s = max(s_old, a / 127);   rows below the first new one: c <- rint(c * (s_old / s));   new rows: c = rint(x / s)
 // A token that fits under its block's scale is written as it is; one that does not rescales the at most 15 rows before it.  Each growth costs the older rows half
 // a step more of rounding; a block written at once is rounded once.  NaN becomes 0 and what lies beyond fp16's range is cut to it, as far as the fp16 cache reaches.
 //
 // A warp takes the runs that begin among one (or four, where there are many tokens) of the list, for one head's keys or values; a run = neighbouring tokens that go
 // to one block of one sequence.  Its rows stay in registers between the maximum and the rounding, so the projection is read once, all of it asked for before the
 // first number is used: what bounds a prompt's portion is that reading.  1954 tokens of four sequences behind 1003 each, in two
-// parts, 32 + 16 heads of 128 (116 MB): 24.6 us, 4.7 TB/s (with the rows read back 29, a row at a time 64); 64 single tokens, 32 + 16 heads of 64: 4.2 us, list, page and scale read one after the other.
+// parts, 32 + 16 heads of 128 (116 MB): 24.8 us, 4.7 TB/s (with the rows read back 29, a row at a time 64); 64 single tokens, 32 + 16 heads of 64: 4.2 us, list, page and scale read one after the other.
 #include <type_traits>
 
 #include "common.cuh"
@@ -21,7 +21,7 @@ namespace ft {
 constexpr int K8_WARPS = 8;
 constexpr int K8_QHEADS = 8;                 // query heads a warp takes
 constexpr int K8_MANY = 512;                 // tokens from which a warp looks at four of them: most of a prompt's begin no run, single ones all do.
-                                             // Four against one, us, their rows read back in 4 to 5 of them: 1800 in portions of 300 14.3 / 18.9, 700 in one 9.8 / 11.9, 400 in portions of 100 11.6 / 10.4, 64 single 15.1 / 7.9
+                                             // Four against one, us, heads of 64: 1800 in portions of 300 10.7 / 15.6, 700 in one 6.5 / 8.6, 400 in portions of 100 6.2 / 7.2, 512 single 13.7 / 14.8, 64 single 10.9 / 4.1
 
 struct Kv8Append {
     const float* qkv;
@@ -218,8 +218,8 @@ kv8_append_kernel(const Kv8Append p, int kv_rows, int kv_ctas) {
 // ------------------------------------------------------------------ reading back
 // Row i of k and v: (c - 128) * s of the request that owns it, in fp16 (cut to its range); rows that no request owns, and rows whose page lies outside the
 // cache, are zeros.  A CTA takes 16 rows of eight (sixteen) heads' keys or values: 16 bytes of codes a load, 32 bytes of fp16 a store, four loads on their way a
-// thread.  Bound by memory (one byte in, two out): 16 sequences of 2048 .. 1987 tokens, 8 heads of 64 (99 MB): 18.9 us, 5.3 TB/s; 5003 tokens of 8 heads of
-// 128 (31 MB): 8.6 us, 3.6 TB/s, too short for more.  With one load at a time 23.7 and 9.9 us.
+// thread.  Bound by memory (one byte in, two out): 16 sequences of 2048 .. 1987 tokens, 8 heads of 64 (99 MB): 16.8 us, 5.9 TB/s (the records partly out of L2, being the same each
+// time); 5003 tokens of 8 heads of 128 (31 MB): 8.6 us, 3.6 TB/s, too short for more.  With one load at a time 23.7 (then 18.9) and 9.9 us.
 constexpr int K8_READ_ROWS = 16, K8_READ_THREADS = 256, K8_READ_TASKS = 4;
 
 template <int D>

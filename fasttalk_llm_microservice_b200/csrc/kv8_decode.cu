@@ -8,8 +8,8 @@
 // Nothing is planned ahead of the kernel: every CTA adds up the sequences' pages itself (one read of ctx_lens).  What the arrival counters need, zeros, is
 // written by a kernel of its own ahead of this one.
 //
-// 64 sequences of about 2000 keys, 32 heads over 8 of 64 (133 MB): 33.0 us, 4.0 TB/s.  The first record lands about 4 us after the start (lengths, page number and record are
-// read one after the other), then the shares stream at about 5.7 TB/s, and the parts are put together in the last 5.  Three of 30011 .. 9377 keys, heads of 128: 30.0 us.  On the
+// 64 sequences of about 2000 keys, 32 heads over 8 of 64 (133 MB): 32.5 us, 4.1 TB/s.  Some 11 us of that are start (lengths, page number and record are read one after the other)
+// and end (the parts): from 4096 to 8192 keys each, 539 MB in 93 us, more bytes stream at 6.6 TB/s (7.0 at heads of 128).  Three of 30011 .. 9377 keys, heads of 128: 28.7 us.  On the
 // way, for the two: shares with the queries in the rows of the first product 36 / 38, the tokens in them 32 / 34, and then all warps putting parts together 32 / 30.
 #include <atomic>
 
@@ -21,7 +21,7 @@ namespace ft {
 
 constexpr int K8D_GROUP = 8;                     // query heads a key head at most
 constexpr int K8D_WHOLE_PAGES = 16;              // with page tables no wider than this, and a CTA for each (sequence, head), there are never parts
-                                                 // (32 sequences of 1000 keys, 8 heads of 128: 14.4 us whole, 18.8 in shares; 8 of 77, heads of 64, 4.3 / 5.0)
+                                                 // (32 sequences of 1000 keys, 8 heads of 128: 14.7 us whole, 20.0 in shares; 8 of 77, heads of 64, 4.5 / 7.7, counters' zeros included)
 constexpr float K8D_LOG2E = 1.4426950408889634f;
 
 __device__ int g_kv8_decode_waits;               // 1: a wait ran out on this device (ft_kv8_waits)

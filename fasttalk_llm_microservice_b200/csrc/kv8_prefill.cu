@@ -6,9 +6,10 @@
 // for the softmax, P to tensor memory, O += P V (A from tensor memory, M128 N=D K64).  A unit whose tokens fill one half only gives both halves the same queries and
 // every other page each.
 //
-// The tensor cores want fp16, so eight warps turn each record into the two operands, swizzled as the instructions read them: key codes as they are (the blocks' scales
-// go to the scores, one multiplication per 16 of them for the maximum and the multiply-add's factor for the exponents), value codes times their block's scale relative
-// to the largest of the stretch of pages at hand, which the same warps look up ahead (the output takes it back).  Both roundings are fp16's 2^-11 of a value.
+// The tensor cores want fp16, so eight warps turn each record into the two operands, swizzled as the instructions read them: codes as they are, which fp16 holds exactly.
+// The keys' scales go to the scores (one multiplication per 16 of them for the maximum, and the multiply-add's factor for the exponents), the values' to the probabilities.
+// Such a weight is rounded to fp16, 2^-11 of it, relative to the largest weight that its own row has met (kKv8Top in kv8.cuh): nothing that a row does not see, and no large
+// value without weight, takes bits from it.
 //
 // The flat list of all (request, key head, tile, page) is cut into equal shares, one for each SM: a causal list's units differ in length by any factor, and shares do
 // not.  A unit that lies in several shares is put together by a second kernel, in the parts' order.  Where there is an SM for every unit and none is much longer than
@@ -17,10 +18,13 @@
 // ahead of the kernel.
 //
 // What bounds it: each half's chain of a page, scores out of tensor memory - exponentials - probabilities into it - products - next scores, and the instructions of
-// eight softmax and eight converting warps around it: about 2200 clocks (1.15 us) a page of both halves at either head size, where the exponentials alone take 1024 (the SFU's
-// 16 a clock and SM).  Four prompts of 2048 .. 1578 tokens, 32 heads over 8 of 64: 152 us, 372 TFLOP/s; six portions of 211 .. 153 tokens behind about 5000, heads of 128:
-// 124 us, 674 TFLOP/s; five tokens behind 16001 on one rank's heads: 25 us, of which 6 pass until the first scores and 3 to 7 in the second kernel.
-// Measured on the way, us for the first two: shares of pages alone, without a unit's start and end, 175 / 176 (with them 153 / 126); the next page's scores read ahead of this
+// eight softmax and eight converting warps around it: 1.2 us (2350 clocks) a page of both halves at heads of 64 and 1.24 at 128, by the time that more pages add to a unit on each
+// SM, where the exponentials alone take 1024 clocks (the SFU's 16 a clock and SM).  A unit of one page on each SM takes 11 us from launch to launch, 15 at heads of 128, the second
+// kernel with nothing to do included.  Four prompts of 2048 .. 1578 tokens, 32 heads over 8 of 64: 160 us, 353 TFLOP/s; six portions of 211 .. 153 tokens behind about 5000, heads
+// of 128: 128 us, 655 TFLOP/s; five tokens behind 16001 on one rank's heads: 25 us.  The weights' multiplication is 5 % of the first: with the scales in the value operands,
+// relative to the largest of a stretch, they took 152 / 122, but what a row did not see took its bits.
+// Measured on the way, us for the first two: scales in the exponents' addends instead, and the sums of p by blocks, 163 / 130 (registers spill); shares of pages alone, without a
+// unit's start and end, 175 / 176 (with them 153 / 126); the next page's scores read ahead of this
 // page's exponentials 251 / 349 (with two buffers they are formed only behind the products that wait for this page's probabilities); copies and conversions that nap between
 // their tries 223 / 339; longer waits written out in every role, 173 / 138 against 153 / 127 (instruction fetch).
 #include "common.cuh"
@@ -41,10 +45,10 @@ constexpr int K8P_ROWS = 128;                    // rows of a half
 constexpr int K8P_GROUP = 8;                     // query heads a key head at most
 constexpr int K8P_PIECE = kKvTile * 128;         // [64 tokens][64 dims] in fp16; 64 rows of a Q block
 constexpr float K8P_LOG2E = 1.4426950408889634f;
-constexpr int K8P_WHOLE = 7;
-// (pages that a share may be shorter than a whole unit for parts not to pay, us with 5 / 7 / 10.  Heads of 128: four portions of 100 tokens behind 300 22.0 / 20.4 / 20.4, three of
+// Pages that a share may be shorter than a whole unit for parts not to pay.  us with 5 / 7 / 10, heads of 128: four portions of 100 tokens behind 300 22.0 / 20.4 / 20.4, three of
 // 150 behind 900 34.1 / 33.8 / 36.9, six of 100 behind 1000 38.8 / 37.0 / 37.0.  Heads of 64: four of 100 behind 300 18.1 / 17.0 / 17.1, 700 and 619 behind 333 with a key head
-// each 28.0 / 28.1 / 31.8, six of 100 behind 1000 31.8 / 32.5 / 32.5)
+// each 28.0 / 28.1 / 31.8, six of 100 behind 1000 31.8 / 32.5 / 32.5
+constexpr int K8P_WHOLE = 7;
 
 template <int D>
 struct K8Prefill {
