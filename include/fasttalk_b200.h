@@ -667,7 +667,8 @@ int ft_attn_prefill(const void* q, const void* kv_layer, const int* page_table, 
  * A code c (one byte) stands for (c - 128) * scale of its block.  Key of token t, dim i: piece i / 64, row t, byte i % 64; value: row t ^ (t >> 1 & 1), byte
  * (i % 64) ^ 8 (t & 4).  A cache of zero bytes is a cache of zeros.  head_dim 64 or 128; q, qkv, out and the cache on 16 bytes.
  * Page numbers outside [0, num_pages), page-table rows outside [0, table_rows) and positions beyond max_pages * 64 name no token: nothing is written there, zeros
- * are read, and attention does not see such keys; a table without rows or pages and a cache without pages may be NULL.  What lies behind a sequence's last token, in its blocks' scales too, may be anything.  A query that sees no key at all gives zeros.  The calls read and write what they are given only; all but
+ * are read, and attention does not see such keys; a table without rows or pages and a cache without pages may be NULL.  What lies behind a sequence's last token, in its blocks' scales too, may be anything.  A query that sees no key at all gives zeros.  Attention rounds each
+ * probability times its value's scale to fp16, relative to the largest such weight that the query has met; results below 2^-93 (1e-28) may come out as zeros.  The calls read and write what they are given only; all but
  * append may run at the same time on any streams, append beside nothing that touches the same pages.
  *
  * ft_rope_kv8_append: ft_rope_kv_append into this cache (n_angles = rows of cos_t / sin_t; a token that has none is not written and its q is 0; one that only the page table lacks is rotated all the same).  Per block and head, with a = max |x| over the block's new
