@@ -2,7 +2,7 @@
 supplies device memory and the stream; all arithmetic happens in the CUDA library."""
 from __future__ import annotations
 
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -421,6 +421,138 @@ def kv8_records(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     body = torch.empty(lead + (2 * KV_TILE * d,), device=codes.device, dtype=torch.uint8)
     body[..., _kv8_offsets(d, codes.device).reshape(-1)] = codes.reshape(body.shape)
     return torch.cat([body, scales.to(torch.float32).contiguous().reshape(lead + (-1,)).view(torch.uint8)], -1)
+
+
+# ---- a decode step of a batch whose sequences have their first tokens in common, over the fp16 cache
+class StepLists(NamedTuple):
+    """What step_lists makes, int32 on the device: request r owns tokens req_start[r] .. req_start[r + 1] - 1 of the step and has ctx_lens[r] tokens with them; each token's
+    position, row of the page table and place in the cache, -1 behind the last token; where the rest of the pool begins."""
+    req_start: torch.Tensor
+    ctx_lens: torch.Tensor
+    positions: torch.Tensor
+    seq_rows: torch.Tensor
+    kv_slots: torch.Tensor
+    taken: torch.Tensor
+
+
+def step_lists(cached_lens, new_lens, req_slot, page_table: torch.Tensor, free_pages: torch.Tensor, max_tokens: int, first_free: Optional[torch.Tensor] = None) -> StepLists:
+    """The lists of one step, built on the GPU: request r has cached_lens[r] tokens in the cache, new_lens[r] new ones and page-table row req_slot[r] (None: row r).  In their
+    order the requests take as many of their new tokens as there is room for in their row, in the pool free_pages[first_free:] and in the budget of max_tokens; the pages that
+    they take are written into page_table.  `first_free` is one int32 on the device (None: 0), `taken` of one step the next one's.  Of several requests with one row the first
+    has it.  The lists are int32 tensors on the device (then nothing goes up, and the call can be captured) or anything a tensor is made of."""
+    what = "step_lists"
+    index = page_table.get_device()
+    if index < 0:
+        _refuse(what, "page_table is contiguous int32 [sequences, pages] on the GPU")
+    rows, most = _kv8_table(page_table, index, what)
+    cached_lens = _kv8_ints(cached_lens, index, what, -1, "cached_lens")
+    R = cached_lens.numel()
+    new_lens = _kv8_ints(new_lens, index, what, R, "new_lens")
+    if req_slot is not None:
+        req_slot = _kv8_ints(req_slot, index, what, R, "req_slot")
+    free_pages = _kv8_ints(free_pages, index, what, -1, "free_pages")
+    if first_free is not None:
+        first_free = _kv8_ints(first_free, index, what, 1, "first_free")
+    if max_tokens < 0:
+        _refuse(what, "a number of tokens")
+    parts = torch.empty(2 * R + 2 + 3 * max_tokens, device=index, dtype=torch.int32).split([R + 1, R, max_tokens, max_tokens, max_tokens, 1])
+    out = StepLists(*parts)
+    at = out.req_start.data_ptr()
+    pos = at + 4 * (2 * R + 1)
+    _kv8_call(index, "ft_step_lists", cached_lens.data_ptr(), new_lens.data_ptr(), 0 if req_slot is None else req_slot.data_ptr(), R, page_table.data_ptr(), rows, most,
+              free_pages.data_ptr(), free_pages.numel(), 0 if first_free is None else first_free.data_ptr(), max_tokens, at, at + 4 * (R + 1), pos, pos + 4 * max_tokens,
+              pos + 8 * max_tokens, pos + 12 * max_tokens)
+    return out
+
+
+_QKV_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _kv16_layer(layer: torch.Tensor, d: int, what: str):
+    """(device, pages, kv heads) of a layer of the fp16 cache."""
+    index = layer.get_device()
+    if index < 0 or layer.dtype is not torch.float16 or layer.dim() != 5 or not layer.is_contiguous() or layer.shape[2:] != (2, KV_TILE, d):
+        _refuse(what, f"the cache is contiguous CUDA fp16 [pages, nkv, 2, {KV_TILE}, head_dim]")
+    return index, layer.shape[0], layer.shape[1]
+
+
+def norm_rope_kv_append(qkv: torch.Tensor, positions, kv_slots, kv_layer: torch.Tensor, nq: int, nkv: int, d: int, cos: Optional[torch.Tensor] = None,
+                        sin: Optional[torch.Tensor] = None, q_gain: Optional[torch.Tensor] = None, k_gain: Optional[torch.Tensor] = None, eps: float = 1e-5,
+                        neighbours: bool = False) -> torch.Tensor:
+    """Queries and keys divided by their head's root mean square, times a gain (fp32 [d], or a row for each head; None: 1), rotated by cos / sin (fp32 [positions, rotated / 2],
+    rotated a multiple of 16 up to d; None: not at all) in pairs (i, i + rotated / 2), or (2 i, 2 i + 1) with neighbours; q comes back as fp16 [T, nq, d], keys and values go to
+    kv_slots (step_lists' or page * 64 + token) of the fp16 cache.  qkv: fp32 [S, T, (nq + 2 nkv) d], S parts that are added up, or [T, ...] in fp32, bf16 or fp16, rows and
+    parts at any distance.  A token without a position (below 0, or beyond the tables) gives q = 0 and is not written; one whose slot is outside the cache is not written."""
+    what = "norm_rope_kv_append"
+    index, pages, heads = _kv16_layer(kv_layer, d, what)
+    if heads != nkv:
+        _refuse(what, "the cache has another number of heads")
+    kind = _QKV_TYPES.get(qkv.dtype)
+    dims = qkv.dim()
+    if kind is None or qkv.get_device() != index or dims not in (2, 3) or (dims == 3 and (kind != 0 or qkv.shape[0] < 1)) or qkv.shape[-1] != (nq + 2 * nkv) * d:
+        _refuse(what, "qkv is fp32 [S, T, (nq + 2 nkv) d], or [T, (nq + 2 nkv) d] in fp32, bf16 or fp16, on the cache's device")
+    T = qkv.shape[-2]
+    stride = qkv.stride()
+    if T and stride[-1] != 1:
+        _refuse(what, "a row of qkv lies in one piece")
+    positions, kv_slots = _kv8_ints(positions, index, what, T, "positions"), _kv8_ints(kv_slots, index, what, T, "kv_slots")
+    angles = rotated = 0
+    if cos is not None or sin is not None:
+        for t in (cos, sin):
+            if t is None or t.dtype is not torch.float32 or t.get_device() != index or t.dim() != 2 or t.shape != cos.shape or not t.is_contiguous():
+                _refuse(what, "cos and sin are contiguous fp32 [positions, rotated / 2] on the cache's device")
+        angles, rotated = cos.shape[0], 2 * cos.shape[1]
+    gains = []
+    for t, n in ((q_gain, nq), (k_gain, nkv)):
+        if t is not None and (t.dtype is not torch.float32 or t.get_device() != index or t.shape not in ((d,), (n, d)) or not t.is_contiguous()):
+            _refuse(what, "gains are contiguous fp32 [d] or [heads, d] on the cache's device")
+        gains += [0, 1] if t is None else [t.data_ptr(), 1 if t.dim() == 1 else n]
+    q = torch.empty(T, nq, d, device=index, dtype=torch.float16)
+    _kv8_call(index, "ft_norm_rope_kv_append", qkv.data_ptr(), kind, qkv.shape[0] if dims == 3 else 1, stride[0] if dims == 3 else 0, stride[-2],
+              0 if cos is None else cos.data_ptr(), 0 if sin is None else sin.data_ptr(), angles, rotated, int(neighbours), *gains, eps, positions.data_ptr(),
+              kv_slots.data_ptr(), q.data_ptr(), kv_layer.data_ptr(), pages, T, nq, nkv, d)
+    return q
+
+
+def attn_decode_shared(q: torch.Tensor, kv_layer: torch.Tensor, page_table: torch.Tensor, ctx_lens, group_start, shared_lens, req_slot=None, planes: int = 2):
+    """attn_decode for a batch that shares prefixes: q fp16 [B, nq, d], up to eight query heads a key head -> bf16 (hi, lo) planes [B, nq * d], lo None with planes = 1.  Query b
+    sees its first ctx_lens[b] tokens and has page-table row req_slot[b] (None: row b).  Group g = queries group_start[g] .. group_start[g + 1] - 1: their first shared_lens[g]
+    tokens are those of the group's first query's row, read once for all of them; what the other rows name below that is not read.  Queries outside all groups stand alone.  A
+    query without keys gives zeros; keys on pages outside the cache are hidden.  The lists are int32 tensors on the device (then nothing goes up, and the call can be captured)
+    or anything a tensor is made of."""
+    what = "attn_decode_shared"
+    if q.dim() != 3 or q.dtype is not torch.float16 or not q.is_contiguous():
+        _refuse(what, "q is contiguous fp16 [B, nq, d]")
+    B, nq, d = q.shape
+    index, pages, nkv = _kv16_layer(kv_layer, d, what)
+    if q.get_device() != index:
+        _refuse(what, "q is on another device than the cache")
+    if planes != 1 and planes != 2:
+        _refuse(what, "one plane or two")
+    rows, most = _kv8_table(page_table, index, what)
+    ctx_lens, shared_lens = _kv8_ints(ctx_lens, index, what, B, "ctx_lens"), _kv8_ints(shared_lens, index, what, -1, "shared_lens")
+    n = shared_lens.numel()
+    group_start = _kv8_ints(group_start, index, what, n + 1, "group_start")
+    if req_slot is not None:
+        req_slot = _kv8_ints(req_slot, index, what, B, "req_slot")
+    out = torch.empty(B, nq * d, device=index, dtype=torch.bfloat16)
+    lo = torch.empty_like(out) if planes == 2 else None
+    size = _kv8_sizes.get((index, B, n, nq, d))
+    if size is None:
+        with torch.cuda.device(index):
+            size = _kv8_sizes[index, B, n, nq, d] = N.check(N.load().ft_attn_decode_shared_scratch_bytes(B, n, nq, d), "ft_attn_decode_shared_scratch_bytes")
+    scratch = torch.empty(size, device=index, dtype=torch.uint8)
+    _kv8_call(index, "ft_attn_decode_shared", q.data_ptr(), kv_layer.data_ptr(), pages, page_table.data_ptr(), rows, most, 0 if req_slot is None else req_slot.data_ptr(),
+              ctx_lens.data_ptr(), group_start.data_ptr(), shared_lens.data_ptr(), n, out.data_ptr(), 0 if lo is None else lo.data_ptr(), scratch.data_ptr(), B, nq, nkv, d)
+    return out, lo
+
+
+def attn_shared_check(device=None) -> None:
+    """Waits for the device (the current one by default) and raises if a kernel of attn_decode_shared has ever given up on a wait there: rows of some call since the library was
+    loaded mean nothing.  No call asks by itself, since that would make the host wait."""
+    with torch.cuda.device(device):
+        if N.check(N.load().ft_attn_shared_waits(), "ft_attn_shared_waits"):
+            raise N.NativeError("attention over shared prefixes: a wait inside a kernel ran out; outputs of this process are not to be trusted")
 
 
 # ---- KV cache (un)swizzle helpers for tests: logical [tokens, d] <-> stored slab
