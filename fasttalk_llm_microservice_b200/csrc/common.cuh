@@ -79,6 +79,20 @@ __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
     return r;
 }
 
+// two fp32 sums in one instruction, and the largest of three
+__device__ __forceinline__ f32x2 sum2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float max3(uint32_t a, uint32_t b, uint32_t c) { return max3(__uint_as_float(a), __uint_as_float(b), __uint_as_float(c)); }
+__device__ __forceinline__ float max3(float a, uint32_t b, uint32_t c) { return max3(a, __uint_as_float(b), __uint_as_float(c)); }
+
 // a whole number that the compiler knows
 template <int I>
 struct Int { static constexpr int value = I; };
@@ -398,6 +412,14 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
         : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Registers that tcgen05.ld fills are there after the wait only, which the compiler cannot see from its operands: nothing that reads them moves ahead of this
+template <int N>
+__device__ __forceinline__ void tmem_arrived(uint32_t* r) {
+    tmem_ld_wait();
+#pragma unroll
+    for (int c = 0; c < N; c += 8)
+        asm volatile("" : "+r"(r[c]), "+r"(r[c + 1]), "+r"(r[c + 2]), "+r"(r[c + 3]), "+r"(r[c + 4]), "+r"(r[c + 5]), "+r"(r[c + 6]), "+r"(r[c + 7]));
+}
 // MN-major SWIZZLE_128B operand (V slab): 8-row groups (8 keys x 128 B) 1024 B apart along K; one 64-element MN block
 // (block_bytes: from one block of 64 MN elements to the next)
 __device__ __forceinline__ uint64_t umma_desc_mn128(uint32_t smem_addr, uint32_t block_bytes = kKvTile * 128) {

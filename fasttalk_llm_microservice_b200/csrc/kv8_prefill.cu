@@ -65,28 +65,6 @@ struct K8Prefill {
     static constexpr size_t PART = (size_t)2 * K8P_ROWS * (D + 2);   // floats of a part: O [D / 4][256 rows][4], then (m, l) [256]
 };
 
-// two fp32 sums in one instruction, and the largest of three
-__device__ __forceinline__ f32x2 sum2(f32x2 a, f32x2 b) {
-    f32x2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
-__device__ __forceinline__ float max3(uint32_t a, uint32_t b, uint32_t c) { return max3(__uint_as_float(a), __uint_as_float(b), __uint_as_float(c)); }
-__device__ __forceinline__ float max3(float a, uint32_t b, uint32_t c) { return max3(a, __uint_as_float(b), __uint_as_float(c)); }
-
-// Registers that tcgen05.ld fills are there after the wait only, which the compiler cannot see from its operands: nothing that reads them moves ahead of this
-template <int N>
-__device__ __forceinline__ void tmem_arrived(uint32_t* r) {
-    tmem_ld_wait();
-#pragma unroll
-    for (int c = 0; c < N; c += 8)
-        asm volatile("" : "+r"(r[c]), "+r"(r[c + 1]), "+r"(r[c + 2]), "+r"(r[c + 3]), "+r"(r[c + 4]), "+r"(r[c + 5]), "+r"(r[c + 6]), "+r"(r[c + 7]));
-}
 constexpr int kStretchWaits = 64;                // times the limit, for what takes a whole stretch: it may be a million keys
 // A warp's wait (all lanes ask, so that the warp stays together)
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* dead, int limit) {

@@ -53,4 +53,7 @@ __host__ __device__ __forceinline__ int shared_head_steps(int size, int th, int 
 // where row 0 of (group, key head, query i of the group) lies among the prefix's results
 __host__ __device__ __forceinline__ size_t shared_row(const SharedGroup& g, int h, int i, int nq, int G) { return (size_t)g.seq0 * nq + ((size_t)h * g.size + i) * G; }
 
+int launch_shared_prefix(const SharedArgs& p, int d, cudaStream_t st);
+int shared_prefix_waits(int* out);
+
 }  // namespace ft

@@ -53,7 +53,7 @@ shared_plan_kernel(const __grid_constant__ SharedArgs p) {
     for (int g = tid; g < p.n_groups; g += SP_THREADS) grows = grows && p.group_start[g] >= 0 && p.group_start[g] <= p.group_start[g + 1] && p.group_start[g + 1] <= p.B;
     grows = __syncthreads_and(grows);
     auto shared_of = [&](int g) { return max(0, min(p.shared_lens[g], reach)); };
-    auto pays = [&](int g) { return false; };
+    auto pays = [&](int g) { return p.group_start[g + 1] - p.group_start[g] >= 2 && shared_of(g) >= 2 * kKvTile; };
     {
         const int chunk = (p.n_groups + SP_THREADS - 1) / SP_THREADS, g0 = min(p.n_groups, tid * chunk), g1 = min(p.n_groups, g0 + chunk);
         int mine = 0, total;
@@ -413,28 +413,53 @@ shared_decode_kernel(const __grid_constant__ SharedArgs p) {
             if (!s_last) continue;
             __threadfence();
         }
-        if (!all) {
-            // each warp takes every WARPS-th part, in their order, and then they are records of the warps once more
+        if (!all || s.group >= 0) {
+            // each warp takes every WARPS-th part, in their order, and of the prefix's results, and then they are records of the warps once more
             float* mine = merge + (size_t)warp * C::PART;
+            int x0 = 0, x1 = -1;                                             // CTAs that have results of the prefix's unit
+            size_t row0 = 0;
+            if (s.group >= 0) {
+                const SharedGroup w = p.groups[s.group];
+                const int i = b - w.seq0, tile = i / (2 * p.th), n = min(2 * p.th, w.size - tile * 2 * p.th), per_x = p.head->prefix_per;
+                const int from = w.base + h * shared_head_steps(w.size, p.th, w.pages) + tile * (w.pages + kSharedStart);
+                x0 = (int)((unsigned)from / (unsigned)per_x);
+                x1 = (int)((unsigned)(from + shared_steps(n, p.th, w.pages) - 1) / (unsigned)per_x);
+                row0 = shared_row(w, h, i, p.nq, G);
+            }
+            __syncwarp();
 #pragma unroll 1
-            for (int e0 = 4 * lane; e0 < G * D; e0 += 128) {
+            for (int eb = 0; eb < G * D; eb += 128) {
+                const int e0 = min(eb + 4 * lane, G * D - 4), hg = e0 / D, dim = e0 % D;
+                float* rec = mine + hg * C::REC;
                 float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
                 float M = -INFINITY, L = 0.f;
-                const int hg = e0 / D, dim = e0 % D;
-#pragma unroll 2
-                for (int c = c0 + warp; c <= c1; c += C::WARPS) {
-                    const float* rec = p.own_parts + (2 * (size_t)c + (c == c0)) * C::PART;
-                    const float4 o = __ldcg(reinterpret_cast<const float4*>(rec + e0));
-                    const float2 ml = __ldcg(reinterpret_cast<const float2*>(rec + kSharedGroup * D + 2 * hg));
+                auto add = [&](const float4& o, const float2& ml) {
                     const float Mn = fmaxf(M, ml.x);
                     const float keep = M == -INFINITY ? 0.f : exp2f(M - Mn), z = ml.x == -INFINITY ? 0.f : exp2f(ml.x - Mn);
                     L = fmaf(ml.y, z, L * keep);
                     acc = fma_f4(o, make_float4(z, z, z, z), make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep));
                     M = Mn;
+                };
+                if (all) {
+                    add(make_float4(rec[dim], rec[dim + 1], rec[dim + 2], rec[dim + 3]), make_float2(rec[D], rec[D + 1]));
+                } else {
+#pragma unroll 2
+                    for (int c = c0 + warp; c <= c1; c += C::WARPS) {
+                        const float* part = p.own_parts + (2 * (size_t)c + (c == c0)) * C::PART;
+                        add(__ldcg(reinterpret_cast<const float4*>(part + e0)), __ldcg(reinterpret_cast<const float2*>(part + kSharedGroup * D + 2 * hg)));
+                    }
                 }
-                *reinterpret_cast<float2*>(mine + hg * C::REC + dim) = make_float2(acc.x, acc.y);
-                *reinterpret_cast<float2*>(mine + hg * C::REC + dim + 2) = make_float2(acc.z, acc.w);
-                if (dim == 0) *reinterpret_cast<float2*>(mine + hg * C::REC + D) = make_float2(M, L);
+#pragma unroll 2
+                for (int c = x0 + warp; c <= x1; c += C::WARPS) {
+                    const size_t at = row0 + (size_t)2 * kSharedRows * c + hg;
+                    add(__ldcg(reinterpret_cast<const float4*>(p.rows_o + at * D + dim)), __ldcg(p.rows_ml + at));
+                }
+                __syncwarp();                                                // all have read what the first lane of a head writes over
+                if (eb + 4 * lane < G * D) {
+                    *reinterpret_cast<float2*>(rec + dim) = make_float2(acc.x, acc.y);
+                    *reinterpret_cast<float2*>(rec + dim + 2) = make_float2(acc.z, acc.w);
+                    if (dim == 0) *reinterpret_cast<float2*>(rec + D) = make_float2(M, L);
+                }
             }
         }
         reduce(true);
@@ -471,6 +496,8 @@ static int launch_shared(const SharedArgs& p, cudaStream_t st) {
         attr_set.mark();
     }
     FT_CHECK_CUDA(launch_after(shared_plan_kernel, dim3(1), dim3(SP_THREADS), 0, st, p));
+    if (p.n_groups)
+        if (int r = launch_shared_prefix(p, D, st)) return r;
     FT_CHECK_CUDA(launch_after(shared_decode_kernel<D>, dim3(p.own_ctas), dim3(C::THREADS), C::SMEM, st, p));
     return 0;
 }
@@ -484,10 +511,11 @@ extern "C" long long ft_attn_decode_shared_scratch_bytes(int B, int n_groups, in
 }
 
 extern "C" int ft_attn_shared_waits(void) {
-    int n = 0;
+    int n = 0, m = 0;
     FT_CHECK_CUDA(cudaDeviceSynchronize());                                  // the copies below wait for the default stream only
     FT_CHECK_CUDA(cudaMemcpyFromSymbol(&n, ft::g_shared_decode_waits, sizeof(n)));
-    return n;
+    if (int r = ft::shared_prefix_waits(&m)) return r;
+    return n | m;
 }
 
 extern "C" int ft_attn_decode_shared(const void* q, const void* kv_layer, int num_pages, const int* page_table, int table_rows, int max_pages, const int* req_slot,
