@@ -1,0 +1,835 @@
+// Attention of one query token per sequence over common prefixes and own tails: out[b][h] = sum_j softmax_j(q . k_j / sqrt(D)) v_j, j < ctx_lens[b], with the first tokens of a
+// group's sequences read once for all of them.  The lists of work are in shared.cuh.
+//
+// One CTA per SM does both kinds of work side by side, since one is bound by the tensor and exponential units and the other by memory:
+//   prefix   tcgen05 / TMEM as in attention_tc.cu: a tile of up to 2 * (128 / G) queries in two halves of up to 128 rows (row = query * G + head of the group).  Per page and
+//            half S = Q K^T (M128 N64 K=D, the cache's slab as it lies), one thread a row for the softmax, P to tensor memory over the scores that it came from,
+//            O += P V (M128 N=D K64).  Queries that fill one half only go to both halves, which take every other page each.  All rows see all pages: the only
+//            mask is the end of the last one.
+//   own      a warp walks a share of its own: chunks of 16 KB by bulk copies that it asks for itself, two of them on their way while it multiplies (mma.sync, the
+//            query heads of a key head in the columns).  No warp waits for another.
+// Each share's results are O, maximum and sum of its rows; a second kernel puts them together in their order.  A (sequence, key head) that one warp has whole and that
+// has no prefix is written right away.
+#include "common.cuh"
+#include "ft_internal.h"
+#include "shared.cuh"
+
+namespace ft {
+
+constexpr float kSharedLog2E = 1.4426950408889634f;
+// Probabilities are formed 2^6 times their size, so that fp16's normal numbers reach down to 2^-20 of the largest; a running maximum may lag by 2^8
+constexpr float kSharedTop = 6.f, kSharedGrow = 8.f;
+
+// Groups of four warps: warp 0 copies the prefix's pages, 1 and 2 issue the halves' products, 3 owns tensor memory; 4 .. 11 softmax (half = (warp - 4) / 4); 12 .. 15 own
+constexpr int SH_THREADS = 512, SH_WARPS = SH_THREADS / 32;
+constexpr int SH_REGS = 128, SH_REGS_ISSUE = 64, SH_REGS_SOFT = 152, SH_REGS_OWN = 144;
+static_assert(SH_REGS_ISSUE + 2 * SH_REGS_SOFT + SH_REGS_OWN <= 4 * SH_REGS, "what the block is launched with");
+constexpr int SH_SOFT = 256;
+constexpr int SH_PIECE = kKvTile * 128;          // [64 tokens][64 dims] in fp16
+
+__device__ int g_shared_waits;                   // 1: a wait ran out on this device (ft_attn_shared_waits)
+
+template <int D>
+struct Shared {
+    static constexpr int KH = D / 64;
+    static constexpr int TILE = 2 * KH * SH_PIECE;                           // K | V of a page
+    // of the prefix.  Three at least: a half that has every other page asks for its scores two of its own pages ahead, whose stage must not wait for a product behind them
+    static constexpr int STAGES = D == 64 ? 4 : 3;
+    static constexpr int QBLK = kSharedRows * 128;                           // [128 rows][64 dims]
+    static constexpr int OWN_WARPS = D == 64 ? 4 : 2, OWN_STAGES = 2;
+    static constexpr int CHUNK = D == 64 ? 64 : 32;                          // tokens
+    static constexpr int CHUNK_BYTES = 2 * CHUNK * D * 2, HALF = CHUNK_BYTES / 2;        // keys | values; of each D / 64 pieces of [CHUNK][64 dims]
+    static constexpr int KV = 2 * KH * QBLK, OWN = KV + STAGES * TILE, SMEM = 1024 + OWN + OWN_WARPS * OWN_STAGES * CHUNK_BYTES;
+    // tensor memory: scores [half][2][64 columns] (probabilities, pairs of fp16, over the first 32 of them), O [half][D]
+    static constexpr int COL_S = 0, COL_O = 256, COLS = 512;
+    static_assert(COL_O + 2 * D <= COLS, "tensor memory");
+    static_assert(SMEM <= 232448 - 1536, "shared memory");
+};
+
+// floats of an own part: O [G][D], (m, l) of the heads; on 16 bytes
+__host__ __device__ __forceinline__ int shared_part(int G, int d) { return (G * (d + 2) + 3) / 4 * 4; }
+
+// ------------------------------------------------------------------ own part
+// A warp's state of one (sequence, key head): S[token][query] = K Q^T with 16 tokens in the rows of mma.sync; the probabilities, transposed 8 x 8 at a time, are the other
+// operand of O^T[dim][query] = V^T P^T, where all 16 rows are dims.
+template <int D>
+struct SharedQuery {
+    static constexpr int CHUNK = Shared<D>::CHUNK, BLOCKS = CHUNK / 16;
+    uint32_t q[D / 16][2];
+    float o[D / 16][4];                  // O^T: dims 16 i + g (+ 8), queries 2 tq (+ 1) at [i][2 * upper + (query & 1)]
+    float m[2], l[2];                    // of queries 2 tq (+ 1): reference, this lane's tokens' sum
+
+    static __device__ __forceinline__ int at(int t, int c) { return (c >> 3) * (CHUNK * 128) + t * 128 + (((c & 7) ^ (t & 7)) << 4); }       // 16-byte chunk c of token t
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.f;
+    }
+    __device__ __forceinline__ void load_query(const __half* row, int tq) {  // row: query head g of the group, or null
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            q[ks][0] = row ? *reinterpret_cast<const uint32_t*>(row + ks * 16 + 2 * tq) : 0u;
+            q[ks][1] = row ? *reinterpret_cast<const uint32_t*>(row + ks * 16 + 8 + 2 * tq) : 0u;
+        }
+    }
+    // tokens lo .. hi - 1 of the chunk at `tile` (an address in shared memory); its hidden values are zeros
+    __device__ __forceinline__ void chunk(uint32_t tile, int lo, int hi, float scale_log2, int lane) {
+        const int g = lane >> 2;
+        float s[BLOCKS][4], most[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b) {
+            s[b][0] = s[b][1] = s[b][2] = s[b][3] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks) {
+                uint32_t a0, a1, a2, a3;
+                ldmatrix_x4(tile + at(16 * b + (lane & 15), 2 * ks + (lane >> 4)), a0, a1, a2, a3);
+                mma_f16_16816(s[b], a0, a1, a2, a3, q[ks][0], q[ks][1]);
+            }
+        }
+        if (lo > 0 || hi < CHUNK) {
+#pragma unroll
+            for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int t = 16 * b + 8 * (e >> 1) + g;
+                    s[b][e] = t >= lo && t < hi ? s[b][e] : -INFINITY;
+                }
+        }
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b) {
+            most[0] = fmaxf(most[0], fmaxf(s[b][0], s[b][2]));
+            most[1] = fmaxf(most[1], fmaxf(s[b][1], s[b][3]));
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) most[e] = fmaxf(most[e], __shfl_xor_sync(0xffffffffu, most[e], x));
+            most[e] *= scale_log2;
+        }
+        if (__any_sync(0xffffffffu, most[0] > m[0] + kSharedGrow || most[1] > m[1] + kSharedGrow)) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float m_new = fmaxf(m[e], most[e]);
+                const float keep = m_new == -INFINITY ? 1.f : ex2_fast(m[e] - m_new);
+                l[e] *= keep;
+                m[e] = m_new;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) o[i][e] *= keep, o[i][2 + e] *= keep;
+            }
+        }
+        const float r0 = kSharedTop - (m[0] == -INFINITY ? 0.f : m[0]), r1 = kSharedTop - (m[1] == -INFINITY ? 0.f : m[1]);
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b) {
+            uint32_t pb[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float p0 = ex2_fast(fmaf(s[b][2 * h], scale_log2, r0)), p1 = ex2_fast(fmaf(s[b][2 * h + 1], scale_log2, r1));
+                l[0] += p0;
+                l[1] += p1;
+                const __half2 t = __floats2half2_rn(p0, p1);
+                asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pb[h]) : "r"(*reinterpret_cast<const uint32_t*>(&t)));
+            }
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                uint32_t a0, a1, a2, a3;
+                ldmatrix_x4_trans(tile + Shared<D>::HALF + at(16 * b + (lane & 7) + (lane >> 4) * 8, 2 * i + (lane >> 3 & 1)), a0, a1, a2, a3);
+                mma_f16_16816(o[i], a0, a1, a2, a3, pb[0], pb[1]);
+            }
+        }
+    }
+    // sums over all lanes' tokens
+    __device__ __forceinline__ void total(float* sum) const {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            sum[e] = l[e];
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], x);
+        }
+    }
+};
+
+template <int D>
+__device__ __forceinline__ void shared_own(const SharedArgs& p, OwnWalk w, int groups, int per, int warp, uint8_t* ring, uint64_t* full, volatile int* dead, int* err) {
+    using C = Shared<D>;
+    constexpr int S = C::OWN_STAGES, CH = C::CHUNK;
+    const int lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3, G = p.G;
+    const uint64_t pol = policy_evict_first();                               // every byte is read once
+    bool ok = true;
+    int it = 0, asked = 0;                                                   // chunks of the share so far, with a page: a stage's phase follows from the count
+    while (w.next(p, groups)) {
+        const int unit = w.b * p.nkv + w.h, n = w.t1 - w.t0;
+        // what each step reads: lane x has step x of the next 32
+        int lo_x, hi_x, page_x, row;
+        auto steps_from = [&](int x0) {
+            w.step(p, x0 + lane, lo_x, hi_x, row);
+            page_x = -1;
+            if (x0 + lane < w.t1 && lo_x < hi_x) {
+                row = p.row_of(row);
+                if (row >= 0) page_x = p.page_table[(size_t)row * p.max_pages + lo_x / kKvTile];
+                if (page_x >= p.num_pages) page_x = -1;
+            }
+        };
+        steps_from(w.t0);
+        // 2 D / 64 pieces of a chunk, a lane each
+        auto copy = [&](int x, int stage) {                                  // x: of the 32
+            const int page = __shfl_sync(0xffffffffu, page_x, x), first = __shfl_sync(0xffffffffu, lo_x, x) / CH * CH % kKvTile;
+            if (page < 0) return;
+            uint8_t* dst = ring + stage * C::CHUNK_BYTES;
+            const uint8_t* src = p.cache + ((size_t)page * p.nkv + w.h) * C::TILE;
+            if (CH == kKvTile) {
+                if (lane == 0) {
+                    mbar_expect_tx(&full[stage], C::CHUNK_BYTES);
+                    tma_bulk_g2s(dst, src, C::CHUNK_BYTES, &full[stage], pol);
+                }
+            } else {
+                if (lane == 0) mbar_expect_tx(&full[stage], C::CHUNK_BYTES);
+                __syncwarp();
+                if (lane < 2 * C::KH) tma_bulk_g2s(dst + lane * (CH * 128), src + lane * SH_PIECE + first * 128, CH * 128, &full[stage], pol);
+            }
+        };
+        SharedQuery<D> a;
+        a.clear();
+        a.load_query(g < G ? p.q + ((size_t)w.b * p.nq + (size_t)w.h * G + g) * D : nullptr, tq);
+        // copies run S chunks ahead
+        for (int x0 = 0; x0 < n; x0 += 32) {
+            if (x0) steps_from(w.t0 + x0);
+            const int here = min(32, n - x0);
+            int next = 0;
+            for (int x = 0; x < here; ++x) {
+                for (; ok && next < here && asked < it + S; ++next)
+                    if (__shfl_sync(0xffffffffu, page_x, next) >= 0) copy(next, asked++ % S);
+                if (!ok) break;
+                if (__shfl_sync(0xffffffffu, page_x, x) < 0) continue;
+                const int stage = it % S;
+                ok = __all_sync(0xffffffffu, mbar_wait_limited(&full[stage], it / S & 1, dead));
+                if (!ok) break;
+                ++it;
+                const int lo = __shfl_sync(0xffffffffu, lo_x, x), hi = __shfl_sync(0xffffffffu, hi_x, x), base = lo / CH * CH;
+                uint8_t* tile = ring + stage * C::CHUNK_BYTES;
+                if (lo > base || hi < base + CH) {                           // hidden values may be anything: 0 * infinity is none
+                    const int ahead = lo - base, hidden = ahead + base + CH - hi;
+                    for (int u = lane; u < hidden * (D / 8); u += 32) {
+                        const int k = u / (D / 8), c = u % (D / 8), tok = k < ahead ? k : hi - base + k - ahead;
+                        *reinterpret_cast<uint4*>(tile + C::HALF + SharedQuery<D>::at(tok, c)) = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    fence_proxy_async();                                     // ahead of the next copy into this stage
+                    __syncwarp();
+                }
+                a.chunk(smem_u32(tile), lo - base, hi - base, p.scale_log2, lane);
+                __syncwarp();                                                // all lanes have read it: the next copy may come
+            }
+        }
+        if (!ok) {                                                           // NaN for all that this (sequence, head) says
+            *err = 1;
+            a.m[0] = a.m[1] = 0.f;
+            a.l[0] = a.l[1] = NAN;
+        }
+        float sum[2];
+        a.total(sum);
+        const bool all = w.t0 == 0 && w.t1 == w.s.steps && !w.s.prefix;
+        if (lane == 0 && w.t0 == 0) {
+            const int last = (int)((unsigned)(w.unit_f + w.s.steps - 1) / (unsigned)per);
+            p.own_units[unit] = all ? make_int4(-1, 0, 0, 0) : make_int4(warp, last, w.s.prefix, 0);
+        }
+        float* part = p.own_parts + (size_t)(unit + warp) * shared_part(G, D);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int head = 2 * tq + e;
+            if (head >= G) continue;
+            if (all) {                                                       // a query without a visible key: zeros
+                const float r = sum[e] == 0.f ? 0.f : 1.f / sum[e];
+                const size_t at = ((size_t)w.b * p.nq + (size_t)w.h * G + head) * D;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const float x = a.o[i][2 * u + e] * r;
+                        const __nv_bfloat16 hi = __float2bfloat16(x);
+                        p.out[at + 16 * i + 8 * u + g] = hi;
+                        if (p.out_lo) p.out_lo[at + 16 * i + 8 * u + g] = __float2bfloat16(x - __bfloat162float(hi));
+                    }
+            } else {
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    part[head * D + 16 * i + g] = a.o[i][e];
+                    part[head * D + 16 * i + 8 + g] = a.o[i][2 + e];
+                }
+                if (g == 0) *reinterpret_cast<float2*>(part + G * D + 2 * head) = make_float2(a.m[e], sum[e]);
+            }
+        }
+    }
+    if (lane == 0)
+        for (int i = it; i < asked; ++i)                                     // nothing may still be on its way into this CTA's memory when it ends
+            for (int k = 0; k < kWaitLimit && !mbar_try_wait(&full[i % S], i / S & 1); ++k) {}
+}
+
+// A page of the prefix that lands in a stage tells who waits for it by one of three barriers: of the pages that half 0 alone takes, of those of half 1, of those of both.  (With
+// one barrier a half that takes every other page could see only every second phase of a stage, and a phase looks complete while the one before it is under way.)
+// Each role keeps the phases of the barriers that it uses: one bit each, turned by every page.
+struct SharedPhases {
+    uint32_t bits = 0;
+    int at;                              // the barrier of the last page asked for
+    __device__ __forceinline__ uint32_t next(int stages, int stage, int set) {
+        at = set * stages + stage;
+        const uint32_t parity = bits >> at & 1;
+        bits ^= 1u << at;
+        return parity;
+    }
+};
+
+// Exclusive sum over the block's threads; `all` is the sum of all
+__device__ __forceinline__ int shared_before(int mine, int* warp_s, int& all) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += up;
+    }
+    if (lane == 31) warp_s[warp] = x;
+    __syncthreads();
+    int w = lane < SH_WARPS ? warp_s[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < SH_WARPS; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += up;
+    }
+    all = __shfl_sync(0xffffffffu, w, SH_WARPS - 1);
+    const int ahead = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+    return x - mine + (warp ? ahead : 0);
+}
+
+template <int D>
+__global__ void __launch_bounds__(SH_THREADS, 1)
+shared_attn_kernel(const __grid_constant__ SharedArgs p) {
+    using C = Shared<D>;
+    constexpr int KH = C::KH;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ uint64_t kv_full[3 * C::STAGES], kv_empty[C::STAGES];         // (full: see SharedPhases)
+    __shared__ uint64_t own_full[C::OWN_WARPS * C::OWN_STAGES];
+    __shared__ uint64_t q_full[2];                                           // the queries of a half
+    __shared__ uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];           // half, buffer: scores are in tensor memory; probabilities are; O += P V retired
+    __shared__ uint64_t drained[2];                                          // all products of a half retired
+    __shared__ int tokens_s[C::STAGES];                                      // of the page in each stage; 0: the page is not there
+    __shared__ int sums_s[2][SH_WARPS];
+    __shared__ int2 prefix_at, own_at[C::OWN_WARPS];                         // the group (sequence) that a share begins in, and where that begins
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int dead;
+    int* const err = &g_shared_waits;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int s = 0; s < 3 * C::STAGES; ++s) mbar_init(&kv_full[s], 1);
+        for (int s = 0; s < C::STAGES; ++s) mbar_init(&kv_empty[s], 2);
+        for (int s = 0; s < C::OWN_WARPS * C::OWN_STAGES; ++s) mbar_init(&own_full[s], 1);
+        for (int h = 0; h < 2; ++h) {
+            mbar_init(&q_full[h], kSharedRows / 32);
+            mbar_init(&drained[h], 1);
+            for (int s = 0; s < 2; ++s) mbar_init(&s_full[h][s], 1), mbar_init(&p_full[h][s], kSharedRows / 32), mbar_init(&pv_done[h][s], 1);
+        }
+        fence_mbar_init();
+        dead = 0;
+    }
+    if (warp == 3) {
+        tmem_alloc(&tmem_slot, C::COLS);
+        tmem_relinquish();
+    }
+    pdl_wait();
+
+    // ---------------- the plan: every CTA adds up both lists.  A list of groups that does not grow, or leaves the batch, shares nothing
+    int groups, prefix_f, prefix_end, prefix_per, own_per, own_total;
+    {
+        const int gc = (p.n_groups + SH_THREADS - 1) / SH_THREADS, g0 = min(p.n_groups, tid * gc), g1 = min(p.n_groups, g0 + gc);
+        const int bc = (p.B + SH_THREADS - 1) / SH_THREADS, b0 = min(p.B, tid * bc), b1 = min(p.B, b0 + bc);
+        bool grows = true;
+        int mine = 0;
+        for (int g = g0; g < g1; ++g) {
+            grows = grows && p.group_start[g] >= 0 && p.group_start[g] <= p.group_start[g + 1] && p.group_start[g + 1] <= p.B;
+            SharedPrefix w;
+            w.load(p, g);
+            if (grows) mine += w.all(p);
+        }
+        groups = __syncthreads_and(grows) ? p.n_groups : 0;
+        if (!groups) mine = 0;
+        int total;
+        int before = shared_before(mine, sums_s[0], total);
+        prefix_per = (int)((unsigned)(total + gridDim.x - 1) / gridDim.x);
+        prefix_f = min(prefix_per * (int)blockIdx.x, total);
+        prefix_end = min(prefix_f + prefix_per, total);
+        if (before <= prefix_f && prefix_f < before + mine) {
+            SharedPrefix w;
+            int g = g0;
+            for (w.load(p, g); before + w.all(p) <= prefix_f; w.load(p, ++g)) before += w.all(p);
+            prefix_at = make_int2(g, before);
+        }
+        mine = 0;
+        int g = shared_group_of(p.group_start, groups, b0);
+        for (int b = b0, x = g; b < b1; ++b) {
+            while (x + 1 < groups && p.group_start[x + 1] <= b) ++x;
+            SharedSeq s;
+            s.load(p, b, x, p.ctx_lens[b]);
+            mine += s.steps;
+        }
+        before = shared_before(mine, sums_s[1], total) * p.nkv;
+        mine *= p.nkv;
+        own_total = total * p.nkv;
+        const int warps = gridDim.x * C::OWN_WARPS;
+        own_per = (int)((unsigned)(own_total + warps - 1) / (unsigned)warps);
+        for (int w = 0; w < C::OWN_WARPS; ++w) {
+            const int f = own_per * (w * (int)gridDim.x + (int)blockIdx.x);  // (neighbouring shares on different SMs)
+            if (before <= f && f < before + mine) {
+                int b = b0, at = before, x = g;
+                for (;; ++b) {
+                    while (x + 1 < groups && p.group_start[x + 1] <= b) ++x;
+                    SharedSeq s;
+                    s.load(p, b, x, p.ctx_lens[b]);
+                    if (f < at + s.steps * p.nkv) break;
+                    at += s.steps * p.nkv;
+                }
+                own_at[w] = make_int2(b, at);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    bool ok = true;                                                          // false: a wait ran out
+    PrefixWalk w;
+    const int2 at_s = prefix_at;
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SH_REGS_ISSUE));
+        if (warp == 0) {
+            // ---------------- copies of the prefix: one page a time
+            w.start(p, prefix_f, prefix_end, at_s.x, at_s.y);
+            const uint64_t pol = policy_evict_first();
+            SharedPhases phases;
+            int it = 0;
+#pragma unroll 1
+            while (w.next(p)) {
+                const int p1 = w.p0 + w.pages, row = p.row_of(w.w.seq0);
+#pragma unroll 1
+                for (int p0 = w.p0; p0 < p1; p0 += 32) {
+                    const int tile = p0 + lane;
+                    int my_page = tile < p1 && row >= 0 ? p.page_table[(size_t)row * p.max_pages + tile] : -1;
+                    if (my_page >= p.num_pages) my_page = -1;
+                    const int n = min(32, p1 - p0);
+#pragma unroll 1
+                    for (int k = 0; k < n; ++k, ++it) {
+                        const int page = __shfl_sync(0xffffffffu, my_page, k);
+                        if (lane == 0 && ok) {
+                            const int s = it % C::STAGES;
+                            ok = mbar_wait_limited(&kv_empty[s], (it / C::STAGES & 1) ^ 1, &dead);
+                            if (!ok) continue;
+                            phases.next(C::STAGES, s, w.few ? (p0 + k - w.p0) & 1 : 2);
+                            tokens_s[s] = page >= 0 ? min(kKvTile, w.w.tokens - (p0 + k) * kKvTile) : 0;
+                            if (page >= 0) {
+                                mbar_expect_tx(&kv_full[phases.at], C::TILE);
+                                tma_bulk_g2s(smem + C::KV + s * C::TILE, p.cache + ((size_t)page * p.nkv + w.h) * C::TILE, C::TILE, &kv_full[phases.at], pol);
+                            } else {
+                                mbar_arrive(&kv_full[phases.at]);
+                            }
+                        }
+                    }
+                }
+            }
+            if (lane == 0)
+                for (int i = 0; i < 3 * C::STAGES; ++i)                      // nothing may still be on its way into this CTA's memory when it ends
+                    for (int k = 0; k < kWaitLimit && !mbar_try_wait(&kv_full[i], (phases.bits >> i & 1) ^ 1); ++k) {}
+            __syncwarp();
+        } else if (warp < 3) {
+            // ---------------- products, one warp a half
+            constexpr uint32_t idesc_qk = umma_idesc_f16(kSharedRows, kKvTile, false), idesc_pv = umma_idesc_f16(kSharedRows, D, true);
+            const int h = warp - 1;
+            w.start(p, prefix_f, prefix_end, at_s.x, at_s.y);
+            if (elect_one()) {
+                const uint64_t q_desc = umma_desc_k128(smem_u32(smem + h * KH * C::QBLK)), k_desc = umma_desc_k128(smem_u32(smem + C::KV)),
+                               v_desc = umma_desc_mn128(smem_u32(smem + C::KV) + KH * SH_PIECE);
+                const uint32_t s_at = tmem + C::COL_S + h * 128, o_at = tmem + C::COL_O + h * D;
+                SharedPhases phases;
+                int base = 0, n_qk = 0, n_pv = 0, n_q = 0;                   // pages of the share, products of this half, stretches of this half so far
+                auto issue_qk = [&](int page, bool alone) {                  // page: counted over the whole share; alone: the other half has no use for it
+                    const int s = page % C::STAGES, buf = n_qk & 1;
+                    const uint32_t parity = phases.next(C::STAGES, s, alone ? h : 2);
+                    ok = mbar_wait_limited(&kv_full[phases.at], parity, &dead);
+                    if (!ok) return;
+                    ++n_qk;
+                    tc_fence_after();
+                    const uint64_t b = k_desc + (uint64_t)(s * (C::TILE >> 4));
+#pragma unroll
+                    for (int kh = 0; kh < KH; ++kh)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) umma_bf16(s_at + buf * 64, q_desc + kh * (C::QBLK >> 4) + 2 * k, b + kh * (SH_PIECE >> 4) + 2 * k, idesc_qk, (kh | k) != 0);
+                    umma_commit(&s_full[h][buf]);
+                };
+                auto issue_pv = [&](int page, bool first, bool alone) {
+                    const int s = page % C::STAGES, buf = n_pv & 1;
+                    ok = mbar_wait_limited(&p_full[h][buf], n_pv >> 1 & 1, &dead);
+                    if (!ok) return;
+                    ++n_pv;
+                    tc_fence_after();
+                    const uint64_t b = v_desc + (uint64_t)(s * (C::TILE >> 4));
+#pragma unroll
+                    for (int k = 0; k < kKvTile / 16; ++k) umma_f16_ts(o_at, s_at + buf * 64 + 8 * k, b + k * (2048 >> 4), idesc_pv, k != 0 || !first);
+                    umma_commit(&pv_done[h][buf]);
+                    umma_commit(&kv_empty[s]);
+                    if (alone) umma_commit(&kv_empty[s]);
+                };
+#pragma unroll 1
+                while (w.next(p)) {
+                    const int mine = w.of_half(h);
+                    auto page_of = [&](int i) { return base + (w.few ? h + 2 * i : i); };      // page i of this half
+                    if (ok && mine) {
+                        ok = mbar_wait_limited(&q_full[h], n_q++ & 1, &dead);
+                        tc_fence_after();
+                        // Scores run two pages ahead, issued behind the product that reads the probabilities in their buffer
+#pragma unroll 1
+                        for (int i = -2; ok && i < mine; ++i) {
+                            if (i >= 0) issue_pv(page_of(i), i == 0, w.few);
+                            if (ok && i + 2 < mine) issue_qk(page_of(i + 2), w.few);
+                        }
+                    }
+                    base += w.pages;
+                }
+                umma_commit(&drained[h]);                                    // nothing may still run in tensor memory when it is given back, whoever gave up
+#pragma unroll 1
+                for (int k = 0; k < kWaitLimit && !mbar_try_wait(&drained[h], 0); ++k) {}
+            }
+            __syncwarp();
+        }
+    } else if (warp < 12) {
+        // ---------------- softmax: one thread a row
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SH_REGS_SOFT));
+        w.start(p, prefix_f, prefix_end, at_s.x, at_s.y);
+        const int h = (warp - 4) >> 2;
+        const int row = (tid - 128) & 127;                                           // lane of tensor memory: warp % 4 is the quarter that a warp may read
+        const int tok = row / p.G;
+        const uint32_t lanes = tmem + ((uint32_t)(row & 96) << 16);
+        const uint32_t s_at0 = lanes + C::COL_S + h * 128, o_at = lanes + C::COL_O + h * D;
+        SharedPhases phases;
+        int base = 0, cnt = 0;                                               // pages of the share, pages of this half so far
+        // maxima and sums of a half, where its queries were: the products that read those have retired
+        auto ml_of = [&](int half) { return reinterpret_cast<float2*>(smem + half * KH * C::QBLK); };
+        auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_limited(bar, parity, &dead)); };
+#pragma unroll 1
+        while (w.next(p)) {
+            const int mine = w.of_half(h);
+            const int tok0 = w.few ? 0 : h * p.th;                           // of the tile
+            const bool valid = tok < p.th && tok0 + tok < w.n;
+            const int i0 = w.tile * 2 * p.th + tok0;                         // of the group
+            if (mine) {
+                // the queries, 16 bytes at a time, zeros for rows without one (the products that read the last stretch's have retired: their scores were here)
+                constexpr int CH = D / 8;
+#pragma unroll 4
+                for (int k = row; k < kSharedRows * CH; k += kSharedRows) {
+                    const int c = k % CH, r = k / CH, tk = r / p.G, head = r - tk * p.G;
+                    const bool on = tk < p.th && tok0 + tk < w.n;
+                    const __half* from = p.q + ((size_t)(w.w.seq0 + i0 + (on ? tk : 0)) * p.nq + (size_t)w.h * p.G + (on ? head : 0)) * D + c * 8;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem + (h * KH + (c >> 3)) * C::QBLK + r * 128 + ((c & 7) ^ (r & 7)) * 16)), "l"(from),
+                                 "r"(on ? 16 : 0)
+                                 : "memory");
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full[h]);
+            }
+            float m_ref = -INFINITY, l_run = 0.f;
+#pragma unroll 1
+            for (int i = 0; i < mine; ++i, ++cnt) {
+                const int buf = cnt & 1, page = base + (w.few ? h + 2 * i : i), stage = page % C::STAGES;
+                const uint32_t landed = phases.next(C::STAGES, stage, w.few ? h : 2);
+                ok = ok && wait(&s_full[h][buf], cnt >> 1 & 1);
+                if (!ok) break;
+                tc_fence_after();
+                uint32_t sr[64];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld16_nowait(s_at0 + buf * 64 + 16 * c, sr + 16 * c);
+                const int seen = tokens_s[stage];                            // (written ahead of the copy that the scores came of)
+                tmem_arrived<64>(sr);
+                if (seen < kKvTile) {
+#pragma unroll
+                    for (int c = 0; c < 64; ++c) sr[c] = c < seen ? sr[c] : 0xff800000u;
+                    // values behind the end may be anything, and 0 * infinity is not 0.  (Both halves may write here: zeros.)
+                    ok = wait(&kv_full[phases.at], landed);
+                    if (!ok) break;
+                    uint8_t* v = smem + C::KV + stage * C::TILE + KH * SH_PIECE;
+#pragma unroll 1
+                    for (int u = row; u < (kKvTile - seen) * 8 * KH; u += kSharedRows) {
+                        const int kh = u / ((kKvTile - seen) * 8), x = u % ((kKvTile - seen) * 8);
+                        *reinterpret_cast<uint4*>(v + kh * SH_PIECE + seen * 128 + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    fence_proxy_async();
+                }
+                float t0 = max3(sr[0], sr[1], sr[2]), t1 = max3(sr[3], sr[4], sr[5]);
+#pragma unroll
+                for (int c = 6; c < 62; c += 4) t0 = max3(t0, sr[c], sr[c + 1]), t1 = max3(t1, sr[c + 2], sr[c + 3]);
+                t0 = max3(t0, sr[62], sr[63]);
+                const float m_new = fmaxf(m_ref, fmaxf(t0, t1) * p.scale_log2);
+                if (i == 0) {
+                    m_ref = m_new;
+                } else if (__any_sync(0xffffffffu, valid && m_new > m_ref + kSharedGrow)) {        // tcgen05.ld / st are warp-wide: all 32 rows
+                    ok = wait(&pv_done[h][buf ^ 1], (cnt - 1) >> 1 & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const float alpha = m_new == -INFINITY ? 1.f : exp2f(m_ref - m_new);
+                    l_run *= alpha;
+                    m_ref = m_new;
+#pragma unroll 1
+                    for (int c = 0; c < D / 16; ++c) {
+                        uint32_t o[16];
+                        tmem_ld16_nowait(o_at + 16 * c, o);
+                        tmem_arrived<16>(o);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+                        tmem_st16(o_at + 16 * c, o);
+                    }
+                }
+                const float mu = kSharedTop - (m_ref == -INFINITY ? 0.f : m_ref);
+                const f32x2 plus = pack2(mu, mu), scale = pack2(p.scale_log2, p.scale_log2);
+                f32x2 sum[2] = {0, 0};                                       // pairs of fp32 zeros
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int c = half * 32 + 2 * e;
+                        float p0, p1;
+                        unpack2(fma2(pack2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), scale, plus), p0, p1);
+                        p0 = ex2_fast(p0), p1 = ex2_fast(p1);
+                        sum[e & 1] = sum2(sum[e & 1], pack2(p0, p1));
+                        const __half2 x = __floats2half2_rn(p0, p1);
+                        pk[e] = *reinterpret_cast<const uint32_t*>(&x);
+                    }
+                    tmem_st16(s_at0 + buf * 64 + 16 * half, pk);             // over the scores that they came from (this row has read them)
+                }
+                tmem_st_wait();
+                float a0, a1;
+                unpack2(sum2(sum[0], sum[1]), a0, a1);
+                l_run += a0 + a1;
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[h][buf]);
+            }
+            if (ok && mine) ok = wait(&pv_done[h][(cnt - 1) & 1], (cnt - 1) >> 1 & 1);
+            tc_fence_after();
+            if (!ok) {                                                       // NaN for all that this unit says
+                l_run = NAN;
+                m_ref = 0.f;
+            }
+            const int row0 = w.w.row(p, w.h, i0);
+            const size_t at = (size_t)row0 + (size_t)2 * kSharedRows * blockIdx.x + row;
+            if (w.p0 == 0 && valid && row == tok * p.G && (!w.few || h == 0))        // the unit begins here: where each of its queries' results will be
+                p.prefix_units[(size_t)(w.w.seq0 + i0 + tok) * p.nkv + w.h] = make_int4(blockIdx.x, (int)((unsigned)(w.unit_f + w.steps - 1) / (unsigned)prefix_per), row0 + row, 0);
+            float z = 1.f, zo = 0.f, m = m_ref, l = l_run;
+            if (w.few) {                                                     // the halves' results as one: each half puts half of the dims together
+                ml_of(h)[row] = make_float2(m_ref, l_run);
+                tc_fence_before();
+                asm volatile("bar.sync 1, %0;" ::"n"(SH_SOFT) : "memory");
+                tc_fence_after();
+                const float2 other = ml_of(1 - h)[row];
+                m = fmaxf(m_ref, other.x);
+                z = m_ref == -INFINITY ? 0.f : exp2f(m_ref - m), zo = other.x == -INFINITY ? 0.f : exp2f(other.x - m);
+                l = h == 0 ? l_run * z + other.y * zo : other.y * zo + l_run * z;
+            }
+            const int c0 = w.few ? h * (D / 32) : 0, c1 = w.few ? c0 + D / 32 : D / 16;
+#pragma unroll 1
+            for (int c = c0; c < c1; ++c) {
+                uint32_t o[16];
+                tmem_ld16_nowait(o_at + 16 * c, o);
+                tmem_arrived<16>(o);
+                if (w.few) {                                                 // a half without a page has nothing in tensor memory
+                    uint32_t x[16];
+                    tmem_ld16_nowait(lanes + C::COL_O + (1 - h) * D + 16 * c, x);
+                    tmem_arrived<16>(x);
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const float u = z == 0.f ? 0.f : __uint_as_float(o[k]) * z, v = zo == 0.f ? 0.f : __uint_as_float(x[k]) * zo;
+                        o[k] = __float_as_uint(h == 0 ? u + v : v + u);
+                    }
+                }
+                if (valid) {
+                    float4* to = reinterpret_cast<float4*>(p.rows_o + at * D + 16 * c);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) to[k] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
+                }
+            }
+            if (valid && (!w.few || h == 0)) p.rows_ml[at] = make_float2(m, l);
+            if (w.few) {                                                     // the other half has read what the next products write over
+                tc_fence_before();
+                asm volatile("bar.sync 1, %0;" ::"n"(SH_SOFT) : "memory");
+            }
+            base += w.pages;
+        }
+        tmem_st_wait();
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SH_REGS_OWN));
+        const int mine = warp - 12;
+        if (mine < C::OWN_WARPS) {
+            const int index = mine * gridDim.x + blockIdx.x, f = min(own_per * index, own_total);
+            OwnWalk o;
+            o.start(p, groups, f, min(f + own_per, own_total), own_at[mine].x, own_at[mine].y);
+            shared_own<D>(p, o, groups, own_per, index, smem + C::OWN + mine * (C::OWN_STAGES * C::CHUNK_BYTES), own_full + mine * C::OWN_STAGES, &dead, err);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (tid == 0 && dead) *err = 1;
+    if (warp == 3) {
+        tc_fence_after();
+        tmem_dealloc(tmem, C::COLS);
+    }
+}
+
+// ------------------------------------------------------------------ all parts of a (sequence, key head) as one
+constexpr int SM_THREADS = 256;
+template <int D>
+__global__ void __launch_bounds__(SM_THREADS)
+shared_merge_kernel(const __grid_constant__ SharedArgs p) {
+    pdl_wait();
+    __shared__ __align__(16) float acc_s[SM_THREADS * 4];
+    __shared__ float2 ml_s[SM_THREADS];
+    const int unit = blockIdx.x, G = p.G;
+    const int4 own = p.own_units[unit];
+    if (own.x < 0) return;
+    int4 pre = make_int4(0, -1, 0, 0);
+    if (own.z) pre = p.prefix_units[unit];
+    // a thread has four dims of a head, and every `lanes`-th part
+    const int size = G * D / 4, lanes = SM_THREADS / size, e = threadIdx.x % size, mine = threadIdx.x / size, hg = 4 * e / D;
+    const int n_own = own.y - own.x + 1, n = n_own + pre.y - pre.x + 1;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float M = -INFINITY, L = 0.f;
+    if (mine < lanes) {
+        for (int k0 = mine; k0 < n; k0 += 4 * lanes) {
+            float4 o[4];
+            float2 ml[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {                                    // four parts asked for at once
+                const int k = k0 + u * lanes;
+                ml[u] = make_float2(-INFINITY, 0.f);
+                o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (k < n_own) {
+                    const float* part = p.own_parts + (size_t)(unit + own.x + k) * shared_part(G, D);
+                    o[u] = __ldcg(reinterpret_cast<const float4*>(part + 4 * e));
+                    ml[u] = __ldcg(reinterpret_cast<const float2*>(part + G * D + 2 * hg));
+                } else if (k < n) {
+                    const size_t at = (size_t)pre.z + (size_t)2 * kSharedRows * (pre.x + k - n_own) + hg;
+                    o[u] = __ldcg(reinterpret_cast<const float4*>(p.rows_o + at * D + 4 * e % D));
+                    ml[u] = __ldcg(p.rows_ml + at);
+                }
+            }
+            const float Mn = fmaxf(fmaxf(M, ml[0].x), fmaxf(ml[1].x, fmaxf(ml[2].x, ml[3].x)));
+            const float keep = M == -INFINITY ? 0.f : exp2f(M - Mn);
+            L *= keep;
+            acc.x *= keep, acc.y *= keep, acc.z *= keep, acc.w *= keep;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const float z = ml[u].x == -INFINITY ? 0.f : exp2f(ml[u].x - Mn);
+                L = fmaf(ml[u].y, z, L);
+                acc = fma_f4(o[u], make_float4(z, z, z, z), acc);
+            }
+            M = Mn;
+        }
+        *reinterpret_cast<float4*>(acc_s + 4 * threadIdx.x) = acc;
+        ml_s[threadIdx.x] = make_float2(M, L);
+    }
+    __syncthreads();
+    if (mine) return;
+    for (int x = 1; x < lanes; ++x) M = fmaxf(M, ml_s[x * size + e].x);
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    L = 0.f;
+    for (int x = 0; x < lanes; ++x) {
+        const float2 ml = ml_s[x * size + e];
+        const float z = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
+        L = fmaf(ml.y, z, L);
+        acc = fma_f4(*reinterpret_cast<const float4*>(acc_s + 4 * (x * size + e)), make_float4(z, z, z, z), acc);
+    }
+    const float r = L == 0.f ? 0.f : 1.f / L;                                // a query without a visible key: zeros
+    const float v[4] = {acc.x * r, acc.y * r, acc.z * r, acc.w * r};
+    const size_t at = ((size_t)(unit / p.nkv) * p.nq + (size_t)(unit % p.nkv) * G) * D + 4 * e;
+    const uint2 hi = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+    *reinterpret_cast<uint2*>(p.out + at) = hi;
+    if (p.out_lo)
+        *reinterpret_cast<uint2*>(p.out_lo + at) = make_uint2(pack_bf16(v[0] - bf16_lo(hi.x), v[1] - bf16_hi(hi.x)), pack_bf16(v[2] - bf16_lo(hi.y), v[3] - bf16_hi(hi.y)));
+}
+
+// ------------------------------------------------------------------ host
+struct SharedLayout { size_t own_units, prefix_units, own_parts, rows_o, rows_ml, bytes; };
+static SharedLayout shared_layout(int B, int n_groups, int nq, int nkv, int d) {
+    const size_t sms = device_sms(), rows = (size_t)B * nq + 2 * kSharedRows * sms, units = (size_t)B * nkv;
+    SharedLayout l;
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += (bytes + 63) / 64 * 64;
+        return here;
+    };
+    l.own_units = take(units * sizeof(int4));
+    l.prefix_units = take(n_groups ? units * sizeof(int4) : 0);
+    l.own_parts = take((units + 4 * sms) * shared_part(nq / nkv, d) * 4);
+    l.rows_o = take(n_groups ? rows * d * 4 : 0);
+    l.rows_ml = take(n_groups ? rows * 8 : 0);
+    l.bytes = at;
+    return l;
+}
+
+template <int D>
+static int launch_shared(SharedArgs& p, cudaStream_t st) {
+    using C = Shared<D>;
+    static PerDeviceFlag attr_set;
+    if (!attr_set.done()) {
+        FT_CHECK_CUDA(cudaFuncSetAttribute(shared_attn_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        cudaFuncAttributes a;
+        FT_CHECK_CUDA(cudaFuncGetAttributes(&a, shared_attn_kernel<D>));
+        FT_REQUIRE(a.numRegs >= SH_REGS, "ft_attn_decode_shared: built with %d registers a thread, its warps share out %d", a.numRegs, SH_REGS);
+        attr_set.mark();
+    }
+    p.chunk = C::CHUNK;
+    FT_CHECK_CUDA(launch_after(shared_attn_kernel<D>, dim3(device_sms()), dim3(SH_THREADS), C::SMEM, st, (const SharedArgs&)p));
+    FT_CHECK_CUDA(launch_after(shared_merge_kernel<D>, dim3(p.B * p.nkv), dim3(SM_THREADS), 0, st, (const SharedArgs&)p));
+    return 0;
+}
+
+}  // namespace ft
+
+extern "C" long long ft_attn_decode_shared_scratch_bytes(int B, int n_groups, int nq, int nkv, int d) {
+    FT_REQUIRE(d == 64 || d == 128, "ft_attn_decode_shared_scratch_bytes: head_dim %d not supported (64 or 128)", d);
+    FT_REQUIRE(nq >= 1 && nkv >= 1 && nq % nkv == 0 && nq / nkv <= ft::kSharedGroup, "ft_attn_decode_shared_scratch_bytes: GQA group %d/%d not supported", nq, nkv);
+    FT_REQUIRE(B >= 0 && n_groups >= 0 && (double)B * nq * d <= INT32_MAX, "ft_attn_decode_shared_scratch_bytes: bad sizes B=%d nq=%d groups=%d", B, nq, n_groups);
+    return (long long)ft::shared_layout(B, n_groups, nq, nkv, d).bytes;
+}
+
+extern "C" int ft_attn_shared_waits(void) {
+    int n = 0;
+    FT_CHECK_CUDA(cudaDeviceSynchronize());                                  // the copy below waits for the default stream only
+    FT_CHECK_CUDA(cudaMemcpyFromSymbol(&n, ft::g_shared_waits, sizeof(n)));
+    return n;
+}
+
+extern "C" int ft_attn_decode_shared(const void* q, const void* kv_layer, int num_pages, const int* page_table, int table_rows, int max_pages, const int* req_slot,
+                                     const int* ctx_lens, const int* group_start, const int* shared_lens, int n_groups, void* out, void* out_lo, void* scratch, int B, int nq,
+                                     int nkv, int d, void* stream) {
+    using namespace ft;
+    FT_REQUIRE(d == 64 || d == 128, "ft_attn_decode_shared: head_dim %d not supported (64 or 128)", d);
+    FT_REQUIRE(nq >= 1 && nkv >= 1 && nq % nkv == 0 && nq / nkv <= kSharedGroup, "ft_attn_decode_shared: GQA group %d/%d not supported", nq, nkv);
+    const int G = nq / nkv, th = kSharedRows / G;
+    FT_REQUIRE(B >= 0 && n_groups >= 0 && num_pages >= 0 && table_rows >= 0 && max_pages >= 0 && max_pages < INT32_MAX / kKvTile && (double)B * nq * d <= INT32_MAX,
+               "ft_attn_decode_shared: bad sizes B=%d nq=%d groups=%d table %d x %d, %d pages", B, nq, n_groups, table_rows, max_pages, num_pages);
+    // both lists: at most so many units of at most so many steps, and what the shares are rounded up by
+    FT_REQUIRE(((double)B + 1) * nkv * (4.0 * max_pages + 4) + 65536 <= INT32_MAX && ((double)B / (2 * th) + n_groups) * nkv * (max_pages + kSharedStart + 1.0) + 65536 <= INT32_MAX,
+               "ft_attn_decode_shared: %d sequences of %d pages in %d groups are more than one call takes", B, max_pages, n_groups);
+    if (B == 0) return 0;
+    FT_REQUIRE(q && ctx_lens && out && scratch && (n_groups == 0 || (group_start && shared_lens)) && (page_table || table_rows == 0 || max_pages == 0) && (kv_layer || num_pages == 0),
+               "ft_attn_decode_shared: null argument");
+    FT_REQUIRE(((uintptr_t)q | (uintptr_t)kv_layer | (uintptr_t)out | (uintptr_t)out_lo | (uintptr_t)scratch) % 16 == 0, "ft_attn_decode_shared: tensors on 16 bytes");
+    const SharedLayout l = shared_layout(B, n_groups, nq, nkv, d);
+    uint8_t* w = (uint8_t*)scratch;
+    SharedArgs p{(const __half*)q, (const uint8_t*)kv_layer, page_table, req_slot, ctx_lens, group_start, shared_lens, (__nv_bfloat16*)out, (__nv_bfloat16*)out_lo,
+                 (int4*)(w + l.own_units), (int4*)(w + l.prefix_units), (float*)(w + l.own_parts), (float*)(w + l.rows_o), (float2*)(w + l.rows_ml), B, n_groups, num_pages, table_rows,
+                 max_pages, nq, nkv, G, th, 0, kSharedLog2E / sqrtf((float)d)};
+    return d == 64 ? launch_shared<64>(p, (cudaStream_t)stream) : launch_shared<128>(p, (cudaStream_t)stream);
+}

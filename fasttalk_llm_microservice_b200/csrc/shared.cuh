@@ -1,10 +1,11 @@
-// Attention of one query token per sequence where groups of sequences have their first tokens in common: what its kernels share.
+// Attention of one query token per sequence where groups of sequences have their first tokens in common: the two lists of work that its kernel (shared.cu) walks.
 //
 // Group g's queries are group_start[g] .. group_start[g + 1] - 1; each sees min(shared, ctx) keys on the pages of the group's first query's row of the page table and
 // the rest of its ctx keys on its own.  Two kinds of work come of that:
-//   shared part   a unit = one group, key head and tile of queries, all pages of the prefix (shared_prefix.cu, tcgen05): keys are read once for all of them;
-//   own part      a unit = one sequence and key head, its own pages (shared_decode.cu); whoever ends it adds the shared part's results and writes the output.
-// A group that does not pay (SharedPlan) has no shared part: its sequences read the first row's pages themselves, as steps ahead of their own.
+//   prefix   a unit = one group, key head and tile of queries; its steps are the pages of the prefix, read once for all queries of the tile
+//   own      a unit = one sequence and key head; its steps are chunks of its own pages
+// A group that does not pay has no prefix units: its sequences read the first row's pages themselves, as steps ahead of their own.  Both lists are cut into equal
+// shares, the prefix list one for each SM, the own list one for each warp that walks it.  Plain arithmetic, the same on the host.
 #pragma once
 #include "common.cuh"
 
@@ -12,48 +13,184 @@ namespace ft {
 
 constexpr int kSharedGroup = 8;                  // query heads a key head at most
 constexpr int kSharedRows = 128;                 // rows (query, head of the group) of a half of a tile
-constexpr float kSharedLog2E = 1.4426950408889634f;
-// Probabilities are formed 2^6 times their size, so that fp16's normal numbers reach down to 2^-20 of the largest; a running maximum may lag by 2^8
-constexpr float kSharedTop = 6.f, kSharedGrow = 8.f;
-constexpr int kSharedStart = 3;                  // what a unit of the shared part costs beyond its pages, in pages: it takes that much more of the list, behind its last step
-
-// one sequence.  Steps: `lead` tiles of the first row's pages, then its own from token `begin` on, and one if there are none of either
-struct SharedSeq { int ctx, begin, lead, group, row_lead, row_own, first, steps; };      // group: whose shared part it takes, or -1; first: steps of the sequences ahead
-// one group's shared part.  base: where it begins in the list of steps; pages 0: none
-struct SharedGroup { int base, seq0, size, tokens, pages, row, pad0, pad1; };
-
-struct SharedHead {                              // of the plan
-    int own_total, own_per, own_whole, prefix_total, prefix_per;
-};
+constexpr int kSharedStart = 3;                  // what a prefix unit costs beyond its pages, in pages: it takes that much more of the list, behind its last step
 
 struct SharedArgs {
     const __half* q;
     const uint8_t* cache;
     const int *page_table, *req_slot, *ctx_lens, *group_start, *shared_lens;
     __nv_bfloat16 *out, *out_lo;
-    SharedHead* head;
-    SharedSeq* seqs;
-    SharedGroup* groups;
-    int *own_from, *prefix_from;                 // where each CTA begins: a sequence, a group
-    int* counters;
-    float *own_parts, *rows_o;
-    float2* rows_ml;                             // prefix results: O [row + 256 CTA][D], (m, l)
+    int4 *own_units, *prefix_units;              // [B][nkv]: first and last warp that has a part, whether there is a prefix part (below 0: the output is written);
+                                                 //           first and last CTA that has a part, its row among the results
+    float* own_parts;                            // [unit + warp][G][D], then (m, l)
+    float* rows_o;                               // prefix results: O [row + 256 CTA][D], (m, l)
+    float2* rows_ml;
     int B, n_groups, num_pages, table_rows, max_pages, nq, nkv, G, th;        // th: queries of a half
-    int own_ctas, prefix_ctas;
+    int chunk;                                   // tokens of an own step: 64 or 32
     float scale_log2;
+
+    __host__ __device__ __forceinline__ int reach() const { return max_pages * kKvTile; }
+    __host__ __device__ __forceinline__ int row_of(int b) const {
+        const int slot = req_slot ? req_slot[b] : b;
+        return slot >= 0 && slot < table_rows ? slot : -1;
+    }
+    __host__ __device__ __forceinline__ int shared_of(int g) const { return max(0, min(shared_lens[g], reach())); }
 };
 
-// steps of a tile of `tokens` queries over `pages` pages: where they fill one half only, each half takes every other page
-__host__ __device__ __forceinline__ int shared_steps(int tokens, int th, int pages) { return tokens <= th ? (pages + 1) / 2 : pages; }
-// of all tiles of one key head
-__host__ __device__ __forceinline__ int shared_head_steps(int size, int th, int pages) {
-    const int tiles = (size + 2 * th - 1) / (2 * th);
-    return (tiles - 1) * (pages + kSharedStart) + shared_steps(size - (tiles - 1) * 2 * th, th, pages) + kSharedStart;
-}
-// where row 0 of (group, key head, query i of the group) lies among the prefix's results
-__host__ __device__ __forceinline__ size_t shared_row(const SharedGroup& g, int h, int i, int nq, int G) { return (size_t)g.seq0 * nq + ((size_t)h * g.size + i) * G; }
+// A group's prefix part; pages 0: none
+struct SharedPrefix {
+    int seq0, size, tokens, pages, tiles;
+    __host__ __device__ __forceinline__ void load(const SharedArgs& p, int g) {
+        seq0 = p.group_start[g];
+        size = p.group_start[g + 1] - seq0;
+        tokens = p.shared_of(g);
+        pages = size >= 2 && tokens >= 2 * kKvTile ? (tokens + kKvTile - 1) / kKvTile : 0;
+        tiles = (size + 2 * p.th - 1) / (2 * p.th);
+    }
+    __host__ __device__ __forceinline__ int queries(const SharedArgs& p, int tile) const { return min(2 * p.th, size - tile * 2 * p.th); }
+    // steps of a tile of n queries: where they fill one half only, each half takes every other page
+    __host__ __device__ __forceinline__ int steps(const SharedArgs& p, int n) const { return n <= p.th ? (pages + 1) / 2 : pages; }
+    // what all tiles of one key head take of the list
+    __host__ __device__ __forceinline__ int each(const SharedArgs& p) const { return (tiles - 1) * (pages + kSharedStart) + steps(p, queries(p, tiles - 1)) + kSharedStart; }
+    __host__ __device__ __forceinline__ int all(const SharedArgs& p) const { return pages ? p.nkv * each(p) : 0; }
+    // where row 0 of (key head, query i of the group) lies among the results
+    __host__ __device__ __forceinline__ int row(const SharedArgs& p, int h, int i) const { return seq0 * p.nq + (h * size + i) * p.G; }
+};
 
-int launch_shared_prefix(const SharedArgs& p, int d, cudaStream_t st);
-int shared_prefix_waits(int* out);
+// A sequence: `lead` chunks of the first row's pages, then its own from token `begin` on, and one step if there are none of either
+struct SharedSeq {
+    int ctx, begin, lead, steps, first;          // first: the query whose row has the shared pages
+    bool prefix;                                 // a prefix part is added
+    // g: the group that b may belong to (below 0: none)
+    __host__ __device__ __forceinline__ void load(const SharedArgs& p, int b, int g, int ctx_len) {
+        ctx = max(0, min(ctx_len, p.reach()));
+        begin = lead = 0;
+        first = -1;
+        prefix = false;
+        if (g >= 0 && p.group_start[g] <= b && b < p.group_start[g + 1]) {
+            SharedPrefix w;
+            w.load(p, g);
+            begin = w.tokens;
+            first = w.seq0;
+            prefix = w.pages > 0 && ctx >= begin;
+            if (!prefix) lead = (min(begin, ctx) + p.chunk - 1) / p.chunk;
+        }
+        const int own = ctx > begin ? (ctx + p.chunk - 1) / p.chunk - begin / p.chunk : 0;
+        steps = max(1, lead + own);
+    }
+};
+
+// the last group that begins at or before b (those without queries begin where the next one does), or -1
+__host__ __device__ __forceinline__ int shared_group_of(const int* group_start, int n, int b) {
+    int lo = -1, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (group_start[mid] <= b) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+// A CTA's share of the prefix list, walked stretch by stretch; a stretch = pages p0 .. p0 + pages - 1 of one unit
+struct PrefixWalk {
+    SharedPrefix w;
+    int f, f_end, unit_f, g, h, tile, t;
+    int n, steps;                                // queries and steps of the tile
+    int p0, pages;
+    bool few;                                    // the queries fill one half only
+    __host__ __device__ __forceinline__ void unit(const SharedArgs& p) {
+        n = w.queries(p, tile);
+        few = n <= p.th;
+        steps = w.steps(p, n);
+    }
+    // the share begins at f, in group g, which begins at base
+    __host__ __device__ __forceinline__ void start(const SharedArgs& p, int f_, int f_end_, int g_, int base) {
+        f = f_;
+        f_end = f_end_;
+        if (f >= f_end) return;
+        g = g_;
+        w.load(p, g);
+        const int each = w.each(p), full = w.pages + kSharedStart;
+        int rest = f - base;
+        h = (int)((unsigned)rest / (unsigned)each);
+        rest -= h * each;
+        tile = min((int)((unsigned)rest / (unsigned)full), w.tiles - 1);
+        t = rest - tile * full;
+        unit(p);
+    }
+    __host__ __device__ __forceinline__ bool next(const SharedArgs& p) {
+#pragma unroll 1
+        for (;;) {
+            if (f >= f_end) return false;
+            if (t >= steps + kSharedStart) {
+                t = 0;
+                if (++tile == w.tiles) {
+                    tile = 0;
+                    if (++h == p.nkv) {
+                        h = 0;
+#pragma unroll 1
+                        do w.load(p, ++g);
+                        while (w.pages == 0);
+                    }
+                }
+                unit(p);
+            }
+            const int take = min(f_end - f, steps + kSharedStart - t), t0 = min(t, steps), t1 = min(t + take, steps);
+            unit_f = f - t;
+            t += take;
+            f += take;
+            if (t1 > t0) {
+                p0 = few ? 2 * t0 : t0;
+                pages = (few ? min(2 * t1, w.pages) : t1) - p0;
+                return true;
+            }                                    // else all of it was behind the unit's last step
+        }
+    }
+    __host__ __device__ __forceinline__ int of_half(int half) const { return few ? (pages - half + 1) / 2 : pages; }      // its pages
+};
+
+// A warp's share of the own list, walked stretch by stretch; a stretch = steps t0 .. t1 - 1 of one unit
+struct OwnWalk {
+    SharedSeq s;
+    int f, f_end, unit_f, b, g, h, t, t0, t1;
+    // the share begins at f, in sequence b, whose units begin at base; groups: how many there are
+    __host__ __device__ __forceinline__ void start(const SharedArgs& p, int groups, int f_, int f_end_, int b_, int base) {
+        f = f_;
+        f_end = f_end_;
+        if (f >= f_end) return;
+        b = b_;
+        g = shared_group_of(p.group_start, groups, b);
+        s.load(p, b, g, p.ctx_lens[b]);
+        const int rest = f - base;
+        h = (int)((unsigned)rest / (unsigned)s.steps);
+        t = rest - h * s.steps;
+    }
+    __host__ __device__ __forceinline__ bool next(const SharedArgs& p, int groups) {
+        if (f >= f_end) return false;
+        if (t >= s.steps) {
+            t = 0;
+            if (++h == p.nkv) {
+                h = 0;
+                ++b;
+                while (g + 1 < groups && p.group_start[g + 1] <= b) ++g;
+                s.load(p, b, g, p.ctx_lens[b]);
+            }
+        }
+        const int take = min(f_end - f, s.steps - t);
+        unit_f = f - t;
+        t0 = t;
+        t1 = t + take;
+        t = t1;
+        f += take;
+        return true;
+    }
+    // tokens lo .. hi - 1 of the sequence that step x reads, on the pages of query `row`'s row (none: lo >= hi)
+    __host__ __device__ __forceinline__ void step(const SharedArgs& p, int x, int& lo, int& hi, int& row) const {
+        const bool led = x < s.lead;
+        const int tile = led ? x : s.begin / p.chunk + x - s.lead;
+        lo = max(tile * p.chunk, led ? 0 : s.begin);
+        hi = min(tile * p.chunk + p.chunk, led ? min(s.begin, s.ctx) : s.ctx);
+        row = led ? s.first : b;
+    }
+};
 
 }  // namespace ft

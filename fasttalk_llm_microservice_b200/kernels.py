@@ -537,10 +537,10 @@ def attn_decode_shared(q: torch.Tensor, kv_layer: torch.Tensor, page_table: torc
         req_slot = _kv8_ints(req_slot, index, what, B, "req_slot")
     out = torch.empty(B, nq * d, device=index, dtype=torch.bfloat16)
     lo = torch.empty_like(out) if planes == 2 else None
-    size = _kv8_sizes.get((index, B, n, nq, d))
+    size = _kv8_sizes.get((index, B, n, nq, nkv, d))
     if size is None:
         with torch.cuda.device(index):
-            size = _kv8_sizes[index, B, n, nq, d] = N.check(N.load().ft_attn_decode_shared_scratch_bytes(B, n, nq, d), "ft_attn_decode_shared_scratch_bytes")
+            size = _kv8_sizes[index, B, n, nq, nkv, d] = N.check(N.load().ft_attn_decode_shared_scratch_bytes(B, n, nq, nkv, d), "ft_attn_decode_shared_scratch_bytes")
     scratch = torch.empty(size, device=index, dtype=torch.uint8)
     _kv8_call(index, "ft_attn_decode_shared", q.data_ptr(), kv_layer.data_ptr(), pages, page_table.data_ptr(), rows, most, 0 if req_slot is None else req_slot.data_ptr(),
               ctx_lens.data_ptr(), group_start.data_ptr(), shared_lens.data_ptr(), n, out.data_ptr(), 0 if lo is None else lo.data_ptr(), scratch.data_ptr(), B, nq, nkv, d)

@@ -135,7 +135,7 @@ SIGNATURES = {
     "ft_attn_prefill_kv8": (_I, [_VP, _VP, _I, _VP, _I, _I, _VP, _VP, _VP, _I, _I, _VP, _VP, _VP, _I, _I, _I, _VP]),
     "ft_step_lists": (_I, [_VP, _VP, _VP, _I, _VP, _I, _I, _VP, _I, _VP, _I, _VP, _VP, _VP, _VP, _VP, _VP, _VP]),
     "ft_norm_rope_kv_append": (_I, [_VP, _I, _I, _LL, _LL, _VP, _VP, _I, _I, _I, _VP, _I, _VP, _I, _F, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _VP]),
-    "ft_attn_decode_shared_scratch_bytes": (_LL, [_I, _I, _I, _I]),
+    "ft_attn_decode_shared_scratch_bytes": (_LL, [_I, _I, _I, _I, _I]),
     "ft_attn_decode_shared": (_I, [_VP, _VP, _I, _VP, _I, _I, _VP, _VP, _VP, _VP, _I, _VP, _VP, _VP, _I, _I, _I, _I, _VP]),
     "ft_attn_shared_waits": (_I, []),
     "ft_sample": (_I, [_VP, _I, _I, _VP, _VP, _VP, _VP, _VP, _VP]),

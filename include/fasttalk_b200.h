@@ -735,7 +735,7 @@ int ft_norm_rope_kv_append(const void* qkv, int type, int n_parts, long long par
  * scratch: work memory of ft_attn_decode_shared_scratch_bytes bytes (of the current device), in any state, not shared by calls that may overlap.
  * ft_attn_shared_waits: 1 if a wait inside one of its kernels has run out on the current device since the library was loaded (rows of some call mean nothing), else 0;
  * waits for all that the device has been given, on every stream. */
-long long ft_attn_decode_shared_scratch_bytes(int B, int n_groups, int nq, int d);
+long long ft_attn_decode_shared_scratch_bytes(int B, int n_groups, int nq, int nkv, int d);
 int ft_attn_decode_shared(const void* q, const void* kv_layer, int num_pages, const int* page_table, int table_rows, int max_pages, const int* req_slot,
                           const int* ctx_lens, const int* group_start, const int* shared_lens, int n_groups, void* out, void* out_lo, void* scratch, int B, int nq,
                           int nkv, int d, void* stream);

@@ -1,0 +1,88 @@
+// The lists of work of attention over shared prefixes on the host: every CTA's and warp's share, walked with the kernel's own arithmetic (csrc/shared.cuh).
+#include <cstring>
+
+#include "shared.cuh"
+
+using namespace ft;
+
+// own: stretches of all warps, nine numbers each: warp, sequence, head, t0, t1, steps, prefix, first and last warp of the unit.
+// else: of all CTAs: cta, group, head, tile, p0, pages, few, first and last CTA of the unit.  -> how many (at most `room` are written), or -1 - share where one is longer than `limit`
+extern "C" int shared_stretches(int own, const int* ctx_lens, int B, const int* starts, const int* shared, int n_groups, int max_pages, int nkv, int G, int chunk, int shares,
+                                int unset, int limit, int* out, int room) {
+    SharedArgs p{};
+    p.ctx_lens = ctx_lens, p.group_start = starts, p.shared_lens = shared;
+    p.B = B, p.n_groups = n_groups, p.max_pages = max_pages, p.table_rows = B, p.nkv = nkv, p.nq = nkv * G, p.G = G, p.th = kSharedRows / G, p.chunk = chunk;
+    bool grows = true;
+    for (int g = 0; g < n_groups; ++g) grows = grows && starts[g] >= 0 && starts[g] <= starts[g + 1] && starts[g + 1] <= B;
+    const int groups = grows ? n_groups : 0;
+    int total = 0, found = 0;
+    for (int g = 0; !own && g < groups; ++g) {
+        SharedPrefix w;
+        w.load(p, g);
+        total += w.all(p);
+    }
+    for (int b = 0; own && b < B; ++b) {
+        SharedSeq s;
+        s.load(p, b, shared_group_of(starts, groups, b), ctx_lens[b]);
+        total += s.steps * nkv;
+    }
+    const int per = (int)((unsigned)(total + shares - 1) / (unsigned)shares);
+    auto tell = [&](const int* row) {
+        if (found < room) memcpy(out + 9 * found, row, 9 * sizeof(int));
+        ++found;
+    };
+    for (int x = 0; x < shares; ++x) {
+        const int f = min(per * x, total), end = min(f + per, total);
+        int base = 0, at = 0;
+        if (own) {
+            SharedSeq s;
+            for (; f < end; base += s.steps * nkv, ++at) {
+                s.load(p, at, shared_group_of(starts, groups, at), ctx_lens[at]);
+                if (f < base + s.steps * nkv) break;
+            }
+            OwnWalk w;
+            memset((void*)&w, unset, sizeof(w));
+            w.start(p, groups, f, end, at, base);
+            for (int n = 0; w.next(p, groups); ++n) {
+                if (n == limit) return -1 - x;
+                const int row[9] = {x, w.b, w.h, w.t0, w.t1, w.s.steps, w.s.prefix, w.unit_f / per, (w.unit_f + w.s.steps - 1) / per};
+                tell(row);
+            }
+        } else {
+            SharedPrefix s;
+            for (; f < end; base += s.all(p), ++at) {
+                s.load(p, at);
+                if (f < base + s.all(p)) break;
+            }
+            PrefixWalk w;
+            memset((void*)&w, unset, sizeof(w));
+            w.start(p, f, end, at, base);
+            for (int n = 0; w.next(p); ++n) {
+                if (n == limit) return -1 - x;
+                const int row[9] = {x, w.g, w.h, w.tile, w.p0, w.pages, w.few, w.unit_f / per, (w.unit_f + w.steps - 1) / per};
+                tell(row);
+            }
+        }
+    }
+    return found;
+}
+
+// What step x of a sequence reads: lo, hi, query
+extern "C" void shared_step(const int* ctx_lens, int B, int b, const int* starts, const int* shared, int n_groups, int max_pages, int chunk, int x, int* out) {
+    SharedArgs p{};
+    p.ctx_lens = ctx_lens, p.group_start = starts, p.shared_lens = shared;
+    p.B = B, p.n_groups = n_groups, p.max_pages = max_pages, p.nkv = 1, p.nq = 1, p.G = 1, p.th = kSharedRows, p.chunk = chunk;
+    OwnWalk w;
+    w.b = b;
+    w.s.load(p, b, shared_group_of(starts, n_groups, b), ctx_lens[b]);
+    w.step(p, x, out[0], out[1], out[2]);
+}
+
+// Where row 0 of (group, head, query i of the group) lies among the prefix's results
+extern "C" int shared_row(const int* starts, const int* shared, int g, int h, int i, int max_pages, int nkv, int G) {
+    SharedArgs p{};
+    p.group_start = starts, p.shared_lens = shared, p.max_pages = max_pages, p.nkv = nkv, p.nq = nkv * G, p.G = G, p.th = kSharedRows / G;
+    SharedPrefix w;
+    w.load(p, g);
+    return w.row(p, h, i);
+}

@@ -68,9 +68,10 @@ def test_refusals_of_attention(lib):
     for bad in (dict(q=P + 8), dict(cache=P + 2), dict(out=P + 8), dict(lo=P + 4), dict(scratch=P + 4)):
         refused(call(**bad), "16 bytes")
     assert call(B=0, q=0) == 0
-    refused(lib.ft_attn_decode_shared_scratch_bytes(1, 1, 4, 32), "head_dim 32")
-    for B, n, nq in ((-1, 1, 4), (1, -1, 4), (1, 1, 0), (1 << 24, 1, 4)):
-        refused(lib.ft_attn_decode_shared_scratch_bytes(B, n, nq, 64), "bad sizes")
+    refused(lib.ft_attn_decode_shared_scratch_bytes(1, 1, 4, 1, 32), "head_dim 32")
+    refused(lib.ft_attn_decode_shared_scratch_bytes(1, 1, 0, 1, 64), "GQA group")
+    for B, n, nq in ((-1, 1, 4), (1, -1, 4), (1 << 24, 1, 4)):
+        refused(lib.ft_attn_decode_shared_scratch_bytes(B, n, nq, 1, 64), "bad sizes")
 
 
 def test_refusals_of_tensors():

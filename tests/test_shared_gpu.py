@@ -547,6 +547,21 @@ def test_two_calls_at_once_and_other_streams(K):
         close(gb, *wb, 1)
 
 
+@pytest.mark.parametrize("nq,nkv,d,sizes,shared,own", [(12, 4, 128, [8, 9, 6, 7, 7], [4099, 2500, 3300, 1640, 2880], 500), (32, 8, 128, [24], [16001], 200), (32, 8, 64, [20, 44], [6000, 900], 300),
+                                                     (16, 4, 128, [64, 60], [1500, 800], 80)])
+def test_many_calls_behind_one_another(K, nq, nkv, d, sizes, shared, own):
+    """Pages that land late, as they do beside other copies and calls, are waited for: every call says the same."""
+    s = make(30, nq, nkv, d, sizes, shared, [i * 97 % own for i in range(sum(sizes))], hidden=0.5)
+    run = lambda: K.attn_decode_shared(s["q"], s["cache"], s["table"], s["ctx"], s["starts"], s["shared"], s["slots"])
+    first = check(K, s)
+    for _ in range(20):
+        outs = [run() for _ in range(15)]
+        torch.cuda.synchronize()
+        for hi, lo in outs:
+            assert torch.equal(hi, first[0]) and torch.equal(lo, first[1])
+    K.attn_shared_check()
+
+
 def test_captured_and_replayed(K):
     s = make(12, 8, 2, 64, [5, 4], [500, 900], [10, 70, 0, 130, 5, 6, 64, 1, 300], hidden=0.25)
     run = lambda: K.attn_decode_shared(s["q"], s["cache"], s["table"], s["ctx"], s["starts"], s["shared"], s["slots"])
