@@ -653,9 +653,9 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
                     }
                 }
                 if (valid) {
-                    float4* to = reinterpret_cast<float4*>(p.rows_o + at * D + 16 * c);
+                    float4* to = reinterpret_cast<float4*>(p.rows_o) + (size_t)(4 * c) * p.rows + at;       // a warp's lanes side by side
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) to[k] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
+                    for (int k = 0; k < 4; ++k) to[(size_t)k * p.rows] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
                 }
             }
             if (valid && (!w.few || h == 0)) p.rows_ml[at] = make_float2(m, l);
@@ -698,8 +698,8 @@ shared_merge_kernel(const __grid_constant__ SharedArgs p) {
     if (own.x < 0) return;
     int4 pre = make_int4(0, -1, 0, 0);
     if (own.z) pre = p.prefix_units[unit];
-    // a thread has four dims of a head, and every `lanes`-th part
-    const int size = G * D / 4, lanes = SM_THREADS / size, e = threadIdx.x % size, mine = threadIdx.x / size, hg = 4 * e / D;
+    // a thread has four dims of a head (neighbours the same of neighbouring heads, as the prefix's results lie), and every `lanes`-th part
+    const int size = G * D / 4, lanes = SM_THREADS / size, e = threadIdx.x % size, mine = threadIdx.x / size, hg = e % G, dim = e / G * 4;
     const int n_own = own.y - own.x + 1, n = n_own + pre.y - pre.x + 1;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float M = -INFINITY, L = 0.f;
@@ -714,11 +714,11 @@ shared_merge_kernel(const __grid_constant__ SharedArgs p) {
                 o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (k < n_own) {
                     const float* part = p.own_parts + (size_t)(unit + own.x + k) * shared_part(G, D);
-                    o[u] = __ldcg(reinterpret_cast<const float4*>(part + 4 * e));
+                    o[u] = __ldcg(reinterpret_cast<const float4*>(part + hg * D + dim));
                     ml[u] = __ldcg(reinterpret_cast<const float2*>(part + G * D + 2 * hg));
                 } else if (k < n) {
                     const size_t at = (size_t)pre.z + (size_t)2 * kSharedRows * (pre.x + k - n_own) + hg;
-                    o[u] = __ldcg(reinterpret_cast<const float4*>(p.rows_o + at * D + 4 * e % D));
+                    o[u] = __ldcg(reinterpret_cast<const float4*>(p.rows_o) + (size_t)(dim / 4) * p.rows + at);
                     ml[u] = __ldcg(p.rows_ml + at);
                 }
             }
@@ -750,7 +750,7 @@ shared_merge_kernel(const __grid_constant__ SharedArgs p) {
     }
     const float r = L == 0.f ? 0.f : 1.f / L;                                // a query without a visible key: zeros
     const float v[4] = {acc.x * r, acc.y * r, acc.z * r, acc.w * r};
-    const size_t at = ((size_t)(unit / p.nkv) * p.nq + (size_t)(unit % p.nkv) * G) * D + 4 * e;
+    const size_t at = ((size_t)(unit / p.nkv) * p.nq + (size_t)(unit % p.nkv) * G + hg) * D + dim;
     const uint2 hi = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
     *reinterpret_cast<uint2*>(p.out + at) = hi;
     if (p.out_lo)
@@ -758,10 +758,11 @@ shared_merge_kernel(const __grid_constant__ SharedArgs p) {
 }
 
 // ------------------------------------------------------------------ host
-struct SharedLayout { size_t own_units, prefix_units, own_parts, rows_o, rows_ml, bytes; };
+struct SharedLayout { size_t own_units, prefix_units, own_parts, rows_o, rows_ml, rows, bytes; };
 static SharedLayout shared_layout(int B, int n_groups, int nq, int nkv, int d) {
     const size_t sms = device_sms(), rows = (size_t)B * nq + 2 * kSharedRows * sms, units = (size_t)B * nkv;
     SharedLayout l;
+    l.rows = rows;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
@@ -830,6 +831,6 @@ extern "C" int ft_attn_decode_shared(const void* q, const void* kv_layer, int nu
     uint8_t* w = (uint8_t*)scratch;
     SharedArgs p{(const __half*)q, (const uint8_t*)kv_layer, page_table, req_slot, ctx_lens, group_start, shared_lens, (__nv_bfloat16*)out, (__nv_bfloat16*)out_lo,
                  (int4*)(w + l.own_units), (int4*)(w + l.prefix_units), (float*)(w + l.own_parts), (float*)(w + l.rows_o), (float2*)(w + l.rows_ml), B, n_groups, num_pages, table_rows,
-                 max_pages, nq, nkv, G, th, 0, kSharedLog2E / sqrtf((float)d)};
+                 max_pages, nq, nkv, G, th, (int)l.rows, 0, kSharedLog2E / sqrtf((float)d)};
     return d == 64 ? launch_shared<64>(p, (cudaStream_t)stream) : launch_shared<128>(p, (cudaStream_t)stream);
 }

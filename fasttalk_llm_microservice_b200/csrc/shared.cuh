@@ -23,9 +23,10 @@ struct SharedArgs {
     int4 *own_units, *prefix_units;              // [B][nkv]: first and last warp that has a part, whether there is a prefix part (below 0: the output is written);
                                                  //           first and last CTA that has a part, its row among the results
     float* own_parts;                            // [unit + warp][G][D], then (m, l)
-    float* rows_o;                               // prefix results: O [row + 256 CTA][D], (m, l)
+    float* rows_o;                               // prefix results: O [D / 4][row + 256 CTA][4], (m, l)
     float2* rows_ml;
     int B, n_groups, num_pages, table_rows, max_pages, nq, nkv, G, th;        // th: queries of a half
+    int rows;                                    // of the prefix's results
     int chunk;                                   // tokens of an own step: 64 or 32
     float scale_log2;
 
