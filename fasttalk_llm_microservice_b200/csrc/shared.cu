@@ -22,9 +22,10 @@ constexpr float kSharedTop = 6.f, kSharedGrow = 8.f;
 
 // Groups of four warps: warp 0 copies the prefix's pages, 1 and 2 issue the halves' products, 3 owns tensor memory; 4 .. 11 softmax (half = (warp - 4) / 4); 12 .. 15 own
 constexpr int SH_THREADS = 512, SH_WARPS = SH_THREADS / 32;
-constexpr int SH_REGS = 128, SH_REGS_ISSUE = 64, SH_REGS_SOFT = 152, SH_REGS_OWN = 144;
+constexpr int SH_REGS = 128, SH_REGS_ISSUE = 88, SH_REGS_SOFT = 144, SH_REGS_OWN = 136;
 static_assert(SH_REGS_ISSUE + 2 * SH_REGS_SOFT + SH_REGS_OWN <= 4 * SH_REGS, "what the block is launched with");
 constexpr int SH_SOFT = 256;
+constexpr int SH_LIST = 128;                     // groups whose lists are kept in shared memory
 constexpr int SH_PIECE = kKvTile * 128;          // [64 tokens][64 dims] in fp16
 
 __device__ int g_shared_waits;                   // 1: a wait ran out on this device (ft_attn_shared_waits)
@@ -34,7 +35,8 @@ struct Shared {
     static constexpr int KH = D / 64;
     static constexpr int TILE = 2 * KH * SH_PIECE;                           // K | V of a page
     // of the prefix.  Three at least: a half that has every other page asks for its scores two of its own pages ahead, whose stage must not wait for a product behind them
-    static constexpr int STAGES = D == 64 ? 4 : 3;
+    static constexpr int STAGES = D == 64 ? 4 : 3, SLAB = TILE / 2, TOKENS = 16;
+    static constexpr int AHEAD = 2;                                          // pages that keys are copied ahead of values
     static constexpr int QBLK = kSharedRows * 128;                           // [128 rows][64 dims]
     static constexpr int OWN_WARPS = D == 64 ? 4 : 2, OWN_STAGES = 2;
     static constexpr int CHUNK = D == 64 ? 64 : 32;                          // tokens
@@ -43,7 +45,7 @@ struct Shared {
     // tensor memory: scores [half][2][64 columns] (probabilities, pairs of fp16, over the first 32 of them), O [half][D]
     static constexpr int COL_S = 0, COL_O = 256, COLS = 512;
     static_assert(COL_O + 2 * D <= COLS, "tensor memory");
-    static_assert(SMEM <= 232448 - 1536, "shared memory");
+    static_assert(SMEM <= 232448 - 1792, "shared memory");
 };
 
 // floats of an own part: O [G][D], (m, l) of the heads; on 16 bytes
@@ -66,13 +68,6 @@ struct SharedQuery {
         for (int i = 0; i < D / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
         m[0] = m[1] = -INFINITY;
         l[0] = l[1] = 0.f;
-    }
-    __device__ __forceinline__ void load_query(const __half* row, int tq) {  // row: query head g of the group, or null
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-            q[ks][0] = row ? *reinterpret_cast<const uint32_t*>(row + ks * 16 + 2 * tq) : 0u;
-            q[ks][1] = row ? *reinterpret_cast<const uint32_t*>(row + ks * 16 + 8 + 2 * tq) : 0u;
-        }
     }
     // tokens lo .. hi - 1 of the chunk at `tile` (an address in shared memory); its hidden values are zeros
     __device__ __forceinline__ void chunk(uint32_t tile, int lo, int hi, float scale_log2, int lane) {
@@ -150,77 +145,22 @@ struct SharedQuery {
     }
 };
 
+// The share f .. f_end - 1 of the own list; sequence b0 begins at `base` of it, and the share in b0.  Thirty-two steps at a time, a lane each, the warp finds out what they
+// read; then copies run ahead and results are written whichever sequences the steps belong to.
 template <int D>
-__device__ __forceinline__ void shared_own(const SharedArgs& p, OwnWalk w, int groups, int per, int warp, uint8_t* ring, uint64_t* full, volatile int* dead, int* err) {
+__device__ __forceinline__ void shared_own(const SharedArgs& p, const SharedGroups& gr, int f, int f_end, int b0, int base, int per, int warp, uint8_t* ring, uint64_t* full,
+                                           volatile int* dead, int* err) {
     using C = Shared<D>;
     constexpr int S = C::OWN_STAGES, CH = C::CHUNK;
     const int lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3, G = p.G;
     const uint64_t pol = policy_evict_first();                               // every byte is read once
     bool ok = true;
     int it = 0, asked = 0;                                                   // chunks of the share so far, with a page: a stage's phase follows from the count
-    while (w.next(p, groups)) {
-        const int unit = w.b * p.nkv + w.h, n = w.t1 - w.t0;
-        // what each step reads: lane x has step x of the next 32
-        int lo_x, hi_x, page_x, row;
-        auto steps_from = [&](int x0) {
-            w.step(p, x0 + lane, lo_x, hi_x, row);
-            page_x = -1;
-            if (x0 + lane < w.t1 && lo_x < hi_x) {
-                row = p.row_of(row);
-                if (row >= 0) page_x = p.page_table[(size_t)row * p.max_pages + lo_x / kKvTile];
-                if (page_x >= p.num_pages) page_x = -1;
-            }
-        };
-        steps_from(w.t0);
-        // 2 D / 64 pieces of a chunk, a lane each
-        auto copy = [&](int x, int stage) {                                  // x: of the 32
-            const int page = __shfl_sync(0xffffffffu, page_x, x), first = __shfl_sync(0xffffffffu, lo_x, x) / CH * CH % kKvTile;
-            if (page < 0) return;
-            uint8_t* dst = ring + stage * C::CHUNK_BYTES;
-            const uint8_t* src = p.cache + ((size_t)page * p.nkv + w.h) * C::TILE;
-            if (CH == kKvTile) {
-                if (lane == 0) {
-                    mbar_expect_tx(&full[stage], C::CHUNK_BYTES);
-                    tma_bulk_g2s(dst, src, C::CHUNK_BYTES, &full[stage], pol);
-                }
-            } else {
-                if (lane == 0) mbar_expect_tx(&full[stage], C::CHUNK_BYTES);
-                __syncwarp();
-                if (lane < 2 * C::KH) tma_bulk_g2s(dst + lane * (CH * 128), src + lane * SH_PIECE + first * 128, CH * 128, &full[stage], pol);
-            }
-        };
-        SharedQuery<D> a;
-        a.clear();
-        a.load_query(g < G ? p.q + ((size_t)w.b * p.nq + (size_t)w.h * G + g) * D : nullptr, tq);
-        // copies run S chunks ahead
-        for (int x0 = 0; x0 < n; x0 += 32) {
-            if (x0) steps_from(w.t0 + x0);
-            const int here = min(32, n - x0);
-            int next = 0;
-            for (int x = 0; x < here; ++x) {
-                for (; ok && next < here && asked < it + S; ++next)
-                    if (__shfl_sync(0xffffffffu, page_x, next) >= 0) copy(next, asked++ % S);
-                if (!ok) break;
-                if (__shfl_sync(0xffffffffu, page_x, x) < 0) continue;
-                const int stage = it % S;
-                ok = __all_sync(0xffffffffu, mbar_wait_limited(&full[stage], it / S & 1, dead));
-                if (!ok) break;
-                ++it;
-                const int lo = __shfl_sync(0xffffffffu, lo_x, x), hi = __shfl_sync(0xffffffffu, hi_x, x), base = lo / CH * CH;
-                uint8_t* tile = ring + stage * C::CHUNK_BYTES;
-                if (lo > base || hi < base + CH) {                           // hidden values may be anything: 0 * infinity is none
-                    const int ahead = lo - base, hidden = ahead + base + CH - hi;
-                    for (int u = lane; u < hidden * (D / 8); u += 32) {
-                        const int k = u / (D / 8), c = u % (D / 8), tok = k < ahead ? k : hi - base + k - ahead;
-                        *reinterpret_cast<uint4*>(tile + C::HALF + SharedQuery<D>::at(tok, c)) = make_uint4(0u, 0u, 0u, 0u);
-                    }
-                    fence_proxy_async();                                     // ahead of the next copy into this stage
-                    __syncwarp();
-                }
-                a.chunk(smem_u32(tile), lo - base, hi - base, p.scale_log2, lane);
-                __syncwarp();                                                // all lanes have read it: the next copy may come
-            }
-        }
+    SharedQuery<D> a;
+    uint32_t q_next[D / 16][2];
+    int unit = -1, first = 0;                                                // the unit under way, and its first step here
+    // what this warp has of the unit under way, of `steps` steps up to `end`, which begins at from
+    auto finish = [&](int end, int steps, bool prefix, int from) {
         if (!ok) {                                                           // NaN for all that this (sequence, head) says
             *err = 1;
             a.m[0] = a.m[1] = 0.f;
@@ -228,11 +168,8 @@ __device__ __forceinline__ void shared_own(const SharedArgs& p, OwnWalk w, int g
         }
         float sum[2];
         a.total(sum);
-        const bool all = w.t0 == 0 && w.t1 == w.s.steps && !w.s.prefix;
-        if (lane == 0 && w.t0 == 0) {
-            const int last = (int)((unsigned)(w.unit_f + w.s.steps - 1) / (unsigned)per);
-            p.own_units[unit] = all ? make_int4(-1, 0, 0, 0) : make_int4(warp, last, w.s.prefix, 0);
-        }
+        const bool all = first == 0 && end == steps && !prefix;
+        if (lane == 0 && first == 0) p.own_units[unit] = all ? make_int4(-1, 0, 0, 0) : make_int4(warp, (int)((unsigned)(from + steps - 1) / (unsigned)per), prefix, 0);
         float* part = p.own_parts + (size_t)(unit + warp) * shared_part(G, D);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -240,7 +177,7 @@ __device__ __forceinline__ void shared_own(const SharedArgs& p, OwnWalk w, int g
             if (head >= G) continue;
             if (all) {                                                       // a query without a visible key: zeros
                 const float r = sum[e] == 0.f ? 0.f : 1.f / sum[e];
-                const size_t at = ((size_t)w.b * p.nq + (size_t)w.h * G + head) * D;
+                const size_t at = ((size_t)unit * G + head) * D;             // (unit = sequence * key heads + key head)
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i)
 #pragma unroll
@@ -259,7 +196,131 @@ __device__ __forceinline__ void shared_own(const SharedArgs& p, OwnWalk w, int g
                 if (g == 0) *reinterpret_cast<float2*>(part + G * D + 2 * head) = make_float2(a.m[e], sum[e]);
             }
         }
+    };
+    auto query_of = [&](int u, uint32_t (*q)[2]) {
+        const __half* row = p.q + ((size_t)u * G + g) * D + 2 * tq;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            q[ks][0] = g < G ? *reinterpret_cast<const uint32_t*>(row + ks * 16) : 0u;
+            q[ks][1] = g < G ? *reinterpret_cast<const uint32_t*>(row + ks * 16 + 8) : 0u;
+        }
+    };
+    int end_t = 0, end_steps = 0, end_from = 0;                              // of the last step so far
+    bool end_prefix = false;
+#pragma unroll 1
+    for (; f < f_end; f += 32) {
+        // ---- lane x: step f + x.  The next 32 sequences hold 32 steps at least
+        int unit_x, t_x, steps_x, from_x, lo_x, hi_x, page_x = -1;
+        bool prefix_x;
+        {
+            const int b = b0 + lane;
+            SharedSeq s;
+            int row = -1, led_row = -1;
+            s.steps = 0;
+            if (b < p.B) {
+                row = p.row_of(b);
+                s.load(p, gr, b, p.ctx_lens[b]);
+                if (s.lead) led_row = p.row_of(s.first);
+            }
+            const int span = s.steps * p.nkv;
+            int end = base + span;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, end, o);
+                if (lane >= o) end += up - base;
+            }
+            const int F = min(f + lane, f_end - 1);
+            int l = 0;                                                       // the first that ends behind F
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1)
+                if (__shfl_sync(0xffffffffu, end, l + o - 1) <= F) l += o;
+            SharedSeq w;
+            w.ctx = __shfl_sync(0xffffffffu, s.ctx, l);
+            w.begin = __shfl_sync(0xffffffffu, s.begin, l);
+            w.lead = __shfl_sync(0xffffffffu, s.lead, l);
+            steps_x = __shfl_sync(0xffffffffu, s.steps, l);
+            prefix_x = __shfl_sync(0xffffffffu, (int)s.prefix, l);
+            const int base_l = __shfl_sync(0xffffffffu, end - span, l), r_own = __shfl_sync(0xffffffffu, row, l), r_led = __shfl_sync(0xffffffffu, led_row, l);
+            const int rest = F - base_l, h = (int)((unsigned)rest / (unsigned)steps_x);
+            t_x = rest - h * steps_x;
+            from_x = F - t_x;
+            unit_x = (b0 + l) * p.nkv + h;
+            const int r = w.step(p, t_x, lo_x, hi_x) ? r_led : r_own;
+            if (f + lane < f_end && lo_x < hi_x && r >= 0) page_x = p.page_table[(size_t)r * p.max_pages + lo_x / kKvTile];
+            if (page_x >= p.num_pages) page_x = -1;
+            b0 += __shfl_sync(0xffffffffu, l, 31);
+            base = __shfl_sync(0xffffffffu, base_l, 31);
+        }
+        const int n = min(32, f_end - f);
+        const unsigned paged = __ballot_sync(0xffffffffu, page_x >= 0);
+        // 2 D / 64 pieces of a chunk, a lane each
+        auto copy = [&](int x, int stage) {
+            const int page = __shfl_sync(0xffffffffu, page_x, x), at = __shfl_sync(0xffffffffu, lo_x, x) / CH * CH % kKvTile, h = __shfl_sync(0xffffffffu, unit_x, x) % p.nkv;
+            uint8_t* dst = ring + stage * C::CHUNK_BYTES;
+            const uint8_t* src = p.cache + ((size_t)page * p.nkv + h) * C::TILE;
+            if (lane == 0) mbar_expect_tx(&full[stage], C::CHUNK_BYTES);
+            if (CH == kKvTile) {
+                if (lane == 0) tma_bulk_g2s(dst, src, C::CHUNK_BYTES, &full[stage], pol);
+            } else {
+                __syncwarp();
+                if (lane < 2 * C::KH) tma_bulk_g2s(dst + lane * (CH * 128), src + lane * SH_PIECE + at * 128, CH * 128, &full[stage], pol);
+            }
+        };
+        unsigned to_ask = paged;
+        auto ask = [&]() {                                                   // copies run S chunks ahead
+            while (ok && to_ask && asked < it + S) {
+                copy(__ffs(to_ask) - 1, asked % S);
+                to_ask &= to_ask - 1;
+                ++asked;
+            }
+        };
+        ask();
+        bool have_next = false;
+#pragma unroll 1
+        for (int x = 0; x < n; ++x) {
+            const int u = __shfl_sync(0xffffffffu, unit_x, x);
+            if (u != unit) {
+                if (unit >= 0) finish(end_t, end_steps, end_prefix, end_from);
+                unit = u;
+                first = __shfl_sync(0xffffffffu, t_x, x);
+                a.clear();
+                if (have_next) {
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ++ks) a.q[ks][0] = q_next[ks][0], a.q[ks][1] = q_next[ks][1];
+                } else {
+                    query_of(u, a.q);
+                }
+                // the next unit's queries are on their way meanwhile
+                const unsigned other = __ballot_sync(0xffffffffu, lane > x && lane < n && unit_x != u);
+                have_next = other != 0;
+                if (have_next) query_of(__shfl_sync(0xffffffffu, unit_x, __ffs(other) - 1), q_next);
+            }
+            end_t = __shfl_sync(0xffffffffu, t_x, x) + 1;
+            end_steps = __shfl_sync(0xffffffffu, steps_x, x);
+            end_from = __shfl_sync(0xffffffffu, from_x, x);
+            end_prefix = __shfl_sync(0xffffffffu, (int)prefix_x, x);
+            if (!ok || !(paged >> x & 1)) continue;
+            const int stage = it % S;
+            ok = __all_sync(0xffffffffu, mbar_wait_limited(&full[stage], it / S & 1, dead));
+            if (!ok) continue;
+            ++it;
+            const int lo = __shfl_sync(0xffffffffu, lo_x, x), hi = __shfl_sync(0xffffffffu, hi_x, x), at = lo / CH * CH;
+            uint8_t* tile = ring + stage * C::CHUNK_BYTES;
+            if (lo > at || hi < at + CH) {                                   // hidden values may be anything: 0 * infinity is none
+                const int ahead = lo - at, hidden = ahead + at + CH - hi;
+                for (int u8 = lane; u8 < hidden * (D / 8); u8 += 32) {
+                    const int k = u8 / (D / 8), c = u8 % (D / 8), tok = k < ahead ? k : hi - at + k - ahead;
+                    *reinterpret_cast<uint4*>(tile + C::HALF + SharedQuery<D>::at(tok, c)) = make_uint4(0u, 0u, 0u, 0u);
+                }
+                fence_proxy_async();                                         // ahead of the next copy into this stage
+                __syncwarp();
+            }
+            a.chunk(smem_u32(tile), lo - at, hi - at, p.scale_log2, lane);
+            __syncwarp();                                                    // all lanes have read it: the next copy may come
+            ask();
+        }
     }
+    if (unit >= 0) finish(end_t, end_steps, end_prefix, end_from);
     if (lane == 0)
         for (int i = it; i < asked; ++i)                                     // nothing may still be on its way into this CTA's memory when it ends
             for (int k = 0; k < kWaitLimit && !mbar_try_wait(&full[i % S], i / S & 1); ++k) {}
@@ -279,26 +340,32 @@ struct SharedPhases {
     }
 };
 
-// Exclusive sum over the block's threads; `all` is the sum of all
-__device__ __forceinline__ int shared_before(int mine, int* warp_s, int& all) {
+// Exclusive sums of two numbers over the block's threads, and whether all say yes; `all` the sums of all
+__device__ __forceinline__ bool shared_before(const int* mine, int (*warp_s)[SH_WARPS], int* before, int* all, bool yes) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int x = mine;
+    int x[2] = {mine[0], mine[1]};
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += up;
-    }
-    if (lane == 31) warp_s[warp] = x;
-    __syncthreads();
-    int w = lane < SH_WARPS ? warp_s[lane] : 0;
+    for (int o = 1; o < 32; o <<= 1)
 #pragma unroll
-    for (int o = 1; o < SH_WARPS; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, w, o);
-        if (lane >= o) w += up;
+        for (int k = 0; k < 2; ++k) {
+            const int up = __shfl_up_sync(0xffffffffu, x[k], o);
+            if (lane >= o) x[k] += up;
+        }
+    if (lane == 31) warp_s[0][warp] = x[0], warp_s[1][warp] = x[1];
+    yes = __syncthreads_and(yes);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        int w = lane < SH_WARPS ? warp_s[k][lane] : 0;
+#pragma unroll
+        for (int o = 1; o < SH_WARPS; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += up;
+        }
+        all[k] = __shfl_sync(0xffffffffu, w, SH_WARPS - 1);
+        const int ahead = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+        before[k] = x[k] - mine[k] + (warp ? ahead : 0);
     }
-    all = __shfl_sync(0xffffffffu, w, SH_WARPS - 1);
-    const int ahead = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
-    return x - mine + (warp ? ahead : 0);
+    return yes;
 }
 
 template <int D>
@@ -308,13 +375,13 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
     constexpr int KH = C::KH;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    __shared__ uint64_t kv_full[3 * C::STAGES], kv_empty[C::STAGES];         // (full: see SharedPhases)
+    __shared__ uint64_t k_full[3 * C::STAGES], v_full[3 * C::STAGES], k_empty[C::STAGES], v_empty[C::STAGES];        // (full: see SharedPhases)
     __shared__ uint64_t own_full[C::OWN_WARPS * C::OWN_STAGES];
     __shared__ uint64_t q_full[2];                                           // the queries of a half
     __shared__ uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];           // half, buffer: scores are in tensor memory; probabilities are; O += P V retired
     __shared__ uint64_t drained[2];                                          // all products of a half retired
-    __shared__ int tokens_s[C::STAGES];                                      // of the page in each stage; 0: the page is not there
-    __shared__ int sums_s[2][SH_WARPS];
+    __shared__ int tokens_s[C::TOKENS];                                      // of the last pages copied; 0: the page is not there
+    __shared__ int sums_s[2][SH_WARPS], start_s[SH_LIST + 1], lens_s[SH_LIST];
     __shared__ int2 prefix_at, own_at[C::OWN_WARPS];                         // the group (sequence) that a share begins in, and where that begins
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int dead;
@@ -322,8 +389,8 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        for (int s = 0; s < 3 * C::STAGES; ++s) mbar_init(&kv_full[s], 1);
-        for (int s = 0; s < C::STAGES; ++s) mbar_init(&kv_empty[s], 2);
+        for (int s = 0; s < 3 * C::STAGES; ++s) mbar_init(&k_full[s], 1), mbar_init(&v_full[s], 1);
+        for (int s = 0; s < C::STAGES; ++s) mbar_init(&k_empty[s], 2), mbar_init(&v_empty[s], 2);
         for (int s = 0; s < C::OWN_WARPS * C::OWN_STAGES; ++s) mbar_init(&own_full[s], 1);
         for (int h = 0; h < 2; ++h) {
             mbar_init(&q_full[h], kSharedRows / 32);
@@ -339,56 +406,61 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
     }
     pdl_wait();
 
-    // ---------------- the plan: every CTA adds up both lists.  A list of groups that does not grow, or leaves the batch, shares nothing
-    int groups, prefix_f, prefix_end, prefix_per, own_per, own_total;
+    // ---------------- the plan: every CTA adds up both lists, a run of groups and one of sequences a thread.  A list of groups that does not grow, or leaves the batch,
+    // shares nothing
+    SharedGroups gr{p.group_start, p.shared_lens, p.n_groups};
+    int prefix_f, prefix_end, prefix_per, own_per, own_total;
     {
         const int gc = (p.n_groups + SH_THREADS - 1) / SH_THREADS, g0 = min(p.n_groups, tid * gc), g1 = min(p.n_groups, g0 + gc);
         const int bc = (p.B + SH_THREADS - 1) / SH_THREADS, b0 = min(p.B, tid * bc), b1 = min(p.B, b0 + bc);
-        bool grows = true;
-        int mine = 0;
-        for (int g = g0; g < g1; ++g) {
-            grows = grows && p.group_start[g] >= 0 && p.group_start[g] <= p.group_start[g + 1] && p.group_start[g + 1] <= p.B;
-            SharedPrefix w;
-            w.load(p, g);
-            if (grows) mine += w.all(p);
+        const int ctx0 = b0 < b1 ? p.ctx_lens[b0] : 0;
+        if (p.n_groups <= SH_LIST) {
+            if (p.n_groups && tid <= p.n_groups) start_s[tid] = p.group_start[tid];
+            if (tid < p.n_groups) lens_s[tid] = p.shared_lens[tid];
+            gr.start = start_s;
+            gr.lens = lens_s;
         }
-        groups = __syncthreads_and(grows) ? p.n_groups : 0;
-        if (!groups) mine = 0;
-        int total;
-        int before = shared_before(mine, sums_s[0], total);
-        prefix_per = (int)((unsigned)(total + gridDim.x - 1) / gridDim.x);
-        prefix_f = min(prefix_per * (int)blockIdx.x, total);
-        prefix_end = min(prefix_f + prefix_per, total);
-        if (before <= prefix_f && prefix_f < before + mine) {
+        __syncthreads();
+        bool grows = true;
+        int mine[2] = {0, 0}, before[2], all[2];
+        for (int g = g0; g < g1; ++g) {
+            grows = grows && gr.start[g] >= 0 && gr.start[g] <= gr.start[g + 1] && gr.start[g + 1] <= p.B;
+            SharedPrefix w;
+            w.load(p, gr, g);
+            if (grows) mine[0] += w.all(p);
+        }
+        auto steps_of = [&](int b) {
+            SharedSeq s;
+            s.load(p, gr, b, b == b0 ? ctx0 : p.ctx_lens[b]);
+            return s.steps;
+        };
+        for (int b = b0; b < b1; ++b) mine[1] += steps_of(b);
+        if (!shared_before(mine, sums_s, before, all, grows)) {
+            gr.n = 0;
+            mine[0] = mine[1] = 0;
+            for (int b = b0; b < b1; ++b) mine[1] += steps_of(b);
+            __syncthreads();
+            shared_before(mine, sums_s, before, all, true);
+        }
+        prefix_per = (int)((unsigned)(all[0] + gridDim.x - 1) / gridDim.x);
+        prefix_f = min(prefix_per * (int)blockIdx.x, all[0]);
+        prefix_end = min(prefix_f + prefix_per, all[0]);
+        if (before[0] <= prefix_f && prefix_f < before[0] + mine[0]) {
             SharedPrefix w;
             int g = g0;
-            for (w.load(p, g); before + w.all(p) <= prefix_f; w.load(p, ++g)) before += w.all(p);
-            prefix_at = make_int2(g, before);
+            for (w.load(p, gr, g); before[0] + w.all(p) <= prefix_f; w.load(p, gr, ++g)) before[0] += w.all(p);
+            prefix_at = make_int2(g, before[0]);
         }
-        mine = 0;
-        int g = shared_group_of(p.group_start, groups, b0);
-        for (int b = b0, x = g; b < b1; ++b) {
-            while (x + 1 < groups && p.group_start[x + 1] <= b) ++x;
-            SharedSeq s;
-            s.load(p, b, x, p.ctx_lens[b]);
-            mine += s.steps;
-        }
-        before = shared_before(mine, sums_s[1], total) * p.nkv;
-        mine *= p.nkv;
-        own_total = total * p.nkv;
+        own_total = all[1] * p.nkv;
         const int warps = gridDim.x * C::OWN_WARPS;
         own_per = (int)((unsigned)(own_total + warps - 1) / (unsigned)warps);
+        const int from = before[1] * p.nkv, to = from + mine[1] * p.nkv;
+#pragma unroll
         for (int w = 0; w < C::OWN_WARPS; ++w) {
             const int f = own_per * (w * (int)gridDim.x + (int)blockIdx.x);  // (neighbouring shares on different SMs)
-            if (before <= f && f < before + mine) {
-                int b = b0, at = before, x = g;
-                for (;; ++b) {
-                    while (x + 1 < groups && p.group_start[x + 1] <= b) ++x;
-                    SharedSeq s;
-                    s.load(p, b, x, p.ctx_lens[b]);
-                    if (f < at + s.steps * p.nkv) break;
-                    at += s.steps * p.nkv;
-                }
+            if (from <= f && f < to) {
+                int b = b0, at = from;
+                for (int n; f >= at + (n = steps_of(b) * p.nkv); ++b) at += n;
                 own_at[w] = make_int2(b, at);
             }
         }
@@ -404,13 +476,30 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SH_REGS_ISSUE));
         if (warp == 0) {
-            // ---------------- copies of the prefix: one page a time
-            w.start(p, prefix_f, prefix_end, at_s.x, at_s.y);
+            // ---------------- copies of the prefix: a page's keys, and the values of the page two ahead of it, which are needed that much later.  (Never a circle: keys wait for
+            // products of keys STAGES pages back, which wait for products of values further back than those that are copied behind them.)
+            w.start(p, gr, prefix_f, prefix_end, at_s.x, at_s.y);
             const uint64_t pol = policy_evict_first();
-            SharedPhases phases;
+            SharedPhases k_phases, v_phases;
             int it = 0;
+            const uint8_t* wait_v[C::AHEAD];                                 // pages whose values are still to be asked for (null: not there), and their sets
+            int wait_set[C::AHEAD];
+            auto ask = [&](SharedPhases& phases, uint64_t* full, uint64_t* empty, int n, int set, const uint8_t* from, uint8_t* to, int tokens) {
+                const int s = n % C::STAGES;
+                ok = ok && mbar_wait_limited(&empty[s], (n / C::STAGES & 1) ^ 1, &dead);
+                if (!ok) return;
+                phases.next(C::STAGES, s, set);
+                if (tokens >= 0) tokens_s[n % C::TOKENS] = tokens;           // (keys are copied when those STAGES back have been multiplied, which is when the scores of eight back were read)
+                if (from) {
+                    mbar_expect_tx(&full[phases.at], C::SLAB);
+                    tma_bulk_g2s(to + s * C::SLAB, from, C::SLAB, &full[phases.at], pol);
+                } else {
+                    mbar_arrive(&full[phases.at]);
+                }
+            };
+            auto values = [&](const uint8_t* page, int set) { ask(v_phases, v_full, v_empty, it - C::AHEAD, set, page ? page + C::SLAB : nullptr, smem + C::KV + C::STAGES * C::SLAB, -1); };
 #pragma unroll 1
-            while (w.next(p)) {
+            while (w.next(p, gr)) {
                 const int p1 = w.p0 + w.pages, row = p.row_of(w.w.seq0);
 #pragma unroll 1
                 for (int p0 = w.p0; p0 < p1; p0 += 32) {
@@ -419,68 +508,70 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
                     if (my_page >= p.num_pages) my_page = -1;
                     const int n = min(32, p1 - p0);
 #pragma unroll 1
-                    for (int k = 0; k < n; ++k, ++it) {
+                    for (int k = 0; k < n; ++k) {
                         const int page = __shfl_sync(0xffffffffu, my_page, k);
-                        if (lane == 0 && ok) {
-                            const int s = it % C::STAGES;
-                            ok = mbar_wait_limited(&kv_empty[s], (it / C::STAGES & 1) ^ 1, &dead);
-                            if (!ok) continue;
-                            phases.next(C::STAGES, s, w.few ? (p0 + k - w.p0) & 1 : 2);
-                            tokens_s[s] = page >= 0 ? min(kKvTile, w.w.tokens - (p0 + k) * kKvTile) : 0;
-                            if (page >= 0) {
-                                mbar_expect_tx(&kv_full[phases.at], C::TILE);
-                                tma_bulk_g2s(smem + C::KV + s * C::TILE, p.cache + ((size_t)page * p.nkv + w.h) * C::TILE, C::TILE, &kv_full[phases.at], pol);
-                            } else {
-                                mbar_arrive(&kv_full[phases.at]);
-                            }
+                        if (lane == 0) {
+                            const uint8_t* from = page >= 0 ? p.cache + ((size_t)page * p.nkv + w.h) * C::TILE : nullptr;
+                            const int set = w.few ? (p0 + k - w.p0) & 1 : 2;
+                            ask(k_phases, k_full, k_empty, it, set, from, smem + C::KV, page >= 0 ? min(kKvTile, w.w.tokens - (p0 + k) * kKvTile) : 0);
+                            if (it >= C::AHEAD) values(wait_v[0], wait_set[0]);
+                            wait_v[0] = wait_v[1], wait_set[0] = wait_set[1];
+                            wait_v[1] = from, wait_set[1] = set;
                         }
+                        ++it;
                     }
                 }
             }
-            if (lane == 0)
+            if (lane == 0) {
+                for (int i = 0; i < C::AHEAD; ++i, ++it)
+                    if (it >= C::AHEAD) values(wait_v[i], wait_set[i]);
                 for (int i = 0; i < 3 * C::STAGES; ++i)                      // nothing may still be on its way into this CTA's memory when it ends
-                    for (int k = 0; k < kWaitLimit && !mbar_try_wait(&kv_full[i], (phases.bits >> i & 1) ^ 1); ++k) {}
+                    for (int k = 0; k < kWaitLimit && !(mbar_try_wait(&k_full[i], (k_phases.bits >> i & 1) ^ 1) && mbar_try_wait(&v_full[i], (v_phases.bits >> i & 1) ^ 1)); ++k) {}
+            }
             __syncwarp();
         } else if (warp < 3) {
             // ---------------- products, one warp a half
             constexpr uint32_t idesc_qk = umma_idesc_f16(kSharedRows, kKvTile, false), idesc_pv = umma_idesc_f16(kSharedRows, D, true);
             const int h = warp - 1;
-            w.start(p, prefix_f, prefix_end, at_s.x, at_s.y);
+            w.start(p, gr, prefix_f, prefix_end, at_s.x, at_s.y);
             if (elect_one()) {
                 const uint64_t q_desc = umma_desc_k128(smem_u32(smem + h * KH * C::QBLK)), k_desc = umma_desc_k128(smem_u32(smem + C::KV)),
-                               v_desc = umma_desc_mn128(smem_u32(smem + C::KV) + KH * SH_PIECE);
+                               v_desc = umma_desc_mn128(smem_u32(smem + C::KV + C::STAGES * C::SLAB));
                 const uint32_t s_at = tmem + C::COL_S + h * 128, o_at = tmem + C::COL_O + h * D;
-                SharedPhases phases;
+                SharedPhases k_phases, v_phases;
                 int base = 0, n_qk = 0, n_pv = 0, n_q = 0;                   // pages of the share, products of this half, stretches of this half so far
                 auto issue_qk = [&](int page, bool alone) {                  // page: counted over the whole share; alone: the other half has no use for it
                     const int s = page % C::STAGES, buf = n_qk & 1;
-                    const uint32_t parity = phases.next(C::STAGES, s, alone ? h : 2);
-                    ok = mbar_wait_limited(&kv_full[phases.at], parity, &dead);
+                    const uint32_t parity = k_phases.next(C::STAGES, s, alone ? h : 2);
+                    ok = mbar_wait_limited(&k_full[k_phases.at], parity, &dead);
                     if (!ok) return;
                     ++n_qk;
                     tc_fence_after();
-                    const uint64_t b = k_desc + (uint64_t)(s * (C::TILE >> 4));
+                    const uint64_t b = k_desc + (uint64_t)(s * (C::SLAB >> 4));
 #pragma unroll
                     for (int kh = 0; kh < KH; ++kh)
 #pragma unroll
                         for (int k = 0; k < 4; ++k) umma_bf16(s_at + buf * 64, q_desc + kh * (C::QBLK >> 4) + 2 * k, b + kh * (SH_PIECE >> 4) + 2 * k, idesc_qk, (kh | k) != 0);
                     umma_commit(&s_full[h][buf]);
+                    umma_commit(&k_empty[s]);
+                    if (alone) umma_commit(&k_empty[s]);
                 };
                 auto issue_pv = [&](int page, bool first, bool alone) {
                     const int s = page % C::STAGES, buf = n_pv & 1;
-                    ok = mbar_wait_limited(&p_full[h][buf], n_pv >> 1 & 1, &dead);
+                    const uint32_t parity = v_phases.next(C::STAGES, s, alone ? h : 2);
+                    ok = mbar_wait_limited(&v_full[v_phases.at], parity, &dead) && mbar_wait_limited(&p_full[h][buf], n_pv >> 1 & 1, &dead);
                     if (!ok) return;
                     ++n_pv;
                     tc_fence_after();
-                    const uint64_t b = v_desc + (uint64_t)(s * (C::TILE >> 4));
+                    const uint64_t b = v_desc + (uint64_t)(s * (C::SLAB >> 4));
 #pragma unroll
                     for (int k = 0; k < kKvTile / 16; ++k) umma_f16_ts(o_at, s_at + buf * 64 + 8 * k, b + k * (2048 >> 4), idesc_pv, k != 0 || !first);
                     umma_commit(&pv_done[h][buf]);
-                    umma_commit(&kv_empty[s]);
-                    if (alone) umma_commit(&kv_empty[s]);
+                    umma_commit(&v_empty[s]);
+                    if (alone) umma_commit(&v_empty[s]);
                 };
 #pragma unroll 1
-                while (w.next(p)) {
+                while (w.next(p, gr)) {
                     const int mine = w.of_half(h);
                     auto page_of = [&](int i) { return base + (w.few ? h + 2 * i : i); };      // page i of this half
                     if (ok && mine) {
@@ -504,7 +595,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
     } else if (warp < 12) {
         // ---------------- softmax: one thread a row
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SH_REGS_SOFT));
-        w.start(p, prefix_f, prefix_end, at_s.x, at_s.y);
+        w.start(p, gr, prefix_f, prefix_end, at_s.x, at_s.y);
         const int h = (warp - 4) >> 2;
         const int row = (tid - 128) & 127;                                           // lane of tensor memory: warp % 4 is the quarter that a warp may read
         const int tok = row / p.G;
@@ -516,7 +607,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
         auto ml_of = [&](int half) { return reinterpret_cast<float2*>(smem + half * KH * C::QBLK); };
         auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_limited(bar, parity, &dead)); };
 #pragma unroll 1
-        while (w.next(p)) {
+        while (w.next(p, gr)) {
             const int mine = w.of_half(h);
             const int tok0 = w.few ? 0 : h * p.th;                           // of the tile
             const bool valid = tok < p.th && tok0 + tok < w.n;
@@ -549,15 +640,15 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
                 uint32_t sr[64];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) tmem_ld16_nowait(s_at0 + buf * 64 + 16 * c, sr + 16 * c);
-                const int seen = tokens_s[stage];                            // (written ahead of the copy that the scores came of)
+                const int seen = tokens_s[page % C::TOKENS];                 // (written ahead of the copy that the scores came of, and not again before they are read)
                 tmem_arrived<64>(sr);
                 if (seen < kKvTile) {
 #pragma unroll
                     for (int c = 0; c < 64; ++c) sr[c] = c < seen ? sr[c] : 0xff800000u;
                     // values behind the end may be anything, and 0 * infinity is not 0.  (Both halves may write here: zeros.)
-                    ok = wait(&kv_full[phases.at], landed);
+                    ok = wait(&v_full[phases.at], landed);
                     if (!ok) break;
-                    uint8_t* v = smem + C::KV + stage * C::TILE + KH * SH_PIECE;
+                    uint8_t* v = smem + C::KV + (C::STAGES + stage) * C::SLAB;
 #pragma unroll 1
                     for (int u = row; u < (kKvTile - seen) * 8 * KH; u += kSharedRows) {
                         const int kh = u / ((kKvTile - seen) * 8), x = u % ((kKvTile - seen) * 8);
@@ -671,9 +762,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
         const int mine = warp - 12;
         if (mine < C::OWN_WARPS) {
             const int index = mine * gridDim.x + blockIdx.x, f = min(own_per * index, own_total);
-            OwnWalk o;
-            o.start(p, groups, f, min(f + own_per, own_total), own_at[mine].x, own_at[mine].y);
-            shared_own<D>(p, o, groups, own_per, index, smem + C::OWN + mine * (C::OWN_STAGES * C::CHUNK_BYTES), own_full + mine * C::OWN_STAGES, &dead, err);
+            shared_own<D>(p, gr, f, min(f + own_per, own_total), own_at[mine].x, own_at[mine].y, own_per, index, smem + C::OWN + mine * (C::OWN_STAGES * C::CHUNK_BYTES), own_full + mine * C::OWN_STAGES, &dead, err);
         }
     }
     tc_fence_before();
@@ -695,9 +784,10 @@ shared_merge_kernel(const __grid_constant__ SharedArgs p) {
     __shared__ float2 ml_s[SM_THREADS];
     const int unit = blockIdx.x, G = p.G;
     const int4 own = p.own_units[unit];
-    if (own.x < 0) return;
     int4 pre = make_int4(0, -1, 0, 0);
-    if (own.z) pre = p.prefix_units[unit];
+    if (p.n_groups) pre = p.prefix_units[unit];
+    if (own.x < 0) return;
+    if (!own.z) pre = make_int4(0, -1, 0, 0);                                // (then nobody has written there)
     // a thread has four dims of a head (neighbours the same of neighbouring heads, as the prefix's results lie), and every `lanes`-th part
     const int size = G * D / 4, lanes = SM_THREADS / size, e = threadIdx.x % size, mine = threadIdx.x / size, hg = e % G, dim = e / G * 4;
     const int n_own = own.y - own.x + 1, n = n_own + pre.y - pre.x + 1;

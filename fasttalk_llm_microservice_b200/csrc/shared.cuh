@@ -35,16 +35,30 @@ struct SharedArgs {
         const int slot = req_slot ? req_slot[b] : b;
         return slot >= 0 && slot < table_rows ? slot : -1;
     }
-    __host__ __device__ __forceinline__ int shared_of(int g) const { return max(0, min(shared_lens[g], reach())); }
+};
+
+// The groups, wherever the lists lie; n = 0: none
+struct SharedGroups {
+    const int *start, *lens;
+    int n;
+    // the last group that begins at or before b (those without queries begin where the next one does), or -1
+    __host__ __device__ __forceinline__ int of(int b) const {
+        int lo = -1, hi = n - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (start[mid] <= b) lo = mid; else hi = mid - 1;
+        }
+        return lo;
+    }
 };
 
 // A group's prefix part; pages 0: none
 struct SharedPrefix {
     int seq0, size, tokens, pages, tiles;
-    __host__ __device__ __forceinline__ void load(const SharedArgs& p, int g) {
-        seq0 = p.group_start[g];
-        size = p.group_start[g + 1] - seq0;
-        tokens = p.shared_of(g);
+    __host__ __device__ __forceinline__ void load(const SharedArgs& p, const SharedGroups& gr, int g) {
+        seq0 = gr.start[g];
+        size = gr.start[g + 1] - seq0;
+        tokens = max(0, min(gr.lens[g], p.reach()));
         pages = size >= 2 && tokens >= 2 * kKvTile ? (tokens + kKvTile - 1) / kKvTile : 0;
         tiles = (size + 2 * p.th - 1) / (2 * p.th);
     }
@@ -62,15 +76,15 @@ struct SharedPrefix {
 struct SharedSeq {
     int ctx, begin, lead, steps, first;          // first: the query whose row has the shared pages
     bool prefix;                                 // a prefix part is added
-    // g: the group that b may belong to (below 0: none)
-    __host__ __device__ __forceinline__ void load(const SharedArgs& p, int b, int g, int ctx_len) {
+    __host__ __device__ __forceinline__ void load(const SharedArgs& p, const SharedGroups& gr, int b, int ctx_len) {
         ctx = max(0, min(ctx_len, p.reach()));
         begin = lead = 0;
         first = -1;
         prefix = false;
-        if (g >= 0 && p.group_start[g] <= b && b < p.group_start[g + 1]) {
+        const int g = gr.of(b);
+        if (g >= 0 && b < gr.start[g + 1]) {
             SharedPrefix w;
-            w.load(p, g);
+            w.load(p, gr, g);
             begin = w.tokens;
             first = w.seq0;
             prefix = w.pages > 0 && ctx >= begin;
@@ -79,17 +93,15 @@ struct SharedSeq {
         const int own = ctx > begin ? (ctx + p.chunk - 1) / p.chunk - begin / p.chunk : 0;
         steps = max(1, lead + own);
     }
-};
-
-// the last group that begins at or before b (those without queries begin where the next one does), or -1
-__host__ __device__ __forceinline__ int shared_group_of(const int* group_start, int n, int b) {
-    int lo = -1, hi = n - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (group_start[mid] <= b) lo = mid; else hi = mid - 1;
+    // tokens lo .. hi - 1 that step t reads (none: lo >= hi); true: on the first row's pages
+    __host__ __device__ __forceinline__ bool step(const SharedArgs& p, int t, int& lo, int& hi) const {
+        const bool led = t < lead;
+        const int tile = led ? t : begin / p.chunk + t - lead;
+        lo = max(tile * p.chunk, led ? 0 : begin);
+        hi = min(tile * p.chunk + p.chunk, led ? min(begin, ctx) : ctx);
+        return led;
     }
-    return lo;
-}
+};
 
 // A CTA's share of the prefix list, walked stretch by stretch; a stretch = pages p0 .. p0 + pages - 1 of one unit
 struct PrefixWalk {
@@ -104,12 +116,12 @@ struct PrefixWalk {
         steps = w.steps(p, n);
     }
     // the share begins at f, in group g, which begins at base
-    __host__ __device__ __forceinline__ void start(const SharedArgs& p, int f_, int f_end_, int g_, int base) {
+    __host__ __device__ __forceinline__ void start(const SharedArgs& p, const SharedGroups& gr, int f_, int f_end_, int g_, int base) {
         f = f_;
         f_end = f_end_;
         if (f >= f_end) return;
         g = g_;
-        w.load(p, g);
+        w.load(p, gr, g);
         const int each = w.each(p), full = w.pages + kSharedStart;
         int rest = f - base;
         h = (int)((unsigned)rest / (unsigned)each);
@@ -118,7 +130,7 @@ struct PrefixWalk {
         t = rest - tile * full;
         unit(p);
     }
-    __host__ __device__ __forceinline__ bool next(const SharedArgs& p) {
+    __host__ __device__ __forceinline__ bool next(const SharedArgs& p, const SharedGroups& gr) {
 #pragma unroll 1
         for (;;) {
             if (f >= f_end) return false;
@@ -129,7 +141,7 @@ struct PrefixWalk {
                     if (++h == p.nkv) {
                         h = 0;
 #pragma unroll 1
-                        do w.load(p, ++g);
+                        do w.load(p, gr, ++g);
                         while (w.pages == 0);
                     }
                 }
@@ -147,51 +159,6 @@ struct PrefixWalk {
         }
     }
     __host__ __device__ __forceinline__ int of_half(int half) const { return few ? (pages - half + 1) / 2 : pages; }      // its pages
-};
-
-// A warp's share of the own list, walked stretch by stretch; a stretch = steps t0 .. t1 - 1 of one unit
-struct OwnWalk {
-    SharedSeq s;
-    int f, f_end, unit_f, b, g, h, t, t0, t1;
-    // the share begins at f, in sequence b, whose units begin at base; groups: how many there are
-    __host__ __device__ __forceinline__ void start(const SharedArgs& p, int groups, int f_, int f_end_, int b_, int base) {
-        f = f_;
-        f_end = f_end_;
-        if (f >= f_end) return;
-        b = b_;
-        g = shared_group_of(p.group_start, groups, b);
-        s.load(p, b, g, p.ctx_lens[b]);
-        const int rest = f - base;
-        h = (int)((unsigned)rest / (unsigned)s.steps);
-        t = rest - h * s.steps;
-    }
-    __host__ __device__ __forceinline__ bool next(const SharedArgs& p, int groups) {
-        if (f >= f_end) return false;
-        if (t >= s.steps) {
-            t = 0;
-            if (++h == p.nkv) {
-                h = 0;
-                ++b;
-                while (g + 1 < groups && p.group_start[g + 1] <= b) ++g;
-                s.load(p, b, g, p.ctx_lens[b]);
-            }
-        }
-        const int take = min(f_end - f, s.steps - t);
-        unit_f = f - t;
-        t0 = t;
-        t1 = t + take;
-        t = t1;
-        f += take;
-        return true;
-    }
-    // tokens lo .. hi - 1 of the sequence that step x reads, on the pages of query `row`'s row (none: lo >= hi)
-    __host__ __device__ __forceinline__ void step(const SharedArgs& p, int x, int& lo, int& hi, int& row) const {
-        const bool led = x < s.lead;
-        const int tile = led ? x : s.begin / p.chunk + x - s.lead;
-        lo = max(tile * p.chunk, led ? 0 : s.begin);
-        hi = min(tile * p.chunk + p.chunk, led ? min(s.begin, s.ctx) : s.ctx);
-        row = led ? s.first : b;
-    }
 };
 
 }  // namespace ft

@@ -15,15 +15,16 @@ extern "C" int shared_stretches(int own, const int* ctx_lens, int B, const int* 
     bool grows = true;
     for (int g = 0; g < n_groups; ++g) grows = grows && starts[g] >= 0 && starts[g] <= starts[g + 1] && starts[g + 1] <= B;
     const int groups = grows ? n_groups : 0;
+    const SharedGroups gr{starts, shared, grows ? n_groups : 0};
     int total = 0, found = 0;
-    for (int g = 0; !own && g < groups; ++g) {
+    for (int g = 0; !own && g < gr.n; ++g) {
         SharedPrefix w;
-        w.load(p, g);
+        w.load(p, gr, g);
         total += w.all(p);
     }
     for (int b = 0; own && b < B; ++b) {
         SharedSeq s;
-        s.load(p, b, shared_group_of(starts, groups, b), ctx_lens[b]);
+        s.load(p, gr, b, ctx_lens[b]);
         total += s.steps * nkv;
     }
     const int per = (int)((unsigned)(total + shares - 1) / (unsigned)shares);
@@ -34,30 +35,29 @@ extern "C" int shared_stretches(int own, const int* ctx_lens, int B, const int* 
     for (int x = 0; x < shares; ++x) {
         const int f = min(per * x, total), end = min(f + per, total);
         int base = 0, at = 0;
-        if (own) {
+        if (own) {                                   // step by step, as the kernel's lanes find them; told as stretches
             SharedSeq s;
             for (; f < end; base += s.steps * nkv, ++at) {
-                s.load(p, at, shared_group_of(starts, groups, at), ctx_lens[at]);
+                s.load(p, gr, at, ctx_lens[at]);
                 if (f < base + s.steps * nkv) break;
             }
-            OwnWalk w;
-            memset((void*)&w, unset, sizeof(w));
-            w.start(p, groups, f, end, at, base);
-            for (int n = 0; w.next(p, groups); ++n) {
-                if (n == limit) return -1 - x;
-                const int row[9] = {x, w.b, w.h, w.t0, w.t1, w.s.steps, w.s.prefix, w.unit_f / per, (w.unit_f + w.s.steps - 1) / per};
+            for (int F = f; F < end;) {
+                for (s.load(p, gr, at, ctx_lens[at]); F >= base + s.steps * nkv; s.load(p, gr, at, ctx_lens[at])) base += s.steps * nkv, ++at;
+                const int rest = F - base, h = rest / s.steps, t = rest - h * s.steps, take = min(s.steps - t, end - F), from = F - t;
+                const int row[9] = {x, at, h, t, t + take, s.steps, s.prefix, from / per, (from + s.steps - 1) / per};
                 tell(row);
+                F += take;
             }
         } else {
             SharedPrefix s;
             for (; f < end; base += s.all(p), ++at) {
-                s.load(p, at);
+                s.load(p, gr, at);
                 if (f < base + s.all(p)) break;
             }
             PrefixWalk w;
             memset((void*)&w, unset, sizeof(w));
-            w.start(p, f, end, at, base);
-            for (int n = 0; w.next(p); ++n) {
+            w.start(p, gr, f, end, at, base);
+            for (int n = 0; w.next(p, gr); ++n) {
                 if (n == limit) return -1 - x;
                 const int row[9] = {x, w.g, w.h, w.tile, w.p0, w.pages, w.few, w.unit_f / per, (w.unit_f + w.steps - 1) / per};
                 tell(row);
@@ -72,10 +72,9 @@ extern "C" void shared_step(const int* ctx_lens, int B, int b, const int* starts
     SharedArgs p{};
     p.ctx_lens = ctx_lens, p.group_start = starts, p.shared_lens = shared;
     p.B = B, p.n_groups = n_groups, p.max_pages = max_pages, p.nkv = 1, p.nq = 1, p.G = 1, p.th = kSharedRows, p.chunk = chunk;
-    OwnWalk w;
-    w.b = b;
-    w.s.load(p, b, shared_group_of(starts, n_groups, b), ctx_lens[b]);
-    w.step(p, x, out[0], out[1], out[2]);
+    SharedSeq s;
+    s.load(p, SharedGroups{starts, shared, n_groups}, b, ctx_lens[b]);
+    out[2] = s.step(p, x, out[0], out[1]) ? s.first : b;
 }
 
 // Where row 0 of (group, head, query i of the group) lies among the prefix's results
@@ -83,6 +82,6 @@ extern "C" int shared_row(const int* starts, const int* shared, int g, int h, in
     SharedArgs p{};
     p.group_start = starts, p.shared_lens = shared, p.max_pages = max_pages, p.nkv = nkv, p.nq = nkv * G, p.G = G, p.th = kSharedRows / G;
     SharedPrefix w;
-    w.load(p, g);
+    w.load(p, SharedGroups{starts, shared, 1 << 30}, g);
     return w.row(p, h, i);
 }
