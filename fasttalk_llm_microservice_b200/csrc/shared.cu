@@ -8,8 +8,7 @@
 //            mask is the end of the last one.
 //   own      a warp walks a share of its own: chunks of 16 KB by bulk copies that it asks for itself, two of them on their way while it multiplies (mma.sync, the
 //            query heads of a key head in the columns).  No warp waits for another.
-// Each share's results are O, maximum and sum of its rows; a second kernel puts them together in their order.  A (sequence, key head) that one warp has whole and that
-// has no prefix is written right away.
+// Each share's results are O, maximum and sum of its rows; a second kernel puts them together in their order.
 #include "common.cuh"
 #include "ft_internal.h"
 #include "shared.cuh"
@@ -20,11 +19,13 @@ constexpr float kSharedLog2E = 1.4426950408889634f;
 // Probabilities are formed 2^6 times their size, so that fp16's normal numbers reach down to 2^-20 of the largest; a running maximum may lag by 2^8
 constexpr float kSharedTop = 6.f, kSharedGrow = 8.f;
 
-// Groups of four warps: warp 0 copies the prefix's pages, 1 and 2 issue the halves' products, 3 owns tensor memory; 4 .. 11 softmax (half = (warp - 4) / 4); 12 .. 15 own
+// Groups of four warps: warp 0 copies the prefix's pages, 1 and 2 issue the halves' products, 3 owns tensor memory and walks the list; 4 .. 11 softmax (half = (warp - 4) / 4); 12 .. 15 own
 constexpr int SH_THREADS = 512, SH_WARPS = SH_THREADS / 32;
 constexpr int SH_REGS = 128, SH_REGS_ISSUE = 88, SH_REGS_SOFT = 144, SH_REGS_OWN = 136;
 static_assert(SH_REGS_ISSUE + 2 * SH_REGS_SOFT + SH_REGS_OWN <= 4 * SH_REGS, "what the block is launched with");
 constexpr int SH_SOFT = 256;
+constexpr int SH_TOLD = 4, SH_LISTENERS = 11;    // stretches told ahead; warps that hear of them
+constexpr int SH_LEAST = 4;
 constexpr int SH_LIST = 128;                     // groups whose lists are kept in shared memory
 constexpr int SH_PIECE = kKvTile * 128;          // [64 tokens][64 dims] in fp16
 
@@ -47,6 +48,18 @@ struct Shared {
     static_assert(COL_O + 2 * D <= COLS, "tensor memory");
     static_assert(SMEM <= 232448 - 1792, "shared memory");
 };
+
+// A wait that ends, in a few instructions: what bounds calls of ten microseconds here is among others how much code they touch for the first time (126 KB, with waits and
+// loops unrolled and the walk in every role, took 3 of 10 issue slots' worth of waiting for instructions)
+__device__ __forceinline__ bool shared_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
+#pragma unroll 1
+    for (int i = 0; i < kWaitLimit; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*dead) return false;
+    }
+    *dead = 1;
+    return false;
+}
 
 // floats of an own part: O [G][D], (m, l) of the heads; on 16 bytes
 __host__ __device__ __forceinline__ int shared_part(int G, int d) { return (G * (d + 2) + 3) / 4 * 4; }
@@ -76,6 +89,7 @@ struct SharedQuery {
 #pragma unroll
         for (int b = 0; b < BLOCKS; ++b) {
             s[b][0] = s[b][1] = s[b][2] = s[b][3] = 0.f;
+            if (16 * b >= hi || 16 * b + 16 <= lo) continue;
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks) {
                 uint32_t a0, a1, a2, a3;
@@ -97,15 +111,12 @@ struct SharedQuery {
             most[0] = fmaxf(most[0], fmaxf(s[b][0], s[b][2]));
             most[1] = fmaxf(most[1], fmaxf(s[b][1], s[b][3]));
         }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1) most[e] = fmaxf(most[e], __shfl_xor_sync(0xffffffffu, most[e], x));
-            most[e] *= scale_log2;
-        }
-        if (__any_sync(0xffffffffu, most[0] > m[0] + kSharedGrow || most[1] > m[1] + kSharedGrow)) {
+        most[0] *= scale_log2, most[1] *= scale_log2;
+        if (__any_sync(0xffffffffu, most[0] > m[0] + kSharedGrow || most[1] > m[1] + kSharedGrow)) {     // after the first chunk rarely
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) most[e] = fmaxf(most[e], __shfl_xor_sync(0xffffffffu, most[e], x));
                 const float m_new = fmaxf(m[e], most[e]);
                 const float keep = m_new == -INFINITY ? 1.f : ex2_fast(m[e] - m_new);
                 l[e] *= keep;
@@ -117,6 +128,7 @@ struct SharedQuery {
         const float r0 = kSharedTop - (m[0] == -INFINITY ? 0.f : m[0]), r1 = kSharedTop - (m[1] == -INFINITY ? 0.f : m[1]);
 #pragma unroll
         for (int b = 0; b < BLOCKS; ++b) {
+            if (16 * b >= hi || 16 * b + 16 <= lo) continue;
             uint32_t pb[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -145,74 +157,40 @@ struct SharedQuery {
     }
 };
 
-// The share f .. f_end - 1 of the own list; sequence b0 begins at `base` of it, and the share in b0.  Thirty-two steps at a time, a lane each, the warp finds out what they
-// read; then copies run ahead and results are written whichever sequences the steps belong to.
+// The share f0 .. f_end - 1 of the own list; sequence b0 begins at `base` of it, and the share in b0.  Thirty-two steps at a time, a lane each, the warp finds out what they
+// read; copies run ahead and results are written whichever sequences the steps belong to.
 template <int D>
-__device__ __forceinline__ void shared_own(const SharedArgs& p, const SharedGroups& gr, int f, int f_end, int b0, int base, int per, int warp, uint8_t* ring, uint64_t* full,
+__device__ __forceinline__ void shared_own(const SharedArgs& p, const SharedGroups& gr, int f0, int f_end, int b0, int base, int per, int warp, uint8_t* ring, uint64_t* full,
                                            volatile int* dead, int* err) {
     using C = Shared<D>;
     constexpr int S = C::OWN_STAGES, CH = C::CHUNK;
     const int lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3, G = p.G;
+    if (f0 >= f_end) return;
     const uint64_t pol = policy_evict_first();                               // every byte is read once
     bool ok = true;
     int it = 0, asked = 0;                                                   // chunks of the share so far, with a page: a stage's phase follows from the count
     SharedQuery<D> a;
-    uint32_t q_next[D / 16][2];
-    int unit = -1, first = 0;                                                // the unit under way, and its first step here
-    // what this warp has of the unit under way, of `steps` steps up to `end`, which begins at from
-    auto finish = [&](int end, int steps, bool prefix, int from) {
-        if (!ok) {                                                           // NaN for all that this (sequence, head) says
-            *err = 1;
-            a.m[0] = a.m[1] = 0.f;
-            a.l[0] = a.l[1] = NAN;
-        }
-        float sum[2];
-        a.total(sum);
-        const bool all = first == 0 && end == steps && !prefix;
-        if (lane == 0 && first == 0) p.own_units[unit] = all ? make_int4(-1, 0, 0, 0) : make_int4(warp, (int)((unsigned)(from + steps - 1) / (unsigned)per), prefix, 0);
-        float* part = p.own_parts + (size_t)(unit + warp) * shared_part(G, D);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int head = 2 * tq + e;
-            if (head >= G) continue;
-            if (all) {                                                       // a query without a visible key: zeros
-                const float r = sum[e] == 0.f ? 0.f : 1.f / sum[e];
-                const size_t at = ((size_t)unit * G + head) * D;             // (unit = sequence * key heads + key head)
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const float x = a.o[i][2 * u + e] * r;
-                        const __nv_bfloat16 hi = __float2bfloat16(x);
-                        p.out[at + 16 * i + 8 * u + g] = hi;
-                        if (p.out_lo) p.out_lo[at + 16 * i + 8 * u + g] = __float2bfloat16(x - __bfloat162float(hi));
-                    }
-            } else {
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    part[head * D + 16 * i + g] = a.o[i][e];
-                    part[head * D + 16 * i + 8 + g] = a.o[i][2 + e];
-                }
-                if (g == 0) *reinterpret_cast<float2*>(part + G * D + 2 * head) = make_float2(a.m[e], sum[e]);
-            }
-        }
-    };
-    auto query_of = [&](int u, uint32_t (*q)[2]) {
-        const __half* row = p.q + ((size_t)u * G + g) * D + 2 * tq;
+    uint32_t q_next[D / 16][2];                                              // the next unit's queries, on their way while this one's chunks are multiplied
+    auto query_of = [&](int u) {
+        const __half* row = p.q + ((size_t)u * G + g) * D + 2 * tq;          // (unit = sequence * key heads + key head)
+        const bool on = g < G && u < p.B * p.nkv;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
-            q[ks][0] = g < G ? *reinterpret_cast<const uint32_t*>(row + ks * 16) : 0u;
-            q[ks][1] = g < G ? *reinterpret_cast<const uint32_t*>(row + ks * 16 + 8) : 0u;
+            q_next[ks][0] = on ? *reinterpret_cast<const uint32_t*>(row + ks * 16) : 0u;
+            q_next[ks][1] = on ? *reinterpret_cast<const uint32_t*>(row + ks * 16 + 8) : 0u;
         }
     };
-    int end_t = 0, end_steps = 0, end_from = 0;                              // of the last step so far
-    bool end_prefix = false;
+    // lane x: step x of the 32 at hand
+    int unit_x = 0, head_x = 0, from_x = 0, last_x = 0, lo_x = 0, hi_x = 0, page_x = -1;
+    bool prefix_x = false;
+    unsigned paged = 0, to_ask = 0;
+    int unit = -1, from = 0, last = 0;                                       // the unit under way: where it begins in the list, its last step
+    bool prefix = false;
 #pragma unroll 1
-    for (; f < f_end; f += 32) {
-        // ---- lane x: step f + x.  The next 32 sequences hold 32 steps at least
-        int unit_x, t_x, steps_x, from_x, lo_x, hi_x, page_x = -1;
-        bool prefix_x;
-        {
+    for (int f = f0;; ++f) {
+        const int x = (f - f0) & 31;
+        if (x == 0 && f < f_end) {
+            // ---- the next 32 sequences hold 32 steps at least
             const int b = b0 + lane;
             SharedSeq s;
             int row = -1, led_row = -1;
@@ -223,12 +201,13 @@ __device__ __forceinline__ void shared_own(const SharedArgs& p, const SharedGrou
                 if (s.lead) led_row = p.row_of(s.first);
             }
             const int span = s.steps * p.nkv;
-            int end = base + span;
+            int end = span;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int up = __shfl_up_sync(0xffffffffu, end, o);
-                if (lane >= o) end += up - base;
+                if (lane >= o) end += up;
             }
+            end += base;
             const int F = min(f + lane, f_end - 1);
             int l = 0;                                                       // the first that ends behind F
 #pragma unroll
@@ -238,91 +217,103 @@ __device__ __forceinline__ void shared_own(const SharedArgs& p, const SharedGrou
             w.ctx = __shfl_sync(0xffffffffu, s.ctx, l);
             w.begin = __shfl_sync(0xffffffffu, s.begin, l);
             w.lead = __shfl_sync(0xffffffffu, s.lead, l);
-            steps_x = __shfl_sync(0xffffffffu, s.steps, l);
+            w.steps = __shfl_sync(0xffffffffu, s.steps, l);
             prefix_x = __shfl_sync(0xffffffffu, (int)s.prefix, l);
             const int base_l = __shfl_sync(0xffffffffu, end - span, l), r_own = __shfl_sync(0xffffffffu, row, l), r_led = __shfl_sync(0xffffffffu, led_row, l);
-            const int rest = F - base_l, h = (int)((unsigned)rest / (unsigned)steps_x);
-            t_x = rest - h * steps_x;
-            from_x = F - t_x;
-            unit_x = (b0 + l) * p.nkv + h;
-            const int r = w.step(p, t_x, lo_x, hi_x) ? r_led : r_own;
+            head_x = (int)((unsigned)(F - base_l) / (unsigned)w.steps);
+            from_x = base_l + head_x * w.steps;
+            last_x = from_x + w.steps - 1;
+            unit_x = (b0 + l) * p.nkv + head_x;
+            const int r = w.step(p, F - from_x, lo_x, hi_x) ? r_led : r_own;
+            page_x = -1;
             if (f + lane < f_end && lo_x < hi_x && r >= 0) page_x = p.page_table[(size_t)r * p.max_pages + lo_x / kKvTile];
             if (page_x >= p.num_pages) page_x = -1;
             b0 += __shfl_sync(0xffffffffu, l, 31);
             base = __shfl_sync(0xffffffffu, base_l, 31);
+            to_ask = paged = __ballot_sync(0xffffffffu, page_x >= 0);
+            if (unit < 0) query_of(__shfl_sync(0xffffffffu, unit_x, 0));
         }
-        const int n = min(32, f_end - f);
-        const unsigned paged = __ballot_sync(0xffffffffu, page_x >= 0);
-        // 2 D / 64 pieces of a chunk, a lane each
-        auto copy = [&](int x, int stage) {
-            const int page = __shfl_sync(0xffffffffu, page_x, x), at = __shfl_sync(0xffffffffu, lo_x, x) / CH * CH % kKvTile, h = __shfl_sync(0xffffffffu, unit_x, x) % p.nkv;
+        // ---- copies run S chunks ahead
+#pragma unroll 1
+        while (ok && to_ask && asked < it + S) {
+            const int y = __ffs(to_ask) - 1, stage = asked % S;
+            const int page = __shfl_sync(0xffffffffu, page_x, y), at = __shfl_sync(0xffffffffu, lo_x, y) / CH * CH % kKvTile, h = __shfl_sync(0xffffffffu, head_x, y);
             uint8_t* dst = ring + stage * C::CHUNK_BYTES;
             const uint8_t* src = p.cache + ((size_t)page * p.nkv + h) * C::TILE;
             if (lane == 0) mbar_expect_tx(&full[stage], C::CHUNK_BYTES);
             if (CH == kKvTile) {
                 if (lane == 0) tma_bulk_g2s(dst, src, C::CHUNK_BYTES, &full[stage], pol);
-            } else {
+            } else {                                                         // 2 D / 64 pieces, a lane each
                 __syncwarp();
                 if (lane < 2 * C::KH) tma_bulk_g2s(dst + lane * (CH * 128), src + lane * SH_PIECE + at * 128, CH * 128, &full[stage], pol);
             }
-        };
-        unsigned to_ask = paged;
-        auto ask = [&]() {                                                   // copies run S chunks ahead
-            while (ok && to_ask && asked < it + S) {
-                copy(__ffs(to_ask) - 1, asked % S);
-                to_ask &= to_ask - 1;
-                ++asked;
-            }
-        };
-        ask();
-        bool have_next = false;
-#pragma unroll 1
-        for (int x = 0; x < n; ++x) {
-            const int u = __shfl_sync(0xffffffffu, unit_x, x);
-            if (u != unit) {
-                if (unit >= 0) finish(end_t, end_steps, end_prefix, end_from);
-                unit = u;
-                first = __shfl_sync(0xffffffffu, t_x, x);
-                a.clear();
-                if (have_next) {
-#pragma unroll
-                    for (int ks = 0; ks < D / 16; ++ks) a.q[ks][0] = q_next[ks][0], a.q[ks][1] = q_next[ks][1];
-                } else {
-                    query_of(u, a.q);
-                }
-                // the next unit's queries are on their way meanwhile
-                const unsigned other = __ballot_sync(0xffffffffu, lane > x && lane < n && unit_x != u);
-                have_next = other != 0;
-                if (have_next) query_of(__shfl_sync(0xffffffffu, unit_x, __ffs(other) - 1), q_next);
-            }
-            end_t = __shfl_sync(0xffffffffu, t_x, x) + 1;
-            end_steps = __shfl_sync(0xffffffffu, steps_x, x);
-            end_from = __shfl_sync(0xffffffffu, from_x, x);
-            end_prefix = __shfl_sync(0xffffffffu, (int)prefix_x, x);
-            if (!ok || !(paged >> x & 1)) continue;
-            const int stage = it % S;
-            ok = __all_sync(0xffffffffu, mbar_wait_limited(&full[stage], it / S & 1, dead));
-            if (!ok) continue;
-            ++it;
-            const int lo = __shfl_sync(0xffffffffu, lo_x, x), hi = __shfl_sync(0xffffffffu, hi_x, x), at = lo / CH * CH;
-            uint8_t* tile = ring + stage * C::CHUNK_BYTES;
-            if (lo > at || hi < at + CH) {                                   // hidden values may be anything: 0 * infinity is none
-                const int ahead = lo - at, hidden = ahead + at + CH - hi;
-                for (int u8 = lane; u8 < hidden * (D / 8); u8 += 32) {
-                    const int k = u8 / (D / 8), c = u8 % (D / 8), tok = k < ahead ? k : hi - at + k - ahead;
-                    *reinterpret_cast<uint4*>(tile + C::HALF + SharedQuery<D>::at(tok, c)) = make_uint4(0u, 0u, 0u, 0u);
-                }
-                fence_proxy_async();                                         // ahead of the next copy into this stage
-                __syncwarp();
-            }
-            a.chunk(smem_u32(tile), lo - at, hi - at, p.scale_log2, lane);
-            __syncwarp();                                                    // all lanes have read it: the next copy may come
-            ask();
+            to_ask &= to_ask - 1;
+            ++asked;
         }
+        const int u = f < f_end ? __shfl_sync(0xffffffffu, unit_x, x) : -1;
+        if (u != unit) {
+            if (unit >= 0) {
+                // ---- what this warp has of the unit that ends here
+                float sum[2];
+                a.total(sum);
+                if (!ok) {                                                   // NaN for all that this (sequence, head) says
+                    *err = 1;
+                    a.m[0] = a.m[1] = 0.f;
+                    sum[0] = sum[1] = NAN;
+                }
+                if (lane == 0 && from >= f0) p.own_units[unit] = make_int4(warp, (int)((unsigned)last / (unsigned)per), prefix, 0);
+                float* part = p.own_parts + (size_t)(unit + warp) * shared_part(G, D);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int head = 2 * tq + e;
+                    if (head >= G) continue;
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        part[head * D + 16 * i + g] = a.o[i][e];
+                        part[head * D + 16 * i + 8 + g] = a.o[i][2 + e];
+                    }
+                    if (g == 0) *reinterpret_cast<float2*>(part + G * D + 2 * head) = make_float2(a.m[e], sum[e]);
+                }
+            }
+            if (u < 0) break;
+            unit = u;
+            from = __shfl_sync(0xffffffffu, from_x, x);
+            last = __shfl_sync(0xffffffffu, last_x, x);
+            prefix = __shfl_sync(0xffffffffu, (int)prefix_x, x);
+            a.clear();
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks) a.q[ks][0] = q_next[ks][0], a.q[ks][1] = q_next[ks][1];
+            query_of(u + 1);
+        }
+        if (!ok || !(paged >> x & 1)) continue;
+        const int stage = it % S;
+        ok = __all_sync(0xffffffffu, shared_wait(&full[stage], it / S & 1, dead));
+        if (!ok) continue;
+        ++it;
+        const int lo = __shfl_sync(0xffffffffu, lo_x, x), hi = __shfl_sync(0xffffffffu, hi_x, x), at = lo / CH * CH;
+        uint8_t* tile = ring + stage * C::CHUNK_BYTES;
+        if (lo > at || hi < at + CH) {                                       // hidden values may be anything: 0 * infinity is none
+            // (in the blocks of 16 that are multiplied)
+#pragma unroll 1
+            for (int b = 0; b < CH; b += 16) {
+                const int from_t = lo - at - b, to_t = hi - at - b;
+                if (from_t >= 16 || to_t <= 0 || (from_t <= 0 && to_t >= 16)) continue;
+#pragma unroll
+                for (int j = 0; j < D / 16; ++j) {
+                    const int v = lane + 32 * j, k = v / (D / 8);
+                    if (k < from_t || k >= to_t) *reinterpret_cast<uint4*>(tile + C::HALF + SharedQuery<D>::at(b + k, v % (D / 8))) = make_uint4(0u, 0u, 0u, 0u);
+                }
+            }
+            fence_proxy_async();                                             // ahead of the next copy into this stage
+            __syncwarp();
+        }
+        a.chunk(smem_u32(tile), lo - at, hi - at, p.scale_log2, lane);
+        __syncwarp();                                                        // all lanes have read it: the next copy may come
     }
-    if (unit >= 0) finish(end_t, end_steps, end_prefix, end_from);
     if (lane == 0)
+#pragma unroll 1
         for (int i = it; i < asked; ++i)                                     // nothing may still be on its way into this CTA's memory when it ends
+#pragma unroll 1
             for (int k = 0; k < kWaitLimit && !mbar_try_wait(&full[i % S], i / S & 1); ++k) {}
 }
 
@@ -379,6 +370,8 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
     __shared__ uint64_t own_full[C::OWN_WARPS * C::OWN_STAGES];
     __shared__ uint64_t q_full[2];                                           // the queries of a half
     __shared__ uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];           // half, buffer: scores are in tensor memory; probabilities are; O += P V retired
+    __shared__ uint64_t told_full[SH_TOLD], told_empty[SH_TOLD];             // a stretch has been told; all have done with it
+    __shared__ SharedStretch told[SH_TOLD];
     __shared__ uint64_t drained[2];                                          // all products of a half retired
     __shared__ int tokens_s[C::TOKENS];                                      // of the last pages copied; 0: the page is not there
     __shared__ int sums_s[2][SH_WARPS], start_s[SH_LIST + 1], lens_s[SH_LIST];
@@ -392,6 +385,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
         for (int s = 0; s < 3 * C::STAGES; ++s) mbar_init(&k_full[s], 1), mbar_init(&v_full[s], 1);
         for (int s = 0; s < C::STAGES; ++s) mbar_init(&k_empty[s], 2), mbar_init(&v_empty[s], 2);
         for (int s = 0; s < C::OWN_WARPS * C::OWN_STAGES; ++s) mbar_init(&own_full[s], 1);
+        for (int s = 0; s < SH_TOLD; ++s) mbar_init(&told_full[s], 1), mbar_init(&told_empty[s], SH_LISTENERS);
         for (int h = 0; h < 2; ++h) {
             mbar_init(&q_full[h], kSharedRows / 32);
             mbar_init(&drained[h], 1);
@@ -414,6 +408,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
         const int gc = (p.n_groups + SH_THREADS - 1) / SH_THREADS, g0 = min(p.n_groups, tid * gc), g1 = min(p.n_groups, g0 + gc);
         const int bc = (p.B + SH_THREADS - 1) / SH_THREADS, b0 = min(p.B, tid * bc), b1 = min(p.B, b0 + bc);
         const int ctx0 = b0 < b1 ? p.ctx_lens[b0] : 0;
+        if (bc == 1 && b0 < b1 && p.req_slot) asm volatile("prefetch.global.L1 [%0];" ::"l"(p.req_slot + b0));       // the own warps look these up first
         if (p.n_groups <= SH_LIST) {
             if (p.n_groups && tid <= p.n_groups) start_s[tid] = p.group_start[tid];
             if (tid < p.n_groups) lens_s[tid] = p.shared_lens[tid];
@@ -421,46 +416,58 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
             gr.lens = lens_s;
         }
         __syncthreads();
-        bool grows = true;
-        int mine[2] = {0, 0}, before[2], all[2];
-        for (int g = g0; g < g1; ++g) {
-            grows = grows && gr.start[g] >= 0 && gr.start[g] <= gr.start[g + 1] && gr.start[g + 1] <= p.B;
-            SharedPrefix w;
-            w.load(p, gr, g);
-            if (grows) mine[0] += w.all(p);
-        }
         auto steps_of = [&](int b) {
             SharedSeq s;
             s.load(p, gr, b, b == b0 ? ctx0 : p.ctx_lens[b]);
             return s.steps;
         };
-        for (int b = b0; b < b1; ++b) mine[1] += steps_of(b);
-        if (!shared_before(mine, sums_s, before, all, grows)) {
-            gr.n = 0;
+        bool grows = true;
+        int mine[2], before[2], all[2];
+#pragma unroll 1
+        for (int g = g0; g < g1; ++g) grows = grows && gr.start[g] >= 0 && gr.start[g] <= gr.start[g + 1] && gr.start[g + 1] <= p.B;
+#pragma unroll 1
+        for (;;) {
             mine[0] = mine[1] = 0;
+#pragma unroll 1
+            for (int g = g0; g < g1 && grows && gr.n; ++g) {
+                SharedPrefix w;
+                w.load(p, gr, g);
+                mine[0] += w.all(p);
+            }
+#pragma unroll 1
             for (int b = b0; b < b1; ++b) mine[1] += steps_of(b);
+            if (shared_before(mine, sums_s, before, all, grows) || gr.n == 0) break;
+            gr.n = 0;
             __syncthreads();
-            shared_before(mine, sums_s, before, all, true);
         }
-        prefix_per = (int)((unsigned)(all[0] + gridDim.x - 1) / gridDim.x);
+        own_total = all[1] * p.nkv;
+        const int warps = gridDim.x * C::OWN_WARPS;
+        own_per = (int)((unsigned)(own_total + warps - 1) / (unsigned)warps);
+        // Prefix shares of four steps at least where the own ones are as long: half the results to put together
+        prefix_per = max((int)((unsigned)(all[0] + gridDim.x - 1) / gridDim.x), min(SH_LEAST, own_per));
         prefix_f = min(prefix_per * (int)blockIdx.x, all[0]);
         prefix_end = min(prefix_f + prefix_per, all[0]);
         if (before[0] <= prefix_f && prefix_f < before[0] + mine[0]) {
             SharedPrefix w;
             int g = g0;
-            for (w.load(p, gr, g); before[0] + w.all(p) <= prefix_f; w.load(p, gr, ++g)) before[0] += w.all(p);
+#pragma unroll 1
+            for (;; ++g) {
+                w.load(p, gr, g);
+                const int n = w.all(p);
+                if (before[0] + n > prefix_f) break;
+                before[0] += n;
+            }
             prefix_at = make_int2(g, before[0]);
         }
-        own_total = all[1] * p.nkv;
-        const int warps = gridDim.x * C::OWN_WARPS;
-        own_per = (int)((unsigned)(own_total + warps - 1) / (unsigned)warps);
         const int from = before[1] * p.nkv, to = from + mine[1] * p.nkv;
-#pragma unroll
+#pragma unroll 1
         for (int w = 0; w < C::OWN_WARPS; ++w) {
             const int f = own_per * (w * (int)gridDim.x + (int)blockIdx.x);  // (neighbouring shares on different SMs)
             if (from <= f && f < to) {
                 int b = b0, at = from;
-                for (int n; f >= at + (n = steps_of(b) * p.nkv); ++b) at += n;
+                if (bc > 1)
+#pragma unroll 1
+                    for (int n; f >= at + (n = steps_of(b) * p.nkv); ++b) at += n;
                 own_at[w] = make_int2(b, at);
             }
         }
@@ -470,71 +477,111 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     bool ok = true;                                                          // false: a wait ran out
-    PrefixWalk w;
-    const int2 at_s = prefix_at;
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, shared_wait(bar, parity, &dead)); };
+    // the n-th stretch of the prefix's share, or one without pages behind the last; and this warp's word that it has done with it
+    auto hear = [&](int n) {
+        ok = ok && wait(&told_full[n % SH_TOLD], n / SH_TOLD & 1);
+        SharedStretch w = told[n % SH_TOLD];
+        if (!ok) w.pages = 0;
+        return w;
+    };
+    auto heard = [&](int n) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&told_empty[n % SH_TOLD]);
+    };
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SH_REGS_ISSUE));
-        if (warp == 0) {
-            // ---------------- copies of the prefix: a page's keys, and the values of the page two ahead of it, which are needed that much later.  (Never a circle: keys wait for
-            // products of keys STAGES pages back, which wait for products of values further back than those that are copied behind them.)
-            w.start(p, gr, prefix_f, prefix_end, at_s.x, at_s.y);
-            const uint64_t pol = policy_evict_first();
-            SharedPhases k_phases, v_phases;
-            int it = 0;
-            const uint8_t* wait_v[C::AHEAD];                                 // pages whose values are still to be asked for (null: not there), and their sets
-            int wait_set[C::AHEAD];
-            auto ask = [&](SharedPhases& phases, uint64_t* full, uint64_t* empty, int n, int set, const uint8_t* from, uint8_t* to, int tokens) {
-                const int s = n % C::STAGES;
-                ok = ok && mbar_wait_limited(&empty[s], (n / C::STAGES & 1) ^ 1, &dead);
-                if (!ok) return;
-                phases.next(C::STAGES, s, set);
-                if (tokens >= 0) tokens_s[n % C::TOKENS] = tokens;           // (keys are copied when those STAGES back have been multiplied, which is when the scores of eight back were read)
-                if (from) {
-                    mbar_expect_tx(&full[phases.at], C::SLAB);
-                    tma_bulk_g2s(to + s * C::SLAB, from, C::SLAB, &full[phases.at], pol);
-                } else {
-                    mbar_arrive(&full[phases.at]);
-                }
-            };
-            auto values = [&](const uint8_t* page, int set) { ask(v_phases, v_full, v_empty, it - C::AHEAD, set, page ? page + C::SLAB : nullptr, smem + C::KV + C::STAGES * C::SLAB, -1); };
-#pragma unroll 1
-            while (w.next(p, gr)) {
-                const int p1 = w.p0 + w.pages, row = p.row_of(w.w.seq0);
-#pragma unroll 1
-                for (int p0 = w.p0; p0 < p1; p0 += 32) {
-                    const int tile = p0 + lane;
-                    int my_page = tile < p1 && row >= 0 ? p.page_table[(size_t)row * p.max_pages + tile] : -1;
-                    if (my_page >= p.num_pages) my_page = -1;
-                    const int n = min(32, p1 - p0);
-#pragma unroll 1
-                    for (int k = 0; k < n; ++k) {
-                        const int page = __shfl_sync(0xffffffffu, my_page, k);
-                        if (lane == 0) {
-                            const uint8_t* from = page >= 0 ? p.cache + ((size_t)page * p.nkv + w.h) * C::TILE : nullptr;
-                            const int set = w.few ? (p0 + k - w.p0) & 1 : 2;
-                            ask(k_phases, k_full, k_empty, it, set, from, smem + C::KV, page >= 0 ? min(kKvTile, w.w.tokens - (p0 + k) * kKvTile) : 0);
-                            if (it >= C::AHEAD) values(wait_v[0], wait_set[0]);
-                            wait_v[0] = wait_v[1], wait_set[0] = wait_set[1];
-                            wait_v[1] = from, wait_set[1] = set;
-                        }
-                        ++it;
-                    }
-                }
-            }
+        if (warp == 3) {
+            // ---------------- the walk
             if (lane == 0) {
-                for (int i = 0; i < C::AHEAD; ++i, ++it)
-                    if (it >= C::AHEAD) values(wait_v[i], wait_set[i]);
-                for (int i = 0; i < 3 * C::STAGES; ++i)                      // nothing may still be on its way into this CTA's memory when it ends
-                    for (int k = 0; k < kWaitLimit && !(mbar_try_wait(&k_full[i], (k_phases.bits >> i & 1) ^ 1) && mbar_try_wait(&v_full[i], (v_phases.bits >> i & 1) ^ 1)); ++k) {}
+                PrefixWalk w;
+                w.start(p, gr, prefix_f, prefix_end, prefix_at.x, prefix_at.y);
+#pragma unroll 1
+                for (int n = 0, more = 1; more; ++n) {
+                    more = w.next(p, gr);
+                    if (!shared_wait(&told_empty[n % SH_TOLD], (n / SH_TOLD & 1) ^ 1, &dead)) break;
+                    SharedStretch s{};
+                    if (more) s = w.stretch(p, prefix_per);
+                    told[n % SH_TOLD] = s;
+                    mbar_arrive(&told_full[n % SH_TOLD]);
+                }
             }
             __syncwarp();
-        } else if (warp < 3) {
+        } else if (warp == 0) {
+            // ---------------- copies of the prefix: a page's keys, and the values of the page two ahead of it, which are needed that much later.  (Never a circle: keys wait for
+            // products of keys STAGES pages back, which wait for products of values further back than those that are copied behind them.)
+            const uint64_t pol = policy_evict_first();
+            SharedPhases phases[2];                                          // keys, values
+            int n = 0, it = 0, k = 0, k1 = 0, my_page = -1, row = -1;        // stretches heard, pages asked for; of the 32 at hand: the next, how many
+            const uint8_t* v_from[C::AHEAD];                                 // pages whose values are still to be asked for (null: not there), and their sets
+            int v_set[C::AHEAD];
+            SharedStretch w;
+            w.pages = 0;
+            int p0 = 0, p1 = 0;                                              // pages of the stretch that are not at hand yet
+            bool more = true;
+#pragma unroll 1
+            for (int drain = 0; drain < C::AHEAD; ++it) {
+                if (more && k == k1) {
+                    if (p0 == p1) {
+                        if (n) heard(n - 1);
+                        w = hear(n++);
+                        more = w.pages != 0;
+                        p0 = w.p0;
+                        p1 = p0 + w.pages;
+                        row = more ? p.row_of(w.seq0) : -1;
+                    }
+                    my_page = p0 + lane < p1 && row >= 0 ? p.page_table[(size_t)row * p.max_pages + p0 + lane] : -1;
+                    if (my_page >= p.num_pages) my_page = -1;
+                    k = 0;
+                    k1 = min(32, p1 - p0);
+                    p0 += k1;
+                }
+                if (!more) ++drain;
+                const int page = __shfl_sync(0xffffffffu, my_page, k), tile = p0 - k1 + k;
+                if (lane == 0) {
+                    const uint8_t* from[2] = {page >= 0 ? p.cache + ((size_t)page * p.nkv + w.h) * C::TILE : nullptr, v_from[0]};
+                    const int set[2] = {w.few ? (tile - w.p0) & 1 : 2, v_set[0]};
+#pragma unroll
+                    for (int i = 0; i < C::AHEAD; ++i) {
+                        v_from[i] = i + 1 < C::AHEAD ? v_from[i + 1] : from[0] ? from[0] + C::SLAB : nullptr;
+                        v_set[i] = i + 1 < C::AHEAD ? v_set[i + 1] : set[0];
+                    }
+#pragma unroll
+                    for (int kind = 0; kind < 2; ++kind) {
+                        if (kind ? it < C::AHEAD : !more) continue;
+                        const int i = it - kind * C::AHEAD, s = i % C::STAGES;
+                        ok = ok && shared_wait(kind ? &v_empty[s] : &k_empty[s], (i / C::STAGES & 1) ^ 1, &dead);
+                        if (!ok) continue;
+                        phases[kind].next(C::STAGES, s, set[kind]);
+                        uint64_t* const full = (kind ? v_full : k_full) + phases[kind].at;
+                        // (keys are copied when those STAGES back have been multiplied, which is when the scores of eight back were read)
+                        if (kind == 0) tokens_s[i % C::TOKENS] = page >= 0 ? min(kKvTile, w.tokens - tile * kKvTile) : 0;
+                        if (from[kind]) {
+                            mbar_expect_tx(full, C::SLAB);
+                            tma_bulk_g2s(smem + C::KV + (kind * C::STAGES + s) * C::SLAB, from[kind], C::SLAB, full, pol);
+                        } else {
+                            mbar_arrive(full);
+                        }
+                    }
+                }
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                if (more) ++k;
+            }
+            if (lane == 0)
+#pragma unroll 1
+                for (int i = 0; i < 6 * C::STAGES; ++i) {                    // nothing may still be on its way into this CTA's memory when it ends
+                    const int kind = i >= 3 * C::STAGES, x = i - kind * 3 * C::STAGES;
+#pragma unroll 1
+                    for (int j = 0; j < kWaitLimit && !mbar_try_wait((kind ? v_full : k_full) + x, (phases[kind].bits >> x & 1) ^ 1); ++j) {}
+                }
+            __syncwarp();
+        } else {
             // ---------------- products, one warp a half
             constexpr uint32_t idesc_qk = umma_idesc_f16(kSharedRows, kKvTile, false), idesc_pv = umma_idesc_f16(kSharedRows, D, true);
             const int h = warp - 1;
-            w.start(p, gr, prefix_f, prefix_end, at_s.x, at_s.y);
-            if (elect_one()) {
+            const bool lead = elect_one();
+            {
                 const uint64_t q_desc = umma_desc_k128(smem_u32(smem + h * KH * C::QBLK)), k_desc = umma_desc_k128(smem_u32(smem + C::KV)),
                                v_desc = umma_desc_mn128(smem_u32(smem + C::KV + C::STAGES * C::SLAB));
                 const uint32_t s_at = tmem + C::COL_S + h * 128, o_at = tmem + C::COL_O + h * D;
@@ -543,7 +590,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
                 auto issue_qk = [&](int page, bool alone) {                  // page: counted over the whole share; alone: the other half has no use for it
                     const int s = page % C::STAGES, buf = n_qk & 1;
                     const uint32_t parity = k_phases.next(C::STAGES, s, alone ? h : 2);
-                    ok = mbar_wait_limited(&k_full[k_phases.at], parity, &dead);
+                    ok = shared_wait(&k_full[k_phases.at], parity, &dead);
                     if (!ok) return;
                     ++n_qk;
                     tc_fence_after();
@@ -559,7 +606,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
                 auto issue_pv = [&](int page, bool first, bool alone) {
                     const int s = page % C::STAGES, buf = n_pv & 1;
                     const uint32_t parity = v_phases.next(C::STAGES, s, alone ? h : 2);
-                    ok = mbar_wait_limited(&v_full[v_phases.at], parity, &dead) && mbar_wait_limited(&p_full[h][buf], n_pv >> 1 & 1, &dead);
+                    ok = shared_wait(&v_full[v_phases.at], parity, &dead) && shared_wait(&p_full[h][buf], n_pv >> 1 & 1, &dead);
                     if (!ok) return;
                     ++n_pv;
                     tc_fence_after();
@@ -571,11 +618,13 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
                     if (alone) umma_commit(&v_empty[s]);
                 };
 #pragma unroll 1
-                while (w.next(p, gr)) {
+                for (int n = 0;; ++n) {
+                    const SharedStretch w = hear(n);
+                    if (w.pages == 0) break;
                     const int mine = w.of_half(h);
                     auto page_of = [&](int i) { return base + (w.few ? h + 2 * i : i); };      // page i of this half
-                    if (ok && mine) {
-                        ok = mbar_wait_limited(&q_full[h], n_q++ & 1, &dead);
+                    if (lead && ok && mine) {
+                        ok = shared_wait(&q_full[h], n_q & 1, &dead);
                         tc_fence_after();
                         // Scores run two pages ahead, issued behind the product that reads the probabilities in their buffer
 #pragma unroll 1
@@ -584,42 +633,47 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
                             if (ok && i + 2 < mine) issue_qk(page_of(i + 2), w.few);
                         }
                     }
+                    if (mine) ++n_q;
                     base += w.pages;
+                    ok = __all_sync(0xffffffffu, ok);
+                    heard(n);
                 }
-                umma_commit(&drained[h]);                                    // nothing may still run in tensor memory when it is given back, whoever gave up
+                if (lead) {
+                    umma_commit(&drained[h]);                                // nothing may still run in tensor memory when it is given back, whoever gave up
 #pragma unroll 1
-                for (int k = 0; k < kWaitLimit && !mbar_try_wait(&drained[h], 0); ++k) {}
+                    for (int k = 0; k < kWaitLimit && !mbar_try_wait(&drained[h], 0); ++k) {}
+                }
             }
             __syncwarp();
         }
     } else if (warp < 12) {
         // ---------------- softmax: one thread a row
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SH_REGS_SOFT));
-        w.start(p, gr, prefix_f, prefix_end, at_s.x, at_s.y);
         const int h = (warp - 4) >> 2;
         const int row = (tid - 128) & 127;                                           // lane of tensor memory: warp % 4 is the quarter that a warp may read
-        const int tok = row / p.G;
+        const int tok = row * p.inv_g >> 16;
         const uint32_t lanes = tmem + ((uint32_t)(row & 96) << 16);
         const uint32_t s_at0 = lanes + C::COL_S + h * 128, o_at = lanes + C::COL_O + h * D;
         SharedPhases phases;
         int base = 0, cnt = 0;                                               // pages of the share, pages of this half so far
         // maxima and sums of a half, where its queries were: the products that read those have retired
         auto ml_of = [&](int half) { return reinterpret_cast<float2*>(smem + half * KH * C::QBLK); };
-        auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_limited(bar, parity, &dead)); };
 #pragma unroll 1
-        while (w.next(p, gr)) {
+        for (int seg = 0;; ++seg) {
+            const SharedStretch w = hear(seg);
+            if (w.pages == 0) break;
             const int mine = w.of_half(h);
             const int tok0 = w.few ? 0 : h * p.th;                           // of the tile
             const bool valid = tok < p.th && tok0 + tok < w.n;
-            const int i0 = w.tile * 2 * p.th + tok0;                         // of the group
             if (mine) {
                 // the queries, 16 bytes at a time, zeros for rows without one (the products that read the last stretch's have retired: their scores were here)
                 constexpr int CH = D / 8;
+                const int c = row % CH;
 #pragma unroll 4
-                for (int k = row; k < kSharedRows * CH; k += kSharedRows) {
-                    const int c = k % CH, r = k / CH, tk = r / p.G, head = r - tk * p.G;
+                for (int r = row / CH; r < kSharedRows; r += kSharedRows / CH) {
+                    const int tk = r * p.inv_g >> 16, head = r - tk * p.G;
                     const bool on = tk < p.th && tok0 + tk < w.n;
-                    const __half* from = p.q + ((size_t)(w.w.seq0 + i0 + (on ? tk : 0)) * p.nq + (size_t)w.h * p.G + (on ? head : 0)) * D + c * 8;
+                    const __half* from = p.q + ((size_t)(w.q0 + tok0 + (on ? tk : 0)) * p.nq + (size_t)w.h * p.G + (on ? head : 0)) * D + c * 8;
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem + (h * KH + (c >> 3)) * C::QBLK + r * 128 + ((c & 7) ^ (r & 7)) * 16)), "l"(from),
                                  "r"(on ? 16 : 0)
                                  : "memory");
@@ -712,10 +766,10 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
                 l_run = NAN;
                 m_ref = 0.f;
             }
-            const int row0 = w.w.row(p, w.h, i0);
+            const int row0 = w.row0 + tok0 * p.G;
             const size_t at = (size_t)row0 + (size_t)2 * kSharedRows * blockIdx.x + row;
             if (w.p0 == 0 && valid && row == tok * p.G && (!w.few || h == 0))        // the unit begins here: where each of its queries' results will be
-                p.prefix_units[(size_t)(w.w.seq0 + i0 + tok) * p.nkv + w.h] = make_int4(blockIdx.x, (int)((unsigned)(w.unit_f + w.steps - 1) / (unsigned)prefix_per), row0 + row, 0);
+                p.prefix_units[(size_t)(w.q0 + tok0 + tok) * p.nkv + w.h] = make_int4(blockIdx.x, w.last, row0 + row, 0);
             float z = 1.f, zo = 0.f, m = m_ref, l = l_run;
             if (w.few) {                                                     // the halves' results as one: each half puts half of the dims together
                 ml_of(h)[row] = make_float2(m_ref, l_run);
@@ -755,6 +809,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
                 asm volatile("bar.sync 1, %0;" ::"n"(SH_SOFT) : "memory");
             }
             base += w.pages;
+            heard(seg);
         }
         tmem_st_wait();
     } else {
@@ -775,9 +830,9 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
 }
 
 // ------------------------------------------------------------------ all parts of a (sequence, key head) as one
-constexpr int SM_THREADS = 256;
+constexpr int SM_THREADS = 256, SM_PARTS = 5;    // parts that a thread asks for at once
 template <int D>
-__global__ void __launch_bounds__(SM_THREADS)
+__global__ void __launch_bounds__(SM_THREADS, 4)
 shared_merge_kernel(const __grid_constant__ SharedArgs p) {
     pdl_wait();
     __shared__ __align__(16) float acc_s[SM_THREADS * 4];
@@ -786,7 +841,6 @@ shared_merge_kernel(const __grid_constant__ SharedArgs p) {
     const int4 own = p.own_units[unit];
     int4 pre = make_int4(0, -1, 0, 0);
     if (p.n_groups) pre = p.prefix_units[unit];
-    if (own.x < 0) return;
     if (!own.z) pre = make_int4(0, -1, 0, 0);                                // (then nobody has written there)
     // a thread has four dims of a head (neighbours the same of neighbouring heads, as the prefix's results lie), and every `lanes`-th part
     const int size = G * D / 4, lanes = SM_THREADS / size, e = threadIdx.x % size, mine = threadIdx.x / size, hg = e % G, dim = e / G * 4;
@@ -794,11 +848,13 @@ shared_merge_kernel(const __grid_constant__ SharedArgs p) {
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float M = -INFINITY, L = 0.f;
     if (mine < lanes) {
-        for (int k0 = mine; k0 < n; k0 += 4 * lanes) {
-            float4 o[4];
-            float2 ml[4];
+#pragma unroll 1
+        for (int k0 = mine; k0 < n; k0 += SM_PARTS * lanes) {
+            float4 o[SM_PARTS];
+            float2 ml[SM_PARTS];
+            float Mn = M;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {                                    // four parts asked for at once
+            for (int u = 0; u < SM_PARTS; ++u) {
                 const int k = k0 + u * lanes;
                 ml[u] = make_float2(-INFINITY, 0.f);
                 o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -812,12 +868,13 @@ shared_merge_kernel(const __grid_constant__ SharedArgs p) {
                     ml[u] = __ldcg(p.rows_ml + at);
                 }
             }
-            const float Mn = fmaxf(fmaxf(M, ml[0].x), fmaxf(ml[1].x, fmaxf(ml[2].x, ml[3].x)));
+#pragma unroll
+            for (int u = 0; u < SM_PARTS; ++u) Mn = fmaxf(Mn, ml[u].x);
             const float keep = M == -INFINITY ? 0.f : exp2f(M - Mn);
             L *= keep;
             acc.x *= keep, acc.y *= keep, acc.z *= keep, acc.w *= keep;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
+            for (int u = 0; u < SM_PARTS; ++u) {
                 const float z = ml[u].x == -INFINITY ? 0.f : exp2f(ml[u].x - Mn);
                 L = fmaf(ml[u].y, z, L);
                 acc = fma_f4(o[u], make_float4(z, z, z, z), acc);
@@ -829,9 +886,11 @@ shared_merge_kernel(const __grid_constant__ SharedArgs p) {
     }
     __syncthreads();
     if (mine) return;
+#pragma unroll 1
     for (int x = 1; x < lanes; ++x) M = fmaxf(M, ml_s[x * size + e].x);
     acc = make_float4(0.f, 0.f, 0.f, 0.f);
     L = 0.f;
+#pragma unroll 1
     for (int x = 0; x < lanes; ++x) {
         const float2 ml = ml_s[x * size + e];
         const float z = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
@@ -879,7 +938,7 @@ static int launch_shared(SharedArgs& p, cudaStream_t st) {
         FT_REQUIRE(a.numRegs >= SH_REGS, "ft_attn_decode_shared: built with %d registers a thread, its warps share out %d", a.numRegs, SH_REGS);
         attr_set.mark();
     }
-    p.chunk = C::CHUNK;
+    p.chunk_log = C::CHUNK == 64 ? 6 : 5;
     FT_CHECK_CUDA(launch_after(shared_attn_kernel<D>, dim3(device_sms()), dim3(SH_THREADS), C::SMEM, st, (const SharedArgs&)p));
     FT_CHECK_CUDA(launch_after(shared_merge_kernel<D>, dim3(p.B * p.nkv), dim3(SM_THREADS), 0, st, (const SharedArgs&)p));
     return 0;
@@ -921,6 +980,6 @@ extern "C" int ft_attn_decode_shared(const void* q, const void* kv_layer, int nu
     uint8_t* w = (uint8_t*)scratch;
     SharedArgs p{(const __half*)q, (const uint8_t*)kv_layer, page_table, req_slot, ctx_lens, group_start, shared_lens, (__nv_bfloat16*)out, (__nv_bfloat16*)out_lo,
                  (int4*)(w + l.own_units), (int4*)(w + l.prefix_units), (float*)(w + l.own_parts), (float*)(w + l.rows_o), (float2*)(w + l.rows_ml), B, n_groups, num_pages, table_rows,
-                 max_pages, nq, nkv, G, th, (int)l.rows, 0, kSharedLog2E / sqrtf((float)d)};
+                 max_pages, nq, nkv, G, th, (int)l.rows, 0, (65536u + G - 1) / G, kSharedLog2E / sqrtf((float)d)};
     return d == 64 ? launch_shared<64>(p, (cudaStream_t)stream) : launch_shared<128>(p, (cudaStream_t)stream);
 }

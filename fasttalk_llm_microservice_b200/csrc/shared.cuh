@@ -20,14 +20,15 @@ struct SharedArgs {
     const uint8_t* cache;
     const int *page_table, *req_slot, *ctx_lens, *group_start, *shared_lens;
     __nv_bfloat16 *out, *out_lo;
-    int4 *own_units, *prefix_units;              // [B][nkv]: first and last warp that has a part, whether there is a prefix part (below 0: the output is written);
+    int4 *own_units, *prefix_units;              // [B][nkv]: first and last warp that has a part, whether there is a prefix part;
                                                  //           first and last CTA that has a part, its row among the results
     float* own_parts;                            // [unit + warp][G][D], then (m, l)
     float* rows_o;                               // prefix results: O [D / 4][row + 256 CTA][4], (m, l)
     float2* rows_ml;
     int B, n_groups, num_pages, table_rows, max_pages, nq, nkv, G, th;        // th: queries of a half
     int rows;                                    // of the prefix's results
-    int chunk;                                   // tokens of an own step: 64 or 32
+    int chunk_log;                               // tokens of an own step: 2^6 or 2^5
+    unsigned inv_g;                              // row / G = row * inv_g >> 16 for a half's rows
     float scale_log2;
 
     __host__ __device__ __forceinline__ int reach() const { return max_pages * kKvTile; }
@@ -41,6 +42,9 @@ struct SharedArgs {
 struct SharedGroups {
     const int *start, *lens;
     int n;
+    __host__ __device__ __forceinline__ int tokens(const SharedArgs& p, int g) const { return max(0, min(lens[g], p.reach())); }
+    // whether group g has a prefix part
+    __host__ __device__ __forceinline__ bool pays(const SharedArgs& p, int g) const { return start[g + 1] - start[g] >= 2 && tokens(p, g) >= 2 * kKvTile; }
     // the last group that begins at or before b (those without queries begin where the next one does), or -1
     __host__ __device__ __forceinline__ int of(int b) const {
         int lo = -1, hi = n - 1;
@@ -58,9 +62,9 @@ struct SharedPrefix {
     __host__ __device__ __forceinline__ void load(const SharedArgs& p, const SharedGroups& gr, int g) {
         seq0 = gr.start[g];
         size = gr.start[g + 1] - seq0;
-        tokens = max(0, min(gr.lens[g], p.reach()));
-        pages = size >= 2 && tokens >= 2 * kKvTile ? (tokens + kKvTile - 1) / kKvTile : 0;
-        tiles = (size + 2 * p.th - 1) / (2 * p.th);
+        tokens = gr.tokens(p, g);
+        pages = gr.pays(p, g) ? (tokens + kKvTile - 1) / kKvTile : 0;
+        tiles = pages ? (int)((unsigned)(size + 2 * p.th - 1) / (unsigned)(2 * p.th)) : 0;
     }
     __host__ __device__ __forceinline__ int queries(const SharedArgs& p, int tile) const { return min(2 * p.th, size - tile * 2 * p.th); }
     // steps of a tile of n queries: where they fill one half only, each half takes every other page
@@ -77,30 +81,36 @@ struct SharedSeq {
     int ctx, begin, lead, steps, first;          // first: the query whose row has the shared pages
     bool prefix;                                 // a prefix part is added
     __host__ __device__ __forceinline__ void load(const SharedArgs& p, const SharedGroups& gr, int b, int ctx_len) {
+        const int up = (1 << p.chunk_log) - 1;
         ctx = max(0, min(ctx_len, p.reach()));
         begin = lead = 0;
         first = -1;
         prefix = false;
         const int g = gr.of(b);
         if (g >= 0 && b < gr.start[g + 1]) {
-            SharedPrefix w;
-            w.load(p, gr, g);
-            begin = w.tokens;
-            first = w.seq0;
-            prefix = w.pages > 0 && ctx >= begin;
-            if (!prefix) lead = (min(begin, ctx) + p.chunk - 1) / p.chunk;
+            begin = gr.tokens(p, g);
+            first = gr.start[g];
+            prefix = ctx >= begin && gr.pays(p, g);
+            if (!prefix) lead = min(begin, ctx) + up >> p.chunk_log;
         }
-        const int own = ctx > begin ? (ctx + p.chunk - 1) / p.chunk - begin / p.chunk : 0;
+        const int own = ctx > begin ? (ctx + up >> p.chunk_log) - (begin >> p.chunk_log) : 0;
         steps = max(1, lead + own);
     }
     // tokens lo .. hi - 1 that step t reads (none: lo >= hi); true: on the first row's pages
     __host__ __device__ __forceinline__ bool step(const SharedArgs& p, int t, int& lo, int& hi) const {
         const bool led = t < lead;
-        const int tile = led ? t : begin / p.chunk + t - lead;
-        lo = max(tile * p.chunk, led ? 0 : begin);
-        hi = min(tile * p.chunk + p.chunk, led ? min(begin, ctx) : ctx);
+        const int at = (led ? t : (begin >> p.chunk_log) + t - lead) << p.chunk_log;
+        lo = max(at, led ? 0 : begin);
+        hi = min(at + (1 << p.chunk_log), led ? min(begin, ctx) : ctx);
         return led;
     }
+};
+
+// n queries from q0 on, over pages p0 .. of the row of query seq0; row0: where the first one's results lie; last: the last share that the unit lies in
+struct SharedStretch {
+    int p0, pages, n, h, seq0, q0, row0, tokens, last;
+    bool few;                                    // the queries fill one half only
+    __host__ __device__ __forceinline__ int of_half(int half) const { return few ? (pages - half + 1) / 2 : pages; }      // its pages
 };
 
 // A CTA's share of the prefix list, walked stretch by stretch; a stretch = pages p0 .. p0 + pages - 1 of one unit
@@ -158,7 +168,17 @@ struct PrefixWalk {
             }                                    // else all of it was behind the unit's last step
         }
     }
-    __host__ __device__ __forceinline__ int of_half(int half) const { return few ? (pages - half + 1) / 2 : pages; }      // its pages
+    // the stretch as the other warps get it; per: steps of a share
+    __host__ __device__ __forceinline__ SharedStretch stretch(const SharedArgs& p, int per) const {
+        SharedStretch s;
+        s.p0 = p0, s.pages = pages, s.few = few, s.n = n, s.h = h;
+        s.seq0 = w.seq0;
+        s.q0 = w.seq0 + tile * 2 * p.th;
+        s.row0 = w.row(p, h, tile * 2 * p.th);
+        s.tokens = w.tokens;
+        s.last = (int)((unsigned)(unit_f + steps - 1) / (unsigned)per);
+        return s;
+    }
 };
 
 }  // namespace ft
