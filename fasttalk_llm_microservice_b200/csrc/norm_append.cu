@@ -2,20 +2,19 @@
 //   y = x * rsqrt(mean(x^2) + eps) * gain   per head of d,   then pairs (a, b) -> (a cos - b sin, b cos + a sin);   q to q_out, k and v to the paged fp16 cache.
 // Pairs are (i, i + rotated / 2) or neighbours (2 i, 2 i + 1); dims from `rotated` on stay as they are.
 //
-// A head belongs to D / (2 E) lanes (E numbers are 16 bytes of the input), each with two chunks of E, chosen so that both numbers of a pair lie in one lane: whatever
-// `rotated` is, lane j's chunks are j and j + rotated / (2 E), and those behind `rotated` follow two by two.  So the only exchange is the sum of squares, and a chunk of
-// eight fp16 results is one 16-byte store, a chunk of a row in the cache.
+// A head belongs to d / 8 lanes, each with two chunks of four numbers, chosen so that both numbers of a pair lie in one lane (lane j's chunks are j and j + rotated / 8, and
+// those behind `rotated` are shared out the same way) and neighbouring lanes have neighbouring chunks.  So the only exchange is the sum of squares, and a load or store
+// of the warp takes whole lines.  The factor rsqrt(..) is the same for a head, so it comes last: gain and rotation do not wait for the sum.
 #include "common.cuh"
 #include "ft_internal.h"
 
 namespace ft {
 
 constexpr int NA_WARPS = 4, NA_THREADS = NA_WARPS * 32;
-
-template <class T> struct NaType;
-template <> struct NaType<float> { static constexpr int E = 4; };
-template <> struct NaType<__half> { static constexpr int E = 8; };
-template <> struct NaType<__nv_bfloat16> { static constexpr int E = 8; };
+constexpr int NA_AHEAD = 2;                          // passes whose reads are on their way together
+constexpr int NA_FILL = 40;                          // warps per SM from which a warp takes more than one pass of a token
+constexpr int NA_E = 4;
+constexpr int NA_CTAS = 5;                           // per SM
 
 struct NormAppend {
     const void* x;
@@ -24,10 +23,9 @@ struct NormAppend {
     const int *positions, *kv_slots;
     __half* q_out;
     uint8_t* kv_layer;
-    long long slots;                                 // pages * 64
+    int slots;                                       // pages * 64
     int parts, T, nq, nkv, n_angles, rotated, gain_q_stride, gain_k_stride;      // gain strides: 0 = one gain for all heads
     int passes, per, per_token;                      // passes of a token (a warp's heads each), of a warp; warps of a token
-    int wide;                                        // 1: 16-byte loads
     float eps;
 };
 
@@ -35,161 +33,184 @@ __device__ __forceinline__ float na_float(float v) { return v; }
 __device__ __forceinline__ float na_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float na_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-template <class T>
-__device__ __forceinline__ void na_load(const T* p, float* v, bool wide) {
-    constexpr int E = NaType<T>::E;
-    alignas(16) T raw[E];
-    if (wide) {
-        *reinterpret_cast<uint4*>(raw) = __ldcg(reinterpret_cast<const uint4*>(p));
+// four numbers as they lie in memory
+template <class T> struct NaRaw { typedef uint2 type; };
+template <> struct NaRaw<float> { typedef uint4 type; };
+template <class T, bool WIDE>
+__device__ __forceinline__ typename NaRaw<T>::type na_load(const T* p) {     // WIDE: a chunk is one load
+    typedef typename NaRaw<T>::type Raw;
+    alignas(16) T raw[NA_E];
+    if (WIDE) {
+        *reinterpret_cast<Raw*>(raw) = __ldcs(reinterpret_cast<const Raw*>(p));      // read once
     } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e) raw[e] = p[e];
+        for (int e = 0; e < NA_E; ++e) raw[e] = p[e];
     }
-#pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = na_float(raw[e]);
-}
-template <int E>
-__device__ __forceinline__ void na_load_f32(const float* p, float* v) {
-#pragma unroll
-    for (int e = 0; e < E; e += 4) {
-        const float4 w = *reinterpret_cast<const float4*>(p + e);
-        v[e] = w.x; v[e + 1] = w.y; v[e + 2] = w.z; v[e + 3] = w.w;
-    }
+    return *reinterpret_cast<const Raw*>(raw);
 }
 // within fp16's range, NaN as it is
-__device__ __forceinline__ __half2 na_half2(float a, float b) {
-    a = a != a ? a : fminf(fmaxf(a, -65504.f), 65504.f);
-    b = b != b ? b : fminf(fmaxf(b, -65504.f), 65504.f);
-    return __floats2half2_rn(a, b);
+__device__ __forceinline__ uint32_t na_half2(float a, float b) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
 }
 
-template <int D, class T, bool NEIGHBOURS>
-__global__ void __launch_bounds__(NA_THREADS)
+template <int D, class T, bool NEIGHBOURS, bool WIDE>
+__global__ void __launch_bounds__(NA_THREADS, NA_CTAS)
 norm_append_kernel(const __grid_constant__ NormAppend p) {
     pdl_wait();
-    constexpr int E = NaType<T>::E, LANES = D / (2 * E), HEADS = 32 / LANES;      // lanes of a head, heads of a pass
+    constexpr int E = NA_E, LANES = D / (2 * E), HEADS = 32 / LANES;         // lanes of a head, heads of a pass
+    typedef typename NaRaw<T>::type Raw;
     const int warp = blockIdx.x * NA_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int t = warp / p.per_token;
     if (t >= p.T) return;
     const int heads = p.nq + 2 * p.nkv, sub = lane / LANES, j = lane % LANES;
-    const int turned = p.rotated / (2 * E);          // lanes of a head that rotate
-    // chunks of this lane; behind the rotated ones they follow two by two
-    int c0, c1;
-    if (NEIGHBOURS) c0 = 2 * j, c1 = 2 * j + 1;
-    else if (j < turned) c0 = j, c1 = j + turned;
-    else c0 = 2 * j, c1 = 2 * j + 1;
-    const int pos = p.positions[t];
-    const long long slot = p.kv_slots[t];
+    const int turned = p.rotated / (2 * E);          // lanes of a head that rotate, where pairs are halves
+    const int c0 = !NEIGHBOURS && j >= turned ? turned + j : j, c1 = !NEIGHBOURS && j < turned ? j + turned : j + LANES;
+    const int p0 = (warp - t * p.per_token) * p.per, p1 = min(p0 + p.per, p.passes);
+    const T* const row = (const T*)p.x + (long long)t * p.row_stride + sub * D;
+    Raw raw[NA_AHEAD][2];
+    auto ask = [&](int u, int first, int s) {        // pass first + u, part s
+        if (first + u < p1 && (first + u) * HEADS + sub < heads) {
+            const T* from = row + s * p.part_stride + (long long)(first + u) * (HEADS * D);
+            raw[u][0] = na_load<T, WIDE>(from + c0 * E);
+            raw[u][1] = na_load<T, WIDE>(from + c1 * E);
+        } else {
+            raw[u][0] = raw[u][1] = Raw{};
+        }
+    };
+#pragma unroll
+    for (int u = 0; u < NA_AHEAD; ++u) ask(u, p0, 0);
+    const int pos = p.positions[t], slot = p.kv_slots[t];
     const bool known = pos >= 0 && (p.rotated == 0 || pos < p.n_angles);
     const bool kept = known && slot >= 0 && slot < p.slots;
-    float cs[E], sn[E];                              // halves: of chunk c0's numbers; neighbours: of c0's pairs, then of c1's
-    const bool rotates = known && (NEIGHBOURS ? j * 2 * E < p.rotated : j < turned);
-    if (rotates) {
-        const float* at = p.cos_t + (size_t)pos * (p.rotated / 2) + j * E;
-        na_load_f32<E>(at, cs);
-        na_load_f32<E>(p.sin_t + (at - p.cos_t), sn);
-    }
-    const int p0 = (warp - t * p.per_token) * p.per, p1 = min(p0 + p.per, p.passes);
-    for (int pass = p0; pass < p1; ++pass) {
-        const int hd = pass * HEADS + sub;
-        const bool on = hd < heads;
-        float v[2][E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) v[0][e] = v[1][e] = 0.f;
-        if (on) {
-            const T* row = (const T*)p.x + (long long)t * p.row_stride + (long long)hd * D;
-            na_load<T>(row + c0 * E, v[0], p.wide);
-            na_load<T>(row + c1 * E, v[1], p.wide);
-            for (int s = 1; s < p.parts; ++s) {
-                float w[2][E];
-                na_load<T>(row + s * p.part_stride + c0 * E, w[0], p.wide);
-                na_load<T>(row + s * p.part_stride + c1 * E, w[1], p.wide);
-#pragma unroll
-                for (int e = 0; e < E; ++e) v[0][e] += w[0][e], v[1][e] += w[1][e];
+    // angles: halves, of chunk c0's numbers; neighbours, of c0's pairs and then of c1's.  Chunks that do not rotate: 1 and 0
+    float cs[E] = {1.f, 1.f, 1.f, 1.f}, sn[E] = {0.f, 0.f, 0.f, 0.f};
+    {
+        const size_t at = (size_t)pos * (p.rotated / 2);
+        if (NEIGHBOURS) {
+            if (known && c0 * E < p.rotated) {
+                *reinterpret_cast<float2*>(cs) = *reinterpret_cast<const float2*>(p.cos_t + at + c0 * (E / 2));
+                *reinterpret_cast<float2*>(sn) = *reinterpret_cast<const float2*>(p.sin_t + at + c0 * (E / 2));
             }
+            if (known && c1 * E < p.rotated) {
+                *reinterpret_cast<float2*>(cs + 2) = *reinterpret_cast<const float2*>(p.cos_t + at + c1 * (E / 2));
+                *reinterpret_cast<float2*>(sn + 2) = *reinterpret_cast<const float2*>(p.sin_t + at + c1 * (E / 2));
+            }
+        } else if (known && j < turned) {
+            *reinterpret_cast<float4*>(cs) = load_f4(p.cos_t + at + c0 * E);
+            *reinterpret_cast<float4*>(sn) = load_f4(p.sin_t + at + c0 * E);
         }
-        float ss = 0.f;
+    }
+    uint8_t* const cache = p.kv_layer + ((size_t)(slot / kKvTile) * p.nkv * 2) * (size_t)(kKvTile * D * 2);
+    const int in0 = kv_swizzled_chunk<D>(slot % kKvTile, c0 / 2) + c0 % 2 * 8, in1 = kv_swizzled_chunk<D>(slot % kKvTile, c1 / 2) + c1 % 2 * 8;      // of a page's head
+    const float* have = nullptr;                     // the gain that is in g
+    float g[2][E];
+#pragma unroll 1
+    for (int first = p0; first < p1; first += NA_AHEAD) {
+        float v[NA_AHEAD][2][E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) ss = fmaf(v[0][e], v[0][e], fmaf(v[1][e], v[1][e], ss));
+        for (int u = 0; u < NA_AHEAD; ++u)
 #pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (!on) continue;
-        if (hd < p.nq + p.nkv) {
-            const float r = rsqrtf(ss * (1.f / D) + p.eps);
-            const float* gain = hd < p.nq ? p.q_gain : p.k_gain;
-            if (gain) {
-                gain += hd < p.nq ? hd * p.gain_q_stride : (hd - p.nq) * p.gain_k_stride;
-                float g0[E], g1[E];
-                na_load_f32<E>(gain + c0 * E, g0);
-                na_load_f32<E>(gain + c1 * E, g1);
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int e = 0; e < E; ++e) v[0][e] *= r * g0[e], v[1][e] *= r * g1[e];
-            } else {
+                for (int e = 0; e < E; ++e) v[u][c][e] = na_float(reinterpret_cast<const T*>(&raw[u][c])[e]);
+        if (sizeof(T) == 4)                          // parts are fp32
+#pragma unroll 1
+            for (int s = 1; s < p.parts; ++s) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) v[0][e] *= r, v[1][e] *= r;
+                for (int u = 0; u < NA_AHEAD; ++u) ask(u, first, s);
+#pragma unroll
+                for (int u = 0; u < NA_AHEAD; ++u)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int e = 0; e < E; ++e) v[u][c][e] += na_float(reinterpret_cast<const T*>(&raw[u][c])[e]);
             }
-            if (rotates) {
+#pragma unroll
+        for (int u = 0; u < NA_AHEAD; ++u) ask(u, first + NA_AHEAD, 0);      // the next passes are on their way meanwhile
+#pragma unroll
+        for (int u = 0; u < NA_AHEAD; ++u) {
+            if (first + u >= p1) break;
+            const int hd = (first + u) * HEADS + sub;
+            float(&x)[2][E] = v[u];
+            float ss = 0.f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) ss = fmaf(x[0][e], x[0][e], fmaf(x[1][e], x[1][e], ss));
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            if (hd >= heads) continue;
+            float r = 1.f;
+            if (hd < p.nq + p.nkv) {
+                const float* gain = hd < p.nq ? p.q_gain : p.k_gain;
+                if (gain) {
+                    gain += hd < p.nq ? hd * p.gain_q_stride : (hd - p.nq) * p.gain_k_stride;
+                    if (gain != have) {
+                        *reinterpret_cast<float4*>(g[0]) = load_f4(gain + c0 * E);
+                        *reinterpret_cast<float4*>(g[1]) = load_f4(gain + c1 * E);
+                        have = gain;
+                    }
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int e = 0; e < E; ++e) x[c][e] *= g[c][e];
+                }
                 if (NEIGHBOURS) {
 #pragma unroll
                     for (int c = 0; c < 2; ++c)
 #pragma unroll
                         for (int e = 0; e < E; e += 2) {
-                            const float a = v[c][e], b = v[c][e + 1], co = cs[c * (E / 2) + e / 2], si = sn[c * (E / 2) + e / 2];
-                            v[c][e] = a * co - b * si;
-                            v[c][e + 1] = b * co + a * si;
+                            const float a = x[c][e], b = x[c][e + 1], co = cs[c * 2 + e / 2], si = sn[c * 2 + e / 2];
+                            x[c][e] = a * co - b * si;
+                            x[c][e + 1] = b * co + a * si;
                         }
                 } else {
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
-                        const float a = v[0][e], b = v[1][e];
-                        v[0][e] = a * cs[e] - b * sn[e];
-                        v[1][e] = b * cs[e] + a * sn[e];
+                        const float a = x[0][e], b = x[1][e];
+                        x[0][e] = a * cs[e] - b * sn[e];
+                        x[1][e] = b * cs[e] + a * sn[e];
                     }
                 }
+                r = rsqrtf(ss * (1.f / D) + p.eps);
             }
-        }
-        uint8_t *to0, *to1;
-        if (hd < p.nq) {
-            to0 = reinterpret_cast<uint8_t*>(p.q_out + ((size_t)t * p.nq + hd) * D);
-            to1 = to0 + c1 * E * 2;
-            to0 += c0 * E * 2;
-            if (!known) {                            // a token without a position: zeros
-#pragma unroll
-                for (int e = 0; e < E; ++e) v[0][e] = v[1][e] = 0.f;
+            uint8_t *to0, *to1;
+            if (hd < p.nq) {
+                to0 = reinterpret_cast<uint8_t*>(p.q_out + ((size_t)t * p.nq + hd) * D);
+                to1 = to0 + c1 * E * 2;
+                to0 += c0 * E * 2;
+            } else {
+                if (!kept) continue;
+                const bool is_v = hd >= p.nq + p.nkv;
+                uint8_t* slab = cache + ((hd - p.nq - (is_v ? p.nkv : 0)) * 2 + is_v) * (kKvTile * D * 2);
+                to0 = slab + in0;
+                to1 = slab + in1;
             }
-        } else {
-            if (!kept) continue;
-            const bool is_v = hd >= p.nq + p.nkv;
-            const int h = hd - p.nq - (is_v ? p.nkv : 0), r = (int)(slot % kKvTile);
-            uint8_t* slab = p.kv_layer + (((size_t)(slot / kKvTile) * p.nkv + h) * 2 + is_v) * (size_t)(kKvTile * D * 2);
-            to0 = slab + kv_swizzled_chunk<D>(r, c0 * E / 8) + c0 * E % 8 * 2;
-            to1 = slab + kv_swizzled_chunk<D>(r, c1 * E / 8) + c1 * E % 8 * 2;
-        }
-        alignas(16) __half2 h[2][E / 2];
+            uint2 h[2];
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int e = 0; e < E; e += 2) h[c][e / 2] = na_half2(v[c][e], v[c][e + 1]);
-        if (E == 8) {
-            *reinterpret_cast<uint4*>(to0) = *reinterpret_cast<const uint4*>(h[0]);
-            *reinterpret_cast<uint4*>(to1) = *reinterpret_cast<const uint4*>(h[1]);
-        } else {
-            *reinterpret_cast<uint2*>(to0) = *reinterpret_cast<const uint2*>(h[0]);
-            *reinterpret_cast<uint2*>(to1) = *reinterpret_cast<const uint2*>(h[1]);
+            for (int c = 0; c < 2; ++c) {
+                h[c] = make_uint2(na_half2(x[c][0] * r, x[c][1] * r), na_half2(x[c][2] * r, x[c][3] * r));
+                if (!known) h[c] = make_uint2(0u, 0u);       // q of a token without a position
+            }
+            *reinterpret_cast<uint2*>(to0) = h[0];
+            *reinterpret_cast<uint2*>(to1) = h[1];
         }
     }
 }
 
 template <int D, class T>
-static int launch_norm_append(NormAppend& p, bool neighbours, cudaStream_t st) {
-    constexpr int E = NaType<T>::E, HEADS = 32 * 2 * E / D;
+static int launch_norm_append(NormAppend& p, bool neighbours, bool wide, cudaStream_t st) {
+    constexpr int HEADS = 32 * 2 * NA_E / D;
     p.passes = (p.nq + 2 * p.nkv + HEADS - 1) / HEADS;
-    p.per = 1;
+    // a warp takes as much of a token as leaves NA_FILL warps an SM: its angles and gains are read once
+    const long long each = (long long)p.T * p.passes / ((long long)NA_FILL * device_sms());
+    p.per = each < 1 ? 1 : each < p.passes ? (int)each : p.passes;
     p.per_token = (p.passes + p.per - 1) / p.per;
     const long long warps = (long long)p.T * p.per_token;
     const dim3 grid((unsigned)((warps + NA_WARPS - 1) / NA_WARPS));
-    if (neighbours) FT_CHECK_CUDA(launch_after(norm_append_kernel<D, T, true>, grid, dim3(NA_THREADS), 0, st, (const NormAppend&)p));
-    else FT_CHECK_CUDA(launch_after(norm_append_kernel<D, T, false>, grid, dim3(NA_THREADS), 0, st, (const NormAppend&)p));
+    const auto kernel = neighbours ? (wide ? norm_append_kernel<D, T, true, true> : norm_append_kernel<D, T, true, false>)
+                                   : (wide ? norm_append_kernel<D, T, false, true> : norm_append_kernel<D, T, false, false>);
+    FT_CHECK_CUDA(launch_after(kernel, grid, dim3(NA_THREADS), 0, st, (const NormAppend&)p));
     return 0;
 }
 
@@ -214,12 +235,13 @@ extern "C" int ft_norm_rope_kv_append(const void* qkv, int type, int n_parts, lo
     const int size = type == FT_F32 ? 4 : 2;
     FT_REQUIRE((uintptr_t)qkv % size == 0, "ft_norm_rope_kv_append: qkv on its own size");
     FT_REQUIRE((double)T * (nq + 2.0 * nkv) <= INT32_MAX, "ft_norm_rope_kv_append: %d tokens are more than one call takes", T);
-    const bool wide = (uintptr_t)qkv % 16 == 0 && row_stride * size % 16 == 0 && (n_parts == 1 || part_stride * size % 16 == 0);
-    NormAppend p{qkv, part_stride, row_stride, cos_t, sin_t, q_gain, k_gain, positions, kv_slots, (__half*)q_out, (uint8_t*)kv_layer, (long long)num_pages * kKvTile, n_parts, T,
-                 nq, nkv, n_angles, rotated, q_gains > 1 ? d : 0, k_gains > 1 ? d : 0, 0, 0, 0, wide, eps};
+    const int chunk = size * NA_E;
+    const bool wide = (uintptr_t)qkv % chunk == 0 && row_stride * size % chunk == 0 && (n_parts == 1 || part_stride * size % chunk == 0);
+    NormAppend p{qkv, part_stride, row_stride, cos_t, sin_t, q_gain, k_gain, positions, kv_slots, (__half*)q_out, (uint8_t*)kv_layer, num_pages * kKvTile, n_parts, T,
+                 nq, nkv, n_angles, rotated, q_gains > 1 ? d : 0, k_gains > 1 ? d : 0, 0, 0, 0, eps};
     const cudaStream_t st = (cudaStream_t)stream;
 #define FT_NA_CASE(D_, TYPE_, T_) \
-    if (d == D_ && type == TYPE_) return launch_norm_append<D_, T_>(p, neighbours != 0, st);
+    if (d == D_ && type == TYPE_) return launch_norm_append<D_, T_>(p, neighbours != 0, wide, st);
     FT_NA_CASE(64, FT_F32, float)
     FT_NA_CASE(64, FT_BF16, __nv_bfloat16)
     FT_NA_CASE(64, FT_F16, __half)
