@@ -216,10 +216,11 @@ static int launch_norm_append(NormAppend& p, bool neighbours, bool wide, cudaStr
 
 }  // namespace ft
 
-extern "C" int ft_norm_rope_kv_append(const void* qkv, int type, int n_parts, long long part_stride, long long row_stride, const float* cos_t, const float* sin_t, int n_angles,
-                                      int rotated, int neighbours, const float* q_gain, int q_gains, const float* k_gain, int k_gains, float eps, const int* positions,
-                                      const int* kv_slots, void* q_out, void* kv_layer, int num_pages, int T, int nq, int nkv, int d, void* stream) {
+extern "C" int ft_norm_rope_kv_append(const ft_norm_append_args* args, void* stream) {
     using namespace ft;
+    FT_REQUIRE(args, "ft_norm_rope_kv_append: null argument");
+    const auto [qkv, part_stride, row_stride, cos_t, sin_t, q_gain, k_gain, positions, kv_slots, q_out, kv_layer, type, n_parts, n_angles, rotated, neighbours, q_gains, k_gains,
+                num_pages, T, nq, nkv, d, eps] = *args;
     FT_REQUIRE(d == 64 || d == 128, "ft_norm_rope_kv_append: head_dim %d not supported (64 or 128)", d);
     FT_REQUIRE(type >= FT_F32 && type <= FT_F16, "ft_norm_rope_kv_append: type %d (FT_F32, FT_BF16 or FT_F16)", type);
     FT_REQUIRE(nq >= 0 && nkv >= 0 && nq + 2LL * nkv >= 1 && (nq + 2LL * nkv) * d <= INT32_MAX && T >= 0 && n_parts >= 1 && num_pages >= 0 && num_pages <= INT32_MAX / kKvTile,

@@ -960,10 +960,10 @@ extern "C" int ft_attn_shared_waits(void) {
     return n;
 }
 
-extern "C" int ft_attn_decode_shared(const void* q, const void* kv_layer, int num_pages, const int* page_table, int table_rows, int max_pages, const int* req_slot,
-                                     const int* ctx_lens, const int* group_start, const int* shared_lens, int n_groups, void* out, void* out_lo, void* scratch, int B, int nq,
-                                     int nkv, int d, void* stream) {
+extern "C" int ft_attn_decode_shared(const ft_attn_shared_args* args, void* stream) {
     using namespace ft;
+    FT_REQUIRE(args, "ft_attn_decode_shared: null argument");
+    const auto [q, kv_layer, page_table, req_slot, ctx_lens, group_start, shared_lens, out, out_lo, scratch, num_pages, table_rows, max_pages, n_groups, B, nq, nkv, d] = *args;
     FT_REQUIRE(d == 64 || d == 128, "ft_attn_decode_shared: head_dim %d not supported (64 or 128)", d);
     FT_REQUIRE(nq >= 1 && nkv >= 1 && nq % nkv == 0 && nq / nkv <= kSharedGroup, "ft_attn_decode_shared: GQA group %d/%d not supported", nq, nkv);
     const int G = nq / nkv, th = kSharedRows / G;

@@ -174,10 +174,11 @@ static int step_lists_hash(int R) {                            // places: a powe
 
 }  // namespace ft
 
-extern "C" int ft_step_lists(const int* cached_lens, const int* new_lens, const int* req_slot, int R, int* page_table, int table_rows, int max_pages,
-                             const int* free_pages, int n_free, const int* first_free, int max_tokens, int* req_start, int* ctx_lens, int* positions, int* seq_rows,
-                             int* kv_slots, int* taken, void* stream) {
+extern "C" int ft_step_lists(const ft_step_lists_args* args, void* stream) {
     using namespace ft;
+    FT_REQUIRE(args, "ft_step_lists: null argument");
+    const auto [cached_lens, new_lens, req_slot, page_table, free_pages, first_free, req_start, ctx_lens, positions, seq_rows, kv_slots, taken, R, table_rows, max_pages, n_free,
+                max_tokens] = *args;
     FT_REQUIRE(R >= 0 && R <= SL_MAX_REQUESTS, "ft_step_lists: %d requests (at most %d)", R, SL_MAX_REQUESTS);
     FT_REQUIRE(max_tokens >= 0 && max_tokens <= 1 << 30 && table_rows >= 0 && n_free >= 0 && max_pages >= 0 && max_pages < INT32_MAX / kKvTile,
                "ft_step_lists: bad sizes max_tokens=%d table %d x %d, %d free pages", max_tokens, table_rows, max_pages, n_free);

@@ -424,6 +424,11 @@ def kv8_records(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
 
 
 # ---- a decode step of a batch whose sequences have their first tokens in common, over the fp16 cache
+# These calls take a few microseconds on the GPU and about ten on the host, where what they ask tensors for counts: numbers, each once, and few views.
+_I32 = torch.int32
+_stream_of, _device_now = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
 class StepLists(NamedTuple):
     """What step_lists makes, int32 on the device: request r owns tokens req_start[r] .. req_start[r + 1] - 1 of the step and has ctx_lens[r] tokens with them; each token's
     position, row of the page table and place in the cache, -1 behind the last token; where the rest of the pool begins."""
@@ -435,34 +440,51 @@ class StepLists(NamedTuple):
     taken: torch.Tensor
 
 
+def _shared_ints(t, index: int, what: str, n: int, name: str) -> torch.Tensor:
+    """_kv8_ints, with what is mostly there first."""
+    if type(t) is torch.Tensor and t.dtype is _I32 and t.get_device() == index and t.is_contiguous() and (n < 0 or t.numel() == n):
+        return t
+    return _kv8_ints(t, index, what, n, name)
+
+
+def _shared_call(index: int, name: str, args: bytes) -> None:
+    """A library call on the device's current stream, whichever device is the current one."""
+    fn = getattr(N.load(), name)
+    if index == _device_now():
+        rc = fn(args, _stream_of(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(args, _stream_of(index))
+    if rc < 0:
+        N.check(rc, name)
+
+
 def step_lists(cached_lens, new_lens, req_slot, page_table: torch.Tensor, free_pages: torch.Tensor, max_tokens: int, first_free: Optional[torch.Tensor] = None) -> StepLists:
     """The lists of one step, built on the GPU: request r has cached_lens[r] tokens in the cache, new_lens[r] new ones and page-table row req_slot[r] (None: row r).  In their
     order the requests take as many of their new tokens as there is room for in their row, in the pool free_pages[first_free:] and in the budget of max_tokens; the pages that
     they take are written into page_table.  `first_free` is one int32 on the device (None: 0), `taken` of one step the next one's.  Of several requests with one row the first
-    has it.  The lists are int32 tensors on the device (then nothing goes up, and the call can be captured) or anything a tensor is made of."""
+    has it.  The lists are int32 tensors on the device (then nothing goes up, and the call can be captured) or anything a tensor is made of.  What comes back lies in one piece
+    of memory, which lives as long as any of it."""
     what = "step_lists"
     index = page_table.get_device()
     if index < 0:
         _refuse(what, "page_table is contiguous int32 [sequences, pages] on the GPU")
     rows, most = _kv8_table(page_table, index, what)
-    cached_lens = _kv8_ints(cached_lens, index, what, -1, "cached_lens")
+    cached_lens = _shared_ints(cached_lens, index, what, -1, "cached_lens")
     R = cached_lens.numel()
-    new_lens = _kv8_ints(new_lens, index, what, R, "new_lens")
-    if req_slot is not None:
-        req_slot = _kv8_ints(req_slot, index, what, R, "req_slot")
-    free_pages = _kv8_ints(free_pages, index, what, -1, "free_pages")
-    if first_free is not None:
-        first_free = _kv8_ints(first_free, index, what, 1, "first_free")
+    new_lens = _shared_ints(new_lens, index, what, R, "new_lens")
+    slots = 0 if req_slot is None else (req_slot := _shared_ints(req_slot, index, what, R, "req_slot")).data_ptr()
+    free_pages = _shared_ints(free_pages, index, what, -1, "free_pages")
+    first = 0 if first_free is None else (first_free := _shared_ints(first_free, index, what, 1, "first_free")).data_ptr()
     if max_tokens < 0:
         _refuse(what, "a number of tokens")
-    parts = torch.empty(2 * R + 2 + 3 * max_tokens, device=index, dtype=torch.int32).split([R + 1, R, max_tokens, max_tokens, max_tokens, 1])
-    out = StepLists(*parts)
-    at = out.req_start.data_ptr()
+    made = cached_lens.new_empty(2 * R + 2 + 3 * max_tokens)
+    at = made.data_ptr()
     pos = at + 4 * (2 * R + 1)
-    _kv8_call(index, "ft_step_lists", cached_lens.data_ptr(), new_lens.data_ptr(), 0 if req_slot is None else req_slot.data_ptr(), R, page_table.data_ptr(), rows, most,
-              free_pages.data_ptr(), free_pages.numel(), 0 if first_free is None else first_free.data_ptr(), max_tokens, at, at + 4 * (R + 1), pos, pos + 4 * max_tokens,
-              pos + 8 * max_tokens, pos + 12 * max_tokens)
-    return out
+    _shared_call(index, "ft_step_lists", N.STEP_LISTS_ARGS.pack(
+        cached_lens.data_ptr(), new_lens.data_ptr(), slots, page_table.data_ptr(), free_pages.data_ptr(), first, at, at + 4 * (R + 1), pos, pos + 4 * max_tokens,
+        pos + 8 * max_tokens, pos + 12 * max_tokens, R, rows, most, free_pages.numel(), max_tokens))
+    return StepLists(*torch.unsafe_split_with_sizes(made, (R + 1, R, max_tokens, max_tokens, max_tokens, 1)))
 
 
 _QKV_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -471,9 +493,12 @@ _QKV_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 def _kv16_layer(layer: torch.Tensor, d: int, what: str):
     """(device, pages, kv heads) of a layer of the fp16 cache."""
     index = layer.get_device()
-    if index < 0 or layer.dtype is not torch.float16 or layer.dim() != 5 or not layer.is_contiguous() or layer.shape[2:] != (2, KV_TILE, d):
+    if index < 0 or layer.dtype is not torch.float16 or layer.dim() != 5 or not layer.is_contiguous():
         _refuse(what, f"the cache is contiguous CUDA fp16 [pages, nkv, 2, {KV_TILE}, head_dim]")
-    return index, layer.shape[0], layer.shape[1]
+    pages, nkv, two, tile, width = layer.shape
+    if two != 2 or tile != KV_TILE or width != d:
+        _refuse(what, f"the cache is contiguous CUDA fp16 [pages, nkv, 2, {KV_TILE}, head_dim]")
+    return index, pages, nkv
 
 
 def norm_rope_kv_append(qkv: torch.Tensor, positions, kv_slots, kv_layer: torch.Tensor, nq: int, nkv: int, d: int, cos: Optional[torch.Tensor] = None,
@@ -487,31 +512,43 @@ def norm_rope_kv_append(qkv: torch.Tensor, positions, kv_slots, kv_layer: torch.
     index, pages, heads = _kv16_layer(kv_layer, d, what)
     if heads != nkv:
         _refuse(what, "the cache has another number of heads")
-    kind = _QKV_TYPES.get(qkv.dtype)
-    dims = qkv.dim()
-    if kind is None or qkv.get_device() != index or dims not in (2, 3) or (dims == 3 and (kind != 0 or qkv.shape[0] < 1)) or qkv.shape[-1] != (nq + 2 * nkv) * d:
+    kind, shape = _QKV_TYPES.get(qkv.dtype), qkv.shape
+    dims = len(shape)
+    if kind is None or qkv.get_device() != index or dims not in (2, 3) or (dims == 3 and (kind != 0 or shape[0] < 1)) or shape[-1] != (nq + 2 * nkv) * d:
         _refuse(what, "qkv is fp32 [S, T, (nq + 2 nkv) d], or [T, (nq + 2 nkv) d] in fp32, bf16 or fp16, on the cache's device")
-    T = qkv.shape[-2]
-    stride = qkv.stride()
+    T, stride = shape[-2], qkv.stride()
     if T and stride[-1] != 1:
         _refuse(what, "a row of qkv lies in one piece")
-    positions, kv_slots = _kv8_ints(positions, index, what, T, "positions"), _kv8_ints(kv_slots, index, what, T, "kv_slots")
-    angles = rotated = 0
+    positions, kv_slots = _shared_ints(positions, index, what, T, "positions"), _shared_ints(kv_slots, index, what, T, "kv_slots")
+    angles = rotated = at_cos = at_sin = 0
     if cos is not None or sin is not None:
         for t in (cos, sin):
-            if t is None or t.dtype is not torch.float32 or t.get_device() != index or t.dim() != 2 or t.shape != cos.shape or not t.is_contiguous():
+            if t is None or t.dtype is not torch.float32 or t.get_device() != index or t.dim() != 2 or not t.is_contiguous():
                 _refuse(what, "cos and sin are contiguous fp32 [positions, rotated / 2] on the cache's device")
-        angles, rotated = cos.shape[0], 2 * cos.shape[1]
-    gains = []
-    for t, n in ((q_gain, nq), (k_gain, nkv)):
-        if t is not None and (t.dtype is not torch.float32 or t.get_device() != index or t.shape not in ((d,), (n, d)) or not t.is_contiguous()):
-            _refuse(what, "gains are contiguous fp32 [d] or [heads, d] on the cache's device")
-        gains += [0, 1] if t is None else [t.data_ptr(), 1 if t.dim() == 1 else n]
-    q = torch.empty(T, nq, d, device=index, dtype=torch.float16)
-    _kv8_call(index, "ft_norm_rope_kv_append", qkv.data_ptr(), kind, qkv.shape[0] if dims == 3 else 1, stride[0] if dims == 3 else 0, stride[-2],
-              0 if cos is None else cos.data_ptr(), 0 if sin is None else sin.data_ptr(), angles, rotated, int(neighbours), *gains, eps, positions.data_ptr(),
-              kv_slots.data_ptr(), q.data_ptr(), kv_layer.data_ptr(), pages, T, nq, nkv, d)
+        if cos.shape != sin.shape:
+            _refuse(what, "cos and sin are contiguous fp32 [positions, rotated / 2] on the cache's device")
+        angles, rotated = cos.shape
+        rotated, at_cos, at_sin = 2 * rotated, cos.data_ptr(), sin.data_ptr()
+    at_q, many_q = _norm_gain(q_gain, index, nq, d, what)
+    at_k, many_k = _norm_gain(k_gain, index, nkv, d, what)
+    q = kv_layer.new_empty((T, nq, d))
+    _shared_call(index, "ft_norm_rope_kv_append", N.NORM_APPEND_ARGS.pack(
+        qkv.data_ptr(), stride[0] if dims == 3 else 0, stride[-2], at_cos, at_sin, at_q, at_k, positions.data_ptr(), kv_slots.data_ptr(), q.data_ptr(), kv_layer.data_ptr(), kind,
+        shape[0] if dims == 3 else 1, angles, rotated, 1 if neighbours else 0, many_q, many_k, pages, T, nq, nkv, d, eps))
     return q
+
+
+def _norm_gain(t, index: int, heads: int, d: int, what: str):
+    """(address, rows) of a gain, (0, 1) without one."""
+    if t is None:
+        return 0, 1
+    shape = t.shape
+    if t.dtype is torch.float32 and t.get_device() == index and t.is_contiguous():
+        if len(shape) == 1 and shape[0] == d:
+            return t.data_ptr(), 1
+        if len(shape) == 2 and shape[0] == heads and shape[1] == d:
+            return t.data_ptr(), heads
+    _refuse(what, "gains are contiguous fp32 [d] or [heads, d] on the cache's device")
 
 
 def attn_decode_shared(q: torch.Tensor, kv_layer: torch.Tensor, page_table: torch.Tensor, ctx_lens, group_start, shared_lens, req_slot=None, planes: int = 2):
@@ -530,21 +567,33 @@ def attn_decode_shared(q: torch.Tensor, kv_layer: torch.Tensor, page_table: torc
     if planes != 1 and planes != 2:
         _refuse(what, "one plane or two")
     rows, most = _kv8_table(page_table, index, what)
-    ctx_lens, shared_lens = _kv8_ints(ctx_lens, index, what, B, "ctx_lens"), _kv8_ints(shared_lens, index, what, -1, "shared_lens")
+    ctx_lens, shared_lens = _shared_ints(ctx_lens, index, what, B, "ctx_lens"), _shared_ints(shared_lens, index, what, -1, "shared_lens")
     n = shared_lens.numel()
-    group_start = _kv8_ints(group_start, index, what, n + 1, "group_start")
-    if req_slot is not None:
-        req_slot = _kv8_ints(req_slot, index, what, B, "req_slot")
-    out = torch.empty(B, nq * d, device=index, dtype=torch.bfloat16)
+    group_start = _shared_ints(group_start, index, what, n + 1, "group_start")
+    slots = 0 if req_slot is None else (req_slot := _shared_ints(req_slot, index, what, B, "req_slot")).data_ptr()
+    out = q.new_empty((B, nq * d), dtype=torch.bfloat16)
     lo = torch.empty_like(out) if planes == 2 else None
-    size = _kv8_sizes.get((index, B, n, nq, nkv, d))
+    size = _shared_sizes.get((index, B, n, nq, nkv, d))
     if size is None:
-        with torch.cuda.device(index):
-            size = _kv8_sizes[index, B, n, nq, nkv, d] = N.check(N.load().ft_attn_decode_shared_scratch_bytes(B, n, nq, nkv, d), "ft_attn_decode_shared_scratch_bytes")
-    scratch = torch.empty(size, device=index, dtype=torch.uint8)
-    _kv8_call(index, "ft_attn_decode_shared", q.data_ptr(), kv_layer.data_ptr(), pages, page_table.data_ptr(), rows, most, 0 if req_slot is None else req_slot.data_ptr(),
-              ctx_lens.data_ptr(), group_start.data_ptr(), shared_lens.data_ptr(), n, out.data_ptr(), 0 if lo is None else lo.data_ptr(), scratch.data_ptr(), B, nq, nkv, d)
+        size = _shared_size(index, B, n, nq, nkv, d)
+    scratch = q.new_empty(size)
+    _shared_call(index, "ft_attn_decode_shared", N.ATTN_SHARED_ARGS.pack(
+        q.data_ptr(), kv_layer.data_ptr(), page_table.data_ptr(), slots, ctx_lens.data_ptr(), group_start.data_ptr(), shared_lens.data_ptr(), out.data_ptr(),
+        0 if lo is None else lo.data_ptr(), scratch.data_ptr(), pages, rows, most, n, B, nq, nkv, d))
     return out, lo
+
+
+_shared_sizes = {}
+
+
+def _shared_size(index: int, *sizes) -> int:
+    """fp16 numbers of work memory; those of the last thousand shapes are remembered."""
+    with torch.cuda.device(index):
+        n = N.check(N.load().ft_attn_decode_shared_scratch_bytes(*sizes), "ft_attn_decode_shared_scratch_bytes") // 2
+    if len(_shared_sizes) >= 1000:
+        _shared_sizes.clear()
+    _shared_sizes[(index, *sizes)] = n
+    return n
 
 
 def attn_shared_check(device=None) -> None:

@@ -706,7 +706,8 @@ int ft_attn_prefill_kv8(const void* q, const void* kv8_layer, int num_pages, con
 /* A decode step of a batch whose sequences have their first tokens in common, over the fp16 cache of ft_rope_kv_append / ft_attn_decode: its lists built on the GPU, heads
  * normed, rotated and appended in one pass, and attention that reads a common prefix once.  A token's place in the cache (kv slot) is page * 64 + token of the page; below 0: none.
  * Page numbers outside [0, num_pages), rows outside [0, table_rows) and positions beyond max_pages * 64 name no token: nothing is written there and attention does not see
- * such keys; a table without rows or pages and a cache without pages may be NULL.  The calls read and write what they are given only.
+ * such keys; a table without rows or pages and a cache without pages may be NULL.  The calls read and write what they are given only; the structs of arguments are read
+ * before they return.
  *
  * ft_step_lists: requests r = 0 .. R - 1 (R up to 8192) in their order, with cached_lens[r] tokens in the cache, new_lens[r] new ones and page-table row req_slot[r] (NULL: row r),
  * each take as many of their new tokens as there is room for: in their row of the table, on their last page and the pages left in the pool, in the budget of max_tokens.
@@ -714,9 +715,14 @@ int ft_attn_prefill_kv8(const void* q, const void* kv8_layer, int num_pages, con
  * tokens, and *taken is where the rest of the pool begins (not the same address as first_free).  Of several requests with one row the first gets it, the others and those
  * whose row is outside the table get nothing.  -> req_start [R + 1], ctx_lens [R] = cached and taken tokens; positions, seq_rows and kv_slots [max_tokens] of every token,
  * -1 behind the last one.  kv_slots is also -1 where the table or the pool names no page (a number below 0 or from 2^25 - 1 on). */
-int ft_step_lists(const int* cached_lens, const int* new_lens, const int* req_slot, int R, int* page_table, int table_rows, int max_pages,
-                  const int* free_pages, int n_free, const int* first_free, int max_tokens, int* req_start, int* ctx_lens, int* positions, int* seq_rows,
-                  int* kv_slots, int* taken, void* stream);
+typedef struct {
+    const int *cached_lens, *new_lens, *req_slot;
+    int* page_table;
+    const int *free_pages, *first_free;
+    int *req_start, *ctx_lens, *positions, *seq_rows, *kv_slots, *taken;
+    int R, table_rows, max_pages, n_free, max_tokens;
+} ft_step_lists_args;
+int ft_step_lists(const ft_step_lists_args* args, void* stream);
 /* ft_norm_rope_kv_append: rows of (nq + 2 nkv) heads of d, queries, keys, values, row_stride elements apart, are
  *   y = x * rsqrt(mean(x^2) + eps) * gain   for each head of q and k (q_gain / k_gain fp32 [q_gains / k_gains][d], one for all heads or one for each; NULL: 1), then
  *   rotated on the first `rotated` dims (a multiple of 16; 0: none) by cos_t / sin_t fp32 [n_angles][rotated / 2]: pairs (i, i + rotated / 2), or (2 i, 2 i + 1) with neighbours,
@@ -724,9 +730,16 @@ int ft_step_lists(const int* cached_lens, const int* new_lens, const int* req_sl
  * up, part_stride elements apart, or one part of FT_BF16 or FT_F16.  A token whose position is below 0 or has no angles gives q = 0 and is not written; one whose slot
  * is outside the cache is not written.  Two tokens for one slot leave it with numbers of either. */
 enum { FT_F32 = 0, FT_BF16 = 1, FT_F16 = 2 };
-int ft_norm_rope_kv_append(const void* qkv, int type, int n_parts, long long part_stride, long long row_stride, const float* cos_t, const float* sin_t, int n_angles,
-                           int rotated, int neighbours, const float* q_gain, int q_gains, const float* k_gain, int k_gains, float eps, const int* positions,
-                           const int* kv_slots, void* q_out, void* kv_layer, int num_pages, int T, int nq, int nkv, int d, void* stream);
+typedef struct {
+    const void* qkv;
+    long long part_stride, row_stride;
+    const float *cos_t, *sin_t, *q_gain, *k_gain;
+    const int *positions, *kv_slots;
+    void *q_out, *kv_layer;
+    int type, n_parts, n_angles, rotated, neighbours, q_gains, k_gains, num_pages, T, nq, nkv, d;
+    float eps;
+} ft_norm_append_args;
+int ft_norm_rope_kv_append(const ft_norm_append_args* args, void* stream);
 /* ft_attn_decode_shared: one query token per sequence, q FP16 [B][nq][d], nq / nkv up to 8, out bf16 [B][nq*d] (+ residual plane out_lo, may be NULL).  Query b sees its first
  * ctx_lens[b] tokens.  Group g = queries group_start[g] .. group_start[g + 1] - 1 (group_start grows; queries outside all groups stand alone): the first shared_lens[g] tokens of
  * all of them are those of page-table row req_slot[group_start[g]], also where a query's own context is shorter or the first one's; what the other rows name below
@@ -736,9 +749,13 @@ int ft_norm_rope_kv_append(const void* qkv, int type, int n_parts, long long par
  * ft_attn_shared_waits: 1 if a wait inside one of its kernels has run out on the current device since the library was loaded (rows of some call mean nothing), else 0;
  * waits for all that the device has been given, on every stream. */
 long long ft_attn_decode_shared_scratch_bytes(int B, int n_groups, int nq, int nkv, int d);
-int ft_attn_decode_shared(const void* q, const void* kv_layer, int num_pages, const int* page_table, int table_rows, int max_pages, const int* req_slot,
-                          const int* ctx_lens, const int* group_start, const int* shared_lens, int n_groups, void* out, void* out_lo, void* scratch, int B, int nq,
-                          int nkv, int d, void* stream);
+typedef struct {
+    const void *q, *kv_layer;
+    const int *page_table, *req_slot, *ctx_lens, *group_start, *shared_lens;
+    void *out, *out_lo, *scratch;
+    int num_pages, table_rows, max_pages, n_groups, B, nq, nkv, d;
+} ft_attn_shared_args;
+int ft_attn_decode_shared(const ft_attn_shared_args* args, void* stream);
 int ft_attn_shared_waits(void);
 
 /* K7: per-row temperature / top-k / top-p sampling (argmax when temperature <= 0; a null temperature says so for all rows).

@@ -1,4 +1,7 @@
 """A decode step over shared prefixes without a GPU: what its calls refuse before anything is launched."""
+import os
+import struct
+
 import pytest
 import torch
 
@@ -21,7 +24,7 @@ BIG = 2 ** 31 - 1
 
 def test_refusals_of_lists(lib):
     call = lambda R=1, rows=1, width=1, free=1, tokens=1, cached=P, new=P, table=P, pool=P, start=P, ctx=P, pos=P, taken=P: lib.ft_step_lists(
-        cached, new, 0, R, table, rows, width, pool, free, 0, tokens, start, ctx, pos, P, P, taken, 0)
+        N.STEP_LISTS_ARGS.pack(cached, new, 0, table, pool, 0, start, ctx, pos, P, P, taken, R, rows, width, free, tokens), 0)
     refused(call(R=-1), "requests")
     refused(call(R=8193), "requests")
     for bad in (dict(rows=-1), dict(width=-1), dict(width=BIG // 64), dict(free=-1), dict(tokens=-1), dict(tokens=(1 << 30) + 1)):
@@ -32,7 +35,7 @@ def test_refusals_of_lists(lib):
 
 def test_refusals_of_appending(lib):
     call = lambda d=64, kind=0, T=1, nq=4, nkv=1, S=1, pages=1, rotated=0, angles=8, cos=P, q_gain=0, q_gains=1, k_gain=0, k_gains=1, qkv=P, pos=P, out=P, cache=P: lib.ft_norm_rope_kv_append(
-        qkv, kind, S, 0, 0, cos, P, angles, rotated, 0, q_gain, q_gains, k_gain, k_gains, 1e-5, pos, P, out, cache, pages, T, nq, nkv, d, 0)
+        N.NORM_APPEND_ARGS.pack(qkv, 0, 0, cos, P, q_gain, k_gain, pos, P, out, cache, kind, S, angles, rotated, 0, q_gains, k_gains, pages, T, nq, nkv, d, 1e-5), 0)
     refused(call(d=96), "head_dim 96")
     refused(call(kind=3), "type 3")
     refused(call(kind=-1), "type -1")
@@ -51,11 +54,12 @@ def test_refusals_of_appending(lib):
     refused(call(kind=2, qkv=P + 1), "own size")
     refused(call(T=BIG), "more than one call takes")
     assert call(T=0, qkv=0) == 0
+    refused(lib.ft_norm_rope_kv_append(None, 0), "null argument")
 
 
 def test_refusals_of_attention(lib):
     call = lambda d=64, B=1, nq=4, nkv=1, n=1, pages=1, rows=1, width=1, q=P, cache=P, table=P, ctx=P, start=P, shared=P, out=P, lo=0, scratch=P: lib.ft_attn_decode_shared(
-        q, cache, pages, table, rows, width, 0, ctx, start, shared, n, out, lo, scratch, B, nq, nkv, d, 0)
+        N.ATTN_SHARED_ARGS.pack(q, cache, table, 0, ctx, start, shared, out, lo, scratch, pages, rows, width, n, B, nq, nkv, d), 0)
     refused(call(d=96), "head_dim 96")
     for nq, nkv in ((0, 1), (1, 0), (3, 2), (9, 1), (-4, -1)):
         refused(call(nq=nq, nkv=nkv), "GQA group")
@@ -68,6 +72,8 @@ def test_refusals_of_attention(lib):
     for bad in (dict(q=P + 8), dict(cache=P + 2), dict(out=P + 8), dict(lo=P + 4), dict(scratch=P + 4)):
         refused(call(**bad), "16 bytes")
     assert call(B=0, q=0) == 0
+    refused(lib.ft_attn_decode_shared(None, 0), "null argument")
+    refused(lib.ft_step_lists(None, 0), "null argument")
     refused(lib.ft_attn_decode_shared_scratch_bytes(1, 1, 4, 1, 32), "head_dim 32")
     refused(lib.ft_attn_decode_shared_scratch_bytes(1, 1, 0, 1, 64), "GQA group")
     for B, n, nq in ((-1, 1, 4), (1, -1, 4), (1 << 24, 1, 4)):
@@ -82,3 +88,30 @@ def test_refusals_of_tensors():
                  lambda: K.attn_decode_shared(torch.zeros(1, 4, 64, dtype=torch.float16), cache, table, i32(1), i32(0, 1), i32(1))):
         with pytest.raises(N.NativeError):
             call()
+
+
+def test_structs_of_arguments_lie_as_in_the_header(lib, tmp_path):
+    """Every field's offset, by the C compiler and by what packs them."""
+    import re
+    import shutil
+    import subprocess
+    if shutil.which("gcc") is None:
+        pytest.skip("no gcc on this box")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    header = re.sub(r"/\*.*?\*/", "", open(os.path.join(root, "include", "fasttalk_b200.h")).read(), flags=re.S)
+    for name, layout in (("ft_step_lists_args", N.STEP_LISTS_ARGS), ("ft_norm_append_args", N.NORM_APPEND_ARGS), ("ft_attn_shared_args", N.ATTN_SHARED_ARGS)):
+        body = re.search(r"typedef struct \{([^}]*)\} " + name, header).group(1)
+        fields = [re.search(r"(\w+)$", v.strip()).group(1) for line in body.split(";") for v in line.split(",") if v.strip()]
+        src = tmp_path / "f.c"
+        src.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "fasttalk_b200.h"\nint main(void) {\n'
+                       + "".join(f'    printf("%d %d\\n", (int)offsetof({name}, {f}), (int)sizeof((({name}*)0)->{f}));\n' for f in fields) + "    return 0;\n}\n")
+        subprocess.run(["gcc", "-std=c99", "-I", os.path.join(root, "include"), str(src), "-o", str(tmp_path / "f")], check=True)
+        want = [tuple(map(int, line.split())) for line in subprocess.run([str(tmp_path / "f")], capture_output=True, text=True, check=True).stdout.splitlines()]
+        kinds = "".join(int(n or 1) * k for n, k in re.findall(r"(\d*)([Pqif])", layout.format))
+        at, got = 0, []
+        for k in kinds:
+            size = struct.calcsize(k)
+            at = -(-at // size) * size
+            got.append((at, size))
+            at += size
+        assert got == want and layout.size == at
