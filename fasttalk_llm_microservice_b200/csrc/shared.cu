@@ -86,15 +86,21 @@ struct SharedQuery {
     __device__ __forceinline__ void chunk(uint32_t tile, int lo, int hi, float scale_log2, int lane) {
         const int g = lane >> 2;
         float s[BLOCKS][4], most[2] = {-INFINITY, -INFINITY};
+        // operands of several products are asked for ahead of the first (one by one, each waited for its own 33 clocks)
+        uint32_t x[8][4];
+        constexpr int TOGETHER = 128 / D;                                    // blocks whose eight reads go together
 #pragma unroll
-        for (int b = 0; b < BLOCKS; ++b) {
-            s[b][0] = s[b][1] = s[b][2] = s[b][3] = 0.f;
-            if (16 * b >= hi || 16 * b + 16 <= lo) continue;
+        for (int b0 = 0; b0 < BLOCKS; b0 += TOGETHER) {
 #pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks) {
-                uint32_t a0, a1, a2, a3;
-                ldmatrix_x4(tile + at(16 * b + (lane & 15), 2 * ks + (lane >> 4)), a0, a1, a2, a3);
-                mma_f16_16816(s[b], a0, a1, a2, a3, q[ks][0], q[ks][1]);
+            for (int i = 0; i < 8; ++i) {
+                const int b = b0 + i / (D / 16), ks = i % (D / 16);
+                ldmatrix_x4(tile + at(16 * b + (lane & 15), 2 * ks + (lane >> 4)), x[i][0], x[i][1], x[i][2], x[i][3]);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int b = b0 + i / (D / 16), ks = i % (D / 16);
+                if (ks == 0) s[b][0] = s[b][1] = s[b][2] = s[b][3] = 0.f;
+                mma_f16_16816(s[b], x[i][0], x[i][1], x[i][2], x[i][3], q[ks][0], q[ks][1]);
             }
         }
         if (lo > 0 || hi < CHUNK) {
@@ -127,22 +133,26 @@ struct SharedQuery {
         }
         const float r0 = kSharedTop - (m[0] == -INFINITY ? 0.f : m[0]), r1 = kSharedTop - (m[1] == -INFINITY ? 0.f : m[1]);
 #pragma unroll
-        for (int b = 0; b < BLOCKS; ++b) {
-            if (16 * b >= hi || 16 * b + 16 <= lo) continue;
-            uint32_t pb[2];
+        for (int b0 = 0; b0 < BLOCKS; b0 += TOGETHER) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float p0 = ex2_fast(fmaf(s[b][2 * h], scale_log2, r0)), p1 = ex2_fast(fmaf(s[b][2 * h + 1], scale_log2, r1));
-                l[0] += p0;
-                l[1] += p1;
-                const __half2 t = __floats2half2_rn(p0, p1);
-                asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pb[h]) : "r"(*reinterpret_cast<const uint32_t*>(&t)));
+            for (int i = 0; i < 8; ++i) {
+                const int b = b0 + i / (D / 16), n = i % (D / 16);
+                ldmatrix_x4_trans(tile + Shared<D>::HALF + at(16 * b + (lane & 7) + (lane >> 4) * 8, 2 * n + (lane >> 3 & 1)), x[i][0], x[i][1], x[i][2], x[i][3]);
             }
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-                uint32_t a0, a1, a2, a3;
-                ldmatrix_x4_trans(tile + Shared<D>::HALF + at(16 * b + (lane & 7) + (lane >> 4) * 8, 2 * i + (lane >> 3 & 1)), a0, a1, a2, a3);
-                mma_f16_16816(o[i], a0, a1, a2, a3, pb[0], pb[1]);
+            for (int u = 0; u < TOGETHER; ++u) {
+                const int b = b0 + u;
+                uint32_t pb[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float p0 = ex2_fast(fmaf(s[b][2 * h], scale_log2, r0)), p1 = ex2_fast(fmaf(s[b][2 * h + 1], scale_log2, r1));
+                    l[0] += p0;
+                    l[1] += p1;
+                    const __half2 t = __floats2half2_rn(p0, p1);
+                    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pb[h]) : "r"(*reinterpret_cast<const uint32_t*>(&t)));
+                }
+#pragma unroll
+                for (int n = 0; n < D / 16; ++n) mma_f16_16816(o[n], x[u * (D / 16) + n][0], x[u * (D / 16) + n][1], x[u * (D / 16) + n][2], x[u * (D / 16) + n][3], pb[0], pb[1]);
             }
         }
     }
@@ -293,11 +303,10 @@ __device__ __forceinline__ void shared_own(const SharedArgs& p, const SharedGrou
         const int lo = __shfl_sync(0xffffffffu, lo_x, x), hi = __shfl_sync(0xffffffffu, hi_x, x), at = lo / CH * CH;
         uint8_t* tile = ring + stage * C::CHUNK_BYTES;
         if (lo > at || hi < at + CH) {                                       // hidden values may be anything: 0 * infinity is none
-            // (in the blocks of 16 that are multiplied)
 #pragma unroll 1
             for (int b = 0; b < CH; b += 16) {
                 const int from_t = lo - at - b, to_t = hi - at - b;
-                if (from_t >= 16 || to_t <= 0 || (from_t <= 0 && to_t >= 16)) continue;
+                if (from_t <= 0 && to_t >= 16) continue;
 #pragma unroll
                 for (int j = 0; j < D / 16; ++j) {
                     const int v = lane + 32 * j, k = v / (D / 8);
@@ -476,6 +485,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
+    uint32_t k_bits = 0, v_bits = 0;                                         // of the warp that copies: the phases of what it has asked for
     bool ok = true;                                                          // false: a wait ran out
     auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, shared_wait(bar, parity, &dead)); };
     // the n-th stretch of the prefix's share, or one without pages behind the last; and this warp's word that it has done with it
@@ -568,13 +578,8 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
                 ok = __shfl_sync(0xffffffffu, ok, 0);
                 if (more) ++k;
             }
-            if (lane == 0)
-#pragma unroll 1
-                for (int i = 0; i < 6 * C::STAGES; ++i) {                    // nothing may still be on its way into this CTA's memory when it ends
-                    const int kind = i >= 3 * C::STAGES, x = i - kind * 3 * C::STAGES;
-#pragma unroll 1
-                    for (int j = 0; j < kWaitLimit && !mbar_try_wait((kind ? v_full : k_full) + x, (phases[kind].bits >> x & 1) ^ 1); ++j) {}
-                }
+            k_bits = phases[0].bits;
+            v_bits = phases[1].bits;
             __syncwarp();
         } else {
             // ---------------- products, one warp a half
@@ -822,7 +827,16 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
     }
     tc_fence_before();
     __syncthreads();
-    if (tid == 0 && dead) *err = 1;
+    if (tid == 0 && dead) {
+        *err = 1;
+#pragma unroll 1
+        for (int i = 0; i < 6 * C::STAGES; ++i) {                            // nothing may still be on its way into this CTA's memory when it ends: who gave up has not waited for it
+            const int x = i % (3 * C::STAGES);
+            uint64_t* const full = (i == x ? k_full : v_full) + x;
+#pragma unroll 1
+            for (int j = 0; j < kWaitLimit && !mbar_try_wait(full, ((i == x ? k_bits : v_bits) >> x & 1) ^ 1); ++j) {}
+        }
+    }
     if (warp == 3) {
         tc_fence_after();
         tmem_dealloc(tmem, C::COLS);
