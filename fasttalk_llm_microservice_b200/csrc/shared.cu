@@ -6,7 +6,7 @@
 //            half S = Q K^T (M128 N64 K=D, the cache's slab as it lies), one thread a row for the softmax, P to tensor memory over the scores that it came from,
 //            O += P V (M128 N=D K64).  Queries that fill one half only go to both halves, which take every other page each.  All rows see all pages: the only
 //            mask is the end of the last one.
-//   own      a warp walks a share of its own: chunks of 16 KB by bulk copies that it asks for itself, two of them on their way while it multiplies (mma.sync, the
+//   own      a warp walks a share of its own: chunks of 16 or 8 KB by bulk copies that it asks for itself, two of them on their way while it multiplies (mma.sync, the
 //            query heads of a key head in the columns).  No warp waits for another.
 // Each share's results are O, maximum and sum of its rows; a second kernel puts them together in their order.
 #include "common.cuh"
@@ -39,8 +39,8 @@ struct Shared {
     static constexpr int STAGES = D == 64 ? 4 : 3, SLAB = TILE / 2, TOKENS = 16;
     static constexpr int AHEAD = 2;                                          // pages that keys are copied ahead of values
     static constexpr int QBLK = kSharedRows * 128;                           // [128 rows][64 dims]
-    static constexpr int OWN_WARPS = D == 64 ? 4 : 2, OWN_STAGES = 2;
-    static constexpr int CHUNK = D == 64 ? 64 : 32;                          // tokens
+    static constexpr int OWN_WARPS = 4, OWN_STAGES = 2;
+    static constexpr int CHUNK = D == 64 ? 64 : 16;                          // tokens
     static constexpr int CHUNK_BYTES = 2 * CHUNK * D * 2, HALF = CHUNK_BYTES / 2;        // keys | values; of each D / 64 pieces of [CHUNK][64 dims]
     static constexpr int KV = 2 * KH * QBLK, OWN = KV + STAGES * TILE, SMEM = 1024 + OWN + OWN_WARPS * OWN_STAGES * CHUNK_BYTES;
     // tensor memory: scores [half][2][64 columns] (probabilities, pairs of fp16, over the first 32 of them), O [half][D]
@@ -191,7 +191,8 @@ __device__ __forceinline__ void shared_own(const SharedArgs& p, const SharedGrou
         }
     };
     // lane x: step x of the 32 at hand
-    int unit_x = 0, head_x = 0, from_x = 0, last_x = 0, lo_x = 0, hi_x = 0, page_x = -1;
+    int unit_x = 0, from_x = 0, last_x = 0, seen_x = 0;                      // seen: of the chunk's tokens, first and behind the last one in bytes
+    const uint8_t* src_x = nullptr;                                          // the chunk's first keys in the cache
     bool prefix_x = false;
     unsigned paged = 0, to_ask = 0;
     int unit = -1, from = 0, last = 0;                                       // the unit under way: where it begins in the list, its last step
@@ -230,32 +231,32 @@ __device__ __forceinline__ void shared_own(const SharedArgs& p, const SharedGrou
             w.steps = __shfl_sync(0xffffffffu, s.steps, l);
             prefix_x = __shfl_sync(0xffffffffu, (int)s.prefix, l);
             const int base_l = __shfl_sync(0xffffffffu, end - span, l), r_own = __shfl_sync(0xffffffffu, row, l), r_led = __shfl_sync(0xffffffffu, led_row, l);
-            head_x = (int)((unsigned)(F - base_l) / (unsigned)w.steps);
-            from_x = base_l + head_x * w.steps;
+            const int head = (int)((unsigned)(F - base_l) / (unsigned)w.steps);
+            from_x = base_l + head * w.steps;
             last_x = from_x + w.steps - 1;
-            unit_x = (b0 + l) * p.nkv + head_x;
-            const int r = w.step(p, F - from_x, lo_x, hi_x) ? r_led : r_own;
-            page_x = -1;
-            if (f + lane < f_end && lo_x < hi_x && r >= 0) page_x = p.page_table[(size_t)r * p.max_pages + lo_x / kKvTile];
-            if (page_x >= p.num_pages) page_x = -1;
+            unit_x = (b0 + l) * p.nkv + head;
+            int lo, hi, page = -1;
+            const int r = w.step(p, F - from_x, lo, hi) ? r_led : r_own, at = lo / CH * CH;
+            if (f + lane < f_end && lo < hi && r >= 0) page = p.page_table[(size_t)r * p.max_pages + at / kKvTile];
+            seen_x = lo - at | hi - at << 8;
+            src_x = p.cache + ((size_t)page * p.nkv + head) * C::TILE + at % kKvTile * 128;
             b0 += __shfl_sync(0xffffffffu, l, 31);
             base = __shfl_sync(0xffffffffu, base_l, 31);
-            to_ask = paged = __ballot_sync(0xffffffffu, page_x >= 0);
+            to_ask = paged = __ballot_sync(0xffffffffu, page >= 0 && page < p.num_pages);
             if (unit < 0) query_of(__shfl_sync(0xffffffffu, unit_x, 0));
         }
         // ---- copies run S chunks ahead
 #pragma unroll 1
         while (ok && to_ask && asked < it + S) {
             const int y = __ffs(to_ask) - 1, stage = asked % S;
-            const int page = __shfl_sync(0xffffffffu, page_x, y), at = __shfl_sync(0xffffffffu, lo_x, y) / CH * CH % kKvTile, h = __shfl_sync(0xffffffffu, head_x, y);
             uint8_t* dst = ring + stage * C::CHUNK_BYTES;
-            const uint8_t* src = p.cache + ((size_t)page * p.nkv + h) * C::TILE;
+            const uint8_t* src = (const uint8_t*)__shfl_sync(0xffffffffu, (unsigned long long)src_x, y);
             if (lane == 0) mbar_expect_tx(&full[stage], C::CHUNK_BYTES);
             if (CH == kKvTile) {
                 if (lane == 0) tma_bulk_g2s(dst, src, C::CHUNK_BYTES, &full[stage], pol);
             } else {                                                         // 2 D / 64 pieces, a lane each
                 __syncwarp();
-                if (lane < 2 * C::KH) tma_bulk_g2s(dst + lane * (CH * 128), src + lane * SH_PIECE + at * 128, CH * 128, &full[stage], pol);
+                if (lane < 2 * C::KH) tma_bulk_g2s(dst + lane * (CH * 128), src + lane * SH_PIECE, CH * 128, &full[stage], pol);
             }
             to_ask &= to_ask - 1;
             ++asked;
@@ -300,12 +301,12 @@ __device__ __forceinline__ void shared_own(const SharedArgs& p, const SharedGrou
         ok = __all_sync(0xffffffffu, shared_wait(&full[stage], it / S & 1, dead));
         if (!ok) continue;
         ++it;
-        const int lo = __shfl_sync(0xffffffffu, lo_x, x), hi = __shfl_sync(0xffffffffu, hi_x, x), at = lo / CH * CH;
+        const int seen = __shfl_sync(0xffffffffu, seen_x, x), lo = seen & 255, hi = seen >> 8;
         uint8_t* tile = ring + stage * C::CHUNK_BYTES;
-        if (lo > at || hi < at + CH) {                                       // hidden values may be anything: 0 * infinity is none
+        if (lo > 0 || hi < CH) {                                             // hidden values may be anything: 0 * infinity is none
 #pragma unroll 1
             for (int b = 0; b < CH; b += 16) {
-                const int from_t = lo - at - b, to_t = hi - at - b;
+                const int from_t = lo - b, to_t = hi - b;
                 if (from_t <= 0 && to_t >= 16) continue;
 #pragma unroll
                 for (int j = 0; j < D / 16; ++j) {
@@ -316,7 +317,7 @@ __device__ __forceinline__ void shared_own(const SharedArgs& p, const SharedGrou
             fence_proxy_async();                                             // ahead of the next copy into this stage
             __syncwarp();
         }
-        a.chunk(smem_u32(tile), lo - at, hi - at, p.scale_log2, lane);
+        a.chunk(smem_u32(tile), lo, hi, p.scale_log2, lane);
         __syncwarp();                                                        // all lanes have read it: the next copy may come
     }
     if (lane == 0)
@@ -844,9 +845,9 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
 }
 
 // ------------------------------------------------------------------ all parts of a (sequence, key head) as one
-constexpr int SM_THREADS = 256, SM_PARTS = 5;    // parts that a thread asks for at once
-template <int D>
-__global__ void __launch_bounds__(SM_THREADS, 4)
+constexpr int SM_PARTS = 5;                      // parts that a thread asks for at once
+template <int D, int SM_THREADS>
+__global__ void __launch_bounds__(SM_THREADS, 1024 / SM_THREADS)
 shared_merge_kernel(const __grid_constant__ SharedArgs p) {
     pdl_wait();
     __shared__ __align__(16) float acc_s[SM_THREADS * 4];
@@ -952,9 +953,12 @@ static int launch_shared(SharedArgs& p, cudaStream_t st) {
         FT_REQUIRE(a.numRegs >= SH_REGS, "ft_attn_decode_shared: built with %d registers a thread, its warps share out %d", a.numRegs, SH_REGS);
         attr_set.mark();
     }
-    p.chunk_log = C::CHUNK == 64 ? 6 : 5;
+    p.chunk_log = C::CHUNK == 64 ? 6 : 4;
     FT_CHECK_CUDA(launch_after(shared_attn_kernel<D>, dim3(device_sms()), dim3(SH_THREADS), C::SMEM, st, (const SharedArgs&)p));
-    FT_CHECK_CUDA(launch_after(shared_merge_kernel<D>, dim3(p.B * p.nkv), dim3(SM_THREADS), 0, st, (const SharedArgs&)p));
+    // few units: more threads for each one's parts (24 sequences x 8 key heads of 128, 20 parts each, 7.0 us with 256)
+    const int units = p.B * p.nkv;
+    if (units <= 2 * device_sms()) FT_CHECK_CUDA(launch_after(shared_merge_kernel<D, 512>, dim3(units), dim3(512), 0, st, (const SharedArgs&)p));
+    else FT_CHECK_CUDA(launch_after(shared_merge_kernel<D, 256>, dim3(units), dim3(256), 0, st, (const SharedArgs&)p));
     return 0;
 }
 
@@ -984,7 +988,7 @@ extern "C" int ft_attn_decode_shared(const ft_attn_shared_args* args, void* stre
     FT_REQUIRE(B >= 0 && n_groups >= 0 && num_pages >= 0 && table_rows >= 0 && max_pages >= 0 && max_pages < INT32_MAX / kKvTile && (double)B * nq * d <= INT32_MAX,
                "ft_attn_decode_shared: bad sizes B=%d nq=%d groups=%d table %d x %d, %d pages", B, nq, n_groups, table_rows, max_pages, num_pages);
     // both lists: at most so many units of at most so many steps, and what the shares are rounded up by
-    FT_REQUIRE(((double)B + 1) * nkv * (4.0 * max_pages + 4) + 65536 <= INT32_MAX && ((double)B / (2 * th) + n_groups) * nkv * (max_pages + kSharedStart + 1.0) + 65536 <= INT32_MAX,
+    FT_REQUIRE(((double)B + 1) * nkv * (8.0 * max_pages + 8) + 65536 <= INT32_MAX && ((double)B / (2 * th) + n_groups) * nkv * (max_pages + kSharedStart + 1.0) + 65536 <= INT32_MAX,
                "ft_attn_decode_shared: %d sequences of %d pages in %d groups are more than one call takes", B, max_pages, n_groups);
     if (B == 0) return 0;
     FT_REQUIRE(q && ctx_lens && out && scratch && (n_groups == 0 || (group_start && shared_lens)) && (page_table || table_rows == 0 || max_pages == 0) && (kv_layer || num_pages == 0),

@@ -27,7 +27,7 @@ struct SharedArgs {
     float2* rows_ml;
     int B, n_groups, num_pages, table_rows, max_pages, nq, nkv, G, th;        // th: queries of a half
     int rows;                                    // of the prefix's results
-    int chunk_log;                               // tokens of an own step: 2^6 or 2^5
+    int chunk_log;                               // tokens of an own step: 2^6 or 2^4
     unsigned inv_g;                              // row / G = row * inv_g >> 16 for a half's rows
     float scale_log2;
 

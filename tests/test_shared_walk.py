@@ -115,7 +115,7 @@ SHAPES = [
 
 
 @pytest.mark.parametrize("shape", range(len(SHAPES)))
-@pytest.mark.parametrize("G,chunk", [(1, 64), (3, 32), (4, 64), (8, 32)])
+@pytest.mark.parametrize("G,chunk", [(1, 64), (3, 16), (4, 64), (8, 16)])
 def test_shapes(lib, shape, G, chunk):
     ctx, starts, shared, max_pages, nkv = SHAPES[shape]
     for ctas in (1, 5, 148):
@@ -132,4 +132,4 @@ def test_random_batches(lib, seed):
     shared = [rng.randint(0, max_pages * 64 + 10) for _ in range(n)]
     ctx = [rng.randint(0, max_pages * 64 + 10) for _ in range(B)]
     ctas = rng.choice([3, 148])
-    check(lib, ctx, starts, shared, max_pages, rng.choice([1, 2, 8]), rng.randint(1, 8), rng.choice([32, 64]), ctas, ctas * rng.choice([3, 4]), unset=rng.randint(0, 1))
+    check(lib, ctx, starts, shared, max_pages, rng.choice([1, 2, 8]), rng.randint(1, 8), rng.choice([16, 64]), ctas, ctas * rng.choice([3, 4]), unset=rng.randint(0, 1))
