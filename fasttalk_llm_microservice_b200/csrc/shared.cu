@@ -26,6 +26,7 @@ static_assert(SH_REGS_ISSUE + 2 * SH_REGS_SOFT + SH_REGS_OWN <= 4 * SH_REGS, "wh
 constexpr int SH_SOFT = 256;
 constexpr int SH_TOLD = 4, SH_LISTENERS = 11;    // stretches told ahead; warps that hear of them
 constexpr int SH_LEAST = 4;
+constexpr int SH_COST = 2;                       // steps of the prefix that cost a warp on its SM one of its own
 constexpr int SH_LIST = 128;                     // groups whose lists are kept in shared memory
 constexpr int SH_PIECE = kKvTile * 128;          // [64 tokens][64 dims] in fp16
 
@@ -170,7 +171,7 @@ struct SharedQuery {
 // The share f0 .. f_end - 1 of the own list; sequence b0 begins at `base` of it, and the share in b0.  Thirty-two steps at a time, a lane each, the warp finds out what they
 // read; copies run ahead and results are written whichever sequences the steps belong to.
 template <int D>
-__device__ __forceinline__ void shared_own(const SharedArgs& p, const SharedGroups& gr, int f0, int f_end, int b0, int base, int per, int warp, uint8_t* ring, uint64_t* full,
+__device__ __forceinline__ void shared_own(const SharedArgs& p, const SharedGroups& gr, int f0, int f_end, int b0, int base, const OwnShares& shares, int warp, uint8_t* ring, uint64_t* full,
                                            volatile int* dead, int* err) {
     using C = Shared<D>;
     constexpr int S = C::OWN_STAGES, CH = C::CHUNK;
@@ -272,7 +273,7 @@ __device__ __forceinline__ void shared_own(const SharedArgs& p, const SharedGrou
                     a.m[0] = a.m[1] = 0.f;
                     sum[0] = sum[1] = NAN;
                 }
-                if (lane == 0 && from >= f0) p.own_units[unit] = make_int4(warp, (int)((unsigned)last / (unsigned)per), prefix, 0);
+                if (lane == 0 && from >= f0) p.own_units[unit] = make_int4(warp, shares.of(last), prefix, 0);
                 float* part = p.own_parts + (size_t)(unit + warp) * shared_part(G, D);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
@@ -413,7 +414,8 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
     // ---------------- the plan: every CTA adds up both lists, a run of groups and one of sequences a thread.  A list of groups that does not grow, or leaves the batch,
     // shares nothing
     SharedGroups gr{p.group_start, p.shared_lens, p.n_groups};
-    int prefix_f, prefix_end, prefix_per, own_per, own_total;
+    int prefix_f, prefix_end, prefix_per, own_total;
+    OwnShares shares;
     {
         const int gc = (p.n_groups + SH_THREADS - 1) / SH_THREADS, g0 = min(p.n_groups, tid * gc), g1 = min(p.n_groups, g0 + gc);
         const int bc = (p.B + SH_THREADS - 1) / SH_THREADS, b0 = min(p.B, tid * bc), b1 = min(p.B, b0 + bc);
@@ -451,10 +453,10 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
             __syncthreads();
         }
         own_total = all[1] * p.nkv;
-        const int warps = gridDim.x * C::OWN_WARPS;
-        own_per = (int)((unsigned)(own_total + warps - 1) / (unsigned)warps);
+        const int own_per = (int)((unsigned)(own_total + gridDim.x * C::OWN_WARPS - 1) / (gridDim.x * C::OWN_WARPS));
         // Prefix shares of four steps at least where the own ones are as long: half the results to put together
         prefix_per = max((int)((unsigned)(all[0] + gridDim.x - 1) / gridDim.x), min(SH_LEAST, own_per));
+        shares.set(own_total, C::OWN_WARPS, gridDim.x, (int)((unsigned)(all[0] + prefix_per - 1) / (unsigned)prefix_per), prefix_per / SH_COST);
         prefix_f = min(prefix_per * (int)blockIdx.x, all[0]);
         prefix_end = min(prefix_f + prefix_per, all[0]);
         if (before[0] <= prefix_f && prefix_f < before[0] + mine[0]) {
@@ -472,7 +474,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
         const int from = before[1] * p.nkv, to = from + mine[1] * p.nkv;
 #pragma unroll 1
         for (int w = 0; w < C::OWN_WARPS; ++w) {
-            const int f = own_per * (w * (int)gridDim.x + (int)blockIdx.x);  // (neighbouring shares on different SMs)
+            const int f = shares.begin(w, blockIdx.x);
             if (from <= f && f < to) {
                 int b = b0, at = from;
                 if (bc > 1)
@@ -822,8 +824,8 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SH_REGS_OWN));
         const int mine = warp - 12;
         if (mine < C::OWN_WARPS) {
-            const int index = mine * gridDim.x + blockIdx.x, f = min(own_per * index, own_total);
-            shared_own<D>(p, gr, f, min(f + own_per, own_total), own_at[mine].x, own_at[mine].y, own_per, index, smem + C::OWN + mine * (C::OWN_STAGES * C::CHUNK_BYTES), own_full + mine * C::OWN_STAGES, &dead, err);
+            const int f = min(shares.begin(mine, blockIdx.x), own_total);
+            shared_own<D>(p, gr, f, min(f + shares.size(blockIdx.x), own_total), own_at[mine].x, own_at[mine].y, shares, mine * gridDim.x + blockIdx.x, smem + C::OWN + mine * (C::OWN_STAGES * C::CHUNK_BYTES), own_full + mine * C::OWN_STAGES, &dead, err);
         }
     }
     tc_fence_before();

@@ -106,6 +106,31 @@ struct SharedSeq {
     }
 };
 
+// The own list's shares: `warps` of each CTA, the first `busy` CTAs (those with a share of the prefix list) shorter ones.  They follow one another CTA by CTA, then warp by
+// warp, so that neighbouring ones are on different SMs; none is empty, but for those behind the list's end.
+struct OwnShares {
+    int ctas, busy, few, many;
+    // as the prefix part takes the time of `cost` steps from each warp of its CTAs
+    __host__ __device__ __forceinline__ void set(int total, int warps, int ctas_, int busy_, int cost) {
+        ctas = ctas_;
+        busy = busy_;
+        const int each = (int)((unsigned)(total + warps - 1) / (unsigned)warps);         // steps of a round over all CTAs
+        few = many = (int)((unsigned)(each + ctas - 1) / (unsigned)ctas);
+        if (busy > 0 && busy < ctas) {
+            few = max(1, (int)((unsigned)(each + busy * cost + ctas - 1) / (unsigned)ctas) - cost);
+            many = max(1, (int)((unsigned)(max(0, each - busy * few) + ctas - busy - 1) / (unsigned)(ctas - busy)));
+        }
+    }
+    __host__ __device__ __forceinline__ int round() const { return busy * few + (ctas - busy) * many; }
+    __host__ __device__ __forceinline__ int size(int cta) const { return cta < busy ? few : many; }
+    __host__ __device__ __forceinline__ int begin(int warp, int cta) const { return warp * round() + (cta < busy ? cta * few : busy * few + (cta - busy) * many); }
+    // the share that step f lies in: warp * CTAs + CTA
+    __host__ __device__ __forceinline__ int of(int f) const {
+        const int warp = (int)((unsigned)f / (unsigned)round()), rest = f - warp * round(), far = rest - busy * few;
+        return warp * ctas + (far < 0 ? (int)((unsigned)rest / (unsigned)few) : busy + (int)((unsigned)far / (unsigned)many));
+    }
+};
+
 // n queries from q0 on, over pages p0 .. of the row of query seq0; row0: where the first one's results lie; last: the last share that the unit lies in
 struct SharedStretch {
     int p0, pages, n, h, seq0, q0, row0, tokens, last;

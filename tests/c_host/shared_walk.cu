@@ -5,10 +5,10 @@
 
 using namespace ft;
 
-// own: stretches of all warps, nine numbers each: warp, sequence, head, t0, t1, steps, prefix, first and last warp of the unit.
+// own: stretches of all warps (`warps` in each of `shares` CTAs, of which `busy` lose `cost` steps), nine numbers each: warp, sequence, head, t0, t1, steps, prefix, first and last warp of the unit.
 // else: of all CTAs: cta, group, head, tile, p0, pages, few, first and last CTA of the unit.  -> how many (at most `room` are written), or -1 - share where one is longer than `limit`
 extern "C" int shared_stretches(int own, const int* ctx_lens, int B, const int* starts, const int* shared, int n_groups, int max_pages, int nkv, int G, int chunk, int shares,
-                                int unset, int limit, int* out, int room) {
+                                int warps, int busy, int cost, int unset, int limit, int* out, int room) {
     SharedArgs p{};
     p.ctx_lens = ctx_lens, p.group_start = starts, p.shared_lens = shared;
     p.B = B, p.n_groups = n_groups, p.max_pages = max_pages, p.table_rows = B, p.nkv = nkv, p.nq = nkv * G, p.G = G, p.th = kSharedRows / G, p.chunk_log = chunk == 64 ? 6 : chunk == 32 ? 5 : 4;
@@ -28,12 +28,14 @@ extern "C" int shared_stretches(int own, const int* ctx_lens, int B, const int* 
         total += s.steps * nkv;
     }
     const int per = (int)((unsigned)(total + shares - 1) / (unsigned)shares);
+    OwnShares of;
+    of.set(total, warps, shares, busy, cost);
     auto tell = [&](const int* row) {
         if (found < room) memcpy(out + 9 * found, row, 9 * sizeof(int));
         ++found;
     };
-    for (int x = 0; x < shares; ++x) {
-        const int f = min(per * x, total), end = min(f + per, total);
+    for (int x = 0; x < (own ? shares * warps : shares); ++x) {
+        const int f = min(own ? of.begin(x / shares, x % shares) : per * x, total), end = min(f + (own ? of.size(x % shares) : per), total);
         int base = 0, at = 0;
         if (own) {                                   // step by step, as the kernel's lanes find them; told as stretches
             SharedSeq s;
@@ -44,7 +46,7 @@ extern "C" int shared_stretches(int own, const int* ctx_lens, int B, const int* 
             for (int F = f; F < end;) {
                 for (s.load(p, gr, at, ctx_lens[at]); F >= base + s.steps * nkv; s.load(p, gr, at, ctx_lens[at])) base += s.steps * nkv, ++at;
                 const int rest = F - base, h = rest / s.steps, t = rest - h * s.steps, take = min(s.steps - t, end - F), from = F - t;
-                const int row[9] = {x, at, h, t, t + take, s.steps, s.prefix, from / per, (from + s.steps - 1) / per};
+                const int row[9] = {x, at, h, t, t + take, s.steps, s.prefix, of.of(from), of.of(from + s.steps - 1)};
                 tell(row);
                 F += take;
             }

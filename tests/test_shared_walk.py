@@ -27,11 +27,11 @@ def at(a):
     return a.ctypes.data_as(C.c_void_p)
 
 
-def stretches(lib, own, ctx, starts, shared, max_pages, nkv, G, chunk, shares, unset=0):
+def stretches(lib, own, ctx, starts, shared, max_pages, nkv, G, chunk, shares, unset=0, warps=1, busy=0, cost=0):
     ctx, starts, shared = (np.asarray(v, np.int32) for v in (ctx, starts, shared))
     room = 200000
     out = np.zeros((room, 9), np.int32)
-    got = lib.shared_stretches(int(own), at(ctx), len(ctx), at(starts), at(shared), len(shared), max_pages, nkv, G, chunk, shares, unset, LIMIT, at(out), room)
+    got = lib.shared_stretches(int(own), at(ctx), len(ctx), at(starts), at(shared), len(shared), max_pages, nkv, G, chunk, shares, warps, busy, cost, unset, LIMIT, at(out), room)
     assert 0 <= got <= room, got
     return out[:got].tolist()
 
@@ -40,8 +40,8 @@ def grows(starts, B):
     return all(0 <= a <= b <= B for a, b in zip(starts, starts[1:]))
 
 
-def check(lib, ctx, starts, shared, max_pages, nkv, G, chunk, ctas=148, warps=592, unset=0):
-    B, reach = len(ctx), max_pages * 64
+def check(lib, ctx, starts, shared, max_pages, nkv, G, chunk, ctas=148, each=4, unset=0, busy=0, cost=0):
+    B, reach, warps = len(ctx), max_pages * 64, each * ctas
     n = len(shared) if grows(starts, B) else 0
     group = [next((g for g in range(n) if starts[g] <= b < starts[g + 1]), None) for b in range(B)]
     tokens = [max(0, min(s, reach)) for s in shared]
@@ -50,7 +50,7 @@ def check(lib, ctx, starts, shared, max_pages, nkv, G, chunk, ctas=148, warps=59
 
     # ---- own: tokens of every sequence, each once; a unit's shares follow one another
     units, last = {}, None
-    for warp, b, h, t0, t1, steps, prefix, first, end in stretches(lib, True, ctx, starts, shared, max_pages, nkv, G, chunk, warps, unset):
+    for warp, b, h, t0, t1, steps, prefix, first, end in stretches(lib, True, ctx, starts, shared, max_pages, nkv, G, chunk, ctas, unset, each, busy, cost):
         c, g = max(0, min(ctx[b], reach)), group[b]
         begin = tokens[g] if g is not None else 0
         assert prefix == (g is not None and pays[g] and c >= begin)
@@ -118,8 +118,8 @@ SHAPES = [
 @pytest.mark.parametrize("G,chunk", [(1, 64), (3, 16), (4, 64), (8, 16)])
 def test_shapes(lib, shape, G, chunk):
     ctx, starts, shared, max_pages, nkv = SHAPES[shape]
-    for ctas in (1, 5, 148):
-        check(lib, ctx, starts, shared, max_pages, nkv, G, chunk, ctas, 4 * ctas, unset=shape % 2)
+    for ctas, busy, cost in ((1, 0, 0), (1, 1, 5), (5, 2, 3), (148, 0, 0), (148, 148, 4), (148, 60, 4), (148, 147, 1)):
+        check(lib, ctx, starts, shared, max_pages, nkv, G, chunk, ctas, 4, unset=shape % 2, busy=busy, cost=cost)
 
 
 @pytest.mark.parametrize("seed", range(25))
@@ -132,4 +132,4 @@ def test_random_batches(lib, seed):
     shared = [rng.randint(0, max_pages * 64 + 10) for _ in range(n)]
     ctx = [rng.randint(0, max_pages * 64 + 10) for _ in range(B)]
     ctas = rng.choice([3, 148])
-    check(lib, ctx, starts, shared, max_pages, rng.choice([1, 2, 8]), rng.randint(1, 8), rng.choice([16, 64]), ctas, ctas * rng.choice([3, 4]), unset=rng.randint(0, 1))
+    check(lib, ctx, starts, shared, max_pages, rng.choice([1, 2, 8]), rng.randint(1, 8), rng.choice([16, 64]), ctas, rng.choice([3, 4]), unset=rng.randint(0, 1), busy=rng.randint(0, ctas), cost=rng.randint(0, 9))
