@@ -417,7 +417,8 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
     int prefix_f, prefix_end, prefix_per, own_total;
     OwnShares shares;
     {
-        const int gc = (p.n_groups + SH_THREADS - 1) / SH_THREADS, g0 = min(p.n_groups, tid * gc), g1 = min(p.n_groups, g0 + gc);
+        // (groups from the last threads back, so that few of them and few sequences are different warps' work)
+        const int gc = (p.n_groups + SH_THREADS - 1) / SH_THREADS, g0 = max(0, p.n_groups - (SH_THREADS - tid) * gc), g1 = max(0, p.n_groups - (SH_THREADS - 1 - tid) * gc);
         const int bc = (p.B + SH_THREADS - 1) / SH_THREADS, b0 = min(p.B, tid * bc), b1 = min(p.B, b0 + bc);
         const int ctx0 = b0 < b1 ? p.ctx_lens[b0] : 0;
         if (bc == 1 && b0 < b1 && p.req_slot) asm volatile("prefetch.global.L1 [%0];" ::"l"(p.req_slot + b0));       // the own warps look these up first
@@ -860,8 +861,11 @@ shared_merge_kernel(const __grid_constant__ SharedArgs p) {
     if (p.n_groups) pre = p.prefix_units[unit];
     if (!own.z) pre = make_int4(0, -1, 0, 0);                                // (then nobody has written there)
     // a thread has four dims of a head (neighbours the same of neighbouring heads, as the prefix's results lie), and every `lanes`-th part
-    const int size = G * D / 4, lanes = SM_THREADS / size, e = threadIdx.x % size, mine = threadIdx.x / size, hg = e % G, dim = e / G * 4;
-    const int n_own = own.y - own.x + 1, n = n_own + pre.y - pre.x + 1;
+    const int mine = (int)((threadIdx.x / (D / 4)) * p.inv_g >> 16), e = threadIdx.x - mine * (G * D / 4), lanes = (int)((SM_THREADS / (D / 4)) * p.inv_g >> 16);
+    const int quad = (int)(e * p.inv_g >> 16), hg = e - quad * G;
+    const int n_own = own.y - own.x + 1, n = n_own + pre.y - pre.x + 1, record = shared_part(G, D);
+    const float* const own0 = p.own_parts + (size_t)(unit + own.x) * record;
+    const size_t pre0 = (size_t)pre.z + (size_t)(2 * kSharedRows) * (pre.x - n_own) + hg;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float M = -INFINITY, L = 0.f;
     if (mine < lanes) {
@@ -871,28 +875,24 @@ shared_merge_kernel(const __grid_constant__ SharedArgs p) {
             float2 ml[SM_PARTS];
             float Mn = M;
 #pragma unroll
-            for (int u = 0; u < SM_PARTS; ++u) {
-                const int k = k0 + u * lanes;
-                ml[u] = make_float2(-INFINITY, 0.f);
-                o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (k < n_own) {
-                    const float* part = p.own_parts + (size_t)(unit + own.x + k) * shared_part(G, D);
-                    o[u] = __ldcg(reinterpret_cast<const float4*>(part + hg * D + dim));
-                    ml[u] = __ldcg(reinterpret_cast<const float2*>(part + G * D + 2 * hg));
-                } else if (k < n) {
-                    const size_t at = (size_t)pre.z + (size_t)2 * kSharedRows * (pre.x + k - n_own) + hg;
-                    o[u] = __ldcg(reinterpret_cast<const float4*>(p.rows_o) + (size_t)(dim / 4) * p.rows + at);
-                    ml[u] = __ldcg(p.rows_ml + at);
-                }
+            for (int u = 0; u < SM_PARTS; ++u) {                             // (behind the last part: it once more, with nothing to say)
+                const int k = min(k0 + u * lanes, n - 1);
+                const float* const part = own0 + (size_t)k * record;
+                const size_t at = pre0 + (size_t)(2 * kSharedRows) * k;
+                o[u] = __ldcg(k < n_own ? reinterpret_cast<const float4*>(part + hg * D + 4 * quad) : reinterpret_cast<const float4*>(p.rows_o) + (size_t)quad * p.rows + at);
+                ml[u] = __ldcg(k < n_own ? reinterpret_cast<const float2*>(part + G * D + 2 * hg) : p.rows_ml + at);
             }
 #pragma unroll
-            for (int u = 0; u < SM_PARTS; ++u) Mn = fmaxf(Mn, ml[u].x);
-            const float keep = M == -INFINITY ? 0.f : exp2f(M - Mn);
+            for (int u = 0; u < SM_PARTS; ++u) {
+                if (k0 + u * lanes >= n) ml[u].x = -INFINITY;
+                Mn = fmaxf(Mn, ml[u].x);
+            }
+            const float keep = M == -INFINITY ? 0.f : ex2_fast(M - Mn);
             L *= keep;
             acc.x *= keep, acc.y *= keep, acc.z *= keep, acc.w *= keep;
 #pragma unroll
             for (int u = 0; u < SM_PARTS; ++u) {
-                const float z = ml[u].x == -INFINITY ? 0.f : exp2f(ml[u].x - Mn);
+                const float z = ml[u].x == -INFINITY ? 0.f : ex2_fast(ml[u].x - Mn);
                 L = fmaf(ml[u].y, z, L);
                 acc = fma_f4(o[u], make_float4(z, z, z, z), acc);
             }
@@ -904,19 +904,19 @@ shared_merge_kernel(const __grid_constant__ SharedArgs p) {
     __syncthreads();
     if (mine) return;
 #pragma unroll 1
-    for (int x = 1; x < lanes; ++x) M = fmaxf(M, ml_s[x * size + e].x);
+    for (int x = 1; x < lanes; ++x) M = fmaxf(M, ml_s[x * (G * D / 4) + e].x);
     acc = make_float4(0.f, 0.f, 0.f, 0.f);
     L = 0.f;
 #pragma unroll 1
     for (int x = 0; x < lanes; ++x) {
-        const float2 ml = ml_s[x * size + e];
-        const float z = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
+        const float2 ml = ml_s[x * (G * D / 4) + e];
+        const float z = ml.x == -INFINITY ? 0.f : ex2_fast(ml.x - M);
         L = fmaf(ml.y, z, L);
-        acc = fma_f4(*reinterpret_cast<const float4*>(acc_s + 4 * (x * size + e)), make_float4(z, z, z, z), acc);
+        acc = fma_f4(*reinterpret_cast<const float4*>(acc_s + 4 * (x * (G * D / 4) + e)), make_float4(z, z, z, z), acc);
     }
     const float r = L == 0.f ? 0.f : 1.f / L;                                // a query without a visible key: zeros
     const float v[4] = {acc.x * r, acc.y * r, acc.z * r, acc.w * r};
-    const size_t at = ((size_t)(unit / p.nkv) * p.nq + (size_t)(unit % p.nkv) * G + hg) * D + dim;
+    const size_t at = ((size_t)unit * G + hg) * D + 4 * quad;                // (unit = sequence * key heads + key head)
     const uint2 hi = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
     *reinterpret_cast<uint2*>(p.out + at) = hi;
     if (p.out_lo)
@@ -1000,6 +1000,6 @@ extern "C" int ft_attn_decode_shared(const ft_attn_shared_args* args, void* stre
     uint8_t* w = (uint8_t*)scratch;
     SharedArgs p{(const __half*)q, (const uint8_t*)kv_layer, page_table, req_slot, ctx_lens, group_start, shared_lens, (__nv_bfloat16*)out, (__nv_bfloat16*)out_lo,
                  (int4*)(w + l.own_units), (int4*)(w + l.prefix_units), (float*)(w + l.own_parts), (float*)(w + l.rows_o), (float2*)(w + l.rows_ml), B, n_groups, num_pages, table_rows,
-                 max_pages, nq, nkv, G, th, (int)l.rows, 0, (65536u + G - 1) / G, kSharedLog2E / sqrtf((float)d)};
+                 max_pages, nq, nkv, G, th, (int)l.rows, 0, (65536u + G - 1) / G, kSharedLog2E / sqrtf((float)d), (unsigned)(((1ull << 32) + 2 * th - 1) / (2 * th))};
     return d == 64 ? launch_shared<64>(p, (cudaStream_t)stream) : launch_shared<128>(p, (cudaStream_t)stream);
 }

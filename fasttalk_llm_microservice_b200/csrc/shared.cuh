@@ -31,7 +31,11 @@ struct SharedArgs {
     unsigned inv_g;                              // row / G = row * inv_g >> 16 for a half's rows
     float scale_log2;
 
+    unsigned inv_tile;                           // 2^32 / (2 th), rounded up
+
     __host__ __device__ __forceinline__ int reach() const { return max_pages * kKvTile; }
+    // tiles of 2 th queries: exact for any batch that fits (up to 2^32 / (2 th) queries)
+    __host__ __device__ __forceinline__ int tiles(int size) const { return (int)((unsigned long long)(unsigned)(size + 2 * th - 1) * inv_tile >> 32); }
     __host__ __device__ __forceinline__ int row_of(int b) const {
         const int slot = req_slot ? req_slot[b] : b;
         return slot >= 0 && slot < table_rows ? slot : -1;
@@ -64,7 +68,7 @@ struct SharedPrefix {
         size = gr.start[g + 1] - seq0;
         tokens = gr.tokens(p, g);
         pages = gr.pays(p, g) ? (tokens + kKvTile - 1) / kKvTile : 0;
-        tiles = pages ? (int)((unsigned)(size + 2 * p.th - 1) / (unsigned)(2 * p.th)) : 0;
+        tiles = pages ? p.tiles(size) : 0;
     }
     __host__ __device__ __forceinline__ int queries(const SharedArgs& p, int tile) const { return min(2 * p.th, size - tile * 2 * p.th); }
     // steps of a tile of n queries: where they fill one half only, each half takes every other page

@@ -11,7 +11,7 @@ extern "C" int shared_stretches(int own, const int* ctx_lens, int B, const int* 
                                 int warps, int busy, int cost, int unset, int limit, int* out, int room) {
     SharedArgs p{};
     p.ctx_lens = ctx_lens, p.group_start = starts, p.shared_lens = shared;
-    p.B = B, p.n_groups = n_groups, p.max_pages = max_pages, p.table_rows = B, p.nkv = nkv, p.nq = nkv * G, p.G = G, p.th = kSharedRows / G, p.chunk_log = chunk == 64 ? 6 : chunk == 32 ? 5 : 4;
+    p.B = B, p.n_groups = n_groups, p.max_pages = max_pages, p.table_rows = B, p.nkv = nkv, p.nq = nkv * G, p.G = G, p.th = kSharedRows / G, p.inv_tile = (unsigned)(((1ull << 32) + 2 * p.th - 1) / (2 * p.th)), p.chunk_log = chunk == 64 ? 6 : chunk == 32 ? 5 : 4;
     bool grows = true;
     for (int g = 0; g < n_groups; ++g) grows = grows && starts[g] >= 0 && starts[g] <= starts[g + 1] && starts[g + 1] <= B;
     const int groups = grows ? n_groups : 0;
@@ -73,7 +73,7 @@ extern "C" int shared_stretches(int own, const int* ctx_lens, int B, const int* 
 extern "C" void shared_step(const int* ctx_lens, int B, int b, const int* starts, const int* shared, int n_groups, int max_pages, int chunk, int x, int* out) {
     SharedArgs p{};
     p.ctx_lens = ctx_lens, p.group_start = starts, p.shared_lens = shared;
-    p.B = B, p.n_groups = n_groups, p.max_pages = max_pages, p.nkv = 1, p.nq = 1, p.G = 1, p.th = kSharedRows, p.chunk_log = chunk == 64 ? 6 : chunk == 32 ? 5 : 4;
+    p.B = B, p.n_groups = n_groups, p.max_pages = max_pages, p.nkv = 1, p.nq = 1, p.G = 1, p.th = kSharedRows, p.inv_tile = (1u << 31) / kSharedRows, p.chunk_log = chunk == 64 ? 6 : chunk == 32 ? 5 : 4;
     SharedSeq s;
     s.load(p, SharedGroups{starts, shared, n_groups}, b, ctx_lens[b]);
     out[2] = s.step(p, x, out[0], out[1]) ? s.first : b;
@@ -82,8 +82,14 @@ extern "C" void shared_step(const int* ctx_lens, int B, int b, const int* starts
 // Where row 0 of (group, head, query i of the group) lies among the prefix's results
 extern "C" int shared_row(const int* starts, const int* shared, int g, int h, int i, int max_pages, int nkv, int G) {
     SharedArgs p{};
-    p.group_start = starts, p.shared_lens = shared, p.max_pages = max_pages, p.nkv = nkv, p.nq = nkv * G, p.G = G, p.th = kSharedRows / G;
+    p.group_start = starts, p.shared_lens = shared, p.max_pages = max_pages, p.nkv = nkv, p.nq = nkv * G, p.G = G, p.th = kSharedRows / G, p.inv_tile = (unsigned)(((1ull << 32) + 2 * p.th - 1) / (2 * p.th));
     SharedPrefix w;
     w.load(p, SharedGroups{starts, shared, 1 << 30}, g);
     return w.row(p, h, i);
+}
+
+extern "C" int shared_tiles(int G, int size) {
+    SharedArgs p{};
+    p.th = kSharedRows / G, p.inv_tile = (unsigned)(((1ull << 32) + 2 * p.th - 1) / (2 * p.th));
+    return p.tiles(size);
 }

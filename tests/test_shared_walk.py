@@ -133,3 +133,12 @@ def test_random_batches(lib, seed):
     ctx = [rng.randint(0, max_pages * 64 + 10) for _ in range(B)]
     ctas = rng.choice([3, 148])
     check(lib, ctx, starts, shared, max_pages, rng.choice([1, 2, 8]), rng.randint(1, 8), rng.choice([16, 64]), ctas, rng.choice([3, 4]), unset=rng.randint(0, 1), busy=rng.randint(0, ctas), cost=rng.randint(0, 9))
+
+
+@pytest.mark.parametrize("G", range(1, 9))
+def test_tiles_without_a_division(lib, G):
+    """The product with a reciprocal is the quotient for every batch that a call takes (B * G * 64 numbers of q below 2^31)."""
+    n, rng = 2 * (128 // G), random.Random(G)
+    most = 2 ** 31 // (64 * G)
+    sizes = {1, 2, n - 1, n, n + 1, most, most - 1} | {k * n + d for k in (rng.randint(1, most // n - 1) for _ in range(3000)) for d in (-1, 0, 1)}
+    assert all(lib.shared_tiles(G, s) == -(-s // n) for s in sizes)
