@@ -9,6 +9,8 @@
 //   own      a warp walks a share of its own: chunks of 16 or 8 KB by bulk copies that it asks for itself, two of them on their way while it multiplies (mma.sync, the
 //            query heads of a key head in the columns).  No warp waits for another.
 // Each share's results are O, maximum and sum of its rows; a second kernel puts them together in their order.
+#include <atomic>
+
 #include "common.cuh"
 #include "ft_internal.h"
 #include "shared.cuh"
@@ -27,7 +29,7 @@ constexpr int SH_SOFT = 256;
 constexpr int SH_TOLD = 4, SH_LISTENERS = 11;    // stretches told ahead; warps that hear of them
 constexpr int SH_LEAST = 4;
 constexpr int SH_COST = 2;                       // steps of the prefix that cost a warp on its SM one of its own
-constexpr int SH_LIST = 128;                     // groups whose lists are kept in shared memory
+constexpr int SH_LIST = 100;                     // groups whose lists are kept in shared memory
 constexpr int SH_PIECE = kKvTile * 128;          // [64 tokens][64 dims] in fp16
 
 __device__ int g_shared_waits;                   // 1: a wait ran out on this device (ft_attn_shared_waits)
@@ -47,7 +49,7 @@ struct Shared {
     // tensor memory: scores [half][2][64 columns] (probabilities, pairs of fp16, over the first 32 of them), O [half][D]
     static constexpr int COL_S = 0, COL_O = 256, COLS = 512;
     static_assert(COL_O + 2 * D <= COLS, "tensor memory");
-    static_assert(SMEM <= 232448 - 1792, "shared memory");
+    static_assert(SMEM <= 232448 - 2048, "shared memory (the rest is what the kernel declares)");
 };
 
 // A wait that ends, in a few instructions: what bounds calls of ten microseconds here is among others how much code they touch for the first time (126 KB, with waits and
@@ -342,30 +344,37 @@ struct SharedPhases {
     }
 };
 
-// Exclusive sums of two numbers over the block's threads, and whether all say yes; `all` the sums of all
-__device__ __forceinline__ bool shared_before(const int* mine, int (*warp_s)[SH_WARPS], int* before, int* all, bool yes) {
+// Exclusive sums of four numbers over the block's threads, and whether all say yes; `all` the sums of all
+__device__ __forceinline__ bool shared_before(const int* mine, int (*warp_s)[4], int* before, int* all, bool yes) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int x[2] = {mine[0], mine[1]};
+    int x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = mine[k];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1)
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+        for (int k = 0; k < 4; ++k) {
             const int up = __shfl_up_sync(0xffffffffu, x[k], o);
             if (lane >= o) x[k] += up;
         }
-    if (lane == 31) warp_s[0][warp] = x[0], warp_s[1][warp] = x[1];
+    if (lane == 31)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) warp_s[warp][k] = x[k];
     yes = __syncthreads_and(yes);
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        int w = lane < SH_WARPS ? warp_s[k][lane] : 0;
+    for (int k = 0; k < 4; ++k) {
+        before[k] = x[k] - mine[k];
+        all[k] = 0;
+    }
+#pragma unroll 4
+    for (int w = 0; w < SH_WARPS; ++w) {                                     // (one 16-byte read a warp, the same for all lanes)
+        const int4 v = *reinterpret_cast<const int4*>(warp_s[w]);
+        const int s[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int o = 1; o < SH_WARPS; o <<= 1) {
-            const int up = __shfl_up_sync(0xffffffffu, w, o);
-            if (lane >= o) w += up;
+        for (int k = 0; k < 4; ++k) {
+            if (w < warp) before[k] += s[k];
+            all[k] += s[k];
         }
-        all[k] = __shfl_sync(0xffffffffu, w, SH_WARPS - 1);
-        const int ahead = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
-        before[k] = x[k] - mine[k] + (warp ? ahead : 0);
     }
     return yes;
 }
@@ -385,7 +394,8 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
     __shared__ SharedStretch told[SH_TOLD];
     __shared__ uint64_t drained[2];                                          // all products of a half retired
     __shared__ int tokens_s[C::TOKENS];                                      // of the last pages copied; 0: the page is not there
-    __shared__ int sums_s[2][SH_WARPS], start_s[SH_LIST + 1], lens_s[SH_LIST];
+    __shared__ __align__(16) int sums_s[SH_WARPS][4];
+    __shared__ int start_s[SH_LIST + 1], lens_s[SH_LIST];
     __shared__ int2 prefix_at, own_at[C::OWN_WARPS];                         // the group (sequence) that a share begins in, and where that begins
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int dead;
@@ -413,7 +423,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
 
     // ---------------- the plan: every CTA adds up both lists, a run of groups and one of sequences a thread.  A list of groups that does not grow, or leaves the batch,
     // shares nothing
-    SharedGroups gr{p.group_start, p.shared_lens, p.n_groups};
+    SharedGroups gr{p.group_start, p.shared_lens, p.n_groups, true};
     int prefix_f, prefix_end, prefix_per, own_total;
     OwnShares shares;
     {
@@ -429,29 +439,39 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
             gr.lens = lens_s;
         }
         __syncthreads();
-        auto steps_of = [&](int b) {
-            SharedSeq s;
-            s.load(p, gr, b, b == b0 ? ctx0 : p.ctx_lens[b]);
-            return s.steps;
-        };
         bool grows = true;
-        int mine[2], before[2], all[2];
+        // prefix steps and own steps where prefixes are shared, own steps where they are not, pages saved
+        int mine[4], before[4], all[4];
 #pragma unroll 1
         for (int g = g0; g < g1; ++g) grows = grows && gr.start[g] >= 0 && gr.start[g] <= gr.start[g + 1] && gr.start[g + 1] <= p.B;
 #pragma unroll 1
         for (;;) {
-            mine[0] = mine[1] = 0;
+            mine[0] = mine[1] = mine[2] = mine[3] = 0;
 #pragma unroll 1
             for (int g = g0; g < g1 && grows && gr.n; ++g) {
                 SharedPrefix w;
                 w.load(p, gr, g);
                 mine[0] += w.all(p);
+                mine[3] = min(mine[3] + gr.saves(p, g), 1 << 20);
             }
 #pragma unroll 1
-            for (int b = b0; b < b1; ++b) mine[1] += steps_of(b);
+            for (int b = b0; b < b1; ++b) {
+                SharedSeq s;
+                s.load(p, gr, b, b == b0 ? ctx0 : p.ctx_lens[b]);
+                mine[1] += s.steps;
+                mine[2] += s.steps_alone(p);
+            }
             if (shared_before(mine, sums_s, before, all, grows) || gr.n == 0) break;
             gr.n = 0;
             __syncthreads();
+        }
+        // Sharing costs a call about 2 us, and a step of the prefix more than an own one (least_size, least_pages: launch_shared)
+        gr.share = all[3] >= p.least_pages;
+        if (!gr.share) {
+            mine[0] = all[0] = 0;
+            mine[1] = mine[2];
+            before[1] = before[2];
+            all[1] = all[2];
         }
         own_total = all[1] * p.nkv;
         const int own_per = (int)((unsigned)(own_total + gridDim.x * C::OWN_WARPS - 1) / (gridDim.x * C::OWN_WARPS));
@@ -480,7 +500,12 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
                 int b = b0, at = from;
                 if (bc > 1)
 #pragma unroll 1
-                    for (int n; f >= at + (n = steps_of(b) * p.nkv); ++b) at += n;
+                    for (;; ++b) {
+                        SharedSeq s;
+                        s.load(p, gr, b, p.ctx_lens[b]);
+                        if (f < at + s.steps * p.nkv) break;
+                        at += s.steps * p.nkv;
+                    }
                 own_at[w] = make_int2(b, at);
             }
         }
@@ -944,6 +969,8 @@ static SharedLayout shared_layout(int B, int n_groups, int nq, int nkv, int d) {
     return l;
 }
 
+static std::atomic<long long> g_shared_least{-1};
+
 template <int D>
 static int launch_shared(SharedArgs& p, cudaStream_t st) {
     using C = Shared<D>;
@@ -956,6 +983,13 @@ static int launch_shared(SharedArgs& p, cudaStream_t st) {
         attr_set.mark();
     }
     p.chunk_log = C::CHUNK == 64 ? 6 : 4;
+    // What sharing has to save, measured with one group and 100 own tokens each, us shared / not: heads of 64 (32 over 8), two sequences of 8000 tokens 16.2 / 14.4, four of
+    // 2000 13.7 / 12.6 (16 MB saved), four of 8000 16.3 / 17.1, sixteen of 130 11.6 / 10.5, of 517 12.1 / 13.6; heads of 128 (32 over 8), two of 2000 15.2 / 15.5 (8 MB), four of
+    // 130 12.6 / 10.7, of 517 12.8 / 13.4 (6 MB); sixteen key heads, two of 517 14.1 / 13.5, four of 130 13.6 / 12.2, of 517 14.2 / 15.7.  At heads of 64 a step of the prefix takes as
+    // long as two own ones.
+    const long long least = g_shared_least.load(std::memory_order_relaxed), pages = (least < 0 ? (D == 64 ? 12 : 6) << 20 : least) / ((long long)C::TILE * p.nkv);
+    p.least_size = D == 64 && least < 0 ? 3 : 2;
+    p.least_pages = (int)(pages < INT32_MAX ? pages : INT32_MAX) + (least < 0);
     FT_CHECK_CUDA(launch_after(shared_attn_kernel<D>, dim3(device_sms()), dim3(SH_THREADS), C::SMEM, st, (const SharedArgs&)p));
     // few units: more threads for each one's parts (24 sequences x 8 key heads of 128, 20 parts each, 7.0 us with 256)
     const int units = p.B * p.nkv;
@@ -972,6 +1006,8 @@ extern "C" long long ft_attn_decode_shared_scratch_bytes(int B, int n_groups, in
     FT_REQUIRE(B >= 0 && n_groups >= 0 && (double)B * nq * d <= INT32_MAX, "ft_attn_decode_shared_scratch_bytes: bad sizes B=%d nq=%d groups=%d", B, nq, n_groups);
     return (long long)ft::shared_layout(B, n_groups, nq, nkv, d).bytes;
 }
+
+extern "C" void ft_attn_shared_set_least(long long bytes) { ft::g_shared_least = bytes < 0 ? -1 : bytes; }
 
 extern "C" int ft_attn_shared_waits(void) {
     int n = 0;
@@ -1000,6 +1036,6 @@ extern "C" int ft_attn_decode_shared(const ft_attn_shared_args* args, void* stre
     uint8_t* w = (uint8_t*)scratch;
     SharedArgs p{(const __half*)q, (const uint8_t*)kv_layer, page_table, req_slot, ctx_lens, group_start, shared_lens, (__nv_bfloat16*)out, (__nv_bfloat16*)out_lo,
                  (int4*)(w + l.own_units), (int4*)(w + l.prefix_units), (float*)(w + l.own_parts), (float*)(w + l.rows_o), (float2*)(w + l.rows_ml), B, n_groups, num_pages, table_rows,
-                 max_pages, nq, nkv, G, th, (int)l.rows, 0, (65536u + G - 1) / G, kSharedLog2E / sqrtf((float)d), (unsigned)(((1ull << 32) + 2 * th - 1) / (2 * th))};
+                 max_pages, nq, nkv, G, th, (int)l.rows, 0, (65536u + G - 1) / G, kSharedLog2E / sqrtf((float)d), (unsigned)(((1ull << 32) + 2 * th - 1) / (2 * th)), 0, 0};
     return d == 64 ? launch_shared<64>(p, (cudaStream_t)stream) : launch_shared<128>(p, (cudaStream_t)stream);
 }

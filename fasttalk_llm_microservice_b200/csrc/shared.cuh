@@ -4,8 +4,8 @@
 // the rest of its ctx keys on its own.  Two kinds of work come of that:
 //   prefix   a unit = one group, key head and tile of queries; its steps are the pages of the prefix, read once for all queries of the tile
 //   own      a unit = one sequence and key head; its steps are chunks of its own pages
-// A group that does not pay has no prefix units: its sequences read the first row's pages themselves, as steps ahead of their own.  Both lists are cut into equal
-// shares, the prefix list one for each SM, the own list one for each warp that walks it.  Plain arithmetic, the same on the host.
+// A group that does not pay has no prefix units: its sequences read the first row's pages themselves, as steps ahead of their own.  The prefix list is cut into equal shares,
+// one for each SM, the own list into one for each warp that walks it.  Plain arithmetic, the same on the host.
 #pragma once
 #include "common.cuh"
 
@@ -32,6 +32,7 @@ struct SharedArgs {
     float scale_log2;
 
     unsigned inv_tile;                           // 2^32 / (2 th), rounded up
+    int least_size, least_pages;                 // sharing pays: queries of a group; pages that the call's groups save in all
 
     __host__ __device__ __forceinline__ int reach() const { return max_pages * kKvTile; }
     // tiles of 2 th queries: exact for any batch that fits (up to 2^32 / (2 th) queries)
@@ -42,13 +43,19 @@ struct SharedArgs {
     }
 };
 
-// The groups, wherever the lists lie; n = 0: none
+// The groups, wherever the lists lie; n = 0: none.  share: their prefixes are read once
 struct SharedGroups {
     const int *start, *lens;
     int n;
+    bool share;
     __host__ __device__ __forceinline__ int tokens(const SharedArgs& p, int g) const { return max(0, min(lens[g], p.reach())); }
     // whether group g has a prefix part
-    __host__ __device__ __forceinline__ bool pays(const SharedArgs& p, int g) const { return start[g + 1] - start[g] >= 2 && tokens(p, g) >= 2 * kKvTile; }
+    __host__ __device__ __forceinline__ bool pays(const SharedArgs& p, int g) const { return share && start[g + 1] - start[g] >= p.least_size && tokens(p, g) >= 2 * kKvTile; }
+    // pages that sharing saves group g (up to a million), beyond what it costs
+    __host__ __device__ __forceinline__ int saves(const SharedArgs& p, int g) const {
+        const long long n = (long long)(start[g + 1] - start[g] - p.least_size + 1) * (tokens(p, g) / kKvTile);
+        return !pays(p, g) ? 0 : n < 1 << 20 ? (int)n : 1 << 20;
+    }
     // the last group that begins at or before b (those without queries begin where the next one does), or -1
     __host__ __device__ __forceinline__ int of(int b) const {
         int lo = -1, hi = n - 1;
@@ -100,6 +107,8 @@ struct SharedSeq {
         const int own = ctx > begin ? (ctx + up >> p.chunk_log) - (begin >> p.chunk_log) : 0;
         steps = max(1, lead + own);
     }
+    // its steps where its group had no prefix part
+    __host__ __device__ __forceinline__ int steps_alone(const SharedArgs& p) const { return prefix ? steps - (ctx == begin) + (begin + (1 << p.chunk_log) - 1 >> p.chunk_log) : steps; }
     // tokens lo .. hi - 1 that step t reads (none: lo >= hi); true: on the first row's pages
     __host__ __device__ __forceinline__ bool step(const SharedArgs& p, int t, int& lo, int& hi) const {
         const bool led = t < lead;

@@ -746,6 +746,8 @@ int ft_norm_rope_kv_append(const ft_norm_append_args* args, void* stream);
  * that is not read, and what lies on a row's pages ahead of its first own token or behind its last may be anything.  req_slot NULL: row b.  A list group_start that
  * does not grow or leaves [0, B] makes no groups.  A query that sees no key gives zeros.  Probabilities are rounded to fp16 down to 2^-30 of the largest.
  * scratch: work memory of ft_attn_decode_shared_scratch_bytes bytes (of the current device), in any state, not shared by calls that may overlap.
+ * A prefix is read once where the call's groups save enough by that (12 MB at heads of 64, counted from the third query of a group on, 6 MB at 128, from the second on), else by
+ * every query; ft_attn_shared_set_least: what they have to save in the calls that follow, 0: nothing (below 0: the library's own).  Results are the same but for rounding.
  * ft_attn_shared_waits: 1 if a wait inside one of its kernels has run out on the current device since the library was loaded (rows of some call mean nothing), else 0;
  * waits for all that the device has been given, on every stream. */
 long long ft_attn_decode_shared_scratch_bytes(int B, int n_groups, int nq, int nkv, int d);
@@ -757,6 +759,7 @@ typedef struct {
 } ft_attn_shared_args;
 int ft_attn_decode_shared(const ft_attn_shared_args* args, void* stream);
 int ft_attn_shared_waits(void);
+void ft_attn_shared_set_least(long long bytes);
 
 /* K7: per-row temperature / top-k / top-p sampling (argmax when temperature <= 0; a null temperature says so for all rows).
  * A row without any logit above minus infinity gives index 0. */

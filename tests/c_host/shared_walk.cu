@@ -8,14 +8,15 @@ using namespace ft;
 // own: stretches of all warps (`warps` in each of `shares` CTAs, of which `busy` lose `cost` steps), nine numbers each: warp, sequence, head, t0, t1, steps, prefix, first and last warp of the unit.
 // else: of all CTAs: cta, group, head, tile, p0, pages, few, first and last CTA of the unit.  -> how many (at most `room` are written), or -1 - share where one is longer than `limit`
 extern "C" int shared_stretches(int own, const int* ctx_lens, int B, const int* starts, const int* shared, int n_groups, int max_pages, int nkv, int G, int chunk, int shares,
-                                int warps, int busy, int cost, int unset, int limit, int* out, int room) {
+                                int warps, int busy, int cost, int share, int unset, int limit, int* out, int room) {
     SharedArgs p{};
     p.ctx_lens = ctx_lens, p.group_start = starts, p.shared_lens = shared;
     p.B = B, p.n_groups = n_groups, p.max_pages = max_pages, p.table_rows = B, p.nkv = nkv, p.nq = nkv * G, p.G = G, p.th = kSharedRows / G, p.inv_tile = (unsigned)(((1ull << 32) + 2 * p.th - 1) / (2 * p.th)), p.chunk_log = chunk == 64 ? 6 : chunk == 32 ? 5 : 4;
     bool grows = true;
     for (int g = 0; g < n_groups; ++g) grows = grows && starts[g] >= 0 && starts[g] <= starts[g + 1] && starts[g + 1] <= B;
     const int groups = grows ? n_groups : 0;
-    const SharedGroups gr{starts, shared, grows ? n_groups : 0};
+    p.least_size = 2;
+    const SharedGroups gr{starts, shared, grows ? n_groups : 0, share != 0};
     int total = 0, found = 0;
     for (int g = 0; !own && g < gr.n; ++g) {
         SharedPrefix w;
@@ -26,6 +27,9 @@ extern "C" int shared_stretches(int own, const int* ctx_lens, int B, const int* 
         SharedSeq s;
         s.load(p, gr, b, ctx_lens[b]);
         total += s.steps * nkv;
+        SharedSeq alone;
+        alone.load(p, SharedGroups{starts, shared, grows ? n_groups : 0, false}, b, ctx_lens[b]);
+        if (alone.steps != s.steps_alone(p)) return -1000000;
     }
     const int per = (int)((unsigned)(total + shares - 1) / (unsigned)shares);
     OwnShares of;
@@ -70,12 +74,13 @@ extern "C" int shared_stretches(int own, const int* ctx_lens, int B, const int* 
 }
 
 // What step x of a sequence reads: lo, hi, query
-extern "C" void shared_step(const int* ctx_lens, int B, int b, const int* starts, const int* shared, int n_groups, int max_pages, int chunk, int x, int* out) {
+extern "C" void shared_step(const int* ctx_lens, int B, int b, const int* starts, const int* shared, int n_groups, int max_pages, int chunk, int share, int x, int* out) {
     SharedArgs p{};
     p.ctx_lens = ctx_lens, p.group_start = starts, p.shared_lens = shared;
     p.B = B, p.n_groups = n_groups, p.max_pages = max_pages, p.nkv = 1, p.nq = 1, p.G = 1, p.th = kSharedRows, p.inv_tile = (1u << 31) / kSharedRows, p.chunk_log = chunk == 64 ? 6 : chunk == 32 ? 5 : 4;
     SharedSeq s;
-    s.load(p, SharedGroups{starts, shared, n_groups}, b, ctx_lens[b]);
+    p.least_size = 2;
+    s.load(p, SharedGroups{starts, shared, n_groups, share != 0}, b, ctx_lens[b]);
     out[2] = s.step(p, x, out[0], out[1]) ? s.first : b;
 }
 
@@ -84,7 +89,7 @@ extern "C" int shared_row(const int* starts, const int* shared, int g, int h, in
     SharedArgs p{};
     p.group_start = starts, p.shared_lens = shared, p.max_pages = max_pages, p.nkv = nkv, p.nq = nkv * G, p.G = G, p.th = kSharedRows / G, p.inv_tile = (unsigned)(((1ull << 32) + 2 * p.th - 1) / (2 * p.th));
     SharedPrefix w;
-    w.load(p, SharedGroups{starts, shared, 1 << 30}, g);
+    w.load(p, SharedGroups{starts, shared, 1 << 30, true}, g);
     return w.row(p, h, i);
 }
 

@@ -308,6 +308,15 @@ def test_append_of_nothing(K):
 
 
 # ------------------------------------------------------------------------------------------------ attention
+@pytest.fixture(params=["always", "as it pays", "never"])
+def sharing(K, request):
+    """Prefixes read once whatever that saves, where it saves enough, and not at all."""
+    set_least = K.N.load().ft_attn_shared_set_least
+    set_least({"always": 0, "as it pays": -1, "never": 2 ** 62}[request.param])
+    yield request.param
+    set_least(-1)
+
+
 def make(case_seed, nq, nkv, d, sizes, shared, own, hidden=NAN, extra_rows=2, ctx=None):
     """A batch: groups of sizes[g] queries with shared[g] tokens in common and own[i] more each (below 0: the context ends inside what they share); queries behind the last
     group stand alone.  Whatever nobody sees is `hidden`."""
@@ -416,25 +425,25 @@ SHAPES = [
 
 @pytest.mark.parametrize("nq,nkv,d", HEADS)
 @pytest.mark.parametrize("shape", range(len(SHAPES)))
-def test_attention(K, nq, nkv, d, shape):
+def test_attention(K, sharing, nq, nkv, d, shape):
     sizes, shared, own = SHAPES[shape]
     check(K, make(shape * 31 + d + nq, nq, nkv, d, sizes, shared, own), 1 + shape % 2)
 
 
 @pytest.mark.parametrize("d", [64, 128])
-def test_a_long_prefix_and_long_tails(K, d):
+def test_a_long_prefix_and_long_tails(K, sharing, d):
     check(K, make(1, 8, 2, d, [6], [9001], [4000, 0, 77, 2000, 1, 640]))
     check(K, make(2, 4, 4, d, [3, 3], [5000, 64], [3, 0, 6400, 1, 2, 3]))
 
 
 @pytest.mark.parametrize("d", [64, 128])
-def test_what_is_hidden_may_be_infinite(K, d):
+def test_what_is_hidden_may_be_infinite(K, sharing, d):
     for hidden in (math.inf, -math.inf, 65504.0, None):
         check(K, make(3, 8, 2, d, [5, 2], [333, 1000], [0, 5, -300, 64, 100, 7, -1000], hidden))
 
 
 @pytest.mark.parametrize("d", [64, 128])
-def test_pages_and_rows_that_are_not_there(K, d):
+def test_pages_and_rows_that_are_not_there(K, sharing, d):
     s = make(4, 8, 2, d, [5, 3], [700, 400], [10, 200, 0, 64, 65, 1, 130, 3], hidden=0.5)
     t, w = s["table"], s["slots"].long()
     t[w[0], 3], t[w[0], 5], t[w[1], 12], t[w[3], 11], t[w[5], 0] = -1, 10 ** 6, 2 ** 31 - 1, -2 ** 31, s["cache"].shape[0]
@@ -452,14 +461,14 @@ def test_pages_and_rows_that_are_not_there(K, d):
     check(K, s)
 
 
-def test_lists_of_groups_that_do_not_grow_share_nothing(K):
+def test_lists_of_groups_that_do_not_grow_share_nothing(K, sharing):
     for starts in ([0, 5, 3], [-1, 4, 8], [0, 4, 9], [2, 2, -7], [2 ** 31 - 1, 0, 8], [8, 8, 0]):
         s = make(5, 8, 2, 64, [], [], [300, 200, 100, 400, 64, 1, 0, 500])
         s["starts"], s["shared"] = i32(starts), i32([128, 64])
         check(K, s)
 
 
-def test_groups_in_the_middle_of_the_batch(K):
+def test_groups_in_the_middle_of_the_batch(K, sharing):
     s = make(6, 8, 2, 128, [3, 4], [300, 500], [5, 6, 7, 8, 9, 70, 80, 100, 90])
     lone = make(7, 8, 2, 128, [], [], [100, 50])
     P = s["cache"].shape[0]
@@ -472,14 +481,14 @@ def test_groups_in_the_middle_of_the_batch(K):
     check(K, both)
 
 
-def test_rows_in_order(K):
+def test_rows_in_order(K, sharing):
     s = make(8, 8, 2, 64, [4], [200], [5, 64, 0, 70], extra_rows=0)
     t = s["table"][s["slots"].long()].contiguous()
     check(K, s | {"table": t, "slots": None})
     check(K, s | {"table": t[:2].contiguous(), "slots": None})                       # fewer rows than queries: the others have no page of their own
 
 
-def test_empty_batches_tables_and_caches(K):
+def test_empty_batches_tables_and_caches(K, sharing):
     z = lambda *n: torch.zeros(*n, device=DEV, dtype=torch.int32)
     cache = torch.randn(2, 2, 2, 64, 64, device=DEV).half()
     hi, lo = K.attn_decode_shared(torch.zeros(0, 4, 64, device=DEV).half(), cache, z(0, 3), z(0), z(1), z(0))
@@ -491,7 +500,7 @@ def test_empty_batches_tables_and_caches(K):
 
 
 @pytest.mark.parametrize("d", [64, 128])
-def test_scores_far_apart(K, d):
+def test_scores_far_apart(K, sharing, d):
     """Scores of hundreds, the largest key late, early, in the prefix, in the tail: the reference moves, and parts with nothing to say drop out."""
     for where in range(6):
         s = make(20 + where, 8, 2, d, [4, 2], [900, 300], [100, 0, 64, 300, 1, 500], hidden=None)
@@ -507,7 +516,7 @@ def test_scores_far_apart(K, d):
         close(got, want, tol * 8 + 0.02, 2)                                         # products of up to 128 * 6 * 12 in all: 2^-24 of them and 4 * 128 in the exponent
 
 
-def test_runs_agree_with_themselves_and_with_plain_decode(K):
+def test_runs_agree_with_themselves_and_with_plain_decode(K, sharing):
     s = make(9, 32, 8, 64, [20, 20], [1000, 700], [i * 13 % 200 + 1 for i in range(40)])
     a = check(K, s)
     for _ in range(3):
@@ -532,7 +541,7 @@ def test_runs_agree_with_themselves_and_with_plain_decode(K):
     close((hi, lo), want, tol * 2, 2)
 
 
-def test_two_calls_at_once_and_other_streams(K):
+def test_two_calls_at_once_and_other_streams(K, sharing):
     a, b = make(10, 8, 2, 64, [9], [900], [i * 30 for i in range(9)]), make(11, 8, 2, 128, [30], [2000], [i for i in range(30)])
     wa, wb = attention(a), attention(b)
     torch.cuda.synchronize()
@@ -549,7 +558,7 @@ def test_two_calls_at_once_and_other_streams(K):
 
 @pytest.mark.parametrize("nq,nkv,d,sizes,shared,own", [(12, 4, 128, [8, 9, 6, 7, 7], [4099, 2500, 3300, 1640, 2880], 500), (32, 8, 128, [24], [16001], 200), (32, 8, 64, [20, 44], [6000, 900], 300),
                                                      (16, 4, 128, [64, 60], [1500, 800], 80)])
-def test_many_calls_behind_one_another(K, nq, nkv, d, sizes, shared, own):
+def test_many_calls_behind_one_another(K, sharing, nq, nkv, d, sizes, shared, own):
     """Pages that land late, as they do beside other copies and calls, are waited for: every call says the same."""
     s = make(30, nq, nkv, d, sizes, shared, [i * 97 % own for i in range(sum(sizes))], hidden=0.5)
     run = lambda: K.attn_decode_shared(s["q"], s["cache"], s["table"], s["ctx"], s["starts"], s["shared"], s["slots"])
@@ -562,7 +571,7 @@ def test_many_calls_behind_one_another(K, nq, nkv, d, sizes, shared, own):
     K.attn_shared_check()
 
 
-def test_captured_and_replayed(K):
+def test_captured_and_replayed(K, sharing):
     s = make(12, 8, 2, 64, [5, 4], [500, 900], [10, 70, 0, 130, 5, 6, 64, 1, 300], hidden=0.25)
     run = lambda: K.attn_decode_shared(s["q"], s["cache"], s["table"], s["ctx"], s["starts"], s["shared"], s["slots"])
     run()
@@ -582,7 +591,7 @@ def test_captured_and_replayed(K):
             close(out, want, tol, 2)
 
 
-def test_a_run_of_all_three(K):
+def test_a_run_of_all_three(K, sharing):
     """Four steps of a batch on one prompt: the prompt written once, then lists, append and attention as one graph a step, replayed."""
     g = gen(77)
     nq, nkv, d, B, prompt = 8, 2, 64, 6, 200

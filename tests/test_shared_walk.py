@@ -27,11 +27,11 @@ def at(a):
     return a.ctypes.data_as(C.c_void_p)
 
 
-def stretches(lib, own, ctx, starts, shared, max_pages, nkv, G, chunk, shares, unset=0, warps=1, busy=0, cost=0):
+def stretches(lib, own, ctx, starts, shared, max_pages, nkv, G, chunk, shares, unset=0, warps=1, busy=0, cost=0, share=1):
     ctx, starts, shared = (np.asarray(v, np.int32) for v in (ctx, starts, shared))
     room = 200000
     out = np.zeros((room, 9), np.int32)
-    got = lib.shared_stretches(int(own), at(ctx), len(ctx), at(starts), at(shared), len(shared), max_pages, nkv, G, chunk, shares, warps, busy, cost, unset, LIMIT, at(out), room)
+    got = lib.shared_stretches(int(own), at(ctx), len(ctx), at(starts), at(shared), len(shared), max_pages, nkv, G, chunk, shares, warps, busy, cost, share, unset, LIMIT, at(out), room)
     assert 0 <= got <= room, got
     return out[:got].tolist()
 
@@ -40,17 +40,17 @@ def grows(starts, B):
     return all(0 <= a <= b <= B for a, b in zip(starts, starts[1:]))
 
 
-def check(lib, ctx, starts, shared, max_pages, nkv, G, chunk, ctas=148, each=4, unset=0, busy=0, cost=0):
+def check(lib, ctx, starts, shared, max_pages, nkv, G, chunk, ctas=148, each=4, unset=0, busy=0, cost=0, share=1):
     B, reach, warps = len(ctx), max_pages * 64, each * ctas
     n = len(shared) if grows(starts, B) else 0
     group = [next((g for g in range(n) if starts[g] <= b < starts[g + 1]), None) for b in range(B)]
     tokens = [max(0, min(s, reach)) for s in shared]
-    pays = [starts[g + 1] - starts[g] >= 2 and tokens[g] >= 128 for g in range(n)]
+    pays = [bool(share) and starts[g + 1] - starts[g] >= 2 and tokens[g] >= 128 for g in range(n)]
     seen = {}
 
     # ---- own: tokens of every sequence, each once; a unit's shares follow one another
     units, last = {}, None
-    for warp, b, h, t0, t1, steps, prefix, first, end in stretches(lib, True, ctx, starts, shared, max_pages, nkv, G, chunk, ctas, unset, each, busy, cost):
+    for warp, b, h, t0, t1, steps, prefix, first, end in stretches(lib, True, ctx, starts, shared, max_pages, nkv, G, chunk, ctas, unset, each, busy, cost, share):
         c, g = max(0, min(ctx[b], reach)), group[b]
         begin = tokens[g] if g is not None else 0
         assert prefix == (g is not None and pays[g] and c >= begin)
@@ -62,7 +62,7 @@ def check(lib, ctx, starts, shared, max_pages, nkv, G, chunk, ctas=148, each=4, 
         if h == 0:
             for x in range(t0, t1):
                 out = np.zeros(3, np.int32)
-                lib.shared_step(at(np.asarray(ctx, np.int32)), B, b, at(np.asarray(starts, np.int32)), at(np.asarray(shared, np.int32)), n, max_pages, chunk, x, at(out))
+                lib.shared_step(at(np.asarray(ctx, np.int32)), B, b, at(np.asarray(starts, np.int32)), at(np.asarray(shared, np.int32)), n, max_pages, chunk, share, x, at(out))
                 lo, hi, query = out.tolist()
                 if lo >= hi:
                     continue
@@ -79,7 +79,7 @@ def check(lib, ctx, starts, shared, max_pages, nkv, G, chunk, ctas=148, each=4, 
     # ---- prefix: pages of every unit, each once
     units, covered, rows = {}, set(), set()
     th = 128 // G
-    for cta, g, h, tile, p0, pages, few, first, end in stretches(lib, False, ctx, starts, shared, max_pages, nkv, G, chunk, ctas, unset):
+    for cta, g, h, tile, p0, pages, few, first, end in stretches(lib, False, ctx, starts, shared, max_pages, nkv, G, chunk, ctas, unset, share=share):
         assert pays[g] and pages > 0 and first <= cta <= end
         size, total = starts[g + 1] - starts[g], -(-tokens[g] // 64)
         q = min(2 * th, size - tile * 2 * th)
@@ -119,7 +119,7 @@ SHAPES = [
 def test_shapes(lib, shape, G, chunk):
     ctx, starts, shared, max_pages, nkv = SHAPES[shape]
     for ctas, busy, cost in ((1, 0, 0), (1, 1, 5), (5, 2, 3), (148, 0, 0), (148, 148, 4), (148, 60, 4), (148, 147, 1)):
-        check(lib, ctx, starts, shared, max_pages, nkv, G, chunk, ctas, 4, unset=shape % 2, busy=busy, cost=cost)
+        check(lib, ctx, starts, shared, max_pages, nkv, G, chunk, ctas, 4, unset=shape % 2, busy=busy, cost=cost, share=busy % 3 != 2)
 
 
 @pytest.mark.parametrize("seed", range(25))
@@ -132,7 +132,7 @@ def test_random_batches(lib, seed):
     shared = [rng.randint(0, max_pages * 64 + 10) for _ in range(n)]
     ctx = [rng.randint(0, max_pages * 64 + 10) for _ in range(B)]
     ctas = rng.choice([3, 148])
-    check(lib, ctx, starts, shared, max_pages, rng.choice([1, 2, 8]), rng.randint(1, 8), rng.choice([16, 64]), ctas, rng.choice([3, 4]), unset=rng.randint(0, 1), busy=rng.randint(0, ctas), cost=rng.randint(0, 9))
+    check(lib, ctx, starts, shared, max_pages, rng.choice([1, 2, 8]), rng.randint(1, 8), rng.choice([16, 64]), ctas, rng.choice([3, 4]), unset=rng.randint(0, 1), busy=rng.randint(0, ctas), cost=rng.randint(0, 9), share=seed % 5 != 0)
 
 
 @pytest.mark.parametrize("G", range(1, 9))
