@@ -29,9 +29,25 @@ struct NormAppend {
     float eps;
 };
 
-__device__ __forceinline__ float na_float(float v) { return v; }
-__device__ __forceinline__ float na_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ float na_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+// four numbers as two pairs of fp32
+__device__ __forceinline__ void na_pairs(const uint4& raw, float, f32x2* v) {
+    v[0] = pack2(__uint_as_float(raw.x), __uint_as_float(raw.y));
+    v[1] = pack2(__uint_as_float(raw.z), __uint_as_float(raw.w));
+}
+__device__ __forceinline__ void na_pairs(const uint2& raw, __nv_bfloat16, f32x2* v) {
+    v[0] = pack2(bf16_lo(raw.x), bf16_hi(raw.x));
+    v[1] = pack2(bf16_lo(raw.y), bf16_hi(raw.y));
+}
+__device__ __forceinline__ void na_pairs(const uint2& raw, __half, f32x2* v) {
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&raw.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&raw.y));
+    v[0] = pack2(a.x, a.y);
+    v[1] = pack2(b.x, b.y);
+}
+__device__ __forceinline__ void na_pairs(const float* p, f32x2* v) {
+    const float4 w = load_f4(p);
+    v[0] = pack2(w.x, w.y);
+    v[1] = pack2(w.z, w.w);
+}
 
 // four numbers as they lie in memory
 template <class T> struct NaRaw { typedef uint2 type; };
@@ -49,8 +65,10 @@ __device__ __forceinline__ typename NaRaw<T>::type na_load(const T* p) {     // 
     return *reinterpret_cast<const Raw*>(raw);
 }
 // within fp16's range, NaN as it is
-__device__ __forceinline__ uint32_t na_half2(float a, float b) {
+__device__ __forceinline__ uint32_t na_half2(f32x2 v) {
     uint32_t r;
+    float a, b;
+    unpack2(v, a, b);
     asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
     return r;
 }
@@ -68,19 +86,20 @@ norm_append_kernel(const __grid_constant__ NormAppend p) {
     const int turned = p.rotated / (2 * E);          // lanes of a head that rotate, where pairs are halves
     const int c0 = !NEIGHBOURS && j >= turned ? turned + j : j, c1 = !NEIGHBOURS && j < turned ? j + turned : j + LANES;
     const int p0 = (warp - t * p.per_token) * p.per, p1 = min(p0 + p.per, p.passes);
-    const T* const row = (const T*)p.x + (long long)t * p.row_stride + sub * D;
+    const int far = (c1 - c0) * E;
+    const T* from = (const T*)p.x + (long long)t * p.row_stride + (p0 * HEADS + sub) * D + c0 * E;      // chunk c0 of the pass whose reads come next
+    int next = p0;                                   // that pass
     Raw raw[NA_AHEAD][2];
-    auto ask = [&](int u, int first, int s) {        // pass first + u, part s
-        if (first + u < p1 && (first + u) * HEADS + sub < heads) {
-            const T* from = row + s * p.part_stride + (long long)(first + u) * (HEADS * D);
-            raw[u][0] = na_load<T, WIDE>(from + c0 * E);
-            raw[u][1] = na_load<T, WIDE>(from + c1 * E);
+    auto ask = [&](int u, const T* x) {              // pass next + u
+        if (next + u < p1 && (next + u) * HEADS + sub < heads) {
+            raw[u][0] = na_load<T, WIDE>(x + u * (HEADS * D));
+            raw[u][1] = na_load<T, WIDE>(x + u * (HEADS * D) + far);
         } else {
             raw[u][0] = raw[u][1] = Raw{};
         }
     };
 #pragma unroll
-    for (int u = 0; u < NA_AHEAD; ++u) ask(u, p0, 0);
+    for (int u = 0; u < NA_AHEAD; ++u) ask(u, from);
     const int pos = p.positions[t], slot = p.kv_slots[t];
     const bool known = pos >= 0 && (p.rotated == 0 || pos < p.n_angles);
     const bool kept = known && slot >= 0 && slot < p.slots;
@@ -102,98 +121,111 @@ norm_append_kernel(const __grid_constant__ NormAppend p) {
             *reinterpret_cast<float4*>(sn) = load_f4(p.sin_t + at + c0 * E);
         }
     }
-    uint8_t* const cache = p.kv_layer + ((size_t)(slot / kKvTile) * p.nkv * 2) * (size_t)(kKvTile * D * 2);
-    const int in0 = kv_swizzled_chunk<D>(slot % kKvTile, c0 / 2) + c0 % 2 * 8, in1 = kv_swizzled_chunk<D>(slot % kKvTile, c1 / 2) + c1 % 2 * 8;      // of a page's head
+    f32x2 c2[2], s2[2], m2[2];                       // cosines, sines, minus sines
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        c2[e] = pack2(cs[2 * e], cs[2 * e + 1]);
+        s2[e] = pack2(sn[2 * e], sn[2 * e + 1]);
+        m2[e] = pack2(-sn[2 * e], -sn[2 * e + 1]);
+    }
+    uint8_t* to_q = reinterpret_cast<uint8_t*>(p.q_out + ((size_t)t * p.nq + p0 * HEADS + sub) * D + c0 * E);      // where the pass at hand goes, if it is queries
+    constexpr int SLAB = kKvTile * D * 2;
+    uint8_t* const cache = p.kv_layer + ((size_t)(slot / kKvTile) * p.nkv * 2) * (size_t)SLAB + kv_swizzled_chunk<D>(slot % kKvTile, c0 / 2) + c0 % 2 * 8;
+    const int far_kv = kv_swizzled_chunk<D>(slot % kKvTile, c1 / 2) + c1 % 2 * 8 - (kv_swizzled_chunk<D>(slot % kKvTile, c0 / 2) + c0 % 2 * 8);
     const float* have = nullptr;                     // the gain that is in g
-    float g[2][E];
+    f32x2 g[2][2];
+    int hd = p0 * HEADS + sub;                       // the head of the pass at hand
 #pragma unroll 1
-    for (int first = p0; first < p1; first += NA_AHEAD) {
-        float v[NA_AHEAD][2][E];
+    while (next < p1) {
+        f32x2 v[NA_AHEAD][2][2];
 #pragma unroll
-        for (int u = 0; u < NA_AHEAD; ++u)
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int e = 0; e < E; ++e) v[u][c][e] = na_float(reinterpret_cast<const T*>(&raw[u][c])[e]);
-        if (sizeof(T) == 4)                          // parts are fp32
+        for (int u = 0; u < NA_AHEAD; ++u) na_pairs(raw[u][0], T(), v[u][0]), na_pairs(raw[u][1], T(), v[u][1]);
+        if (sizeof(T) == 4) {                        // parts are fp32
+            const T* part = from;
 #pragma unroll 1
             for (int s = 1; s < p.parts; ++s) {
+                part += p.part_stride;
 #pragma unroll
-                for (int u = 0; u < NA_AHEAD; ++u) ask(u, first, s);
+                for (int u = 0; u < NA_AHEAD; ++u) ask(u, part);
 #pragma unroll
                 for (int u = 0; u < NA_AHEAD; ++u)
 #pragma unroll
-                    for (int c = 0; c < 2; ++c)
-#pragma unroll
-                        for (int e = 0; e < E; ++e) v[u][c][e] += na_float(reinterpret_cast<const T*>(&raw[u][c])[e]);
+                    for (int c = 0; c < 2; ++c) {
+                        f32x2 more[2];
+                        na_pairs(raw[u][c], T(), more);
+                        v[u][c][0] = sum2(v[u][c][0], more[0]);
+                        v[u][c][1] = sum2(v[u][c][1], more[1]);
+                    }
             }
+        }
+        const int here = p1 - next;
+        next += NA_AHEAD;
+        from += NA_AHEAD * HEADS * D;
 #pragma unroll
-        for (int u = 0; u < NA_AHEAD; ++u) ask(u, first + NA_AHEAD, 0);      // the next passes are on their way meanwhile
+        for (int u = 0; u < NA_AHEAD; ++u) ask(u, from);                     // the next passes are on their way meanwhile
 #pragma unroll
-        for (int u = 0; u < NA_AHEAD; ++u) {
-            if (first + u >= p1) break;
-            const int hd = (first + u) * HEADS + sub;
-            float(&x)[2][E] = v[u];
-            float ss = 0.f;
-#pragma unroll
-            for (int e = 0; e < E; ++e) ss = fmaf(x[0][e], x[0][e], fmaf(x[1][e], x[1][e], ss));
+        for (int u = 0; u < NA_AHEAD; ++u, hd += HEADS, to_q += HEADS * D * 2) {
+            if (u >= here) break;
+            f32x2(&x)[2][2] = v[u];
+            f32x2 sq = mul2(x[0][0], x[0][0]);
+            sq = fma2(x[0][1], x[0][1], sq);
+            sq = fma2(x[1][0], x[1][0], sq);
+            sq = fma2(x[1][1], x[1][1], sq);
+            float ss, s1;
+            unpack2(sq, ss, s1);
+            ss += s1;
 #pragma unroll
             for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
             if (hd >= heads) continue;
-            float r = 1.f;
             if (hd < p.nq + p.nkv) {
                 const float* gain = hd < p.nq ? p.q_gain : p.k_gain;
                 if (gain) {
                     gain += hd < p.nq ? hd * p.gain_q_stride : (hd - p.nq) * p.gain_k_stride;
                     if (gain != have) {
-                        *reinterpret_cast<float4*>(g[0]) = load_f4(gain + c0 * E);
-                        *reinterpret_cast<float4*>(g[1]) = load_f4(gain + c1 * E);
+                        na_pairs(gain + c0 * E, g[0]);
+                        na_pairs(gain + c1 * E, g[1]);
                         have = gain;
                     }
 #pragma unroll
                     for (int c = 0; c < 2; ++c)
 #pragma unroll
-                        for (int e = 0; e < E; ++e) x[c][e] *= g[c][e];
+                        for (int e = 0; e < 2; ++e) x[c][e] = mul2(x[c][e], g[c][e]);
                 }
                 if (NEIGHBOURS) {
 #pragma unroll
                     for (int c = 0; c < 2; ++c)
 #pragma unroll
-                        for (int e = 0; e < E; e += 2) {
-                            const float a = x[c][e], b = x[c][e + 1], co = cs[c * 2 + e / 2], si = sn[c * 2 + e / 2];
-                            x[c][e] = a * co - b * si;
-                            x[c][e + 1] = b * co + a * si;
+                        for (int e = 0; e < 2; ++e) {
+                            float a, b;
+                            unpack2(x[c][e], a, b);
+                            x[c][e] = pack2(a * cs[2 * c + e] - b * sn[2 * c + e], b * cs[2 * c + e] + a * sn[2 * c + e]);
                         }
                 } else {
 #pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        const float a = x[0][e], b = x[1][e];
-                        x[0][e] = a * cs[e] - b * sn[e];
-                        x[1][e] = b * cs[e] + a * sn[e];
+                    for (int e = 0; e < 2; ++e) {
+                        const f32x2 a = x[0][e], b = x[1][e];
+                        x[0][e] = fma2(a, c2[e], mul2(b, m2[e]));
+                        x[1][e] = fma2(b, c2[e], mul2(a, s2[e]));
                     }
                 }
-                r = rsqrtf(ss * (1.f / D) + p.eps);
-            }
-            uint8_t *to0, *to1;
-            if (hd < p.nq) {
-                to0 = reinterpret_cast<uint8_t*>(p.q_out + ((size_t)t * p.nq + hd) * D);
-                to1 = to0 + c1 * E * 2;
-                to0 += c0 * E * 2;
-            } else {
-                if (!kept) continue;
-                const bool is_v = hd >= p.nq + p.nkv;
-                uint8_t* slab = cache + ((hd - p.nq - (is_v ? p.nkv : 0)) * 2 + is_v) * (kKvTile * D * 2);
-                to0 = slab + in0;
-                to1 = slab + in1;
-            }
-            uint2 h[2];
+                const float r = rsqrtf(ss * (1.f / D) + p.eps);
+                const f32x2 r2 = pack2(r, r);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                h[c] = make_uint2(na_half2(x[c][0] * r, x[c][1] * r), na_half2(x[c][2] * r, x[c][3] * r));
-                if (!known) h[c] = make_uint2(0u, 0u);       // q of a token without a position
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) x[c][e] = mul2(x[c][e], r2);
             }
-            *reinterpret_cast<uint2*>(to0) = h[0];
-            *reinterpret_cast<uint2*>(to1) = h[1];
+            uint2 h0 = make_uint2(na_half2(x[0][0]), na_half2(x[0][1])), h1 = make_uint2(na_half2(x[1][0]), na_half2(x[1][1]));
+            if (hd < p.nq) {
+                if (!known) h0 = h1 = make_uint2(0u, 0u);                    // a token without a position
+                *reinterpret_cast<uint2*>(to_q) = h0;
+                *reinterpret_cast<uint2*>(to_q + far * 2) = h1;
+            } else if (kept) {
+                const int is_v = hd >= p.nq + p.nkv;
+                uint8_t* to = cache + ((hd - p.nq - is_v * p.nkv) * 2 + is_v) * SLAB;
+                *reinterpret_cast<uint2*>(to) = h0;
+                *reinterpret_cast<uint2*>(to + far_kv) = h1;
+            }
         }
     }
 }
@@ -204,7 +236,8 @@ static int launch_norm_append(NormAppend& p, bool neighbours, bool wide, cudaStr
     p.passes = (p.nq + 2 * p.nkv + HEADS - 1) / HEADS;
     // a warp takes as much of a token as leaves NA_FILL warps an SM: its angles and gains are read once
     const long long each = (long long)p.T * p.passes / ((long long)NA_FILL * device_sms());
-    p.per = each < 1 ? 1 : each < p.passes ? (int)each : p.passes;
+    p.per_token = each < 1 ? p.passes : each < p.passes ? (int)((p.passes + each - 1) / each) : 1;
+    p.per = (p.passes + p.per_token - 1) / p.per_token;
     p.per_token = (p.passes + p.per - 1) / p.per;
     const long long warps = (long long)p.T * p.per_token;
     const dim3 grid((unsigned)((warps + NA_WARPS - 1) / NA_WARPS));
