@@ -27,6 +27,7 @@ constexpr int SH_REGS = 128, SH_REGS_ISSUE = 88, SH_REGS_SOFT = 144, SH_REGS_OWN
 static_assert(SH_REGS_ISSUE + 2 * SH_REGS_SOFT + SH_REGS_OWN <= 4 * SH_REGS, "what the block is launched with");
 constexpr int SH_SOFT = 256;
 constexpr int SH_TOLD = 4, SH_LISTENERS = 11;    // stretches told ahead; warps that hear of them
+constexpr int SH_STRETCH = 64;                   // times the limit, for what takes a whole stretch: it may be a million keys
 constexpr int SH_LEAST = 4;
 constexpr int SH_COST = 2;                       // steps of the prefix that cost a warp on its SM one of its own
 constexpr int SH_LIST = 100;                     // groups whose lists are kept in shared memory
@@ -54,9 +55,10 @@ struct Shared {
 
 // A wait that ends, in a few instructions: what bounds calls of ten microseconds here is among others how much code they touch for the first time (126 KB, with waits and
 // loops unrolled and the walk in every role, took 3 of 10 issue slots' worth of waiting for instructions)
-__device__ __forceinline__ bool shared_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
+// Who gives up touches none of the barriers again: what it skipped would make it take one phase for another.
+__device__ __forceinline__ bool shared_wait(uint64_t* bar, uint32_t parity, volatile int* dead, int limit) {
 #pragma unroll 1
-    for (int i = 0; i < kWaitLimit; ++i) {
+    for (int i = 0; i < limit; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
         if (*dead) return false;
     }
@@ -301,7 +303,7 @@ __device__ __forceinline__ void shared_own(const SharedArgs& p, const SharedGrou
         }
         if (!ok || !(paged >> x & 1)) continue;
         const int stage = it % S;
-        ok = __all_sync(0xffffffffu, shared_wait(&full[stage], it / S & 1, dead));
+        ok = __all_sync(0xffffffffu, shared_wait(&full[stage], it / S & 1, dead, p.wait_limit));
         if (!ok) continue;
         ++it;
         const int seen = __shfl_sync(0xffffffffu, seen_x, x), lo = seen & 255, hi = seen >> 8;
@@ -392,6 +394,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
     __shared__ uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];           // half, buffer: scores are in tensor memory; probabilities are; O += P V retired
     __shared__ uint64_t told_full[SH_TOLD], told_empty[SH_TOLD];             // a stretch has been told; all have done with it
     __shared__ SharedStretch told[SH_TOLD];
+    __shared__ uint64_t met;                                                 // all softmax warps are here
     __shared__ uint64_t drained[2];                                          // all products of a half retired
     __shared__ int tokens_s[C::TOKENS];                                      // of the last pages copied; 0: the page is not there
     __shared__ __align__(16) int sums_s[SH_WARPS][4];
@@ -407,6 +410,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
         for (int s = 0; s < C::STAGES; ++s) mbar_init(&k_empty[s], 2), mbar_init(&v_empty[s], 2);
         for (int s = 0; s < C::OWN_WARPS * C::OWN_STAGES; ++s) mbar_init(&own_full[s], 1);
         for (int s = 0; s < SH_TOLD; ++s) mbar_init(&told_full[s], 1), mbar_init(&told_empty[s], SH_LISTENERS);
+        mbar_init(&met, SH_SOFT / 32);
         for (int h = 0; h < 2; ++h) {
             mbar_init(&q_full[h], kSharedRows / 32);
             mbar_init(&drained[h], 1);
@@ -516,10 +520,10 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
     const uint32_t tmem = tmem_slot;
     uint32_t k_bits = 0, v_bits = 0;                                         // of the warp that copies: the phases of what it has asked for
     bool ok = true;                                                          // false: a wait ran out
-    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, shared_wait(bar, parity, &dead)); };
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, shared_wait(bar, parity, &dead, p.wait_limit)); };
     // the n-th stretch of the prefix's share, or one without pages behind the last; and this warp's word that it has done with it
     auto hear = [&](int n) {
-        ok = ok && wait(&told_full[n % SH_TOLD], n / SH_TOLD & 1);
+        ok = ok && __all_sync(0xffffffffu, shared_wait(&told_full[n % SH_TOLD], n / SH_TOLD & 1, &dead, SH_STRETCH * p.wait_limit));
         SharedStretch w = told[n % SH_TOLD];
         if (!ok) w.pages = 0;
         return w;
@@ -539,7 +543,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
 #pragma unroll 1
                 for (int n = 0, more = 1; more; ++n) {
                     more = w.next(p, gr);
-                    if (!shared_wait(&told_empty[n % SH_TOLD], (n / SH_TOLD & 1) ^ 1, &dead)) break;
+                    if (!shared_wait(&told_empty[n % SH_TOLD], (n / SH_TOLD & 1) ^ 1, &dead, SH_STRETCH * p.wait_limit)) break;
                     SharedStretch s{};
                     if (more) s = w.stretch(p, prefix_per);
                     told[n % SH_TOLD] = s;
@@ -590,7 +594,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
                     for (int kind = 0; kind < 2; ++kind) {
                         if (kind ? it < C::AHEAD : !more) continue;
                         const int i = it - kind * C::AHEAD, s = i % C::STAGES;
-                        ok = ok && shared_wait(kind ? &v_empty[s] : &k_empty[s], (i / C::STAGES & 1) ^ 1, &dead);
+                        ok = ok && shared_wait(kind ? &v_empty[s] : &k_empty[s], (i / C::STAGES & 1) ^ 1, &dead, p.wait_limit);
                         if (!ok) continue;
                         phases[kind].next(C::STAGES, s, set[kind]);
                         uint64_t* const full = (kind ? v_full : k_full) + phases[kind].at;
@@ -624,7 +628,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
                 auto issue_qk = [&](int page, bool alone) {                  // page: counted over the whole share; alone: the other half has no use for it
                     const int s = page % C::STAGES, buf = n_qk & 1;
                     const uint32_t parity = k_phases.next(C::STAGES, s, alone ? h : 2);
-                    ok = shared_wait(&k_full[k_phases.at], parity, &dead);
+                    ok = shared_wait(&k_full[k_phases.at], parity, &dead, p.wait_limit);
                     if (!ok) return;
                     ++n_qk;
                     tc_fence_after();
@@ -640,7 +644,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
                 auto issue_pv = [&](int page, bool first, bool alone) {
                     const int s = page % C::STAGES, buf = n_pv & 1;
                     const uint32_t parity = v_phases.next(C::STAGES, s, alone ? h : 2);
-                    ok = shared_wait(&v_full[v_phases.at], parity, &dead) && shared_wait(&p_full[h][buf], n_pv >> 1 & 1, &dead);
+                    ok = shared_wait(&v_full[v_phases.at], parity, &dead, p.wait_limit) && shared_wait(&p_full[h][buf], n_pv >> 1 & 1, &dead, p.wait_limit);
                     if (!ok) return;
                     ++n_pv;
                     tc_fence_after();
@@ -658,7 +662,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
                     const int mine = w.of_half(h);
                     auto page_of = [&](int i) { return base + (w.few ? h + 2 * i : i); };      // page i of this half
                     if (lead && ok && mine) {
-                        ok = shared_wait(&q_full[h], n_q & 1, &dead);
+                        ok = shared_wait(&q_full[h], n_q & 1, &dead, p.wait_limit);
                         tc_fence_after();
                         // Scores run two pages ahead, issued behind the product that reads the probabilities in their buffer
 #pragma unroll 1
@@ -692,6 +696,14 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
         int base = 0, cnt = 0;                                               // pages of the share, pages of this half so far
         // maxima and sums of a half, where its queries were: the products that read those have retired
         auto ml_of = [&](int half) { return reinterpret_cast<float2*>(smem + half * KH * C::QBLK); };
+        int meetings = 0;
+        auto meet = [&]() {
+            tc_fence_before();
+            __syncwarp();
+            if (ok && lane == 0) mbar_arrive(&met);
+            ok = ok && wait(&met, meetings++ & 1);
+            tc_fence_after();
+        };
 #pragma unroll 1
         for (int seg = 0;; ++seg) {
             const SharedStretch w = hear(seg);
@@ -807,13 +819,12 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
             float z = 1.f, zo = 0.f, m = m_ref, l = l_run;
             if (w.few) {                                                     // the halves' results as one: each half puts half of the dims together
                 ml_of(h)[row] = make_float2(m_ref, l_run);
-                tc_fence_before();
-                asm volatile("bar.sync 1, %0;" ::"n"(SH_SOFT) : "memory");
-                tc_fence_after();
+                meet();
                 const float2 other = ml_of(1 - h)[row];
                 m = fmaxf(m_ref, other.x);
                 z = m_ref == -INFINITY ? 0.f : exp2f(m_ref - m), zo = other.x == -INFINITY ? 0.f : exp2f(other.x - m);
                 l = h == 0 ? l_run * z + other.y * zo : other.y * zo + l_run * z;
+                if (!ok) l = NAN;
             }
             const int c0 = w.few ? h * (D / 32) : 0, c1 = w.few ? c0 + D / 32 : D / 16;
 #pragma unroll 1
@@ -839,8 +850,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
             }
             if (valid && (!w.few || h == 0)) p.rows_ml[at] = make_float2(m, l);
             if (w.few) {                                                     // the other half has read what the next products write over
-                tc_fence_before();
-                asm volatile("bar.sync 1, %0;" ::"n"(SH_SOFT) : "memory");
+                meet();
             }
             base += w.pages;
             heard(seg);
@@ -884,7 +894,9 @@ shared_merge_kernel(const __grid_constant__ SharedArgs p) {
     const int4 own = p.own_units[unit];
     int4 pre = make_int4(0, -1, 0, 0);
     if (p.n_groups) pre = p.prefix_units[unit];
-    if (!own.z) pre = make_int4(0, -1, 0, 0);                                // (then nobody has written there)
+    // (without a prefix part nobody has written there, nor where a wait ran out ahead of that: then the result is NaN)
+    const bool lost = own.z && !(pre.x >= 0 && pre.x <= pre.y && pre.y < p.ctas && pre.z >= 0 && pre.z < p.rows && pre.z + 2 * kSharedRows * pre.y + G <= p.rows);
+    if (!own.z || lost) pre = make_int4(0, -1, 0, 0);
     // a thread has four dims of a head (neighbours the same of neighbouring heads, as the prefix's results lie), and every `lanes`-th part
     const int mine = (int)((threadIdx.x / (D / 4)) * p.inv_g >> 16), e = threadIdx.x - mine * (G * D / 4), lanes = (int)((SM_THREADS / (D / 4)) * p.inv_g >> 16);
     const int quad = (int)(e * p.inv_g >> 16), hg = e - quad * G;
@@ -939,6 +951,7 @@ shared_merge_kernel(const __grid_constant__ SharedArgs p) {
         L = fmaf(ml.y, z, L);
         acc = fma_f4(*reinterpret_cast<const float4*>(acc_s + 4 * (x * (G * D / 4) + e)), make_float4(z, z, z, z), acc);
     }
+    if (lost) L = NAN;
     const float r = L == 0.f ? 0.f : 1.f / L;                                // a query without a visible key: zeros
     const float v[4] = {acc.x * r, acc.y * r, acc.z * r, acc.w * r};
     const size_t at = ((size_t)unit * G + hg) * D + 4 * quad;                // (unit = sequence * key heads + key head)
@@ -970,6 +983,7 @@ static SharedLayout shared_layout(int B, int n_groups, int nq, int nkv, int d) {
 }
 
 static std::atomic<long long> g_shared_least{-1};
+static std::atomic<int> g_shared_wait_limit{kWaitLimit};
 
 template <int D>
 static int launch_shared(SharedArgs& p, cudaStream_t st) {
@@ -990,7 +1004,9 @@ static int launch_shared(SharedArgs& p, cudaStream_t st) {
     const long long least = g_shared_least.load(std::memory_order_relaxed), pages = (least < 0 ? (D == 64 ? 12 : 6) << 20 : least) / ((long long)C::TILE * p.nkv);
     p.least_size = D == 64 && least < 0 ? 3 : 2;
     p.least_pages = (int)(pages < INT32_MAX ? pages : INT32_MAX) + (least < 0);
-    FT_CHECK_CUDA(launch_after(shared_attn_kernel<D>, dim3(device_sms()), dim3(SH_THREADS), C::SMEM, st, (const SharedArgs&)p));
+    p.wait_limit = g_shared_wait_limit.load(std::memory_order_relaxed);
+    p.ctas = device_sms();
+    FT_CHECK_CUDA(launch_after(shared_attn_kernel<D>, dim3(p.ctas), dim3(SH_THREADS), C::SMEM, st, (const SharedArgs&)p));
     // few units: more threads for each one's parts (24 sequences x 8 key heads of 128, 20 parts each, 7.0 us with 256)
     const int units = p.B * p.nkv;
     if (units <= 2 * device_sms()) FT_CHECK_CUDA(launch_after(shared_merge_kernel<D, 512>, dim3(units), dim3(512), 0, st, (const SharedArgs&)p));
@@ -1006,6 +1022,8 @@ extern "C" long long ft_attn_decode_shared_scratch_bytes(int B, int n_groups, in
     FT_REQUIRE(B >= 0 && n_groups >= 0 && (double)B * nq * d <= INT32_MAX, "ft_attn_decode_shared_scratch_bytes: bad sizes B=%d nq=%d groups=%d", B, nq, n_groups);
     return (long long)ft::shared_layout(B, n_groups, nq, nkv, d).bytes;
 }
+
+extern "C" void ft_attn_shared_set_wait_limit(int tries) { ft::g_shared_wait_limit = tries < 0 || tries > ft::kWaitLimit ? ft::kWaitLimit : tries; }
 
 extern "C" void ft_attn_shared_set_least(long long bytes) { ft::g_shared_least = bytes < 0 ? -1 : bytes; }
 
@@ -1036,6 +1054,6 @@ extern "C" int ft_attn_decode_shared(const ft_attn_shared_args* args, void* stre
     uint8_t* w = (uint8_t*)scratch;
     SharedArgs p{(const __half*)q, (const uint8_t*)kv_layer, page_table, req_slot, ctx_lens, group_start, shared_lens, (__nv_bfloat16*)out, (__nv_bfloat16*)out_lo,
                  (int4*)(w + l.own_units), (int4*)(w + l.prefix_units), (float*)(w + l.own_parts), (float*)(w + l.rows_o), (float2*)(w + l.rows_ml), B, n_groups, num_pages, table_rows,
-                 max_pages, nq, nkv, G, th, (int)l.rows, 0, (65536u + G - 1) / G, kSharedLog2E / sqrtf((float)d), (unsigned)(((1ull << 32) + 2 * th - 1) / (2 * th)), 0, 0};
+                 max_pages, nq, nkv, G, th, (int)l.rows, 0, (65536u + G - 1) / G, kSharedLog2E / sqrtf((float)d), (unsigned)(((1ull << 32) + 2 * th - 1) / (2 * th)), 0, 0, 0, 0};
     return d == 64 ? launch_shared<64>(p, (cudaStream_t)stream) : launch_shared<128>(p, (cudaStream_t)stream);
 }

@@ -657,6 +657,85 @@ def test_a_run_of_all_three(K, sharing):
     assert ctx.tolist() == [prompt + 70] * B
 
 
+@pytest.mark.parametrize("nq,nkv,d,groups", [(4, 1, 64, 99), (4, 1, 64, 100), (4, 2, 128, 101), (2, 2, 64, 700), (8, 1, 128, 1100)])
+def test_hundreds_of_groups(K, sharing, nq, nkv, d, groups):
+    """More groups than the kernel keeps the lists of, and more sequences than it has threads: some groups empty, some of one, some of many."""
+    import random
+    rng = random.Random(groups)
+    sizes = [rng.choice([0, 1, 1, 2, 2, 3, 5]) for _ in range(groups)]
+    shared = [rng.choice([0, 64, 130, 200, 300]) for _ in range(groups)]
+    own = [rng.choice([0, 1, 30, 70, -20]) for _ in range(sum(sizes) + 3)]
+    check(K, make(groups, nq, nkv, d, sizes, shared, own))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_thousands_of_sequences(K, sharing, d):
+    n = 3000
+    check(K, make(50 + d, 2, 1, d, [2000, 900], [300, 150], [i * 7 % 40 for i in range(n)]))
+
+
+@pytest.mark.parametrize("nq,nkv,d", [(8, 8, 64), (8, 8, 128)])
+def test_pages_beyond_four_gigabytes(K, sharing, nq, nkv, d):
+    """Byte offsets into the cache pass 32 bits, and numbers of fp16 31 bits."""
+    s = make(60, nq, nkv, d, [5], [700], [10, 0, 64, 100, 1], hidden=0.5)
+    P, bytes_ = s["cache"].shape[0], s["cache"][0].numel() * 2
+    far = (5 << 30) // bytes_
+    big = torch.empty(far + P, nkv, 2, 64, d, device=DEV, dtype=torch.float16)
+    big[far:] = s["cache"]
+    want, tol = attention(s)
+    t = torch.where(s["table"] >= 0, s["table"] + far, -1)
+    close(K.attn_decode_shared(s["q"], big, t, s["ctx"], s["starts"], s["shared"], s["slots"]), want, tol, 2)
+    # and appending there
+    g = gen(61)
+    T, W = 9, (nq + 2 * nkv) * d
+    slots = (torch.randperm(P * 64, generator=g, device=DEV)[:T] + far * 64).int()
+    qkv, pos = torch.randn(T, W, generator=g, device=DEV), i32(list(range(T)))
+    q = K.norm_rope_kv_append(qkv, pos, slots, big, nq, nkv, d)
+    small = s["cache"].clone()
+    q2 = K.norm_rope_kv_append(qkv, pos, slots - far * 64, small, nq, nkv, d)
+    assert torch.equal(q, q2) and torch.equal(big[far:], small)
+
+
+GIVE_UP = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch
+from tests import test_shared_gpu as T
+from fasttalk_llm_microservice_b200 import kernels as K, native as N
+lib = N.load()
+lib.ft_attn_shared_set_least(0)
+for d, sizes, shared, own in ((64, [9, 40], [900, 300], 70), (128, [5, 30], [700, 2000], 90)):
+    s = T.make(d, 8, 2, d, sizes, shared, [i * 13 % own for i in range(sum(sizes))], hidden=0.5)
+    run = lambda: K.attn_decode_shared(s["q"], s["cache"], s["table"], s["ctx"], s["starts"], s["shared"], s["slots"])
+    want = run()
+    torch.cuda.synchronize()
+    assert d == 128 or lib.ft_attn_shared_waits() == 0
+    lib.ft_attn_shared_set_wait_limit(0)
+    lost = run()
+    assert lib.ft_attn_shared_waits() == 1
+    seen = (s["ctx"] > 0)
+    assert not torch.equal(lost[0][seen], want[0][seen])
+    lib.ft_attn_shared_set_wait_limit(-1)
+    again = run()
+    torch.cuda.synchronize()
+    assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
+try:
+    K.attn_shared_check()
+except N.NativeError:
+    print("TOLD")
+"""
+
+
+def test_waits_that_run_out_are_told(K):
+    """In a process of its own, since the word stays: with no tries at all every wait gives up, the call ends, says so, and the next one is right again."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", GIVE_UP, root], capture_output=True, text=True, timeout=300, cwd=root)
+    assert r.returncode == 0 and "TOLD" in r.stdout, r.stdout + r.stderr
+
+
 # ------------------------------------------------------------------------------------------------ refusals
 def test_refusals_of_tensors(K):
     z = lambda *n: torch.zeros(*n, device=DEV, dtype=torch.int32)
