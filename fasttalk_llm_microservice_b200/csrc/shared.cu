@@ -56,9 +56,9 @@ struct Shared {
 // A wait that ends, in a few instructions: what bounds calls of ten microseconds here is among others how much code they touch for the first time (126 KB, with waits and
 // loops unrolled and the walk in every role, took 3 of 10 issue slots' worth of waiting for instructions)
 // Who gives up touches none of the barriers again: what it skipped would make it take one phase for another.
-__device__ __forceinline__ bool shared_wait(uint64_t* bar, uint32_t parity, volatile int* dead, int limit) {
+__device__ __forceinline__ bool shared_wait(uint64_t* bar, uint32_t parity, volatile int* dead, int times = 1) {
 #pragma unroll 1
-    for (int i = 0; i < limit; ++i) {
+    for (int i = 0; i < times * kWaitLimit; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
         if (*dead) return false;
     }
@@ -303,7 +303,7 @@ __device__ __forceinline__ void shared_own(const SharedArgs& p, const SharedGrou
         }
         if (!ok || !(paged >> x & 1)) continue;
         const int stage = it % S;
-        ok = __all_sync(0xffffffffu, shared_wait(&full[stage], it / S & 1, dead, p.wait_limit));
+        ok = __all_sync(0xffffffffu, shared_wait(&full[stage], it / S & 1, dead));
         if (!ok) continue;
         ++it;
         const int seen = __shfl_sync(0xffffffffu, seen_x, x), lo = seen & 255, hi = seen >> 8;
@@ -417,7 +417,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
             for (int s = 0; s < 2; ++s) mbar_init(&s_full[h][s], 1), mbar_init(&p_full[h][s], kSharedRows / 32), mbar_init(&pv_done[h][s], 1);
         }
         fence_mbar_init();
-        dead = 0;
+        dead = p.give_up;
     }
     if (warp == 3) {
         tmem_alloc(&tmem_slot, C::COLS);
@@ -520,10 +520,10 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
     const uint32_t tmem = tmem_slot;
     uint32_t k_bits = 0, v_bits = 0;                                         // of the warp that copies: the phases of what it has asked for
     bool ok = true;                                                          // false: a wait ran out
-    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, shared_wait(bar, parity, &dead, p.wait_limit)); };
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, shared_wait(bar, parity, &dead)); };
     // the n-th stretch of the prefix's share, or one without pages behind the last; and this warp's word that it has done with it
     auto hear = [&](int n) {
-        ok = ok && __all_sync(0xffffffffu, shared_wait(&told_full[n % SH_TOLD], n / SH_TOLD & 1, &dead, SH_STRETCH * p.wait_limit));
+        ok = ok && __all_sync(0xffffffffu, shared_wait(&told_full[n % SH_TOLD], n / SH_TOLD & 1, &dead, SH_STRETCH));
         SharedStretch w = told[n % SH_TOLD];
         if (!ok) w.pages = 0;
         return w;
@@ -543,7 +543,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
 #pragma unroll 1
                 for (int n = 0, more = 1; more; ++n) {
                     more = w.next(p, gr);
-                    if (!shared_wait(&told_empty[n % SH_TOLD], (n / SH_TOLD & 1) ^ 1, &dead, SH_STRETCH * p.wait_limit)) break;
+                    if (!shared_wait(&told_empty[n % SH_TOLD], (n / SH_TOLD & 1) ^ 1, &dead, SH_STRETCH)) break;
                     SharedStretch s{};
                     if (more) s = w.stretch(p, prefix_per);
                     told[n % SH_TOLD] = s;
@@ -594,7 +594,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
                     for (int kind = 0; kind < 2; ++kind) {
                         if (kind ? it < C::AHEAD : !more) continue;
                         const int i = it - kind * C::AHEAD, s = i % C::STAGES;
-                        ok = ok && shared_wait(kind ? &v_empty[s] : &k_empty[s], (i / C::STAGES & 1) ^ 1, &dead, p.wait_limit);
+                        ok = ok && shared_wait(kind ? &v_empty[s] : &k_empty[s], (i / C::STAGES & 1) ^ 1, &dead);
                         if (!ok) continue;
                         phases[kind].next(C::STAGES, s, set[kind]);
                         uint64_t* const full = (kind ? v_full : k_full) + phases[kind].at;
@@ -628,7 +628,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
                 auto issue_qk = [&](int page, bool alone) {                  // page: counted over the whole share; alone: the other half has no use for it
                     const int s = page % C::STAGES, buf = n_qk & 1;
                     const uint32_t parity = k_phases.next(C::STAGES, s, alone ? h : 2);
-                    ok = shared_wait(&k_full[k_phases.at], parity, &dead, p.wait_limit);
+                    ok = shared_wait(&k_full[k_phases.at], parity, &dead);
                     if (!ok) return;
                     ++n_qk;
                     tc_fence_after();
@@ -644,7 +644,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
                 auto issue_pv = [&](int page, bool first, bool alone) {
                     const int s = page % C::STAGES, buf = n_pv & 1;
                     const uint32_t parity = v_phases.next(C::STAGES, s, alone ? h : 2);
-                    ok = shared_wait(&v_full[v_phases.at], parity, &dead, p.wait_limit) && shared_wait(&p_full[h][buf], n_pv >> 1 & 1, &dead, p.wait_limit);
+                    ok = shared_wait(&v_full[v_phases.at], parity, &dead) && shared_wait(&p_full[h][buf], n_pv >> 1 & 1, &dead);
                     if (!ok) return;
                     ++n_pv;
                     tc_fence_after();
@@ -662,7 +662,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
                     const int mine = w.of_half(h);
                     auto page_of = [&](int i) { return base + (w.few ? h + 2 * i : i); };      // page i of this half
                     if (lead && ok && mine) {
-                        ok = shared_wait(&q_full[h], n_q & 1, &dead, p.wait_limit);
+                        ok = shared_wait(&q_full[h], n_q & 1, &dead);
                         tc_fence_after();
                         // Scores run two pages ahead, issued behind the product that reads the probabilities in their buffer
 #pragma unroll 1
@@ -983,7 +983,7 @@ static SharedLayout shared_layout(int B, int n_groups, int nq, int nkv, int d) {
 }
 
 static std::atomic<long long> g_shared_least{-1};
-static std::atomic<int> g_shared_wait_limit{kWaitLimit};
+static std::atomic<int> g_shared_give_up{0};
 
 template <int D>
 static int launch_shared(SharedArgs& p, cudaStream_t st) {
@@ -1004,7 +1004,7 @@ static int launch_shared(SharedArgs& p, cudaStream_t st) {
     const long long least = g_shared_least.load(std::memory_order_relaxed), pages = (least < 0 ? (D == 64 ? 12 : 6) << 20 : least) / ((long long)C::TILE * p.nkv);
     p.least_size = D == 64 && least < 0 ? 3 : 2;
     p.least_pages = (int)(pages < INT32_MAX ? pages : INT32_MAX) + (least < 0);
-    p.wait_limit = g_shared_wait_limit.load(std::memory_order_relaxed);
+    p.give_up = g_shared_give_up.load(std::memory_order_relaxed);
     p.ctas = device_sms();
     FT_CHECK_CUDA(launch_after(shared_attn_kernel<D>, dim3(p.ctas), dim3(SH_THREADS), C::SMEM, st, (const SharedArgs&)p));
     // few units: more threads for each one's parts (24 sequences x 8 key heads of 128, 20 parts each, 7.0 us with 256)
@@ -1023,7 +1023,7 @@ extern "C" long long ft_attn_decode_shared_scratch_bytes(int B, int n_groups, in
     return (long long)ft::shared_layout(B, n_groups, nq, nkv, d).bytes;
 }
 
-extern "C" void ft_attn_shared_set_wait_limit(int tries) { ft::g_shared_wait_limit = tries < 0 || tries > ft::kWaitLimit ? ft::kWaitLimit : tries; }
+extern "C" void ft_attn_shared_give_up(int on) { ft::g_shared_give_up = on != 0; }
 
 extern "C" void ft_attn_shared_set_least(long long bytes) { ft::g_shared_least = bytes < 0 ? -1 : bytes; }
 

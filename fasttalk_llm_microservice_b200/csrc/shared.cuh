@@ -33,7 +33,7 @@ struct SharedArgs {
 
     unsigned inv_tile;                           // 2^32 / (2 th), rounded up
     int least_size, least_pages;                 // sharing pays: queries of a group; pages that the call's groups save in all
-    int wait_limit;                              // tries of a wait
+    int give_up;                                 // 1: at the first wait that is not over yet
     int ctas;
 
     __host__ __device__ __forceinline__ int reach() const { return max_pages * kKvTile; }

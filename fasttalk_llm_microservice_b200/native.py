@@ -145,7 +145,7 @@ SIGNATURES = {
     "ft_attn_decode_shared": (_I, [_VP, _VP]),
     "ft_attn_shared_waits": (_I, []),
     "ft_attn_shared_set_least": (None, [_LL]),
-    "ft_attn_shared_set_wait_limit": (None, [_I]),
+    "ft_attn_shared_give_up": (None, [_I]),
     "ft_sample": (_I, [_VP, _I, _I, _VP, _VP, _VP, _VP, _VP, _VP]),
 }
 

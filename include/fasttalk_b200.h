@@ -749,8 +749,8 @@ int ft_norm_rope_kv_append(const ft_norm_append_args* args, void* stream);
  * A prefix is read once where the call's groups save enough by that (12 MB at heads of 64, counted from the third query of a group on, 6 MB at 128, from the second on), else by
  * every query; ft_attn_shared_set_least: what they have to save in the calls that follow, 0: nothing (below 0: the library's own).  Results are the same but for rounding.
  * ft_attn_shared_waits: 1 if a wait inside one of its kernels has run out on the current device since the library was loaded (rows of some call mean nothing), else 0;
- * waits for all that the device has been given, on every stream.  ft_attn_shared_set_wait_limit: tries of a wait in the calls that follow (below 0: the library's own, a
- * million); with 0 every wait runs out at once, so that a host can see what it does then. */
+ * waits for all that the device has been given, on every stream.  ft_attn_shared_give_up(1): the kernels of the calls that follow give up at the first
+ * wait that is not over yet, so that a host can see what it does then; (0): after a million tries, as ever. */
 long long ft_attn_decode_shared_scratch_bytes(int B, int n_groups, int nq, int nkv, int d);
 typedef struct {
     const void *q, *kv_layer;
@@ -761,7 +761,7 @@ typedef struct {
 int ft_attn_decode_shared(const ft_attn_shared_args* args, void* stream);
 int ft_attn_shared_waits(void);
 void ft_attn_shared_set_least(long long bytes);
-void ft_attn_shared_set_wait_limit(int tries);
+void ft_attn_shared_give_up(int on);
 
 /* K7: per-row temperature / top-k / top-p sampling (argmax when temperature <= 0; a null temperature says so for all rows).
  * A row without any logit above minus infinity gives index 0. */

@@ -710,12 +710,12 @@ for d, sizes, shared, own in ((64, [9, 40], [900, 300], 70), (128, [5, 30], [700
     want = run()
     torch.cuda.synchronize()
     assert d == 128 or lib.ft_attn_shared_waits() == 0
-    lib.ft_attn_shared_set_wait_limit(0)
+    lib.ft_attn_shared_give_up(1)
     lost = run()
     assert lib.ft_attn_shared_waits() == 1
     seen = (s["ctx"] > 0)
     assert not torch.equal(lost[0][seen], want[0][seen])
-    lib.ft_attn_shared_set_wait_limit(-1)
+    lib.ft_attn_shared_give_up(0)
     again = run()
     torch.cuda.synchronize()
     assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
@@ -727,7 +727,7 @@ except N.NativeError:
 
 
 def test_waits_that_run_out_are_told(K):
-    """In a process of its own, since the word stays: with no tries at all every wait gives up, the call ends, says so, and the next one is right again."""
+    """In a process of its own, since the word stays: where every wait gives up at once, the call ends, says so, and the next one is right again."""
     import os
     import subprocess
     import sys
