@@ -74,7 +74,7 @@ __host__ __device__ __forceinline__ int shared_part(int G, int d) { return (G * 
 // operand of O^T[dim][query] = V^T P^T, where all 16 rows are dims.
 template <int D>
 struct SharedQuery {
-    static constexpr int CHUNK = Shared<D>::CHUNK, BLOCKS = CHUNK / 16;
+    static constexpr int CHUNK = Shared<D>::CHUNK, TOGETHER = 128 / D;        // blocks of 16 tokens that are multiplied together
     uint32_t q[D / 16][2];
     float o[D / 16][4];                  // O^T: dims 16 i + g (+ 8), queries 2 tq (+ 1) at [i][2 * upper + (query & 1)]
     float m[2], l[2];                    // of queries 2 tq (+ 1): reference, this lane's tokens' sum
@@ -87,38 +87,31 @@ struct SharedQuery {
         m[0] = m[1] = -INFINITY;
         l[0] = l[1] = 0.f;
     }
-    // tokens lo .. hi - 1 of the chunk at `tile` (an address in shared memory); its hidden values are zeros
-    __device__ __forceinline__ void chunk(uint32_t tile, int lo, int hi, float scale_log2, int lane) {
+    // tokens lo .. hi - 1 of the chunk at `tile` (an address in shared memory) as far as they are among the 16 * TOGETHER from t0 on; hidden values are zeros
+    __device__ __forceinline__ void blocks(uint32_t tile, int t0, int lo, int hi, float scale_log2, int lane) {
         const int g = lane >> 2;
-        float s[BLOCKS][4], most[2] = {-INFINITY, -INFINITY};
+        float s[TOGETHER][4], most[2] = {-INFINITY, -INFINITY};
         // operands of several products are asked for ahead of the first (one by one, each waited for its own 33 clocks)
         uint32_t x[8][4];
-        constexpr int TOGETHER = 128 / D;                                    // blocks whose eight reads go together
 #pragma unroll
-        for (int b0 = 0; b0 < BLOCKS; b0 += TOGETHER) {
+        for (int i = 0; i < 8; ++i) ldmatrix_x4(tile + at(t0 + i / (D / 16) * 16 + (lane & 15), 2 * (i % (D / 16)) + (lane >> 4)), x[i][0], x[i][1], x[i][2], x[i][3]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int b = b0 + i / (D / 16), ks = i % (D / 16);
-                ldmatrix_x4(tile + at(16 * b + (lane & 15), 2 * ks + (lane >> 4)), x[i][0], x[i][1], x[i][2], x[i][3]);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int b = b0 + i / (D / 16), ks = i % (D / 16);
-                if (ks == 0) s[b][0] = s[b][1] = s[b][2] = s[b][3] = 0.f;
-                mma_f16_16816(s[b], x[i][0], x[i][1], x[i][2], x[i][3], q[ks][0], q[ks][1]);
-            }
+        for (int i = 0; i < 8; ++i) {
+            const int b = i / (D / 16), ks = i % (D / 16);
+            if (ks == 0) s[b][0] = s[b][1] = s[b][2] = s[b][3] = 0.f;
+            mma_f16_16816(s[b], x[i][0], x[i][1], x[i][2], x[i][3], q[ks][0], q[ks][1]);
         }
-        if (lo > 0 || hi < CHUNK) {
+        if (lo > t0 || hi < t0 + 16 * TOGETHER) {
 #pragma unroll
-            for (int b = 0; b < BLOCKS; ++b)
+            for (int b = 0; b < TOGETHER; ++b)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int t = 16 * b + 8 * (e >> 1) + g;
+                    const int t = t0 + 16 * b + 8 * (e >> 1) + g;
                     s[b][e] = t >= lo && t < hi ? s[b][e] : -INFINITY;
                 }
         }
 #pragma unroll
-        for (int b = 0; b < BLOCKS; ++b) {
+        for (int b = 0; b < TOGETHER; ++b) {
             most[0] = fmaxf(most[0], fmaxf(s[b][0], s[b][2]));
             most[1] = fmaxf(most[1], fmaxf(s[b][1], s[b][3]));
         }
@@ -138,27 +131,21 @@ struct SharedQuery {
         }
         const float r0 = kSharedTop - (m[0] == -INFINITY ? 0.f : m[0]), r1 = kSharedTop - (m[1] == -INFINITY ? 0.f : m[1]);
 #pragma unroll
-        for (int b0 = 0; b0 < BLOCKS; b0 += TOGETHER) {
+        for (int i = 0; i < 8; ++i)
+            ldmatrix_x4_trans(tile + Shared<D>::HALF + at(t0 + i / (D / 16) * 16 + (lane & 7) + (lane >> 4) * 8, 2 * (i % (D / 16)) + (lane >> 3 & 1)), x[i][0], x[i][1], x[i][2], x[i][3]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int b = b0 + i / (D / 16), n = i % (D / 16);
-                ldmatrix_x4_trans(tile + Shared<D>::HALF + at(16 * b + (lane & 7) + (lane >> 4) * 8, 2 * n + (lane >> 3 & 1)), x[i][0], x[i][1], x[i][2], x[i][3]);
+        for (int b = 0; b < TOGETHER; ++b) {
+            uint32_t pb[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float p0 = ex2_fast(fmaf(s[b][2 * h], scale_log2, r0)), p1 = ex2_fast(fmaf(s[b][2 * h + 1], scale_log2, r1));
+                l[0] += p0;
+                l[1] += p1;
+                const __half2 t = __floats2half2_rn(p0, p1);
+                asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pb[h]) : "r"(*reinterpret_cast<const uint32_t*>(&t)));
             }
 #pragma unroll
-            for (int u = 0; u < TOGETHER; ++u) {
-                const int b = b0 + u;
-                uint32_t pb[2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float p0 = ex2_fast(fmaf(s[b][2 * h], scale_log2, r0)), p1 = ex2_fast(fmaf(s[b][2 * h + 1], scale_log2, r1));
-                    l[0] += p0;
-                    l[1] += p1;
-                    const __half2 t = __floats2half2_rn(p0, p1);
-                    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pb[h]) : "r"(*reinterpret_cast<const uint32_t*>(&t)));
-                }
-#pragma unroll
-                for (int n = 0; n < D / 16; ++n) mma_f16_16816(o[n], x[u * (D / 16) + n][0], x[u * (D / 16) + n][1], x[u * (D / 16) + n][2], x[u * (D / 16) + n][3], pb[0], pb[1]);
-            }
+            for (int n = 0; n < D / 16; ++n) mma_f16_16816(o[n], x[b * (D / 16) + n][0], x[b * (D / 16) + n][1], x[b * (D / 16) + n][2], x[b * (D / 16) + n][3], pb[0], pb[1]);
         }
     }
     // sums over all lanes' tokens
@@ -308,9 +295,10 @@ __device__ __forceinline__ void shared_own(const SharedArgs& p, const SharedGrou
         ++it;
         const int seen = __shfl_sync(0xffffffffu, seen_x, x), lo = seen & 255, hi = seen >> 8;
         uint8_t* tile = ring + stage * C::CHUNK_BYTES;
+        constexpr int STEP = 16 * SharedQuery<D>::TOGETHER;                  // (steps that nothing sees are left out)
         if (lo > 0 || hi < CH) {                                             // hidden values may be anything: 0 * infinity is none
 #pragma unroll 1
-            for (int b = 0; b < CH; b += 16) {
+            for (int b = lo / STEP * STEP; b < (hi + STEP - 1) / STEP * STEP; b += 16) {
                 const int from_t = lo - b, to_t = hi - b;
                 if (from_t <= 0 && to_t >= 16) continue;
 #pragma unroll
@@ -322,7 +310,12 @@ __device__ __forceinline__ void shared_own(const SharedArgs& p, const SharedGrou
             fence_proxy_async();                                             // ahead of the next copy into this stage
             __syncwarp();
         }
-        a.chunk(smem_u32(tile), lo, hi, p.scale_log2, lane);
+        if constexpr (CH == STEP) {
+            a.blocks(smem_u32(tile), 0, lo, hi, p.scale_log2, lane);
+        } else {
+#pragma unroll 1
+            for (int t = lo / STEP * STEP; t < hi; t += STEP) a.blocks(smem_u32(tile), t, lo, hi, p.scale_log2, lane);
+        }
         __syncwarp();                                                        // all lanes have read it: the next copy may come
     }
     if (lane == 0)
@@ -883,7 +876,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
 }
 
 // ------------------------------------------------------------------ all parts of a (sequence, key head) as one
-constexpr int SM_PARTS = 5;                      // parts that a thread asks for at once
+constexpr int SM_PARTS = 3;                      // parts that a thread asks for at once
 template <int D, int SM_THREADS>
 __global__ void __launch_bounds__(SM_THREADS, 1024 / SM_THREADS)
 shared_merge_kernel(const __grid_constant__ SharedArgs p) {
