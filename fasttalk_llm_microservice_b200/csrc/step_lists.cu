@@ -7,13 +7,13 @@
 // cut so and S_r their sum ahead, the budget leaves max(0, budget - S_r), and nobody behind the one that it cuts gets any; so P_r is also where r's pages begin.
 //
 // What bounds it: latency alone (a launch, two rounds of reads, two scans, a search, a store).  Every CTA makes the scans for itself, one request a thread, which costs less
-// than a kernel ahead of this one, and then looks up 1024 tokens and writes its part of the table.
+// than a kernel ahead of this one, and then looks up 512 tokens and writes its part of the table.
 #include "common.cuh"
 #include "ft_internal.h"
 
 namespace ft {
 
-constexpr int SL_THREADS = 1024, SL_WARPS = SL_THREADS / 32;
+constexpr int SL_THREADS = 512, SL_WARPS = SL_THREADS / 32;
 constexpr int SL_MAX_REQUESTS = 8192;
 constexpr int SL_NONE = -1;
 
@@ -31,7 +31,7 @@ __device__ __forceinline__ long long block_before(long long mine, long long* war
     __syncthreads();                                           // the last call's sums have been read
     if (lane == 31) warp_s[warp] = x;
     __syncthreads();
-    long long w = warp_s[lane];
+    long long w = lane < SL_WARPS ? warp_s[lane] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const long long up = __shfl_up_sync(0xffffffffu, w, o);
@@ -185,6 +185,7 @@ extern "C" int ft_step_lists(const ft_step_lists_args* args, void* stream) {
     FT_REQUIRE(req_start && taken && (R == 0 || (cached_lens && new_lens && ctx_lens)) && (max_tokens == 0 || (positions && seq_rows && kv_slots)) &&
                    (page_table || table_rows == 0 || max_pages == 0) && (free_pages || n_free == 0),
                "ft_step_lists: null argument");
+    FT_REQUIRE(taken != first_free, "ft_step_lists: taken at the address of first_free, which other CTAs may read later");
     static PerDeviceFlag attr_set;
     if (!attr_set.done()) {
         FT_CHECK_CUDA(cudaFuncSetAttribute(step_lists_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,

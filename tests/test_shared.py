@@ -33,6 +33,11 @@ def test_refusals_of_lists(lib):
         refused(call(**bad), "null argument")
 
 
+def test_the_rest_of_the_pool_is_told_elsewhere(lib):
+    """Where a step's lists are told from the rest of a pool, that address may still be read when the new rest is written."""
+    refused(lib.ft_step_lists(N.STEP_LISTS_ARGS.pack(P, P, 0, P, P, 2 * P, P, P, P, P, P, 2 * P, 1, 1, 1, 1, 1), 0), "first_free")
+
+
 def test_refusals_of_appending(lib):
     call = lambda d=64, kind=0, T=1, nq=4, nkv=1, S=1, pages=1, rotated=0, angles=8, cos=P, q_gain=0, q_gains=1, k_gain=0, k_gains=1, qkv=P, pos=P, out=P, cache=P: lib.ft_norm_rope_kv_append(
         N.NORM_APPEND_ARGS.pack(qkv, 0, 0, cos, P, q_gain, k_gain, pos, P, out, cache, kind, S, angles, rotated, 0, q_gains, k_gains, pages, T, nq, nkv, d, 1e-5), 0)
