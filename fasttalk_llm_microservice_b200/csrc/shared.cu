@@ -66,6 +66,21 @@ __device__ __forceinline__ bool shared_wait(uint64_t* bar, uint32_t parity, vola
     return false;
 }
 
+// Whether two of them are over already: tries that do not sleep, on their way together
+__device__ __forceinline__ void shared_over(uint64_t* bar0, uint32_t parity0, uint64_t* bar1, uint32_t parity1, bool& over0, bool& over1) {
+    uint32_t x, y;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%2], %3;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 q, [%4], %5;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "selp.u32 %1, 1, 0, q;\n\t}\n"
+        : "=r"(x), "=r"(y)
+        : "r"(smem_u32(bar0)), "r"(parity0), "r"(smem_u32(bar1)), "r"(parity1)
+        : "memory");
+    over0 = x, over1 = y;
+}
+
 // floats of an own part: O [G][D], (m, l) of the heads; on 16 bytes
 __host__ __device__ __forceinline__ int shared_part(int G, int d) { return (G * (d + 2) + 3) / 4 * 4; }
 
@@ -243,12 +258,14 @@ __device__ __forceinline__ void shared_own(const SharedArgs& p, const SharedGrou
             const int y = __ffs(to_ask) - 1, stage = asked % S;
             uint8_t* dst = ring + stage * C::CHUNK_BYTES;
             const uint8_t* src = (const uint8_t*)__shfl_sync(0xffffffffu, (unsigned long long)src_x, y);
-            if (lane == 0) mbar_expect_tx(&full[stage], C::CHUNK_BYTES);
-            if (CH == kKvTile) {
-                if (lane == 0) tma_bulk_g2s(dst, src, C::CHUNK_BYTES, &full[stage], pol);
-            } else {                                                         // 2 D / 64 pieces, a lane each
-                __syncwarp();
-                if (lane < 2 * C::KH) tma_bulk_g2s(dst + lane * (CH * 128), src + lane * SH_PIECE, CH * 128, &full[stage], pol);
+            if (elect_one()) {
+                mbar_expect_tx(&full[stage], C::CHUNK_BYTES);
+                if (CH == kKvTile) {
+                    tma_bulk_g2s(dst, src, C::CHUNK_BYTES, &full[stage], pol);
+                } else {                                                     // 2 D / 64 pieces
+#pragma unroll
+                    for (int j = 0; j < 2 * C::KH; ++j) tma_bulk_g2s(dst + j * (CH * 128), src + j * SH_PIECE, CH * 128, &full[stage], pol);
+                }
             }
             to_ask &= to_ask - 1;
             ++asked;
@@ -429,13 +446,15 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
         const int bc = (p.B + SH_THREADS - 1) / SH_THREADS, b0 = min(p.B, tid * bc), b1 = min(p.B, b0 + bc);
         const int ctx0 = b0 < b1 ? p.ctx_lens[b0] : 0;
         if (bc == 1 && b0 < b1 && p.req_slot) asm volatile("prefetch.global.L1 [%0];" ::"l"(p.req_slot + b0));       // the own warps look these up first
-        if (p.n_groups <= SH_LIST) {
-            if (p.n_groups && tid <= p.n_groups) start_s[tid] = p.group_start[tid];
+        // Groups that are looked for are kept in shared memory: two of them 22.5 us a call, not kept 23.3, five 23.1 and 24.0; for one alone the round through it
+        // costs more than it saves (21.0 and 20.4)
+        if (p.n_groups > 1 && p.n_groups <= SH_LIST) {
+            if (tid <= p.n_groups) start_s[tid] = p.group_start[tid];
             if (tid < p.n_groups) lens_s[tid] = p.shared_lens[tid];
             gr.start = start_s;
             gr.lens = lens_s;
+            __syncthreads();
         }
-        __syncthreads();
         bool grows = true;
         // prefix steps and own steps where prefixes are shared, own steps where they are not, pages saved
         int mine[4], before[4], all[4];
@@ -547,17 +566,22 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
         } else if (warp == 0) {
             // ---------------- copies of the prefix: a page's keys, and the values of the page two ahead of it, which are needed that much later.  (Never a circle: keys wait for
             // products of keys STAGES pages back, which wait for products of values further back than those that are copied behind them.)
+            // Lane 0 the keys, lane 1 the values, side by side: what a warp asks shared memory for comes back after some 200 clocks here, behind the exponentials of the same
+            // scheduler, and one lane that did one after the other took 1350 to 2050 clocks a page, whatever its size (now 1000; one prefix of 40960 tokens, heads of 64, for 65
+            // queries 123 -> 65 us, for 8 36.7 -> 29.9)
             const uint64_t pol = policy_evict_first();
             SharedPhases phases[2];                                          // keys, values
-            int n = 0, it = 0, k = 0, k1 = 0, my_page = -1, row = -1;        // stretches heard, pages asked for; of the 32 at hand: the next, how many
-            const uint8_t* v_from[C::AHEAD];                                 // pages whose values are still to be asked for (null: not there), and their sets
-            int v_set[C::AHEAD];
+            int at[2] = {0, 0};                                              // the next stages
+            uint32_t turn[2] = {1, 1};
+            int n = 0, k = 0, k1 = 0, my_page = -1, row = -1;                // stretches heard; of the 32 pages at hand: the next, how many
+            const uint8_t* from[C::AHEAD + 1];                               // the last pages (null: not there), the newest first, and their sets
+            int set[C::AHEAD + 1], page = -1;
             SharedStretch w;
             w.pages = 0;
             int p0 = 0, p1 = 0;                                              // pages of the stretch that are not at hand yet
             bool more = true;
 #pragma unroll 1
-            for (int drain = 0; drain < C::AHEAD; ++it) {
+            for (int drain = 0, it = 0; drain < C::AHEAD; ++it) {
                 if (more && k == k1) {
                     if (p0 == p1) {
                         if (n) heard(n - 1);
@@ -572,36 +596,43 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
                     k = 0;
                     k1 = min(32, p1 - p0);
                     p0 += k1;
+                    page = __shfl_sync(0xffffffffu, my_page, 0);
                 }
                 if (!more) ++drain;
-                const int page = __shfl_sync(0xffffffffu, my_page, k), tile = p0 - k1 + k;
-                if (lane == 0) {
-                    const uint8_t* from[2] = {page >= 0 ? p.cache + ((size_t)page * p.nkv + w.h) * C::TILE : nullptr, v_from[0]};
-                    const int set[2] = {w.few ? (tile - w.p0) & 1 : 2, v_set[0]};
+                const int tile = p0 - k1 + k, next_page = __shfl_sync(0xffffffffu, my_page, (k + 1) & 31);
 #pragma unroll
-                    for (int i = 0; i < C::AHEAD; ++i) {
-                        v_from[i] = i + 1 < C::AHEAD ? v_from[i + 1] : from[0] ? from[0] + C::SLAB : nullptr;
-                        v_set[i] = i + 1 < C::AHEAD ? v_set[i + 1] : set[0];
-                    }
+                for (int i = C::AHEAD; i > 0; --i) from[i] = from[i - 1], set[i] = set[i - 1];
+                from[0] = page >= 0 ? p.cache + ((size_t)page * p.nkv + w.h) * C::TILE : nullptr;
+                set[0] = w.few ? (tile - w.p0) & 1 : 2;
+                if (ok) {
+                    uint64_t* full[2];
+                    bool over[2];
+                    const uint8_t* const src[2] = {from[0], from[C::AHEAD]};
+                    shared_over(&k_empty[at[0]], turn[0], &v_empty[at[1]], turn[1], over[0], over[1]);
 #pragma unroll
                     for (int kind = 0; kind < 2; ++kind) {
-                        if (kind ? it < C::AHEAD : !more) continue;
-                        const int i = it - kind * C::AHEAD, s = i % C::STAGES;
-                        ok = ok && shared_wait(kind ? &v_empty[s] : &k_empty[s], (i / C::STAGES & 1) ^ 1, &dead);
-                        if (!ok) continue;
-                        phases[kind].next(C::STAGES, s, set[kind]);
-                        uint64_t* const full = (kind ? v_full : k_full) + phases[kind].at;
-                        // (keys are copied when those STAGES back have been multiplied, which is when the scores of eight back were read)
-                        if (kind == 0) tokens_s[i % C::TOKENS] = page >= 0 ? min(kKvTile, w.tokens - tile * kKvTile) : 0;
-                        if (from[kind]) {
-                            mbar_expect_tx(full, C::SLAB);
-                            tma_bulk_g2s(smem + C::KV + (kind * C::STAGES + s) * C::SLAB, from[kind], C::SLAB, full, pol);
-                        } else {
-                            mbar_arrive(full);
+                        if (!ok || (kind ? it < C::AHEAD : !more)) continue;
+                        phases[kind].next(C::STAGES, at[kind], set[kind * C::AHEAD]);
+                        full[kind] = (kind ? v_full : k_full) + phases[kind].at;
+                        if (!over[kind]) ok = wait((kind ? v_empty : k_empty) + at[kind], turn[kind]);
+                        if (!ok) {
+                            phases[kind].bits ^= 1u << phases[kind].at;
+                            continue;
                         }
+                        if (elect_one()) {
+                            // (keys are copied when those STAGES back have been multiplied, which is when the scores of eight back were read)
+                            if (kind == 0) tokens_s[it % C::TOKENS] = page >= 0 ? min(kKvTile, w.tokens - tile * kKvTile) : 0;
+                            if (src[kind]) {
+                                mbar_expect_tx(full[kind], C::SLAB);
+                                tma_bulk_g2s(smem + C::KV + (kind * C::STAGES + at[kind]) * C::SLAB, src[kind] + kind * C::SLAB, C::SLAB, full[kind], pol);
+                            } else {
+                                mbar_arrive(full[kind]);
+                            }
+                        }
+                        if (++at[kind] == C::STAGES) at[kind] = 0, turn[kind] ^= 1;
                     }
                 }
-                ok = __shfl_sync(0xffffffffu, ok, 0);
+                page = next_page;
                 if (more) ++k;
             }
             k_bits = phases[0].bits;
@@ -618,10 +649,14 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
                 const uint32_t s_at = tmem + C::COL_S + h * 128, o_at = tmem + C::COL_O + h * D;
                 SharedPhases k_phases, v_phases;
                 int base = 0, n_qk = 0, n_pv = 0, n_q = 0;                   // pages of the share, products of this half, stretches of this half so far
-                auto issue_qk = [&](int page, bool alone) {                  // page: counted over the whole share; alone: the other half has no use for it
+                struct Landing { uint64_t* bar; uint32_t parity; bool over; };
+                auto landing = [&](SharedPhases& phases, uint64_t* full, int page, bool alone) {       // page: counted over the whole share; alone: the other half has no use for it
+                    const uint32_t parity = phases.next(C::STAGES, page % C::STAGES, alone ? h : 2);
+                    return Landing{full + phases.at, parity, false};
+                };
+                auto issue_qk = [&](int page, bool alone, const Landing& k_in) {
                     const int s = page % C::STAGES, buf = n_qk & 1;
-                    const uint32_t parity = k_phases.next(C::STAGES, s, alone ? h : 2);
-                    ok = shared_wait(&k_full[k_phases.at], parity, &dead);
+                    ok = k_in.over || shared_wait(k_in.bar, k_in.parity, &dead);
                     if (!ok) return;
                     ++n_qk;
                     tc_fence_after();
@@ -634,10 +669,9 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
                     umma_commit(&k_empty[s]);
                     if (alone) umma_commit(&k_empty[s]);
                 };
-                auto issue_pv = [&](int page, bool first, bool alone) {
+                auto issue_pv = [&](int page, bool first, bool alone, const Landing& v_in) {
                     const int s = page % C::STAGES, buf = n_pv & 1;
-                    const uint32_t parity = v_phases.next(C::STAGES, s, alone ? h : 2);
-                    ok = shared_wait(&v_full[v_phases.at], parity, &dead) && shared_wait(&p_full[h][buf], n_pv >> 1 & 1, &dead);
+                    ok = shared_wait(&p_full[h][buf], n_pv >> 1 & 1, &dead) && (v_in.over || shared_wait(v_in.bar, v_in.parity, &dead));
                     if (!ok) return;
                     ++n_pv;
                     tc_fence_after();
@@ -660,8 +694,12 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
                         // Scores run two pages ahead, issued behind the product that reads the probabilities in their buffer
 #pragma unroll 1
                         for (int i = -2; ok && i < mine; ++i) {
-                            if (i >= 0) issue_pv(page_of(i), i == 0, w.few);
-                            if (ok && i + 2 < mine) issue_qk(page_of(i + 2), w.few);
+                            Landing v_in{v_full, 0, false}, k_in{k_full, 0, false};
+                            if (i >= 0) v_in = landing(v_phases, v_full, page_of(i), w.few);
+                            if (i + 2 < mine) k_in = landing(k_phases, k_full, page_of(i + 2), w.few);
+                            shared_over(v_in.bar, v_in.parity, k_in.bar, k_in.parity, v_in.over, k_in.over);
+                            if (i >= 0) issue_pv(page_of(i), i == 0, w.few, v_in);
+                            if (ok && i + 2 < mine) issue_qk(page_of(i + 2), w.few, k_in);
                         }
                     }
                     if (mine) ++n_q;
@@ -876,8 +914,8 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
 }
 
 // ------------------------------------------------------------------ all parts of a (sequence, key head) as one
-constexpr int SM_PARTS = 3;                      // parts that a thread asks for at once
-template <int D, int SM_THREADS>
+constexpr int SM_PARTS = 3, SM_THREADS = 256;     // parts that a thread asks for at once
+template <int D>
 __global__ void __launch_bounds__(SM_THREADS, 1024 / SM_THREADS)
 shared_merge_kernel(const __grid_constant__ SharedArgs p) {
     pdl_wait();
@@ -1000,10 +1038,7 @@ static int launch_shared(SharedArgs& p, cudaStream_t st) {
     p.give_up = g_shared_give_up.load(std::memory_order_relaxed);
     p.ctas = device_sms();
     FT_CHECK_CUDA(launch_after(shared_attn_kernel<D>, dim3(p.ctas), dim3(SH_THREADS), C::SMEM, st, (const SharedArgs&)p));
-    // few units: more threads for each one's parts (24 sequences x 8 key heads of 128, 20 parts each, 7.0 us with 256)
-    const int units = p.B * p.nkv;
-    if (units <= 2 * device_sms()) FT_CHECK_CUDA(launch_after(shared_merge_kernel<D, 512>, dim3(units), dim3(512), 0, st, (const SharedArgs&)p));
-    else FT_CHECK_CUDA(launch_after(shared_merge_kernel<D, 256>, dim3(units), dim3(256), 0, st, (const SharedArgs&)p));
+    FT_CHECK_CUDA(launch_after(shared_merge_kernel<D>, dim3(p.B * p.nkv), dim3(SM_THREADS), 0, st, (const SharedArgs&)p));
     return 0;
 }
 
