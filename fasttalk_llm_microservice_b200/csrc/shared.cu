@@ -9,6 +9,11 @@
 //   own      a warp walks a share of its own: chunks of 16 or 8 KB by bulk copies that it asks for itself, two of them on their way while it multiplies (mma.sync, the
 //            query heads of a key head in the columns).  No warp waits for another.
 // Each share's results are O, maximum and sum of its rows; a second kernel puts them together in their order.
+//
+// Measured in a graph, us (launch included), what it has to read at 6.46 TB/s in brackets: 64 sequences behind one prefix of 2048 tokens, 600 own, 32 heads of 64 over 8, 20.4 (7.4);
+// 24 behind one of 16001, 300 own, 32 heads of 128 over 8, 25.5 (12.6); two behind 517, 9.8 (0.2).  What bounds it: 4.4 us from the launch to the first page asked for (the
+// plan 2.0, what the shares begin with 1.4, a copy 1.3), then memory (74 MB in about 11 us) or, where all 256 rows of a tile are in use, the softmax (2000 clocks a page and
+// half pair of which 1024 are exponentials), 1 to 2 us to write O, and the second kernel, 3.5 to 6 with its launch.
 #include <atomic>
 
 #include "common.cuh"
@@ -28,8 +33,10 @@ static_assert(SH_REGS_ISSUE + 2 * SH_REGS_SOFT + SH_REGS_OWN <= 4 * SH_REGS, "wh
 constexpr int SH_SOFT = 256;
 constexpr int SH_TOLD = 4, SH_LISTENERS = 11;    // stretches told ahead; warps that hear of them
 constexpr int SH_STRETCH = 64;                   // times the limit, for what takes a whole stretch: it may be a million keys
+// Steps of a share of the prefix at least: fewer CTAs have one, with fewer results, and the others more of the own list.  Per share 3 / 4 / 5 / 6 steps, us: 64 sequences behind 2048
+// tokens 22.5 / 20.4 / 20.6 / 20.6, 128 behind two prefixes of 1500 22.3 / 22.4 / 22.6 / 22.8, 37 behind five of 4099 23.0 / 23.0 / 23.0 / 23.3
 constexpr int SH_LEAST = 4;
-constexpr int SH_COST = 2;                       // steps of the prefix that cost a warp on its SM one of its own
+constexpr int SH_COST = 2;                       // steps of the prefix that cost a warp on its SM one of its own (1 / 2 / 3 / none: the first of these 23.7 / 20.4 / 21.9 / 22.3)
 constexpr int SH_LIST = 100;                     // groups whose lists are kept in shared memory
 constexpr int SH_PIECE = kKvTile * 128;          // [64 tokens][64 dims] in fp16
 
@@ -44,7 +51,8 @@ struct Shared {
     static constexpr int AHEAD = 2;                                          // pages that keys are copied ahead of values
     static constexpr int QBLK = kSharedRows * 128;                           // [128 rows][64 dims]
     static constexpr int OWN_WARPS = 4, OWN_STAGES = 2;
-    static constexpr int CHUNK = D == 64 ? 64 : 16;                          // tokens
+    // tokens: what is left of shared memory, for four warps (at heads of 128 two warps with 32 tokens each: 128 sequences with 150 own 30.3 us, four with 16 24.5)
+    static constexpr int CHUNK = D == 64 ? 64 : 16;
     static constexpr int CHUNK_BYTES = 2 * CHUNK * D * 2, HALF = CHUNK_BYTES / 2;        // keys | values; of each D / 64 pieces of [CHUNK][64 dims]
     static constexpr int KV = 2 * KH * QBLK, OWN = KV + STAGES * TILE, SMEM = 1024 + OWN + OWN_WARPS * OWN_STAGES * CHUNK_BYTES;
     // tensor memory: scores [half][2][64 columns] (probabilities, pairs of fp16, over the first 32 of them), O [half][D]
@@ -53,8 +61,8 @@ struct Shared {
     static_assert(SMEM <= 232448 - 2048, "shared memory (the rest is what the kernel declares)");
 };
 
-// A wait that ends, in a few instructions: what bounds calls of ten microseconds here is among others how much code they touch for the first time (126 KB, with waits and
-// loops unrolled and the walk in every role, took 3 of 10 issue slots' worth of waiting for instructions)
+// A wait that ends, in a few instructions: calls of ten microseconds touch most of their code for the first time.  (With waits and loops unrolled and the walk in every role
+// the two kernels were 126 KB and a call over 16001 tokens took 35.8 us; with a loop here and the walk in one warp, 78 KB, 31.)
 // Who gives up touches none of the barriers again: what it skipped would make it take one phase for another.
 __device__ __forceinline__ bool shared_wait(uint64_t* bar, uint32_t parity, volatile int* dead, int times = 1) {
 #pragma unroll 1
@@ -566,9 +574,9 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
         } else if (warp == 0) {
             // ---------------- copies of the prefix: a page's keys, and the values of the page two ahead of it, which are needed that much later.  (Never a circle: keys wait for
             // products of keys STAGES pages back, which wait for products of values further back than those that are copied behind them.)
-            // Lane 0 the keys, lane 1 the values, side by side: what a warp asks shared memory for comes back after some 200 clocks here, behind the exponentials of the same
-            // scheduler, and one lane that did one after the other took 1350 to 2050 clocks a page, whatever its size (now 1000; one prefix of 40960 tokens, heads of 64, for 65
-            // queries 123 -> 65 us, for 8 36.7 -> 29.9)
+            // What a warp asks shared memory for comes back after some 200 clocks here, behind the exponentials of the same scheduler.  So both empty stages are asked for at once, and one
+            // elected thread copies (with a lane picked by its number the compiler cannot know that it is alone): with one after the other a page took 1350 to 2050 clocks, whatever its
+            // size, now 1000 (one prefix of 40960 tokens, heads of 64: for 8 queries 36.7 -> 29.8 us, for 65 123 -> 65.8).  A lane for each kind was slower (35.8, 116).
             const uint64_t pol = policy_evict_first();
             SharedPhases phases[2];                                          // keys, values
             int at[2] = {0, 0};                                              // the next stages
@@ -719,7 +727,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
         // ---------------- softmax: one thread a row
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SH_REGS_SOFT));
         const int h = (warp - 4) >> 2;
-        const int row = (tid - 128) & 127;                                           // lane of tensor memory: warp % 4 is the quarter that a warp may read
+        const int row = (tid - 128) & 127;                                   // lane of tensor memory: warp % 4 is the quarter that a warp may read
         const int tok = row * p.inv_g >> 16;
         const uint32_t lanes = tmem + ((uint32_t)(row & 96) << 16);
         const uint32_t s_at0 = lanes + C::COL_S + h * 128, o_at = lanes + C::COL_O + h * D;
@@ -914,7 +922,9 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
 }
 
 // ------------------------------------------------------------------ all parts of a (sequence, key head) as one
-constexpr int SM_PARTS = 3, SM_THREADS = 256;     // parts that a thread asks for at once
+// Parts that a thread asks for at once, threads.  64 sequences behind 2048 tokens: five parts cost 0.7 us more, 512 threads 2.9; one unit an SM (37 sequences, four key heads):
+// 512 threads 0.2 us less.  The kernel takes 3.5 to 6 us, of which 1 is the launch and 3 are waits for what was written last
+constexpr int SM_PARTS = 3, SM_THREADS = 256;
 template <int D>
 __global__ void __launch_bounds__(SM_THREADS, 1024 / SM_THREADS)
 shared_merge_kernel(const __grid_constant__ SharedArgs p) {
@@ -1028,10 +1038,10 @@ static int launch_shared(SharedArgs& p, cudaStream_t st) {
         attr_set.mark();
     }
     p.chunk_log = C::CHUNK == 64 ? 6 : 4;
-    // What sharing has to save, measured with one group and 100 own tokens each, us shared / not: heads of 64 (32 over 8), two sequences of 8000 tokens 16.2 / 14.4, four of
-    // 2000 13.7 / 12.6 (16 MB saved), four of 8000 16.3 / 17.1, sixteen of 130 11.6 / 10.5, of 517 12.1 / 13.6; heads of 128 (32 over 8), two of 2000 15.2 / 15.5 (8 MB), four of
-    // 130 12.6 / 10.7, of 517 12.8 / 13.4 (6 MB); sixteen key heads, two of 517 14.1 / 13.5, four of 130 13.6 / 12.2, of 517 14.2 / 15.7.  At heads of 64 a step of the prefix takes as
-    // long as two own ones.
+    // What sharing has to save, measured with one group and 100 own tokens each, us shared / not: heads of 64 (32 over 8), two sequences of 8000 tokens 15.0 / 15.5, of 16000
+    // 18.3 / 18.2, three of 2000 12.8 / 12.6, of 8000 15.1 / 16.8 (16 MB saved, from the third on), eight of 1000 12.1 / 11.8, of 2000 13.2 / 14.4 (24 MB), sixteen of 130 11.8 / 10.4,
+    // of 517 11.9 / 13.4 (15 MB); heads of 128 (32 over 8), two of 1000 13.6 / 13.3, of 2000 15.3 / 15.3 (8 MB), of 8000 17.8 / 23.5, four of 517 12.8 / 13.0 (6 MB), eight of
+    // 130 12.9 / 11.9, of 517 13.1 / 13.6; sixteen key heads, two of 1000 15.0 / 12.9, of 2000 16.2 / 15.8 (16 MB), four of 130 13.2 / 11.4, of 517 13.5 / 14.1 (13 MB).
     const long long least = g_shared_least.load(std::memory_order_relaxed), pages = (least < 0 ? (D == 64 ? 12 : 6) << 20 : least) / ((long long)C::TILE * p.nkv);
     p.least_size = D == 64 && least < 0 ? 3 : 2;
     p.least_pages = (int)(pages < INT32_MAX ? pages : INT32_MAX) + (least < 0);

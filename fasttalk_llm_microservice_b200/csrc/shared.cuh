@@ -80,7 +80,8 @@ struct SharedPrefix {
         tiles = pages ? p.tiles(size) : 0;
     }
     __host__ __device__ __forceinline__ int queries(const SharedArgs& p, int tile) const { return min(2 * p.th, size - tile * 2 * p.th); }
-    // steps of a tile of n queries: where they fill one half only, each half takes every other page
+    // steps of a tile of n queries: where they fill one half only, each half takes every other page (40960 tokens, heads of 64, four to a key head: 32 queries in this way
+    // 31.5 us, 33 in the other 46.5)
     __host__ __device__ __forceinline__ int steps(const SharedArgs& p, int n) const { return n <= p.th ? (pages + 1) / 2 : pages; }
     // what all tiles of one key head take of the list
     __host__ __device__ __forceinline__ int each(const SharedArgs& p) const { return (tiles - 1) * (pages + kSharedStart) + steps(p, queries(p, tiles - 1)) + kSharedStart; }
