@@ -613,28 +613,24 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
                 from[0] = page >= 0 ? p.cache + ((size_t)page * p.nkv + w.h) * C::TILE : nullptr;
                 set[0] = w.few ? (tile - w.p0) & 1 : 2;
                 if (ok) {
-                    uint64_t* full[2];
                     bool over[2];
                     const uint8_t* const src[2] = {from[0], from[C::AHEAD]};
                     shared_over(&k_empty[at[0]], turn[0], &v_empty[at[1]], turn[1], over[0], over[1]);
 #pragma unroll
                     for (int kind = 0; kind < 2; ++kind) {
                         if (!ok || (kind ? it < C::AHEAD : !more)) continue;
+                        if (!__all_sync(0xffffffffu, over[kind])) ok = wait((kind ? v_empty : k_empty) + at[kind], turn[kind]);       // (one lane may have seen it later than another)
+                        if (!ok) continue;
                         phases[kind].next(C::STAGES, at[kind], set[kind * C::AHEAD]);
-                        full[kind] = (kind ? v_full : k_full) + phases[kind].at;
-                        if (!over[kind]) ok = wait((kind ? v_empty : k_empty) + at[kind], turn[kind]);
-                        if (!ok) {
-                            phases[kind].bits ^= 1u << phases[kind].at;
-                            continue;
-                        }
+                        uint64_t* const full = (kind ? v_full : k_full) + phases[kind].at;
                         if (elect_one()) {
                             // (keys are copied when those STAGES back have been multiplied, which is when the scores of eight back were read)
                             if (kind == 0) tokens_s[it % C::TOKENS] = page >= 0 ? min(kKvTile, w.tokens - tile * kKvTile) : 0;
                             if (src[kind]) {
-                                mbar_expect_tx(full[kind], C::SLAB);
-                                tma_bulk_g2s(smem + C::KV + (kind * C::STAGES + at[kind]) * C::SLAB, src[kind] + kind * C::SLAB, C::SLAB, full[kind], pol);
+                                mbar_expect_tx(full, C::SLAB);
+                                tma_bulk_g2s(smem + C::KV + (kind * C::STAGES + at[kind]) * C::SLAB, src[kind] + kind * C::SLAB, C::SLAB, full, pol);
                             } else {
-                                mbar_arrive(full[kind]);
+                                mbar_arrive(full);
                             }
                         }
                         if (++at[kind] == C::STAGES) at[kind] = 0, turn[kind] ^= 1;
