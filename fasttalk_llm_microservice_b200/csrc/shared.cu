@@ -216,7 +216,7 @@ __device__ __forceinline__ void shared_own(const SharedArgs& p, const SharedGrou
     for (int f = f0;; ++f) {
         const int x = (f - f0) & 31;
         if (x == 0 && f < f_end) {
-            // ---- the next 32 sequences hold 32 steps at least
+            // ---- the next 32 steps, in the 32 sequences from b0 on (own_sequence says why they are there)
             const int b = b0 + lane;
             SharedSeq s;
             int row = -1, led_row = -1;
@@ -235,10 +235,7 @@ __device__ __forceinline__ void shared_own(const SharedArgs& p, const SharedGrou
             }
             end += base;
             const int F = min(f + lane, f_end - 1);
-            int l = 0;                                                       // the first that ends behind F
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1)
-                if (__shfl_sync(0xffffffffu, end, l + o - 1) <= F) l += o;
+            const int l = own_sequence(F, [&](int i) { return __shfl_sync(0xffffffffu, end, i); });
             SharedSeq w;
             w.ctx = __shfl_sync(0xffffffffu, s.ctx, l);
             w.begin = __shfl_sync(0xffffffffu, s.begin, l);
@@ -246,17 +243,18 @@ __device__ __forceinline__ void shared_own(const SharedArgs& p, const SharedGrou
             w.steps = __shfl_sync(0xffffffffu, s.steps, l);
             prefix_x = __shfl_sync(0xffffffffu, (int)s.prefix, l);
             const int base_l = __shfl_sync(0xffffffffu, end - span, l), r_own = __shfl_sync(0xffffffffu, row, l), r_led = __shfl_sync(0xffffffffu, led_row, l);
-            const int head = (int)((unsigned)(F - base_l) / (unsigned)w.steps);
-            from_x = base_l + head * w.steps;
-            last_x = from_x + w.steps - 1;
-            unit_x = (b0 + l) * p.nkv + head;
+            OwnStep step;
+            step.set(p, F, b0 + l, base_l, w.steps);
+            from_x = step.from;
+            last_x = step.last;
+            unit_x = (b0 + l) * p.nkv + step.head;
             int lo, hi, page = -1;
             const int r = w.step(p, F - from_x, lo, hi) ? r_led : r_own, at = lo / CH * CH;
             if (f + lane < f_end && lo < hi && r >= 0) page = p.page_table[(size_t)r * p.max_pages + at / kKvTile];
             seen_x = lo - at | hi - at << 8;
-            src_x = p.cache + ((size_t)page * p.nkv + head) * C::TILE + at % kKvTile * 128;
-            b0 += __shfl_sync(0xffffffffu, l, 31);
-            base = __shfl_sync(0xffffffffu, base_l, 31);
+            src_x = p.cache + ((size_t)page * p.nkv + step.head) * C::TILE + at % kKvTile * 128;
+            b0 = __shfl_sync(0xffffffffu, step.next_seq, 31);
+            base = __shfl_sync(0xffffffffu, step.next_base, 31);
             to_ask = paged = __ballot_sync(0xffffffffu, page >= 0 && page < p.num_pages);
             if (unit < 0) query_of(__shfl_sync(0xffffffffu, unit_x, 0));
         }

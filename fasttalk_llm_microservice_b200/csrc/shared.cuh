@@ -147,6 +147,31 @@ struct OwnShares {
     }
 };
 
+// A warp looks up 32 steps of the own list at once, a lane each: F, F + 1 .. among 32 sequences, the first of which holds step F.  Every sequence has a step at least, so that the 32 hold
+// all of these; a sequence that is over by F would leave 31, which with one key head and a step each is one too few.  Which of them holds F; end_of(i): behind the last step of the i-th
+template <class EndOf>
+__host__ __device__ __forceinline__ int own_sequence(int F, EndOf&& end_of) {
+    int l = 0;                                   // the first that ends behind F
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        if (end_of(l + o - 1) <= F) l += o;
+    return l;
+}
+
+// Step F, in sequence `seq`, whose steps (so many for each key head) begin at `base`
+struct OwnStep {
+    int head, from, last;                        // the unit: its key head, its first and last step
+    int next_seq, next_base;                     // the sequence that holds step F + 1, and where that begins
+    __host__ __device__ __forceinline__ void set(const SharedArgs& p, int F, int seq, int base, int steps) {
+        head = (int)((unsigned)(F - base) / (unsigned)steps);
+        from = base + head * steps;
+        last = from + steps - 1;
+        const bool over = F == last && head == p.nkv - 1;
+        next_seq = seq + over;
+        next_base = over ? last + 1 : base;
+    }
+};
+
 // n queries from q0 on, over pages p0 .. of the row of query seq0; row0: where the first one's results lie; last: the last share that the unit lies in
 struct SharedStretch {
     int p0, pages, n, h, seq0, q0, row0, tokens, last;

@@ -41,7 +41,7 @@ extern "C" int shared_stretches(int own, const int* ctx_lens, int B, const int* 
     for (int x = 0; x < (own ? shares * warps : shares); ++x) {
         const int f = min(own ? of.begin(x / shares, x % shares) : per * x, total), end = min(f + (own ? of.size(x % shares) : per), total);
         int base = 0, at = 0;
-        if (own) {                                   // step by step, as the kernel's lanes find them; told as stretches
+        if (own) {                                   // step by step, told as stretches (how the kernel looks steps up: shared_windows.cu)
             SharedSeq s;
             for (; f < end; base += s.steps * nkv, ++at) {
                 s.load(p, gr, at, ctx_lens[at]);

@@ -674,6 +674,34 @@ def test_thousands_of_sequences(K, sharing, d):
     check(K, make(50 + d, 2, 1, d, [2000, 900], [300, 150], [i * 7 % 40 for i in range(n)]))
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_tens_of_thousands_of_short_sequences(K, sharing, d):
+    """One key head and a step for nearly every sequence: a warp's share is several times the 32 steps that it looks up at once."""
+    g = gen(70 + d)
+    n, pages, L = 75000, 300, 100
+    x = torch.randn(pages, 1, 2, 64, d, generator=g, device=DEV).half()
+    q = (1.5 * torch.randn(n, 2, d, generator=g, device=DEV)).half()
+    table = torch.randint(0, pages, (n, 2), generator=g, device=DEV).int()
+    ctx = torch.randint(0, 17, (n,), generator=g, device=DEV).int()
+    ctx[::501] = torch.randint(0, L + 1, (len(ctx[::501]),), generator=g, device=DEV).int()
+    got = K.attn_decode_shared(q, stored(x), table, ctx, i32([0]), i32([]).reshape(-1))
+    p = torch.arange(L, device=DEV)
+    for at in range(0, n, 5000):
+        rows = slice(at, at + 5000)
+        kv = x[table[rows].long()[:, p // 64], 0, :, p % 64].to(F64)
+        w = torch.einsum("bhd,bnd->bhn", q[rows].to(F64), kv[:, :, 0]) / math.sqrt(d)
+        unseen = p >= ctx[rows, None]
+        w = torch.softmax(w.masked_fill(unseen[:, None], -math.inf), -1).nan_to_num(0.0)      # no key at all: zeros
+        want = torch.einsum("bhn,bnd->bhd", w, kv[:, :, 1]).reshape(-1, 2 * d)
+        tol = kv[:, :, 1].abs().masked_fill(unseen[:, :, None], 0).amax((1, 2))[:, None] * (2.0 ** -11 + 6e-4 + L * 2.0 ** -30)
+        close((got[0][rows], got[1][rows]), want, tol.expand_as(want), 2)
+
+
+def test_one_sm_with_nearly_all_own_parts(K, sharing):
+    """A prefix that keeps all SMs but one busy: the last one's warps have 71 steps each, one of every sequence."""
+    check(K, make(71, 4, 1, 128, [2048], [40960], [i % 17 for i in range(2048)], hidden=0.5))
+
+
 @pytest.mark.parametrize("nq,nkv,d", [(8, 8, 64), (8, 8, 128)])
 def test_pages_beyond_four_gigabytes(K, sharing, nq, nkv, d):
     """Byte offsets into the cache pass 32 bits, and numbers of fp16 31 bits."""
