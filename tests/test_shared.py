@@ -120,3 +120,18 @@ def test_structs_of_arguments_lie_as_in_the_header(lib, tmp_path):
             got.append((at, size))
             at += size
         assert got == want and layout.size == at
+
+
+@pytest.mark.parametrize("name,layout,fields", [("ft_step_lists_args", N.STEP_LISTS_ARGS, 17), ("ft_norm_append_args", N.NORM_APPEND_ARGS, 24), ("ft_attn_shared_args", N.ATTN_SHARED_ARGS, 18)])
+def test_what_is_packed_is_as_long_as_the_struct(tmp_path, name, layout, fields):
+    """The library copies whole structs: with what the C compiler pads them with, they lie in the bytes that a call hands over."""
+    import shutil
+    import subprocess
+    if shutil.which("gcc") is None:
+        pytest.skip("no gcc on this box")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src = tmp_path / "f.c"
+    src.write_text(f'#include <stdio.h>\n#include "fasttalk_b200.h"\nint main(void) {{\n    printf("%d\\n", (int)sizeof({name}));\n    return 0;\n}}\n')
+    subprocess.run(["gcc", "-std=c99", "-I", os.path.join(root, "include"), str(src), "-o", str(tmp_path / "f")], check=True)
+    size = int(subprocess.run([str(tmp_path / "f")], capture_output=True, text=True, check=True).stdout)
+    assert len(layout.pack(*[0] * fields)) == size
