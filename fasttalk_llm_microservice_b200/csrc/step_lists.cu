@@ -187,6 +187,16 @@ extern "C" int ft_step_lists(const ft_step_lists_args* args, void* stream) {
                    (page_table || table_rows == 0 || max_pages == 0) && (free_pages || n_free == 0),
                "ft_step_lists: null argument");
     FT_REQUIRE(taken != first_free, "ft_step_lists: taken at the address of first_free, which other CTAs may read later");
+    // Every CTA makes the scans for itself, when it comes to run: what one writes must be nothing that another may still read (lengths advanced in place, say)
+    const struct { const int* at; size_t n; } arrays[] = {
+        {req_start, (size_t)R + 1}, {ctx_lens, (size_t)R}, {positions, (size_t)max_tokens}, {seq_rows, (size_t)max_tokens}, {kv_slots, (size_t)max_tokens}, {taken, 1},
+        {page_table, (size_t)table_rows * max_pages}, {cached_lens, (size_t)R}, {new_lens, (size_t)R}, {req_slot, req_slot ? (size_t)R : 0}, {free_pages, (size_t)n_free},
+        {first_free, first_free ? 1u : 0u}};
+    constexpr int kWritten = 7;                                // the first of these
+    for (int i = 0; i < kWritten; ++i)
+        for (int j = i + 1; j < (int)(sizeof(arrays) / sizeof(arrays[0])); ++j)
+            FT_REQUIRE(!arrays[i].n || !arrays[j].n || (uintptr_t)arrays[i].at + arrays[i].n * 4 <= (uintptr_t)arrays[j].at || (uintptr_t)arrays[j].at + arrays[j].n * 4 <= (uintptr_t)arrays[i].at,
+                       "ft_step_lists: an array that it writes overlaps another one");
     static PerDeviceFlag attr_set;
     if (!attr_set.done()) {
         FT_CHECK_CUDA(cudaFuncSetAttribute(step_lists_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,

@@ -712,7 +712,8 @@ int ft_attn_prefill_kv8(const void* q, const void* kv8_layer, int num_pages, con
  * ft_step_lists: requests r = 0 .. R - 1 (R up to 8192) in their order, with cached_lens[r] tokens in the cache, new_lens[r] new ones and page-table row req_slot[r] (NULL: row r),
  * each take as many of their new tokens as there is room for: in their row of the table, on their last page and the pages left in the pool, in the budget of max_tokens.
  * The pool is free_pages[first .. n_free - 1], first = *first_free (NULL: 0); pages are taken from it in order and written into page_table behind those that hold the cached
- * tokens, and *taken is where the rest of the pool begins (not the same address as first_free).  Of several requests with one row the first gets it, the others and those
+ * tokens, and *taken is where the rest of the pool begins.  What it writes, the table among it, overlaps neither what it reads nor each other: lengths and the pool's rest are
+ * not advanced in place.  Of several requests with one row the first gets it, the others and those
  * whose row is outside the table get nothing.  -> req_start [R + 1], ctx_lens [R] = cached and taken tokens; positions, seq_rows and kv_slots [max_tokens] of every token,
  * -1 behind the last one.  kv_slots is also -1 where the table or the pool names no page (a number below 0 or from 2^25 - 1 on). */
 typedef struct {

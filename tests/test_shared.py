@@ -38,6 +38,25 @@ def test_the_rest_of_the_pool_is_told_elsewhere(lib):
     refused(lib.ft_step_lists(N.STEP_LISTS_ARGS.pack(P, P, 0, P, P, 2 * P, P, P, P, P, P, 2 * P, 1, 1, 1, 1, 1), 0), "first_free")
 
 
+def test_lists_are_not_made_in_place(lib):
+    """What the call writes is nothing that it reads, nor the same memory twice: one CTA would write what another has yet to read."""
+    R, rows, width, free, tokens = 5, 7, 3, 9, 600
+    sizes = dict(cached=R, new=R, slot=R, table=rows * width, pool=free, first=1, start=R + 1, ctx=R, pos=tokens, row=tokens, kv=tokens, taken=1)
+    apart, at = {}, 1 << 12
+    for name, n in sizes.items():
+        apart[name] = at
+        at += 4 * n
+    call = lambda **over: lib.ft_step_lists(N.STEP_LISTS_ARGS.pack(*{**apart, **over}.values(), R, rows, width, free, tokens), 0)
+    written = ("table", "start", "ctx", "pos", "row", "kv", "taken")
+    for w in written:
+        for other in sizes:
+            if other != w and {w, other} != {"taken", "first"}:
+                refused(call(**{w: apart[other]}), "overlaps")
+                refused(call(**{w: apart[other] + 4 * (sizes[other] - 1)}), "overlaps")
+                refused(call(**{w: apart[other] - 4 * (sizes[w] - 1)}), "overlaps")
+    refused(call(taken=apart["first"]), "first_free")
+
+
 def test_refusals_of_appending(lib):
     call = lambda d=64, kind=0, T=1, nq=4, nkv=1, S=1, pages=1, rotated=0, angles=8, cos=P, q_gain=0, q_gains=1, k_gain=0, k_gains=1, qkv=P, pos=P, out=P, cache=P: lib.ft_norm_rope_kv_append(
         N.NORM_APPEND_ARGS.pack(qkv, 0, 0, cos, P, q_gain, k_gain, pos, P, out, cache, kind, S, angles, rotated, 0, q_gains, k_gains, pages, T, nq, nkv, d, 1e-5), 0)
