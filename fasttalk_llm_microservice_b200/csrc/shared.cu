@@ -899,6 +899,7 @@ shared_attn_kernel(const __grid_constant__ SharedArgs p) {
     }
     tc_fence_before();
     __syncthreads();
+    if (tid == 0) p.gave_up_at[blockIdx.x] = dead;                           // every call writes all of them: the second kernel reads none of an earlier one's
     if (tid == 0 && dead) {
         *err = 1;
 #pragma unroll 1
@@ -929,9 +930,12 @@ shared_merge_kernel(const __grid_constant__ SharedArgs p) {
     const int4 own = p.own_units[unit];
     int4 pre = make_int4(0, -1, 0, 0);
     if (p.n_groups) pre = p.prefix_units[unit];
-    // (without a prefix part nobody has written there, nor where a wait ran out ahead of that: then the result is NaN)
-    const bool lost = own.z && !(pre.x >= 0 && pre.x <= pre.y && pre.y < p.ctas && pre.z >= 0 && pre.z < p.rows && pre.z + 2 * kSharedRows * pre.y + G <= p.rows);
-    if (!own.z || lost) pre = make_int4(0, -1, 0, 0);
+    // Where a wait ran out anywhere, parts of this call may be missing and those of an earlier one in their place: all that the call says is NaN
+    int gave_up = 0;
+    for (int i = threadIdx.x; i < p.ctas; i += SM_THREADS) gave_up |= __ldcg(p.gave_up_at + i);
+    // (nobody has written there without a prefix part, or where a wait ran out ahead of that: what is there then may be anything, and nothing is read by it)
+    const bool there = own.z && pre.x >= 0 && pre.x <= pre.y && pre.y < p.ctas && pre.z >= 0 && pre.z < p.rows && pre.z + 2 * kSharedRows * pre.y + G <= p.rows;
+    if (!there) pre = make_int4(0, -1, 0, 0);
     // a thread has four dims of a head (neighbours the same of neighbouring heads, as the prefix's results lie), and every `lanes`-th part
     const int mine = (int)((threadIdx.x / (D / 4)) * p.inv_g >> 16), e = threadIdx.x - mine * (G * D / 4), lanes = (int)((SM_THREADS / (D / 4)) * p.inv_g >> 16);
     const int quad = (int)(e * p.inv_g >> 16), hg = e - quad * G;
@@ -973,7 +977,7 @@ shared_merge_kernel(const __grid_constant__ SharedArgs p) {
         *reinterpret_cast<float4*>(acc_s + 4 * threadIdx.x) = acc;
         ml_s[threadIdx.x] = make_float2(M, L);
     }
-    __syncthreads();
+    gave_up = __syncthreads_or(gave_up);
     if (mine) return;
 #pragma unroll 1
     for (int x = 1; x < lanes; ++x) M = fmaxf(M, ml_s[x * (G * D / 4) + e].x);
@@ -986,7 +990,7 @@ shared_merge_kernel(const __grid_constant__ SharedArgs p) {
         L = fmaf(ml.y, z, L);
         acc = fma_f4(*reinterpret_cast<const float4*>(acc_s + 4 * (x * (G * D / 4) + e)), make_float4(z, z, z, z), acc);
     }
-    if (lost) L = NAN;
+    if (gave_up) L = NAN;
     const float r = L == 0.f ? 0.f : 1.f / L;                                // a query without a visible key: zeros
     const float v[4] = {acc.x * r, acc.y * r, acc.z * r, acc.w * r};
     const size_t at = ((size_t)unit * G + hg) * D + 4 * quad;                // (unit = sequence * key heads + key head)
@@ -997,7 +1001,7 @@ shared_merge_kernel(const __grid_constant__ SharedArgs p) {
 }
 
 // ------------------------------------------------------------------ host
-struct SharedLayout { size_t own_units, prefix_units, own_parts, rows_o, rows_ml, rows, bytes; };
+struct SharedLayout { size_t own_units, prefix_units, own_parts, rows_o, rows_ml, gave_up_at, rows, bytes; };
 static SharedLayout shared_layout(int B, int n_groups, int nq, int nkv, int d) {
     const size_t sms = device_sms(), rows = (size_t)B * nq + 2 * kSharedRows * sms, units = (size_t)B * nkv;
     SharedLayout l;
@@ -1013,6 +1017,7 @@ static SharedLayout shared_layout(int B, int n_groups, int nq, int nkv, int d) {
     l.own_parts = take((units + 4 * sms) * shared_part(nq / nkv, d) * 4);
     l.rows_o = take(n_groups ? rows * d * 4 : 0);
     l.rows_ml = take(n_groups ? rows * 8 : 0);
+    l.gave_up_at = take(sms * sizeof(int));
     l.bytes = at;
     return l;
 }
@@ -1085,7 +1090,7 @@ extern "C" int ft_attn_decode_shared(const ft_attn_shared_args* args, void* stre
     const SharedLayout l = shared_layout(B, n_groups, nq, nkv, d);
     uint8_t* w = (uint8_t*)scratch;
     SharedArgs p{(const __half*)q, (const uint8_t*)kv_layer, page_table, req_slot, ctx_lens, group_start, shared_lens, (__nv_bfloat16*)out, (__nv_bfloat16*)out_lo,
-                 (int4*)(w + l.own_units), (int4*)(w + l.prefix_units), (float*)(w + l.own_parts), (float*)(w + l.rows_o), (float2*)(w + l.rows_ml), B, n_groups, num_pages, table_rows,
+                 (int4*)(w + l.own_units), (int4*)(w + l.prefix_units), (float*)(w + l.own_parts), (float*)(w + l.rows_o), (float2*)(w + l.rows_ml), (int*)(w + l.gave_up_at), B, n_groups, num_pages, table_rows,
                  max_pages, nq, nkv, G, th, (int)l.rows, 0, (65536u + G - 1) / G, kSharedLog2E / sqrtf((float)d), (unsigned)(((1ull << 32) + 2 * th - 1) / (2 * th)), 0, 0, 0, 0};
     return d == 64 ? launch_shared<64>(p, (cudaStream_t)stream) : launch_shared<128>(p, (cudaStream_t)stream);
 }

@@ -25,6 +25,7 @@ struct SharedArgs {
     float* own_parts;                            // [unit + warp][G][D], then (m, l)
     float* rows_o;                               // prefix results: O [D / 4][row + 256 CTA][4], (m, l)
     float2* rows_ml;
+    int* gave_up_at;                             // [CTA]: 1 where a wait of this call ran out
     int B, n_groups, num_pages, table_rows, max_pages, nq, nkv, G, th;        // th: queries of a half
     int rows;                                    // of the prefix's results
     int chunk_log;                               // tokens of an own step: 2^6 or 2^4

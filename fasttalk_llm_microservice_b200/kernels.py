@@ -597,8 +597,8 @@ def _shared_size(index: int, *sizes) -> int:
 
 
 def attn_shared_check(device=None) -> None:
-    """Waits for the device (the current one by default) and raises if a kernel of attn_decode_shared has ever given up on a wait there: rows of some call since the library was
-    loaded mean nothing.  No call asks by itself, since that would make the host wait."""
+    """Waits for the device (the current one by default) and raises if a kernel of attn_decode_shared has ever given up on a wait there: all rows of some call since the library
+    was loaded are NaN.  No call asks by itself, since that would make the host wait."""
     with torch.cuda.device(device):
         if N.check(N.load().ft_attn_shared_waits(), "ft_attn_shared_waits"):
             raise N.NativeError("attention over shared prefixes: a wait inside a kernel ran out; outputs of this process are not to be trusted")

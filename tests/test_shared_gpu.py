@@ -764,6 +764,49 @@ def test_waits_that_run_out_are_told(K):
     assert r.returncode == 0 and "TOLD" in r.stdout, r.stdout + r.stderr
 
 
+STALE = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch
+from tests import test_shared_gpu as T
+from fasttalk_llm_microservice_b200 import native as N
+lib = N.load()
+for d, sizes, shared, own, least in ((64, [9, 40], [900, 300], 70, 0), (128, [5, 30], [700, 2000], 90, 0), (64, [70], [5000], 3, 0), (128, [3, 2], [130, 200], 400, 2 ** 62)):
+    lib.ft_attn_shared_set_least(least)
+    s = T.make(d, 8, 2, d, sizes, shared, [i * 13 % own for i in range(sum(sizes))], hidden=0.5)
+    B = sum(sizes)
+    s["ctx"][1] = 0
+    scratch = torch.zeros(lib.ft_attn_decode_shared_scratch_bytes(B, len(sizes), 8, 2, d), device="cuda", dtype=torch.uint8)
+    def run(q):
+        out = torch.zeros(2, B, 8 * d, device="cuda", dtype=torch.bfloat16)
+        N.check(lib.ft_attn_decode_shared(N.ATTN_SHARED_ARGS.pack(
+            q.data_ptr(), s["cache"].data_ptr(), s["table"].data_ptr(), s["slots"].data_ptr(), s["ctx"].data_ptr(), s["starts"].data_ptr(), s["shared"].data_ptr(), out[0].data_ptr(),
+            out[1].data_ptr(), scratch.data_ptr(), s["cache"].shape[0], *s["table"].shape, len(sizes), B, 8, 2, d), torch.cuda.current_stream().cuda_stream), "ft_attn_decode_shared")
+        torch.cuda.synchronize()
+        return out
+    other = -s["q"].flip(0).contiguous()
+    want = run(s["q"])
+    run(other)
+    lib.ft_attn_shared_give_up(1)
+    lost = run(s["q"])
+    lib.ft_attn_shared_give_up(0)
+    print(d, "rows that are numbers:", int((~lost.isnan().all(-1)).sum()), "of", 2 * B)
+    assert lost.isnan().all()
+    assert torch.equal(run(s["q"]), want)
+print("NAN")
+"""
+
+
+def test_nothing_of_an_earlier_call_is_left_where_waits_run_out(K):
+    """Work memory still holds the last call's parts: a call whose waits run out gives NaN for all that it says, not numbers made of those."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", STALE, root], capture_output=True, text=True, timeout=300, cwd=root)
+    assert r.returncode == 0 and "NAN" in r.stdout, r.stdout + r.stderr
+
+
 # ------------------------------------------------------------------------------------------------ refusals
 def test_refusals_of_tensors(K):
     z = lambda *n: torch.zeros(*n, device=DEV, dtype=torch.int32)
