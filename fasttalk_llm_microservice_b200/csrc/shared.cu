@@ -14,8 +14,6 @@
 // 24 behind one of 16001, 300 own, 32 heads of 128 over 8, 25.5 (12.6); two behind 517, 9.8 (0.2).  What bounds it: 4.4 us from the launch to the first page asked for (the
 // plan 2.0, what the shares begin with 1.4, a copy 1.3), then memory (74 MB in about 11 us) or, where all 256 rows of a tile are in use, the softmax (2000 clocks a page and
 // half pair of which 1024 are exponentials), 1 to 2 us to write O, and the second kernel, 3.5 to 6 with its launch.
-#include <atomic>
-
 #include "common.cuh"
 #include "ft_internal.h"
 #include "shared.cuh"
@@ -1022,8 +1020,9 @@ static SharedLayout shared_layout(int B, int n_groups, int nq, int nkv, int d) {
     return l;
 }
 
-static std::atomic<long long> g_shared_least{-1};
-static std::atomic<int> g_shared_give_up{0};
+// settings of the calling thread: another one's calls do not change with them
+static thread_local long long g_shared_least = -1;
+static thread_local int g_shared_give_up = 0;
 
 template <int D>
 static int launch_shared(SharedArgs& p, cudaStream_t st) {
@@ -1041,10 +1040,10 @@ static int launch_shared(SharedArgs& p, cudaStream_t st) {
     // 18.3 / 18.2, three of 2000 12.8 / 12.6, of 8000 15.1 / 16.8 (16 MB saved, from the third on), eight of 1000 12.1 / 11.8, of 2000 13.2 / 14.4 (24 MB), sixteen of 130 11.8 / 10.4,
     // of 517 11.9 / 13.4 (15 MB); heads of 128 (32 over 8), two of 1000 13.6 / 13.3, of 2000 15.3 / 15.3 (8 MB), of 8000 17.8 / 23.5, four of 517 12.8 / 13.0 (6 MB), eight of
     // 130 12.9 / 11.9, of 517 13.1 / 13.6; sixteen key heads, two of 1000 15.0 / 12.9, of 2000 16.2 / 15.8 (16 MB), four of 130 13.2 / 11.4, of 517 13.5 / 14.1 (13 MB).
-    const long long least = g_shared_least.load(std::memory_order_relaxed), pages = (least < 0 ? (D == 64 ? 12 : 6) << 20 : least) / ((long long)C::TILE * p.nkv);
+    const long long least = g_shared_least, pages = (least < 0 ? (D == 64 ? 12 : 6) << 20 : least) / ((long long)C::TILE * p.nkv);
     p.least_size = D == 64 && least < 0 ? 3 : 2;
     p.least_pages = (int)(pages < INT32_MAX ? pages : INT32_MAX) + (least < 0);
-    p.give_up = g_shared_give_up.load(std::memory_order_relaxed);
+    p.give_up = g_shared_give_up;
     p.ctas = device_sms();
     FT_CHECK_CUDA(launch_after(shared_attn_kernel<D>, dim3(p.ctas), dim3(SH_THREADS), C::SMEM, st, (const SharedArgs&)p));
     FT_CHECK_CUDA(launch_after(shared_merge_kernel<D>, dim3(p.B * p.nkv), dim3(SM_THREADS), 0, st, (const SharedArgs&)p));

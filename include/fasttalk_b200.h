@@ -748,9 +748,10 @@ int ft_norm_rope_kv_append(const ft_norm_append_args* args, void* stream);
  * does not grow or leaves [0, B] makes no groups.  A query that sees no key gives zeros.  Probabilities are rounded to fp16 down to 2^-30 of the largest.
  * scratch: work memory of ft_attn_decode_shared_scratch_bytes bytes (of the current device), in any state, not shared by calls that may overlap.
  * A prefix is read once where the call's groups save enough by that (12 MB at heads of 64, counted from the third query of a group on, 6 MB at 128, from the second on), else by
- * every query; ft_attn_shared_set_least: what they have to save in the calls that follow, 0: nothing (below 0: the library's own).  Results are the same but for rounding.
+ * every query; ft_attn_shared_set_least: what they have to save in the calls that this thread makes from now on, 0: nothing (below 0: the library's own).  Results are the same but
+ * for rounding.
  * ft_attn_shared_waits: 1 if a wait inside one of its kernels has run out on the current device since the library was loaded (all that such a call says is NaN), else 0;
- * waits for all that the device has been given, on every stream.  ft_attn_shared_give_up(1): the kernels of the calls that follow give up at the first
+ * waits for all that the device has been given, on every stream.  ft_attn_shared_give_up(1): the kernels of this thread's calls from now on give up at the first
  * wait that is not over yet, so that a host can see what it does then; (0): after a million tries, as ever. */
 long long ft_attn_decode_shared_scratch_bytes(int B, int n_groups, int nq, int nkv, int d);
 typedef struct {

@@ -807,6 +807,40 @@ def test_nothing_of_an_earlier_call_is_left_where_waits_run_out(K):
     assert r.returncode == 0 and "NAN" in r.stdout, r.stdout + r.stderr
 
 
+def test_what_one_thread_sets_holds_for_its_own_calls(K):
+    """Both settings are the calling thread's: another one's calls take the form that they took before, and wait."""
+    import threading
+    lib = K.N.load()
+    s = make(80, 8, 2, 64, [20], [2000], [i * 7 % 60 for i in range(20)], hidden=0.5)
+    runs = {}
+
+    def call(name):
+        runs[name] = torch.cat(K.attn_decode_shared(s["q"], s["cache"], s["table"], s["ctx"], s["starts"], s["shared"], s["slots"]))
+        torch.cuda.synchronize()
+
+    def inside(f):
+        t = threading.Thread(target=f)
+        t.start()
+        t.join()
+    for name, least in (("as it pays", -1), ("always", 0), ("never", 2 ** 62)):
+        lib.ft_attn_shared_set_least(least)
+        call(name)
+    lib.ft_attn_shared_set_least(-1)
+    assert not torch.equal(runs["always"], runs["never"])                              # (sums in another order)
+    for least in (0, 2 ** 62):
+        inside(lambda: lib.ft_attn_shared_set_least(least))
+        call("here")
+        assert torch.equal(runs["here"], runs["as it pays"])
+        lib.ft_attn_shared_set_least(least)
+        inside(lambda: call("there"))
+        lib.ft_attn_shared_set_least(-1)
+        assert torch.equal(runs["there"], runs["as it pays"])
+    inside(lambda: lib.ft_attn_shared_give_up(1))
+    call("here")
+    assert torch.equal(runs["here"], runs["as it pays"])
+    K.attn_shared_check()
+
+
 # ------------------------------------------------------------------------------------------------ refusals
 def test_refusals_of_tensors(K):
     z = lambda *n: torch.zeros(*n, device=DEV, dtype=torch.int32)
