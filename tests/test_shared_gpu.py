@@ -657,6 +657,121 @@ def test_a_run_of_all_three(K, sharing):
     assert ctx.tolist() == [prompt + 70] * B
 
 
+def bounded(s):
+    """attention() with a bound for each number: (out, how far off it may be).  A score is a sum of d products in fp32, off by (d + 8) * 2^-23 of their magnitudes' sum, and its exponent by
+    the scale's and the subtraction's roundings, 2^-22 of it, and 2^-21: e together.  With weights w e^+-e for w the result moves by sum w (exp(e) - 1) |v - out| over what is left of the sum.
+    Then probabilities in fp16 (2^-11 of each, 2^-30 of the largest below normal numbers), sixteen keys an instruction added up in fp32 (2^-26 a key), and a few fp32 steps to
+    put parts together (2^-18)."""
+    q, x = s["q"], logical(s["cache"])
+    B, nq, d = q.shape
+    nkv = x.shape[1]
+    starts, shared, where, ctx = s["starts"].tolist(), s["shared"].tolist(), s["slots"].tolist(), s["ctx"].tolist()
+    out, off = torch.zeros(B, nq, d, device=DEV, dtype=F64), torch.zeros(B, nq, d, device=DEV, dtype=F64)
+    for i, n in enumerate(ctx):
+        k = next((k for k in range(len(shared)) if starts[k] <= i < starts[k + 1]), None)
+        p = torch.arange(n, device=DEV)
+        row = torch.where(p < (0 if k is None else shared[k]), where[i if k is None else starts[k]], where[i])
+        kv = x[s["table"][row, p // 64].long(), :, :, p % 64].to(F64)
+        keys, v, qq = kv[:, :, 0], kv[:, :, 1], q[i].to(F64).reshape(nkv, nq // nkv, d)
+        score = torch.einsum("hgd,nhd->hgn", qq, keys) / math.sqrt(d)
+        e = torch.einsum("hgd,nhd->hgn", qq.abs(), keys.abs()) / math.sqrt(d) * (d + 8) * 2.0 ** -23 + score.abs() * 2.0 ** -22 + 2.0 ** -21
+        w = torch.softmax(score, -1)
+        o = torch.einsum("hgn,nhd->hgd", w, v)
+        moved = w * torch.expm1(e)
+        size = torch.einsum("hgn,nhd->hgd", w, v.abs())
+        off[i] = (((v.permute(1, 0, 2)[:, None] - o[:, :, None]).abs() * moved[..., None]).sum(2) / (1 - moved.sum(-1))[..., None]
+                  + size * (2.0 ** -11 + n * 2.0 ** -26 + 2.0 ** -18) + n * 2.0 ** -30 * v.abs().amax((0, 2))[:, None, None]).reshape(nq, d)
+        out[i] = o.reshape(nq, d)
+    return out.reshape(B, -1), off.reshape(B, -1)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_scores_far_apart_number_by_number(K, sharing, d):
+    """test_scores_far_apart's inputs and others against a bound for each number, which goes by how far each score may be off."""
+    for where in range(8):
+        s = make(120 + where, 8, 2, d, [4, 2], [900, 300], [100, 3, 64, 300, 1, 500], hidden=None)
+        s["q"] = s["q"] * (4 if where < 6 else 0.5)
+        x = logical(s["cache"])
+        g = gen(where)
+        x[:, :, 0] *= torch.exp(torch.randn(x.shape[0], x.shape[1], 64, 1, generator=g, device=DEV)).half()
+        if where < 6:
+            page = s["table"][s["slots"][0].long(), [0, 13, 14, 7, 3, 15][where]].long()
+            x[page, :, 0, where] = s["q"][0, :2].half()
+        s["cache"] = stored(x)
+        got = K.attn_decode_shared(s["q"], s["cache"], s["table"], s["ctx"], s["starts"], s["shared"], s["slots"])
+        close(got, *bounded(s), 2)
+
+
+@pytest.mark.parametrize("nq,nkv,d,neighbours", [(8, 2, 64, False), (12, 4, 128, True)])
+def test_steps_of_all_three_token_by_token(K, sharing, nq, nkv, d, neighbours):
+    """Two groups behind their prompts, a prompt's last page among what a step writes.  Each new key looks like its token's query, so that most of the weight is on the last token: one
+    that is missing would show in all numbers, and whatever nobody wrote is NaN.  Attention is held against what lies in the cache, and that against the rows that were appended."""
+    g = gen(d)
+    sizes, prompts, width, pages, gap = [3, 2], [200, 64], 6, 40, 2
+    B, W, R = sum(sizes), (nq + 2 * nkv) * d, sum(sizes) + gap
+    cos, sin = angles(width * 64, d)
+    q_gain, k_gain = 1 + 0.2 * torch.randn(nq, d, generator=g, device=DEV), 1 + 0.2 * torch.randn(nkv, d, generator=g, device=DEV)
+    cache = torch.full((pages, nkv, 2, 64, d), NAN, device=DEV, dtype=torch.float16)
+    table = torch.full((R, width), -1, device=DEV, dtype=torch.int32)
+    free, taken = torch.randperm(pages, generator=g, device=DEV).int(), i32([0])
+    slots = torch.randperm(R, generator=g, device=DEV)[:B].int()
+    starts, shared = i32([0, 3, 5]), i32(prompts)
+    firsts, held = [0, 3], [0] * B
+
+    def token(n):
+        x = torch.randn(n, nq + 2 * nkv, d, generator=g, device=DEV)
+        x[:, nq:nq + nkv] = x[:, :nq:nq // nkv] + 0.2 * torch.randn(n, nkv, d, generator=g, device=DEV)
+        return x.reshape(n, W).bfloat16()
+
+    def append(l, x):
+        return check_append(K, x, l.positions, l.kv_slots, cache, nq, nkv, d, cos, sin, q_gain, k_gain, 1e-5, neighbours)
+    for f, n in zip(firsts, prompts):                                              # prompts, written once
+        l = K.step_lists([0], [n], slots[f:f + 1].contiguous(), table, free, n, taken)
+        append(l, token(n))
+        taken, held[f] = l.taken, n
+    # the page on which the first prompt ends is the first sequence's: the others have the prompt's tokens below that, and a page of their own from there on
+    for k, f in enumerate(firsts):
+        for b in range(f + 1, f + sizes[k]):
+            held[b] = prompts[k]
+            if prompts[k] % 64:
+                table[slots[b].long(), prompts[k] // 64] = free[taken[0].long()]
+                taken = taken + 1
+    ctx = i32(held)
+    for n in range(66):
+        new = [1 if (n + b) % 5 or n < 2 else 0 for b in range(B)]                  # now and then a sequence waits
+        total = sum(new)
+        l = K.step_lists(ctx, i32(new), slots, table, free, B + 1, taken)
+        held = [h + m for h, m in zip(held, new)]
+        assert l.ctx_lens.tolist() == held and l.req_start.tolist()[-1] == total and l.positions.tolist() == [h - 1 for h, m in zip(held, new) if m] + [-1] * (B + 1 - total)
+        q = append(l, token(B + 1))
+        rows = torch.tensor([l.req_start[b].item() if m else total for b, m in enumerate(new)], device=DEV)
+        s = {"q": q[rows], "cache": cache, "table": table, "ctx": l.ctx_lens, "starts": starts, "shared": shared, "slots": slots}
+        got = K.attn_decode_shared(s["q"], cache, table, l.ctx_lens, starts, shared, slots)
+        if n % 5 == 0 or n in (55, 56, 57, 63, 64):
+            want, off = bounded(s | {"ctx": i32(held)})
+            close(got, want, off, 2)
+        ctx, taken = l.ctx_lens, l.taken
+
+
+@pytest.mark.parametrize("nq,nkv,d,sizes,shared,shares", [
+    # heads of 64: 12 MB counted from the third query on: at 8 key heads 97 pages
+    (32, 8, 64, [2], [40000], False), (32, 8, 64, [3], [96 * 64], False), (32, 8, 64, [3], [97 * 64], True), (32, 8, 64, [6, 3], [20 * 64, 16 * 64], False), (32, 8, 64, [6, 3], [20 * 64, 17 * 64], True),
+    # heads of 128: 6 MB from the second on: 25 pages
+    (32, 8, 128, [2], [24 * 64 + 63], False), (32, 8, 128, [2], [25 * 64], True), (32, 8, 128, [1], [9000], False), (32, 8, 128, [26], [127], False), (32, 8, 128, [14], [128], True),
+    (8, 2, 128, [2], [96 * 64], False), (8, 2, 128, [2], [97 * 64], True)])
+def test_prefixes_are_read_once_where_that_pays(K, nq, nkv, d, sizes, shared, shares):
+    """Which of both forms a call takes, by its bits: sums of a prefix that is read once stand in another order."""
+    s = make(90, nq, nkv, d, sizes, shared, [70 + i for i in range(sum(sizes))], hidden=0.5)
+    set_least = K.N.load().ft_attn_shared_set_least
+    got = {}
+    for least in (0, 2 ** 62, -1):
+        set_least(least)
+        got[least] = torch.cat(K.attn_decode_shared(s["q"], s["cache"], s["table"], s["ctx"], s["starts"], s["shared"], s["slots"]))
+    if max(sizes) > 1 and max(shared) >= 128:
+        assert not torch.equal(got[0], got[2 ** 62])
+    assert torch.equal(got[-1], got[0 if shares else 2 ** 62])
+
+
 @pytest.mark.parametrize("nq,nkv,d,groups", [(4, 1, 64, 99), (4, 1, 64, 100), (4, 2, 128, 101), (2, 2, 64, 700), (8, 1, 128, 1100)])
 def test_hundreds_of_groups(K, sharing, nq, nkv, d, groups):
     """More groups than the kernel keeps the lists of, and more sequences than it has threads: some groups empty, some of one, some of many."""
