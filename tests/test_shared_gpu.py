@@ -265,6 +265,23 @@ def test_append_of_parts_and_strides(K, nq, nkv, d, parts):
     check_append(K, same, pos, slots, torch.randn(3, nkv, 2, 64, d, generator=g, device=DEV).half(), nq, nkv, d, cos, sin)
 
 
+@pytest.mark.parametrize("nq,nkv,d", [(12, 4, 128), (32, 8, 64), (5, 1, 64), (6, 1, 128), (16, 16, 128)])
+@pytest.mark.parametrize("T", [700, 2103, 8195])
+@pytest.mark.parametrize("kind,parts,turned,neighbours,gains,pad", [(torch.float32, 2, 1, False, 1, 0), (torch.float32, 1, 0.5, True, 2, 1), (torch.bfloat16, 1, 1, False, 2, 8), (torch.float16, 1, 0.5, False, 0, 3),
+                                                                   (torch.bfloat16, 1, 1, True, 1, 0)])
+def test_append_of_many_tokens(K, nq, nkv, d, T, kind, parts, turned, neighbours, gains, pad):
+    """Steps with so many tokens that a warp takes several heads after one another, up to all of a token's."""
+    g = gen(T + nq)
+    W, pages = (nq + 2 * nkv) * d, T // 64 + 3
+    x = torch.randn(parts, T, W + pad, generator=g, device=DEV).to(kind)
+    x = x[..., pad:] if kind is torch.float32 else x[0, :, pad:]
+    cos, sin = angles(500, int(turned * d))
+    pos, slots = torch.randint(-1, 500, (T,), generator=g, device=DEV).int(), torch.randperm(pages * 64, generator=g, device=DEV)[:T].int()
+    slots[::97] = -1
+    gain = lambda n: None if gains == 0 else 1 + 0.3 * torch.randn(*((d,) if gains == 1 else (n, d)), generator=g, device=DEV)
+    check_append(K, x, pos, slots, torch.randn(pages, nkv, 2, 64, d, generator=g, device=DEV).half(), nq, nkv, d, cos, sin, gain(nq), gain(nkv), 1e-5, neighbours)
+
+
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
 def test_append_of_tokens_without_a_place_and_of_extremes(K, d, kind):
