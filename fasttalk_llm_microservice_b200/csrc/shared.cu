@@ -929,8 +929,7 @@ shared_merge_kernel(const __grid_constant__ SharedArgs p) {
     int4 pre = make_int4(0, -1, 0, 0);
     if (p.n_groups) pre = p.prefix_units[unit];
     // Where a wait ran out anywhere, parts of this call may be missing and those of an earlier one in their place: all that the call says is NaN
-    int gave_up = 0;
-    for (int i = threadIdx.x; i < p.ctas; i += SM_THREADS) gave_up |= __ldcg(p.gave_up_at + i);
+    int gave_up = (int)threadIdx.x < p.ctas ? __ldcg(p.gave_up_at + threadIdx.x) : 0;      // (no loop: it would wait for this ahead of the reads below, 0.2 us)
     // (nobody has written there without a prefix part, or where a wait ran out ahead of that: what is there then may be anything, and nothing is read by it)
     const bool there = own.z && pre.x >= 0 && pre.x <= pre.y && pre.y < p.ctas && pre.z >= 0 && pre.z < p.rows && pre.z + 2 * kSharedRows * pre.y + G <= p.rows;
     if (!there) pre = make_int4(0, -1, 0, 0);
@@ -1045,6 +1044,7 @@ static int launch_shared(SharedArgs& p, cudaStream_t st) {
     p.least_pages = (int)(pages < INT32_MAX ? pages : INT32_MAX) + (least < 0);
     p.give_up = g_shared_give_up;
     p.ctas = device_sms();
+    FT_REQUIRE(p.ctas <= SM_THREADS, "ft_attn_decode_shared: %d SMs (at most %d)", p.ctas, SM_THREADS);      // a thread of the second kernel for each
     FT_CHECK_CUDA(launch_after(shared_attn_kernel<D>, dim3(p.ctas), dim3(SH_THREADS), C::SMEM, st, (const SharedArgs&)p));
     FT_CHECK_CUDA(launch_after(shared_merge_kernel<D>, dim3(p.B * p.nkv), dim3(SM_THREADS), 0, st, (const SharedArgs&)p));
     return 0;
