@@ -6,20 +6,22 @@
 // those behind `rotated` are shared out the same way) and neighbouring lanes have neighbouring chunks.  So the only exchange is the sum of squares, and a load or store
 // of the warp takes whole lines.  The factor rsqrt(..) is the same for a head, so it comes last: gain and rotation do not wait for the sum.
 //
-// Measured in a graph, us: one token of 48 heads of 64 1.9; 64 of 48 heads of 128 in two fp32 parts 2.5 (latency: a launch, two reads, a store); 8195 of 48 heads of 128 from bf16,
-// neighbouring pairs, 35.4 for 180 MB = 5.1 TB/s, 79 % of a copy: six of ten issue slots are in use, and a warp waits for its reads at the end of each token.
+// Measured in a graph, us: one token of 48 heads of 64 1.9; 64 of 48 heads of 128 in two fp32 parts 2.5 (latency: a launch, two reads, a store).
+// 7299 of 48 heads of 128 from bf16 (180 MB): neighbouring pairs 35.4 = 5.1 TB/s, 79 % of a copy; halves 41.8 = 4.3 TB/s.  From fp32 (270 MB): 55.1, and halves 48.2 = 5.6 TB/s.  With
+// neighbouring pairs six of ten issue slots are in use, and a warp waits for its reads at the end of each token.  Registers, at heads of 128: 72 with neighbours and 83 in halves from
+// 16 bits, 80 and 91 from 32, so seven, five, six and five CTAs fit an SM: 1825 CTAs are 1.8 rounds of them with neighbours from 16 bits and 2.5 in halves.
 #include "common.cuh"
 #include "ft_internal.h"
 
 namespace ft {
 
 constexpr int NA_WARPS = 4, NA_THREADS = NA_WARPS * 32;
-// 8195 tokens of 48 heads of 128, us: passes whose reads are on their way together, 1 / 2 / 3: 47.9 / 35.6 / 45.8 (registers); numbers of a chunk, 4 / 8: 35.6 / 54
+// 7299 tokens of 48 heads of 128, neighbouring pairs, from bf16, us: passes whose reads are on their way together, 1 / 2 / 3: 47.9 / 35.6 / 45.8 (registers); numbers of a chunk, 4 / 8: 35.6 / 54
 constexpr int NA_AHEAD = 2;
 constexpr int NA_E = 4;
-// Warps per SM from which a warp takes more than one pass of a token, 16 / 40 / 100: the same 35.4 / 35.4 / 37.5, and for 2103 tokens of 20 heads 8.7 / 8.7 / 12.1
+// Warps per SM from which a warp takes more than one pass of a token, 16 / 40 / 100: the same 35.4 / 35.4 / 37.5, and for 1861 tokens of 20 heads 8.7 / 8.7 / 12.1
 constexpr int NA_FILL = 40;
-constexpr int NA_CTAS = 5;                           // per SM (6 and 7 take as long)
+constexpr int NA_CTAS = 5;                           // per SM at least (6 and 7 take as long)
 
 struct NormAppend {
     const void* x;
@@ -275,7 +277,7 @@ extern "C" int ft_norm_rope_kv_append(const ft_norm_append_args* args, void* str
     FT_REQUIRE((uintptr_t)qkv % size == 0, "ft_norm_rope_kv_append: qkv on its own size");
     FT_REQUIRE((double)T * (nq + 2.0 * nkv) <= INT32_MAX, "ft_norm_rope_kv_append: %d tokens are more than one call takes", T);
     const int chunk = size * NA_E;
-    // chunks that lie on their size are one load each (the calls above 35.4 us, with four loads 44.7; 64 single tokens 2.5 and 2.7)
+    // chunks that lie on their size are one load each (7299 tokens, neighbouring pairs, from bf16 35.4 us, with four loads 44.7; 64 single tokens 2.5 and 2.7)
     const bool wide = (uintptr_t)qkv % chunk == 0 && row_stride * size % chunk == 0 && (n_parts == 1 || part_stride * size % chunk == 0);
     NormAppend p{qkv, part_stride, row_stride, cos_t, sin_t, q_gain, k_gain, positions, kv_slots, (__half*)q_out, (uint8_t*)kv_layer, num_pages * kKvTile, n_parts, T,
                  nq, nkv, n_angles, rotated, q_gains > 1 ? d : 0, k_gains > 1 ? d : 0, 0, 0, 0, eps};

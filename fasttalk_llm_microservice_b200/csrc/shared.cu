@@ -10,8 +10,9 @@
 //            query heads of a key head in the columns).  No warp waits for another.
 // Each share's results are O, maximum and sum of its rows; a second kernel puts them together in their order.
 //
-// Measured in a graph, us (launch included), what it has to read at 6.46 TB/s in brackets: 64 sequences behind one prefix of 2048 tokens, 600 own, 32 heads of 64 over 8, 20.4 (7.4);
-// 24 behind one of 16001, 300 own, 32 heads of 128 over 8, 25.5 (12.6); two behind 517, 9.8 (0.2).  What bounds it: 4.4 us from the launch to the first page asked for (the
+// Measured in a graph, us (launch included), what it has to read at 6.46 TB/s in brackets: 64 sequences behind one prefix of 2048 tokens, up to 600 own (329 on
+// average), 32 heads of 64 over 8, 20.6 (7.4), a key head for each of 16 of 128 52.5 (29.4), 16 of 64 over 2 15.6 (1.9); 24 behind one of 16001, up to 300 own, 32 heads of 128 over 8,
+// 25.5 (12.6); two behind 517, 10.0 (0.2).  What bounds it: 4.4 us from the launch to the first page asked for (the
 // plan 2.0, what the shares begin with 1.4, a copy 1.3), then memory (74 MB in about 11 us) or, where all 256 rows of a tile are in use, the softmax (2000 clocks a page and
 // half pair of which 1024 are exponentials), 1 to 2 us to write O, and the second kernel, 3.5 to 6 with its launch.
 #include "common.cuh"
@@ -1039,6 +1040,8 @@ static int launch_shared(SharedArgs& p, cudaStream_t st) {
     // 18.3 / 18.2, three of 2000 12.8 / 12.6, of 8000 15.1 / 16.8 (16 MB saved, from the third on), eight of 1000 12.1 / 11.8, of 2000 13.2 / 14.4 (24 MB), sixteen of 130 11.8 / 10.4,
     // of 517 11.9 / 13.4 (15 MB); heads of 128 (32 over 8), two of 1000 13.6 / 13.3, of 2000 15.3 / 15.3 (8 MB), of 8000 17.8 / 23.5, four of 517 12.8 / 13.0 (6 MB), eight of
     // 130 12.9 / 11.9, of 517 13.1 / 13.6; sixteen key heads, two of 1000 15.0 / 12.9, of 2000 16.2 / 15.8 (16 MB), four of 130 13.2 / 11.4, of 517 13.5 / 14.1 (13 MB).
+    // The bytes that a call saves decide alone, not what its units cost: so two of 1000 at sixteen key heads are shared where that takes 2.1 us more, two of 2000 there 0.4 more, and
+    // two of 8000 at heads of 64 are not where it would take 0.5 less.
     const long long least = g_shared_least, pages = (least < 0 ? (D == 64 ? 12 : 6) << 20 : least) / ((long long)C::TILE * p.nkv);
     p.least_size = D == 64 && least < 0 ? 3 : 2;
     p.least_pages = (int)(pages < INT32_MAX ? pages : INT32_MAX) + (least < 0);

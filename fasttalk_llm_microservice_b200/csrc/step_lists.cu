@@ -7,8 +7,8 @@
 // cut so and S_r their sum ahead, the budget leaves max(0, budget - S_r), and nobody behind the one that it cuts gets any; so P_r is also where r's pages begin.
 //
 // What bounds it: latency alone (a launch, two rounds of reads, two scans, a search, a store).  Every CTA makes the scans for itself, one request a thread, which costs less
-// than a kernel ahead of this one, and then looks up 512 tokens and writes its part of the table.  Measured in a graph: 64 requests of one token 4.5 us, 21 of 541 with a budget
-// of 8192 4.4, 1021 of 77 with one of 65536 6.4 (CTAs of 256: 4.5, 4.4, 8.3; of 1024: 5.9, 5.8, 7.2); a call after another takes 12, the host's time.
+// than a kernel ahead of this one, and then looks up 512 tokens and writes its part of the table.  Measured in a graph: 64 requests of one token 4.5 us, 21 with 4419 tokens of a
+// budget of 8192 4.4, 1021 with 28977 of one of 65536 6.4 (CTAs of 256: 4.5, 4.4, 8.3; of 1024: 5.9, 5.8, 7.2); a call after another takes 12, the host's time.
 #include "common.cuh"
 #include "ft_internal.h"
 

@@ -729,7 +729,7 @@ int ft_step_lists(const ft_step_lists_args* args, void* stream);
  *   rotated on the first `rotated` dims (a multiple of 16; 0: none) by cos_t / sin_t fp32 [n_angles][rotated / 2]: pairs (i, i + rotated / 2), or (2 i, 2 i + 1) with neighbours,
  * all in fp32 and rounded once to fp16 (cut to its range; NaN stays): q to q_out [T][nq][d], k and v to kv_slots[t] of the cache.  qkv: FT_F32 in n_parts parts that are added
  * up, part_stride elements apart, or one part of FT_BF16 or FT_F16.  A token whose position is below 0 or has no angles gives q = 0 and is not written; one whose slot
- * is outside the cache is not written.  Two tokens for one slot leave it with numbers of either. */
+ * is outside the cache is not written.  Two tokens for one slot leave it with numbers of either.  q_out and the cache overlap nothing else. */
 enum { FT_F32 = 0, FT_BF16 = 1, FT_F16 = 2 };
 typedef struct {
     const void* qkv;
@@ -746,7 +746,7 @@ int ft_norm_rope_kv_append(const ft_norm_append_args* args, void* stream);
  * all of them are those of page-table row req_slot[group_start[g]], also where a query's own context is shorter or the first one's; what the other rows name below
  * that is not read, and what lies on a row's pages ahead of its first own token or behind its last may be anything.  req_slot NULL: row b.  A list group_start that
  * does not grow or leaves [0, B] makes no groups.  A query that sees no key gives zeros.  Probabilities are rounded to fp16 down to 2^-30 of the largest.
- * scratch: work memory of ft_attn_decode_shared_scratch_bytes bytes (of the current device), in any state, not shared by calls that may overlap.
+ * scratch: work memory of ft_attn_decode_shared_scratch_bytes bytes (of the current device), in any state, not shared by calls that may overlap.  It and the results overlap nothing else.
  * A prefix is read once where the call's groups save enough by that (12 MB at heads of 64, counted from the third query of a group on, 6 MB at 128, from the second on), else by
  * every query; ft_attn_shared_set_least: what they have to save in the calls that this thread makes from now on, 0: nothing (below 0: the library's own).  Results are the same but
  * for rounding.
